@@ -1,0 +1,1249 @@
+// 8-bit KV cache (sm_100a): quantising append, read-back, and attention over
+// the cache for single tokens, dense or over selected blocks. The prompt form
+// of the attention is in kv8_prompt.cu.
+//
+// The reference keeps K and V in fp32 (src/brain_runtime.c:2019-2020) and
+// attends per token (gqa_single_token, :1407-1528); this cache takes a quarter
+// of the bytes, and the attention over it keeps fp32-level accuracy for the
+// values that the codes stand for.
+#include <cfloat>
+#include <cmath>
+#include <algorithm>
+#include <atomic>
+#include "../../include/atlas_cuda.h"
+#include "common.cuh"
+#include "kv8.h"
+
+namespace atlas {
+
+int api_fail(int code, const char *fmt, ...);
+int api_device(int device, int *sms);
+
+namespace k8 {
+namespace {
+
+// Every kernel here is launched with programmatic stream serialization: it
+// may start while its predecessor drains, so it first waits for it. Inputs are
+// then read through L2 (__ldcg, cp.async.cg): this SM's L1 may hold lines from
+// before the predecessor wrote them.
+// `early`: let the successor start at once (it waits in turn). Only where all
+// of this grid fits on the device with room to spare: CTAs of a successor that
+// take the first slots to fall free would crowd on a few SMs.
+__device__ __forceinline__ void wait_predecessor(uint32_t early)
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// --------------------------------------------------------------- append ----
+
+struct AppendArgs {
+    Cache c;
+    Rows r;
+    const float *k, *v;   // [seq][tokens][kv_heads][128], ld floats between tokens
+    uint64_t ld;
+    uint32_t early;
+};
+
+// Nearest integer to x / s (ties to even), exactly, for |x| <= 127.5 s: the
+// product with the rounded reciprocal is off by at most 127 * 2^-23 < 2^-15,
+// so it decides everything but quotients within 2^-13 of a tie, which are
+// divided in 64 bits (two 24-bit values whose quotient is no tie differ from
+// it by 2^-25 or more). `slow`: s too small for the reciprocal.
+__device__ __forceinline__ int quantise(float x, float s, float inv, bool slow)
+{
+    const float t = x * inv;
+    float r = rintf(t);
+    if (slow || fabsf(t - r) > 0.5f - 1.220703125e-4f) r = (float)rint((double)x / (double)s);
+    return (int)fminf(fmaxf(r, -127.f), 127.f);
+}
+
+// One CTA per (touched block, K or V of a KV head, sequence). Warp w holds
+// rows w, w + 8, ... of the block in registers (lane = 4 dimensions), new ones
+// as values and earlier ones as codes, so the rows are read once: maximum,
+// then codes. scale = max(scale so far, max|new| / 127); rows that were in the
+// block before are rounded again where the scale grew. A block that a
+// non-finite value joins gets a NaN scale.
+// Bound by HBM: 4 bytes read and 1 written per value.
+template <int B>
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a)
+{
+    constexpr int kRows = B / 8;
+    __shared__ uint32_t s_max[8];
+    __shared__ int32_t s_sum[8][kDim];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    wait_predecessor(a.early);
+    const uint32_t s = blockIdx.z, h = blockIdx.y >> 1, is_v = blockIdx.y & 1u;
+    const uint64_t p0 = __ldcg(a.r.pos0 + s), end = min(p0 + row_count(a.r, s), (uint64_t)a.c.max_context);
+    const uint64_t blk = p0 / B + blockIdx.x, b0 = blk * B;
+    if (max(p0, b0) >= end) return;                                   // no new row in this block
+    const uint32_t lo = b0 < p0 ? (uint32_t)(p0 - b0) : 0u;          // rows [0, lo) were there before
+    const uint32_t hi = (uint32_t)min((uint64_t)B, end - b0);        // rows [lo, hi) are new
+    const size_t head = (size_t)s * a.c.kv_heads + h;
+    int8_t *code = (is_v ? a.c.v : a.c.k) + (head * a.c.max_context + b0) * kDim;
+    float *sp = (is_v ? a.c.v_scale : a.c.k_scale) + head * a.c.n_blocks + blk;
+    const float *src = (is_v ? a.v : a.k) + (size_t)s * a.r.tokens * a.ld + (size_t)h * kDim;
+
+    float4 x[kRows];   // a row that was there before: its 4 codes in the bits of .x
+    uint32_t mx = 0u;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const uint32_t r = warp + 8u * (uint32_t)i;
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < lo) x[i].x = __int_as_float(__ldcg(reinterpret_cast<const int *>(code + (size_t)r * kDim) + lane));
+        else if (r < hi) x[i] = __ldcg(reinterpret_cast<const float4 *>(src + (b0 + r - p0) * a.ld) + lane);
+    }
+    const float was = lo ? __ldcg(sp) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const uint32_t r = warp + 8u * (uint32_t)i;
+        if (r >= lo && r < hi)   // absolute values order as their bits do, NaN above infinity
+            mx = max(max(max(mx, __float_as_uint(x[i].x) & 0x7fffffffu), __float_as_uint(x[i].y) & 0x7fffffffu),
+                     max(__float_as_uint(x[i].z) & 0x7fffffffu, __float_as_uint(x[i].w) & 0x7fffffffu));
+    }
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (lane == 0) s_max[warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) mx = max(mx, s_max[w]);
+    const bool bad = mx >= 0x7f800000u || was != was;
+    // divided in 64 bits and rounded once
+    const float fresh = (float)((double)__uint_as_float(mx) / 127.0);
+    const float now = bad ? __int_as_float(0x7fffffff) : fmaxf(fresh, was);
+    const float inv = 1.0f / now;
+    const bool slow = now < 7.8886090522101181e-31f, grew = !bad && now > was;
+    if (threadIdx.x == 0) *sp = now;
+    int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const uint32_t r = warp + 8u * (uint32_t)i;
+        if (r >= hi) continue;
+        int q[4];
+        if (r < lo) {
+            const int w = __float_as_int(x[i].x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                q[j] = (int)(int8_t)(w >> (8 * j));
+                if (grew) q[j] = (int)rint((double)q[j] * (double)was / (double)now);
+            }
+        } else if (bad || now == 0.f) {
+            q[0] = q[1] = q[2] = q[3] = 0;
+        } else {
+            q[0] = quantise(x[i].x, now, inv, slow);
+            q[1] = quantise(x[i].y, now, inv, slow);
+            q[2] = quantise(x[i].z, now, inv, slow);
+            q[3] = quantise(x[i].w, now, inv, slow);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += q[j];
+        if (r >= lo || grew)
+            reinterpret_cast<uint32_t *>(code + (size_t)r * kDim)[lane] =
+                (uint32_t)(q[0] & 255) | (uint32_t)(q[1] & 255) << 8 | (uint32_t)(q[2] & 255) << 16 | (uint32_t)q[3] << 24;
+    }
+    if (is_v || !a.c.k_sum) return;
+    *reinterpret_cast<int4 *>(&s_sum[warp][4 * lane]) = make_int4(sum[0], sum[1], sum[2], sum[3]);
+    __syncthreads();
+    if (threadIdx.x < kDim) {
+        int t = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += s_sum[w][threadIdx.x];
+        a.c.k_sum[(head * a.c.n_blocks + blk) * kDim + threadIdx.x] = (int16_t)t;
+    }
+}
+
+// ----------------------------------------------------------------- read ----
+
+struct ReadArgs {
+    Cache c;
+    Rows r;
+    float *k, *v;
+    uint64_t ld;
+    uint32_t early;
+};
+
+constexpr int kReadRows = 8;   // rows per warp, all loaded before the first is stored
+
+// value = code * scale, one warp per 8 consecutive rows of a KV head (lane = 4
+// dimensions). Bound by HBM: 1 byte read and 4 written per value.
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadArgs a)
+{
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    wait_predecessor(a.early);
+    const uint32_t s = blockIdx.z, h = blockIdx.y >> 1, is_v = blockIdx.y & 1u;
+    const uint32_t n = row_count(a.r, s), i0 = (blockIdx.x * 8u + warp) * kReadRows;
+    if (i0 >= n) return;
+    const uint64_t p0 = __ldcg(a.r.pos0 + s);
+    const size_t head = (size_t)s * a.c.kv_heads + h;
+    const int8_t *code = (is_v ? a.c.v : a.c.k) + head * a.c.max_context * kDim;
+    const float *scale = (is_v ? a.c.v_scale : a.c.k_scale) + head * a.c.n_blocks;
+    float *dst = (is_v ? a.v : a.k) + (size_t)s * a.r.tokens * a.ld + (size_t)h * kDim;
+    int w[kReadRows];
+    float sc[kReadRows];
+#pragma unroll
+    for (int i = 0; i < kReadRows; ++i) {
+        const uint64_t p = p0 + i0 + i;
+        w[i] = 0;
+        sc[i] = __int_as_float(0x7fffffff);   // a position past the cache reads as NaN
+        if (i0 + i < n && p < a.c.max_context) {
+            w[i] = __ldcg(reinterpret_cast<const int *>(code + p * kDim) + lane);
+            sc[i] = __ldcg(scale + (p >> a.c.block_log2));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kReadRows; ++i)
+        if (i0 + i < n)
+            reinterpret_cast<float4 *>(dst + (size_t)(i0 + i) * a.ld)[lane] =
+                make_float4((float)(int8_t)w[i] * sc[i], (float)(int8_t)(w[i] >> 8) * sc[i],
+                            (float)(int8_t)(w[i] >> 16) * sc[i], (float)(w[i] >> 24) * sc[i]);
+}
+
+
+// ------------------------------------------------------ attention, few rows --
+//
+// One cluster of CTAs per (sequence, KV head, tile of 8 NT query rows; rows
+// are (token, head of the group), token-major). The cached positions come in
+// chunks of 16, dealt out over all warps of the cluster; each warp keeps a
+// softmax state of its own (running maximum, sum, output), and the states
+// merge through shared memory, then through the cluster's distributed shared
+// memory: one launch, no workspace.
+//
+// Chunks arrive by cp.async, kStages deep. A lane copies exactly the 16-byte
+// pieces that it reads itself (K: rows g and g + 8, V: rows 2t, 2t + 1,
+// 2t + 8, 2t + 9 of the lane's g = lane / 4, t = lane % 4), so a chunk needs
+// no barrier and its slot [piece][lane] has no bank conflict.
+//
+//   S^T = K Q^T   m16n8k32 integer MMAs straight on the codes (rows are
+//                 positions, columns query rows). Q is staged as three int8
+//                 planes, q = max|q| / 127 (p0 + p1 / 254 + p2 / 254^2), off by
+//                 at most 2^-22 max|q|; the integer sums are exact.
+//   O^T += V^T P^T  m16n8k16 binary16 MMAs (rows are dimensions): the codes are
+//                 exact in binary16, P is split into two terms hi + lo (22
+//                 bits). P enters as p * v_scale / vref * 64, with vref the
+//                 power of two below the largest V scale so far, so that blocks
+//                 of different scales share one accumulator; p <= 2^8 and
+//                 v_scale < 2 vref keep it below 2^15.
+//
+// The maximum is lazy: a warp raises it only when a score passes it by 8 (in
+// the exponent's base 2), which is rare after the first chunk, so a chunk
+// needs no reduction over lanes.
+// Bound by HBM for long caches (256 bytes per position and KV head, read once),
+// by launch and first-byte latency for short ones.
+
+constexpr uint32_t kStages = 3;
+constexpr uint32_t kWarps = 8, kWarpsLog2 = 3, kThreads = kWarps * 32;
+constexpr uint32_t kSlot = 8 * 32 * 16;                     // bytes of a chunk: 16 rows of K and V
+
+constexpr uint32_t kMaxCluster = 16;                        // >= 8 NT: the rows of a tile, or their states
+constexpr uint32_t kRecStride = kDim + 4;                   // output, maximum, sum
+constexpr float kLazy = 8.0f;
+constexpr float kScoreScale = (float)(1.4426950408889634 / 11.313708498984761);   // log2(e) / sqrt(128)
+constexpr uint32_t kTinyScale = 7u << 23;                   // bits of 2^-120: where vref starts
+constexpr int kSumBits = 0x4B400000;                  // 2^23 + 2^22: integer sums below 2^22 read as floats
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], const int (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The first of a sum: onto the constant c in every element
+__device__ __forceinline__ void mma_s8_first(int (&d)[4], const int (&a)[4], uint32_t b0, uint32_t b1, int c)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c));
+}
+
+__device__ __forceinline__ void mma_h(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The transpose of an 8 x 8 matrix of 16-bit values (row = lane / 4, two columns a lane)
+__device__ __forceinline__ uint32_t transpose8(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t h2_bits(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Signed bytes 0 and 2 (odd: 1 and 3) of y as two binary16 numbers: 0x6400 | u
+// is 1024 + u, and u = code + 128 with the sign bit flipped.
+template <bool ODD>
+__device__ __forceinline__ uint32_t codes_h2(uint32_t y)
+{
+    const uint32_t u = ((ODD ? y >> 8 : y) & 0x00ff00ffu) ^ 0x64806480u;
+    const __half2 c = __hsub2(*reinterpret_cast<const __half2 *>(&u), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t *>(&c);
+}
+
+// 16 bytes global -> shared; in the second form nothing is read and zeros are stored where !there
+template <int DST, int SRC>
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
+}
+template <int DST, int SRC>
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there)
+{
+    asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16, %4;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC),
+                 "r"(there ? 16u : 0u)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint32_t cluster_size()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Split: arrive once the CTA runs, wait before the first access to another CTA's shared memory
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_cluster(const float *p, uint32_t cta, float4 v)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(cta));
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(r), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
+}
+__device__ __forceinline__ void st_cluster(unsigned long long *p, uint32_t cta, unsigned long long v)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(cta));
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(r), "l"(v) : "memory");
+}
+
+template <int NT>
+struct alignas(16) Smem {
+    union {
+        uint8_t ring[kWarps][kStages][kSlot];
+        float wrec[kWarps][8 * NT][kRecStride];   // the warps' outputs, once the ring is done with
+    } u;
+    float rec[kMaxCluster][kRecStride];        // the states that the cluster's CTAs send of this CTA's rows
+    float2 wml[kWarps][8 * NT];                // the warps' maxima and sums
+    uint32_t plane[3][8 * NT][kDim / 4 + 16];  // rows 48 words apart: the fragment reads have no bank conflict
+    float qs[8 * NT];                          // what a unit of the first plane is worth in each row
+};
+
+// Which positions a tile's keys are: chunk c holds key0(c) .. key0(c) + 15.
+struct Dense {
+    __device__ __forceinline__ uint32_t key0(uint32_t c) const { return c * kChunk; }
+};
+
+// Query rows of a tile: row i is head `rem + i` of token `tok`, counted on through the group (no division: the
+// factor is 1 / group, a little high, and exact for rem + i < group + 16).
+struct TileRows {
+    uint32_t tok, rem, group;
+    float inv;
+    __device__ __forceinline__ uint2 at(uint32_t i) const   // (token, head of the group)
+    {
+        const uint32_t t = rem + i, q = (uint32_t)((float)t * inv);
+        return make_uint2(tok + q, t - q * group);
+    }
+};
+
+// Four dimensions of the output of the tile's row i; NaN where its position lies past the cache
+__device__ __forceinline__ void store_row(const AttnArgs &a, const TileRows &tr, uint32_t s, uint32_t h, uint32_t i,
+                                          uint64_t p0, uint32_t d4, float4 x)
+{
+    const uint2 r = tr.at(i);
+    const float nan = __int_as_float(0x7fffffff);
+    if (p0 + r.x >= a.c.max_context) x = make_float4(nan, nan, nan, nan);
+    reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo + (size_t)(h * a.group + r.y) * kDim)[d4] = x;
+}
+
+__device__ __forceinline__ float rcp(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// This warp's query rows warp, warp + 8, ... of the tile (lane = 4 dimensions). Rows of tokens that the call does
+// not have are zeros; rows past n_tok are read and their results dropped.
+template <int NT>
+__device__ __forceinline__ void load_queries(const AttnArgs &a, const TileRows &tr, uint32_t s, uint32_t h, float4 (&x)[NT])
+{
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const uint2 r = tr.at(warp + kWarps * (uint32_t)i);
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r.x < a.r.tokens)
+            x[i] = __ldcg(reinterpret_cast<const float4 *>(a.q + ((size_t)s * a.r.tokens + r.x) * a.ldq +
+                                                          (size_t)(h * a.group + r.y) * kDim) + lane);
+    }
+}
+
+// One (sequence, KV head, tile of query rows) on this cluster. `rows`: the
+// tile's rows that exist. KEYS deals chunks [0, chunks); positions at or above
+// `limit` are not read. `open`: every row sees the positions up to it. The
+// CTAs of a cluster have arrived on its barrier once before.
+template <int NT, class KEYS>
+__device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KEYS &keys, const float4 (&qx)[NT],
+                                       const TileRows &tr, uint32_t s, uint32_t h, uint32_t rows, uint64_t p0,
+                                       uint32_t chunks, uint32_t limit)
+{
+    constexpr uint32_t R = 8 * NT;
+    static_assert(R == kWarps * NT, "a warp stages NT query rows");
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t C = cluster_size(), clog = 31u - __clz(C), rank = cluster_rank();
+    const size_t head = (size_t)s * a.c.kv_heads + h;
+    const int8_t *kc = a.c.k + head * a.c.max_context * kDim + g * kDim + 16u * t;
+    const int8_t *vc = a.c.v + head * a.c.max_context * kDim + 2u * t * kDim + 16u * g;
+    const float *ksc = a.c.k_scale + head * a.c.n_blocks, *vsc = a.c.v_scale + head * a.c.n_blocks;
+
+    // this warp's chunks are first, first + step, ...
+    const uint32_t first = rank + (warp << clog), slog = clog + kWarpsLog2;
+    const uint32_t n = chunks > first ? ((chunks - first - 1u) >> slog) + 1u : 0u;
+    const uint32_t slot0 = smem_addr(sm.u.ring[warp][0]) + lane * 16u;
+    auto issue = [&](uint32_t i, uint32_t slot) {
+        if (i < n) {
+            const uint32_t key = keys.key0(first + (i << slog)), dst = slot0 + slot * kSlot;
+            const int8_t *kr = kc + (size_t)key * kDim, *vr = vc + (size_t)key * kDim;
+            if (key + kChunk <= limit) {
+                copy16<0, 0>(dst, kr);
+                copy16<512, 64>(dst, kr);
+                copy16<1024, 8 * kDim>(dst, kr);
+                copy16<1536, 8 * kDim + 64>(dst, kr);
+                copy16<2048, 0>(dst, vr);
+                copy16<2560, kDim>(dst, vr);
+                copy16<3072, 8 * kDim>(dst, vr);
+                copy16<3584, 9 * kDim>(dst, vr);
+            } else {
+                copy16<0, 0>(dst, kr, key + g < limit);
+                copy16<512, 64>(dst, kr, key + g < limit);
+                copy16<1024, 8 * kDim>(dst, kr, key + g + 8u < limit);
+                copy16<1536, 8 * kDim + 64>(dst, kr, key + g + 8u < limit);
+                copy16<2048, 0>(dst, vr, key + 2u * t < limit);
+                copy16<2560, kDim>(dst, vr, key + 2u * t + 1u < limit);
+                copy16<3072, 8 * kDim>(dst, vr, key + 2u * t + 8u < limit);
+                copy16<3584, 9 * kDim>(dst, vr, key + 2u * t + 9u < limit);
+            }
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kStages - 1; ++i) issue(i, i);
+    float ksl, vsl;   // lane: the scales of the warp's chunk 32 (i / 32) + lane
+    auto scales = [&](uint32_t i) {
+        const uint32_t b = keys.key0(min(first + ((i + lane) << slog), chunks - 1u)) >> a.c.block_log2;
+        ksl = __ldcg(ksc + b);
+        vsl = __ldcg(vsc + b);
+    };
+    scales(0u);
+
+    // the query rows as int8 planes; powers of two keep max|q| and its reciprocal away from the ends of the range
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const float v[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
+        uint32_t mx = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = max(mx, __float_as_uint(v[j]) & 0x7fffffffu);
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        const float amax = __uint_as_float(mx);
+        const float up = amax < 0x1p-60f ? 0x1p64f : amax > 0x1p60f ? 0x1p-64f : 1.0f;
+        const float r = 127.0f * rcp(amax * up);
+        uint32_t w[3] = {0u, 0u, 0u};
+        if (mx && mx < 0x7f800000u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float y = v[j] * up * r;
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    const float c = rintf(y);
+                    y = (y - c) * 254.0f;
+                    w[p] |= (uint32_t)((int)c & 255) << (8 * j);
+                }
+            }
+        }
+        const uint32_t row = warp + kWarps * (uint32_t)i;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) sm.plane[p][row][lane] = w[p];
+        // a row with a non-finite value: every score NaN
+        if (lane == 0) sm.qs[row] = mx >= 0x7f800000u ? __int_as_float(0x7fffffff) : mx ? rcp(r) * (amax < 0x1p-60f ? 0x1p-64f : amax > 0x1p60f ? 0x1p64f : 1.0f) : 0.f;
+    }
+    __syncthreads();
+
+    float qs[NT][2];
+    uint32_t last[NT][2];   // the last position that columns 2 t and 2 t + 1 see
+    const uint32_t open = (uint32_t)min(p0 + tr.tok, (uint64_t)0x7fffffffu);   // every row sees the positions up to it
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t i = 8u * (uint32_t)nt + 2u * t + (uint32_t)e;
+            qs[nt][e] = sm.qs[i] * kScoreScale;
+            last[nt][e] = i < rows ? (uint32_t)min(p0 + tr.at(i).x, (uint64_t)0x7fffffffu) : open;
+        }
+
+    float o[NT][8][4], m[NT][2], l[NT][2];
+    uint32_t vref = kTinyScale;   // bits of a power of two
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+    }
+    uint32_t slot = 0u;
+    for (uint32_t i = 0; i < n; ++i) {
+        if ((i & 31u) == 0u && i) scales(i);
+        issue(i + kStages - 1, slot ? slot - 1u : kStages - 1u);   // into the slot that chunk i - 1 left
+        copy_wait<kStages - 1>();
+        const uint32_t key = keys.key0(first + (i << slog));
+        const uint4 *in = reinterpret_cast<const uint4 *>(sm.u.ring[warp][slot]) + lane;
+        slot = slot + 1u == kStages ? 0u : slot + 1u;
+        const float sk = __shfl_sync(0xffffffffu, ksl, i & 31u), sv = __shfl_sync(0xffffffffu, vsl, i & 31u);
+        if (sv >= 2.0f * __uint_as_float(vref)) {   // not where sv is NaN
+            const uint32_t now = __float_as_uint(sv) & 0x7f800000u;
+            const float f = now - vref > 120u << 23 ? 0.f : __uint_as_float((127u << 23) - (now - vref));
+            vref = now;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][j][e] *= f;
+        }
+        const float pf = sv * __uint_as_float((260u << 23) - vref);   // sv / vref * 2^6
+        // scores: positions key + g (elements 0, 1) and key + g + 8 (2, 3), columns 2 t and 2 t + 1
+        float y[NT][4];
+        bool raise = false;
+        const uint32_t pa = key + g, pb = key + g + 8u;
+        const bool masked = key + kChunk - 1u > open;   // some row does not see all of the chunk
+        {
+            const uint4 k0 = in[0], k1 = in[32], k2 = in[64], k3 = in[96];
+            const int ka[4][4] = {{(int)k0.x, (int)k2.x, (int)k0.y, (int)k2.y}, {(int)k0.z, (int)k2.z, (int)k0.w, (int)k2.w},
+                                  {(int)k1.x, (int)k3.x, (int)k1.y, (int)k3.y}, {(int)k1.z, (int)k3.z, (int)k1.w, (int)k3.w}};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                int d[3][4];
+                // B operands: column g, the dimensions of the lane's K pieces (16 t and 64 + 16 t on)
+#pragma unroll
+                for (int pl = 0; pl < 3; ++pl) {
+                    const uint4 lo = *reinterpret_cast<const uint4 *>(&sm.plane[pl][8 * nt + g][4u * t]);
+                    mma_s8_first(d[pl], ka[0], lo.x, lo.y, kSumBits);
+                    mma_s8(d[pl], ka[1], lo.z, lo.w);
+                }
+#pragma unroll
+                for (int pl = 0; pl < 3; ++pl) {
+                    const uint4 hi = *reinterpret_cast<const uint4 *>(&sm.plane[pl][8 * nt + g][16u + 4u * t]);
+                    mma_s8(d[pl], ka[2], hi.x, hi.y);
+                    mma_s8(d[pl], ka[3], hi.z, hi.w);
+                }
+                const float f[2] = {sk * qs[nt][0], sk * qs[nt][1]};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float big = 12582912.0f;
+                    const float x = fmaf(__int_as_float(d[2][e]) - big, 1.0f / 254.0f, __int_as_float(d[1][e]) - big);
+                    y[nt][e] = fmaf(x, 1.0f / 254.0f, __int_as_float(d[0][e]) - big) * f[e & 1];
+                    if (masked && (e < 2 ? pa : pb) > last[nt][e & 1]) y[nt][e] = -INFINITY;
+                    raise |= y[nt][e] > m[nt][e & 1] + kLazy;
+                }
+            }
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaxf(m[nt][e], fmaxf(y[nt][e], y[nt][2 + e]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - x);
+                    m[nt][e] = x;
+                    l[nt][e] *= f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        o[nt][j][e] *= f;
+                        o[nt][j][2 + e] *= f;
+                    }
+                }
+        }
+        uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                z[e] = ex2(y[nt][e] - m[nt][e & 1]);
+                // a masked position counts nothing, whatever its block's scales are
+                const bool seen = !masked || (e < 2 ? pa : pb) <= last[nt][e & 1];
+                if (!seen) z[e] = 0.f;
+                l[nt][e & 1] += z[e];
+                z[e] *= pf;
+                if (!seen) z[e] = 0.f;
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float hi[2], lo[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    hi[e] = __uint_as_float(__float_as_uint(z[2 * half + e]) & 0xffffe000u);   // exact in binary16
+                    lo[e] = z[2 * half + e] - hi[e];
+                }
+                bh[nt][half] = transpose8(h2_bits(hi[0], hi[1]));
+                bl[nt][half] = transpose8(h2_bits(lo[0], lo[1]));
+            }
+        }
+        // O^T += V^T P^T: rows g and g + 8 of MMA j are dimensions 16 g + 2 j and 16 g + 2 j + 1
+        {
+            const uint4 v0 = in[128], v1 = in[160], v2 = in[192], v3 = in[224];
+            const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+            const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t pick = (j & 1) ? 0x7632u : 0x5410u;
+                const uint32_t ya = __byte_perm(w0[j >> 1], w1[j >> 1], pick), yb = __byte_perm(w2[j >> 1], w3[j >> 1], pick);
+                const uint32_t va[4] = {codes_h2<false>(ya), codes_h2<true>(ya), codes_h2<false>(yb), codes_h2<true>(yb)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_h(o[nt][j], va, bh[nt][0], bh[nt][1]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_h(o[nt][j], va, bl[nt][0], bl[nt][1]);
+            }
+        }
+    }
+    copy_wait<0>();
+    __syncthreads();   // every warp is done with the ring: it takes the warps' outputs
+
+    const float back = __uint_as_float(vref) * (1.0f / 64.0f);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float x = l[nt][e];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            const uint32_t i = 8u * (uint32_t)nt + 2u * t + (uint32_t)e;
+            if (g == 0u) sm.wml[warp][i] = make_float2(m[nt][e], x);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                *reinterpret_cast<float4 *>(&sm.u.wrec[warp][i][16u * g + 2u * (uint32_t)j]) =
+                    make_float4(o[nt][j][e] * back, o[nt][j][2 + e] * back, o[nt][j + 1][e] * back, o[nt][j + 1][2 + e] * back);
+        }
+    if (C > 1u) cluster_wait();   // the other CTAs run: their shared memory may be written
+    __syncthreads();
+    // The warps' states -> the CTA's state of each row, straight to the CTA of
+    // the cluster that owns the row (row i: CTA i % C). A state that saw no
+    // position (maximum -inf, sum 0) counts nothing.
+    const uint32_t plog = 3u + (NT - 1u) > clog ? 3u + (NT - 1u) - clog : 0u;   // log2 of the rows that a CTA owns
+    {
+        constexpr uint32_t kPer = kThreads / R;   // threads per row, 4 dimensions at a time
+        const uint32_t i = threadIdx.x / kPer, part = threadIdx.x % kPer;
+        float2 ml[kWarps];
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            ml[w] = sm.wml[w][i];
+            M = fmaxf(M, ml[w].x);
+        }
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            ml[w].x = ml[w].x == -INFINITY && ml[w].y == 0.f ? 0.f : ex2(ml[w].x - M);
+            L = fmaf(ml[w].x, ml[w].y, L);
+        }
+        const float inv = 1.0f / L;
+#pragma unroll
+        for (uint32_t d = part; d < kDim / 4u; d += kPer) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                const float4 y = *reinterpret_cast<const float4 *>(&sm.u.wrec[w][i][4u * d]);
+                x.x = fmaf(ml[w].x, y.x, x.x);
+                x.y = fmaf(ml[w].x, y.y, x.y);
+                x.z = fmaf(ml[w].x, y.z, x.z);
+                x.w = fmaf(ml[w].x, y.w, x.w);
+            }
+            if (i >= rows) continue;
+            if (C == 1u) store_row(a, tr, s, h, i, p0, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+            else st_cluster(&sm.rec[(rank << plog) + (i >> clog)][4u * d], i & (C - 1u), x);
+        }
+        if (C > 1u && part == 0u && i < rows)
+            st_cluster(&sm.rec[(rank << plog) + (i >> clog)][kDim], i & (C - 1u), make_float4(M, L, 0.f, 0.f));
+    }
+    if (C == 1u) return;
+    cluster_sync();   // every record has arrived; nothing remote is touched from here on
+    // warp k: row rank + k C; lane: a CTA's maximum and sum, then 4 dimensions
+    const uint32_t i = rank + (warp << clog);
+    if (warp >= (1u << plog) || i >= min(rows, R)) return;
+    const float *rec = sm.rec[(lane << plog) + warp];
+    const float mc = lane < C ? rec[kDim] : -INFINITY, lc = lane < C ? rec[kDim + 1] : 0.f;
+    float M = mc;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o, 16));
+    const float f = mc == -INFINITY && lc == 0.f ? 0.f : ex2(mc - M);
+    float L = f * lc;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o, 16);
+    L = __shfl_sync(0xffffffffu, L, 0);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (uint32_t c = 0; c < C; ++c) {
+        const float4 y = *reinterpret_cast<const float4 *>(&sm.rec[(c << plog) + warp][4u * lane]);
+        const float fc = __shfl_sync(0xffffffffu, f, (int)c);
+        x.x = fmaf(fc, y.x, x.x);
+        x.y = fmaf(fc, y.y, x.y);
+        x.z = fmaf(fc, y.z, x.z);
+        x.w = fmaf(fc, y.w, x.w);
+    }
+    const float inv = 1.0f / L;
+    store_row(a, tr, s, h, i, p0, lane, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) attn_kernel(const __grid_constant__ AttnArgs a)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(smem_raw);
+    const uint32_t s = blockIdx.z, h = blockIdx.y, r0 = (blockIdx.x >> (31 - __clz(cluster_size()))) * 8u * NT;
+    if (cluster_size() > 1u) cluster_arrive();
+    TileRows tr{0u, 0u, a.group, a.group_inv};
+    if (r0) {
+        tr.tok = r0 / a.group;
+        tr.rem = r0 - tr.tok * a.group;
+    }
+    wait_predecessor(a.early);
+    const uint64_t p0 = __ldcg(a.r.pos0 + s);
+    const uint32_t all = row_count(a.r, s) * a.group;
+    float4 q[NT];
+    load_queries<NT>(a, tr, s, h, q);
+    if (r0 >= all) {   // the whole cluster leaves
+        if (cluster_size() > 1u) cluster_wait();
+        return;
+    }
+    const uint32_t rows = min(all - r0, 8u * NT);
+    const uint32_t limit = (uint32_t)min(p0 + tr.at(rows - 1u).x + 1u, (uint64_t)a.c.max_context);
+    attend<NT>(a, sm, Dense{}, q, tr, s, h, rows, p0, (limit + kChunk - 1u) / kChunk, limit);
+}
+
+// ------------------------------------------------- attention, chosen blocks --
+//
+// One cluster per (sequence, token, KV head): the blocks before the token's own
+// are scored, the best n_sel - 1 of them and the token's own block are
+// attended. Score of block b: the group's query rows are summed (64 bits) and
+// rounded to int8, c = rint(127 qbar / max|qbar|); the score is
+// (c . k_sum_b) * k_scale_b, an integer dot product times one fp32 factor.
+// Both are exact in 64 bits (28 + 24 bits), so the choice does not depend on
+// the order of any sum; equal scores go to the lower block. A NaN score stands
+// above every number: a poisoned block is chosen and shows in the output.
+// The CTAs of the cluster score every C-th block each, send the keys to all of
+// them, and each picks the blocks on its own (a radix search from the highest
+// bit in which the keys differ), so the whole operator is one launch.
+// Bound by latency: 260 bytes per candidate block, then n_sel blocks.
+
+struct Chosen {
+    const uint32_t *list;
+    uint32_t per_log2, block_log2;   // chunks per block, positions per block
+    __device__ __forceinline__ uint32_t key0(uint32_t c) const
+    {
+        return (list[c >> per_log2] << block_log2) + (c & ((1u << per_log2) - 1u)) * kChunk;
+    }
+};
+
+struct PickSmem {
+    int8_t code[kDim];
+    unsigned long long red[2][kWarps];
+    uint32_t hist[256];
+    uint32_t digit, need, exact, scan[kWarps];
+};
+
+// The keys lie behind PickSmem in the ring, which the attention fills later.
+constexpr uint32_t kMaxBlocks = (uint32_t)((kWarps * kStages * kSlot - sizeof(PickSmem)) / 8u);
+
+// The group's pooled query of one token as int8 codes. All threads; threads 0 .. 127 = dimensions.
+__device__ __forceinline__ void pool_query(const AttnArgs &a, PickSmem &ps, const float *q)
+{
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    double x = 0.0;
+    if (threadIdx.x < kDim)
+#pragma unroll 8
+        for (uint32_t i = 0; i < a.group; ++i) x += (double)__ldcg(q + (size_t)i * kDim + threadIdx.x);
+    unsigned long long b = (unsigned long long)__double_as_longlong(fabs(x));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    if (lane == 0) ps.red[0][warp] = b;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) b = max(b, ps.red[0][w]);
+    const double most = __longlong_as_double((long long)b);
+    if (threadIdx.x < kDim)
+        ps.code[threadIdx.x] = most > 0.0 && most < INFINITY ? (int8_t)(int)rint(127.0 * x / most) : (int8_t)0;
+    __syncthreads();
+}
+
+// Keys of blocks rank, rank + C, ... below nb, into every CTA's `key`: 8 lanes per block, 16 dimensions each.
+__device__ __forceinline__ void score_blocks(const AttnArgs &a, const PickSmem &ps, size_t head, uint32_t nb,
+                                             unsigned long long *key, uint32_t C, uint32_t rank)
+{
+    const uint32_t part = threadIdx.x & 7u, grp = threadIdx.x >> 3;
+    const int4 qc = *reinterpret_cast<const int4 *>(ps.code + 16u * part);
+    const int16_t *sums = a.c.k_sum + head * a.c.n_blocks * kDim + 16u * part;
+    const float *scale = a.c.k_scale + head * a.c.n_blocks;
+    const uint32_t step = C * (kThreads / 8u);
+#pragma unroll 4
+    for (uint32_t base = rank; base < nb; base += step) {   // uniform over the CTA: the shuffles are whole
+        const uint32_t b = base + C * grp;
+        int4 u = make_int4(0, 0, 0, 0), v = u;
+        float sc = 0.f;
+        if (b < nb) {
+            const int4 *row = reinterpret_cast<const int4 *>(sums + (size_t)b * kDim);
+            u = __ldcg(row);
+            v = __ldcg(row + 1);
+            sc = __ldcg(scale + b);
+        }
+        int d = __dp2a_lo(u.x, qc.x, 0);
+        d = __dp2a_hi(u.y, qc.x, d);
+        d = __dp2a_lo(u.z, qc.y, d);
+        d = __dp2a_hi(u.w, qc.y, d);
+        d = __dp2a_lo(v.x, qc.z, d);
+        d = __dp2a_hi(v.y, qc.z, d);
+        d = __dp2a_lo(v.z, qc.w, d);
+        d = __dp2a_hi(v.w, qc.w, d);
+        d += __shfl_xor_sync(0xffffffffu, d, 1);
+        d += __shfl_xor_sync(0xffffffffu, d, 2);
+        d += __shfl_xor_sync(0xffffffffu, d, 4);
+        const double x = (double)d * (double)sc + 0.0;   // + 0: one zero
+        unsigned long long k = (unsigned long long)__double_as_longlong(x);
+        k = x != x ? ~0ull : (k >> 63) ? ~k : k | 1ull << 63;   // orders as the scores do
+        if (b < nb) {
+            if (C == 1u) {
+                if (part == 0u) key[b] = k;
+            } else {
+                for (uint32_t c = part; c < C; c += 8u) st_cluster(key + b, c, k);
+            }
+        }
+    }
+}
+
+// The `want` largest of key[0, nb), 0 < want < nb, as ascending block numbers
+// in list[0, want); equal keys go to the lower number. All threads.
+__device__ __forceinline__ void pick_blocks(PickSmem &ps, const unsigned long long *key, uint32_t nb, uint32_t want,
+                                            uint32_t *list)
+{
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    unsigned long long all = ~0ull, any = 0ull;
+    for (uint32_t i = threadIdx.x; i < nb; i += kThreads) {
+        all &= key[i];
+        any |= key[i];
+    }
+    all = (unsigned long long)__reduce_and_sync(0xffffffffu, (uint32_t)(all >> 32)) << 32 |
+          __reduce_and_sync(0xffffffffu, (uint32_t)all);
+    any = (unsigned long long)__reduce_or_sync(0xffffffffu, (uint32_t)(any >> 32)) << 32 |
+          __reduce_or_sync(0xffffffffu, (uint32_t)any);
+    if (lane == 0) {
+        ps.red[0][warp] = all;
+        ps.red[1][warp] = any;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) {
+        all &= ps.red[0][w];
+        any |= ps.red[1][w];
+    }
+    // Invariant: keys with (key >> shift) > prefix are chosen, and `need` of those with (key >> shift) == prefix
+    const int top = 64 - __clzll((long long)(all ^ any));   // bits above it are common to all keys
+    int shift = top;
+    unsigned long long prefix = top < 64 ? all >> top : 0ull;
+    uint32_t need = want;
+    bool exact = false;   // every key with that prefix is chosen
+    while (shift > 0 && !exact) {
+        const int width = min(8, shift), next = shift - width;
+        for (uint32_t i = threadIdx.x; i < 256u; i += kThreads) ps.hist[i] = 0u;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < nb; i += kThreads) {
+            const unsigned long long k = key[i];
+            if (shift >= 64 || (k >> shift) == prefix) atomicAdd(&ps.hist[(uint32_t)(k >> next) & ((1u << width) - 1u)], 1u);
+        }
+        __syncthreads();
+        if (warp == 0) {   // lane: digits 255 - 8 lane down to 248 - 8 lane
+            uint32_t c[8], sum = 0u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                c[j] = ps.hist[255u - 8u * lane - (uint32_t)j];
+                sum += c[j];
+            }
+            uint32_t inc = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= (uint32_t)o) inc += up;
+            }
+            uint32_t above = inc - sum;
+            if (above < need && inc >= need) {   // one lane: the digit at which the count passes `need`
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (above < need && above + c[j] >= need) {
+                        ps.digit = 255u - 8u * lane - (uint32_t)j;
+                        ps.need = need - above;
+                        ps.exact = c[j] == need - above;
+                    }
+                    above += c[j];
+                }
+            }
+        }
+        __syncthreads();
+        prefix = prefix << width | ps.digit;
+        need = ps.need;
+        exact = ps.exact != 0u;
+        shift = next;
+    }
+    // thread: a run of consecutive blocks; (chosen above, equal) counts of the runs before it in one word
+    const uint32_t per = (nb + kThreads - 1u) / kThreads, b0 = min(threadIdx.x * per, nb), b1 = min(b0 + per, nb);
+    uint32_t cnt = 0u;
+    for (uint32_t b = b0; b < b1; ++b) {
+        const unsigned long long k = shift < 64 ? key[b] >> shift : 0ull;
+        cnt += k > prefix ? 1u : k == prefix ? 1u << 16 : 0u;
+    }
+    uint32_t inc = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= (uint32_t)o) inc += up;
+    }
+    if (lane == 31u) ps.scan[warp] = inc;
+    __syncthreads();
+    uint32_t before = inc - cnt;
+    for (uint32_t w = 0; w < warp; ++w) before += ps.scan[w];
+    uint32_t gt = before & 0xffffu, eq = before >> 16;
+    for (uint32_t b = b0; b < b1; ++b) {
+        const unsigned long long k = shift < 64 ? key[b] >> shift : 0ull;
+        const bool take = k > prefix || (k == prefix && eq < need);
+        if (take) list[gt + min(eq, need)] = b;
+        gt += k > prefix ? 1u : 0u;
+        eq += k == prefix ? 1u : 0u;
+    }
+    __syncthreads();
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const __grid_constant__ AttnArgs a)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(smem_raw);
+    PickSmem &ps = *reinterpret_cast<PickSmem *>(sm.u.ring);
+    unsigned long long *key = reinterpret_cast<unsigned long long *>(&ps + 1);
+    uint32_t *list = reinterpret_cast<uint32_t *>(smem_raw + sizeof(Smem<NT>));
+    const uint32_t C = cluster_size(), rank = cluster_rank();
+    const uint32_t s = blockIdx.z, h = blockIdx.y, unit = blockIdx.x >> (31 - __clz(C));
+    const uint32_t token = a.tiles == 1u ? unit : unit / a.tiles, tile = unit - token * a.tiles;
+    const TileRows tr{token, tile * 8u * NT, a.group, a.group_inv};
+    if (C > 1u) cluster_arrive();
+    wait_predecessor(a.early);
+    const uint64_t p0 = __ldcg(a.r.pos0 + s);
+    const uint32_t n = row_count(a.r, s);
+    float4 q[NT];
+    load_queries<NT>(a, tr, s, h, q);
+    if (token >= n) {   // the whole cluster leaves
+        if (C > 1u) cluster_wait();
+        return;
+    }
+    const bool inside = p0 + token < a.c.max_context;
+    const uint32_t p = inside ? (uint32_t)(p0 + token) : a.c.max_context - 1u;
+    const uint32_t own = p >> a.c.block_log2, want = min(own, a.n_sel - 1u);
+    const size_t head = (size_t)s * a.c.kv_heads + h;
+    if (own > want && want) {
+        pool_query(a, ps, a.q + ((size_t)s * a.r.tokens + token) * a.ldq + (size_t)h * a.group * kDim);
+        // the other CTAs' shared memory is written from here on: they have to run
+        if (C > 1u) cluster_wait();
+        score_blocks(a, ps, head, own, key, C, rank);
+        if (C > 1u) {
+            cluster_sync();
+            cluster_arrive();
+        } else {
+            __syncthreads();
+        }
+        pick_blocks(ps, key, own, want, list);
+    } else {
+        for (uint32_t i = threadIdx.x; i < want; i += kThreads) list[i] = i;
+    }
+    if (threadIdx.x == 0) list[want] = own;
+    __syncthreads();
+    if (rank == 0 && tile == 0) {
+        int32_t *sel = a.sel + (((size_t)s * a.r.tokens + token) * a.c.kv_heads + h) * a.n_sel;
+        for (uint32_t i = threadIdx.x; i < a.n_sel; i += kThreads) sel[i] = inside && i <= want ? (int32_t)list[i] : -1;
+    }
+    const uint32_t per = a.c.block_log2 - 4u;
+    const uint32_t chunks = (want << per) + ((p & ((1u << a.c.block_log2) - 1u)) / kChunk) + 1u;
+    attend<NT>(a, sm, Chosen{list, per, a.c.block_log2}, q, tr, s, h, min(a.group - tile * 8u * NT, 8u * NT), p0, chunks,
+               p + 1u);
+}
+
+// ------------------------------------------------------------- host side ----
+
+// A launch that may overlap its predecessor's end (the kernels wait for it), in clusters of `cluster` CTAs along x.
+template <class ARGS>
+cudaError_t launch(void (*kernel)(ARGS), dim3 grid, uint32_t threads, size_t smem, uint32_t cluster, ARGS a, int sms,
+                   cudaStream_t stream)
+{
+    a.early = (uint64_t)grid.x * grid.y * grid.z <= (uint64_t)sms;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// Lets a kernel take up to the device's shared memory and clusters of 16, once per device.
+template <auto KERNEL>
+cudaError_t allow(int dev, int bytes)
+{
+    static std::atomic<bool> done[64];
+    if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+    return e;
+}
+
+constexpr size_t kMaxSmem = 232448;   // shared memory a CTA may have
+
+// CTAs per unit of work: as many as fill the device, at most 16 (the largest
+// cluster) and one per 64 positions (a chunk for each warp).
+uint32_t cluster_of(uint64_t units, uint64_t slots, uint64_t positions)
+{
+    uint32_t c = 1;
+    while (c < 16 && units * c * 2 <= slots && (uint64_t)c * 2 * kChunk * kWarps <= positions + kChunk * kWarps) c *= 2;
+    return c;
+}
+
+bool on_device(const void *p, int dev)
+{
+    cudaPointerAttributes at{};
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev);
+}
+
+bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// The checks that all calls share; fills the kernel's view of the cache.
+int open_cache(const char *who, const AtlasKv8 *c, uint32_t tokens, const uint32_t *pos0, const uint32_t *n_tok, Cache &out,
+               Rows &rows, int &dev, int &sms)
+{
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !pos0)
+        return api_fail(ATLAS_EINVAL, "%s: null argument", who);
+    if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)
+        return api_fail(ATLAS_EINVAL, "%s: blocks of 16, 32, 64 or 128 positions, not %u", who, c->block);
+    if (!c->nseq || c->nseq > 65535u || !c->kv_heads || c->kv_heads > 16384u || !c->max_context ||
+        c->max_context > 0x7fffff00u)
+        return api_fail(ATLAS_EINVAL, "%s: bad cache shape (%u sequences, %u KV heads, %u positions)", who, c->nseq,
+                        c->kv_heads, c->max_context);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_sum, 16) || !aligned(c->k_scale, 4) ||
+        !aligned(c->v_scale, 4) || !aligned(pos0, 4) || !aligned(n_tok, 4))
+        return api_fail(ATLAS_EINVAL, "%s: codes and sums must be 16-byte aligned, the rest 4-byte", who);
+    if (tokens > 0x00ffffffu) return api_fail(ATLAS_EINVAL, "%s: at most 2^24 - 1 tokens, not %u", who, tokens);
+    dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || api_device(dev, &sms) != ATLAS_OK)
+        return api_fail(ATLAS_ENODEV, "%s: no sm_100 device", who);
+    const void *need[] = {c->k, c->v, c->k_scale, c->v_scale, pos0, c->k_sum, n_tok};
+    for (const void *p : need)
+        if (p && !on_device(p, dev))
+            return api_fail(ATLAS_EINVAL, "%s: the cache, pos0 and n_tok must be memory of the current device", who);
+    out.k = static_cast<int8_t *>(c->k);
+    out.v = static_cast<int8_t *>(c->v);
+    out.k_scale = c->k_scale;
+    out.v_scale = c->v_scale;
+    out.k_sum = c->k_sum;
+    out.nseq = c->nseq;
+    out.kv_heads = c->kv_heads;
+    out.max_context = c->max_context;
+    out.block_log2 = c->block == 16 ? 4 : c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
+    out.n_blocks = (c->max_context + c->block - 1) / c->block;
+    rows.pos0 = pos0;
+    rows.n_tok = n_tok;
+    rows.tokens = tokens;
+    return ATLAS_OK;
+}
+
+// Token rows of `heads` x 128 floats, ld floats apart (0: dense).
+int check_rows(const char *who, const void *p, const void *q, uint32_t heads, uint64_t &ld, int dev)
+{
+    if (!p || !q) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
+    if (!ld) ld = (uint64_t)heads * kDim;
+    if (ld < (uint64_t)heads * kDim || ld % 4 || ld > 0xffffffffull)
+        return api_fail(ATLAS_EINVAL, "%s: token rows %llu floats apart: at least heads x 128, a multiple of 4", who,
+                        (unsigned long long)ld);
+    if (!aligned(p, 16) || !aligned(q, 16)) return api_fail(ATLAS_EINVAL, "%s: token rows must be 16-byte aligned", who);
+    if (!on_device(p, dev) || !on_device(q, dev))
+        return api_fail(ATLAS_EINVAL, "%s: token rows must be memory of the current device", who);
+    return ATLAS_OK;
+}
+
+int done(const char *who, cudaError_t e)
+{
+    if (e == cudaSuccess) return ATLAS_OK;
+    cudaGetLastError();
+    return api_fail(ATLAS_ECUDA, "%s: %s", who, cudaGetErrorString(e));
+}
+
+template <int NT>
+cudaError_t launch_attn(const AttnArgs &a, int dev, int sms, cudaStream_t stream)
+{
+    cudaError_t e = allow<attn_kernel<NT>>(dev, (int)kMaxSmem);
+    if (e != cudaSuccess) return e;
+    const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
+    const uint32_t C = cluster_of(units, (uint64_t)sms * (NT == 1 ? 2 : 1), a.c.max_context);
+    return launch(attn_kernel<NT>, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), kThreads, sizeof(Smem<NT>), C, a, sms, stream);
+}
+
+template <int NT>
+cudaError_t launch_sparse(const AttnArgs &a, int dev, int sms, cudaStream_t stream)
+{
+    cudaError_t e = allow<sparse_kernel<NT>>(dev, (int)kMaxSmem);
+    if (e != cudaSuccess) return e;
+    const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.r.tokens * a.tiles;
+    const uint32_t C = cluster_of(units, (uint64_t)sms * (NT == 1 ? 2 : 1), (uint64_t)a.n_sel << a.c.block_log2);
+    return launch(sparse_kernel<NT>, dim3(C * a.r.tokens * a.tiles, a.c.kv_heads, a.c.nseq), kThreads,
+                  sizeof(Smem<NT>) + (size_t)a.n_sel * 4u, C, a, sms, stream);
+}
+
+}  // namespace
+}  // namespace k8
+}  // namespace atlas
+
+using namespace atlas;
+using namespace atlas::k8;
+
+extern "C" int atlas_cuda_kv8_append(const AtlasKv8 *cache, uint32_t tokens, const uint32_t *d_pos0, const uint32_t *d_ntok,
+                                     const float *d_k, const float *d_v, uint64_t ld, void *stream)
+{
+    const char *who = "kv8_append";
+    AppendArgs a{};
+    int dev, sms, rc = open_cache(who, cache, tokens, d_pos0, d_ntok, a.c, a.r, dev, sms);
+    if (rc == ATLAS_OK) rc = check_rows(who, d_k, d_v, cache->kv_heads, ld, dev);
+    if (rc != ATLAS_OK || !tokens) return rc;
+    a.k = d_k;
+    a.v = d_v;
+    a.ld = ld;
+    // the first row may be the last of its block
+    const dim3 grid((tokens + 2 * cache->block - 2) / cache->block, 2 * cache->kv_heads, cache->nseq);
+    auto *kernel = cache->block == 16   ? append_kernel<16>
+                   : cache->block == 32 ? append_kernel<32>
+                   : cache->block == 64 ? append_kernel<64>
+                                        : append_kernel<128>;
+    return done(who, launch(kernel, grid, 256, 0, 1, a, sms, (cudaStream_t)stream));
+}
+
+extern "C" int atlas_cuda_kv8_read(const AtlasKv8 *cache, uint32_t tokens, const uint32_t *d_pos0, const uint32_t *d_ntok,
+                                   float *d_k, float *d_v, uint64_t ld, void *stream)
+{
+    const char *who = "kv8_read";
+    ReadArgs a{};
+    int dev, sms, rc = open_cache(who, cache, tokens, d_pos0, d_ntok, a.c, a.r, dev, sms);
+    if (rc == ATLAS_OK) rc = check_rows(who, d_k, d_v, cache->kv_heads, ld, dev);
+    if (rc != ATLAS_OK || !tokens) return rc;
+    a.k = d_k;
+    a.v = d_v;
+    a.ld = ld;
+    const dim3 grid((tokens + 8 * kReadRows - 1) / (8 * kReadRows), 2 * cache->kv_heads, cache->nseq);
+    return done(who, launch(read_kernel, grid, 256, 0, 1, a, sms, (cudaStream_t)stream));
+}
+
+namespace {
+
+int attn_args(const char *who, const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
+              const uint32_t *d_ntok, const float *d_q, uint64_t ldq, float *d_out, uint64_t ldo, AttnArgs &a, int &dev,
+              int &sms)
+{
+    int rc = open_cache(who, cache, tokens, d_pos0, d_ntok, a.c, a.r, dev, sms);
+    if (rc != ATLAS_OK) return rc;
+    if (!q_heads || q_heads % cache->kv_heads || q_heads > 32768u || (uint64_t)q_heads * tokens > 0x3fffffffull)
+        return api_fail(ATLAS_EINVAL, "%s: %u query heads over %u KV heads, %u tokens", who, q_heads, cache->kv_heads, tokens);
+    if ((rc = check_rows(who, d_q, d_q, q_heads, ldq, dev)) != ATLAS_OK) return rc;
+    if ((rc = check_rows(who, d_out, d_out, q_heads, ldo, dev)) != ATLAS_OK) return rc;
+    a.q = d_q;
+    a.out = d_out;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.q_heads = q_heads;
+    a.group = q_heads / cache->kv_heads;
+    a.group_inv = 1.000001f / (float)a.group;
+    return ATLAS_OK;
+}
+
+}  // namespace
+
+extern "C" int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
+                                   const uint32_t *d_ntok, const float *d_q, uint64_t ldq, float *d_out, uint64_t ldo,
+                                   void *stream)
+{
+    const char *who = "kv8_attn";
+    AttnArgs a{};
+    int dev, sms;
+    const int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
+    if (rc != ATLAS_OK || !tokens) return rc;
+    const uint32_t rows = tokens * a.group;
+    const bool one = rows <= 8;
+    a.tiles = one ? 1 : (rows + 15) / 16;
+    return done(who, one ? launch_attn<1>(a, dev, sms, (cudaStream_t)stream) : launch_attn<2>(a, dev, sms, (cudaStream_t)stream));
+}
+
+extern "C" int atlas_cuda_kv8_attn_sparse(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, uint32_t n_sel,
+                                          const uint32_t *d_pos0, const uint32_t *d_ntok, const float *d_q, uint64_t ldq,
+                                          float *d_out, uint64_t ldo, int32_t *d_sel, void *stream)
+{
+    const char *who = "kv8_attn_sparse";
+    AttnArgs a{};
+    int dev, sms;
+    const int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
+    if (rc != ATLAS_OK) return rc;
+    if (!cache->k_sum) return api_fail(ATLAS_EINVAL, "%s: the cache has no k_sum", who);
+    if (!d_sel || !aligned(d_sel, 4) || !on_device(d_sel, dev))
+        return api_fail(ATLAS_EINVAL, "%s: sel must be 4-byte aligned memory of the current device", who);
+    if (!n_sel || n_sel > 4096u) return api_fail(ATLAS_EINVAL, "%s: 1 to 4096 blocks per token, not %u", who, n_sel);
+    if (a.c.n_blocks > kMaxBlocks)
+        return api_fail(ATLAS_EINVAL, "%s: a cache of %u blocks: %u can be scored; take larger blocks", who, a.c.n_blocks,
+                        kMaxBlocks);
+    const bool one = a.group <= 8;
+    a.tiles = one ? 1 : (a.group + 15) / 16;
+    if ((uint64_t)tokens * a.tiles > 0x7ffffffull) return api_fail(ATLAS_EINVAL, "%s: too many rows", who);
+    if (!tokens) return ATLAS_OK;
+    a.n_sel = n_sel;
+    a.sel = d_sel;
+    return done(who, one ? launch_sparse<1>(a, dev, sms, (cudaStream_t)stream)
+                         : launch_sparse<2>(a, dev, sms, (cudaStream_t)stream));
+}

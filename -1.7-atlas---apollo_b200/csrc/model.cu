@@ -2158,6 +2158,22 @@ int run_graphb(AtlasCuda *h, uint32_t nseq, const uint32_t *tok, const uint32_t 
 
 }  // namespace
 
+// For the other files' entry points: the last-error text and the cached device check.
+namespace atlas {
+
+int api_fail(int code, const char *fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_tls_error, sizeof(g_tls_error), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+int api_device(int device, int *sms) { return device_ok(device, sms); }
+
+}  // namespace atlas
+
 extern "C" {
 
 int atlas_cuda_device_info(int device, int *sm_count, int *cc_major, int *cc_minor)

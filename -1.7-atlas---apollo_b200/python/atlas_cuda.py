@@ -29,6 +29,7 @@ EXPORTS = [
     "atlas_cuda_gemv", "atlas_cuda_gemm", "atlas_cuda_device_info", "atlas_cuda_trace_step",
     "atlas_cuda_device_ms", "atlas_cuda_trace_graph", "atlas_cuda_gemv_noalloc", "atlas_cuda_tp_slice", "atlas_cuda_tp_handle",
     "atlas_cuda_tp_connect", "atlas_cuda_prefill_seq", "atlas_cuda_generate_batch", "atlas_cuda_decode_batch",
+    "atlas_cuda_kv8_append", "atlas_cuda_kv8_read", "atlas_cuda_kv8_attn", "atlas_cuda_kv8_attn_sparse",
     "brain_gpu_init", "brain_gpu_matvec_batch", "brain_gpu_matvec", "brain_gpu_shutdown",
     "atlas_rt_open", "atlas_rt_close", "atlas_rt_error", "atlas_rt_shape", "atlas_rt_data_base",
     "atlas_rt_find_tensor", "atlas_rt_file_bytes", "atlas_rt_device", "atlas_rt_forward_token",
@@ -89,6 +90,12 @@ class TpSlice(ctypes.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+class Kv8Desc(ctypes.Structure):
+    """AtlasKv8 (include/atlas_cuda.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_sum")] + [
+        (n, ctypes.c_uint32) for n in ("nseq", "kv_heads", "max_context", "block")]
+
+
 TP_HANDLE_BYTES = 64
 
 
@@ -143,6 +150,10 @@ def lib() -> ctypes.CDLL:
         L.atlas_cuda_prefill_seq.argtypes = [P, U32, P, U32, U32, P, P]
         L.atlas_cuda_generate_batch.argtypes = [P, U32, P, P, U32, P]
         L.atlas_cuda_decode_batch.argtypes = [P, U32, P, P, P, P]
+        L.atlas_cuda_kv8_append.argtypes = [P, U32, P, P, P, P, U64, P]
+        L.atlas_cuda_kv8_read.argtypes = [P, U32, P, P, P, P, U64, P]
+        L.atlas_cuda_kv8_attn.argtypes = [P, U32, U32, P, P, P, U64, P, U64, P]
+        L.atlas_cuda_kv8_attn_sparse.argtypes = [P, U32, U32, U32, P, P, P, U64, P, U64, P, P]
         L.atlas_synth_write_gguf.argtypes = [P, ctypes.c_char_p]
         L.atlas_synth_q4k_blocks.argtypes = [U64, U64, P, U64]
         L.atlas_synth_q6k_blocks.argtypes = [U64, U64, P, U64]
@@ -394,3 +405,58 @@ def gemv_noalloc(type_id: int, d_w, rows: int, cols: int, d_x, d_y, stream: int 
 def gemm(type_id: int, d_w, rows: int, cols: int, d_x, tokens: int, d_y, stream: int = 0) -> None:
     check(lib().atlas_cuda_gemm(type_id, _ptr(d_w), rows, cols, _ptr(d_x), tokens, _ptr(d_y),
                                 ctypes.c_void_p(stream)), "atlas_cuda_gemm")
+
+
+class Kv8Cache:
+    """An 8-bit KV cache of one layer in caller-owned device buffers (AtlasKv8, include/atlas_cuda.h).
+
+    k, v: int8 [nseq, kv_heads, max_context, 128]; k_scale, v_scale: float32 [nseq, kv_heads, ceil(max_context / block)];
+    k_sum: int16 [nseq, kv_heads, ceil(max_context / block), 128], or None (kv8_attn_sparse then refuses the cache).
+    The object keeps references to the buffers; they must be dense, which is checked where they say so."""
+
+    def __init__(self, k, v, k_scale, v_scale, k_sum=None, *, nseq: int, kv_heads: int, max_context: int, block: int):
+        blocks = -(-max_context // block) if block > 0 else 0
+        for t, n, size in ((k, max_context * 128, 1), (v, max_context * 128, 1), (k_scale, blocks, 4),
+                           (v_scale, blocks, 4), (k_sum, blocks * 128, 2)):
+            if hasattr(t, "is_contiguous") and (not t.is_contiguous() or t.element_size() != size
+                                                or t.numel() != nseq * kv_heads * n):
+                raise ValueError("Kv8Cache: a buffer of another size or type, or one that is not dense")
+        self.buffers = (k, v, k_scale, v_scale, k_sum)
+        self.nseq, self.kv_heads, self.max_context, self.block = nseq, kv_heads, max_context, block
+        self.desc = Kv8Desc(*(None if t is None else t.data_ptr() for t in self.buffers), nseq, kv_heads, max_context,
+                            block)
+        self._ref = ctypes.byref(self.desc)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def kv8_append(cache: Kv8Cache, tokens: int, pos0, k, v, n_tok=None, ld: int = 0, stream: int = 0) -> None:
+    """Stores up to `tokens` new rows k, v [nseq, tokens, kv_heads, 128] of each sequence s at positions pos0[s], ...
+    (pos0, n_tok: 32-bit device integers; n_tok None: all of them). atlas_cuda_kv8_append."""
+    check(lib().atlas_cuda_kv8_append(cache._ref, tokens, pos0.data_ptr(), _addr(n_tok), k.data_ptr(), v.data_ptr(), ld,
+                                      stream), "kv8_append")
+
+
+def kv8_read(cache: Kv8Cache, tokens: int, pos0, k, v, n_tok=None, ld: int = 0, stream: int = 0) -> None:
+    """The rows at positions pos0[s], ... as the values that they stand for, into k, v [nseq, tokens, kv_heads, 128].
+    atlas_cuda_kv8_read."""
+    check(lib().atlas_cuda_kv8_read(cache._ref, tokens, pos0.data_ptr(), _addr(n_tok), k.data_ptr(), v.data_ptr(), ld,
+                                    stream), "kv8_read")
+
+
+def kv8_attn(cache: Kv8Cache, q_heads: int, tokens: int, pos0, q, out, n_tok=None, ldq: int = 0, ldo: int = 0,
+             stream: int = 0) -> None:
+    """Causal attention of q [nseq, tokens, q_heads, 128] over the cache into out. atlas_cuda_kv8_attn."""
+    check(lib().atlas_cuda_kv8_attn(cache._ref, q_heads, tokens, pos0.data_ptr(), _addr(n_tok), q.data_ptr(), ldq,
+                                    out.data_ptr(), ldo, stream), "kv8_attn")
+
+
+def kv8_attn_sparse(cache: Kv8Cache, q_heads: int, tokens: int, n_sel: int, pos0, q, out, sel, n_tok=None, ldq: int = 0,
+                    ldo: int = 0, stream: int = 0) -> None:
+    """Attention over the n_sel blocks that each token and KV head selects; sel [nseq, tokens, kv_heads, n_sel] (int32)
+    receives them. atlas_cuda_kv8_attn_sparse."""
+    check(lib().atlas_cuda_kv8_attn_sparse(cache._ref, q_heads, tokens, n_sel, pos0.data_ptr(), _addr(n_tok),
+                                           q.data_ptr(), ldq, out.data_ptr(), ldo, sel.data_ptr(), stream),
+          "kv8_attn_sparse")

@@ -240,6 +240,71 @@ int atlas_cuda_gemv_noalloc(uint32_t type, const void *d_weights, uint64_t rows,
 int atlas_cuda_gemm(uint32_t type, const void *d_weights, uint64_t rows, uint64_t cols,
                     const float *d_x, uint64_t tokens, float *d_y, void *stream);
 
+/* ---- 8-bit KV cache over caller-owned DEVICE memory ----
+
+   One layer's K and V as int8 codes with one fp32 scale per block of positions
+   and KV head: value = code * scale. A quarter of the bytes of the reference's
+   fp32 cache (src/brain_runtime.c:2019-2020), and read once per step by the
+   attention (gqa_single_token, :1407-1528). Heads have 128 dimensions.
+
+   All calls are asynchronous on `stream` (a cudaStream_t or NULL), allocate
+   nothing, keep nothing between calls and may be captured into a graph: the
+   positions are read on the device. They run on the current device; every
+   pointer must be memory of that device, or the call returns ATLAS_EINVAL.
+   Calls on the same cache, or the same outputs, must be ordered by their
+   streams; others may overlap.
+
+   A call handles all `nseq` sequences of the cache: sequence s has n_tok[s]
+   token rows (d_ntok NULL: all `tokens`; a larger n_tok[s] counts as `tokens`)
+   at positions pos0[s], pos0[s] + 1, ... Rows from n_tok[s] on are left as they
+   were, so 0 leaves a sequence out. Token rows are [seq][tokens][heads][128]
+   floats, `ld` floats from token to token (0: dense; a multiple of 4; the
+   sequence stride is tokens * ld), 16-byte aligned. A position at or past
+   max_context is not stored, and reads and attends as NaN. */
+typedef struct {
+    void *k, *v;                /* int8 [nseq][kv_heads][max_context][128], 16-byte aligned */
+    float *k_scale, *v_scale;   /* [nseq][kv_heads][n_blocks], n_blocks = ceil(max_context / block) */
+    int16_t *k_sum;             /* [nseq][kv_heads][n_blocks][128], or NULL (then no atlas_cuda_kv8_attn_sparse) */
+    uint32_t nseq, kv_heads, max_context;
+    uint32_t block;             /* positions per scale: 16, 32, 64 or 128 */
+} AtlasKv8;
+
+/* Stores new rows. A block's scale is max(its scale so far, max|new| / 127),
+   divided in 64 bits and rounded once; its scale so far counts where the call
+   starts inside the block, and the rows before pos0 are then rounded again if
+   the scale grew: code = rint(code * old / new). New codes are rint(x / scale)
+   of the exact quotient, ties to even, within -127 .. 127. k_sum gets the sums
+   of the block's K codes. Positions are filled in order: before a call starts
+   inside a block, the block's earlier rows have been stored. Starting earlier
+   than a previous call drops what was stored from there on. A NaN or infinity
+   among a block's rows makes the block's scale NaN (its new codes 0): whoever
+   attends to the block gets NaN, until it is stored again from its start. */
+int atlas_cuda_kv8_append(const AtlasKv8 *cache, uint32_t tokens, const uint32_t *d_pos0, const uint32_t *d_ntok,
+                          const float *d_k, const float *d_v, uint64_t ld, void *stream);
+
+/* Rows of the cache as the fp32 values that they stand for. */
+int atlas_cuda_kv8_read(const AtlasKv8 *cache, uint32_t tokens, const uint32_t *d_pos0, const uint32_t *d_ntok,
+                        float *d_k, float *d_v, uint64_t ld, void *stream);
+
+/* Causal grouped-query attention: the query rows of position p attend to the
+   cached positions 0 .. p (the rows of p itself must have been stored), scores
+   q.k / sqrt(128), softmax in fp32, fp32-level accuracy for the values that
+   the codes stand for. q_heads is a multiple of kv_heads. */
+int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
+                        const uint32_t *d_ntok, const float *d_q, uint64_t ldq, float *d_out, uint64_t ldo,
+                        void *stream);
+
+/* The same over n_sel (1 .. 4096) blocks per token and KV head: the block of
+   the token's own position, and the n_sel - 1 blocks before it with the highest
+   scores (all of them where there are no more). Score of a block: (c . k_sum) *
+   k_scale, where c = rint(127 qbar / max|qbar|) and qbar is the sum of the
+   group's query rows; it is compared exactly, and equal scores go to the lower
+   block. sel [seq][tokens][kv_heads][n_sel] receives the blocks, ascending, -1
+   behind the last. */
+int atlas_cuda_kv8_attn_sparse(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, uint32_t n_sel,
+                               const uint32_t *d_pos0, const uint32_t *d_ntok, const float *d_q, uint64_t ldq,
+                               float *d_out, uint64_t ldo, int32_t *d_sel, void *stream);
+
 /* Number of SMs / compute capability of `device`, or a negative code. */
 int atlas_cuda_device_info(int device, int *sm_count, int *cc_major, int *cc_minor);
 

@@ -1,0 +1,550 @@
+"""GPU: the 8-bit KV cache (append, read, attention, attention over chosen blocks) against the definitions in 64 bits.
+
+Codes, scales, sums and chosen blocks are equal; attention is within the bound that kv8_ref.attend derives."""
+import numpy as np
+import pytest
+
+import atlas_cuda
+from kv8_ref import DIM, RefCache, attend, choose
+
+pytestmark = pytest.mark.gpu
+
+
+class DevCache:
+    """A RefCache's buffers on the device."""
+
+    def __init__(self, torch, ref, sums=True):
+        n, h, ctx, b, _ = ref.shape
+        self.t = [torch.from_numpy(x.copy()).cuda() for x in (ref.k, ref.v, ref.ks, ref.vs, ref.ksum)]
+        self.c = atlas_cuda.Kv8Cache(*self.t[:4], self.t[4] if sums else None, nseq=n, kv_heads=h, max_context=ctx,
+                                     block=b)
+
+    def equals(self, ref):
+        for t, x in zip(self.t, (ref.k, ref.v, ref.ks, ref.vs, ref.ksum)):
+            np.testing.assert_array_equal(t.cpu().numpy(), x)
+
+
+def _i32(torch, x):
+    return torch.tensor([int(np.uint32(i).view(np.int32)) for i in x], dtype=torch.int32, device="cuda")
+
+
+def _f32(torch, x):
+    return torch.from_numpy(np.array(x, dtype=np.float32, order="C")).cuda()
+
+
+def filled(rng, nseq, heads, ctx, block, lens, v_spread=0.5, k_size=1.0):
+    """A cache whose first lens[s] positions are stored, in blocks of different scales."""
+    ref = RefCache(nseq, heads, ctx, block, rng)
+    n = max(max(lens), 1)
+    grow = lambda a: np.exp(a * rng.standard_normal((nseq, -(-n // block), heads)))[:, np.arange(n) // block]  # noqa: E731
+    k = (k_size * rng.standard_normal((nseq, n, heads, DIM)) * grow(0.3)[..., None]).astype(np.float32)
+    v = (rng.standard_normal((nseq, n, heads, DIM)) * grow(v_spread)[..., None]).astype(np.float32)
+    ref.append([0] * nseq, lens, k, v)
+    return ref
+
+
+# ------------------------------------------------------------- append, read --
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("nseq,heads,ctx,pieces", [
+    (1, 1, 40, [(0, 1), (1, 1), (2, 14), (16, 1), (17, 23)]),
+    (1, 3, 300, [(0, 299), (299, 1)]),
+    (2, 2, 260, [(0, 130), (130, 1), (131, 129)]),
+    (1, 2, 200, [(0, 150), (37, 3), (40, 100)]),     # starts again earlier
+])
+def test_append_equals_the_definition(torch_cuda, block, nseq, heads, ctx, pieces):
+    torch = torch_cuda
+    rng = np.random.default_rng(block + ctx)
+    ref = RefCache(nseq, heads, ctx, block, rng)
+    dev = DevCache(torch, ref)
+    for p, n in pieces:
+        x, y = ((rng.standard_normal((nseq, n, heads, DIM)) * np.exp(rng.standard_normal((nseq, n, heads, 1)))
+                 ).astype(np.float32) for _ in range(2))
+        ref.append([p] * nseq, [n] * nseq, x, y)
+        atlas_cuda.kv8_append(dev.c, n, _i32(torch, [p] * nseq), _f32(torch, x), _f32(torch, y))
+        dev.equals(ref)
+
+
+@pytest.mark.parametrize("block", [16, 128])
+def test_append_ragged_strided(torch_cuda, block):
+    """Sequences of different lengths (0 and one past the buffer among them), rows inside a wider buffer."""
+    torch = torch_cuda
+    rng = np.random.default_rng(7)
+    nseq, heads, ctx, tokens, ld = 6, 2, 150, 70, 5 * DIM
+    ref = RefCache(nseq, heads, ctx, block, rng)
+    lens = [0, 3, 64, 100, 0, 17]
+    x = rng.standard_normal((nseq, 128, heads, DIM)).astype(np.float32)
+    ref.append([0] * nseq, lens, x, x[::-1])
+    dev = DevCache(torch, ref)
+    ntok = [70, 0, 1, 70, 33, 1000]              # 100 + 70 passes the cache's end, 1000 counts as 70
+    wide = rng.standard_normal((nseq, tokens, 5, DIM)).astype(np.float32)
+    ref.append(lens, ntok, wide[:, :, 1:3], wide[:, :, 3:5])
+    w = _f32(torch, wide)
+    atlas_cuda.kv8_append(dev.c, tokens, _i32(torch, lens), w[:, :, 1:], w[:, :, 3:], n_tok=_i32(torch, ntok), ld=ld)
+    dev.equals(ref)
+    # and back, into a buffer whose other rows stay
+    back = torch.full((nseq, tokens, 5, DIM), 7.0, device="cuda")
+    atlas_cuda.kv8_read(dev.c, tokens, _i32(torch, lens), back[:, :, 1:], back[:, :, 3:], n_tok=_i32(torch, ntok), ld=ld)
+    got = back.cpu().numpy()
+    want = np.full_like(got, 7.0)
+    for s in range(nseq):
+        for i in range(min(ntok[s], tokens)):
+            p = lens[s] + i
+            for j, (codes, scales) in enumerate(((ref.k, ref.ks), (ref.v, ref.vs))):
+                want[s, i, 1 + 2 * j:3 + 2 * j] = (codes[s, :, p].astype(np.float32) * scales[s, :, p // block, None]
+                                                   if p < ctx else np.nan)
+    np.testing.assert_array_equal(got, want)
+
+
+def test_append_rounds_ties_to_even_and_clamps(torch_cuda):
+    torch = torch_cuda
+    x = np.zeros((1, 4, 1, DIM), np.float32)
+    x[0, 0, 0, :4] = [127.0, -127.0, 0.5, 1.5]          # scale 1: ties
+    x[0, 1, 0, :6] = [2.5, -2.5, 126.5, -126.5, 125.5, np.nextafter(np.float32(2.5), np.float32(3))]
+    x[0, 2, 0, :2] = [np.nextafter(np.float32(0.5), np.float32(0)), 1e-38]
+    ref = RefCache(1, 1, 16, 16)
+    dev = DevCache(torch, ref)
+    ref.append([0], [4], x, -x)
+    atlas_cuda.kv8_append(dev.c, 4, _i32(torch, [0]), _f32(torch, x), _f32(torch, -x))
+    dev.equals(ref)
+    assert ref.k[0, 0, 0, 2:4].tolist() == [0, 2] and ref.k[0, 0, 1, :6].tolist() == [2, -2, 126, -126, 126, 3]
+
+
+@pytest.mark.parametrize("size", [0.0, 1e-45, 1.9e-43, 1e-40, 1.2e-36, 1e30, 3.4e38])
+def test_append_extreme_sizes(torch_cuda, size):
+    """All zeros, subnormal scales (rounded coarsely: codes are clamped), the largest values; then a larger row."""
+    torch = torch_cuda
+    rng = np.random.default_rng(5)
+    x = np.clip(rng.uniform(-1, 1, (1, 9, 2, DIM)) * size, -3.4e38, 3.4e38).astype(np.float32)
+    y = np.clip(np.float64(x[:, :1]) * 2.5, -3.4e38, 3.4e38).astype(np.float32)
+    ref = RefCache(1, 2, 16, 16)
+    dev = DevCache(torch, ref)
+    for p, z in ((0, x), (9, y)):
+        ref.append([p], [z.shape[1]], z, z[:, ::-1])
+        atlas_cuda.kv8_append(dev.c, z.shape[1], _i32(torch, [p]), _f32(torch, z), _f32(torch, z[:, ::-1]))
+        dev.equals(ref)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_append_non_finite(torch_cuda, bad):
+    """A poisoned block stays poisoned until it is stored again from its start; the other blocks are untouched."""
+    torch = torch_cuda
+    rng = np.random.default_rng(6)
+    ref = RefCache(1, 1, 64, 16)
+    dev = DevCache(torch, ref)
+    x = rng.standard_normal((1, 40, 1, DIM)).astype(np.float32)
+    x[0, 20, 0, 77] = bad
+    for p, n in ((0, 40), (24, 4), (16, 8)):            # the last call stores the block from its start, without the value
+        z = x[:, :n] if p == 0 else rng.standard_normal((1, n, 1, DIM)).astype(np.float32)
+        ref.append([p], [n], z, z)
+        atlas_cuda.kv8_append(dev.c, n, _i32(torch, [p]), _f32(torch, z), _f32(torch, z))
+        dev.equals(ref)
+        assert np.isnan(ref.ks[0, 0, 1]) == (p != 16) and np.isfinite(ref.ks[0, 0, [0, 2]]).all()
+
+
+def test_append_past_the_cache(torch_cuda):
+    torch = torch_cuda
+    ref = RefCache(2, 1, 30, 16)
+    dev = DevCache(torch, ref)
+    x = np.ones((2, 3, 1, DIM), np.float32)
+    for pos in ([30, 31], [0xffffffff, 0x80000000]):    # nothing is stored
+        atlas_cuda.kv8_append(dev.c, 3, _i32(torch, pos), _f32(torch, x), _f32(torch, x))
+        dev.equals(ref)
+    ref.append([29, 0], [3, 3], x, x)
+    atlas_cuda.kv8_append(dev.c, 3, _i32(torch, [29, 0]), _f32(torch, x), _f32(torch, x))
+    dev.equals(ref)
+
+
+# ---------------------------------------------------------------- attention --
+
+
+def check_attn(torch, rng, ref, q_heads, tokens, pos, ntok=None, n_sel=0, q=None, ldq=0, dev=None):
+    """One call against the definition; rows that do not exist stay, positions past the cache give NaN."""
+    nseq, heads, ctx, b, _ = ref.shape
+    group = q_heads // heads
+    dev = dev or DevCache(torch, ref)
+    if q is None:
+        q = rng.standard_normal((nseq, tokens, q_heads, DIM)).astype(np.float32)
+    wide = max(ldq // DIM, q_heads)
+    qw = np.full((nseq, tokens, wide, DIM), np.nan, np.float32)
+    qw[:, :, :q_heads] = q
+    out = torch.full((nseq, tokens, wide, DIM), 7.0, device="cuda")
+    sel = torch.full((nseq, tokens, heads, max(n_sel, 1)), -5, dtype=torch.int32, device="cuda")
+    n = None if ntok is None else _i32(torch, ntok)
+    if n_sel:
+        atlas_cuda.kv8_attn_sparse(dev.c, q_heads, tokens, n_sel, _i32(torch, pos), _f32(torch, qw), out, sel, n_tok=n,
+                                   ldq=ldq, ldo=ldq)
+    else:
+        atlas_cuda.kv8_attn(dev.c, q_heads, tokens, _i32(torch, pos), _f32(torch, qw), out, n_tok=n, ldq=ldq, ldo=ldq)
+    torch.cuda.synchronize()
+    got, sel = out.cpu().numpy(), sel.cpu().numpy()
+    assert (got[:, :, q_heads:] == 7.0).all()
+    got = got[:, :, :q_heads]
+    for s in range(nseq):
+        m = tokens if ntok is None else min(ntok[s], tokens)
+        assert (got[s, m:] == 7.0).all() and (sel[s, m:] == -5).all()
+        for h in range(heads):
+            at = pos[s] + np.arange(m)
+            past = at >= ctx
+            assert np.isnan(got[s, :m][past]).all()
+            live = np.flatnonzero(~past)
+            if not live.size:
+                continue
+            end = int(at[live].max()) + 1
+            k, v = ref.values(s, h, end)
+            seen = np.arange(end)[None] <= at[live, None]
+            if n_sel:
+                for j, i in enumerate(live):
+                    blocks = choose(q[s, i, h * group:(h + 1) * group], ref, s, h, int(at[i]), n_sel)
+                    want = np.full(n_sel, -1)
+                    want[:len(blocks)] = blocks
+                    np.testing.assert_array_equal(sel[s, i, h], want)
+                    seen[j] &= np.isin(np.arange(end) // b, blocks)
+            rows = q[s, live, h * group:(h + 1) * group].astype(np.float64).reshape(-1, DIM)
+            want, bound = attend(rows, k, v, np.repeat(seen, group, 0))
+            err = np.abs(got[s, live, h * group:(h + 1) * group].reshape(-1, DIM) - want)
+            assert (err <= bound).all(), float((err / bound).max())
+            if n_sel:
+                assert (sel[s, :m, h][past] == -1).all()
+    return got, sel
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("pos", [0, 1, 15, 16, 17, 63, 64, 127, 255, 1000])
+def test_decode_lengths(torch_cuda, block, pos):
+    rng = np.random.default_rng(pos * 7 + block)
+    ref = filled(rng, 1, 2, pos + 1 + pos % 3, block, [pos + 1])
+    check_attn(torch_cuda, rng, ref, 14, 1, [pos])
+
+
+@pytest.mark.parametrize("q_heads,heads", [(1, 1), (2, 2), (6, 2), (5, 1), (7, 1), (8, 1), (9, 1), (24, 2), (16, 1), (33, 1)])
+def test_decode_groups(torch_cuda, q_heads, heads):
+    rng = np.random.default_rng(q_heads)
+    ref = filled(rng, 2, heads, 401, 32, [401, 130])
+    check_attn(torch_cuda, rng, ref, q_heads, 1, [400, 129])
+
+
+@pytest.mark.parametrize("q_heads,heads", [(2, 2), (12, 2), (7, 1)])
+@pytest.mark.parametrize("tokens,pos", [(2, 0), (3, 61), (5, 100), (16, 0), (17, 300), (33, 15), (64, 64), (129, 0),
+                                        (130, 77), (300, 211)])
+def test_prompt_pieces(torch_cuda, q_heads, heads, tokens, pos):
+    rng = np.random.default_rng(tokens + pos)
+    ref = filled(rng, 1, heads, pos + tokens, 64, [pos + tokens])
+    check_attn(torch_cuda, rng, ref, q_heads, tokens, [pos])
+
+
+@pytest.mark.parametrize("block", [16, 32, 128])
+def test_prompt_blocks(torch_cuda, block):
+    rng = np.random.default_rng(block)
+    ref = filled(rng, 1, 1, 400, block, [390])
+    check_attn(torch_cuda, rng, ref, 5, 190, [200])
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 70, 150])
+def test_attn_ragged_strided(torch_cuda, tokens):
+    """Pieces of different lengths, an idle sequence, rows past the cache's end, rows inside wider buffers."""
+    rng = np.random.default_rng(tokens)
+    ctx, pos = 500, [0, 310, 499, 33, 128, 500 - tokens // 2]
+    ntok = [tokens, max(1, tokens // 2), tokens, 0, tokens + 9, tokens]
+    lens = [min(ctx, p + n) for p, n in zip(pos, ntok)]
+    ref = filled(rng, 6, 2, ctx, 32, lens)
+    check_attn(torch_cuda, rng, ref, 10, tokens, pos, ntok, ldq=13 * DIM)
+
+
+@pytest.mark.parametrize("tokens", [1, 80])
+def test_attn_positions_past_the_cache(torch_cuda, tokens):
+    rng = np.random.default_rng(9)
+    ref = filled(rng, 3, 1, 70, 16, [70, 70, 70])
+    check_attn(torch_cuda, rng, ref, 3, tokens, [70, 0xffffffff, 0x7fffffff])
+
+
+@pytest.mark.parametrize("tokens", [1, 90])
+@pytest.mark.parametrize("q_size,k_size,v_spread", [(30.0, 3.0, 0.5), (1e-3, 1.0, 0.5), (1.0, 1.0, 4.0), (1e-30, 1e10, 0.1),
+                                                    (1e8, 1e-8, 0.1)])
+def test_attn_sizes(torch_cuda, tokens, q_size, k_size, v_spread):
+    """Scores in the hundreds, flat ones, V blocks of very different scales, large and tiny queries."""
+    rng = np.random.default_rng(11)
+    ref = filled(rng, 1, 2, 300, 16, [300], v_spread=v_spread, k_size=k_size)
+    q = (q_size * rng.standard_normal((1, tokens, 6, DIM))).astype(np.float32)
+    check_attn(torch_cuda, rng, ref, 6, tokens, [300 - tokens], q=q)
+
+
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_attn_zero_blocks_and_queries(torch_cuda, tokens):
+    """Blocks of zeros (scale 0) at the start, in the middle and alone; a query of zeros weighs all positions alike."""
+    rng = np.random.default_rng(12)
+    ref = RefCache(1, 1, 160, 16, rng)
+    x = rng.standard_normal((1, 160, 1, DIM)).astype(np.float32)
+    x[:, :32] = 0
+    x[:, 64:80] = 0
+    ref.append([0], [160], x, x)
+    q = rng.standard_normal((1, tokens, 4, DIM)).astype(np.float32)
+    q[:, :, 1] = 0
+    check_attn(torch_cuda, rng, ref, 4, tokens, [160 - tokens], q=q)
+    z = RefCache(1, 1, 160, 16, rng)
+    z.append([0], [160], 0 * x, 0 * x)
+    got, _ = check_attn(torch_cuda, rng, z, 4, tokens, [160 - tokens], q=q)
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_attn_non_finite(torch_cuda, where, tokens):
+    """A poisoned block shows in the rows that attend to it, and in no other; neither does what lies behind the end."""
+    torch = torch_cuda
+    rng = np.random.default_rng(13)
+    ref = filled(rng, 1, 1, 256, 16, [256])
+    (ref.ks if where == "k" else ref.vs)[0, 0, 12] = np.nan          # positions 192 .. 207
+    for pos, hit in ((192 - tokens, False), (208, True), (150, tokens > 42)):
+        q = rng.standard_normal((1, tokens, 2, DIM)).astype(np.float32)
+        out = torch.zeros(1, tokens, 2, DIM, device="cuda")
+        atlas_cuda.kv8_attn(DevCache(torch, ref).c, 2, tokens, _i32(torch, [pos]), _f32(torch, q), out)
+        got = out.cpu().numpy()[0]
+        at = pos + np.arange(tokens)
+        inside = at < 256
+        assert np.isnan(got[(at >= 192)]).all()
+        assert np.isfinite(got[(at < 192) & inside]).all()
+        if not hit:
+            check_attn(torch, rng, ref, 2, tokens, [pos], q=q)
+
+
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_attn_non_finite_query(torch_cuda, tokens):
+    """A query row with a NaN or an infinity gives NaN, the others are as without it."""
+    torch = torch_cuda
+    rng = np.random.default_rng(14)
+    ref = filled(rng, 1, 1, 256, 64, [256])
+    q = rng.standard_normal((1, tokens, 4, DIM)).astype(np.float32)
+    want, _ = check_attn(torch, rng, ref, 4, tokens, [256 - tokens], q=q)
+    q[0, 0, 1, 5], q[0, -1, 2, 100] = np.nan, np.inf
+    out = torch.zeros(1, tokens, 4, DIM, device="cuda")
+    atlas_cuda.kv8_attn(DevCache(torch, ref).c, 4, tokens, _i32(torch, [256 - tokens]), _f32(torch, q), out)
+    got = out.cpu().numpy()
+    assert np.isnan(got[0, 0, 1]).all() and np.isnan(got[0, -1, 2]).all()
+    ok = np.ones(got.shape[:3], bool)
+    ok[0, 0, 1] = ok[0, -1, 2] = False
+    np.testing.assert_array_equal(got[ok], want[ok])
+
+
+def test_attn_many_positions(torch_cuda):
+    """More positions than one round of the 32 scales that a warp holds, over all CTAs of a cluster."""
+    rng = np.random.default_rng(15)
+    ref = filled(rng, 1, 1, 40000, 16, [40000])
+    check_attn(torch_cuda, rng, ref, 8, 1, [39999])
+
+
+def test_attn_large_batch(torch_cuda):
+    """More units of work than CTAs fit on the device (clusters of one)."""
+    rng = np.random.default_rng(16)
+    ref = filled(rng, 40, 16, 70, 32, list(range(30, 70)))
+    check_attn(torch_cuda, rng, ref, 32, 1, list(range(29, 69)))
+
+
+# ------------------------------------------------------------ chosen blocks --
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("n_sel", [1, 2, 5, 16, 100])
+def test_sparse_decode(torch_cuda, block, n_sel):
+    rng = np.random.default_rng(n_sel + block)
+    ref = filled(rng, 2, 2, 1500, block, [1500, 700])
+    check_attn(torch_cuda, rng, ref, 10, 1, [1499, 699], n_sel=n_sel)
+
+
+@pytest.mark.parametrize("q_heads,heads", [(1, 1), (16, 2), (28, 4), (24, 2), (40, 1)])
+@pytest.mark.parametrize("tokens,pos", [(1, 0), (5, 14), (37, 500)])
+def test_sparse_tokens_and_groups(torch_cuda, q_heads, heads, tokens, pos):
+    rng = np.random.default_rng(q_heads + tokens)
+    ref = filled(rng, 1, heads, pos + tokens + 1, 16, [pos + tokens])
+    check_attn(torch_cuda, rng, ref, q_heads, tokens, [pos], n_sel=7)
+
+
+def test_sparse_many_tokens(torch_cuda):
+    """Enough tokens that no clusters are formed."""
+    rng = np.random.default_rng(21)
+    ref = filled(rng, 2, 2, 900, 32, [900, 400])
+    check_attn(torch_cuda, rng, ref, 4, 300, [600, 100], [300, 300], n_sel=4)
+
+
+def test_sparse_ragged_strided(torch_cuda):
+    rng = np.random.default_rng(22)
+    pos, ntok = [0, 310, 499, 33], [6, 2, 3, 0]
+    ref = filled(rng, 4, 2, 500, 16, [6, 312, 500, 33])
+    check_attn(torch_cuda, rng, ref, 10, 6, pos, ntok, n_sel=3, ldq=11 * DIM)
+
+
+def test_sparse_ties_go_to_the_lower_block(torch_cuda):
+    """A query of zeros (all scores equal), and blocks that repeat."""
+    torch = torch_cuda
+    rng = np.random.default_rng(23)
+    x = np.tile(rng.standard_normal((1, 48, 1, DIM)).astype(np.float32), (1, 20, 1, 1))   # 20 times the same 3 blocks
+    ref = RefCache(1, 1, 960, 16, rng)
+    ref.append([0], [960], x, x)
+    check_attn(torch, rng, ref, 4, 1, [959], n_sel=30)
+    _, sel = check_attn(torch, rng, ref, 4, 1, [959], n_sel=9, q=np.zeros((1, 1, 4, DIM), np.float32))
+    assert sel[0, 0, 0].tolist() == list(range(8)) + [59]
+
+
+def test_sparse_scores_of_both_signs_and_zero(torch_cuda):
+    """Scores below, at and above zero, and -0 beside 0: a block of zeros has scale 0."""
+    rng = np.random.default_rng(24)
+    x = rng.standard_normal((1, 640, 1, DIM)).astype(np.float32)
+    for b in range(0, 40, 3):
+        x[:, 16 * b:16 * b + 16] = 0
+    ref = RefCache(1, 1, 640, 16, rng)
+    ref.append([0], [640], x, x)
+    ref.ksum[0, 0, [6, 12]] = [[-5], [5]]          # a scale of 0 with sums of either sign: equal scores
+    for n in range(2, 41, 5):
+        check_attn(torch_cuda, rng, ref, 3, 1, [639], n_sel=n)
+
+
+def test_sparse_poisoned_block_is_chosen(torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(25)
+    ref = filled(rng, 1, 1, 640, 16, [640])
+    ref.ks[0, 0, 17] = np.nan
+    out = torch.zeros(1, 1, 2, DIM, device="cuda")
+    sel = torch.zeros(1, 1, 1, 4, dtype=torch.int32, device="cuda")
+    q = rng.standard_normal((1, 1, 2, DIM)).astype(np.float32)
+    atlas_cuda.kv8_attn_sparse(DevCache(torch, ref).c, 2, 1, 4, _i32(torch, [639]), _f32(torch, q), out, sel)
+    assert 17 in sel.cpu().tolist()[0][0][0] and torch.isnan(out).all()
+    assert sel.cpu().numpy()[0, 0, 0].tolist() == choose(q[0, 0], ref, 0, 0, 639, 4).tolist()
+
+
+def test_sparse_past_the_cache(torch_cuda):
+    rng = np.random.default_rng(26)
+    ref = filled(rng, 2, 1, 100, 16, [100, 100])
+    check_attn(torch_cuda, rng, ref, 2, 3, [98, 0xfffffff0], n_sel=3)
+
+
+def test_sparse_of_all_blocks_is_dense(torch_cuda):
+    """Choosing at least as many blocks as there are is the dense attention, to the bit where the split is the same."""
+    rng = np.random.default_rng(27)
+    ref = filled(rng, 1, 2, 777, 64, [777])
+    q = rng.standard_normal((1, 1, 8, DIM)).astype(np.float32)
+    a, _ = check_attn(torch_cuda, rng, ref, 8, 1, [776], q=q)
+    b, sel = check_attn(torch_cuda, rng, ref, 8, 1, [776], q=q, n_sel=64)
+    assert np.abs(a - b).max() <= 2e-6 and sel[0, 0, 0, :13].tolist() == list(range(13))
+
+
+# ------------------------------------------------------ refusals, together --
+
+
+def test_refusals_leave_outputs_alone(torch_cuda):
+    torch = torch_cuda
+    ref = RefCache(1, 2, 64, 16)
+    dev = DevCache(torch, ref)
+    pos, q = _i32(torch, [3]), torch.zeros(1, 1, 4, DIM, device="cuda")
+    host, out = torch.zeros(1, 1, 4, DIM), torch.full((1, 1, 4, DIM), 7.0, device="cuda")
+    sel = torch.full((1, 1, 2, 2), -5, dtype=torch.int32, device="cuda")
+    C = dev.c
+    bad = [lambda: atlas_cuda.kv8_attn(C, 3, 1, pos, q, out), lambda: atlas_cuda.kv8_attn(C, 0, 1, pos, q, out),
+           lambda: atlas_cuda.kv8_attn(C, 4, 1, pos, q.view(-1)[1:], out), lambda: atlas_cuda.kv8_attn(C, 4, 1, pos, host, out),
+           lambda: atlas_cuda.kv8_attn(C, 4, 1, pos.cpu(), q, out), lambda: atlas_cuda.kv8_attn(C, 4, 1, pos, q, host),
+           lambda: atlas_cuda.kv8_attn(C, 4, 1, pos, q, out, ldq=508), lambda: atlas_cuda.kv8_attn(C, 4, 1, pos, q, out, ldo=514),
+           lambda: atlas_cuda.kv8_attn(C, 4, 1 << 24, pos, q, out), lambda: atlas_cuda.kv8_attn(C, 4, 1, pos, q, out, n_tok=pos.cpu()),
+           lambda: atlas_cuda.kv8_attn_sparse(C, 4, 1, 0, pos, q, out, sel),
+           lambda: atlas_cuda.kv8_attn_sparse(C, 4, 1, 5000, pos, q, out, sel),
+           lambda: atlas_cuda.kv8_attn_sparse(C, 4, 1, 2, pos, q, out, sel.cpu()),
+           lambda: atlas_cuda.kv8_attn_sparse(DevCache(torch, ref, sums=False).c, 4, 1, 2, pos, q, out, sel),
+           lambda: atlas_cuda.kv8_append(C, 1, pos, q, host), lambda: atlas_cuda.kv8_append(C, 1, pos, q, q, ld=128),
+           lambda: atlas_cuda.kv8_read(C, 1, pos, out, host), lambda: atlas_cuda.kv8_read(C, 1, pos, out, out.view(-1)[2:])]
+    for f in bad:
+        with pytest.raises(atlas_cuda.AtlasError) as e:
+            f()
+        assert e.value.code == -1
+    torch.cuda.synchronize()
+    assert (out == 7.0).all() and (sel == -5).all()
+    dev.equals(ref)
+    # more blocks than fit beside the attention's buffers
+    big = atlas_cuda.Kv8Desc(*(t.data_ptr() for t in dev.t), 1, 1, 1 << 20, 16)
+    import ctypes
+    assert atlas_cuda.lib().atlas_cuda_kv8_attn_sparse(ctypes.byref(big), 4, 1, 2, pos.data_ptr(), None, q.data_ptr(), 0,
+                                                       out.data_ptr(), 0, sel.data_ptr(), None) == -1
+    # no tokens: nothing to do
+    atlas_cuda.kv8_attn(C, 4, 0, pos, q, out)
+    atlas_cuda.kv8_append(C, 0, pos, q, q)
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+
+
+def test_a_prompt_and_steps_together_in_a_graph(torch_cuda):
+    """As a decode loop uses them: a prompt is stored and attended, then one captured graph (append, attention, attention
+    over chosen blocks, the positions advancing on the device) is replayed on a stream of its own, and every step is
+    compared; at the end the cache is."""
+    torch = torch_cuda
+    rng = np.random.default_rng(31)
+    nseq, heads, q_heads, ctx, block, steps = 2, 2, 10, 200, 16, 40
+    lens = [70, 33]
+    ref = RefCache(nseq, heads, ctx, block, rng)
+    dev = DevCache(torch, ref)
+    x, y = (rng.standard_normal((nseq, 70, heads, DIM)).astype(np.float32) for _ in range(2))
+    ref.append([0, 0], lens, x, y)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        raw = stream.cuda_stream
+        zero, n = _i32(torch, [0, 0]), _i32(torch, lens)
+        q = rng.standard_normal((nseq, 70, q_heads, DIM)).astype(np.float32)
+        dq, dk, dv, out = _f32(torch, q), _f32(torch, x), _f32(torch, y), torch.zeros(nseq, 70, q_heads, DIM, device="cuda")
+        atlas_cuda.kv8_append(dev.c, 70, zero, dk, dv, n_tok=n, stream=raw)
+        atlas_cuda.kv8_attn(dev.c, q_heads, 70, zero, dq, out, n_tok=n, stream=raw)
+        stream.synchronize()
+        dev.equals(ref)
+        k_all, v_all = ((rng.standard_normal((steps, nseq, 1, heads, DIM)) * np.linspace(0.5, 2, steps)[:, None, None, None, None]
+                         ).astype(np.float32) for _ in range(2))
+        q_all = rng.standard_normal((steps, nseq, 1, q_heads, DIM)).astype(np.float32)
+        dk, dv, dq = _f32(torch, k_all[0]), _f32(torch, v_all[0]), _f32(torch, q_all[0])
+        pos = _i32(torch, lens)
+        dense, sparse = torch.zeros(nseq, 1, q_heads, DIM, device="cuda"), torch.zeros(nseq, 1, q_heads, DIM, device="cuda")
+        sel = torch.zeros(nseq, 1, heads, 3, dtype=torch.int32, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            raw = torch.cuda.current_stream().cuda_stream
+            atlas_cuda.kv8_append(dev.c, 1, pos, dk, dv, stream=raw)
+            atlas_cuda.kv8_attn(dev.c, q_heads, 1, pos, dq, dense, stream=raw)
+            atlas_cuda.kv8_attn_sparse(dev.c, q_heads, 1, 3, pos, dq, sparse, sel, stream=raw)
+            pos += 1
+        for i in range(steps):
+            dk.copy_(_f32(torch, k_all[i]))
+            dv.copy_(_f32(torch, v_all[i]))
+            dq.copy_(_f32(torch, q_all[i]))
+            graph.replay()
+            stream.synchronize()
+            at = [p + i for p in lens]
+            ref.append(at, [1] * nseq, k_all[i], v_all[i])
+            for s in range(nseq):
+                for h in range(heads):
+                    rows = slice(5 * h, 5 * h + 5)
+                    k, v = ref.values(s, h, at[s] + 1)
+                    qq = q_all[i, s, 0, rows].astype(np.float64)
+                    blocks = choose(q_all[i, s, 0, rows], ref, s, h, at[s], 3)
+                    assert sel[s, 0, h].tolist()[:len(blocks)] == blocks.tolist()
+                    every = np.ones((5, at[s] + 1), bool)
+                    some = every & np.isin(np.arange(at[s] + 1) // block, blocks)
+                    for got, seen in ((dense, every), (sparse, some)):
+                        want, bound = attend(qq, k, v, seen)
+                        assert (np.abs(got[s, 0, rows].cpu().numpy() - want) <= bound).all()
+    dev.equals(ref)
+    assert pos.tolist() == [p + steps for p in lens]
+
+
+def test_two_streams_at_once(torch_cuda):
+    """Calls on different caches overlap freely: nothing is shared between them."""
+    torch = torch_cuda
+    rng = np.random.default_rng(32)
+    work = []
+    for i in range(4):
+        ref = filled(rng, 1, 2, 3000, 64, [3000])
+        q = rng.standard_normal((1, 1, 10, DIM)).astype(np.float32)
+        want, _ = check_attn(torch, rng, ref, 10, 1, [2999], q=q)
+        work.append((DevCache(torch, ref), _f32(torch, q), torch.zeros(1, 1, 10, DIM, device="cuda"), want, torch.cuda.Stream()))
+    pos = _i32(torch, [2999])
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for dev, q, out, _, stream in work:
+            atlas_cuda.kv8_attn(dev.c, 10, 1, pos, q, out, stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    for _, _, out, want, _ in work:
+        np.testing.assert_array_equal(out.cpu().numpy(), want)
