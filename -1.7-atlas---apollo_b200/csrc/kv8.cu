@@ -12,7 +12,7 @@
 #include <atomic>
 #include "../../include/atlas_cuda.h"
 #include "common.cuh"
-#include "kv8.h"
+#include "kv8.cuh"
 
 namespace atlas {
 
@@ -20,20 +20,10 @@ int api_fail(int code, const char *fmt, ...);
 int api_device(int device, int *sms);
 
 namespace k8 {
-namespace {
 
-// Every kernel here is launched with programmatic stream serialization: it
-// may start while its predecessor drains, so it first waits for it. Inputs are
-// then read through L2 (__ldcg, cp.async.cg): this SM's L1 may hold lines from
-// before the predecessor wrote them.
-// `early`: let the successor start at once (it waits in turn). Only where all
-// of this grid fits on the device with room to spare: CTAs of a successor that
-// take the first slots to fall free would crowd on a few SMs.
-__device__ __forceinline__ void wait_predecessor(uint32_t early)
-{
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
+cudaError_t launch_prompt(AttnArgs a, int dev, int sms, cudaStream_t stream);   // kv8_prompt.cu
+
+namespace {
 
 // --------------------------------------------------------------- append ----
 
@@ -229,23 +219,14 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
 // Bound by HBM for long caches (256 bytes per position and KV head, read once),
 // by launch and first-byte latency for short ones.
 
+constexpr uint32_t kFewRows = 48;   // query rows of a KV head up to which this form is taken
 constexpr uint32_t kStages = 3;
 constexpr uint32_t kWarps = 8, kWarpsLog2 = 3, kThreads = kWarps * 32;
 constexpr uint32_t kSlot = 8 * 32 * 16;                     // bytes of a chunk: 16 rows of K and V
 
 constexpr uint32_t kMaxCluster = 16;                        // >= 8 NT: the rows of a tile, or their states
 constexpr uint32_t kRecStride = kDim + 4;                   // output, maximum, sum
-constexpr float kLazy = 8.0f;
-constexpr float kScoreScale = (float)(1.4426950408889634 / 11.313708498984761);   // log2(e) / sqrt(128)
-constexpr uint32_t kTinyScale = 7u << 23;                   // bits of 2^-120: where vref starts
 constexpr int kSumBits = 0x4B400000;                  // 2^23 + 2^22: integer sums below 2^22 read as floats
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const int (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -277,22 +258,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x)
     return y;
 }
 
-__device__ __forceinline__ uint32_t h2_bits(float lo, float hi)
-{
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// Signed bytes 0 and 2 (odd: 1 and 3) of y as two binary16 numbers: 0x6400 | u
-// is 1024 + u, and u = code + 128 with the sign bit flipped.
-template <bool ODD>
-__device__ __forceinline__ uint32_t codes_h2(uint32_t y)
-{
-    const uint32_t u = ((ODD ? y >> 8 : y) & 0x00ff00ffu) ^ 0x64806480u;
-    const __half2 c = __hsub2(*reinterpret_cast<const __half2 *>(&u), __float2half2_rn(1152.0f));
-    return *reinterpret_cast<const uint32_t *>(&c);
-}
-
 // 16 bytes global -> shared; in the second form nothing is read and zeros are stored where !there
 template <int DST, int SRC>
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src)
@@ -310,22 +275,6 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ uint32_t cluster_size()
-{
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_rank()
-{
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // Split: arrive once the CTA runs, wait before the first access to another CTA's shared memory
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
@@ -360,18 +309,6 @@ struct Dense {
     __device__ __forceinline__ uint32_t key0(uint32_t c) const { return c * kChunk; }
 };
 
-// Query rows of a tile: row i is head `rem + i` of token `tok`, counted on through the group (no division: the
-// factor is 1 / group, a little high, and exact for rem + i < group + 16).
-struct TileRows {
-    uint32_t tok, rem, group;
-    float inv;
-    __device__ __forceinline__ uint2 at(uint32_t i) const   // (token, head of the group)
-    {
-        const uint32_t t = rem + i, q = (uint32_t)((float)t * inv);
-        return make_uint2(tok + q, t - q * group);
-    }
-};
-
 // Four dimensions of the output of the tile's row i; NaN where its position lies past the cache
 __device__ __forceinline__ void store_row(const AttnArgs &a, const TileRows &tr, uint32_t s, uint32_t h, uint32_t i,
                                           uint64_t p0, uint32_t d4, float4 x)
@@ -380,13 +317,6 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, const TileRows &tr,
     const float nan = __int_as_float(0x7fffffff);
     if (p0 + r.x >= a.c.max_context) x = make_float4(nan, nan, nan, nan);
     reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo + (size_t)(h * a.group + r.y) * kDim)[d4] = x;
-}
-
-__device__ __forceinline__ float rcp(float x)
-{
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 // This warp's query rows warp, warp + 8, ... of the tile (lane = 4 dimensions). Rows of tokens that the call does
@@ -1003,42 +933,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const
 
 // ------------------------------------------------------------- host side ----
 
-// A launch that may overlap its predecessor's end (the kernels wait for it), in clusters of `cluster` CTAs along x.
-template <class ARGS>
-cudaError_t launch(void (*kernel)(ARGS), dim3 grid, uint32_t threads, size_t smem, uint32_t cluster, ARGS a, int sms,
-                   cudaStream_t stream)
-{
-    a.early = (uint64_t)grid.x * grid.y * grid.z <= (uint64_t)sms;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = cluster;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = at;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a);
-}
-
-// Lets a kernel take up to the device's shared memory and clusters of 16, once per device.
-template <auto KERNEL>
-cudaError_t allow(int dev, int bytes)
-{
-    static std::atomic<bool> done[64];
-    if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
-    return e;
-}
-
-constexpr size_t kMaxSmem = 232448;   // shared memory a CTA may have
-
 // CTAs per unit of work: as many as fill the device, at most 16 (the largest
 // cluster) and one per 64 positions (a chunk for each warp).
 uint32_t cluster_of(uint64_t units, uint64_t slots, uint64_t positions)
@@ -1217,6 +1111,7 @@ extern "C" int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint
     const int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
     if (rc != ATLAS_OK || !tokens) return rc;
     const uint32_t rows = tokens * a.group;
+    if (rows > kFewRows) return done(who, launch_prompt(a, dev, sms, (cudaStream_t)stream));
     const bool one = rows <= 8;
     a.tiles = one ? 1 : (rows + 15) / 16;
     return done(who, one ? launch_attn<1>(a, dev, sms, (cudaStream_t)stream) : launch_attn<2>(a, dev, sms, (cudaStream_t)stream));
