@@ -14,18 +14,20 @@
 // (over a running power of two vref, so that one accumulator serves blocks of
 // different scales; p <= 2^8 and v_scale < 2 vref keep P below 2^15).
 //
-// Warps of a CTA (13, so that a thread may have 128 registers):
-//   0-7    softmax, one warpgroup per tile, one thread per row: maximum and
-//          exponentials of the scores straight from tensor memory, P back into
-//          the columns that the scores leave; the maximum is lazy (raised only
-//          when a score passes it by 2^8), so the output is rescaled rarely;
-//   8-11   codes -> binary16 in 128-byte swizzled K-major tiles: K [key][dimension],
-//          V transposed on the way, [dimension][key]; the next tiles' codes are in
-//          registers while the MMAs still read the current ones;
-//   12     issues the MMAs: P V of a tile, then the next keys' scores of the
+// Warps of a CTA (21):
+//   0-15   softmax, 8 per tile, two threads per row (half of the keys each):
+//          maximum and exponentials of the scores straight from tensor memory, P
+//          back into the columns that the scores leave; the maximum is lazy
+//          (raised only when a score passes it by 2^8), so the output is
+//          rescaled and the halves exchange maxima rarely;
+//   16-19  codes -> binary16 in 128-byte swizzled K-major tiles: K [key][dimension],
+//          V transposed on the way, [dimension][key]; the next codes are on their
+//          way by cp.async while the MMAs still read the current ones;
+//   20     issues the MMAs: P V of a tile, then the next keys' scores of the
 //          same tile, so that one tile's softmax runs under the other's MMAs.
 // Tensor memory: 2 x 128 columns of scores / weights, 2 x 128 of output.
-// Shared memory: Q hi / lo 128 KB, K 32 KB, V 32 KB; Q's place stages the output.
+// Shared memory: Q hi / lo 128 KB, K 32 KB, V 32 KB, their next codes 32 KB; Q's
+// place stages the output.
 //
 // Few rows over many positions: the positions are split over a cluster of CTAs,
 // and each merges a share of the rows through distributed shared memory.
@@ -33,6 +35,7 @@
 // Bound by the tensor pipe (4096 cycles per 256 rows x 128 keys) next to the
 // softmax's issue slots. Every wait is bounded; after a timeout the CTA's rows
 // are NaN.
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include "../../include/atlas_cuda.h"
@@ -43,18 +46,25 @@ namespace k8 {
 namespace {
 
 constexpr uint32_t kTileRows = 128, kTileKeys = 128;
-constexpr uint32_t kPromptThreads = 13 * 32, kMmaWarp = 12;
+constexpr uint32_t kConvWarp = 16, kMmaWarp = 20, kPromptThreads = 21 * 32;   // first converter, the MMA warp
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 binary16, swizzled
 constexpr uint32_t kQTile = 4 * kHalf;             // one tile's Q: [hi, lo][2 x 64 dimensions]
 
 struct PromptBars {
-    uint64_t s_full[2], p_full[2], o_full[2], k_full, k_empty, v_full, v_empty, fin;
+    uint64_t s_full[2], p_full[2], o_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], fin;   // [tile], [half]
     uint32_t tmem, status;
-    float row_factor[2][kTileRows];                // what a score of the row is worth, in the exponent's base 2
-    float row_max[2][kTileRows], row_sum[2][kTileRows];
+    // what a score of the row is worth, in the exponent's base 2 (in [tile][0], until the first exchange);
+    // then the two threads of a row exchange their maxima and sums here
+    float half[2][2][kTileRows];
 };
 
-constexpr size_t kPromptSmem = 2 * kQTile + 4 * kHalf + sizeof(PromptBars) + 1024;
+// In the place of the next codes once they are used up
+struct RowStates {
+    float max[2][kTileRows], sum[2][kTileRows];
+};
+
+constexpr size_t kRawTile = 128 * 128;             // bytes of 128 rows of codes
+constexpr size_t kPromptSmem = 2 * kQTile + 4 * kHalf + 2 * kRawTile + sizeof(PromptBars);
 static_assert(kPromptSmem <= kMaxSmem, "the tiles exceed a CTA's shared memory");
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -91,35 +101,47 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
                  : "memory");
 }
 
-// Arrives on `bar` once every MMA that this thread issued is done
+// Arrives on `bar` once every MMA that this lane issued is done
 __device__ __forceinline__ void commit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&r)[32])
+// One lane of the (converged) warp
+__device__ __forceinline__ bool elected()
+{
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+    return e != 0u;
+}
+
+// 16 columns of this warp's lanes; the values are there after tmem_wait_ld
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&r)[16])
 {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-        "tcgen05.wait::ld.sync.aligned;"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
-          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
-          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
         : "r"(addr)
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[32])
+// Names the registers, so that no use of them moves before the wait
+__device__ __forceinline__ void tmem_wait_ld(float (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
+                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[16])
 {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
@@ -148,75 +170,131 @@ __device__ __forceinline__ float ld_cluster1(const void *p, uint32_t cta)
     return v;
 }
 
-// A row's softmax over one tile of keys: scores at tensor memory `at` (this
-// warp's lanes), scale of 16-key group i in lane i (K) and 8 + i (V) of `sc`,
-// of which the row sees the first `nvis` keys (MASK; else all).
-template <bool MASK>
-__device__ __forceinline__ float tile_max(uint32_t at, float sc, float factor, int nvis)
+__device__ __forceinline__ float max3(float a, float b, float c)
 {
-    float m = -INFINITY;
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// A thread's half of a row's softmax over one tile of keys: 64 scores at tensor
+// memory `at` (this warp's lanes), what a score of their 16-key group i is
+// worth in f[i], of which the row sees the first `nvis` keys (MASK; else all).
+// The next 16 columns are on their way while 16 are worked on.
+template <bool MASK>
+__device__ __forceinline__ float tile_max(uint32_t at, const float (&f)[4], int nvis)
+{
+    float m = -INFINITY, s[2][16];
+    tmem_ld(at, s[0]);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-        float s[32];
-        tmem_ld(at + 32u * (uint32_t)c, s);
+        float(&v)[16] = s[c & 1];
+        tmem_wait_ld(v);
+        if (c < 3) tmem_ld(at + 16u * (uint32_t)(c + 1), s[(c + 1) & 1]);
+        if (MASK)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float x = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                x = fmaxf(x, MASK && 32 * c + 16 * h + i >= nvis ? -INFINITY : s[16 * h + i]);
-            const float f = __shfl_sync(0xffffffffu, sc, 2 * c + h) * factor;
-            if (!MASK || x != -INFINITY) m = fmaxf(m, x * f);
-        }
+            for (int i = 0; i < 16; ++i) v[i] = 16 * c + i < nvis ? v[i] : -INFINITY;
+        const float x = max3(max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8])),
+                             max3(v[9], v[10], v[11]), max3(max3(v[12], v[13], v[14]), v[15], v[15]));
+        if (!MASK || x != -INFINITY) m = fmaxf(m, x * f[c]);
     }
     return m;
 }
 
-// The weights into the scores' columns, 32 keys at a time: 16 columns of hi, 16 of lo. Returns their sum.
-template <bool MASK>
-__device__ __forceinline__ float tile_weights(uint32_t at, float sc, float factor, int nvis, float m, float vinv)
+// Two floats in one register pair, for the packed fp32 instructions
+__device__ __forceinline__ uint64_t pair(float a, float b)
 {
-    float sum = 0.f;
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void unpair(uint64_t d, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// The weights into the scores' columns, 16 keys at a time: 8 columns of hi, 8
+// of lo. The V scale over vref enters the exponent: lg[i] is its base-2
+// logarithm for group i, and ipf[i], its reciprocal, takes it out of the
+// group's sum again. Returns the sum of the weights without it.
+template <bool MASK>
+__device__ __forceinline__ float tile_weights(uint32_t at, const float (&f)[4], const float (&lg)[4], const float (&ipf)[4],
+                                              int nvis, float m)
+{
+    float sum = 0.f, s[2][16];
+    const uint64_t minus = pair(-1.0f, -1.0f);
+    tmem_ld(at, s[0]);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-        float s[32];
-        tmem_ld(at + 32u * (uint32_t)c, s);
-        uint32_t p[32];
+        const float(&v)[16] = s[c & 1];
+        tmem_wait_ld(s[c & 1]);
+        if (c < 3) tmem_ld(at + 16u * (uint32_t)(c + 1), s[(c + 1) & 1]);
+        const float off = lg[c] - m;
+        const uint64_t f2 = pair(f[c], f[c]), off2 = pair(off, off);
+        uint32_t p[16];
+        uint64_t part = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float f = __shfl_sync(0xffffffffu, sc, 2 * c + h) * factor;
-            const float pf = __shfl_sync(0xffffffffu, sc, 8 + 2 * c + h) * vinv;
-            float part = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                float hi[2], lo[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const bool seen = !MASK || 32 * c + 16 * h + i + e < nvis;
-                    float w = ex2(fmaf(s[16 * h + i + e], f, -m));
-                    if (MASK && !seen) w = 0.f;
-                    part += w;
-                    w *= pf;
-                    if (MASK && !seen) w = 0.f;   // whatever the block's scale is
-                    hi[e] = __uint_as_float(__float_as_uint(w) & 0xffffe000u);   // exact in binary16
-                    lo[e] = w - hi[e];
-                }
-                p[8 * h + i / 2] = h2_bits(hi[0], hi[1]);
-                p[16 + 8 * h + i / 2] = h2_bits(lo[0], lo[1]);
+        for (int i = 0; i < 16; i += 2) {
+            float w0, w1;
+            unpair(fma2(pair(v[i], v[i + 1]), f2, off2), w0, w1);
+            w0 = ex2(w0);
+            w1 = ex2(w1);
+            if (MASK) {   // a masked position counts nothing, whatever its block's scales are
+                w0 = 16 * c + i < nvis ? w0 : 0.f;
+                w1 = 16 * c + i + 1 < nvis ? w1 : 0.f;
             }
-            sum += part;
+            const uint64_t w = pair(w0, w1);
+            part = add2(part, w);
+            // the upper 11 bits are exact in binary16
+            const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
+            float l0, l1;
+            unpair(fma2(pair(h0, h1), minus, w), l0, l1);
+            p[i / 2] = h2_bits(h0, h1);
+            p[8 + i / 2] = h2_bits(l0, l1);
         }
-        tmem_st(at + 32u * (uint32_t)c, p);
+        float a0, a1;
+        unpair(part, a0, a1);
+        if (!MASK || 16 * c < nvis) sum = fmaf(a0 + a1, ipf[c], sum);
+        tmem_st(at + 16u * (uint32_t)c, p);
     }
     return sum;
 }
 
+// Barrier `id` of `threads` threads (whole warps); the second tells whether any of them brought a true
+__device__ __forceinline__ void meet(uint32_t id, uint32_t threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ bool meet_any(uint32_t id, uint32_t threads, bool x)
+{
+    uint32_t r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %3, 0;\n bar.red.or.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(r)
+                 : "r"(id), "r"(threads), "r"((uint32_t)x)
+                 : "memory");
+    return r != 0u;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there)   // zeros where !there
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait0() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_constant__ AttnArgs a)
 {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-    uint8_t *const qs = smem, *const ks = smem + 2 * kQTile, *const vs = ks + 2 * kHalf;
-    PromptBars &b = *reinterpret_cast<PromptBars *>(vs + 2 * kHalf);
+    extern __shared__ __align__(1024) uint8_t prompt_smem[];
+    uint8_t *const qs = prompt_smem, *const ks = qs + 2 * kQTile, *const vs = ks + 2 * kHalf, *const raw = vs + 2 * kHalf;
+    PromptBars &b = *reinterpret_cast<PromptBars *>(raw + 2 * kRawTile);
+    RowStates &rs = *reinterpret_cast<RowStates *>(raw);
     volatile uint32_t *const err = &b.status;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t C = cluster_size(), rank = cluster_rank(), s = blockIdx.z, h = blockIdx.y;
@@ -227,13 +305,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; ++t) {
             mbar_init(&b.s_full[t], 1u);
-            mbar_init(&b.p_full[t], 4u);
+            mbar_init(&b.p_full[t], 8u);
             mbar_init(&b.o_full[t], 1u);
+            mbar_init(&b.k_full[t], 4u);
+            mbar_init(&b.v_full[t], 2u);
+            mbar_init(&b.k_empty[t], 1u);
+            mbar_init(&b.v_empty[t], 1u);
         }
-        mbar_init(&b.k_full, 4u);
-        mbar_init(&b.v_full, 4u);
-        mbar_init(&b.k_empty, 1u);
-        mbar_init(&b.v_empty, 1u);
         mbar_init(&b.fin, 1u);
         b.status = kStatusOk;
         fence_mbar_init();
@@ -287,7 +365,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                     lo[k] = v[k] - hi[k];
                 }
                 if (lane == 0)
-                    b.row_factor[i / kTileRows][row] = bad ? __int_as_float(0x7fffffff) : kScoreScale * g0 * g1;
+                    b.half[i / kTileRows][0][row] = bad ? __int_as_float(0x7fffffff) : kScoreScale * g0 * g1;
                 uint8_t *q = qs + (i / kTileRows) * kQTile + (lane >> 4) * kHalf + swizzled(row, (lane & 15u) >> 1) + (lane & 1u) * 8u;
                 *reinterpret_cast<uint2 *>(q) = make_uint2(h2_bits(hi[0], hi[1]), h2_bits(hi[2], hi[3]));
                 *reinterpret_cast<uint2 *>(q + 2 * kHalf) = make_uint2(h2_bits(lo[0], lo[1]), h2_bits(lo[2], lo[3]));
@@ -298,49 +376,55 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     fence_before();
     __syncthreads();
     fence_after();
+    float row_m = -INFINITY, row_l = 0.f;   // softmax threads of half 0: their row's state, for the cluster
     const uint32_t tmem = b.tmem;   // scores / weights of tile t: column 128 t; output: 256 + 128 t
 
     if (warp == kMmaWarp) {
         // ------------------------------------------------------------- MMA --
-        if (lane == 0) {
-            const uint32_t qa = smem_addr(qs), ka = smem_addr(ks), va = smem_addr(vs);
-            auto scores = [&](uint32_t t) {
-                for (uint32_t st = 0; st < 8u; ++st) {
-                    const uint32_t off = (st >> 2) * kHalf + (st & 3u) * 32u;
-                    const uint64_t k = operand(ka + off);
-                    mma_ss(tmem + 128u * t, operand(qa + t * kQTile + off), k, st != 0u);
-                    mma_ss(tmem + 128u * t, operand(qa + t * kQTile + 2u * kHalf + off), k, 1u);
+        if (elected()) {
+            // a step of 16 along K is 32 bytes, 2 in a descriptor; 4 steps fill a swizzled tile
+            const uint64_t qd = operand(smem_addr(qs)), kd = operand(smem_addr(ks)), vd = operand(smem_addr(vs));
+            // K and V go by halves (64 dimensions, 64 keys): a half is converted
+            // while the MMAs still read, or already read, the other.
+            bool ok = n != 0u;
+            auto scores = [&](uint32_t t, uint32_t j) {   // of keys j: the first tile waits for K, the last one releases it
+                const uint64_t q = qd + (uint64_t)(t * (kQTile >> 4));
+#pragma unroll
+                for (uint32_t hf = 0; hf < 2u; ++hf) {
+                    if (t == 0u) {
+                        if (!(ok = ok && mbar_wait(&b.k_full[hf], j & 1u, err))) return;
+                        fence_after();
+                    }
+#pragma unroll
+                    for (uint32_t st = 0; st < 4u; ++st) {
+                        const uint32_t off = hf * (kHalf >> 4) + st * 2u;
+                        mma_ss(tmem + 128u * t, q + off, kd + off, hf != 0u || st != 0u);
+                        mma_ss(tmem + 128u * t, q + (2u * kHalf >> 4) + off, kd + off, 1u);
+                    }
+                    if (t + 1u == tiles) commit(&b.k_empty[hf]);
                 }
                 commit(&b.s_full[t]);
             };
-            bool ok = n != 0u;
-            if (ok && (ok = mbar_wait(&b.k_full, 0u, err))) {
-                fence_after();
-                for (uint32_t t = 0; t < tiles; ++t) scores(t);
-                commit(&b.k_empty);
-            }
+            for (uint32_t t = 0; ok && t < tiles; ++t) scores(t, 0u);
             for (uint32_t j = 0; ok && j < n; ++j) {
-                if (!(ok = mbar_wait(&b.v_full, j & 1u, err))) break;
-                for (uint32_t t = 0; t < tiles; ++t) {
+                for (uint32_t t = 0; ok && t < tiles; ++t) {
                     if (!(ok = mbar_wait(&b.p_full[t], j & 1u, err))) break;
-                    fence_after();
-                    for (uint32_t st = 0; st < 8u; ++st) {
-                        const uint64_t v = operand(va + (st >> 2) * kHalf + (st & 3u) * 32u);
-                        const uint32_t p = tmem + 128u * t + (st >> 1) * 32u + (st & 1u) * 8u;
-                        mma_ts(tmem + 256u + 128u * t, p, v, j != 0u || st != 0u);
-                        mma_ts(tmem + 256u + 128u * t, p + 16u, v, 1u);
-                    }
-                    if (t + 1u == tiles) commit(&b.v_empty);
-                    if (j + 1u == n) {
-                        commit(&b.o_full[t]);
-                        continue;
-                    }
-                    if (t == 0u) {
-                        if (!(ok = mbar_wait(&b.k_full, (j + 1u) & 1u, err))) break;
+#pragma unroll
+                    for (uint32_t hf = 0; hf < 2u; ++hf) {
+                        if (t == 0u && !(ok = ok && mbar_wait(&b.v_full[hf], j & 1u, err))) break;
                         fence_after();
+#pragma unroll
+                        for (uint32_t st = 0; st < 4u; ++st) {
+                            const uint64_t v = vd + hf * (kHalf >> 4) + st * 2u;
+                            const uint32_t p = tmem + 128u * t + 64u * hf + 16u * st;
+                            mma_ts(tmem + 256u + 128u * t, p, v, j != 0u || hf != 0u || st != 0u);
+                            mma_ts(tmem + 256u + 128u * t, p + 8u, v, 1u);
+                        }
+                        if (t + 1u == tiles) commit(&b.v_empty[hf]);
                     }
-                    scores(t);
-                    if (t + 1u == tiles) commit(&b.k_empty);
+                    if (!ok) break;
+                    if (j + 1u < n) scores(t, j + 1u);
+                    else commit(&b.o_full[t]);
                 }
             }
             // nothing of this CTA is left in flight when tensor memory is freed
@@ -350,60 +434,73 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             }
         }
         __syncwarp();
-    } else if (warp >= 8) {
+    } else if (warp >= kConvWarp) {
         // ------------------------------------------------------- converters --
         // K: a thread takes 16 dimensions of 8 keys (8 lanes write the same
         // chunk of 8 rows); V: 8 keys x 16 dimensions (8 lanes write the 8
-        // chunks of a row): neither has a bank conflict.
-        const uint32_t w = warp - 8u, l8 = lane & 7u, q8 = lane >> 3;
+        // chunks of a row): neither has a bank conflict. A thread copies just
+        // the codes that it converts, into slots [piece][thread].
+        const uint32_t w = warp - kConvWarp, l8 = lane & 7u, q8 = lane >> 3;
         const int8_t *ksrc = a.c.k + (head * a.c.max_context + 8u * w + l8) * kDim + 16u * q8;
         const uint32_t kg = l8 + 8u * (w >> 1), dg = q8 + 4u * (w & 1u);
         const int8_t *vsrc = a.c.v + (head * a.c.max_context + 8u * kg) * kDim + 16u * dg;
-        uint4 x[8], y[8];
-        auto load_k = [&](uint32_t j) {
-            const uint32_t key0 = (j0 + j) * kTileKeys;
+        uint4 *const kslot = reinterpret_cast<uint4 *>(raw) + (w * 32u + lane), *const vslot = kslot + kRawTile / 16u;
+        auto copy_k = [&](uint32_t j) {
+            if (j < n) {
+                const uint32_t key0 = (j0 + j) * kTileKeys;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t row = 32u * (i >> 1);
-                x[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (key0 + row + 8u * w + l8 < limit)
-                    x[i] = __ldcg(reinterpret_cast<const uint4 *>(ksrc + (size_t)(key0 + row) * kDim + 64u * (i & 1u)));
-            }
-        };
-        auto load_v = [&](uint32_t j) {
-            const uint32_t key0 = (j0 + j) * kTileKeys;
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                y[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (key0 + 8u * kg + i < limit) y[i] = __ldcg(reinterpret_cast<const uint4 *>(vsrc + (size_t)(key0 + i) * kDim));
-            }
-        };
-        if (n) {
-            load_k(0u);
-            load_v(0u);
-        }
-        for (uint32_t j = 0; j < n; ++j) {
-            if (j && !wait_warp(&b.k_empty, (j - 1u) & 1u, err)) break;
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t row = 32u * (i >> 1) + 8u * w + l8;
-                uint8_t *dst = ks + (i & 1u) * kHalf;
-                const uint32_t words[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                uint32_t o[8];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {   // two neighbouring dimensions, each in the low byte of a half
-                    o[2 * q] = codes_h2<false>(__byte_perm(words[q], 0u, 0x4140u));
-                    o[2 * q + 1] = codes_h2<false>(__byte_perm(words[q], 0u, 0x4342u));
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint32_t row = 32u * (i >> 1);
+                    copy16(smem_addr(kslot + 128u * i), ksrc + (size_t)(key0 + row) * kDim + 64u * (i & 1u),
+                           key0 + row + 8u * w + l8 < limit);
                 }
-                *reinterpret_cast<uint4 *>(dst + swizzled(row, 2u * q8)) = make_uint4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<uint4 *>(dst + swizzled(row, 2u * q8 + 1u)) = make_uint4(o[4], o[5], o[6], o[7]);
             }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&b.k_full);
-            if (j + 1u < n) load_k(j + 1u);
-            if (j && !wait_warp(&b.v_empty, (j - 1u) & 1u, err)) break;
-            uint8_t *dst = vs + (kg >> 3) * kHalf;
+            copy_commit();
+        };
+        auto copy_v = [&](uint32_t j) {
+            if (j < n) {
+                const uint32_t key0 = (j0 + j) * kTileKeys;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    copy16(smem_addr(vslot + 128u * i), vsrc + (size_t)(key0 + i) * kDim, key0 + 8u * kg + i < limit);
+            }
+            copy_commit();
+        };
+        copy_k(0u);
+        copy_v(0u);
+        for (uint32_t j = 0; j < n; ++j) {
+            copy_wait1();   // K of this tile; V may still be on its way
+            bool ok = true;
+#pragma unroll
+            for (uint32_t hf = 0; hf < 2u; ++hf) {
+                if (j && !(ok = ok && wait_warp(&b.k_empty[hf], (j - 1u) & 1u, err))) break;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t row = 32u * i + 8u * w + l8;
+                    const uint4 x = kslot[128u * (2u * i + hf)];
+                    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+                    uint32_t o[8];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {   // two neighbouring dimensions, each in the low byte of a half
+                        o[2 * q] = codes_h2<false>(__byte_perm(words[q], 0u, 0x4140u));
+                        o[2 * q + 1] = codes_h2<false>(__byte_perm(words[q], 0u, 0x4342u));
+                    }
+                    uint8_t *dst = ks + hf * kHalf;
+                    *reinterpret_cast<uint4 *>(dst + swizzled(row, 2u * q8)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4 *>(dst + swizzled(row, 2u * q8 + 1u)) = make_uint4(o[4], o[5], o[6], o[7]);
+                }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b.k_full[hf]);
+            }
+            if (!ok) break;
+            copy_k(j + 1u);
+            copy_wait1();   // V of this tile; warps 0, 1 have its first 64 keys, 2, 3 the others
+            if (j && !wait_warp(&b.v_empty[w >> 1], (j - 1u) & 1u, err)) break;
+            uint8_t *dst = vs + (w >> 1) * kHalf;
+            uint4 y[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) y[i] = vslot[128u * i];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t o[4][4];   // dimension 4 q + ., key pair
@@ -420,20 +517,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 }
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
-                    *reinterpret_cast<uint4 *>(dst + swizzled(16u * dg + 4u * (uint32_t)q + (uint32_t)d, kg & 7u)) =
+                    *reinterpret_cast<uint4 *>(dst + swizzled(16u * dg + 4u * (uint32_t)q + (uint32_t)d, l8)) =
                         make_uint4(o[d][0], o[d][1], o[d][2], o[d][3]);
             }
             fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.v_full);
-            if (j + 1u < n) load_v(j + 1u);
+            if (lane == 0) mbar_arrive(&b.v_full[w >> 1]);
+            copy_v(j + 1u);
         }
+        copy_wait0();
     } else {
         // --------------------------------------------------------- softmax --
-        const uint32_t t = warp >> 2, quarter = warp & 3u, row = quarter * 32u + lane, i = t * kTileRows + row;
+        // Warps w and w + 4 of a tile share 32 rows. A warp whose wait ran out
+        // goes on through the barriers, without touching tensor memory.
+        const uint32_t t = warp >> 3, half = (warp >> 2) & 1u, quarter = warp & 3u, row = quarter * 32u + lane;
+        const uint32_t i = t * kTileRows + row;
         if (t < tiles) {
-            const uint32_t at = tmem + ((quarter * 32u) << 16) + 128u * t;
-            const float factor = b.row_factor[t][row];
+            const uint32_t at = tmem + ((quarter * 32u) << 16) + 128u * t + 64u * half, g0 = 4u * half;
+            const float factor = b.half[t][0][row];
             const uint32_t open = (uint32_t)min(p0 + tr.at(t * kTileRows).x, (uint64_t)0x7fffffffu);
             const uint32_t last = i < rows ? (uint32_t)min(p0 + tr.at(i).x, (uint64_t)0x7fffffffu) : open;
             const float *scales = (lane & 8u ? a.c.v_scale : a.c.k_scale) + head * a.c.n_blocks;
@@ -442,75 +543,108 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             };
             float m = -INFINITY, l = 0.f, next = n ? scale_of(0u) : 0.f;
             uint32_t vref = kTinyScale;
+            bool ok = true;
             for (uint32_t j = 0; j < n; ++j) {
                 const float sc = next;
                 if (j + 1u < n) next = scale_of(j + 1u);
-                const uint32_t key0 = (j0 + j) * kTileKeys;
+                const uint32_t key0 = (j0 + j) * kTileKeys, mine = key0 + 64u * half;
                 const bool masked = key0 + kTileKeys - 1u > open;   // some row does not see all of the tile
-                const int nvis = last < key0 ? 0 : (int)min(last - key0 + 1u, kTileKeys);
+                const int nvis = last < mine ? 0 : (int)min(last - mine + 1u, 64u);
                 // the largest V scale of the tile's stored positions (a NaN counts nothing)
                 float top = lane >= 8u && lane < 16u && key0 + 16u * (lane & 7u) < limit ? sc : 0.f;
                 top = __uint_as_float(__reduce_max_sync(0xffffffffu, top > 0.f && top < INFINITY ? __float_as_uint(top) : 0u));
-                if (!wait_warp(&b.s_full[t], j & 1u, err)) break;
-                fence_after();
-                const float x = masked ? tile_max<true>(at, sc, factor, nvis) : tile_max<false>(at, sc, factor, 128);
-                float f = 1.0f;
-                if (x > m + kLazy) {
-                    f = m == -INFINITY ? 0.f : ex2(m - x);
-                    m = x;
-                    l *= f;
-                }
+                float fv = 1.0f;   // what the output is rescaled by for a larger vref
                 if (top >= 2.0f * __uint_as_float(vref)) {
                     const uint32_t now = __float_as_uint(top) & 0x7f800000u;
-                    f *= now - vref > 120u << 23 ? 0.f : __uint_as_float((127u << 23) - (now - vref));
+                    fv = now - vref > 120u << 23 ? 0.f : __uint_as_float((127u << 23) - (now - vref));
                     vref = now;
                 }
-                if (j && __any_sync(0xffffffffu, f != 1.0f)) {
-#pragma unroll 1
-                    for (uint32_t c = 0; c < 128u; c += 32u) {
-                        float o[32];
-                        uint32_t u[32];
-                        tmem_ld(at + 256u + c, o);
+                // All that needs no scores is done before they come. pf = v_scale / vref * 2^6, at least 2^-40
+                // (below that nothing of it is left in binary16; a block of zeros has scale 0).
+                const float pv = sc * __uint_as_float((260u << 23) - vref), pf = pv < 0x1p-40f ? 0x1p-40f : pv;
+                const float pl = __log2f(pf), pr = rcp(pf);
+                float f[4], lg[4], ipf[4];
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) u[k] = __float_as_uint(o[k] * f);
-                        tmem_st(at + 256u + c, u);
+                for (uint32_t c = 0; c < 4u; ++c) {
+                    f[c] = __shfl_sync(0xffffffffu, sc, g0 + c) * factor;
+                    lg[c] = __shfl_sync(0xffffffffu, pl, 8u + g0 + c);
+                    ipf[c] = __shfl_sync(0xffffffffu, pr, 8u + g0 + c);
+                }
+                ok = ok && wait_warp(&b.s_full[t], j & 1u, err);
+                fence_after();
+                float x = -INFINITY;
+                if (ok) x = masked ? tile_max<true>(at, f, nvis) : tile_max<false>(at, f, 64);
+                const bool raise = meet_any(1u + t, 256u, x > m + kLazy);
+                if (raise || fv != 1.0f) {
+                    if (raise) {
+                        b.half[t][half][row] = x;
+                        meet(1u + t, 256u);
+                        x = fmaxf(x, b.half[t][half ^ 1u][row]);
+                    }
+                    if (x > m + kLazy) {
+                        const float fm = m == -INFINITY ? 0.f : ex2(m - x);
+                        m = x;
+                        l *= fm;
+                        fv *= fm;
+                    }
+                    if (j && ok) {
+#pragma unroll 1
+                        for (uint32_t c = 0; c < 64u; c += 16u) {
+                            float o[16];
+                            uint32_t u[16];
+                            tmem_ld(at + 256u + c, o);
+                            tmem_wait_ld(o);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(o[k] * fv);
+                            tmem_st(at + 256u + c, u);
+                        }
                     }
                 }
-                const float vinv = __uint_as_float((260u << 23) - vref);   // 2^6 / vref
-                l += masked ? tile_weights<true>(at, sc, factor, nvis, m, vinv) : tile_weights<false>(at, sc, factor, 128, m, vinv);
+                if (ok)
+                    l += masked ? tile_weights<true>(at, f, lg, ipf, nvis, m) : tile_weights<false>(at, f, lg, ipf, 64, m);
                 tmem_wait_st();
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&b.p_full[t]);
             }
+            // the sum of both halves
+            meet(1u + t, 256u);
+            b.half[t][half][row] = l;
+            meet(1u + t, 256u);
+            l += b.half[t][half ^ 1u][row];
             // the output into Q's place: row-major, 16-byte chunks XORed with the row
-            const bool have = n && wait_warp(&b.o_full[t], 0u, err);
+            const bool have = n && ok && wait_warp(&b.o_full[t], 0u, err);
             fence_after();
             const float back = C > 1u ? __uint_as_float(vref) * (1.0f / 64.0f) : __uint_as_float(vref) * (1.0f / 64.0f) / l;
             float4 *stage = reinterpret_cast<float4 *>(qs + t * kQTile);
 #pragma unroll 1
             for (uint32_t c = 0; c < 4u; ++c) {
-                float o[32];
-                if (have) tmem_ld(at + 256u + 32u * c, o);
+                float o[16];
+                if (have) {
+                    tmem_ld(at + 256u + 16u * c, o);
+                    tmem_wait_ld(o);
+                }
 #pragma unroll
-                for (uint32_t k = 0; k < 8; ++k)
-                    stage[row * 32u + ((8u * c + k) ^ (row & 31u))] =
+                for (uint32_t k = 0; k < 4; ++k)
+                    stage[row * 32u + ((16u * half + 4u * c + k) ^ (row & 31u))] =
                         have ? make_float4(o[4 * k] * back, o[4 * k + 1] * back, o[4 * k + 2] * back, o[4 * k + 3] * back)
                              : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            b.row_max[t][row] = m;
-            b.row_sum[t][row] = l;
-            __syncwarp();
+            meet(1u + t, 256u);
             if (C == 1u) {
-                for (uint32_t k = 0; k < 32u && t * kTileRows + quarter * 32u + k < rows; ++k) {
-                    const uint32_t rr = quarter * 32u + k;
-                    const uint2 r = tr.at(t * kTileRows + rr);
-                    float4 x = stage[rr * 32u + (lane ^ (rr & 31u))];
+                // warp w of the tile: rows 16 w .. 16 w + 15
+                const uint32_t w0 = (warp & 7u) * 16u;
+                for (uint32_t k = w0; k < w0 + 16u && t * kTileRows + k < rows; ++k) {
+                    const uint2 r = tr.at(t * kTileRows + k);
+                    float4 x = stage[k * 32u + (lane ^ (k & 31u))];
                     if (*err != kStatusOk || p0 + r.x >= a.c.max_context)
                         x.x = x.y = x.z = x.w = __int_as_float(0x7fffffff);
                     reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo +
                                                (size_t)(h * a.group + r.y) * kDim)[lane] = x;
                 }
+            } else if (half == 0u) {
+                row_m = m;
+                row_l = l;
             }
         }
     }
@@ -521,14 +655,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
     if (C == 1u) return;
+    // the converters' slots are free now
+    if (warp < kConvWarp && (warp & 4u) == 0u) {
+        rs.max[warp >> 3][(warp & 3u) * 32u + lane] = row_m;
+        rs.sum[warp >> 3][(warp & 3u) * 32u + lane] = row_l;
+    }
     // Rows rank, rank + C, ... of the cluster's states: a warp per row, lane = 4
     // dimensions. A state that saw no position counts nothing.
     cluster_sync();
     if (warp < kMmaWarp) {
         for (uint32_t i = rank + C * warp; i < rows; i += C * kMmaWarp) {
             const uint32_t t = i / kTileRows, row = i & (kTileRows - 1u);
-            const float mc = lane < C ? ld_cluster1(&b.row_max[t][row], lane) : -INFINITY;
-            const float lc = lane < C ? ld_cluster1(&b.row_sum[t][row], lane) : 0.f;
+            const float mc = lane < C ? ld_cluster1(&rs.max[t][row], lane) : -INFINITY;
+            const float lc = lane < C ? ld_cluster1(&rs.sum[t][row], lane) : 0.f;
             const bool bad = lane < C && __float_as_uint(ld_cluster1(&b.status, lane)) != kStatusOk;
             float M = mc;
 #pragma unroll
@@ -567,10 +706,10 @@ cudaError_t launch_prompt(AttnArgs a, int dev, int sms, cudaStream_t stream)
     cudaError_t e = allow<prompt_kernel>(dev, (int)kPromptSmem);
     if (e != cudaSuccess) return e;
     a.tiles = (a.r.tokens * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
-    // CTAs per unit: while they all fit at once, at most 8, and 2 tiles of keys each
+    // CTAs per unit: as many as fit the device at once (one per SM), at most 8, two tiles of keys each at least
     const uint64_t units = (uint64_t)a.tiles * a.c.kv_heads * a.c.nseq;
-    uint32_t C = 1;
-    while (C < 8 && units * C * 2 <= (uint64_t)sms && (uint64_t)C * 2 * 2 * kTileKeys <= a.c.max_context) C *= 2;
+    const uint64_t fit = std::min<uint64_t>((uint64_t)sms / units, a.c.max_context / (2 * kTileKeys));
+    const uint32_t C = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(fit, 1), 8);
     return launch(prompt_kernel, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), kPromptThreads, kPromptSmem, C, a, sms, stream);
 }
 
