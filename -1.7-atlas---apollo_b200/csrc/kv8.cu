@@ -10,6 +10,7 @@
 #include <cmath>
 #include <algorithm>
 #include <atomic>
+#include <cuda.h>
 #include "../../include/atlas_cuda.h"
 #include "common.cuh"
 #include "kv8.cuh"
@@ -197,10 +198,13 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
 // merge through shared memory, then through the cluster's distributed shared
 // memory: one launch, no workspace.
 //
-// Chunks arrive by cp.async, kStages deep. A lane copies exactly the 16-byte
-// pieces that it reads itself (K: rows g and g + 8, V: rows 2t, 2t + 1,
-// 2t + 8, 2t + 9 of the lane's g = lane / 4, t = lane % 4), so a chunk needs
-// no barrier and its slot [piece][lane] has no bank conflict.
+// Chunks arrive as two TMA copies (16 rows of K, 16 of V, swizzled) into a ring
+// of the warp's own, kStages deep, with a barrier per slot: no CTA-wide step
+// until the merge. ldmatrix reads K as the MMAs want it; of V a lane reads the
+// 16 dimensions g of rows 2t, 2t + 1, 2t + 8, 2t + 9 (g = lane / 4, t = lane
+// % 4), which two byte permutations turn into pairs of rows. Neither has a bank
+// conflict. (16-byte cp.async copies by the lanes instead: 4.7 TB/s without any
+// arithmetic, bound by the load/store unit.)
 //
 //   S^T = K Q^T   m16n8k32 integer MMAs straight on the codes (rows are
 //                 positions, columns query rows). Q is staged as three int8
@@ -221,10 +225,10 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
 
 constexpr uint32_t kFewRows = 48;   // query rows of a KV head up to which this form is taken
 constexpr uint32_t kStages = 3;
-constexpr uint32_t kWarps = 8, kWarpsLog2 = 3, kThreads = kWarps * 32;
+constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;   // block selection
 constexpr uint32_t kSlot = 8 * 32 * 16;                     // bytes of a chunk: 16 rows of K and V
 
-constexpr uint32_t kMaxCluster = 16;                        // >= 8 NT: the rows of a tile, or their states
+constexpr uint32_t kMaxCluster = 16;                        // also the states that a CTA receives: C ceil(8 NT / C)
 constexpr uint32_t kRecStride = kDim + 4;                   // output, maximum, sum
 constexpr int kSumBits = 0x4B400000;                  // 2^23 + 2^22: integer sums below 2^22 read as floats
 
@@ -258,22 +262,31 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x)
     return y;
 }
 
-// 16 bytes global -> shared; in the second form nothing is read and zeros are stored where !there
-template <int DST, int SRC>
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src)
+// 16 rows of 128 bytes from row `row` of a tensor of codes to shared memory, 16-byte
+// chunk c of row r at chunk c ^ (r % 8); rows behind the tensor's end are zeros
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, uint32_t row, uint64_t *bar)
 {
-    asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
-}
-template <int DST, int SRC>
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there)
-{
-    asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16, %4;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC),
-                 "r"(there ? 16u : 0u)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"((int)row), "r"(smem_addr(bar))
                  : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Four 8 x 16-byte matrices: lane i has the address of row i % 8 of matrix i / 8, and gets bytes 4 t .. 4 t + 3 of
+// row g of each (g = lane / 4, t = lane % 4)
+__device__ __forceinline__ void load_matrices(int (&d)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared4(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 
 // Split: arrive once the CTA runs, wait before the first access to another CTA's shared memory
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
@@ -292,15 +305,23 @@ __device__ __forceinline__ void st_cluster(unsigned long long *p, uint32_t cta, 
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(r), "l"(v) : "memory");
 }
 
-template <int NT>
-struct alignas(16) Smem {
+// The arguments of the few-rows kernels: the codes as tensors of 128-byte rows, too
+struct FewArgs : AttnArgs {
+    CUtensorMap kmap, vmap;
+};
+
+template <int NT, uint32_t W>
+struct alignas(1024) Smem {
     union {
-        uint8_t ring[kWarps][kStages][kSlot];
-        float wrec[kWarps][8 * NT][kRecStride];   // the warps' outputs, once the ring is done with
+        uint8_t ring[W][kStages][kSlot];
+        float wrec[W][8 * NT][kRecStride];     // the warps' outputs, once the ring is done with
     } u;
     float rec[kMaxCluster][kRecStride];        // the states that the cluster's CTAs send of this CTA's rows
-    float2 wml[kWarps][8 * NT];                // the warps' maxima and sums
-    uint32_t plane[3][8 * NT][kDim / 4 + 16];  // rows 48 words apart: the fragment reads have no bank conflict
+    uint64_t full[W][kStages];                 // a chunk has landed
+    uint32_t err;
+    float2 wml[W][8 * NT];                     // the warps' maxima and sums
+    alignas(16) uint32_t plane[3][8 * NT][kDim / 4 + 16];   // in the order of the B operands (lane t: 8 words from 8 t);
+                                               // rows 48 words apart: their reads have no bank conflict
     float qs[8 * NT];                          // what a unit of the first plane is worth in each row
 };
 
@@ -319,81 +340,81 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, const TileRows &tr,
     reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo + (size_t)(h * a.group + r.y) * kDim)[d4] = x;
 }
 
-// This warp's query rows warp, warp + 8, ... of the tile (lane = 4 dimensions). Rows of tokens that the call does
-// not have are zeros; rows past n_tok are read and their results dropped.
+// This warp's query rows warp, warp + 8, ... of the tile (lane = 4 dimensions; warps from 8 on have none). Rows of
+// tokens that the call does not have are zeros; rows past n_tok are read and their results dropped.
 template <int NT>
 __device__ __forceinline__ void load_queries(const AttnArgs &a, const TileRows &tr, uint32_t s, uint32_t h, float4 (&x)[NT])
 {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-        const uint2 r = tr.at(warp + kWarps * (uint32_t)i);
+        const uint2 r = tr.at(warp + 8u * (uint32_t)i);
         x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r.x < a.r.tokens)
+        if (warp < 8u && r.x < a.r.tokens)
             x[i] = __ldcg(reinterpret_cast<const float4 *>(a.q + ((size_t)s * a.r.tokens + r.x) * a.ldq +
                                                           (size_t)(h * a.group + r.y) * kDim) + lane);
     }
 }
 
+// The ring's barriers, by the lane that will use them; before anything is read
+template <int NT, uint32_t W>
+__device__ __forceinline__ void init_ring(const FewArgs &a, Smem<NT, W> &sm)
+{
+    if ((threadIdx.x & 31u) == 0u) {
+        for (uint32_t i = 0; i < kStages; ++i) mbar_init(&sm.full[threadIdx.x >> 5][i], 1u);
+        fence_mbar_init();
+    }
+    if (threadIdx.x == 0u) {
+        sm.err = kStatusOk;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a.kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a.vmap) : "memory");
+    }
+    __syncthreads();
+}
+
 // One (sequence, KV head, tile of query rows) on this cluster. `rows`: the
-// tile's rows that exist. KEYS deals chunks [0, chunks); positions at or above
-// `limit` are not read. `open`: every row sees the positions up to it. The
-// CTAs of a cluster have arrived on its barrier once before.
-template <int NT, class KEYS>
-__device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KEYS &keys, const float4 (&qx)[NT],
+// tile's rows that exist. KEYS deals chunks [0, chunks). The CTAs of a cluster
+// have arrived on its barrier once before.
+template <int NT, uint32_t W, class KEYS>
+__device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const KEYS &keys, const float4 (&qx)[NT],
                                        const TileRows &tr, uint32_t s, uint32_t h, uint32_t rows, uint64_t p0,
-                                       uint32_t chunks, uint32_t limit)
+                                       uint32_t chunks)
 {
     constexpr uint32_t R = 8 * NT;
-    static_assert(R == kWarps * NT, "a warp stages NT query rows");
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    const uint32_t C = cluster_size(), clog = 31u - __clz(C), rank = cluster_rank();
+    const uint32_t C = cluster_size(), rank = cluster_rank();
     const size_t head = (size_t)s * a.c.kv_heads + h;
-    const int8_t *kc = a.c.k + head * a.c.max_context * kDim + g * kDim + 16u * t;
-    const int8_t *vc = a.c.v + head * a.c.max_context * kDim + 2u * t * kDim + 16u * g;
+    const uint32_t row0 = (uint32_t)head * a.c.max_context;   // of the tensors of codes
     const float *ksc = a.c.k_scale + head * a.c.n_blocks, *vsc = a.c.v_scale + head * a.c.n_blocks;
 
     // this warp's chunks are first, first + step, ...
-    const uint32_t first = rank + (warp << clog), slog = clog + kWarpsLog2;
-    const uint32_t n = chunks > first ? ((chunks - first - 1u) >> slog) + 1u : 0u;
-    const uint32_t slot0 = smem_addr(sm.u.ring[warp][0]) + lane * 16u;
+    const uint32_t first = rank + C * warp, step = C * W;
+    const uint32_t ring = smem_addr(sm.u.ring[warp][0]);
+    uint64_t *const full = sm.full[warp];
     auto issue = [&](uint32_t i, uint32_t slot) {
-        if (i < n) {
-            const uint32_t key = keys.key0(first + (i << slog)), dst = slot0 + slot * kSlot;
-            const int8_t *kr = kc + (size_t)key * kDim, *vr = vc + (size_t)key * kDim;
-            if (key + kChunk <= limit) {
-                copy16<0, 0>(dst, kr);
-                copy16<512, 64>(dst, kr);
-                copy16<1024, 8 * kDim>(dst, kr);
-                copy16<1536, 8 * kDim + 64>(dst, kr);
-                copy16<2048, 0>(dst, vr);
-                copy16<2560, kDim>(dst, vr);
-                copy16<3072, 8 * kDim>(dst, vr);
-                copy16<3584, 9 * kDim>(dst, vr);
-            } else {
-                copy16<0, 0>(dst, kr, key + g < limit);
-                copy16<512, 64>(dst, kr, key + g < limit);
-                copy16<1024, 8 * kDim>(dst, kr, key + g + 8u < limit);
-                copy16<1536, 8 * kDim + 64>(dst, kr, key + g + 8u < limit);
-                copy16<2048, 0>(dst, vr, key + 2u * t < limit);
-                copy16<2560, kDim>(dst, vr, key + 2u * t + 1u < limit);
-                copy16<3072, 8 * kDim>(dst, vr, key + 2u * t + 8u < limit);
-                copy16<3584, 9 * kDim>(dst, vr, key + 2u * t + 9u < limit);
-            }
+        const uint32_t c = first + i * step;
+        if (c < chunks && lane == 0) {
+            const uint32_t row = row0 + keys.key0(c), dst = ring + slot * kSlot;
+            mbar_arrive_expect_tx(full + slot, kSlot);
+            load_rows(dst, &a.kmap, row, full + slot);
+            load_rows(dst + kSlot / 2u, &a.vmap, row, full + slot);
         }
-        copy_commit();
     };
 #pragma unroll
     for (uint32_t i = 0; i < kStages - 1; ++i) issue(i, i);
+    // K: matrices (rows 0-7, 8-15) x (chunks 2 st, 2 st + 1) of step st; V: rows 2 t, 2 t + 1 (and 8 on), chunk g
+    const uint32_t kx = (lane >> 4) ^ (lane & 7u), koff = (lane & 15u) * 128u;
+    const uint32_t voff0 = kSlot / 2u + 256u * t + ((g ^ (2u * t)) << 4), voff1 = kSlot / 2u + 256u * t + 128u + ((g ^ (2u * t + 1u)) << 4);
     float ksl, vsl;   // lane: the scales of the warp's chunk 32 (i / 32) + lane
     auto scales = [&](uint32_t i) {
-        const uint32_t b = keys.key0(min(first + ((i + lane) << slog), chunks - 1u)) >> a.c.block_log2;
+        const uint32_t b = keys.key0(min(first + (i + lane) * step, chunks - 1u)) >> a.c.block_log2;
         ksl = __ldcg(ksc + b);
         vsl = __ldcg(vsc + b);
     };
     scales(0u);
 
     // the query rows as int8 planes; powers of two keep max|q| and its reciprocal away from the ends of the range
+    if (warp < 8u)
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         const float v[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
@@ -417,9 +438,9 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
                 }
             }
         }
-        const uint32_t row = warp + kWarps * (uint32_t)i;
+        const uint32_t row = warp + 8u * (uint32_t)i;
 #pragma unroll
-        for (int p = 0; p < 3; ++p) sm.plane[p][row][lane] = w[p];
+        for (int p = 0; p < 3; ++p) sm.plane[p][row][8u * (lane & 3u) + (lane >> 2)] = w[p];
         // a row with a non-finite value: every score NaN
         if (lane == 0) sm.qs[row] = mx >= 0x7f800000u ? __int_as_float(0x7fffffff) : mx ? rcp(r) * (amax < 0x1p-60f ? 0x1p-64f : amax > 0x1p60f ? 0x1p64f : 1.0f) : 0.f;
     }
@@ -446,14 +467,24 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
-    uint32_t slot = 0u;
-    for (uint32_t i = 0; i < n; ++i) {
+    uint32_t slot = 0u, phase = 0u;
+    bool ok = true;
+    for (uint32_t i = 0, c = first; c < chunks; ++i, c += step) {
         if ((i & 31u) == 0u && i) scales(i);
-        issue(i + kStages - 1, slot ? slot - 1u : kStages - 1u);   // into the slot that chunk i - 1 left
-        copy_wait<kStages - 1>();
-        const uint32_t key = keys.key0(first + (i << slog));
-        const uint4 *in = reinterpret_cast<const uint4 *>(sm.u.ring[warp][slot]) + lane;
-        slot = slot + 1u == kStages ? 0u : slot + 1u;
+        __syncwarp();   // every lane is done with the slot that chunk i - 1 left
+        issue(i + kStages - 1, slot ? slot - 1u : kStages - 1u);
+        ok = __all_sync(0xffffffffu, mbar_wait(full + slot, phase, &sm.err));
+        if (!ok) {   // nothing of this warp is left in flight
+            for (uint32_t k = 0; k < kStages && c + k * step < chunks; ++k) {
+                const uint64_t w0 = global_ns();
+                while (!mbar_try_wait(full + slot, phase) && global_ns() - w0 < kWaitLimitNs) {
+                }
+                if (++slot == kStages) slot = 0u, phase ^= 1u;
+            }
+            break;
+        }
+        const uint32_t key = keys.key0(c), in = ring + slot * kSlot;
+        if (++slot == kStages) slot = 0u, phase ^= 1u;
         const float sk = __shfl_sync(0xffffffffu, ksl, i & 31u), sv = __shfl_sync(0xffffffffu, vsl, i & 31u);
         if (sv >= 2.0f * __uint_as_float(vref)) {   // not where sv is NaN
             const uint32_t now = __float_as_uint(sv) & 0x7f800000u;
@@ -473,22 +504,22 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
         const uint32_t pa = key + g, pb = key + g + 8u;
         const bool masked = key + kChunk - 1u > open;   // some row does not see all of the chunk
         {
-            const uint4 k0 = in[0], k1 = in[32], k2 = in[64], k3 = in[96];
-            const int ka[4][4] = {{(int)k0.x, (int)k2.x, (int)k0.y, (int)k2.y}, {(int)k0.z, (int)k2.z, (int)k0.w, (int)k2.w},
-                                  {(int)k1.x, (int)k3.x, (int)k1.y, (int)k3.y}, {(int)k1.z, (int)k3.z, (int)k1.w, (int)k3.w}};
+            int ka[4][4];
+#pragma unroll
+            for (uint32_t st = 0; st < 4; ++st) load_matrices(ka[st], in + koff + ((kx ^ (2u * st)) << 4));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 int d[3][4];
-                // B operands: column g, the dimensions of the lane's K pieces (16 t and 64 + 16 t on)
+                // B operands: column g, dimensions 32 st + 4 t on and 32 st + 16 + 4 t on
 #pragma unroll
                 for (int pl = 0; pl < 3; ++pl) {
-                    const uint4 lo = *reinterpret_cast<const uint4 *>(&sm.plane[pl][8 * nt + g][4u * t]);
+                    const uint4 lo = *reinterpret_cast<const uint4 *>(&sm.plane[pl][8 * nt + g][8u * t]);
                     mma_s8_first(d[pl], ka[0], lo.x, lo.y, kSumBits);
                     mma_s8(d[pl], ka[1], lo.z, lo.w);
                 }
 #pragma unroll
                 for (int pl = 0; pl < 3; ++pl) {
-                    const uint4 hi = *reinterpret_cast<const uint4 *>(&sm.plane[pl][8 * nt + g][16u + 4u * t]);
+                    const uint4 hi = *reinterpret_cast<const uint4 *>(&sm.plane[pl][8 * nt + g][8u * t + 4u]);
                     mma_s8(d[pl], ka[2], hi.x, hi.y);
                     mma_s8(d[pl], ka[3], hi.z, hi.w);
                 }
@@ -550,7 +581,8 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
         }
         // O^T += V^T P^T: rows g and g + 8 of MMA j are dimensions 16 g + 2 j and 16 g + 2 j + 1
         {
-            const uint4 v0 = in[128], v1 = in[160], v2 = in[192], v3 = in[224];
+            const uint4 v0 = ld_shared4(in + voff0), v1 = ld_shared4(in + voff1), v2 = ld_shared4(in + voff0 + 1024u),
+                        v3 = ld_shared4(in + voff1 + 1024u);
             const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
             const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
 #pragma unroll
@@ -565,7 +597,7 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
             }
         }
     }
-    copy_wait<0>();
+    if (!ok) l[0][0] = l[0][1] = l[NT - 1][0] = l[NT - 1][1] = __int_as_float(0x7fffffff);   // the output will be NaN
     __syncthreads();   // every warp is done with the ring: it takes the warps' outputs
 
     const float back = __uint_as_float(vref) * (1.0f / 64.0f);
@@ -587,21 +619,23 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
     if (C > 1u) cluster_wait();   // the other CTAs run: their shared memory may be written
     __syncthreads();
     // The warps' states -> the CTA's state of each row, straight to the CTA of
-    // the cluster that owns the row (row i: CTA i % C). A state that saw no
-    // position (maximum -inf, sum 0) counts nothing.
-    const uint32_t plog = 3u + (NT - 1u) > clog ? 3u + (NT - 1u) - clog : 0u;   // log2 of the rows that a CTA owns
-    {
-        constexpr uint32_t kPer = kThreads / R;   // threads per row, 4 dimensions at a time
-        const uint32_t i = threadIdx.x / kPer, part = threadIdx.x % kPer;
-        float2 ml[kWarps];
+    // the cluster that owns the row (row i: CTA i % C, which has `per` slots
+    // from each CTA). A state that saw no position (maximum -inf, sum 0) counts
+    // nothing.
+    const float cinv = rcp((float)C);
+    const uint32_t per = (uint32_t)(((float)(R + C) - 0.5f) * cinv);   // ceil(R / C)
+    if (threadIdx.x < 256u) {
+        constexpr uint32_t kPer = 256u / R;   // threads per row, 4 dimensions at a time
+        const uint32_t i = threadIdx.x / kPer, part = threadIdx.x % kPer, q = (uint32_t)(((float)i + 0.5f) * cinv);   // i / C
+        float2 ml[W];
         float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) {
+        for (uint32_t w = 0; w < W; ++w) {
             ml[w] = sm.wml[w][i];
             M = fmaxf(M, ml[w].x);
         }
 #pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) {
+        for (uint32_t w = 0; w < W; ++w) {
             ml[w].x = ml[w].x == -INFINITY && ml[w].y == 0.f ? 0.f : ex2(ml[w].x - M);
             L = fmaf(ml[w].x, ml[w].y, L);
         }
@@ -610,7 +644,7 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
         for (uint32_t d = part; d < kDim / 4u; d += kPer) {
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) {
+            for (uint32_t w = 0; w < W; ++w) {
                 const float4 y = *reinterpret_cast<const float4 *>(&sm.u.wrec[w][i][4u * d]);
                 x.x = fmaf(ml[w].x, y.x, x.x);
                 x.y = fmaf(ml[w].x, y.y, x.y);
@@ -619,17 +653,17 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
             }
             if (i >= rows) continue;
             if (C == 1u) store_row(a, tr, s, h, i, p0, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-            else st_cluster(&sm.rec[(rank << plog) + (i >> clog)][4u * d], i & (C - 1u), x);
+            else st_cluster(&sm.rec[rank * per + q][4u * d], i - q * C, x);
         }
         if (C > 1u && part == 0u && i < rows)
-            st_cluster(&sm.rec[(rank << plog) + (i >> clog)][kDim], i & (C - 1u), make_float4(M, L, 0.f, 0.f));
+            st_cluster(&sm.rec[rank * per + q][kDim], i - q * C, make_float4(M, L, 0.f, 0.f));
     }
     if (C == 1u) return;
     cluster_sync();   // every record has arrived; nothing remote is touched from here on
     // warp k: row rank + k C; lane: a CTA's maximum and sum, then 4 dimensions
-    const uint32_t i = rank + (warp << clog);
-    if (warp >= (1u << plog) || i >= min(rows, R)) return;
-    const float *rec = sm.rec[(lane << plog) + warp];
+    const uint32_t i = rank + warp * C;
+    if (warp >= per || i >= min(rows, R)) return;
+    const float *rec = sm.rec[lane * per + warp];
     const float mc = lane < C ? rec[kDim] : -INFINITY, lc = lane < C ? rec[kDim + 1] : 0.f;
     float M = mc;
 #pragma unroll
@@ -642,7 +676,7 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
     for (uint32_t c = 0; c < C; ++c) {
-        const float4 y = *reinterpret_cast<const float4 *>(&sm.rec[(c << plog) + warp][4u * lane]);
+        const float4 y = *reinterpret_cast<const float4 *>(&sm.rec[c * per + warp][4u * lane]);
         const float fc = __shfl_sync(0xffffffffu, f, (int)c);
         x.x = fmaf(fc, y.x, x.x);
         x.y = fmaf(fc, y.y, x.y);
@@ -653,18 +687,19 @@ __device__ __forceinline__ void attend(const AttnArgs &a, Smem<NT> &sm, const KE
     store_row(a, tr, s, h, i, p0, lane, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
-template <int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) attn_kernel(const __grid_constant__ AttnArgs a)
+template <int NT, uint32_t W>
+__global__ void __launch_bounds__(W * 32, 1) attn_kernel(const __grid_constant__ FewArgs a)
 {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(smem_raw);
-    const uint32_t s = blockIdx.z, h = blockIdx.y, r0 = (blockIdx.x >> (31 - __clz(cluster_size()))) * 8u * NT;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem<NT, W> &sm = *reinterpret_cast<Smem<NT, W> *>(smem_raw);
+    const uint32_t s = blockIdx.z, h = blockIdx.y, r0 = (a.tiles == 1u ? 0u : blockIdx.x / cluster_size()) * 8u * NT;
     if (cluster_size() > 1u) cluster_arrive();
     TileRows tr{0u, 0u, a.group, a.group_inv};
     if (r0) {
         tr.tok = r0 / a.group;
         tr.rem = r0 - tr.tok * a.group;
     }
+    init_ring(a, sm);
     wait_predecessor(a.early);
     const uint64_t p0 = __ldcg(a.r.pos0 + s);
     const uint32_t all = row_count(a.r, s) * a.group;
@@ -676,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) attn_kernel(const _
     }
     const uint32_t rows = min(all - r0, 8u * NT);
     const uint32_t limit = (uint32_t)min(p0 + tr.at(rows - 1u).x + 1u, (uint64_t)a.c.max_context);
-    attend<NT>(a, sm, Dense{}, q, tr, s, h, rows, p0, (limit + kChunk - 1u) / kChunk, limit);
+    attend<NT, W>(a, sm, Dense{}, q, tr, s, h, rows, p0, (limit + kChunk - 1u) / kChunk);
 }
 
 // ------------------------------------------------- attention, chosen blocks --
@@ -879,18 +914,19 @@ __device__ __forceinline__ void pick_blocks(PickSmem &ps, const unsigned long lo
 }
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const __grid_constant__ FewArgs a)
 {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(smem_raw);
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem<NT, kWarps> &sm = *reinterpret_cast<Smem<NT, kWarps> *>(smem_raw);
     PickSmem &ps = *reinterpret_cast<PickSmem *>(sm.u.ring);
     unsigned long long *key = reinterpret_cast<unsigned long long *>(&ps + 1);
-    uint32_t *list = reinterpret_cast<uint32_t *>(smem_raw + sizeof(Smem<NT>));
+    uint32_t *list = reinterpret_cast<uint32_t *>(smem_raw + sizeof(Smem<NT, kWarps>));
     const uint32_t C = cluster_size(), rank = cluster_rank();
-    const uint32_t s = blockIdx.z, h = blockIdx.y, unit = blockIdx.x >> (31 - __clz(C));
+    const uint32_t s = blockIdx.z, h = blockIdx.y, unit = C == 1u ? blockIdx.x : blockIdx.x / C;
     const uint32_t token = a.tiles == 1u ? unit : unit / a.tiles, tile = unit - token * a.tiles;
     const TileRows tr{token, tile * 8u * NT, a.group, a.group_inv};
     if (C > 1u) cluster_arrive();
+    init_ring(a, sm);
     wait_predecessor(a.early);
     const uint64_t p0 = __ldcg(a.r.pos0 + s);
     const uint32_t n = row_count(a.r, s);
@@ -920,6 +956,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const
         for (uint32_t i = threadIdx.x; i < want; i += kThreads) list[i] = i;
     }
     if (threadIdx.x == 0) list[want] = own;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's copies come after the keys' stores there
     __syncthreads();
     if (rank == 0 && tile == 0) {
         int32_t *sel = a.sel + (((size_t)s * a.r.tokens + token) * a.c.kv_heads + h) * a.n_sel;
@@ -927,19 +964,48 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const
     }
     const uint32_t per = a.c.block_log2 - 4u;
     const uint32_t chunks = (want << per) + ((p & ((1u << a.c.block_log2) - 1u)) / kChunk) + 1u;
-    attend<NT>(a, sm, Chosen{list, per, a.c.block_log2}, q, tr, s, h, min(a.group - tile * 8u * NT, 8u * NT), p0, chunks,
-               p + 1u);
+    attend<NT, kWarps>(a, sm, Chosen{list, per, a.c.block_log2}, q, tr, s, h, min(a.group - tile * 8u * NT, 8u * NT), p0, chunks);
 }
 
 // ------------------------------------------------------------- host side ----
 
-// CTAs per unit of work: as many as fill the device, at most 16 (the largest
-// cluster) and one per 64 positions (a chunk for each warp).
-uint32_t cluster_of(uint64_t units, uint64_t slots, uint64_t positions)
+// How many clusters of `c` CTAs of a kernel are on the device at once; asked once per device and size.
+template <auto KERNEL>
+uint32_t clusters_at_once(int dev, uint32_t c, uint32_t threads, size_t smem)
 {
-    uint32_t c = 1;
-    while (c < 16 && units * c * 2 <= slots && (uint64_t)c * 2 * kChunk * kWarps <= positions + kChunk * kWarps) c *= 2;
-    return c;
+    static std::atomic<uint32_t> known[64][kMaxCluster + 1];   // + 1; 0: not asked yet
+    uint32_t n = known[dev][c].load(std::memory_order_relaxed);
+    if (!n) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = c;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.gridDim = dim3(c);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        int most = 0;
+        if (cudaOccupancyMaxActiveClusters(&most, KERNEL, &cfg) != cudaSuccess) cudaGetLastError();
+        n = (uint32_t)std::max(most, 0) + 1;
+        known[dev][c].store(n, std::memory_order_relaxed);
+    }
+    return n - 1;
+}
+
+// CTAs per unit of work: the largest cluster of which all units are on the
+// device at once (a second wave costs more than the smaller share saves: 8
+// units of 8447 positions take 16.2 us as clusters of 16, of which 7 fit, and
+// 11.0 us as clusters of 8), with 128 positions per CTA at least. `any`: not
+// only powers of two.
+template <auto KERNEL>
+uint32_t cluster_of(int dev, uint32_t threads, size_t smem, uint64_t units, uint64_t positions, bool any)
+{
+    for (uint32_t c = kMaxCluster; c > 1; --c)
+        if ((any || !(c & (c - 1))) && (c - 1) * 128ull < positions && clusters_at_once<KERNEL>(dev, c, threads, smem) >= units)
+            return c;
+    return 1;
 }
 
 bool on_device(const void *p, int dev)
@@ -1007,6 +1073,35 @@ int check_rows(const char *who, const void *p, const void *q, uint32_t heads, ui
     return ATLAS_OK;
 }
 
+// The codes as tensors of 128-byte rows, for copies of 16 rows into swizzled shared memory
+int map_codes(const char *who, FewArgs &a)
+{
+    using Encode = decltype(&cuTensorMapEncodeTiled);
+    static std::atomic<Encode> known{nullptr};
+    Encode encode = known.load(std::memory_order_acquire);
+    if (!encode) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess || !p) {
+            cudaGetLastError();
+            return api_fail(ATLAS_ECUDA, "%s: the driver has no cuTensorMapEncodeTiled", who);
+        }
+        encode = reinterpret_cast<Encode>(p);
+        known.store(encode, std::memory_order_release);
+    }
+    const cuuint64_t rows = (cuuint64_t)a.c.nseq * a.c.kv_heads * a.c.max_context;
+    if (rows > 0x7fffffffull) return api_fail(ATLAS_EINVAL, "%s: more than 2^31 - 1 rows of codes", who);
+    const cuuint64_t dims[2] = {kDim, rows}, strides[1] = {kDim};
+    const cuuint32_t box[2] = {kDim, kChunk}, steps[2] = {1, 1};
+    for (int i = 0; i < 2; ++i)
+        if (encode(i ? &a.vmap : &a.kmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i ? a.c.v : a.c.k, dims, strides, box, steps,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return api_fail(ATLAS_ECUDA, "%s: the codes cannot be described to the copy engine", who);
+    return ATLAS_OK;
+}
+
 int done(const char *who, cudaError_t e)
 {
     if (e == cudaSuccess) return ATLAS_OK;
@@ -1014,25 +1109,27 @@ int done(const char *who, cudaError_t e)
     return api_fail(ATLAS_ECUDA, "%s: %s", who, cudaGetErrorString(e));
 }
 
-template <int NT>
-cudaError_t launch_attn(const AttnArgs &a, int dev, int sms, cudaStream_t stream)
+template <int NT, uint32_t W>
+cudaError_t launch_attn(const FewArgs &a, int dev, int sms, cudaStream_t stream)
 {
-    cudaError_t e = allow<attn_kernel<NT>>(dev, (int)kMaxSmem);
+    cudaError_t e = allow<attn_kernel<NT, W>>(dev, (int)kMaxSmem);
     if (e != cudaSuccess) return e;
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
-    const uint32_t C = cluster_of(units, (uint64_t)sms * (NT == 1 ? 2 : 1), a.c.max_context);
-    return launch(attn_kernel<NT>, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), kThreads, sizeof(Smem<NT>), C, a, sms, stream);
+    const uint32_t C = cluster_of<attn_kernel<NT, W>>(dev, W * 32, sizeof(Smem<NT, W>), units, a.c.max_context, NT == 1);
+    return launch(attn_kernel<NT, W>, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), W * 32, sizeof(Smem<NT, W>), C, a, sms, stream);
 }
 
 template <int NT>
-cudaError_t launch_sparse(const AttnArgs &a, int dev, int sms, cudaStream_t stream)
+cudaError_t launch_sparse(const FewArgs &a, int dev, int sms, cudaStream_t stream)
 {
     cudaError_t e = allow<sparse_kernel<NT>>(dev, (int)kMaxSmem);
     if (e != cudaSuccess) return e;
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.r.tokens * a.tiles;
-    const uint32_t C = cluster_of(units, (uint64_t)sms * (NT == 1 ? 2 : 1), (uint64_t)a.n_sel << a.c.block_log2);
+    const size_t smem = sizeof(Smem<NT, kWarps>) + (size_t)a.n_sel * 4u;
+    const uint32_t C = cluster_of<sparse_kernel<NT>>(dev, kThreads, sizeof(Smem<NT, kWarps>), units,
+                                                     std::max<uint64_t>((uint64_t)a.n_sel << a.c.block_log2, a.c.max_context / 8), NT == 1);
     return launch(sparse_kernel<NT>, dim3(C * a.r.tokens * a.tiles, a.c.kv_heads, a.c.nseq), kThreads,
-                  sizeof(Smem<NT>) + (size_t)a.n_sel * 4u, C, a, sms, stream);
+                  smem, C, a, sms, stream);
 }
 
 }  // namespace
@@ -1106,15 +1203,17 @@ extern "C" int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint
                                    void *stream)
 {
     const char *who = "kv8_attn";
-    AttnArgs a{};
+    FewArgs a{};
     int dev, sms;
-    const int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
+    int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
     if (rc != ATLAS_OK || !tokens) return rc;
     const uint32_t rows = tokens * a.group;
     if (rows > kFewRows) return done(who, launch_prompt(a, dev, sms, (cudaStream_t)stream));
+    if ((rc = map_codes(who, a)) != ATLAS_OK) return rc;
     const bool one = rows <= 8;
     a.tiles = one ? 1 : (rows + 15) / 16;
-    return done(who, one ? launch_attn<1>(a, dev, sms, (cudaStream_t)stream) : launch_attn<2>(a, dev, sms, (cudaStream_t)stream));
+    return done(who, one ? launch_attn<1, 16>(a, dev, sms, (cudaStream_t)stream)
+                         : launch_attn<2, 8>(a, dev, sms, (cudaStream_t)stream));
 }
 
 extern "C" int atlas_cuda_kv8_attn_sparse(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, uint32_t n_sel,
@@ -1122,9 +1221,9 @@ extern "C" int atlas_cuda_kv8_attn_sparse(const AtlasKv8 *cache, uint32_t q_head
                                           float *d_out, uint64_t ldo, int32_t *d_sel, void *stream)
 {
     const char *who = "kv8_attn_sparse";
-    AttnArgs a{};
+    FewArgs a{};
     int dev, sms;
-    const int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
+    int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
     if (rc != ATLAS_OK) return rc;
     if (!cache->k_sum) return api_fail(ATLAS_EINVAL, "%s: the cache has no k_sum", who);
     if (!d_sel || !aligned(d_sel, 4) || !on_device(d_sel, dev))
@@ -1137,6 +1236,7 @@ extern "C" int atlas_cuda_kv8_attn_sparse(const AtlasKv8 *cache, uint32_t q_head
     a.tiles = one ? 1 : (a.group + 15) / 16;
     if ((uint64_t)tokens * a.tiles > 0x7ffffffull) return api_fail(ATLAS_EINVAL, "%s: too many rows", who);
     if (!tokens) return ATLAS_OK;
+    if ((rc = map_codes(who, a)) != ATLAS_OK) return rc;
     a.n_sel = n_sel;
     a.sel = d_sel;
     return done(who, one ? launch_sparse<1>(a, dev, sms, (cudaStream_t)stream)
