@@ -725,8 +725,8 @@ __global__ void __launch_bounds__(W * 32, 1) attn_kernel(const __grid_constant__
 // the order of any sum; equal scores go to the lower block. A NaN score stands
 // above every number: a poisoned block is chosen and shows in the output.
 // The CTAs of the cluster score every C-th block each, send the keys to all of
-// them, and each picks the blocks on its own (a radix search from the highest
-// bit in which the keys differ), so the whole operator is one launch.
+// them, and each picks the blocks on its own (a search for the lowest chosen
+// key, three bits at a time), so the whole operator is one launch.
 // Bound by latency: 260 bytes per candidate block, then n_sel blocks.
 
 struct Chosen {
@@ -739,33 +739,40 @@ struct Chosen {
 };
 
 struct PickSmem {
-    int8_t code[kDim];
-    unsigned long long red[2][kWarps];
-    uint32_t hist[256];
-    uint32_t digit, need, exact, scan[kWarps];
+    alignas(16) int8_t code[kDim];
+    unsigned long long most[4], least;
+    alignas(16) uint4 count[2][kWarps];
+    uint32_t scan[kWarps];
 };
 
 // The keys lie behind PickSmem in the ring, which the attention fills later.
 constexpr uint32_t kMaxBlocks = (uint32_t)((kWarps * kStages * kSlot - sizeof(PickSmem)) / 8u);
 
-// The group's pooled query of one token as int8 codes. All threads; threads 0 .. 127 = dimensions.
-__device__ __forceinline__ void pool_query(const AttnArgs &a, PickSmem &ps, const float *q)
+// The sum of the group's query rows; thread = dimension (128 of them)
+__device__ __forceinline__ double pool_query(const AttnArgs &a, const float *q)
 {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     double x = 0.0;
     if (threadIdx.x < kDim)
 #pragma unroll 8
         for (uint32_t i = 0; i < a.group; ++i) x += (double)__ldcg(q + (size_t)i * kDim + threadIdx.x);
+    return x;
+}
+
+// The pooled query as int8 codes. All threads.
+__device__ __forceinline__ void code_query(PickSmem &ps, double x)
+{
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     unsigned long long b = (unsigned long long)__double_as_longlong(fabs(x));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-    if (lane == 0) ps.red[0][warp] = b;
+    if (lane == 0 && warp < 4u) ps.most[warp] = b;
     __syncthreads();
+    if (warp < 4u) {
 #pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) b = max(b, ps.red[0][w]);
-    const double most = __longlong_as_double((long long)b);
-    if (threadIdx.x < kDim)
+        for (uint32_t w = 0; w < 4u; ++w) b = max(b, ps.most[w]);
+        const double most = __longlong_as_double((long long)b);
         ps.code[threadIdx.x] = most > 0.0 && most < INFINITY ? (int8_t)(int)rint(127.0 * x / most) : (int8_t)0;
+    }
     __syncthreads();
 }
 
@@ -813,85 +820,97 @@ __device__ __forceinline__ void score_blocks(const AttnArgs &a, const PickSmem &
     }
 }
 
+// The largest value that at least `want` of key[0, nb) reach, 0 < want < nb, or
+// one that exactly `want` of them do. One warp, nb <= 512: bit by bit with the
+// keys' upper words in registers (a step is 16 comparisons a lane and one sum
+// over the warp), mostly 20 steps; the lower words count only where the upper
+// ones do not part the keys.
+constexpr uint32_t kWarpPick = 512;
+__device__ __forceinline__ unsigned long long search_warp(const unsigned long long *key, uint32_t nb, uint32_t want)
+{
+    constexpr uint32_t kPer = kWarpPick / 32u;
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t k[kPer], least = 0u, n = nb;
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j) k[j] = 32u * j + lane < nb ? (uint32_t)(key[32u * j + lane] >> 32) : 0u;
+    for (uint32_t bit = 1u << 31; bit && n != want; bit >>= 1) {
+        const uint32_t at = least | bit;
+        uint32_t c = 0u;
+#pragma unroll
+        for (uint32_t j = 0; j < kPer; ++j) c += k[j] >= at ? 1u : 0u;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= want) least = at, n = c;
+    }
+    unsigned long long all = (unsigned long long)least << 32;
+    for (uint32_t bit = 1u << 31; bit && n != want; bit >>= 1) {
+        uint32_t c = 0u;
+        for (uint32_t i = lane; i < nb; i += 32u) c += key[i] >= (all | bit) ? 1u : 0u;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= want) all |= bit, n = c;
+    }
+    return all;
+}
+
+// The same by all threads, for more blocks: three bits at a time, the keys at or
+// above each of their values 1 .. 7 counted in one pass, two counts of 16 bits a word
+__device__ __forceinline__ unsigned long long search_all(PickSmem &ps, const unsigned long long *key, uint32_t nb, uint32_t want)
+{
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    unsigned long long least = 0ull;
+    for (int bit = 61, turn = 0;; bit = max(bit - 3, 0), turn ^= 1) {   // the last step sees two bits again
+        uint32_t c[4] = {0u, 0u, 0u, 0u};
+        for (uint32_t i = threadIdx.x; i < nb; i += kThreads) {
+            const unsigned long long k = key[i];
+#pragma unroll
+            for (uint32_t v = 1; v < 8u; ++v)
+                if (k >= (least | (unsigned long long)v << bit)) c[v >> 1] += 1u << (16u * (v & 1u));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = __reduce_add_sync(0xffffffffu, c[j]);
+        if (lane == 0) ps.count[turn][warp] = make_uint4(c[0], c[1], c[2], c[3]);
+        __syncthreads();
+        uint4 all = ps.count[turn][0];
+#pragma unroll
+        for (uint32_t w = 1; w < kWarps; ++w) {
+            const uint4 n = ps.count[turn][w];
+            all.x += n.x;
+            all.y += n.y;
+            all.z += n.z;
+            all.w += n.w;
+        }
+        // the largest value that `want` keys reach
+        const uint32_t n[8] = {nb, all.x >> 16, all.y & 0xffffu, all.y >> 16, all.z & 0xffffu, all.z >> 16, all.w & 0xffffu,
+                               all.w >> 16};
+        uint32_t v = 0u, at = nb;
+#pragma unroll
+        for (uint32_t j = 1; j < 8u; ++j)
+            if (n[j] >= want) v = j, at = n[j];
+        least |= (unsigned long long)v << bit;
+        if (bit == 0 || (v && at == want)) return least;
+    }
+}
+
 // The `want` largest of key[0, nb), 0 < want < nb, as ascending block numbers
 // in list[0, want); equal keys go to the lower number. All threads.
 __device__ __forceinline__ void pick_blocks(PickSmem &ps, const unsigned long long *key, uint32_t nb, uint32_t want,
                                             uint32_t *list)
 {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    unsigned long long all = ~0ull, any = 0ull;
-    for (uint32_t i = threadIdx.x; i < nb; i += kThreads) {
-        all &= key[i];
-        any |= key[i];
-    }
-    all = (unsigned long long)__reduce_and_sync(0xffffffffu, (uint32_t)(all >> 32)) << 32 |
-          __reduce_and_sync(0xffffffffu, (uint32_t)all);
-    any = (unsigned long long)__reduce_or_sync(0xffffffffu, (uint32_t)(any >> 32)) << 32 |
-          __reduce_or_sync(0xffffffffu, (uint32_t)any);
-    if (lane == 0) {
-        ps.red[0][warp] = all;
-        ps.red[1][warp] = any;
-    }
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) {
-        all &= ps.red[0][w];
-        any |= ps.red[1][w];
-    }
-    // Invariant: keys with (key >> shift) > prefix are chosen, and `need` of those with (key >> shift) == prefix
-    const int top = 64 - __clzll((long long)(all ^ any));   // bits above it are common to all keys
-    int shift = top;
-    unsigned long long prefix = top < 64 ? all >> top : 0ull;
-    uint32_t need = want;
-    bool exact = false;   // every key with that prefix is chosen
-    while (shift > 0 && !exact) {
-        const int width = min(8, shift), next = shift - width;
-        for (uint32_t i = threadIdx.x; i < 256u; i += kThreads) ps.hist[i] = 0u;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < nb; i += kThreads) {
-            const unsigned long long k = key[i];
-            if (shift >= 64 || (k >> shift) == prefix) atomicAdd(&ps.hist[(uint32_t)(k >> next) & ((1u << width) - 1u)], 1u);
+    unsigned long long least;
+    if (nb <= kWarpPick) {
+        if (warp == 0) {
+            least = search_warp(key, nb, want);
+            if (lane == 0) ps.least = least;
         }
         __syncthreads();
-        if (warp == 0) {   // lane: digits 255 - 8 lane down to 248 - 8 lane
-            uint32_t c[8], sum = 0u;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                c[j] = ps.hist[255u - 8u * lane - (uint32_t)j];
-                sum += c[j];
-            }
-            uint32_t inc = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= (uint32_t)o) inc += up;
-            }
-            uint32_t above = inc - sum;
-            if (above < need && inc >= need) {   // one lane: the digit at which the count passes `need`
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (above < need && above + c[j] >= need) {
-                        ps.digit = 255u - 8u * lane - (uint32_t)j;
-                        ps.need = need - above;
-                        ps.exact = c[j] == need - above;
-                    }
-                    above += c[j];
-                }
-            }
-        }
-        __syncthreads();
-        prefix = prefix << width | ps.digit;
-        need = ps.need;
-        exact = ps.exact != 0u;
-        shift = next;
+        least = ps.least;
+    } else {
+        least = search_all(ps, key, nb, want);
     }
-    // thread: a run of consecutive blocks; (chosen above, equal) counts of the runs before it in one word
+    // thread: a run of consecutive blocks; (above, equal) counts of the runs before it in one word
     const uint32_t per = (nb + kThreads - 1u) / kThreads, b0 = min(threadIdx.x * per, nb), b1 = min(b0 + per, nb);
     uint32_t cnt = 0u;
-    for (uint32_t b = b0; b < b1; ++b) {
-        const unsigned long long k = shift < 64 ? key[b] >> shift : 0ull;
-        cnt += k > prefix ? 1u : k == prefix ? 1u << 16 : 0u;
-    }
+    for (uint32_t b = b0; b < b1; ++b) cnt += key[b] > least ? 1u : key[b] == least ? 1u << 16 : 0u;
     uint32_t inc = cnt;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -900,15 +919,19 @@ __device__ __forceinline__ void pick_blocks(PickSmem &ps, const unsigned long lo
     }
     if (lane == 31u) ps.scan[warp] = inc;
     __syncthreads();
-    uint32_t before = inc - cnt;
-    for (uint32_t w = 0; w < warp; ++w) before += ps.scan[w];
+    uint32_t before = inc - cnt, all = 0u;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) {
+        if (w < warp) before += ps.scan[w];
+        all += ps.scan[w];
+    }
     uint32_t gt = before & 0xffffu, eq = before >> 16;
+    const uint32_t need = want - (all & 0xffffu);   // of the equal ones, the first
     for (uint32_t b = b0; b < b1; ++b) {
-        const unsigned long long k = shift < 64 ? key[b] >> shift : 0ull;
-        const bool take = k > prefix || (k == prefix && eq < need);
-        if (take) list[gt + min(eq, need)] = b;
-        gt += k > prefix ? 1u : 0u;
-        eq += k == prefix ? 1u : 0u;
+        const unsigned long long k = key[b];
+        if (k > least || (k == least && eq < need)) list[gt + min(eq, need)] = b;
+        gt += k > least ? 1u : 0u;
+        eq += k == least ? 1u : 0u;
     }
     __syncthreads();
 }
@@ -930,6 +953,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const
     wait_predecessor(a.early);
     const uint64_t p0 = __ldcg(a.r.pos0 + s);
     const uint32_t n = row_count(a.r, s);
+    const double pooled = pool_query(a, a.q + ((size_t)s * a.r.tokens + token) * a.ldq + (size_t)h * a.group * kDim);
     float4 q[NT];
     load_queries<NT>(a, tr, s, h, q);
     if (token >= n) {   // the whole cluster leaves
@@ -941,7 +965,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const
     const uint32_t own = p >> a.c.block_log2, want = min(own, a.n_sel - 1u);
     const size_t head = (size_t)s * a.c.kv_heads + h;
     if (own > want && want) {
-        pool_query(a, ps, a.q + ((size_t)s * a.r.tokens + token) * a.ldq + (size_t)h * a.group * kDim);
+        code_query(ps, pooled);
         // the other CTAs' shared memory is written from here on: they have to run
         if (C > 1u) cluster_wait();
         score_blocks(a, ps, head, own, key, C, rank);
