@@ -36,17 +36,27 @@ struct AppendArgs {
     uint32_t early;
 };
 
-// Nearest integer to x / s (ties to even), exactly, for |x| <= 127.5 s: the
-// product with the rounded reciprocal is off by at most 127 * 2^-23 < 2^-15,
-// so it decides everything but quotients within 2^-13 of a tie, which are
-// divided in 64 bits (two 24-bit values whose quotient is no tie differ from
-// it by 2^-25 or more). `slow`: s too small for the reciprocal.
-__device__ __forceinline__ int quantise(float x, float s, float inv, bool slow)
+// Nearest integers to x / s (ties to even), exactly, for |x| <= 127.5 s, as the
+// low bytes of the results. x * inv + 2^23 + 2^22, rounded once, has the integer
+// nearest to x * inv in its low bits; the rounded reciprocal inv = 1 / s puts
+// x * inv off by at most 127 * 2^-24 < 2^-17, so that decides everything but
+// quotients within 2^-13 of a tie. If one of the four is, they are divided in 64
+// bits (two 24-bit values whose quotient is no tie differ from it by 2^-25 or
+// more). `slow`: s too small for the reciprocal.
+__device__ __forceinline__ void quantise(const float4 &x, float s, float inv, bool slow, uint32_t (&q)[4])
 {
-    const float t = x * inv;
-    float r = rintf(t);
-    if (slow || fabsf(t - r) > 0.5f - 1.220703125e-4f) r = (float)rint((double)x / (double)s);
-    return (int)fminf(fmaxf(r, -127.f), 127.f);
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    constexpr float kInt = 12582912.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float u = fmaf(v[j], inv, kInt);
+        slow |= fabsf(fmaf(v[j], inv, kInt - u)) > 0.5f - 1.220703125e-4f;
+        q[j] = __float_as_uint(u);
+    }
+    if (slow)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            q[j] = (uint32_t)(int)fmin(fmax(rint((double)v[j] / (double)s), -127.0), 127.0) + 0x4B400000u;
 }
 
 // One CTA per (touched block, K or V of a KV head, sequence). Warp w holds
@@ -61,7 +71,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 {
     constexpr int kRows = B / 8;
     __shared__ uint32_t s_max[8];
-    __shared__ int32_t s_sum[8][kDim];
+    __shared__ alignas(16) uint32_t s_sum[8][kDim];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     wait_predecessor(a.early);
     const uint32_t s = blockIdx.z, h = blockIdx.y >> 1, is_v = blockIdx.y & 1u;
@@ -104,38 +114,36 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     const float inv = 1.0f / now;
     const bool slow = now < 7.8886090522101181e-31f, grew = !bad && now > was;
     if (threadIdx.x == 0) *sp = now;
-    int sum[4] = {0, 0, 0, 0};
+    uint32_t sum[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const uint32_t r = warp + 8u * (uint32_t)i;
         if (r >= hi) continue;
-        int q[4];
+        uint32_t q[4];   // 0x4B400000 + code
         if (r < lo) {
             const int w = __float_as_int(x[i].x);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                q[j] = (int)(int8_t)(w >> (8 * j));
-                if (grew) q[j] = (int)rint((double)q[j] * (double)was / (double)now);
+                int c = (int)(int8_t)(w >> (8 * j));
+                if (grew) c = (int)rint((double)c * (double)was / (double)now);
+                q[j] = (uint32_t)c + 0x4B400000u;
             }
         } else if (bad || now == 0.f) {
-            q[0] = q[1] = q[2] = q[3] = 0;
+            q[0] = q[1] = q[2] = q[3] = 0x4B400000u;
         } else {
-            q[0] = quantise(x[i].x, now, inv, slow);
-            q[1] = quantise(x[i].y, now, inv, slow);
-            q[2] = quantise(x[i].z, now, inv, slow);
-            q[3] = quantise(x[i].w, now, inv, slow);
+            quantise(x[i], now, inv, slow, q);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += q[j];
+        for (int j = 0; j < 4; ++j) sum[j] += q[j] - 0x4B400000u;
         if (r >= lo || grew)
             reinterpret_cast<uint32_t *>(code + (size_t)r * kDim)[lane] =
-                (uint32_t)(q[0] & 255) | (uint32_t)(q[1] & 255) << 8 | (uint32_t)(q[2] & 255) << 16 | (uint32_t)q[3] << 24;
+                __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
     }
     if (is_v || !a.c.k_sum) return;
-    *reinterpret_cast<int4 *>(&s_sum[warp][4 * lane]) = make_int4(sum[0], sum[1], sum[2], sum[3]);
+    *reinterpret_cast<uint4 *>(&s_sum[warp][4 * lane]) = make_uint4(sum[0], sum[1], sum[2], sum[3]);
     __syncthreads();
     if (threadIdx.x < kDim) {
-        int t = 0;
+        uint32_t t = 0;
 #pragma unroll
         for (int w = 0; w < 8; ++w) t += s_sum[w][threadIdx.x];
         a.c.k_sum[(head * a.c.n_blocks + blk) * kDim + threadIdx.x] = (int16_t)t;
