@@ -46,12 +46,13 @@ namespace k8 {
 namespace {
 
 constexpr uint32_t kTileRows = 128, kTileKeys = 128;
+constexpr uint32_t kMaxSplit = 8;                  // CTAs that share the positions of a tile's rows
 constexpr uint32_t kConvWarp = 16, kMmaWarp = 20, kPromptThreads = 21 * 32;   // first converter, the MMA warp
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 binary16, swizzled
 constexpr uint32_t kQTile = 4 * kHalf;             // one tile's Q: [hi, lo][2 x 64 dimensions]
 
 struct PromptBars {
-    uint64_t s_full[2], p_full[2], o_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], fin;   // [tile], [half]
+    uint64_t s_full[2], p_full[2], o_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full, fin;   // [tile], [half]
     uint32_t tmem, status;
     // what a score of the row is worth, in the exponent's base 2 (in [tile][0], until the first exchange);
     // then the two threads of a row exchange their maxima and sums here
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t C = cluster_size(), rank = cluster_rank(), s = blockIdx.z, h = blockIdx.y;
     // the last rows first: they see the most positions
-    const uint32_t r0 = (a.tiles - 1u - blockIdx.x / C) * 2u * kTileRows;
+    const uint32_t r0 = (a.tiles - 1u - blockIdx.x / C) * a.cta_tiles * kTileRows;
     TileRows tr{r0 / a.group, 0u, a.group, a.group_inv};
     tr.rem = r0 - tr.tok * a.group;
     if (threadIdx.x == 0) {
@@ -312,72 +313,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             mbar_init(&b.k_empty[t], 1u);
             mbar_init(&b.v_empty[t], 1u);
         }
+        mbar_init(&b.q_full, kConvWarp);
         mbar_init(&b.fin, 1u);
         b.status = kStatusOk;
         fence_mbar_init();
     }
-    wait_predecessor(a.early);
-    const uint64_t p0 = __ldcg(a.r.pos0 + s);
-    const uint32_t all = row_count(a.r, s) * a.group;
-    if (r0 >= all) return;   // the whole cluster leaves
-    const uint32_t rows = min(all - r0, 2u * kTileRows), tiles = rows > kTileRows ? 2u : 1u;
-    const uint32_t limit = (uint32_t)min(p0 + tr.at(rows - 1u).x + 1u, (uint64_t)a.c.max_context);
-    const uint32_t total = (limit + kTileKeys - 1u) / kTileKeys;
-    const uint32_t j0 = (uint32_t)((uint64_t)total * rank / C), n = (uint32_t)((uint64_t)total * (rank + 1u) / C) - j0;
-    const size_t head = (size_t)s * a.c.kv_heads + h;
-
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&b.tmem)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    } else {
-        // Q: four rows at a time per warp, lane = 4 dimensions; a power of two
-        // brings each row's largest value to [2^8, 2^9)
-#pragma unroll 1
-        for (uint32_t i0 = 4u * warp; i0 < tiles * kTileRows; i0 += 4u * kMmaWarp) {
-            float4 x[4];
-#pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) {
-                const uint2 r = tr.at(i0 + u);
-                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (i0 + u < rows)
-                    x[u] = __ldcg(reinterpret_cast<const float4 *>(a.q + ((size_t)s * a.r.tokens + r.x) * a.ldq +
-                                                                  (size_t)(h * a.group + r.y) * kDim) + lane);
-            }
-#pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) {
-                const uint32_t i = i0 + u, row = i & (kTileRows - 1u);
-                float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-                uint32_t mx = 0u;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx = max(mx, __float_as_uint(v[e]) & 0x7fffffffu);
-                mx = __reduce_max_sync(0xffffffffu, mx);
-                const bool bad = mx >= 0x7f800000u;   // a non-finite value: every score of the row NaN
-                // v * 2^(8 - e) as two factors, so that neither leaves the range
-                const int e = bad ? 0 : max((int)(mx >> 23) - 127, -126), half = (8 - e) / 2;
-                const float f0 = __int_as_float((127 + half) << 23), f1 = __int_as_float((127 + 8 - e - half) << 23);
-                const float g0 = __int_as_float((127 - half) << 23), g1 = __int_as_float((127 - 8 + e + half) << 23);
-                float hi[4], lo[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[k] = bad ? 0.f : v[k] * f0 * f1;
-                    hi[k] = __uint_as_float(__float_as_uint(v[k]) & 0xffffe000u);
-                    lo[k] = v[k] - hi[k];
-                }
-                if (lane == 0)
-                    b.half[i / kTileRows][0][row] = bad ? __int_as_float(0x7fffffff) : kScoreScale * g0 * g1;
-                uint8_t *q = qs + (i / kTileRows) * kQTile + (lane >> 4) * kHalf + swizzled(row, (lane & 15u) >> 1) + (lane & 1u) * 8u;
-                *reinterpret_cast<uint2 *>(q) = make_uint2(h2_bits(hi[0], hi[1]), h2_bits(hi[2], hi[3]));
-                *reinterpret_cast<uint2 *>(q + 2 * kHalf) = make_uint2(h2_bits(lo[0], lo[1]), h2_bits(lo[2], lo[3]));
-            }
-        }
-        fence_async();
     }
     fence_before();
     __syncthreads();
     fence_after();
-    float row_m = -INFINITY, row_l = 0.f;   // softmax threads of half 0: their row's state, for the cluster
     const uint32_t tmem = b.tmem;   // scores / weights of tile t: column 128 t; output: 256 + 128 t
+    wait_predecessor(a.early);
+    const uint64_t p0 = __ldcg(a.r.pos0 + s);
+    const uint32_t all = row_count(a.r, s) * a.group;
+    if (r0 >= all) {   // the whole cluster leaves
+        if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        return;
+    }
+    const uint32_t rows = min(all - r0, a.cta_tiles * kTileRows), tiles = rows > kTileRows ? 2u : 1u;
+    const uint32_t limit = (uint32_t)min(p0 + tr.at(rows - 1u).x + 1u, (uint64_t)a.c.max_context);
+    const uint32_t total = (limit + kTileKeys - 1u) / kTileKeys;
+    uint32_t j0 = 0u, n = total;   // this CTA's tiles of keys
+    if (C > 1u) {
+        const uint32_t base = total / C, more = total - base * C;
+        j0 = rank * base + min(rank, more);
+        n = base + (rank < more ? 1u : 0u);
+    }
+    const size_t head = (size_t)s * a.c.kv_heads + h;
+
+    float row_m = -INFINITY, row_l = 0.f;   // softmax threads of half 0: their row's state, for the cluster
 
     if (warp == kMmaWarp) {
         // ------------------------------------------------------------- MMA --
@@ -386,7 +354,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             const uint64_t qd = operand(smem_addr(qs)), kd = operand(smem_addr(ks)), vd = operand(smem_addr(vs));
             // K and V go by halves (64 dimensions, 64 keys): a half is converted
             // while the MMAs still read, or already read, the other.
-            bool ok = n != 0u;
+            bool ok = n != 0u && mbar_wait(&b.q_full, 0u, err);
             auto scores = [&](uint32_t t, uint32_t j) {   // of keys j: the first tile waits for K, the last one releases it
                 const uint64_t q = qd + (uint64_t)(t * (kQTile >> 4));
 #pragma unroll
@@ -528,6 +496,53 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         copy_wait0();
     } else {
         // --------------------------------------------------------- softmax --
+        // First Q: a warp takes eight rows at a time, four per step (eight lanes a
+        // row, rows 0 4 1 5 and 2 6 3 7: so two rows' swizzled chunks do not meet
+        // in a bank). A power of two brings each row's largest value to [2^8, 2^9).
+#pragma unroll 1
+        for (uint32_t i0 = 8u * warp; i0 < tiles * kTileRows; i0 += 8u * kConvWarp) {
+            const uint32_t l8 = lane & 7u, first = i0 + 4u * ((lane >> 3) & 1u) + (lane >> 4);
+            float4 x[2][4];
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u) {
+                const uint2 r = tr.at(first + 2u * u);
+                const float4 *src = reinterpret_cast<const float4 *>(a.q + ((size_t)s * a.r.tokens + r.x) * a.ldq + (size_t)(h * a.group + r.y) * kDim) + l8;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) x[u][k] = first + 2u * u < rows ? __ldcg(src + 8u * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u) {
+                const uint32_t i = first + 2u * u, row = i & (kTileRows - 1u);
+                uint32_t mx = 0u;   // absolute values order as their bits do, NaN above infinity
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mx = max(max(max(mx, __float_as_uint(x[u][k].x) & 0x7fffffffu), __float_as_uint(x[u][k].y) & 0x7fffffffu),
+                             max(__float_as_uint(x[u][k].z) & 0x7fffffffu, __float_as_uint(x[u][k].w) & 0x7fffffffu));
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const bool bad = mx >= 0x7f800000u;   // a non-finite value: every score of the row NaN
+                const int e = max((int)(mx >> 23) - 127, -118);
+                const float f = bad ? 0.f : __int_as_float((135 - e) << 23);
+                if (l8 == 0u) b.half[i / kTileRows][0][row] = bad ? __int_as_float(0x7fffffff) : kScoreScale * __int_as_float((119 + e) << 23);
+                uint8_t *q = qs + (i / kTileRows) * kQTile + (l8 & 1u) * 8u;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const float v[4] = {x[u][k].x * f, x[u][k].y * f, x[u][k].z * f, x[u][k].w * f};
+                    float hi[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) hi[c] = bad ? 0.f : __uint_as_float(__float_as_uint(v[c]) & 0xffffe000u);
+                    uint8_t *dst = q + (k >> 1) * kHalf + swizzled(row, (l8 >> 1) + 4u * (k & 1u));
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(h2_bits(hi[0], hi[1]), h2_bits(hi[2], hi[3]));
+                    *reinterpret_cast<uint2 *>(dst + 2 * kHalf) =
+                        bad ? make_uint2(0u, 0u) : make_uint2(h2_bits(v[0] - hi[0], v[1] - hi[1]), h2_bits(v[2] - hi[2], v[3] - hi[3]));
+                }
+            }
+        }
+        fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b.q_full);
+        meet(3u, 32u * kConvWarp);   // the rows' factors are there
+
         // Warps w and w + 4 of a tile share 32 rows. A warp whose wait ran out
         // goes on through the barriers, without touching tensor memory.
         const uint32_t t = warp >> 3, half = (warp >> 2) & 1u, quarter = warp & 3u, row = quarter * 32u + lane;
@@ -633,14 +648,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             meet(1u + t, 256u);
             if (C == 1u) {
                 // warp w of the tile: rows 16 w .. 16 w + 15
-                const uint32_t w0 = (warp & 7u) * 16u;
-                for (uint32_t k = w0; k < w0 + 16u && t * kTileRows + k < rows; ++k) {
+                const uint32_t w0 = (warp & 7u) * 16u, end = rows - t * kTileRows;
+                const bool failed = *err != kStatusOk;
+#pragma unroll 4
+                for (uint32_t k = w0; k < w0 + 16u; ++k) {
                     const uint2 r = tr.at(t * kTileRows + k);
                     float4 x = stage[k * 32u + (lane ^ (k & 31u))];
-                    if (*err != kStatusOk || p0 + r.x >= a.c.max_context)
-                        x.x = x.y = x.z = x.w = __int_as_float(0x7fffffff);
-                    reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo +
-                                               (size_t)(h * a.group + r.y) * kDim)[lane] = x;
+                    if (failed || p0 + r.x >= a.c.max_context) x.x = x.y = x.z = x.w = __int_as_float(0x7fffffff);
+                    if (k < end)
+                        reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo +
+                                                   (size_t)(h * a.group + r.y) * kDim)[lane] = x;
                 }
             } else if (half == 0u) {
                 row_m = m;
@@ -660,39 +677,64 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         rs.max[warp >> 3][(warp & 3u) * 32u + lane] = row_m;
         rs.sum[warp >> 3][(warp & 3u) * 32u + lane] = row_l;
     }
-    // Rows rank, rank + C, ... of the cluster's states: a warp per row, lane = 4
-    // dimensions. A state that saw no position counts nothing.
+    // Rows rank, rank + C, ... of the cluster's states, four at a time per warp:
+    // lane = (row, CTA) for the maxima and sums, then 4 dimensions. A state that
+    // saw no position counts nothing.
+    static_assert(kMaxSplit == 8, "eight lanes per row");
     cluster_sync();
-    if (warp < kMmaWarp) {
-        for (uint32_t i = rank + C * warp; i < rows; i += C * kMmaWarp) {
-            const uint32_t t = i / kTileRows, row = i & (kTileRows - 1u);
-            const float mc = lane < C ? ld_cluster1(&rs.max[t][row], lane) : -INFINITY;
-            const float lc = lane < C ? ld_cluster1(&rs.sum[t][row], lane) : 0.f;
-            const bool bad = lane < C && __float_as_uint(ld_cluster1(&b.status, lane)) != kStatusOk;
-            float M = mc;
+    for (uint32_t k0 = 4u * warp; rank + C * k0 < rows; k0 += 4u * (kPromptThreads / 32u)) {
+        // two CTAs' outputs are on their way meanwhile
+        float4 y[2][4];
+        auto load = [&](float4(&to)[4], uint32_t c) {
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o, 16));
-            const float f = mc == -INFINITY && lc == 0.f ? 0.f : ex2(mc - M);
-            float L = f * lc;
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o, 16);
-            L = __shfl_sync(0xffffffffu, L, 0);
-            const bool any_bad = __any_sync(0xffffffffu, bad);
-            const float4 *stage = reinterpret_cast<const float4 *>(qs + t * kQTile);
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (uint32_t c = 0; c < C; ++c) {
-                const float4 y = ld_cluster4(&stage[row * 32u + (lane ^ (row & 31u))], c);
-                const float fc = __shfl_sync(0xffffffffu, f, (int)c);
-                x.x = fmaf(fc, y.x, x.x);
-                x.y = fmaf(fc, y.y, x.y);
-                x.z = fmaf(fc, y.z, x.z);
-                x.w = fmaf(fc, y.w, x.w);
+            for (uint32_t v = 0; v < 4; ++v) {
+                const uint32_t r = min(rank + C * (k0 + v), rows - 1u), row = r & (kTileRows - 1u);
+                to[v] = ld_cluster4(reinterpret_cast<const float4 *>(qs + (r / kTileRows) * kQTile) + row * 32u + (lane ^ (row & 31u)), c);
             }
-            const uint2 r = tr.at(i);
-            const float inv = any_bad || p0 + r.x >= a.c.max_context ? __int_as_float(0x7fffffff) : 1.0f / L;
-            reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo + (size_t)(h * a.group + r.y) * kDim)[lane] =
-                make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        };
+        auto add = [&](float4(&x)[4], const float4(&from)[4], float f, uint32_t c) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float fc = __shfl_sync(0xffffffffu, f, 8 * v + (int)c);
+                x[v].x = fmaf(fc, from[v].x, x[v].x);
+                x[v].y = fmaf(fc, from[v].y, x[v].y);
+                x[v].z = fmaf(fc, from[v].z, x[v].z);
+                x[v].w = fmaf(fc, from[v].w, x[v].w);
+            }
+        };
+        load(y[0], 0u);
+        load(y[1], 1u);
+        const uint32_t u = lane >> 3, cta = lane & 7u, i = rank + C * (k0 + u);
+        const bool there = cta < C && i < rows;
+        const float mc = there ? ld_cluster1(&rs.max[i / kTileRows][i & (kTileRows - 1u)], cta) : -INFINITY;
+        const float lc = there ? ld_cluster1(&rs.sum[i / kTileRows][i & (kTileRows - 1u)], cta) : 0.f;
+        const bool bad = there && __float_as_uint(ld_cluster1(&b.status, cta)) != kStatusOk;
+        float M = mc;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float f = mc == -INFINITY && lc == 0.f ? 0.f : ex2(mc - M);
+        float L = f * lc;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        const bool any_bad = __any_sync(0xffffffffu, bad);
+        float4 x[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t c = 0; c < C; c += 2u) {
+            add(x, y[0], f, c);
+            if (c + 2u < C) load(y[0], c + 2u);
+            if (c + 1u < C) add(x, y[1], f, c + 1u);
+            if (c + 3u < C) load(y[1], c + 3u);
+        }
+#pragma unroll
+        for (uint32_t v = 0; v < 4; ++v) {
+            const uint32_t r = rank + C * (k0 + v);
+            const float sum = __shfl_sync(0xffffffffu, L, 8 * v);
+            if (r >= rows) continue;
+            const uint2 at = tr.at(r);
+            const float inv = any_bad || p0 + at.x >= a.c.max_context ? __int_as_float(0x7fffffff) : 1.0f / sum;
+            reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + at.x) * a.ldo + (size_t)(h * a.group + at.y) * kDim)[lane] =
+                make_float4(x[v].x * inv, x[v].y * inv, x[v].z * inv, x[v].w * inv);
         }
     }
     cluster_sync();   // no CTA leaves while the cluster may read its states
@@ -705,11 +747,28 @@ cudaError_t launch_prompt(AttnArgs a, int dev, int sms, cudaStream_t stream)
 {
     cudaError_t e = allow<prompt_kernel>(dev, (int)kPromptSmem);
     if (e != cudaSuccess) return e;
-    a.tiles = (a.r.tokens * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
-    // CTAs per unit: as many as fit the device at once (one per SM), at most 8, two tiles of keys each at least
-    const uint64_t units = (uint64_t)a.tiles * a.c.kv_heads * a.c.nseq;
-    const uint64_t fit = std::min<uint64_t>((uint64_t)sms / units, a.c.max_context / (2 * kTileKeys));
-    const uint32_t C = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(fit, 1), 8);
+    // Two tiles per CTA, or one; and up to 8 CTAs per unit, two tiles of keys
+    // each at least. What does not fit the device at once takes two tiles and
+    // whole units. What does goes by the longest unit's time, in cycles: 4000
+    // for one tile of rows against a tile of keys, 5600 for two; 9000 and
+    // 13000 before and after the loop, and 5000 per tile of rows for a merge.
+    const uint32_t rows = a.r.tokens * a.group, keys = (a.c.max_context + kTileKeys - 1) / kTileKeys;
+    const uint64_t heads = (uint64_t)a.c.kv_heads * a.c.nseq;
+    uint32_t C = 1;
+    uint64_t best = ~0ull;
+    a.cta_tiles = 2;
+    for (uint32_t t = 1; t <= 2; ++t) {
+        const uint64_t units = (rows + t * kTileRows - 1) / (t * kTileRows) * heads;
+        for (uint32_t c = 1; c <= kMaxSplit && units * c <= (uint64_t)sms && (c == 1 || 2 * c <= keys); ++c) {
+            const uint64_t cost = (uint64_t)(t == 1 ? 4000 : 5600) * ((keys + c - 1) / c) + 5000 + 4000 * t + (c > 1 ? 5000 * t : 0);
+            if (cost < best) {
+                best = cost;
+                a.cta_tiles = t;
+                C = c;
+            }
+        }
+    }
+    a.tiles = (rows + a.cta_tiles * kTileRows - 1) / (a.cta_tiles * kTileRows);
     return launch(prompt_kernel, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), kPromptThreads, kPromptSmem, C, a, sms, stream);
 }
 
