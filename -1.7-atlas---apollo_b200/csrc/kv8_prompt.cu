@@ -25,6 +25,9 @@
 //          way by cp.async while the MMAs still read the current ones;
 //   20     issues the MMAs: P V of a tile, then the next keys' scores of the
 //          same tile, so that one tile's softmax runs under the other's MMAs.
+// Where few rows leave SMs idle, a CTA takes one tile of 128 rows: both softmax
+// groups then have the same rows and take turns at the tiles of keys, each with
+// an output and a state of its own, which are merged at the end.
 // Tensor memory: 2 x 128 columns of scores / weights, 2 x 128 of output.
 // Shared memory: Q hi / lo 128 KB, K 32 KB, V 32 KB, their next codes 32 KB; Q's
 // place stages the output.
@@ -335,6 +338,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         return;
     }
     const uint32_t rows = min(all - r0, a.cta_tiles * kTileRows), tiles = rows > kTileRows ? 2u : 1u;
+    const bool one = a.cta_tiles == 1u;
     const uint32_t limit = (uint32_t)min(p0 + tr.at(rows - 1u).x + 1u, (uint64_t)a.c.max_context);
     const uint32_t total = (limit + kTileKeys - 1u) / kTileKeys;
     uint32_t j0 = 0u, n = total;   // this CTA's tiles of keys
@@ -355,11 +359,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             // K and V go by halves (64 dimensions, 64 keys): a half is converted
             // while the MMAs still read, or already read, the other.
             bool ok = n != 0u && mbar_wait(&b.q_full, 0u, err);
-            auto scores = [&](uint32_t t, uint32_t j) {   // of keys j: the first tile waits for K, the last one releases it
-                const uint64_t q = qd + (uint64_t)(t * (kQTile >> 4));
+            // scores of keys j against Q tile `qt` into S of group t; P V of keys j into the group's output
+            auto scores = [&](uint32_t t, uint32_t qt, uint32_t j, bool first_use, bool last_use) {
+                const uint64_t q = qd + (uint64_t)(qt * (kQTile >> 4));
 #pragma unroll
                 for (uint32_t hf = 0; hf < 2u; ++hf) {
-                    if (t == 0u) {
+                    if (first_use) {
                         if (!(ok = ok && mbar_wait(&b.k_full[hf], j & 1u, err))) return;
                         fence_after();
                     }
@@ -369,30 +374,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                         mma_ss(tmem + 128u * t, q + off, kd + off, hf != 0u || st != 0u);
                         mma_ss(tmem + 128u * t, q + (2u * kHalf >> 4) + off, kd + off, 1u);
                     }
-                    if (t + 1u == tiles) commit(&b.k_empty[hf]);
+                    if (last_use) commit(&b.k_empty[hf]);
                 }
                 commit(&b.s_full[t]);
             };
-            for (uint32_t t = 0; ok && t < tiles; ++t) scores(t, 0u);
-            for (uint32_t j = 0; ok && j < n; ++j) {
-                for (uint32_t t = 0; ok && t < tiles; ++t) {
-                    if (!(ok = mbar_wait(&b.p_full[t], j & 1u, err))) break;
+            auto output = [&](uint32_t t, uint32_t j, uint32_t turn, bool first_use, bool last_use) {
+                if (!(ok = ok && mbar_wait(&b.p_full[t], turn & 1u, err))) return;
 #pragma unroll
-                    for (uint32_t hf = 0; hf < 2u; ++hf) {
-                        if (t == 0u && !(ok = ok && mbar_wait(&b.v_full[hf], j & 1u, err))) break;
-                        fence_after();
+                for (uint32_t hf = 0; hf < 2u; ++hf) {
+                    if (first_use && !(ok = ok && mbar_wait(&b.v_full[hf], j & 1u, err))) return;
+                    fence_after();
 #pragma unroll
-                        for (uint32_t st = 0; st < 4u; ++st) {
-                            const uint64_t v = vd + hf * (kHalf >> 4) + st * 2u;
-                            const uint32_t p = tmem + 128u * t + 64u * hf + 16u * st;
-                            mma_ts(tmem + 256u + 128u * t, p, v, j != 0u || hf != 0u || st != 0u);
-                            mma_ts(tmem + 256u + 128u * t, p + 8u, v, 1u);
-                        }
-                        if (t + 1u == tiles) commit(&b.v_empty[hf]);
+                    for (uint32_t st = 0; st < 4u; ++st) {
+                        const uint64_t v = vd + hf * (kHalf >> 4) + st * 2u;
+                        const uint32_t p = tmem + 128u * t + 64u * hf + 16u * st;
+                        mma_ts(tmem + 256u + 128u * t, p, v, turn != 0u || hf != 0u || st != 0u);
+                        mma_ts(tmem + 256u + 128u * t, p + 8u, v, 1u);
                     }
+                    if (last_use) commit(&b.v_empty[hf]);
+                }
+            };
+            if (one) {   // the groups take turns at the keys
+                for (uint32_t j = 0; ok && j < min(n, 2u); ++j) scores(j, 0u, j, true, true);
+                for (uint32_t j = 0; ok && j < n; ++j) {
+                    output(j & 1u, j, j >> 1, true, true);
                     if (!ok) break;
-                    if (j + 1u < n) scores(t, j + 1u);
-                    else commit(&b.o_full[t]);
+                    if (j + 2u < n) scores(j & 1u, 0u, j + 2u, true, true);
+                    else commit(&b.o_full[j & 1u]);
+                }
+            } else {
+                for (uint32_t t = 0; ok && t < tiles; ++t) scores(t, t, 0u, t == 0u, t + 1u == tiles);
+                for (uint32_t j = 0; ok && j < n; ++j) {
+                    for (uint32_t t = 0; ok && t < tiles; ++t) {
+                        output(t, j, j, t == 0u, t + 1u == tiles);
+                        if (!ok) break;
+                        if (j + 1u < n) scores(t, t, j + 1u, t == 0u, t + 1u == tiles);
+                        else commit(&b.o_full[t]);
+                    }
                 }
             }
             // nothing of this CTA is left in flight when tensor memory is freed
@@ -546,22 +564,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         // Warps w and w + 4 of a tile share 32 rows. A warp whose wait ran out
         // goes on through the barriers, without touching tensor memory.
         const uint32_t t = warp >> 3, half = (warp >> 2) & 1u, quarter = warp & 3u, row = quarter * 32u + lane;
-        const uint32_t i = t * kTileRows + row;
-        if (t < tiles) {
+        const uint32_t i = (one ? 0u : t * kTileRows) + row;
+        if (one || t < tiles) {
             const uint32_t at = tmem + ((quarter * 32u) << 16) + 128u * t + 64u * half, g0 = 4u * half;
-            const float factor = b.half[t][0][row];
-            const uint32_t open = (uint32_t)min(p0 + tr.at(t * kTileRows).x, (uint64_t)0x7fffffffu);
+            const float factor = b.half[one ? 0u : t][0][row];
+            if (one) meet(3u, 32u * kConvWarp);   // both groups have read it
+            const uint32_t open = (uint32_t)min(p0 + tr.at(one ? 0u : t * kTileRows).x, (uint64_t)0x7fffffffu);
             const uint32_t last = i < rows ? (uint32_t)min(p0 + tr.at(i).x, (uint64_t)0x7fffffffu) : open;
             const float *scales = (lane & 8u ? a.c.v_scale : a.c.k_scale) + head * a.c.n_blocks;
             auto scale_of = [&](uint32_t j) {
                 return __ldcg(scales + min(((j0 + j) * kTileKeys + 16u * (lane & 7u)) >> a.c.block_log2, a.c.n_blocks - 1u));
             };
-            float m = -INFINITY, l = 0.f, next = n ? scale_of(0u) : 0.f;
+            const uint32_t j_first = one ? t : 0u, j_step = one ? 2u : 1u;
+            float m = -INFINITY, l = 0.f, next = j_first < n ? scale_of(j_first) : 0.f;
             uint32_t vref = kTinyScale;
             bool ok = true;
-            for (uint32_t j = 0; j < n; ++j) {
+            for (uint32_t j = j_first, turn = 0; j < n; j += j_step, ++turn) {
                 const float sc = next;
-                if (j + 1u < n) next = scale_of(j + 1u);
+                if (j + j_step < n) next = scale_of(j + j_step);
                 const uint32_t key0 = (j0 + j) * kTileKeys, mine = key0 + 64u * half;
                 const bool masked = key0 + kTileKeys - 1u > open;   // some row does not see all of the tile
                 const int nvis = last < mine ? 0 : (int)min(last - mine + 1u, 64u);
@@ -585,7 +605,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                     lg[c] = __shfl_sync(0xffffffffu, pl, 8u + g0 + c);
                     ipf[c] = __shfl_sync(0xffffffffu, pr, 8u + g0 + c);
                 }
-                ok = ok && wait_warp(&b.s_full[t], j & 1u, err);
+                ok = ok && wait_warp(&b.s_full[t], turn & 1u, err);
                 fence_after();
                 float x = -INFINITY;
                 if (ok) x = masked ? tile_max<true>(at, f, nvis) : tile_max<false>(at, f, 64);
@@ -602,7 +622,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                         l *= fm;
                         fv *= fm;
                     }
-                    if (j && ok) {
+                    if (turn && ok) {
 #pragma unroll 1
                         for (uint32_t c = 0; c < 64u; c += 16u) {
                             float o[16];
@@ -628,9 +648,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             meet(1u + t, 256u);
             l += b.half[t][half ^ 1u][row];
             // the output into Q's place: row-major, 16-byte chunks XORed with the row
-            const bool have = n && ok && wait_warp(&b.o_full[t], 0u, err);
+            const bool have = j_first < n && ok && wait_warp(&b.o_full[t], 0u, err);
             fence_after();
-            const float back = C > 1u ? __uint_as_float(vref) * (1.0f / 64.0f) : __uint_as_float(vref) * (1.0f / 64.0f) / l;
+            const float back = __uint_as_float(vref) * (1.0f / 64.0f) * (one || C > 1u ? 1.0f : 1.0f / l);
             float4 *stage = reinterpret_cast<float4 *>(qs + t * kQTile);
 #pragma unroll 1
             for (uint32_t c = 0; c < 4u; ++c) {
@@ -645,23 +665,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                         have ? make_float4(o[4 * k] * back, o[4 * k + 1] * back, o[4 * k + 2] * back, o[4 * k + 3] * back)
                              : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            meet(1u + t, 256u);
-            if (C == 1u) {
-                // warp w of the tile: rows 16 w .. 16 w + 15
-                const uint32_t w0 = (warp & 7u) * 16u, end = rows - t * kTileRows;
+            if (one) {
+                // both groups' states of a row -> one, in the place of group 0's
+                meet(3u, 32u * kConvWarp);   // the sums have been read
+                if (half == 0u) {
+                    b.half[t][0][row] = m;
+                    b.half[t][1][row] = l;
+                }
+                meet(3u, 32u * kConvWarp);
+                const float m1 = b.half[t ^ 1u][0][row], l1 = b.half[t ^ 1u][1][row], M = fmaxf(m, m1);
+                // what the own state counts; a state that saw no position counts nothing
+                const float own = m == -INFINITY && l == 0.f ? 0.f : ex2(m - M), other = m1 == -INFINITY && l1 == 0.f ? 0.f : ex2(m1 - M);
+                row_m = M;
+                row_l = l * own + l1 * other;
+                meet(3u, 32u * kConvWarp);
+                if (half == 0u) b.half[t][0][row] = C > 1u ? own : own / row_l;
+            } else {
+                row_m = m;
+                row_l = l;
+            }
+            if (one) meet(3u, 32u * kConvWarp);
+            else meet(1u + t, 256u);
+            if (C == 1u || one) {
+                // rows of the tile for this warp: 16, or 8 where both groups have one tile
+                const uint32_t each = one ? 8u : 16u, w0 = (one ? warp : warp & 7u) * each, end = rows - (one ? 0u : t * kTileRows);
                 const bool failed = *err != kStatusOk;
+                float4 *const other = reinterpret_cast<float4 *>(qs + kQTile);
+                stage = reinterpret_cast<float4 *>(qs + (one ? 0u : t * kQTile));
 #pragma unroll 4
-                for (uint32_t k = w0; k < w0 + 16u; ++k) {
-                    const uint2 r = tr.at(t * kTileRows + k);
-                    float4 x = stage[k * 32u + (lane ^ (k & 31u))];
+                for (uint32_t k = w0; k < w0 + each; ++k) {
+                    const uint32_t at4 = k * 32u + (lane ^ (k & 31u));
+                    float4 x = stage[at4];
+                    if (one) {
+                        const float4 y = other[at4];
+                        const float f0 = b.half[0][0][k], f1 = b.half[1][0][k];
+                        x = make_float4(x.x * f0 + y.x * f1, x.y * f0 + y.y * f1, x.z * f0 + y.z * f1, x.w * f0 + y.w * f1);
+                    }
+                    if (C > 1u) {
+                        stage[at4] = x;
+                        continue;
+                    }
+                    const uint2 r = tr.at((one ? 0u : t * kTileRows) + k);
                     if (failed || p0 + r.x >= a.c.max_context) x.x = x.y = x.z = x.w = __int_as_float(0x7fffffff);
                     if (k < end)
                         reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo +
                                                    (size_t)(h * a.group + r.y) * kDim)[lane] = x;
                 }
-            } else if (half == 0u) {
-                row_m = m;
-                row_l = l;
             }
         }
     }
@@ -672,7 +721,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
     if (C == 1u) return;
-    // the converters' slots are free now
+    // the converters' slots are free now (a state per row: of the first group where the groups shared the rows)
     if (warp < kConvWarp && (warp & 4u) == 0u) {
         rs.max[warp >> 3][(warp & 3u) * 32u + lane] = row_m;
         rs.sum[warp >> 3][(warp & 3u) * 32u + lane] = row_l;
@@ -749,9 +798,9 @@ cudaError_t launch_prompt(AttnArgs a, int dev, int sms, cudaStream_t stream)
     if (e != cudaSuccess) return e;
     // Two tiles per CTA, or one; and up to 8 CTAs per unit, two tiles of keys
     // each at least. What does not fit the device at once takes two tiles and
-    // whole units. What does goes by the longest unit's time, in cycles: 4000
-    // for one tile of rows against a tile of keys, 5600 for two; 9000 and
-    // 13000 before and after the loop, and 5000 per tile of rows for a merge.
+    // whole units. What does goes by the longest unit's time, in cycles: 2500
+    // for one tile of rows against a tile of keys, 5600 for two; 12000 and
+    // 16000 before and after the loop, and 5000 per tile of rows for a merge.
     const uint32_t rows = a.r.tokens * a.group, keys = (a.c.max_context + kTileKeys - 1) / kTileKeys;
     const uint64_t heads = (uint64_t)a.c.kv_heads * a.c.nseq;
     uint32_t C = 1;
@@ -760,7 +809,7 @@ cudaError_t launch_prompt(AttnArgs a, int dev, int sms, cudaStream_t stream)
     for (uint32_t t = 1; t <= 2; ++t) {
         const uint64_t units = (rows + t * kTileRows - 1) / (t * kTileRows) * heads;
         for (uint32_t c = 1; c <= kMaxSplit && units * c <= (uint64_t)sms && (c == 1 || 2 * c <= keys); ++c) {
-            const uint64_t cost = (uint64_t)(t == 1 ? 4000 : 5600) * ((keys + c - 1) / c) + 5000 + 4000 * t + (c > 1 ? 5000 * t : 0);
+            const uint64_t cost = (uint64_t)(t == 1 ? 2500 : 5600) * ((keys + c - 1) / c) + 8000 + 4000 * t + (c > 1 ? 5000 * t : 0);
             if (cost < best) {
                 best = cost;
                 a.cta_tiles = t;

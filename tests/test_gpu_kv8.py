@@ -234,6 +234,21 @@ def test_prompt_pieces(torch_cuda, q_heads, heads, tokens, pos):
     check_attn(torch_cuda, rng, ref, q_heads, tokens, [pos])
 
 
+@pytest.mark.parametrize("nseq,q_heads,heads,tokens,pos,ctx", [
+    (1, 2, 1, 100, 1, 4000),        # one tile of rows, its positions over a cluster
+    (1, 8, 1, 40, 1000, 5000),      # two tiles of rows, over a cluster
+    (3, 14, 2, 150, 300, 480),      # one tile per CTA, none split
+    (5, 40, 8, 60, 77, 140),        # two tiles per CTA, more units than fit at once
+    (2, 28, 4, 99, 1500, 1700),     # odd row counts in the last tile
+    (1, 130, 1, 3, 400, 500),       # a group larger than a tile of rows
+])
+def test_prompt_splits(torch_cuda, nseq, q_heads, heads, tokens, pos, ctx):
+    rng = np.random.default_rng(ctx)
+    at = [pos + 13 * s for s in range(nseq)]
+    ref = filled(rng, nseq, heads, ctx, 32, [p + tokens for p in at])
+    check_attn(torch_cuda, rng, ref, q_heads, tokens, at)
+
+
 @pytest.mark.parametrize("block", [16, 32, 128])
 def test_prompt_blocks(torch_cuda, block):
     rng = np.random.default_rng(block)
