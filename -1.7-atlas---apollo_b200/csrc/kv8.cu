@@ -598,10 +598,15 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
                 const uint32_t pick = (j & 1) ? 0x7632u : 0x5410u;
                 const uint32_t ya = __byte_perm(w0[j >> 1], w1[j >> 1], pick), yb = __byte_perm(w2[j >> 1], w3[j >> 1], pick);
                 const uint32_t va[4] = {codes_h2<false>(ya), codes_h2<true>(ya), codes_h2<false>(yb), codes_h2<true>(yb)};
+                // the MMAs truncate their sums, so only a chunk's are left to them
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_h(o[nt][j], va, bh[nt][0], bh[nt][1]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    float x[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_h(x, va, bl[nt][0], bl[nt][1]);
+                    mma_h(x, va, bh[nt][0], bh[nt][1]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_h(o[nt][j], va, bl[nt][0], bl[nt][1]);
+                    for (int e = 0; e < 4; ++e) o[nt][j][e] += x[e];
+                }
             }
         }
     }
