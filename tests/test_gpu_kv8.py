@@ -349,6 +349,51 @@ def test_attn_many_positions(torch_cuda):
     check_attn(torch_cuda, rng, ref, 8, 1, [39999])
 
 
+@pytest.mark.parametrize("q_heads,tokens,ctx", [
+    (64, 300, 3300),      # two tiles of rows per CTA, all positions: three segments of 1024 in tensor memory
+    (60, 150, 2500),      # one tile per CTA, the two groups of warps take turns at the keys
+    (8, 7, 19000),        # over a cluster
+    (1, 150, 20000),
+])
+@pytest.mark.parametrize("rising", [False, True])
+def test_prompt_segments(torch_cuda, q_heads, tokens, ctx, rising):
+    """Outputs of more positions than tensor memory sums up at once; scores and V scales that grow along the positions,
+    so that maximum and V scale are raised in every segment, at its first tile as well as within."""
+    rng = np.random.default_rng(ctx)
+    q = rng.standard_normal((1, tokens, q_heads, DIM)).astype(np.float32)
+    if not rising:
+        ref = filled(rng, 1, 1, ctx, 64, [ctx])
+    else:
+        q[..., 0] = 4.0
+        at = np.arange(ctx) / ctx
+        k = 0.1 * rng.standard_normal((1, ctx, 1, DIM)).astype(np.float32)
+        k[0, :, 0, 0] = 200.0 * at                # scores up to 70
+        v = rng.standard_normal((1, ctx, 1, DIM)).astype(np.float32) * np.exp2(np.rint(12 * at)).astype(np.float32)[:, None, None]
+        ref = RefCache(1, 1, ctx, 64, rng)
+        ref.append([0], [ctx], k, v)
+    check_attn(torch_cuda, rng, ref, q_heads, tokens, [ctx - tokens], q=q)
+
+
+@pytest.mark.parametrize("heads,q_heads,tokens", [(8, 8, 1), (1, 1, 200), (1, 64, 300)])
+def test_attn_sums_keep_their_precision(torch_cuda, heads, q_heads, tokens):
+    """Equal weights over values of one sign. Relative to the output, with u = 2^-24: tensor cores truncate each of the 128
+    sums of a segment (2 u of a sum that grows evenly: 128 u; the mean of that, at most 50 u, is made up for), the weights'
+    terms 16 u, their sum and the segments' at most 64 u."""
+    torch, ctx = torch_cuda, 8000
+    rng = np.random.default_rng(17)
+    ref = RefCache(1, heads, ctx, 128, rng)
+    x = rng.uniform(0.5, 1.0, (1, ctx, heads, DIM)).astype(np.float32)
+    ref.append([0], [ctx], x, x)
+    out = torch.zeros(1, tokens, q_heads, DIM, device="cuda")
+    atlas_cuda.kv8_attn(DevCache(torch, ref).c, q_heads, tokens, _i32(torch, [ctx - tokens]), torch.zeros_like(out), out)
+    got = out.cpu().numpy().astype(np.float64)[0]
+    for h in range(heads):
+        v = ref.values(0, h, ctx)[1]
+        want = (np.cumsum(v, 0) / np.arange(1, ctx + 1)[:, None])[ctx - tokens:]
+        rows = got[:, h * q_heads // heads:(h + 1) * q_heads // heads]
+        assert (np.abs(rows / want[:, None] - 1) <= 258 * 2.0 ** -24).all()
+
+
 def test_attn_large_batch(torch_cuda):
     """More units of work than CTAs fit on the device (clusters of one)."""
     rng = np.random.default_rng(16)
