@@ -324,7 +324,7 @@ struct alignas(1024) Smem {
         uint8_t ring[W][kStages][kSlot];
         float wrec[W][8 * NT][kRecStride];     // the warps' outputs, once the ring is done with
     } u;
-    float rec[kMaxCluster][kRecStride];        // the states that the cluster's CTAs send of this CTA's rows
+    float rec[W < 8 ? 1 : kMaxCluster][kRecStride];   // the states that the cluster's CTAs send of this CTA's rows (W < 8: no cluster)
     uint64_t full[W][kStages];                 // a chunk has landed
     uint32_t err;
     float2 wml[W][8 * NT];                     // the warps' maxima and sums
@@ -348,15 +348,22 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, const TileRows &tr,
     reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo + (size_t)(h * a.group + r.y) * kDim)[d4] = x;
 }
 
-// This warp's query rows warp, warp + 8, ... of the tile (lane = 4 dimensions; warps from 8 on have none). Rows of
-// tokens that the call does not have are zeros; rows past n_tok are read and their results dropped.
-template <int NT>
-__device__ __forceinline__ void load_queries(const AttnArgs &a, const TileRows &tr, uint32_t s, uint32_t h, float4 (&x)[NT])
+// This warp's query rows warp, warp + 8, ... of the tile (lane = 4 dimensions; warps from 8 on have none; of W < 8
+// warps, every W-th row). Rows of tokens that the call does not have are zeros; rows past n_tok are read and their
+// results dropped.
+constexpr uint32_t row_warps(uint32_t W) { return W < 8u ? W : 8u; }
+template <int NT, uint32_t W>
+struct Queries {
+    float4 x[8 * NT / row_warps(W)];
+};
+template <int NT, uint32_t W>
+__device__ __forceinline__ void load_queries(const AttnArgs &a, const TileRows &tr, uint32_t s, uint32_t h, Queries<NT, W> &q)
 {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const uint2 r = tr.at(warp + 8u * (uint32_t)i);
+    for (uint32_t i = 0; i < 8u * NT / row_warps(W); ++i) {
+        const uint2 r = tr.at(warp + row_warps(W) * i);
+        float4(&x)[8 * NT / row_warps(W)] = q.x;
         x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (warp < 8u && r.x < a.r.tokens)
             x[i] = __ldcg(reinterpret_cast<const float4 *>(a.q + ((size_t)s * a.r.tokens + r.x) * a.ldq +
@@ -384,7 +391,7 @@ __device__ __forceinline__ void init_ring(const FewArgs &a, Smem<NT, W> &sm)
 // tile's rows that exist. KEYS deals chunks [0, chunks). The CTAs of a cluster
 // have arrived on its barrier once before.
 template <int NT, uint32_t W, class KEYS>
-__device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const KEYS &keys, const float4 (&qx)[NT],
+__device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const KEYS &keys, const Queries<NT, W> &q,
                                        const TileRows &tr, uint32_t s, uint32_t h, uint32_t rows, uint64_t p0,
                                        uint32_t chunks)
 {
@@ -424,8 +431,8 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
     // the query rows as int8 planes; powers of two keep max|q| and its reciprocal away from the ends of the range
     if (warp < 8u)
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const float v[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
+    for (uint32_t i = 0; i < 8u * NT / row_warps(W); ++i) {
+        const float v[4] = {q.x[i].x, q.x[i].y, q.x[i].z, q.x[i].w};
         uint32_t mx = 0u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) mx = max(mx, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -446,7 +453,7 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
                 }
             }
         }
-        const uint32_t row = warp + 8u * (uint32_t)i;
+        const uint32_t row = warp + row_warps(W) * i;
 #pragma unroll
         for (int p = 0; p < 3; ++p) sm.plane[p][row][8u * (lane & 3u) + (lane >> 2)] = w[p];
         // a row with a non-finite value: every score NaN
@@ -638,8 +645,8 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
     const float cinv = rcp((float)C);
     const uint32_t per = (uint32_t)(((float)(R + C) - 0.5f) * cinv);   // ceil(R / C)
     if (threadIdx.x < 256u) {
-        constexpr uint32_t kPer = 256u / R;   // threads per row, 4 dimensions at a time
-        const uint32_t i = threadIdx.x / kPer, part = threadIdx.x % kPer, q = (uint32_t)(((float)i + 0.5f) * cinv);   // i / C
+        constexpr uint32_t kPer = 32u * row_warps(W) / R;   // threads per row, 4 dimensions at a time
+        const uint32_t i = threadIdx.x / kPer, part = threadIdx.x % kPer, turn = (uint32_t)(((float)i + 0.5f) * cinv);   // i / C
         float2 ml[W];
         float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -666,12 +673,12 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
             }
             if (i >= rows) continue;
             if (C == 1u) store_row(a, tr, s, h, i, p0, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-            else st_cluster(&sm.rec[rank * per + q][4u * d], i - q * C, x);
+            else st_cluster(&sm.rec[rank * per + turn][4u * d], i - turn * C, x);
         }
         if (C > 1u && part == 0u && i < rows)
-            st_cluster(&sm.rec[rank * per + q][kDim], i - q * C, make_float4(M, L, 0.f, 0.f));
+            st_cluster(&sm.rec[rank * per + turn][kDim], i - turn * C, make_float4(M, L, 0.f, 0.f));
     }
-    if (C == 1u) return;
+    if (W < 8u || C == 1u) return;
     cluster_sync();   // every record has arrived; nothing remote is touched from here on
     // warp k: row rank + k C; lane: a CTA's maximum and sum, then 4 dimensions
     const uint32_t i = rank + warp * C;
@@ -716,8 +723,8 @@ __global__ void __launch_bounds__(W * 32, 1) attn_kernel(const __grid_constant__
     wait_predecessor(a.early);
     const uint64_t p0 = __ldcg(a.r.pos0 + s);
     const uint32_t all = row_count(a.r, s) * a.group;
-    float4 q[NT];
-    load_queries<NT>(a, tr, s, h, q);
+    Queries<NT, W> q;
+    load_queries(a, tr, s, h, q);
     if (r0 >= all) {   // the whole cluster leaves
         if (cluster_size() > 1u) cluster_wait();
         return;
@@ -739,7 +746,7 @@ __global__ void __launch_bounds__(W * 32, 1) attn_kernel(const __grid_constant__
 // above every number: a poisoned block is chosen and shows in the output.
 // The CTAs of the cluster score every C-th block each, send the keys to all of
 // them, and each picks the blocks on its own (a search for the lowest chosen
-// key, three bits at a time), so the whole operator is one launch.
+// key), so the whole operator is one launch.
 // Bound by latency: 260 bytes per candidate block, then n_sel blocks.
 
 struct Chosen {
@@ -766,8 +773,13 @@ __device__ __forceinline__ double pool_query(const AttnArgs &a, const float *q)
 {
     double x = 0.0;
     if (threadIdx.x < kDim)
-#pragma unroll 8
-        for (uint32_t i = 0; i < a.group; ++i) x += (double)__ldcg(q + (size_t)i * kDim + threadIdx.x);
+        for (uint32_t i = 0; i < a.group; i += 8u) {   // eight on their way at a time
+            float v[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) v[k] = i + k < a.group ? __ldcg(q + (size_t)(i + k) * kDim + threadIdx.x) : 0.f;
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) x += (double)v[k];
+        }
     return x;
 }
 
@@ -787,6 +799,14 @@ __device__ __forceinline__ void code_query(PickSmem &ps, double x)
         ps.code[threadIdx.x] = most > 0.0 && most < INFINITY ? (int8_t)(int)rint(127.0 * x / most) : (int8_t)0;
     }
     __syncthreads();
+}
+
+// A word that orders as the scores do
+__device__ __forceinline__ unsigned long long block_key(int d, float sc)
+{
+    const double x = (double)d * (double)sc + 0.0;   // + 0: one zero
+    const unsigned long long k = (unsigned long long)__double_as_longlong(x);
+    return x != x ? ~0ull : (k >> 63) ? ~k : k | 1ull << 63;
 }
 
 // Keys of blocks rank, rank + C, ... below nb, into every CTA's `key`: 8 lanes per block, 16 dimensions each.
@@ -820,9 +840,7 @@ __device__ __forceinline__ void score_blocks(const AttnArgs &a, const PickSmem &
         d += __shfl_xor_sync(0xffffffffu, d, 1);
         d += __shfl_xor_sync(0xffffffffu, d, 2);
         d += __shfl_xor_sync(0xffffffffu, d, 4);
-        const double x = (double)d * (double)sc + 0.0;   // + 0: one zero
-        unsigned long long k = (unsigned long long)__double_as_longlong(x);
-        k = x != x ? ~0ull : (k >> 63) ? ~k : k | 1ull << 63;   // orders as the scores do
+        const unsigned long long k = block_key(d, sc);
         if (b < nb) {
             if (C == 1u) {
                 if (part == 0u) key[b] = k;
@@ -844,19 +862,22 @@ __device__ __forceinline__ unsigned long long search_warp(const unsigned long lo
     constexpr uint32_t kPer = kWarpPick / 32u;
     const uint32_t lane = threadIdx.x & 31u;
     uint32_t k[kPer], least = 0u, n = nb;
+    if (nb <= kWarpPick) {
 #pragma unroll
-    for (uint32_t j = 0; j < kPer; ++j) k[j] = 32u * j + lane < nb ? (uint32_t)(key[32u * j + lane] >> 32) : 0u;
-    for (uint32_t bit = 1u << 31; bit && n != want; bit >>= 1) {
-        const uint32_t at = least | bit;
-        uint32_t c = 0u;
+        for (uint32_t j = 0; j < kPer; ++j) k[j] = 32u * j + lane < nb ? (uint32_t)(key[32u * j + lane] >> 32) : 0u;
+        for (uint32_t bit = 1u << 31; bit && n != want; bit >>= 1) {
+            const uint32_t at = least | bit;
+            uint32_t c = 0u;
 #pragma unroll
-        for (uint32_t j = 0; j < kPer; ++j) c += k[j] >= at ? 1u : 0u;
-        c = __reduce_add_sync(0xffffffffu, c);
-        if (c >= want) least = at, n = c;
+            for (uint32_t j = 0; j < kPer; ++j) c += k[j] >= at ? 1u : 0u;
+            c = __reduce_add_sync(0xffffffffu, c);
+            if (c >= want) least = at, n = c;
+        }
     }
     unsigned long long all = (unsigned long long)least << 32;
-    for (uint32_t bit = 1u << 31; bit && n != want; bit >>= 1) {
+    for (unsigned long long bit = nb <= kWarpPick ? 1ull << 31 : 1ull << 63; bit && n != want; bit >>= 1) {
         uint32_t c = 0u;
+#pragma unroll 8
         for (uint32_t i = lane; i < nb; i += 32u) c += key[i] >= (all | bit) ? 1u : 0u;
         c = __reduce_add_sync(0xffffffffu, c);
         if (c >= want) all |= bit, n = c;
@@ -967,8 +988,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const
     const uint64_t p0 = __ldcg(a.r.pos0 + s);
     const uint32_t n = row_count(a.r, s);
     const double pooled = pool_query(a, a.q + ((size_t)s * a.r.tokens + token) * a.ldq + (size_t)h * a.group * kDim);
-    float4 q[NT];
-    load_queries<NT>(a, tr, s, h, q);
+    Queries<NT, kWarps> q;
+    load_queries(a, tr, s, h, q);
     if (token >= n) {   // the whole cluster leaves
         if (C > 1u) cluster_wait();
         return;
@@ -1002,6 +1023,172 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) sparse_kernel(const
     const uint32_t per = a.c.block_log2 - 4u;
     const uint32_t chunks = (want << per) + ((p & ((1u << a.c.block_log2) - 1u)) / kChunk) + 1u;
     attend<NT, kWarps>(a, sm, Chosen{list, per, a.c.block_log2}, q, tr, s, h, min(a.group - tile * 8u * NT, 8u * NT), p0, chunks);
+}
+
+// The same in two launches, for many tokens: a pass that only chooses, eight
+// tokens of a KV head per CTA, and one that attends to what `sel` then holds, in
+// CTAs of four warps, four of them per SM. The scores of eight tokens are one
+// product of integer MMAs (m16n8k32: rows are blocks, columns tokens), in which
+// the sums enter as 256 hi + lo, a signed and an unsigned byte; a warp per token
+// then searches. Taken where the CTAs of the one launch above, two per SM, do
+// not all fit at once: 256 and 516 units (28 heads on 4, 16 of 250 blocks of
+// 32) and 4128 (40 on 8, 16 of 125 blocks of 64) take 18.0, 36.1 and 302.6 us
+// as one launch, 23.9, 26.6 and 195.7 us as two. Bound by instruction issue
+// (400 per 16 positions) and the latency of a unit's short way.
+
+constexpr uint32_t kPickTokens = 8;
+struct TokensSmem {
+    alignas(16) uint32_t code[kPickTokens][kDim / 4];
+};   // then the keys, a row of n_blocks per token
+
+// u8 x s8
+__device__ __forceinline__ void mma_u8(int (&d)[4], const int (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ size_t sel_row(const AttnArgs &a, uint32_t s, uint32_t token, uint32_t h)
+{
+    return (((size_t)s * a.r.tokens + token) * a.c.kv_heads + h) * a.n_sel;
+}
+
+__global__ void __launch_bounds__(32 * kPickTokens) choose_kernel(const __grid_constant__ AttnArgs a)
+{
+    extern __shared__ __align__(16) uint8_t choose_smem[];
+    TokensSmem &sm = *reinterpret_cast<TokensSmem *>(choose_smem);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, s = blockIdx.z, h = blockIdx.y;
+    const uint32_t first = blockIdx.x * kPickTokens, token = first + warp;
+    unsigned long long *const keys = reinterpret_cast<unsigned long long *>(&sm + 1), *const key = keys + (size_t)warp * a.c.n_blocks;
+    wait_predecessor(a.early);
+    const uint64_t p0 = __ldcg(a.r.pos0 + s);
+    const uint32_t n = row_count(a.r, s);
+    if (first >= n) return;
+    auto own_block = [&](uint32_t tok) { return (uint32_t)min(p0 + tok, (uint64_t)a.c.max_context - 1u) >> a.c.block_log2; };
+    const bool inside = p0 + token < a.c.max_context;
+    const uint32_t own = own_block(token), want = min(own, a.n_sel - 1u);
+    const uint32_t most = own_block(min(first + kPickTokens, n) - 1u);   // blocks that some token scores
+    int32_t *sel = a.sel + sel_row(a, s, token, h);
+    if (a.n_sel > 1u && most >= a.n_sel) {
+        const size_t head = (size_t)s * a.c.kv_heads + h;
+        const int4 *const sums = reinterpret_cast<const int4 *>(a.c.k_sum + head * a.c.n_blocks * kDim);
+        const float *const scale = a.c.k_scale + head * a.c.n_blocks;
+        const uint32_t g = lane >> 2, t = lane & 3u;
+        // the pooled query: lane = 4 dimensions
+        double x[4] = {0.0, 0.0, 0.0, 0.0};
+        if (token < n) {
+            const float4 *q = reinterpret_cast<const float4 *>(a.q + ((size_t)s * a.r.tokens + token) * a.ldq + (size_t)h * a.group * kDim) + lane;
+            for (uint32_t i = 0; i < a.group; i += 8u) {   // eight on their way at a time
+                float4 v[8];
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k) v[k] = i + k < a.group ? __ldcg(q + (size_t)(i + k) * (kDim / 4u)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k) {
+                    x[0] += (double)v[k].x;
+                    x[1] += (double)v[k].y;
+                    x[2] += (double)v[k].z;
+                    x[3] += (double)v[k].w;
+                }
+            }
+        }
+        unsigned long long top = 0ull;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, (unsigned long long)__double_as_longlong(fabs(x[j])));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const double amax = __longlong_as_double((long long)top);
+        uint32_t word = 0u;
+        if (amax > 0.0 && amax < INFINITY)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) word |= ((uint32_t)(int)rint(127.0 * x[j] / amax) & 255u) << (8 * j);
+        sm.code[warp][lane] = word;
+        __syncthreads();
+        // Step st of the product takes dimensions 8 (4 st + t) + 0 .. 7 of lane t: 16 bytes of a block's sums
+        uint2 qc[4];
+#pragma unroll
+        for (uint32_t st = 0; st < 4u; ++st) qc[st] = *reinterpret_cast<const uint2 *>(&sm.code[g][2u * (4u * st + t)]);
+#pragma unroll 2
+        for (uint32_t b0 = 16u * warp; b0 < most; b0 += 16u * kPickTokens) {
+            const uint32_t ba = min(b0 + g, most - 1u), bb = min(b0 + g + 8u, most - 1u);
+            int4 u[4], v[4];
+#pragma unroll
+            for (uint32_t st = 0; st < 4u; ++st) {
+                u[st] = __ldcg(sums + (size_t)ba * (kDim / 8u) + 4u * st + t);
+                v[st] = __ldcg(sums + (size_t)bb * (kDim / 8u) + 4u * st + t);
+            }
+            const float sa = __ldcg(scale + ba), sb = __ldcg(scale + bb);
+            int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t st = 0; st < 4u; ++st) {
+                const int l[4] = {(int)__byte_perm(u[st].x, u[st].y, 0x6420u), (int)__byte_perm(v[st].x, v[st].y, 0x6420u),
+                                  (int)__byte_perm(u[st].z, u[st].w, 0x6420u), (int)__byte_perm(v[st].z, v[st].w, 0x6420u)};
+                const int m[4] = {(int)__byte_perm(u[st].x, u[st].y, 0x7531u), (int)__byte_perm(v[st].x, v[st].y, 0x7531u),
+                                  (int)__byte_perm(u[st].z, u[st].w, 0x7531u), (int)__byte_perm(v[st].z, v[st].w, 0x7531u)};
+                mma_u8(lo, l, qc[st].x, qc[st].y);
+                mma_s8(hi, m, qc[st].x, qc[st].y);
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t b = b0 + g + (e < 2u ? 0u : 8u);
+                if (b < most) keys[(size_t)(2u * t + (e & 1u)) * a.c.n_blocks + b] = block_key(256 * hi[e] + lo[e], e < 2u ? sa : sb);
+            }
+        }
+    }
+    __syncthreads();
+    if (token >= n) return;
+    if (!inside) {
+        for (uint32_t i = lane; i < a.n_sel; i += 32u) sel[i] = -1;
+        return;
+    }
+    if (own > want && want) {
+        const unsigned long long least = search_warp(key, own, want);
+        uint32_t need = want;   // of the keys equal to `least`, the first
+        for (uint32_t b = lane; b - lane < own; b += 32u) need -= __popc(__ballot_sync(0xffffffffu, b < own && key[b] > least));
+        const uint32_t below = (1u << lane) - 1u;
+        uint32_t at = 0u, equal = 0u;
+        for (uint32_t b = lane; b - lane < own; b += 32u) {
+            const unsigned long long k = b < own ? key[b] : 0ull;
+            const bool same = b < own && k == least;
+            const uint32_t sames = __ballot_sync(0xffffffffu, same);
+            const bool take = (b < own && k > least) || (same && equal + __popc(sames & below) < need);
+            const uint32_t takes = __ballot_sync(0xffffffffu, take);
+            if (take) sel[at + __popc(takes & below)] = (int32_t)b;
+            at += __popc(takes);
+            equal += __popc(sames);
+        }
+    } else {
+        for (uint32_t i = lane; i < want; i += 32u) sel[i] = (int32_t)i;
+    }
+    for (uint32_t i = want + lane; i < a.n_sel; i += 32u) sel[i] = i == want ? (int32_t)own : -1;
+}
+
+constexpr uint32_t kChosenWarps = 4;
+
+template <int NT>
+__global__ void __launch_bounds__(32 * kChosenWarps, (NT == 1 ? 16 : 8) / kChosenWarps) chosen_kernel(const __grid_constant__ FewArgs a)
+{
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem<NT, kChosenWarps> &sm = *reinterpret_cast<Smem<NT, kChosenWarps> *>(smem_raw);
+    uint32_t *list = reinterpret_cast<uint32_t *>(smem_raw + sizeof(Smem<NT, kChosenWarps>));
+    const uint32_t s = blockIdx.z, h = blockIdx.y, token = a.tiles == 1u ? blockIdx.x : blockIdx.x / a.tiles;
+    const uint32_t tile = blockIdx.x - token * a.tiles;
+    const TileRows tr{token, tile * 8u * NT, a.group, a.group_inv};
+    init_ring(a, sm);
+    wait_predecessor(a.early);
+    const uint64_t p0 = __ldcg(a.r.pos0 + s);
+    const uint32_t n = row_count(a.r, s);
+    if (token >= n) return;
+    const int32_t *sel = a.sel + sel_row(a, s, token, h);
+    const bool inside = p0 + token < a.c.max_context;   // else one chunk of any block, and NaN
+    const uint32_t p = inside ? (uint32_t)(p0 + token) : 0u, own = p >> a.c.block_log2, want = min(own, a.n_sel - 1u);
+    for (uint32_t i = threadIdx.x; i <= want; i += 32u * kChosenWarps) list[i] = min((uint32_t)__ldcg(sel + i), own);
+    Queries<NT, kChosenWarps> q;
+    load_queries(a, tr, s, h, q);
+    __syncthreads();
+    const uint32_t per = a.c.block_log2 - 4u;
+    const uint32_t chunks = (want << per) + ((p & ((1u << a.c.block_log2) - 1u)) / kChunk) + 1u;
+    attend<NT, kChosenWarps>(a, sm, Chosen{list, per, a.c.block_log2}, q, tr, s, h, min(a.group - tile * 8u * NT, 8u * NT), p0, chunks);
 }
 
 // ------------------------------------------------------------- host side ----
@@ -1159,9 +1346,19 @@ cudaError_t launch_attn(const FewArgs &a, int dev, int sms, cudaStream_t stream)
 template <int NT>
 cudaError_t launch_sparse(const FewArgs &a, int dev, int sms, cudaStream_t stream)
 {
-    cudaError_t e = allow<sparse_kernel<NT>>(dev, (int)kMaxSmem);
-    if (e != cudaSuccess) return e;
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.r.tokens * a.tiles;
+    const size_t keys = sizeof(TokensSmem) + (size_t)kPickTokens * a.c.n_blocks * 8u;
+    cudaError_t e;
+    if (units > 2u * (uint32_t)sms && keys <= kMaxSmem) {
+        if ((e = allow<choose_kernel>(dev, (int)kMaxSmem)) != cudaSuccess || (e = allow<chosen_kernel<NT>>(dev, (int)kMaxSmem)) != cudaSuccess)
+            return e;
+        e = launch(choose_kernel, dim3((a.r.tokens + kPickTokens - 1) / kPickTokens, a.c.kv_heads, a.c.nseq), 32 * kPickTokens, keys, 1,
+                   static_cast<AttnArgs>(a), sms, stream);
+        if (e != cudaSuccess) return e;
+        return launch(chosen_kernel<NT>, dim3(a.r.tokens * a.tiles, a.c.kv_heads, a.c.nseq), 32 * kChosenWarps,
+                      sizeof(Smem<NT, kChosenWarps>) + (size_t)a.n_sel * 4u, 1, a, sms, stream);
+    }
+    if ((e = allow<sparse_kernel<NT>>(dev, (int)kMaxSmem)) != cudaSuccess) return e;
     const size_t smem = sizeof(Smem<NT, kWarps>) + (size_t)a.n_sel * 4u;
     const uint32_t C = cluster_of<sparse_kernel<NT>>(dev, kThreads, sizeof(Smem<NT, kWarps>), units,
                                                      std::max<uint64_t>((uint64_t)a.n_sel << a.c.block_log2, a.c.max_context / 8), NT == 1);

@@ -427,6 +427,50 @@ def test_sparse_many_tokens(torch_cuda):
     check_attn(torch_cuda, rng, ref, 4, 300, [600, 100], [300, 300], n_sel=4)
 
 
+@pytest.mark.parametrize("nseq,q_heads,heads,tokens,pos,ctx,block,n_sel", [
+    (2, 14, 2, 90, 700, 800, 16, 5),      # 360 units: chosen in one pass, attended in another
+    (1, 24, 2, 90, 1000, 1100, 32, 8),    # two tiles of query rows per token
+    (1, 4, 4, 100, 0, 100, 16, 3),        # the first tokens have no more blocks than they may choose
+    (1, 4, 4, 100, 0, 100, 16, 100),      # nor has any
+    (1, 8, 4, 80, 300, 380, 64, 1),       # the own block alone
+    (1, 4, 4, 77, 9900, 10000, 16, 7),    # more blocks than a warp's registers hold the keys of
+    (1, 8, 8, 43, 60000, 60050, 16, 4),   # more than the first pass takes
+])
+def test_sparse_many_units(torch_cuda, nseq, q_heads, heads, tokens, pos, ctx, block, n_sel):
+    rng = np.random.default_rng(ctx + n_sel)
+    at = [pos - 7 * s for s in range(nseq)]
+    ref = filled(rng, nseq, heads, ctx, block, [p + tokens for p in at])
+    check_attn(torch_cuda, rng, ref, q_heads, tokens, at, n_sel=n_sel)
+
+
+def test_sparse_many_units_ragged_strided(torch_cuda):
+    """Pieces of different lengths, an idle sequence, rows past the cache's end, rows inside wider buffers."""
+    rng = np.random.default_rng(18)
+    ctx, tokens, ntok, pos = 500, 61, [61, 8, 61, 0, 70], [400, 310, 460, 33, 0xffffffff]
+    ref = filled(rng, 5, 2, ctx, 32, [461, 318, 500, 0, 500])
+    check_attn(torch_cuda, rng, ref, 10, tokens, pos, ntok, n_sel=6, ldq=13 * DIM)
+
+
+def test_sparse_many_units_ties_and_poison(torch_cuda):
+    """Equal scores go to the lower block, a poisoned block is chosen, and scores of both signs and zero are in order."""
+    torch = torch_cuda
+    rng = np.random.default_rng(19)
+    ref = RefCache(1, 4, 500, 16, rng)
+    k = rng.standard_normal((1, 16, 4, DIM)).astype(np.float32)
+    sign = np.array([1, -1, 0, 2, 1, 0, -1, 1])
+    rows = np.concatenate([k * sign[i % 8] for i in range(32)], 1)[:, :500]
+    ref.append([0], [500], rows, rng.standard_normal(rows.shape).astype(np.float32))
+    q = rng.standard_normal((1, 90, 8, DIM)).astype(np.float32)
+    q[0, 3] = 0                                   # every score 0: the lowest blocks
+    check_attn(torch, rng, ref, 8, 90, [400], n_sel=9, q=q)
+    ref.ks[0, 1, 17] = np.nan
+    sel = torch.zeros(1, 90, 4, 9, dtype=torch.int32, device="cuda")
+    out = torch.zeros(1, 90, 8, DIM, device="cuda")
+    atlas_cuda.kv8_attn_sparse(DevCache(torch, ref).c, 8, 90, 9, _i32(torch, [400]), _f32(torch, q), out, sel)
+    assert (sel[0, :, 1] == 17).any(-1).all() and torch.isnan(out[0, :, 2:4]).all()
+    assert torch.isfinite(out[0, :, :2]).all() and torch.isfinite(out[0, :, 4:]).all()
+
+
 def test_sparse_ragged_strided(torch_cuda):
     rng = np.random.default_rng(22)
     pos, ntok = [0, 310, 499, 33], [6, 2, 3, 0]
