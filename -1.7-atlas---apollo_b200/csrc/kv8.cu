@@ -1414,6 +1414,8 @@ int attn_args(const char *who, const AtlasKv8 *cache, uint32_t q_heads, uint32_t
               const uint32_t *d_ntok, const float *d_q, uint64_t ldq, float *d_out, uint64_t ldo, AttnArgs &a, int &dev,
               int &sms)
 {
+    // a row of `out` may be written before another CTA has read its neighbours in `q`
+    if (d_q && d_q == d_out) return api_fail(ATLAS_EINVAL, "%s: out must not be q", who);
     int rc = open_cache(who, cache, tokens, d_pos0, d_ntok, a.c, a.r, dev, sms);
     if (rc != ATLAS_OK) return rc;
     if (!q_heads || q_heads % cache->kv_heads || q_heads > 32768u || (uint64_t)q_heads * tokens > 0x3fffffffull)

@@ -289,7 +289,8 @@ int atlas_cuda_kv8_read(const AtlasKv8 *cache, uint32_t tokens, const uint32_t *
 /* Causal grouped-query attention: the query rows of position p attend to the
    cached positions 0 .. p (the rows of p itself must have been stored), scores
    q.k / sqrt(128), softmax in fp32, fp32-level accuracy for the values that
-   the codes stand for. q_heads is a multiple of kv_heads. */
+   the codes stand for. q_heads is a multiple of kv_heads; q and out must not
+   overlap. */
 int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
                         const uint32_t *d_ntok, const float *d_q, uint64_t ldq, float *d_out, uint64_t ldo,
                         void *stream);

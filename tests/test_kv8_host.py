@@ -41,6 +41,10 @@ def test_bad_calls_are_refused(lib, change):
     assert _calls(lib, _desc(), **change) == [EINVAL] * 4
 
 
+def test_attention_in_place_is_refused(lib):
+    assert _calls(lib, _desc(), rows=0x300)[2:] == [EINVAL] * 2
+
+
 def test_null_cache_is_refused(lib):
     assert _calls(lib, None) == [EINVAL] * 4
 
