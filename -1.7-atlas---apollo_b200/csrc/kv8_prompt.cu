@@ -36,9 +36,13 @@
 // Few rows over many positions: the positions are split over a cluster of CTAs,
 // and each merges a share of the rows through distributed shared memory.
 //
-// Bound by the tensor pipe (4096 cycles per 256 rows x 128 keys) next to the
-// softmax's issue slots. Every wait is bounded; after a timeout the CTA's rows
-// are NaN.
+// 256 rows x 128 keys take 6700 cycles, of which the MMAs alone are 4130; with
+// neither softmax nor conversion the chain of barriers leaves 5700, and the
+// conversions, the softmax and the move of the segments (128 KB through L2 every
+// 8 tiles, while the MMAs wait) add about 300 each. 8192 tokens of 40 heads on 8
+// run 1130 us, 73 % of the measured binary16-rate peak for two products, and 1310
+// us when repeated until the power cap lowers the clock.
+// Every wait is bounded; after a timeout the CTA's rows are NaN.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -53,14 +57,19 @@ constexpr uint32_t kTileRows = 128, kTileKeys = 128;
 constexpr uint32_t kMaxSplit = 8;                  // CTAs that share the positions of a tile's rows
 constexpr uint32_t kConvWarp = 16, kMmaWarp = 20, kPromptThreads = 21 * 32;   // first converter, the MMA warp
 // Tensor cores truncate their sums: per tile of keys (16 steps) the output
-// loses 3.7e-7 of itself on average, 2e-5 over 8192 positions. So a segment of
-// eight tiles is summed in tensor memory, made up for the average loss, and
-// added to the earlier ones with rounding: at most 1.9e-6 over any number of
-// positions up to 32300, where one sum for all tiles measured 7.5e-5. Segments
-// of 4 / 8 / 16 tiles: 1234 / 1125 / 1072 us for 2048 rows of 5 heads over 8192
-// positions, errors 1.0e-6 / 1.4e-6 / 2.6e-6.
-constexpr uint32_t kSegment = 8;
-constexpr float kLoss = 3.7e-7f;
+// loses 5.6e-7 of itself on average while it grows, 2e-5 over 8192 positions. So
+// a segment of eight tiles is summed in tensor memory and added to the earlier
+// ones with rounding, and what is lost on average is made up for every two
+// tiles, in place or with the move: errors of 1.0e-6 over 8192 positions and
+// 1.5e-6 over 32300, where one sum for all tiles had 2.0e-5 and 7.5e-5. Where a
+// row's later weights in a segment are zeros, nothing is lost, and 4.5e-6 at most
+// is made up for nothing. 8192 tokens of 40 heads on 8: segments of 4 / 8 / 16
+// tiles 1234 / 1125 / 1072 us, errors 1.0e-6 / 1.4e-6 / 2.6e-6 without the
+// amends in place, which take 10 us. (Sums in registers instead, one thread per
+// row with 200 of them, registers moved between the warps: 1175 us, and 512
+// tokens of 28 heads on 4 21.6 instead of 18.9 us.)
+constexpr uint32_t kSegment = 8, kAmends = 2;
+constexpr float kLoss = 5.6e-7f;
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 binary16, swizzled
 constexpr uint32_t kQTile = 4 * kHalf;             // one tile's Q: [hi, lo][2 x 64 dimensions]
 
@@ -595,7 +604,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 if (turn && turn % kSegment == 0u) {   // while the next scores are made
                     ok = ok && wait_warp(&b.o_full[t], (turn / kSegment - 1u) & 1u, err);
                     fence_after();
-                    constexpr float kGain = 1.0f + kLoss * kSegment;
+                    constexpr float kGain = 1.0f + kLoss * kAmends;
 #pragma unroll 1
                     for (uint32_t c = 0; ok && c < 4u; ++c) {
                         float o[16];
@@ -642,7 +651,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 float x = -INFINITY;
                 if (ok) x = masked ? tile_max<true>(at, f, nvis) : tile_max<false>(at, f, 64);
                 const bool raise = meet_any(1u + t, 256u, x > m + kLazy);
-                if (raise || fv != 1.0f) {
+                const bool amends = turn % kSegment && turn % kAmends == 0u;
+                if (raise || fv != 1.0f || amends) {
                     if (raise) {
                         b.half[t][half][row] = x;
                         meet(1u + t, 256u);
@@ -654,9 +664,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                         l *= fm;
                         fv *= fm;
                     }
-                    if (turn >= kSegment)
+                    if (turn >= kSegment && __any_sync(0xffffffffu, fv != 1.0f))
 #pragma unroll 1
                         for (uint32_t c = 0; c < 16u; ++c) acc[c] = make_float4(acc[c].x * fv, acc[c].y * fv, acc[c].z * fv, acc[c].w * fv);
+                    if (amends) fv *= 1.0f + kLoss * kAmends;
                     if (turn % kSegment && ok) {
 #pragma unroll 1
                         for (uint32_t c = 0; c < 64u; c += 16u) {
@@ -685,7 +696,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             // the output into Q's place: row-major, 16-byte chunks XORed with the row
             const bool have = turn && ok && wait_warp(&b.o_full[t], ((turn - 1u) / kSegment) & 1u, err);
             fence_after();
-            const float gain = 1.0f + kLoss * (float)((turn - 1u) % kSegment + 1u);
+            const float gain = 1.0f + kLoss * (float)((turn - 1u) % kAmends + 1u);
             const float back = __uint_as_float(vref) * (1.0f / 64.0f) * (one || C > 1u ? 1.0f : 1.0f / l);
             float4 *stage = reinterpret_cast<float4 *>(qs + t * kQTile);
 #pragma unroll 1

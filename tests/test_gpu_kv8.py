@@ -374,6 +374,30 @@ def test_prompt_segments(torch_cuda, q_heads, tokens, ctx, rising):
     check_attn(torch_cuda, rng, ref, q_heads, tokens, [ctx - tokens], q=q)
 
 
+@pytest.mark.parametrize("heads,q_heads,tokens", [(2, 2, 1), (1, 1, 200), (1, 64, 300)])
+@pytest.mark.parametrize("at", [0, 100, 700, 2100])
+def test_attn_of_one_position(torch_cuda, heads, q_heads, tokens, at):
+    """One position takes all the weight, every other one rounds to none: the output is its value. With u = 2^-24, off by
+    what a segment's sums are made up for though nothing was lost, 4.5e-6 = 75 u, and 24 u for the value's two terms, their
+    scales and the states' merges."""
+    torch, ctx = torch_cuda, 2500
+    rng = np.random.default_rng(20)
+    ref = RefCache(1, heads, ctx, 64, rng)
+    k = np.zeros((1, ctx, heads, DIM), np.float32)
+    k[..., 0] = -1.0
+    k[:, at, :, 0] = 1.0
+    ref.append([0], [ctx], k, rng.uniform(0.5, 1.0, k.shape).astype(np.float32))
+    q = torch.zeros(1, tokens, q_heads, DIM, device="cuda")
+    q[..., 0] = 2000.0
+    out = torch.zeros_like(q)
+    atlas_cuda.kv8_attn(DevCache(torch, ref).c, q_heads, tokens, _i32(torch, [ctx - tokens]), q, out)
+    got = out.cpu().numpy().astype(np.float64)[0]
+    for h in range(heads):
+        want = ref.values(0, h, ctx)[1][at]
+        rows = got[:, h * q_heads // heads:(h + 1) * q_heads // heads]
+        assert (np.abs(rows / want - 1) <= 99 * 2.0 ** -24).all()
+
+
 @pytest.mark.parametrize("heads,q_heads,tokens", [(8, 8, 1), (1, 1, 200), (1, 64, 300)])
 def test_attn_sums_keep_their_precision(torch_cuda, heads, q_heads, tokens):
     """Equal weights over values of one sign. Relative to the output, with u = 2^-24: tensor cores truncate each of the 128
