@@ -22,7 +22,9 @@ int api_device(int device, int *sms);
 
 namespace k8 {
 
-cudaError_t launch_prompt(AttnArgs a, int dev, int sms, cudaStream_t stream);   // kv8_prompt.cu
+// kv8_prompt.cu
+PromptCut prompt_cut(const AttnArgs &a, int sms);
+cudaError_t launch_prompt(AttnArgs a, const PromptCut &cut, int dev, int sms, cudaStream_t stream);
 
 namespace {
 
@@ -235,7 +237,6 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
 // copy rate, instruction issue at 64 %), by launch, first-byte latency and the
 // chain of one chunk for short ones (640 positions 4.9 us, 8448 10.2 us).
 
-constexpr uint32_t kFewRows = 48;   // query rows of a KV head up to which this form is taken
 constexpr uint32_t kStages = 3;
 constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;   // block selection
 constexpr uint32_t kSlot = 8 * 32 * 16;                     // bytes of a chunk: 16 rows of K and V
@@ -1296,7 +1297,7 @@ int check_rows(const char *who, const void *p, const void *q, uint32_t heads, ui
         return api_fail(ATLAS_EINVAL, "%s: token rows %llu floats apart: at least heads x 128, a multiple of 4", who,
                         (unsigned long long)ld);
     if (!aligned(p, 16) || !aligned(q, 16)) return api_fail(ATLAS_EINVAL, "%s: token rows must be 16-byte aligned", who);
-    if (!on_device(p, dev) || !on_device(q, dev))
+    if (!on_device(p, dev) || (q != p && !on_device(q, dev)))
         return api_fail(ATLAS_EINVAL, "%s: token rows must be memory of the current device", who);
     return ATLAS_OK;
 }
@@ -1345,6 +1346,22 @@ cudaError_t launch_attn(const FewArgs &a, int dev, int sms, cudaStream_t stream)
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
     const uint32_t C = cluster_of<attn_kernel<NT, W>>(dev, W * 32, sizeof(Smem<NT, W>), units, a.c.max_context, NT == 1);
     return launch(attn_kernel<NT, W>, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), W * 32, sizeof(Smem<NT, W>), C, a, sms, stream);
+}
+
+// The longest CTA's time in cycles for more than eight rows, to be compared with
+// the prompt form's: 18.5 per position of a tile of 16 rows (8 warps), 9000
+// before and after. Rows: this form, the prompt form, in us: one sequence of 28
+// heads on 4, 500 positions, 112: 7.2, 20.7; 8000, 42 and 112: 16.4, 32.1 and
+// 26.7, 34.0; 40 heads on 8, 30000, 40 and 65: 82, 101 and 160, 103; 8 sequences
+// of them, 2000, 20 and 35: 26, 32 and 50, 32; 16000: 165, 205 and 328, 205.
+uint64_t few_cycles(const FewArgs &a, int dev)
+{
+    constexpr auto kernel = attn_kernel<2, 8>;
+    if (allow<kernel>(dev, (int)kMaxSmem) != cudaSuccess) return 0;   // the launch will say so
+    const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
+    const uint32_t C = cluster_of<kernel>(dev, 256, sizeof(Smem<2, 8>), units, a.c.max_context, false);
+    const uint64_t at_once = std::max(clusters_at_once<kernel>(dev, C, 256, sizeof(Smem<2, 8>)), 1u);
+    return (units + at_once - 1) / at_once * ((a.c.max_context + C - 1) / C) * 37 / 2 + 9000;
 }
 
 template <int NT>
@@ -1448,10 +1465,13 @@ extern "C" int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint
     int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
     if (rc != ATLAS_OK || !tokens) return rc;
     const uint32_t rows = tokens * a.group;
-    if (rows > kFewRows) return done(who, launch_prompt(a, dev, sms, (cudaStream_t)stream));
-    if ((rc = map_codes(who, a)) != ATLAS_OK) return rc;
     const bool one = rows <= 8;
     a.tiles = one ? 1 : (rows + 15) / 16;
+    if (!one) {
+        const PromptCut cut = prompt_cut(a, sms);
+        if (cut.cycles < few_cycles(a, dev)) return done(who, launch_prompt(a, cut, dev, sms, (cudaStream_t)stream));
+    }
+    if ((rc = map_codes(who, a)) != ATLAS_OK) return rc;
     return done(who, one ? launch_attn<1, 16>(a, dev, sms, (cudaStream_t)stream)
                          : launch_attn<2, 8>(a, dev, sms, (cudaStream_t)stream));
 }

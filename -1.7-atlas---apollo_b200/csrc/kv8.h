@@ -46,6 +46,12 @@ struct AttnArgs {
     uint32_t early;                   // the successor may start at once
 };
 
+// The prompt form's tiles of 128 rows per CTA, CTAs that share a unit's positions, and estimated time
+struct PromptCut {
+    uint32_t tiles, split;
+    uint64_t cycles;
+};
+
 __device__ __forceinline__ uint32_t row_count(const Rows &r, uint32_t s)
 {
     return r.n_tok ? min(__ldcg(r.n_tok + s), r.tokens) : r.tokens;

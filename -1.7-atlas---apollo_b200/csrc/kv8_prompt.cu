@@ -846,32 +846,41 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 
 }  // namespace
 
-// Attention of many query rows; see AttnArgs. a.tiles is set here.
-cudaError_t launch_prompt(AttnArgs a, int dev, int sms, cudaStream_t stream)
+// How a call is cut up, and an estimate of its longest CTA's time in cycles.
+// Two tiles per CTA, or one; and up to 8 CTAs per unit, two tiles of keys each
+// at least. What does not fit the device at once takes two tiles and whole
+// units; what does goes by the time: a tile of keys takes 5700 cycles with one
+// tile of rows and 6300 with two, what is before and after 11000 and 18000, a
+// merge of two tiles 10000 (of one, nothing that shows). Measured on 333 tokens
+// over 5001 positions (44 units of two tiles: 160 / 89 / 67 us as 1 / 2 / 3 CTAs,
+// 84 of one: 133 / 73 us) and 512 tokens (112 units of one tile 18.9 us, 56 of
+// two 23.6 us, as 2 CTAs each 20.5 us).
+PromptCut prompt_cut(const AttnArgs &a, int sms)
 {
-    cudaError_t e = allow<prompt_kernel>(dev, (int)kPromptSmem);
-    if (e != cudaSuccess) return e;
-    // Two tiles per CTA, or one; and up to 8 CTAs per unit, two tiles of keys
-    // each at least. What does not fit the device at once takes two tiles and
-    // whole units. What does goes by the longest unit's time, in cycles: 2500
-    // for one tile of rows against a tile of keys, 5600 for two; 12000 and
-    // 16000 before and after the loop, and 5000 per tile of rows for a merge.
     const uint32_t rows = a.r.tokens * a.group, keys = (a.c.max_context + kTileKeys - 1) / kTileKeys;
     const uint64_t heads = (uint64_t)a.c.kv_heads * a.c.nseq;
-    uint32_t C = 1;
-    uint64_t best = ~0ull;
-    a.cta_tiles = 2;
+    PromptCut best{2u, 1u, ~0ull};
     for (uint32_t t = 1; t <= 2; ++t) {
         const uint64_t units = (rows + t * kTileRows - 1) / (t * kTileRows) * heads;
         for (uint32_t c = 1; c <= kMaxSplit && units * c <= (uint64_t)sms && (c == 1 || 2 * c <= keys); ++c) {
-            const uint64_t cost = (uint64_t)(t == 1 ? 2500 : 5600) * ((keys + c - 1) / c) + 8000 + 4000 * t + (c > 1 ? 5000 * t : 0);
-            if (cost < best) {
-                best = cost;
-                a.cta_tiles = t;
-                C = c;
-            }
+            const uint64_t cycles = (uint64_t)(t == 1 ? 5700 : 6300) * ((keys + c - 1) / c) + (t == 1 ? 11000 : c == 1 ? 18000 : 28000);
+            if (cycles < best.cycles) best = PromptCut{t, c, cycles};
         }
     }
+    if (best.cycles == ~0ull) {
+        const uint64_t units = (rows + 2u * kTileRows - 1) / (2u * kTileRows) * heads;
+        best.cycles = (units + (uint64_t)sms - 1) / (uint64_t)sms * (6300ull * keys + 18000ull);
+    }
+    return best;
+}
+
+// Attention of many query rows; see AttnArgs
+cudaError_t launch_prompt(AttnArgs a, const PromptCut &cut, int dev, int sms, cudaStream_t stream)
+{
+    cudaError_t e = allow<prompt_kernel>(dev, (int)kPromptSmem);
+    if (e != cudaSuccess) return e;
+    const uint32_t rows = a.r.tokens * a.group, C = cut.split;
+    a.cta_tiles = cut.tiles;
     a.tiles = (rows + a.cta_tiles * kTileRows - 1) / (a.cta_tiles * kTileRows);
     return launch(prompt_kernel, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), kPromptThreads, kPromptSmem, C, a, sms, stream);
 }

@@ -354,6 +354,7 @@ def test_attn_many_positions(torch_cuda):
     (60, 150, 2500),      # one tile per CTA, the two groups of warps take turns at the keys
     (8, 7, 19000),        # over a cluster
     (1, 150, 20000),
+    (64, 60, 12000),
 ])
 @pytest.mark.parametrize("rising", [False, True])
 def test_prompt_segments(torch_cuda, q_heads, tokens, ctx, rising):
@@ -372,6 +373,59 @@ def test_prompt_segments(torch_cuda, q_heads, tokens, ctx, rising):
         ref = RefCache(1, 1, ctx, 64, rng)
         ref.append([0], [ctx], k, v)
     check_attn(torch_cuda, rng, ref, q_heads, tokens, [ctx - tokens], q=q)
+
+
+# Enough units of work for the prompt form also over few positions: 8 sequences, 2 KV heads, 600 rows each.
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_wide_prompts(torch_cuda, block):
+    """Pieces of different lengths, an idle sequence, rows past the cache's end, rows inside wider buffers."""
+    rng = np.random.default_rng(block)
+    ctx, tokens, pos = 300, 150, [0, 150, 77, 33, 299, 128, 200, 0xfffffff0]
+    ntok = [150, 150, 149, 0, 150, 1, 190, 150]
+    ref = filled(rng, 8, 2, ctx, block, [min(ctx, p + n) for p, n in zip(pos, ntok)])
+    check_attn(torch_cuda, rng, ref, 8, tokens, pos, ntok, ldq=11 * DIM)
+
+
+@pytest.mark.parametrize("q_heads,tokens", [(2, 600), (14, 90), (130, 9)])
+def test_wide_prompt_groups(torch_cuda, q_heads, tokens):
+    rng = np.random.default_rng(q_heads)
+    ref = filled(rng, 8, 2, 640, 32, [640] * 8)
+    check_attn(torch_cuda, rng, ref, q_heads, tokens, [640 - tokens - 5 * s for s in range(8)])
+
+
+@pytest.mark.parametrize("q_size,k_size,v_spread", [(30.0, 3.0, 0.5), (1e-3, 1.0, 0.5), (1.0, 1.0, 4.0), (1e-30, 1e10, 0.1),
+                                                    (1e8, 1e-8, 0.1)])
+def test_wide_prompt_sizes(torch_cuda, q_size, k_size, v_spread):
+    rng = np.random.default_rng(31)
+    ref = filled(rng, 8, 2, 300, 16, [300] * 8, v_spread=v_spread, k_size=k_size)
+    q = (q_size * rng.standard_normal((8, 150, 8, DIM))).astype(np.float32)
+    check_attn(torch_cuda, rng, ref, 8, 150, [150] * 8, q=q)
+
+
+def test_wide_prompt_zeros_and_non_finite(torch_cuda):
+    """Blocks of zeros, queries of zeros; a poisoned block of K or V shows in the rows that attend to it and in no other, a
+    query row with a NaN or an infinity is NaN alone."""
+    torch = torch_cuda
+    rng = np.random.default_rng(32)
+    ref = RefCache(8, 2, 300, 16, rng)
+    x = rng.standard_normal((8, 300, 2, DIM)).astype(np.float32)
+    x[:, :32] = 0
+    x[:, 64:80] = 0
+    ref.append([0] * 8, [300] * 8, x, x)
+    q = rng.standard_normal((8, 150, 8, DIM)).astype(np.float32)
+    q[:, :, 1] = 0
+    want, _ = check_attn(torch, rng, ref, 8, 150, [100] * 8, q=q)
+    ref.ks[2, 0, 12] = ref.vs[3, 1, 12] = np.nan      # positions 192 .. 207: tokens from 92 on
+    q[5, 7, 3, 5], q[6, 149, 6, 100] = np.nan, np.inf
+    out = torch.zeros(8, 150, 8, DIM, device="cuda")
+    atlas_cuda.kv8_attn(DevCache(torch, ref).c, 8, 150, _i32(torch, [100] * 8), _f32(torch, q), out)
+    got = out.cpu().numpy()
+    bad = np.zeros(got.shape[:3], bool)
+    bad[2, 92:, :4] = bad[3, 92:, 4:] = bad[5, 7, 3] = bad[6, 149, 6] = True
+    assert np.isnan(got[bad]).all()
+    np.testing.assert_array_equal(got[~bad], want[~bad])
 
 
 @pytest.mark.parametrize("heads,q_heads,tokens", [(2, 2, 1), (1, 1, 200), (1, 64, 300)])
