@@ -1351,9 +1351,9 @@ cudaError_t launch_attn(const FewArgs &a, int dev, int sms, cudaStream_t stream)
 // The longest CTA's time in cycles for more than eight rows, to be compared with
 // the prompt form's: 18.5 per position of a tile of 16 rows (8 warps), 9000
 // before and after. Rows: this form, the prompt form, in us: one sequence of 28
-// heads on 4, 500 positions, 112: 7.2, 20.7; 8000, 42 and 112: 16.4, 32.1 and
-// 26.7, 34.0; 40 heads on 8, 30000, 40 and 65: 82, 101 and 160, 103; 8 sequences
-// of them, 2000, 20 and 35: 26, 32 and 50, 32; 16000: 165, 205 and 328, 205.
+// heads on 4, 500 positions, 112: 7.2, 19; 8000, 42 and 112: 16.4, 27 and 26.7,
+// 28; 40 heads on 8, 30000, 40 and 65: 82, 83 and 160, 83; 8 sequences of them,
+// 2000, 20 and 35: 26, 28 and 50, 28; 16000: 165, 161 and 328, 161.
 uint64_t few_cycles(const FewArgs &a, int dev)
 {
     constexpr auto kernel = attn_kernel<2, 8>;

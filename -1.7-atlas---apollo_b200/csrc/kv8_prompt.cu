@@ -27,7 +27,9 @@
 //          same tile, so that one tile's softmax runs under the other's MMAs.
 // Where few rows leave SMs idle, a CTA takes one tile of 128 rows: both softmax
 // groups then have the same rows and take turns at the tiles of keys, each with
-// an output and a state of its own, which are merged at the end.
+// an output and a state of its own, which are merged at the end. The place of the
+// second tile's Q holds a second buffer of K and one of V then, group 1's (5700
+// cycles per tile of keys with one buffer, 4400 with two).
 // Tensor memory: 2 x 128 columns of scores / weights, 2 x 128 of output (of up to
 // kSegment tiles of keys; the softmax warps hold the sum of the earlier ones).
 // Shared memory: Q hi / lo 128 KB, K 32 KB, V 32 KB, their next codes 32 KB; Q's
@@ -40,7 +42,7 @@
 // neither softmax nor conversion the chain of barriers leaves 5700, and the
 // conversions, the softmax and the move of the segments (128 KB through L2 every
 // 8 tiles, while the MMAs wait) add about 300 each. 8192 tokens of 40 heads on 8
-// run 1130 us, 73 % of the measured binary16-rate peak for two products, and 1310
+// run 1150 us, 72 % of the measured binary16-rate peak for two products, and 1310
 // us when repeated until the power cap lowers the clock.
 // Every wait is bounded; after a timeout the CTA's rows are NaN.
 #include <algorithm>
@@ -67,14 +69,15 @@ constexpr uint32_t kConvWarp = 16, kMmaWarp = 20, kPromptThreads = 21 * 32;   //
 // tiles 1234 / 1125 / 1072 us, errors 1.0e-6 / 1.4e-6 / 2.6e-6 without the
 // amends in place, which take 10 us. (Sums in registers instead, one thread per
 // row with 200 of them, registers moved between the warps: 1175 us, and 512
-// tokens of 28 heads on 4 21.6 instead of 18.9 us.)
+// tokens of 28 heads on 4 3 us more.)
 constexpr uint32_t kSegment = 8, kAmends = 2;
 constexpr float kLoss = 5.6e-7f;
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 binary16, swizzled
 constexpr uint32_t kQTile = 4 * kHalf;             // one tile's Q: [hi, lo][2 x 64 dimensions]
 
 struct PromptBars {
-    uint64_t s_full[2], p_full[2], o_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full, fin;   // [tile], [half]
+    uint64_t s_full[2], p_full[2], o_full[2];                                       // [tile]
+    uint64_t k_full[2][2], k_empty[2][2], v_full[2][2], v_empty[2][2], q_full, fin;   // [buffer][half]
     uint32_t tmem, status;
     // what a score of the row is worth, in the exponent's base 2 (in [tile][0], until the first exchange);
     // then the two threads of a row exchange their maxima and sums here
@@ -330,10 +333,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             mbar_init(&b.s_full[t], 1u);
             mbar_init(&b.p_full[t], 8u);
             mbar_init(&b.o_full[t], 1u);
-            mbar_init(&b.k_full[t], 4u);
-            mbar_init(&b.v_full[t], 2u);
-            mbar_init(&b.k_empty[t], 1u);
-            mbar_init(&b.v_empty[t], 1u);
+            for (int hf = 0; hf < 2; ++hf) {
+                mbar_init(&b.k_full[t][hf], 4u);
+                mbar_init(&b.v_full[t][hf], 2u);
+                mbar_init(&b.k_empty[t][hf], 1u);
+                mbar_init(&b.v_empty[t][hf], 1u);
+            }
         }
         mbar_init(&b.q_full, kConvWarp);
         mbar_init(&b.fin, 1u);
@@ -367,6 +372,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         n = base + (rank < more ? 1u : 0u);
     }
     const size_t head = (size_t)s * a.c.kv_heads + h;
+    // K's and V's buffer for tile of keys j, and how often it was used before
+    auto buffer = [&](uint32_t j) { return one ? j & 1u : 0u; };
+    auto uses = [&](uint32_t j) { return one ? j >> 1 : j; };
+    uint8_t *const ks2 = qs + kQTile, *const vs2 = ks2 + 2 * kHalf;
 
     float row_m = -INFINITY, row_l = 0.f;   // softmax threads of half 0: their row's state, for the cluster
 
@@ -374,26 +383,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         // ------------------------------------------------------------- MMA --
         if (elected()) {
             // a step of 16 along K is 32 bytes, 2 in a descriptor; 4 steps fill a swizzled tile
-            const uint64_t qd = operand(smem_addr(qs)), kd = operand(smem_addr(ks)), vd = operand(smem_addr(vs));
+            const uint64_t qd = operand(smem_addr(qs)), kd[2] = {operand(smem_addr(ks)), operand(smem_addr(ks2))},
+                           vd[2] = {operand(smem_addr(vs)), operand(smem_addr(vs2))};
             // K and V go by halves (64 dimensions, 64 keys): a half is converted
             // while the MMAs still read, or already read, the other.
             bool ok = n != 0u && mbar_wait(&b.q_full, 0u, err);
             // scores of keys j against Q tile `qt` into S of group t; P V of keys j into the group's output
             auto scores = [&](uint32_t t, uint32_t qt, uint32_t j, bool first_use, bool last_use) {
-                const uint64_t q = qd + (uint64_t)(qt * (kQTile >> 4));
+                const uint64_t q = qd + (uint64_t)(qt * (kQTile >> 4)), k = buffer(j) ? kd[1] : kd[0];
 #pragma unroll
                 for (uint32_t hf = 0; hf < 2u; ++hf) {
                     if (first_use) {
-                        if (!(ok = ok && mbar_wait(&b.k_full[hf], j & 1u, err))) return;
+                        if (!(ok = ok && mbar_wait(&b.k_full[buffer(j)][hf], uses(j) & 1u, err))) return;
                         fence_after();
                     }
 #pragma unroll
                     for (uint32_t st = 0; st < 4u; ++st) {
                         const uint32_t off = hf * (kHalf >> 4) + st * 2u;
-                        mma_ss(tmem + 128u * t, q + off, kd + off, hf != 0u || st != 0u);
-                        mma_ss(tmem + 128u * t, q + (2u * kHalf >> 4) + off, kd + off, 1u);
+                        mma_ss(tmem + 128u * t, q + off, k + off, hf != 0u || st != 0u);
+                        mma_ss(tmem + 128u * t, q + (2u * kHalf >> 4) + off, k + off, 1u);
                     }
-                    if (last_use) commit(&b.k_empty[hf]);
+                    if (last_use) commit(&b.k_empty[buffer(j)][hf]);
                 }
                 commit(&b.s_full[t]);
             };
@@ -401,16 +411,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 if (!(ok = ok && mbar_wait(&b.p_full[t], turn & 1u, err))) return;
 #pragma unroll
                 for (uint32_t hf = 0; hf < 2u; ++hf) {
-                    if (first_use && !(ok = ok && mbar_wait(&b.v_full[hf], j & 1u, err))) return;
+                    if (first_use && !(ok = ok && mbar_wait(&b.v_full[buffer(j)][hf], uses(j) & 1u, err))) return;
                     fence_after();
 #pragma unroll
                     for (uint32_t st = 0; st < 4u; ++st) {
-                        const uint64_t v = vd + hf * (kHalf >> 4) + st * 2u;
+                        const uint64_t v = (buffer(j) ? vd[1] : vd[0]) + hf * (kHalf >> 4) + st * 2u;
                         const uint32_t p = tmem + 128u * t + 64u * hf + 16u * st;
                         mma_ts(tmem + 256u + 128u * t, p, v, turn % kSegment != 0u || hf != 0u || st != 0u);
                         mma_ts(tmem + 256u + 128u * t, p + 8u, v, 1u);
                     }
-                    if (last_use) commit(&b.v_empty[hf]);
+                    if (last_use) commit(&b.v_empty[buffer(j)][hf]);
                 }
             };
             if (one) {   // the groups take turns at the keys
@@ -474,11 +484,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         copy_k(0u);
         copy_v(0u);
         for (uint32_t j = 0; j < n; ++j) {
+            const uint32_t buf = buffer(j), used = uses(j);
             copy_wait1();   // K of this tile; V may still be on its way
             bool ok = true;
 #pragma unroll
             for (uint32_t hf = 0; hf < 2u; ++hf) {
-                if (j && !(ok = ok && wait_warp(&b.k_empty[hf], (j - 1u) & 1u, err))) break;
+                if (used && !(ok = ok && wait_warp(&b.k_empty[buf][hf], (used - 1u) & 1u, err))) break;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
                     const uint32_t row = 32u * i + 8u * w + l8;
@@ -490,19 +501,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                         o[2 * q] = codes_h2<false>(__byte_perm(words[q], 0u, 0x4140u));
                         o[2 * q + 1] = codes_h2<false>(__byte_perm(words[q], 0u, 0x4342u));
                     }
-                    uint8_t *dst = ks + hf * kHalf;
+                    uint8_t *dst = (buf ? ks2 : ks) + hf * kHalf;
                     *reinterpret_cast<uint4 *>(dst + swizzled(row, 2u * q8)) = make_uint4(o[0], o[1], o[2], o[3]);
                     *reinterpret_cast<uint4 *>(dst + swizzled(row, 2u * q8 + 1u)) = make_uint4(o[4], o[5], o[6], o[7]);
                 }
                 fence_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&b.k_full[hf]);
+                if (lane == 0) mbar_arrive(&b.k_full[buf][hf]);
             }
             if (!ok) break;
             copy_k(j + 1u);
             copy_wait1();   // V of this tile; warps 0, 1 have its first 64 keys, 2, 3 the others
-            if (j && !wait_warp(&b.v_empty[w >> 1], (j - 1u) & 1u, err)) break;
-            uint8_t *dst = vs + (w >> 1) * kHalf;
+            if (used && !wait_warp(&b.v_empty[buf][w >> 1], (used - 1u) & 1u, err)) break;
+            uint8_t *dst = (buf ? vs2 : vs) + (w >> 1) * kHalf;
             uint4 y[8];
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) y[i] = vslot[128u * i];
@@ -527,7 +538,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             }
             fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.v_full[w >> 1]);
+            if (lane == 0) mbar_arrive(&b.v_full[buf][w >> 1]);
             copy_v(j + 1u);
         }
         copy_wait0();
@@ -849,12 +860,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 // How a call is cut up, and an estimate of its longest CTA's time in cycles.
 // Two tiles per CTA, or one; and up to 8 CTAs per unit, two tiles of keys each
 // at least. What does not fit the device at once takes two tiles and whole
-// units; what does goes by the time: a tile of keys takes 5700 cycles with one
-// tile of rows and 6300 with two, what is before and after 11000 and 18000, a
+// units; what does goes by the time: a tile of keys takes 4400 cycles with one
+// tile of rows and 6300 with two, what is before and after 14500 and 18000, a
 // merge of two tiles 10000 (of one, nothing that shows). Measured on 333 tokens
-// over 5001 positions (44 units of two tiles: 160 / 89 / 67 us as 1 / 2 / 3 CTAs,
-// 84 of one: 133 / 73 us) and 512 tokens (112 units of one tile 18.9 us, 56 of
-// two 23.6 us, as 2 CTAs each 20.5 us).
+// over 5001 positions (44 units of two tiles: 160 / 89 / 67 us as 1 / 2 / 3
+// CTAs), 64 units of one tile as 2 CTAs each (2000 and 16000 positions: 28 and
+// 161 us) and 512 tokens (112 units of one tile 17.3 us, 56 of two 23.6 us, as 2
+// CTAs each 20.5 us).
 PromptCut prompt_cut(const AttnArgs &a, int sms)
 {
     const uint32_t rows = a.r.tokens * a.group, keys = (a.c.max_context + kTileKeys - 1) / kTileKeys;
@@ -863,7 +875,7 @@ PromptCut prompt_cut(const AttnArgs &a, int sms)
     for (uint32_t t = 1; t <= 2; ++t) {
         const uint64_t units = (rows + t * kTileRows - 1) / (t * kTileRows) * heads;
         for (uint32_t c = 1; c <= kMaxSplit && units * c <= (uint64_t)sms && (c == 1 || 2 * c <= keys); ++c) {
-            const uint64_t cycles = (uint64_t)(t == 1 ? 5700 : 6300) * ((keys + c - 1) / c) + (t == 1 ? 11000 : c == 1 ? 18000 : 28000);
+            const uint64_t cycles = (uint64_t)(t == 1 ? 4400 : 6300) * ((keys + c - 1) / c) + (t == 1 ? 14500 : c == 1 ? 18000 : 28000);
             if (cycles < best.cycles) best = PromptCut{t, c, cycles};
         }
     }
