@@ -543,12 +543,17 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
                     mma_s8(d[pl], ka[2], hi.x, hi.y);
                     mma_s8(d[pl], ka[3], hi.z, hi.w);
                 }
-                const float f[2] = {sk * qs[nt][0], sk * qs[nt][1]};
+                const uint64_t f = pair(sk * qs[nt][0], sk * qs[nt][1]);
+                const uint64_t big = pair(-12582912.0f, -12582912.0f), step = pair(1.0f / 254.0f, 1.0f / 254.0f);
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    uint64_t v[3];
+#pragma unroll
+                    for (int pl = 0; pl < 3; ++pl) v[pl] = add2(pair(__int_as_float(d[pl][e]), __int_as_float(d[pl][e + 1])), big);
+                    unpair(mul2(fma2(fma2(v[2], step, v[1]), step, v[0]), f), y[nt][e], y[nt][e + 1]);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float big = 12582912.0f;
-                    const float x = fmaf(__int_as_float(d[2][e]) - big, 1.0f / 254.0f, __int_as_float(d[1][e]) - big);
-                    y[nt][e] = fmaf(x, 1.0f / 254.0f, __int_as_float(d[0][e]) - big) * f[e & 1];
                     if (masked && (e < 2 ? pa : pb) > last[nt][e & 1]) y[nt][e] = -INFINITY;
                     raise |= y[nt][e] > m[nt][e & 1] + kLazy;
                 }

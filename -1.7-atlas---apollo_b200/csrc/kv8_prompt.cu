@@ -227,27 +227,6 @@ __device__ __forceinline__ float tile_max(uint32_t at, const float (&f)[4], int 
     return m;
 }
 
-// Two floats in one register pair, for the packed fp32 instructions
-__device__ __forceinline__ uint64_t pair(float a, float b)
-{
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-    return d;
-}
-__device__ __forceinline__ void unpair(uint64_t d, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 // The weights into the scores' columns, 16 keys at a time: 8 columns of hi, 8
 // of lo. The V scale over vref enters the exponent: lg[i] is its base-2
 // logarithm for group i, and ipf[i], its reciprocal, takes it out of the
