@@ -241,7 +241,9 @@ constexpr uint32_t kStages = 3;
 constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;   // block selection
 constexpr uint32_t kSlot = 8 * 32 * 16;                     // bytes of a chunk: 16 rows of K and V
 
-constexpr uint32_t kMaxCluster = 16;                        // also the states that a CTA receives: C ceil(8 NT / C)
+constexpr uint32_t kMaxCluster = 16;
+// The states that a CTA receives at most, C ceil(8 NT / C) over the sizes of a cluster: 16, or 30 at C = 15
+constexpr uint32_t received(int NT) { return NT == 1 ? 16u : 30u; }
 constexpr uint32_t kRecStride = kDim + 4;                   // output, maximum, sum
 constexpr int kSumBits = 0x4B400000;                  // 2^23 + 2^22: integer sums below 2^22 read as floats
 
@@ -329,7 +331,7 @@ struct alignas(1024) Smem {
         uint8_t ring[W][kStages][kSlot];
         float wrec[W][8 * NT][kRecStride];     // the warps' outputs, once the ring is done with
     } u;
-    float rec[W < 8 ? 1 : kMaxCluster][kRecStride];   // the states that the cluster's CTAs send of this CTA's rows (W < 8: no cluster)
+    float rec[W < 8 ? 1 : received(NT)][kRecStride];   // the states that the cluster's CTAs send of this CTA's rows (W < 8: no cluster)
     uint64_t full[W][kStages];                 // a chunk has landed
     uint32_t err;
     float2 wml[W][8 * NT];                     // the warps' maxima and sums
@@ -1231,13 +1233,12 @@ uint32_t clusters_at_once(int dev, uint32_t c, uint32_t threads, size_t smem)
 // CTAs per unit of work: the largest cluster of which all units are on the
 // device at once (a second wave costs more than the smaller share saves: 8
 // units of 8447 positions take 16.2 us as clusters of 16, of which 7 fit, and
-// 11.0 us as clusters of 8), with 128 positions per CTA at least. `any`: not
-// only powers of two.
+// 11.0 us as clusters of 8), with 128 positions per CTA at least.
 template <auto KERNEL>
-uint32_t cluster_of(int dev, uint32_t threads, size_t smem, uint64_t units, uint64_t positions, bool any)
+uint32_t cluster_of(int dev, uint32_t threads, size_t smem, uint64_t units, uint64_t positions)
 {
     for (uint32_t c = kMaxCluster; c > 1; --c)
-        if ((any || !(c & (c - 1))) && (c - 1) * 128ull < positions && clusters_at_once<KERNEL>(dev, c, threads, smem) >= units)
+        if ((c - 1) * 128ull < positions && clusters_at_once<KERNEL>(dev, c, threads, smem) >= units)
             return c;
     return 1;
 }
@@ -1349,22 +1350,22 @@ cudaError_t launch_attn(const FewArgs &a, int dev, int sms, cudaStream_t stream)
     cudaError_t e = allow<attn_kernel<NT, W>>(dev, (int)kMaxSmem);
     if (e != cudaSuccess) return e;
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
-    const uint32_t C = cluster_of<attn_kernel<NT, W>>(dev, W * 32, sizeof(Smem<NT, W>), units, a.c.max_context, NT == 1);
+    const uint32_t C = cluster_of<attn_kernel<NT, W>>(dev, W * 32, sizeof(Smem<NT, W>), units, a.c.max_context);
     return launch(attn_kernel<NT, W>, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), W * 32, sizeof(Smem<NT, W>), C, a, sms, stream);
 }
 
 // The longest CTA's time in cycles for more than eight rows, to be compared with
 // the prompt form's: 18.5 per position of a tile of 16 rows (8 warps), 9000
 // before and after. Rows: this form, the prompt form, in us: one sequence of 28
-// heads on 4, 500 positions, 112: 7.2, 19; 8000, 42 and 112: 16.4, 27 and 26.7,
-// 28; 40 heads on 8, 30000, 40 and 65: 82, 83 and 160, 83; 8 sequences of them,
-// 2000, 20 and 35: 26, 28 and 50, 28; 16000: 165, 161 and 328, 161.
+// heads on 4, 500 positions, 112: 7.2, 19; 8000, 42 and 112: 14.7, 27 and 25.7,
+// 28; 40 heads on 8, 30000, 20 and 65: 54, 83 and 160, 83; 8 sequences of them,
+// 2000, 20 and 35: 25, 28 and 50, 28; 16000: 165, 161 and 328, 161.
 uint64_t few_cycles(const FewArgs &a, int dev)
 {
     constexpr auto kernel = attn_kernel<2, 8>;
     if (allow<kernel>(dev, (int)kMaxSmem) != cudaSuccess) return 0;   // the launch will say so
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
-    const uint32_t C = cluster_of<kernel>(dev, 256, sizeof(Smem<2, 8>), units, a.c.max_context, false);
+    const uint32_t C = cluster_of<kernel>(dev, 256, sizeof(Smem<2, 8>), units, a.c.max_context);
     const uint64_t at_once = std::max(clusters_at_once<kernel>(dev, C, 256, sizeof(Smem<2, 8>)), 1u);
     return (units + at_once - 1) / at_once * ((a.c.max_context + C - 1) / C) * 37 / 2 + 9000;
 }
@@ -1387,7 +1388,7 @@ cudaError_t launch_sparse(const FewArgs &a, int dev, int sms, cudaStream_t strea
     if ((e = allow<sparse_kernel<NT>>(dev, (int)kMaxSmem)) != cudaSuccess) return e;
     const size_t smem = sizeof(Smem<NT, kWarps>) + (size_t)a.n_sel * 4u;
     const uint32_t C = cluster_of<sparse_kernel<NT>>(dev, kThreads, sizeof(Smem<NT, kWarps>), units,
-                                                     std::max<uint64_t>((uint64_t)a.n_sel << a.c.block_log2, a.c.max_context / 8), NT == 1);
+                                                     std::max<uint64_t>((uint64_t)a.n_sel << a.c.block_log2, a.c.max_context / 8));
     return launch(sparse_kernel<NT>, dim3(C * a.r.tokens * a.tiles, a.c.kv_heads, a.c.nseq), kThreads,
                   smem, C, a, sms, stream);
 }
