@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
 // the exponent's base 2), which is rare after the first chunk, so a chunk
 // needs no reduction over lanes.
 // Bound by HBM for long caches (256 bytes per position and KV head, read once: 8
-// sequences of 32768 positions, 40 heads on 8, 90.9 us, 5.9 TB/s or 90 % of the
+// sequences of 32768 positions, 40 heads on 8, 89 to 91 us, 5.9 to 6.0 TB/s or 90 to 92 % of the
 // copy rate, instruction issue at 64 %), by launch, first-byte latency and the
 // chain of one chunk for short ones (640 positions 4.9 us, 8448 10.2 us).
 

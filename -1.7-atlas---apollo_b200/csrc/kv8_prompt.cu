@@ -42,8 +42,8 @@
 // neither softmax nor conversion the chain of barriers leaves 5700, and the
 // conversions, the softmax and the move of the segments (128 KB through L2 every
 // 8 tiles, while the MMAs wait) add about 300 each. 8192 tokens of 40 heads on 8
-// run 1150 us, 72 % of the measured binary16-rate peak for two products, and 1310
-// us when repeated until the power cap lowers the clock.
+// run 1150 us, 72 % of the measured binary16-rate peak for two products, and 1290
+// to 1360 us when repeated until the power cap lowers the clock.
 // Every wait is bounded; after a timeout the CTA's rows are NaN.
 #include <algorithm>
 #include <cfloat>
