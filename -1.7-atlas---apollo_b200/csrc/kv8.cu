@@ -224,18 +224,25 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
 //                 at most 2^-22 max|q|; the integer sums are exact.
 //   O^T += V^T P^T  m16n8k16 binary16 MMAs (rows are dimensions): the codes are
 //                 exact in binary16, P is split into two terms hi + lo (22
-//                 bits). P enters as p * v_scale / vref * 64, with vref the
-//                 power of two below the largest V scale so far, so that blocks
-//                 of different scales share one accumulator; p <= 2^8 and
-//                 v_scale < 2 vref keep it below 2^15.
+//                 bits). A chunk lies in one block, so its V scale is a factor
+//                 of the chunk's own sums as they join the output: blocks
+//                 without weight, or that a row does not see, cost no bits.
+//                 P enters as 2^9 p <= 2^15 and is off by 2^-34 of the row's
+//                 largest weight where it is small. That would show where a
+//                 small weight meets a large V scale, so a chunk whose scale is
+//                 more than 64 times the smallest so far takes its weights
+//                 against its own maximum (a warp's scales come 32 chunks at a
+//                 time, and one ballot marks those chunks; the maximum of every
+//                 chunk instead: 108 us where this takes 89, three bfloat16
+//                 terms of P: 110).
 //
-// The maximum is lazy: a warp raises it only when a score passes it by 8 (in
+// The maximum is lazy: a row's is raised only when a score passes it by 6 (in
 // the exponent's base 2), which is rare after the first chunk, so a chunk
 // needs no reduction over lanes.
 // Bound by HBM for long caches (256 bytes per position and KV head, read once: 8
-// sequences of 32768 positions, 40 heads on 8, 89 to 91 us, 5.9 to 6.0 TB/s or 90 to 92 % of the
-// copy rate, instruction issue at 64 %), by launch, first-byte latency and the
-// chain of one chunk for short ones (640 positions 4.9 us, 8448 10.2 us).
+// sequences of 32768 positions, 40 heads on 8, 89 us, 6.0 TB/s or 92 % of the
+// copy rate), by launch, first-byte latency and the chain of one chunk for short
+// ones (640 positions 5.4 us, 8448 10.6 us).
 
 constexpr uint32_t kStages = 3;
 constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;   // block selection
@@ -378,6 +385,10 @@ __device__ __forceinline__ void load_queries(const AttnArgs &a, const TileRows &
     }
 }
 
+// The maximum is raised by a score that passes it by kFewLazy; weights enter their MMAs times kWeightUnit; a V scale
+// kSteep times the smallest takes its chunk's own maximum.
+constexpr float kFewLazy = 6.0f, kWeightUnit = 0x1p9f, kSteep = 64.0f;
+
 // The ring's barriers, by the lane that will use them; before anything is read
 template <int NT, uint32_t W>
 __device__ __forceinline__ void init_ring(const FewArgs &a, Smem<NT, W> &sm)
@@ -428,10 +439,16 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
     const uint32_t kx = (lane >> 4) ^ (lane & 7u), koff = (lane & 15u) * 128u;
     const uint32_t voff0 = kSlot / 2u + 256u * t + ((g ^ (2u * t)) << 4), voff1 = kSlot / 2u + 256u * t + 128u + ((g ^ (2u * t + 1u)) << 4);
     float ksl, vsl;   // lane: the scales of the warp's chunk 32 (i / 32) + lane
+    float least = INFINITY;   // the smallest V scale of the chunks so far and these
+    uint32_t far = 0u;        // which of them have one far above it
     auto scales = [&](uint32_t i) {
         const uint32_t b = keys.key0(min(first + (i + lane) * step, chunks - 1u)) >> a.c.block_log2;
         ksl = __ldcg(ksc + b);
         vsl = __ldcg(vsc + b);
+    };
+    auto mark = [&]() {
+        least = fminf(least, __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(vsl) & 0x7fffffffu)));
+        far = __ballot_sync(0xffffffffu, !(fabsf(vsl) <= kSteep * least));
     };
     scales(0u);
 
@@ -480,19 +497,23 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
             last[nt][e] = i < rows ? (uint32_t)min(p0 + tr.at(i).x, (uint64_t)0x7fffffffu) : open;
         }
 
-    float o[NT][8][4], m[NT][2], l[NT][2];
-    uint32_t vref = kTinyScale;   // bits of a power of two
+    uint64_t o[NT][8][2];   // dimension rows g and g + 8 of MMA j: columns 2 t and 2 t + 1
+    float m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+        for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = 0ull;
     }
+    mark();
     uint32_t slot = 0u, phase = 0u;
     bool ok = true;
     for (uint32_t i = 0, c = first; c < chunks; ++i, c += step) {
-        if ((i & 31u) == 0u && i) scales(i);
+        if ((i & 31u) == 0u && i) {
+            scales(i);
+            mark();
+        }
         __syncwarp();   // every lane is done with the slot that chunk i - 1 left
         issue(i + kStages - 1, slot ? slot - 1u : kStages - 1u);
         ok = __all_sync(0xffffffffu, mbar_wait(full + slot, phase, &sm.err));
@@ -508,18 +529,6 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
         const uint32_t key = keys.key0(c), in = ring + slot * kSlot;
         if (++slot == kStages) slot = 0u, phase ^= 1u;
         const float sk = __shfl_sync(0xffffffffu, ksl, i & 31u), sv = __shfl_sync(0xffffffffu, vsl, i & 31u);
-        if (sv >= 2.0f * __uint_as_float(vref)) {   // not where sv is NaN
-            const uint32_t now = __float_as_uint(sv) & 0x7f800000u;
-            const float f = now - vref > 120u << 23 ? 0.f : __uint_as_float((127u << 23) - (now - vref));
-            vref = now;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][j][e] *= f;
-        }
-        const float pf = sv * __uint_as_float((260u << 23) - vref);   // sv / vref * 2^6
         // scores: positions key + g (elements 0, 1) and key + g + 8 (2, 3), columns 2 t and 2 t + 1
         float y[NT][4];
         bool raise = false;
@@ -557,30 +566,48 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (masked && (e < 2 ? pa : pb) > last[nt][e & 1]) y[nt][e] = -INFINITY;
-                    raise |= y[nt][e] > m[nt][e & 1] + kLazy;
+                    raise |= y[nt][e] > m[nt][e & 1] + kFewLazy;
                 }
             }
         }
-        if (__any_sync(0xffffffffu, raise)) {
+        float w[NT][2];   // what the weights below count against the row's maximum
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) w[nt][0] = w[nt][1] = 1.0f;
+        float unit = sv * (kOutUnit / kWeightUnit);
+        const bool steep = far >> (i & 31u) & 1u;
+        if (__any_sync(0xffffffffu, raise) || steep) {
+            const float poison = sv != sv ? sv : 0.f;   // a NaN scale, into the rows that see the chunk
+            if (sv != sv) unit = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float f[2] = {1.0f, 1.0f};
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float x = fmaxf(m[nt][e], fmaxf(y[nt][e], y[nt][2 + e]));
+                    float x = fmaxf(y[nt][e], y[nt][2 + e]);
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - x);
-                    m[nt][e] = x;
-                    l[nt][e] *= f;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        o[nt][j][e] *= f;
-                        o[nt][j][2 + e] *= f;
+                    if (x > m[nt][e] + kFewLazy) {   // each row by itself
+                        f[e] = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - x);
+                        m[nt][e] = x;
+                        l[nt][e] *= f[e];
                     }
+                    const float d = !steep || x == -INFINITY ? 0.f : x - m[nt][e];
+                    w[nt][e] = ex2(d);
+                    y[nt][e] += poison - d;
+                    y[nt][2 + e] += poison - d;
                 }
+                const uint64_t f2 = pair(f[0], f[1]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    o[nt][j][0] = mul2(o[nt][j][0], f2);
+                    o[nt][j][1] = mul2(o[nt][j][1], f2);
+                }
+            }
         }
+        const uint64_t unit2 = pair(unit, unit);
         uint32_t bh[NT][2], bl[NT][2];
+        uint64_t by[NT];   // what the chunk's sums count in the output
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float z[4];
@@ -588,17 +615,17 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
             for (int e = 0; e < 4; ++e) {
                 z[e] = ex2(y[nt][e] - m[nt][e & 1]);
                 // a masked position counts nothing, whatever its block's scales are
-                const bool seen = !masked || (e < 2 ? pa : pb) <= last[nt][e & 1];
-                if (!seen) z[e] = 0.f;
-                l[nt][e & 1] += z[e];
-                z[e] *= pf;
-                if (!seen) z[e] = 0.f;
+                if (masked && (e < 2 ? pa : pb) > last[nt][e & 1]) z[e] = 0.f;
             }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) l[nt][e] = fmaf(w[nt][e], z[e] + z[2 + e], l[nt][e]);
+            by[nt] = mul2(pair(w[nt][0], w[nt][1]), unit2);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 float hi[2], lo[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
+                    z[2 * half + e] *= kWeightUnit;
                     hi[e] = __uint_as_float(__float_as_uint(z[2 * half + e]) & 0xffffe000u);   // exact in binary16
                     lo[e] = z[2 * half + e] - hi[e];
                 }
@@ -623,8 +650,8 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
                     float x[4] = {0.f, 0.f, 0.f, 0.f};
                     mma_h(x, va, bl[nt][0], bl[nt][1]);
                     mma_h(x, va, bh[nt][0], bh[nt][1]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][j][e] += x[e];
+                    o[nt][j][0] = fma2(pair(x[0], x[1]), by[nt], o[nt][j][0]);
+                    o[nt][j][1] = fma2(pair(x[2], x[3]), by[nt], o[nt][j][1]);
                 }
             }
         }
@@ -632,7 +659,6 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
     if (!ok) l[0][0] = l[0][1] = l[NT - 1][0] = l[NT - 1][1] = __int_as_float(0x7fffffff);   // the output will be NaN
     __syncthreads();   // every warp is done with the ring: it takes the warps' outputs
 
-    const float back = __uint_as_float(vref) * (1.0f / 64.0f);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -644,9 +670,12 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
             const uint32_t i = 8u * (uint32_t)nt + 2u * t + (uint32_t)e;
             if (g == 0u) sm.wml[warp][i] = make_float2(m[nt][e], x);
 #pragma unroll
-            for (int j = 0; j < 8; j += 2)
-                *reinterpret_cast<float4 *>(&sm.u.wrec[warp][i][16u * g + 2u * (uint32_t)j]) =
-                    make_float4(o[nt][j][e] * back, o[nt][j][2 + e] * back, o[nt][j + 1][e] * back, o[nt][j + 1][2 + e] * back);
+            for (int j = 0; j < 8; j += 2) {
+                float v[4][2];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) unpair(o[nt][j + (k >> 1)][k & 1], v[k][0], v[k][1]);
+                *reinterpret_cast<float4 *>(&sm.u.wrec[warp][i][16u * g + 2u * (uint32_t)j]) = make_float4(v[0][e], v[1][e], v[2][e], v[3][e]);
+            }
         }
     if (C > 1u) cluster_wait();   // the other CTAs run: their shared memory may be written
     __syncthreads();
@@ -671,7 +700,7 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
             ml[w].x = ml[w].x == -INFINITY && ml[w].y == 0.f ? 0.f : ex2(ml[w].x - M);
             L = fmaf(ml[w].x, ml[w].y, L);
         }
-        const float inv = 1.0f / L;
+        const float inv = (1.0f / kOutUnit) / L;
 #pragma unroll
         for (uint32_t d = part; d < kDim / 4u; d += kPer) {
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -715,7 +744,7 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
         x.z = fmaf(fc, y.z, x.z);
         x.w = fmaf(fc, y.w, x.w);
     }
-    const float inv = 1.0f / L;
+    const float inv = (1.0f / kOutUnit) / L;
     store_row(a, tr, s, h, i, p0, lane, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 

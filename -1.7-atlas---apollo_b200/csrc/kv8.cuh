@@ -23,6 +23,9 @@ __device__ __forceinline__ void wait_predecessor(uint32_t early)
 
 constexpr float kScoreScale = (float)(1.4426950408889634 / 11.313708498984761);   // log2(e) / sqrt(128)
 constexpr float kLazy = 8.0f;                 // a running maximum is raised once a score passes it by this (base 2)
+// Outputs are kept times this until the last division: the sum of 2^16 weights of 1 and any finite values stays finite,
+// and V scales of 2^-100 and more keep all their bits.
+constexpr float kOutUnit = 0x1p-16f;
 constexpr uint32_t kTinyScale = 7u << 23;     // bits of 2^-120: where a running power of two of V scales starts
 
 __device__ __forceinline__ float ex2(float x)
