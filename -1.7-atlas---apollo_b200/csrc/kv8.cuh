@@ -26,7 +26,6 @@ constexpr float kLazy = 8.0f;                 // a running maximum is raised onc
 // Outputs are kept times this until the last division: the sum of 2^16 weights of 1 and any finite values stays finite,
 // and V scales of 2^-100 and more keep all their bits.
 constexpr float kOutUnit = 0x1p-16f;
-constexpr uint32_t kTinyScale = 7u << 23;     // bits of 2^-120: where a running power of two of V scales starts
 
 __device__ __forceinline__ float ex2(float x)
 {

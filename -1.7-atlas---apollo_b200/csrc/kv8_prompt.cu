@@ -10,9 +10,11 @@
 // The codes of K and V are exact in binary16. Q (after a power of two per row)
 // and P enter as two binary16 terms hi + lo, 22 bits, summed in the same fp32
 // accumulator: twice the products of a binary16 attention for fp32-level
-// accuracy. The block scales of K multiply the scores, those of V the weights
-// (over a running power of two vref, so that one accumulator serves blocks of
-// different scales; p <= 2^8 and v_scale < 2 vref keep P below 2^15).
+// accuracy. The block scales of K multiply the scores, those of V the weights:
+// P = 2^6 p v_scale over the row's largest p v_scale so far (a second running
+// maximum, of the score plus the scale's logarithm), so that one accumulator
+// serves blocks of different scales, and the row loses bits neither to blocks
+// that it gives no weight nor to blocks that it does not see.
 //
 // Warps of a CTA (21):
 //   0-15   softmax, 8 per tile, two threads per row (half of the keys each):
@@ -203,18 +205,28 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 
+// What a warp knows of a tile's 16-key groups: lane i has the scale of the K codes (i < 8) or V codes (8 <= i < 16) of
+// group i % 8, and of V's the base-2 logarithm
+struct Scales {
+    float scale, log2;
+};
+
 // A thread's half of a row's softmax over one tile of keys: 64 scores at tensor
-// memory `at` (this warp's lanes), what a score of their 16-key group i is
-// worth in f[i], of which the row sees the first `nvis` keys (MASK; else all).
-// The next 16 columns are on their way while 16 are worked on.
+// memory `at` (this warp's lanes), their groups from `g0` on, what a unit of a
+// score is worth in `factor`, of which the row sees the first `nvis` keys (MASK;
+// else all). Returns the largest score; in `mw`, the largest sum of a score and
+// the logarithm of its V scale. The next 16 columns are on their way while 16
+// are worked on.
 template <bool MASK>
-__device__ __forceinline__ float tile_max(uint32_t at, const float (&f)[4], int nvis)
+__device__ __forceinline__ float tile_max(uint32_t at, const Scales &sc, uint32_t g0, float factor, int nvis, float &mw)
 {
     float m = -INFINITY, s[2][16];
+    mw = -INFINITY;
     tmem_ld(at, s[0]);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         float(&v)[16] = s[c & 1];
+        const float f = __shfl_sync(0xffffffffu, sc.scale, g0 + c) * factor, lg = __shfl_sync(0xffffffffu, sc.log2, 8u + g0 + c);
         tmem_wait_ld(v);
         if (c < 3) tmem_ld(at + 16u * (uint32_t)(c + 1), s[(c + 1) & 1]);
         if (MASK)
@@ -222,18 +234,22 @@ __device__ __forceinline__ float tile_max(uint32_t at, const float (&f)[4], int 
             for (int i = 0; i < 16; ++i) v[i] = 16 * c + i < nvis ? v[i] : -INFINITY;
         const float x = max3(max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8])),
                              max3(v[9], v[10], v[11]), max3(max3(v[12], v[13], v[14]), v[15], v[15]));
-        if (!MASK || x != -INFINITY) m = fmaxf(m, x * f[c]);
+        if (!MASK || x != -INFINITY) {
+            m = fmaxf(m, x * f);
+            mw = fmaxf(mw, fmaf(x, f, lg));
+        }
     }
     return m;
 }
 
 // The weights into the scores' columns, 16 keys at a time: 8 columns of hi, 8
-// of lo. The V scale over vref enters the exponent: lg[i] is its base-2
-// logarithm for group i, and ipf[i], its reciprocal, takes it out of the
-// group's sum again. Returns the sum of the weights without it.
+// of lo. They are 2^(score + log2 v_scale - ref), so their rounding is that of
+// the group's sum, which returns without the V scale, times 2^k. A group with so
+// small a scale that binary16 would hold nothing even of the row's largest
+// weight takes a larger one, still small enough for that, so that the sum keeps
+// its part.
 template <bool MASK>
-__device__ __forceinline__ float tile_weights(uint32_t at, const float (&f)[4], const float (&lg)[4], const float (&ipf)[4],
-                                              int nvis, float m)
+__device__ __forceinline__ float tile_weights(uint32_t at, const Scales &sc, uint32_t g0, float factor, int nvis, float ref, int k)
 {
     float sum = 0.f, s[2][16];
     const uint64_t minus = pair(-1.0f, -1.0f);
@@ -241,10 +257,12 @@ __device__ __forceinline__ float tile_weights(uint32_t at, const float (&f)[4], 
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const float(&v)[16] = s[c & 1];
+        const float f = __shfl_sync(0xffffffffu, sc.scale, g0 + c) * factor, lg = __shfl_sync(0xffffffffu, sc.log2, 8u + g0 + c);
+        const float sv = __shfl_sync(0xffffffffu, sc.scale, 8u + g0 + c), least = (float)(k - 80);
+        const float off = (lg < least ? least : lg) - ref;   // a NaN stays
         tmem_wait_ld(s[c & 1]);
         if (c < 3) tmem_ld(at + 16u * (uint32_t)(c + 1), s[(c + 1) & 1]);
-        const float off = lg[c] - m;
-        const uint64_t f2 = pair(f[c], f[c]), off2 = pair(off, off);
+        const uint64_t f2 = pair(f, f), off2 = pair(off, off);
         uint32_t p[16];
         uint64_t part = 0;
 #pragma unroll
@@ -259,7 +277,7 @@ __device__ __forceinline__ float tile_weights(uint32_t at, const float (&f)[4], 
             }
             const uint64_t w = pair(w0, w1);
             part = add2(part, w);
-            // the upper 11 bits are exact in binary16
+            // the upper 11 bits are exact in binary16, but for weights below 2^-14
             const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
             float l0, l1;
             unpair(fma2(pair(h0, h1), minus, w), l0, l1);
@@ -268,11 +286,19 @@ __device__ __forceinline__ float tile_weights(uint32_t at, const float (&f)[4], 
         }
         float a0, a1;
         unpair(part, a0, a1);
-        if (!MASK || 16 * c < nvis) sum = fmaf(a0 + a1, ipf[c], sum);
+        if (!MASK || 16 * c < nvis) {
+            // 2^k / v_scale by halves: either may pass fp32's range
+            const int k0 = k / 2, k1 = k - k0;
+            const float r = rcp(sv * __int_as_float((127 - k0) << 23) * __int_as_float((127 - k1) << 23));
+            sum = fmaf(a0 + a1, lg < least ? 0x1p80f : r, sum);
+        }
         tmem_st(at + 16u * (uint32_t)c, p);
     }
     return sum;
 }
+
+// The integer below x; 0 for none
+__device__ __forceinline__ int below(float x) { return x == x ? (int)fminf(fmaxf(floorf(x), -250.0f), 250.0f) : 0; }
 
 // Barrier `id` of `threads` threads (whole warps); the second tells whether any of them brought a true
 __device__ __forceinline__ void meet(uint32_t id, uint32_t threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -585,8 +611,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 return __ldcg(scales + min(((j0 + j) * kTileKeys + 16u * (lane & 7u)) >> a.c.block_log2, a.c.n_blocks - 1u));
             };
             const uint32_t j_first = one ? t : 0u, j_step = one ? 2u : 1u;
-            float m = -INFINITY, l = 0.f, next = j_first < n ? scale_of(j_first) : 0.f;
-            uint32_t vref = kTinyScale;
+            // m: the largest score of this thread's half; mw: of the row, the largest score + logarithm of the V scale,
+            // against which weights are taken; l: this half's sum of weights without their V scales, times 2^k, k the
+            // integer below mw - m that keeps it in range
+            float m = -INFINITY, l = 0.f, mw = -INFINITY, next = j_first < n ? scale_of(j_first) : 0.f;
+            int k = 0;
             uint32_t turn = 0u;
             float4 acc[16];   // the output of the segments before the current one, in local memory (128 KB for the CTA)
             bool ok = true;
@@ -611,48 +640,33 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                         }
                     }
                 }
-                const float sc = next;
+                // a V scale of 0 counts as fp32's smallest number, 2^-149
+                Scales sc;
+                sc.scale = next == 0.f && lane >= 8u ? __uint_as_float(1u) : next;
+                sc.log2 = __log2f(sc.scale);
+                if (sc.log2 < -149.0f) sc.log2 = -149.0f;
                 if (j + j_step < n) next = scale_of(j + j_step);
                 const uint32_t key0 = (j0 + j) * kTileKeys, mine = key0 + 64u * half;
                 const bool masked = key0 + kTileKeys - 1u > open;   // some row does not see all of the tile
                 const int nvis = last < mine ? 0 : (int)min(last - mine + 1u, 64u);
-                // the largest V scale of the tile's stored positions (a NaN counts nothing)
-                float top = lane >= 8u && lane < 16u && key0 + 16u * (lane & 7u) < limit ? sc : 0.f;
-                top = __uint_as_float(__reduce_max_sync(0xffffffffu, top > 0.f && top < INFINITY ? __float_as_uint(top) : 0u));
-                float fv = 1.0f;   // what the output is rescaled by for a larger vref
-                if (top >= 2.0f * __uint_as_float(vref)) {
-                    const uint32_t now = __float_as_uint(top) & 0x7f800000u;
-                    fv = now - vref > 120u << 23 ? 0.f : __uint_as_float((127u << 23) - (now - vref));
-                    vref = now;
-                }
-                // All that needs no scores is done before they come. pf = v_scale / vref * 2^6, at least 2^-40
-                // (below that nothing of it is left in binary16; a block of zeros has scale 0).
-                const float pv = sc * __uint_as_float((260u << 23) - vref), pf = pv < 0x1p-40f ? 0x1p-40f : pv;
-                const float pl = __log2f(pf), pr = rcp(pf);
-                float f[4], lg[4], ipf[4];
-#pragma unroll
-                for (uint32_t c = 0; c < 4u; ++c) {
-                    f[c] = __shfl_sync(0xffffffffu, sc, g0 + c) * factor;
-                    lg[c] = __shfl_sync(0xffffffffu, pl, 8u + g0 + c);
-                    ipf[c] = __shfl_sync(0xffffffffu, pr, 8u + g0 + c);
-                }
                 ok = ok && wait_warp(&b.s_full[t], turn & 1u, err);
                 fence_after();
-                float x = -INFINITY;
-                if (ok) x = masked ? tile_max<true>(at, f, nvis) : tile_max<false>(at, f, 64);
-                const bool raise = meet_any(1u + t, 256u, x > m + kLazy);
+                float x = -INFINITY, xw = -INFINITY;
+                if (ok) x = masked ? tile_max<true>(at, sc, g0, factor, nvis, xw) : tile_max<false>(at, sc, g0, factor, 64, xw);
+                const float was = m, before = mw;
+                if (x > m + kLazy) m = x;
+                const bool raise = meet_any(1u + t, 256u, xw > mw + kLazy);
                 const bool amends = turn % kSegment && turn % kAmends == 0u;
-                if (raise || fv != 1.0f || amends) {
+                if (raise || amends) {
+                    float fv = 1.0f;   // what the output is rescaled by
                     if (raise) {
-                        b.half[t][half][row] = x;
+                        b.half[t][half][row] = xw;
                         meet(1u + t, 256u);
-                        x = fmaxf(x, b.half[t][half ^ 1u][row]);
-                    }
-                    if (x > m + kLazy) {
-                        const float fm = m == -INFINITY ? 0.f : ex2(m - x);
-                        m = x;
-                        l *= fm;
-                        fv *= fm;
+                        xw = fmaxf(xw, b.half[t][half ^ 1u][row]);
+                        if (xw > mw + kLazy) {
+                            fv = mw == -INFINITY ? 0.f : ex2(mw - xw);
+                            mw = xw;
+                        }
                     }
                     if (turn >= kSegment && __any_sync(0xffffffffu, fv != 1.0f))
 #pragma unroll 1
@@ -671,14 +685,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                         }
                     }
                 }
+                if (m != was || mw != before) {
+                    const int now = below(mw - m);
+                    l *= was == -INFINITY ? 0.f : ex2(before - mw + (float)(now - k));
+                    k = now;
+                }
                 if (ok)
-                    l += masked ? tile_weights<true>(at, f, lg, ipf, nvis, m) : tile_weights<false>(at, f, lg, ipf, 64, m);
+                    l += masked ? tile_weights<true>(at, sc, g0, factor, nvis, mw - 6.0f, k)
+                                : tile_weights<false>(at, sc, g0, factor, 64, mw - 6.0f, k);
                 tmem_wait_st();
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&b.p_full[t]);
             }
-            // the sum of both halves
+            // both halves' largest score and sum; a half that saw no position counts nothing
+            meet(1u + t, 256u);
+            b.half[t][half][row] = m;
+            meet(1u + t, 256u);
+            const float top = fmaxf(m, b.half[t][half ^ 1u][row]);
+            const int both = below(mw - top);
+            l = m == -INFINITY && l == 0.f ? 0.f : l * ex2((float)(both - k));
+            m = top;
             meet(1u + t, 256u);
             b.half[t][half][row] = l;
             meet(1u + t, 256u);
@@ -687,7 +714,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             const bool have = turn && ok && wait_warp(&b.o_full[t], ((turn - 1u) / kSegment) & 1u, err);
             fence_after();
             const float gain = 1.0f + kLoss * (float)((turn - 1u) % kAmends + 1u);
-            const float back = __uint_as_float(vref) * (1.0f / 64.0f) * (one || C > 1u ? 1.0f : 1.0f / l);
+            // The output is acc 2^k / l. What is merged with other states is taken against the largest score instead, both
+            // times 2^(mw - m), less the 2^6 of the weights (and kOutUnit).
+            const bool whole = !one && C == 1u;
+            const float rest = m == -INFINITY ? 0.f : ex2(mw - m - (float)both) * 0x1p-6f;
+            const float back = (whole ? 1.0f / l : rest * kOutUnit) * ex2((float)both);
+            l *= rest;
             float4 *stage = reinterpret_cast<float4 *>(qs + t * kQTile);
 #pragma unroll 1
             for (uint32_t c = 0; c < 4u; ++c) {
@@ -724,7 +756,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 row_m = M;
                 row_l = l * own + l1 * other;
                 meet(3u, 32u * kConvWarp);
-                if (half == 0u) b.half[t][0][row] = C > 1u ? own : own / row_l;
+                if (half == 0u) b.half[t][0][row] = C > 1u ? own : own * (1.0f / kOutUnit) / row_l;
             } else {
                 row_m = m;
                 row_l = l;
@@ -826,7 +858,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             const float sum = __shfl_sync(0xffffffffu, L, 8 * v);
             if (r >= rows) continue;
             const uint2 at = tr.at(r);
-            const float inv = any_bad || p0 + at.x >= a.c.max_context ? __int_as_float(0x7fffffff) : 1.0f / sum;
+            const float inv = any_bad || p0 + at.x >= a.c.max_context ? __int_as_float(0x7fffffff) : (1.0f / kOutUnit) / sum;
             reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + at.x) * a.ldo + (size_t)(h * a.group + at.y) * kDim)[lane] =
                 make_float4(x[v].x * inv, x[v].y * inv, x[v].z * inv, x[v].w * inv);
         }
