@@ -40,7 +40,6 @@ struct AttnArgs {
     uint32_t q_heads, group;
     float group_inv;                  // 1 / group, a little high
     uint32_t tiles;                   // row tiles per (sequence, KV head) - or per (sequence, KV head, token)
-    uint32_t cta_tiles;               // prompts: tiles of 128 rows per CTA (1 or 2)
     uint32_t n_sel;                   // block selection: blocks per token and KV head
     int32_t *sel;                     // [seq][tokens][kv_heads][n_sel]
     uint32_t early;                   // the successor may start at once

@@ -16,36 +16,44 @@
 // serves blocks of different scales, and the row loses bits neither to blocks
 // that it gives no weight nor to blocks that it does not see.
 //
-// Warps of a CTA (21):
-//   0-15   softmax, 8 per tile, two threads per row (half of the keys each):
-//          maximum and exponentials of the scores straight from tensor memory, P
-//          back into the columns that the scores leave; the maximum is lazy
-//          (raised only when a score passes it by 2^8), so the output is
-//          rescaled and the halves exchange maxima rarely;
-//   16-19  codes -> binary16 in 128-byte swizzled K-major tiles: K [key][dimension],
+// Warps of a CTA (16):
+//   0-7    softmax, four per tile, one thread per row: maximum and exponentials
+//          of the scores straight from tensor memory, P back into the columns
+//          that the scores leave; the maximum is lazy (raised only when a score
+//          passes it by 2^8). Each tile of keys' output is added to the earlier
+//          ones in these threads' registers, which the other warps leave them;
+//   8-11   codes -> binary16 in 128-byte swizzled K-major tiles: K [key][dimension],
 //          V transposed on the way, [dimension][key]; the next codes are on their
 //          way by cp.async while the MMAs still read the current ones;
-//   20     issues the MMAs: P V of a tile, then the next keys' scores of the
+//   12     issues the MMAs: P V of a tile, then the next keys' scores of the
 //          same tile, so that one tile's softmax runs under the other's MMAs.
 // Where few rows leave SMs idle, a CTA takes one tile of 128 rows: both softmax
 // groups then have the same rows and take turns at the tiles of keys, each with
 // an output and a state of its own, which are merged at the end. The place of the
-// second tile's Q holds a second buffer of K and one of V then, group 1's (5700
-// cycles per tile of keys with one buffer, 4400 with two).
-// Tensor memory: 2 x 128 columns of scores / weights, 2 x 128 of output (of up to
-// kSegment tiles of keys; the softmax warps hold the sum of the earlier ones).
+// second tile's Q holds a second buffer of K and one of V then, group 1's.
+//
+// Tensor cores truncate their sums: an MMA that adds to an output loses 2^-24 of
+// it on average where the values have one sign, a fifth of that where they have
+// not, and nothing where its weights are zeros. So only a tile of keys (16 MMAs)
+// is summed in tensor memory and then added to the earlier ones with rounding.
+// Over 1024 positions of one sign, sums of 1 / 2 / 8 tiles lose 17 / 31 / 130 x
+// 2^-24, at most 33 / 55 / 253 (one position with most of the weight). Taking the
+// outputs out after every tile costs no time, as it runs beside the next scores.
+// (Two threads per row, with the sums of eight tiles in local memory: 512 tokens
+// of 28 heads on 4 17.3 us where this takes 19.4, 8192 of 40 heads on 8 1165 and
+// 1264, 333 over 5001 of 16 on 2 73 to 84 and 68 to 73; eight tiles are too many,
+// and with two 8192 take 1557.)
+// Tensor memory: 2 x 128 columns of scores / weights, 2 x 128 of output.
 // Shared memory: Q hi / lo 128 KB, K 32 KB, V 32 KB, their next codes 32 KB; Q's
 // place stages the output.
 //
 // Few rows over many positions: the positions are split over a cluster of CTAs,
 // and each merges a share of the rows through distributed shared memory.
 //
-// 256 rows x 128 keys take 6700 cycles, of which the MMAs alone are 4130; with
-// neither softmax nor conversion the chain of barriers leaves 5700, and the
-// conversions, the softmax and the move of the segments (128 KB through L2 every
-// 8 tiles, while the MMAs wait) add about 300 each. 8192 tokens of 40 heads on 8
-// run 1150 us, 72 % of the measured binary16-rate peak for two products, and 1290
-// to 1360 us when repeated until the power cap lowers the clock.
+// Bound by the chain of a tile's scores, softmax and output with one thread per
+// row, next to the MMAs, which need 4130 cycles for 256 rows x 128 keys. 8192
+// tokens of 40 heads on 8 run 1264 us, 66 % of the measured binary16-rate peak
+// for two products.
 // Every wait is bounded; after a timeout the CTA's rows are NaN.
 #include <algorithm>
 #include <cfloat>
@@ -59,21 +67,11 @@ namespace {
 
 constexpr uint32_t kTileRows = 128, kTileKeys = 128;
 constexpr uint32_t kMaxSplit = 8;                  // CTAs that share the positions of a tile's rows
-constexpr uint32_t kConvWarp = 16, kMmaWarp = 20, kPromptThreads = 21 * 32;   // first converter, the MMA warp
-// Tensor cores truncate their sums: per tile of keys (16 steps) the output
-// loses 5.6e-7 of itself on average while it grows, 2e-5 over 8192 positions. So
-// a segment of eight tiles is summed in tensor memory and added to the earlier
-// ones with rounding, and what is lost on average is made up for every two
-// tiles, in place or with the move: errors of 1.0e-6 over 8192 positions and
-// 1.5e-6 over 32300, where one sum for all tiles had 2.0e-5 and 7.5e-5. Where a
-// row's later weights in a segment are zeros, nothing is lost, and 4.5e-6 at most
-// is made up for nothing. 8192 tokens of 40 heads on 8: segments of 4 / 8 / 16
-// tiles 1234 / 1125 / 1072 us, errors 1.0e-6 / 1.4e-6 / 2.6e-6 without the
-// amends in place, which take 10 us. (Sums in registers instead, one thread per
-// row with 200 of them, registers moved between the warps: 1175 us, and 512
-// tokens of 28 heads on 4 3 us more.)
-constexpr uint32_t kSegment = 8, kAmends = 2;
-constexpr float kLoss = 5.6e-7f;
+// Warps by number: eight of softmax, four converters, the one that issues the MMAs (and three that fill up its warpgroup)
+constexpr uint32_t kConvWarp = 8, kMmaWarp = 12, kPromptThreads = 16 * 32;
+// Registers per thread of a warpgroup after the split, of 128 at launch
+constexpr uint32_t kSoftmaxRegs = 192, kConvertRegs = 72, kMmaRegs = 56;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kMmaRegs == 4 * 128, "what two warpgroups get is what the others leave");
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 binary16, swizzled
 constexpr uint32_t kQTile = 4 * kHalf;             // one tile's Q: [hi, lo][2 x 64 dimensions]
 
@@ -81,9 +79,9 @@ struct PromptBars {
     uint64_t s_full[2], p_full[2], o_full[2];                                       // [tile]
     uint64_t k_full[2][2], k_empty[2][2], v_full[2][2], v_empty[2][2], q_full, fin;   // [buffer][half]
     uint32_t tmem, status;
-    // what a score of the row is worth, in the exponent's base 2 (in [tile][0], until the first exchange);
-    // then the two threads of a row exchange their maxima and sums here
-    float half[2][2][kTileRows];
+    // what a score of the row is worth, in the exponent's base 2 (in [tile][0]); one tile: then what the groups'
+    // states are
+    float state[2][2][kTileRows];
 };
 
 // In the place of the next codes once they are used up
@@ -211,24 +209,35 @@ struct Scales {
     float scale, log2;
 };
 
-// A thread's half of a row's softmax over one tile of keys: 64 scores at tensor
-// memory `at` (this warp's lanes), their groups from `g0` on, what a unit of a
-// score is worth in `factor`, of which the row sees the first `nvis` keys (MASK;
-// else all). Returns the largest score; in `mw`, the largest sum of a score and
-// the logarithm of its V scale. The next 16 columns are on their way while 16
-// are worked on.
+// From this lane's scale. A V scale of 0 counts as fp32's smallest number, 2^-149.
+__device__ __forceinline__ Scales scales_from(float x, uint32_t lane)
+{
+    Scales s;
+    s.scale = x == 0.f && lane >= 8u ? __uint_as_float(1u) : x;
+    s.log2 = __log2f(s.scale);
+    if (s.log2 < -149.0f) s.log2 = -149.0f;
+    return s;
+}
+
+constexpr int kGroups = kTileKeys / 16;
+
+// A row's softmax over one tile of keys: scores at tensor memory `at` (this
+// warp's lanes), what a unit of one is worth in `factor`, of which the row sees
+// the first `nvis` keys (MASK; else all). Returns the largest score; in `mw`, the
+// largest sum of a score and the logarithm of its V scale. The next 16 columns
+// are on their way while 16 are worked on.
 template <bool MASK>
-__device__ __forceinline__ float tile_max(uint32_t at, const Scales &sc, uint32_t g0, float factor, int nvis, float &mw)
+__device__ __forceinline__ float tile_max(uint32_t at, const Scales &sc, float factor, int nvis, float &mw)
 {
     float m = -INFINITY, s[2][16];
     mw = -INFINITY;
     tmem_ld(at, s[0]);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < kGroups; ++c) {
         float(&v)[16] = s[c & 1];
-        const float f = __shfl_sync(0xffffffffu, sc.scale, g0 + c) * factor, lg = __shfl_sync(0xffffffffu, sc.log2, 8u + g0 + c);
+        const float f = __shfl_sync(0xffffffffu, sc.scale, c) * factor, lg = __shfl_sync(0xffffffffu, sc.log2, 8 + c);
         tmem_wait_ld(v);
-        if (c < 3) tmem_ld(at + 16u * (uint32_t)(c + 1), s[(c + 1) & 1]);
+        if (c + 1 < kGroups) tmem_ld(at + 16u * (uint32_t)(c + 1), s[(c + 1) & 1]);
         if (MASK)
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = 16 * c + i < nvis ? v[i] : -INFINITY;
@@ -249,19 +258,19 @@ __device__ __forceinline__ float tile_max(uint32_t at, const Scales &sc, uint32_
 // weight takes a larger one, still small enough for that, so that the sum keeps
 // its part.
 template <bool MASK>
-__device__ __forceinline__ float tile_weights(uint32_t at, const Scales &sc, uint32_t g0, float factor, int nvis, float ref, int k)
+__device__ __forceinline__ float tile_weights(uint32_t at, const Scales &sc, float factor, int nvis, float ref, int k)
 {
     float sum = 0.f, s[2][16];
     const uint64_t minus = pair(-1.0f, -1.0f);
     tmem_ld(at, s[0]);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < kGroups; ++c) {
         const float(&v)[16] = s[c & 1];
-        const float f = __shfl_sync(0xffffffffu, sc.scale, g0 + c) * factor, lg = __shfl_sync(0xffffffffu, sc.log2, 8u + g0 + c);
-        const float sv = __shfl_sync(0xffffffffu, sc.scale, 8u + g0 + c), least = (float)(k - 80);
+        const float f = __shfl_sync(0xffffffffu, sc.scale, c) * factor, lg = __shfl_sync(0xffffffffu, sc.log2, 8 + c);
+        const float sv = __shfl_sync(0xffffffffu, sc.scale, 8 + c), least = (float)(k - 80);
         const float off = (lg < least ? least : lg) - ref;   // a NaN stays
         tmem_wait_ld(s[c & 1]);
-        if (c < 3) tmem_ld(at + 16u * (uint32_t)(c + 1), s[(c + 1) & 1]);
+        if (c + 1 < kGroups) tmem_ld(at + 16u * (uint32_t)(c + 1), s[(c + 1) & 1]);
         const uint64_t f2 = pair(f, f), off2 = pair(off, off);
         uint32_t p[16];
         uint64_t part = 0;
@@ -300,17 +309,8 @@ __device__ __forceinline__ float tile_weights(uint32_t at, const Scales &sc, uin
 // The integer below x; 0 for none
 __device__ __forceinline__ int below(float x) { return x == x ? (int)fminf(fmaxf(floorf(x), -250.0f), 250.0f) : 0; }
 
-// Barrier `id` of `threads` threads (whole warps); the second tells whether any of them brought a true
+// Barrier `id` of `threads` threads (whole warps)
 __device__ __forceinline__ void meet(uint32_t id, uint32_t threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ bool meet_any(uint32_t id, uint32_t threads, bool x)
-{
-    uint32_t r;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %3, 0;\n bar.red.or.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-                 : "=r"(r)
-                 : "r"(id), "r"(threads), "r"((uint32_t)x)
-                 : "memory");
-    return r != 0u;
-}
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there)   // zeros where !there
 {
@@ -320,6 +320,13 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 __device__ __forceinline__ void copy_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 __device__ __forceinline__ void copy_wait0() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
+// Registers of the calling warpgroup's threads: taken once others have left them
+template <uint32_t N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <uint32_t N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <bool ONE>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_constant__ AttnArgs a)
 {
     extern __shared__ __align__(1024) uint8_t prompt_smem[];
@@ -330,13 +337,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t C = cluster_size(), rank = cluster_rank(), s = blockIdx.z, h = blockIdx.y;
     // the last rows first: they see the most positions
-    const uint32_t r0 = (a.tiles - 1u - blockIdx.x / C) * a.cta_tiles * kTileRows;
+    const uint32_t r0 = (a.tiles - 1u - blockIdx.x / C) * (ONE ? 1u : 2u) * kTileRows;
     TileRows tr{r0 / a.group, 0u, a.group, a.group_inv};
     tr.rem = r0 - tr.tok * a.group;
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; ++t) {
             mbar_init(&b.s_full[t], 1u);
-            mbar_init(&b.p_full[t], 8u);
+            mbar_init(&b.p_full[t], 4u);
             mbar_init(&b.o_full[t], 1u);
             for (int hf = 0; hf < 2; ++hf) {
                 mbar_init(&b.k_full[t][hf], 4u);
@@ -366,8 +373,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
         return;
     }
-    const uint32_t rows = min(all - r0, a.cta_tiles * kTileRows), tiles = rows > kTileRows ? 2u : 1u;
-    const bool one = a.cta_tiles == 1u;
+    const uint32_t rows = min(all - r0, (ONE ? 1u : 2u) * kTileRows), tiles = rows > kTileRows ? 2u : 1u;
     const uint32_t limit = (uint32_t)min(p0 + tr.at(rows - 1u).x + 1u, (uint64_t)a.c.max_context);
     const uint32_t total = (limit + kTileKeys - 1u) / kTileKeys;
     uint32_t j0 = 0u, n = total;   // this CTA's tiles of keys
@@ -378,15 +384,99 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     }
     const size_t head = (size_t)s * a.c.kv_heads + h;
     // K's and V's buffer for tile of keys j, and how often it was used before
-    auto buffer = [&](uint32_t j) { return one ? j & 1u : 0u; };
-    auto uses = [&](uint32_t j) { return one ? j >> 1 : j; };
+    auto buffer = [&](uint32_t j) { return ONE ? j & 1u : 0u; };
+    auto uses = [&](uint32_t j) { return ONE ? j >> 1 : j; };
     uint8_t *const ks2 = qs + kQTile, *const vs2 = ks2 + 2 * kHalf;
 
-    float row_m = -INFINITY, row_l = 0.f;   // softmax threads of half 0: their row's state, for the cluster
+    float row_m = -INFINITY, row_l = 0.f;   // softmax threads: their row's state, for the cluster
 
-    if (warp == kMmaWarp) {
+    // The end of a CTA, for every warp in the branch of its registers
+    auto leave = [&]() {
+        fence_before();
+        __syncthreads();
+        if (warp == kMmaWarp) {
+            fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        }
+    };
+    auto merge = [&]() {
+        // the converters' slots are free now
+        rs.max[warp >> 2][(warp & 3u) * 32u + lane] = row_m;
+        rs.sum[warp >> 2][(warp & 3u) * 32u + lane] = row_l;
+        // Rows rank, rank + C, ... of the cluster's states, four at a time per warp:
+        // lane = (row, CTA) for the maxima and sums, then 4 dimensions. A state that
+        // saw no position counts nothing.
+        static_assert(kMaxSplit == 8, "eight lanes per row");
+        cluster_sync();
+        for (uint32_t k0 = 4u * warp; rank + C * k0 < rows; k0 += 4u * kConvWarp) {
+            // two CTAs' outputs are on their way meanwhile
+            float4 y[2][4];
+            auto load = [&](float4(&to)[4], uint32_t c) {
+#pragma unroll
+                for (uint32_t v = 0; v < 4; ++v) {
+                    const uint32_t r = min(rank + C * (k0 + v), rows - 1u), row = r & (kTileRows - 1u);
+                    to[v] = ld_cluster4(reinterpret_cast<const float4 *>(qs + (r / kTileRows) * kQTile) + row * 32u + (lane ^ (row & 31u)), c);
+                }
+            };
+            auto add = [&](float4(&x)[4], const float4(&from)[4], float f, uint32_t c) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const float fc = __shfl_sync(0xffffffffu, f, 8 * v + (int)c);
+                    x[v].x = fmaf(fc, from[v].x, x[v].x);
+                    x[v].y = fmaf(fc, from[v].y, x[v].y);
+                    x[v].z = fmaf(fc, from[v].z, x[v].z);
+                    x[v].w = fmaf(fc, from[v].w, x[v].w);
+                }
+            };
+            load(y[0], 0u);
+            load(y[1], 1u);
+            const uint32_t u = lane >> 3, cta = lane & 7u, i = rank + C * (k0 + u);
+            const bool there = cta < C && i < rows;
+            const float mc = there ? ld_cluster1(&rs.max[i / kTileRows][i & (kTileRows - 1u)], cta) : -INFINITY;
+            const float lc = there ? ld_cluster1(&rs.sum[i / kTileRows][i & (kTileRows - 1u)], cta) : 0.f;
+            const bool bad = there && __float_as_uint(ld_cluster1(&b.status, cta)) != kStatusOk;
+            float M = mc;
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+            const float f = mc == -INFINITY && lc == 0.f ? 0.f : ex2(mc - M);
+            float L = f * lc;
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            const bool any_bad = __any_sync(0xffffffffu, bad);
+            float4 x[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) x[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t c = 0; c < C; c += 2u) {
+                add(x, y[0], f, c);
+                if (c + 2u < C) load(y[0], c + 2u);
+                if (c + 1u < C) add(x, y[1], f, c + 1u);
+                if (c + 3u < C) load(y[1], c + 3u);
+            }
+#pragma unroll
+            for (uint32_t v = 0; v < 4; ++v) {
+                const uint32_t r = rank + C * (k0 + v);
+                const float sum = __shfl_sync(0xffffffffu, L, 8 * v);
+                if (r >= rows) continue;
+                const uint2 at = tr.at(r);
+                const float inv = any_bad || p0 + at.x >= a.c.max_context ? __int_as_float(0x7fffffff) : (1.0f / kOutUnit) / sum;
+                reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + at.x) * a.ldo + (size_t)(h * a.group + at.y) * kDim)[lane] =
+                    make_float4(x[v].x * inv, x[v].y * inv, x[v].z * inv, x[v].w * inv);
+            }
+        }
+        cluster_sync();   // no CTA leaves while the cluster may read its states
+    };
+
+    auto leave_unmerged = [&]() {   // the warps that have left their registers to the others
+        leave();
+        if (C > 1u) {
+            cluster_sync();
+            cluster_sync();
+        }
+    };
+    if (warp >= kMmaWarp) {
         // ------------------------------------------------------------- MMA --
-        if (elected()) {
+        fewer_registers<kMmaRegs>();
+        if (warp == kMmaWarp && elected()) {
             // a step of 16 along K is 32 bytes, 2 in a descriptor; 4 steps fill a swizzled tile
             const uint64_t qd = operand(smem_addr(qs)), kd[2] = {operand(smem_addr(ks)), operand(smem_addr(ks2))},
                            vd[2] = {operand(smem_addr(vs)), operand(smem_addr(vs2))};
@@ -422,18 +512,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                     for (uint32_t st = 0; st < 4u; ++st) {
                         const uint64_t v = (buffer(j) ? vd[1] : vd[0]) + hf * (kHalf >> 4) + st * 2u;
                         const uint32_t p = tmem + 128u * t + 64u * hf + 16u * st;
-                        mma_ts(tmem + 256u + 128u * t, p, v, turn % kSegment != 0u || hf != 0u || st != 0u);
+                        mma_ts(tmem + 256u + 128u * t, p, v, hf != 0u || st != 0u);
                         mma_ts(tmem + 256u + 128u * t, p + 8u, v, 1u);
                     }
                     if (last_use) commit(&b.v_empty[buffer(j)][hf]);
                 }
             };
-            if (one) {   // the groups take turns at the keys
+            if (ONE) {   // the groups take turns at the keys
                 for (uint32_t j = 0; ok && j < min(n, 2u); ++j) scores(j, 0u, j, true, true);
                 for (uint32_t j = 0; ok && j < n; ++j) {
                     output(j & 1u, j, j >> 1, true, true);
                     if (!ok) break;
-                    if (j + 2u >= n || (j >> 1) % kSegment == kSegment - 1u) commit(&b.o_full[j & 1u]);
+                    commit(&b.o_full[j & 1u]);
                     if (j + 2u < n) scores(j & 1u, 0u, j + 2u, true, true);
                 }
             } else {
@@ -442,7 +532,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                     for (uint32_t t = 0; ok && t < tiles; ++t) {
                         output(t, j, j, t == 0u, t + 1u == tiles);
                         if (!ok) break;
-                        if (j + 1u == n || j % kSegment == kSegment - 1u) commit(&b.o_full[t]);
+                        commit(&b.o_full[t]);
                         if (j + 1u < n) scores(t, t, j + 1u, t == 0u, t + 1u == tiles);
                     }
                 }
@@ -454,7 +544,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             }
         }
         __syncwarp();
+        leave_unmerged();
+        return;
     } else if (warp >= kConvWarp) {
+        fewer_registers<kConvertRegs>();
         // ------------------------------------------------------- converters --
         // K: a thread takes 16 dimensions of 8 keys (8 lanes write the same
         // chunk of 8 rows); V: 8 keys x 16 dimensions (8 lanes write the 8
@@ -547,7 +640,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             copy_v(j + 1u);
         }
         copy_wait0();
+        leave_unmerged();
+        return;
     } else {
+        more_registers<kSoftmaxRegs>();
         // --------------------------------------------------------- softmax --
         // First Q: a warp takes eight rows at a time, four per step (eight lanes a
         // row, rows 0 4 1 5 and 2 6 3 7: so two rows' swizzled chunks do not meet
@@ -576,7 +672,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 const bool bad = mx >= 0x7f800000u;   // a non-finite value: every score of the row NaN
                 const int e = max((int)(mx >> 23) - 127, -118);
                 const float f = bad ? 0.f : __int_as_float((135 - e) << 23);
-                if (l8 == 0u) b.half[i / kTileRows][0][row] = bad ? __int_as_float(0x7fffffff) : kScoreScale * __int_as_float((119 + e) << 23);
+                if (l8 == 0u) b.state[i / kTileRows][0][row] = bad ? __int_as_float(0x7fffffff) : kScoreScale * __int_as_float((119 + e) << 23);
                 uint8_t *q = qs + (i / kTileRows) * kQTile + (l8 & 1u) * 8u;
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) {
@@ -596,274 +692,135 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         if (lane == 0) mbar_arrive(&b.q_full);
         meet(3u, 32u * kConvWarp);   // the rows' factors are there
 
-        // Warps w and w + 4 of a tile share 32 rows. A warp whose wait ran out
-        // goes on through the barriers, without touching tensor memory.
-        const uint32_t t = warp >> 3, half = (warp >> 2) & 1u, quarter = warp & 3u, row = quarter * 32u + lane;
-        const uint32_t i = (one ? 0u : t * kTileRows) + row;
-        if (one || t < tiles) {
-            const uint32_t at = tmem + ((quarter * 32u) << 16) + 128u * t + 64u * half, g0 = 4u * half;
-            const float factor = b.half[one ? 0u : t][0][row];
-            if (one) meet(3u, 32u * kConvWarp);   // both groups have read it
-            const uint32_t open = (uint32_t)min(p0 + tr.at(one ? 0u : t * kTileRows).x, (uint64_t)0x7fffffffu);
+        // One thread per row, with the output of the tiles of keys before the current one in registers. A warp whose wait
+        // ran out goes on to the barriers, without touching tensor memory.
+        const uint32_t t = warp >> 2, quarter = warp & 3u, row = quarter * 32u + lane, base = ONE ? 0u : t * kTileRows;
+        if (ONE || t < tiles) {
+            const uint32_t at = tmem + ((quarter * 32u) << 16) + 128u * t, i = base + row;
+            const float factor = b.state[ONE ? 0u : t][0][row];
+            const uint32_t open = (uint32_t)min(p0 + tr.at(base).x, (uint64_t)0x7fffffffu);
             const uint32_t last = i < rows ? (uint32_t)min(p0 + tr.at(i).x, (uint64_t)0x7fffffffu) : open;
             const float *scales = (lane & 8u ? a.c.v_scale : a.c.k_scale) + head * a.c.n_blocks;
             auto scale_of = [&](uint32_t j) {
                 return __ldcg(scales + min(((j0 + j) * kTileKeys + 16u * (lane & 7u)) >> a.c.block_log2, a.c.n_blocks - 1u));
             };
-            const uint32_t j_first = one ? t : 0u, j_step = one ? 2u : 1u;
-            // m: the largest score of this thread's half; mw: of the row, the largest score + logarithm of the V scale,
-            // against which weights are taken; l: this half's sum of weights without their V scales, times 2^k, k the
-            // integer below mw - m that keeps it in range
+            constexpr uint32_t j_step = ONE ? 2u : 1u;
+            const uint32_t j_first = ONE ? t : 0u;
+            // m: the row's largest score; mw: the largest score + logarithm of the V scale, against which weights are
+            // taken; l: the sum of weights without their V scales, times 2^k, k the integer below mw - m that keeps it in
+            // range
             float m = -INFINITY, l = 0.f, mw = -INFINITY, next = j_first < n ? scale_of(j_first) : 0.f;
             int k = 0;
-            uint32_t turn = 0u;
-            float4 acc[16];   // the output of the segments before the current one, in local memory (128 KB for the CTA)
-            bool ok = true;
-            for (uint32_t j = j_first; j < n; j += j_step, ++turn) {
-                if (turn && turn % kSegment == 0u) {   // while the next scores are made
-                    ok = ok && wait_warp(&b.o_full[t], (turn / kSegment - 1u) & 1u, err);
-                    fence_after();
-                    constexpr float kGain = 1.0f + kLoss * kAmends;
-#pragma unroll 1
-                    for (uint32_t c = 0; ok && c < 4u; ++c) {
-                        float o[16];
-                        tmem_ld(at + 256u + 16u * c, o);
-                        tmem_wait_ld(o);
+            uint64_t acc[kDim / 2];   // two dimensions each
 #pragma unroll
-                        for (uint32_t k = 0; k < 4u; ++k) {
-                            float4 y = turn == kSegment ? make_float4(0.f, 0.f, 0.f, 0.f) : acc[4u * c + k];
-                            y.x = fmaf(o[4 * k], kGain, y.x);
-                            y.y = fmaf(o[4 * k + 1], kGain, y.y);
-                            y.z = fmaf(o[4 * k + 2], kGain, y.z);
-                            y.w = fmaf(o[4 * k + 3], kGain, y.w);
-                            acc[4u * c + k] = y;
-                        }
-                    }
+            for (int c = 0; c < (int)kDim / 2; ++c) acc[c] = 0ull;
+            bool ok = true;
+            auto take_output = [&](uint32_t turn) {
+                ok = ok && wait_warp(&b.o_full[t], turn & 1u, err);
+                fence_after();
+                if (!ok) return;
+                float o[2][16];
+                tmem_ld(at + 256u, o[0]);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    tmem_wait_ld(o[c & 1]);
+                    if (c < 7) tmem_ld(at + 256u + 16u * (uint32_t)(c + 1), o[(c + 1) & 1]);
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) acc[8 * c + d] = add2(acc[8 * c + d], pair(o[c & 1][2 * d], o[c & 1][2 * d + 1]));
                 }
-                // a V scale of 0 counts as fp32's smallest number, 2^-149
-                Scales sc;
-                sc.scale = next == 0.f && lane >= 8u ? __uint_as_float(1u) : next;
-                sc.log2 = __log2f(sc.scale);
-                if (sc.log2 < -149.0f) sc.log2 = -149.0f;
+            };
+            for (uint32_t j = j_first; j < n; j += j_step) {
+                const uint32_t turn = j / j_step;
+                if (turn) take_output(turn - 1u);   // while the next scores are made
+                const Scales sc = scales_from(next, lane);
                 if (j + j_step < n) next = scale_of(j + j_step);
-                const uint32_t key0 = (j0 + j) * kTileKeys, mine = key0 + 64u * half;
+                const uint32_t key0 = (j0 + j) * kTileKeys;
                 const bool masked = key0 + kTileKeys - 1u > open;   // some row does not see all of the tile
-                const int nvis = last < mine ? 0 : (int)min(last - mine + 1u, 64u);
+                const int nvis = last < key0 ? 0 : (int)min(last - key0 + 1u, kTileKeys);
                 ok = ok && wait_warp(&b.s_full[t], turn & 1u, err);
                 fence_after();
-                float x = -INFINITY, xw = -INFINITY;
-                if (ok) x = masked ? tile_max<true>(at, sc, g0, factor, nvis, xw) : tile_max<false>(at, sc, g0, factor, 64, xw);
+                if (!ok) break;
+                float xw;
+                const float x = masked ? tile_max<true>(at, sc, factor, nvis, xw) : tile_max<false>(at, sc, factor, kTileKeys, xw);
                 const float was = m, before = mw;
                 if (x > m + kLazy) m = x;
-                const bool raise = meet_any(1u + t, 256u, xw > mw + kLazy);
-                const bool amends = turn % kSegment && turn % kAmends == 0u;
-                if (raise || amends) {
-                    float fv = 1.0f;   // what the output is rescaled by
-                    if (raise) {
-                        b.half[t][half][row] = xw;
-                        meet(1u + t, 256u);
-                        xw = fmaxf(xw, b.half[t][half ^ 1u][row]);
-                        if (xw > mw + kLazy) {
-                            fv = mw == -INFINITY ? 0.f : ex2(mw - xw);
-                            mw = xw;
-                        }
-                    }
-                    if (turn >= kSegment && __any_sync(0xffffffffu, fv != 1.0f))
-#pragma unroll 1
-                        for (uint32_t c = 0; c < 16u; ++c) acc[c] = make_float4(acc[c].x * fv, acc[c].y * fv, acc[c].z * fv, acc[c].w * fv);
-                    if (amends) fv *= 1.0f + kLoss * kAmends;
-                    if (turn % kSegment && ok) {
-#pragma unroll 1
-                        for (uint32_t c = 0; c < 64u; c += 16u) {
-                            float o[16];
-                            uint32_t u[16];
-                            tmem_ld(at + 256u + c, o);
-                            tmem_wait_ld(o);
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(o[k] * fv);
-                            tmem_st(at + 256u + c, u);
-                        }
-                    }
-                }
+                if (xw > mw + kLazy) mw = xw;
                 if (m != was || mw != before) {
                     const int now = below(mw - m);
                     l *= was == -INFINITY ? 0.f : ex2(before - mw + (float)(now - k));
                     k = now;
                 }
-                if (ok)
-                    l += masked ? tile_weights<true>(at, sc, g0, factor, nvis, mw - 6.0f, k)
-                                : tile_weights<false>(at, sc, g0, factor, 64, mw - 6.0f, k);
+                if (__any_sync(0xffffffffu, mw != before)) {
+                    const float fv = mw == before ? 1.0f : before == -INFINITY ? 0.f : ex2(before - mw);
+                    const uint64_t fv2 = pair(fv, fv);
+#pragma unroll
+                    for (int c = 0; c < (int)kDim / 2; ++c) acc[c] = mul2(acc[c], fv2);
+                }
+                l += masked ? tile_weights<true>(at, sc, factor, nvis, mw - 6.0f, k)
+                            : tile_weights<false>(at, sc, factor, kTileKeys, mw - 6.0f, k);
                 tmem_wait_st();
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&b.p_full[t]);
             }
-            // both halves' largest score and sum; a half that saw no position counts nothing
-            meet(1u + t, 256u);
-            b.half[t][half][row] = m;
-            meet(1u + t, 256u);
-            const float top = fmaxf(m, b.half[t][half ^ 1u][row]);
-            const int both = below(mw - top);
-            l = m == -INFINITY && l == 0.f ? 0.f : l * ex2((float)(both - k));
-            m = top;
-            meet(1u + t, 256u);
-            b.half[t][half][row] = l;
-            meet(1u + t, 256u);
-            l += b.half[t][half ^ 1u][row];
-            // the output into Q's place: row-major, 16-byte chunks XORed with the row
-            const bool have = turn && ok && wait_warp(&b.o_full[t], ((turn - 1u) / kSegment) & 1u, err);
-            fence_after();
-            const float gain = 1.0f + kLoss * (float)((turn - 1u) % kAmends + 1u);
-            // The output is acc 2^k / l. What is merged with other states is taken against the largest score instead, both
-            // times 2^(mw - m), less the 2^6 of the weights (and kOutUnit).
-            const bool whole = !one && C == 1u;
-            const float rest = m == -INFINITY ? 0.f : ex2(mw - m - (float)both) * 0x1p-6f;
-            const float back = (whole ? 1.0f / l : rest * kOutUnit) * ex2((float)both);
-            l *= rest;
+            if (j_first < n) take_output((n - 1u - j_first) / j_step);
+            // output = acc 2^k / l; what is merged is taken against the largest score: both times 2^(mw - m), less the 2^6 of
+            // the weights, and kOutUnit
+            const float rest = m == -INFINITY ? 0.f : ex2(mw - m - (float)k) * 0x1p-6f;
+            const float back = (ONE || C > 1u ? rest * kOutUnit : 1.0f / l) * ex2((float)k);
+            row_m = m;
+            row_l = l * rest;
             float4 *stage = reinterpret_cast<float4 *>(qs + t * kQTile);
-#pragma unroll 1
-            for (uint32_t c = 0; c < 4u; ++c) {
-                float o[16];
-                if (have) {
-                    tmem_ld(at + 256u + 16u * c, o);
-                    tmem_wait_ld(o);
-                }
 #pragma unroll
-                for (uint32_t k = 0; k < 4u; ++k) {
-                    const float4 y = turn > kSegment ? acc[4u * c + k] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    o[4 * k] = fmaf(o[4 * k], gain, y.x);
-                    o[4 * k + 1] = fmaf(o[4 * k + 1], gain, y.y);
-                    o[4 * k + 2] = fmaf(o[4 * k + 2], gain, y.z);
-                    o[4 * k + 3] = fmaf(o[4 * k + 3], gain, y.w);
-                }
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k)
-                    stage[row * 32u + ((16u * half + 4u * c + k) ^ (row & 31u))] =
-                        have ? make_float4(o[4 * k] * back, o[4 * k + 1] * back, o[4 * k + 2] * back, o[4 * k + 3] * back)
-                             : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t c = 0; c < kDim / 4u; ++c) {
+                float4 v;
+                unpair(acc[2 * c], v.x, v.y);
+                unpair(acc[2 * c + 1], v.z, v.w);
+                stage[row * 32u + (c ^ (row & 31u))] = make_float4(v.x * back, v.y * back, v.z * back, v.w * back);
             }
-            if (one) {
-                // both groups' states of a row -> one, in the place of group 0's
-                meet(3u, 32u * kConvWarp);   // the sums have been read
-                if (half == 0u) {
-                    b.half[t][0][row] = m;
-                    b.half[t][1][row] = l;
-                }
+            if constexpr (ONE) {
+                // both groups' states of a row -> one, in the place of group 0's; a state that saw no position counts nothing
+                meet(3u, 32u * kConvWarp);   // both groups have the rows' factors
+                b.state[t][0][row] = row_m;
+                b.state[t][1][row] = row_l;
                 meet(3u, 32u * kConvWarp);
-                const float m1 = b.half[t ^ 1u][0][row], l1 = b.half[t ^ 1u][1][row], M = fmaxf(m, m1);
-                // what the own state counts; a state that saw no position counts nothing
-                const float own = m == -INFINITY && l == 0.f ? 0.f : ex2(m - M), other = m1 == -INFINITY && l1 == 0.f ? 0.f : ex2(m1 - M);
+                const float m1 = b.state[t ^ 1u][0][row], l1 = b.state[t ^ 1u][1][row], M = fmaxf(row_m, m1);
+                const float own = row_m == -INFINITY && row_l == 0.f ? 0.f : ex2(row_m - M), other = m1 == -INFINITY && l1 == 0.f ? 0.f : ex2(m1 - M);
+                row_l = row_l * own + l1 * other;
                 row_m = M;
-                row_l = l * own + l1 * other;
                 meet(3u, 32u * kConvWarp);
-                if (half == 0u) b.half[t][0][row] = C > 1u ? own : own * (1.0f / kOutUnit) / row_l;
+                b.state[t][0][row] = C > 1u ? own : own * (1.0f / kOutUnit) / row_l;
+                meet(3u, 32u * kConvWarp);
             } else {
-                row_m = m;
-                row_l = l;
+                meet(1u + t, 128u);
             }
-            if (one) meet(3u, 32u * kConvWarp);
-            else meet(1u + t, 256u);
-            if (C == 1u || one) {
-                // rows of the tile for this warp: 16, or 8 where both groups have one tile
-                const uint32_t each = one ? 8u : 16u, w0 = (one ? warp : warp & 7u) * each, end = rows - (one ? 0u : t * kTileRows);
+            if (ONE || C == 1u) {
                 const bool failed = *err != kStatusOk;
-                float4 *const other = reinterpret_cast<float4 *>(qs + kQTile);
-                stage = reinterpret_cast<float4 *>(qs + (one ? 0u : t * kQTile));
-#pragma unroll 4
-                for (uint32_t k = w0; k < w0 + each; ++k) {
-                    const uint32_t at4 = k * 32u + (lane ^ (k & 31u));
+                const uint32_t each = ONE ? 16u : 32u, w0 = (ONE ? warp : quarter) * each;   // rows of the tile for this warp
+                stage = reinterpret_cast<float4 *>(qs + (ONE ? 0u : t * kQTile));
+#pragma unroll 8
+                for (uint32_t i0 = w0; i0 < w0 + each; ++i0) {
+                    const uint32_t at4 = i0 * 32u + (lane ^ (i0 & 31u));
                     float4 x = stage[at4];
-                    if (one) {
-                        const float4 y = other[at4];
-                        const float f0 = b.half[0][0][k], f1 = b.half[1][0][k];
+                    if constexpr (ONE) {
+                        const float4 y = reinterpret_cast<float4 *>(qs + kQTile)[at4];
+                        const float f0 = b.state[0][0][i0], f1 = b.state[1][0][i0];
                         x = make_float4(x.x * f0 + y.x * f1, x.y * f0 + y.y * f1, x.z * f0 + y.z * f1, x.w * f0 + y.w * f1);
+                        if (C > 1u) {
+                            stage[at4] = x;
+                            continue;
+                        }
                     }
-                    if (C > 1u) {
-                        stage[at4] = x;
-                        continue;
-                    }
-                    const uint2 r = tr.at((one ? 0u : t * kTileRows) + k);
+                    const uint2 r = tr.at(base + i0);
                     if (failed || p0 + r.x >= a.c.max_context) x.x = x.y = x.z = x.w = __int_as_float(0x7fffffff);
-                    if (k < end)
-                        reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo +
-                                                   (size_t)(h * a.group + r.y) * kDim)[lane] = x;
+                    if (base + i0 < rows)
+                        reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + r.x) * a.ldo + (size_t)(h * a.group + r.y) * kDim)[lane] = x;
                 }
             }
         }
     }
-    fence_before();
-    __syncthreads();
-    if (warp == kMmaWarp) {
-        fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    }
-    if (C == 1u) return;
-    // the converters' slots are free now (a state per row: of the first group where the groups shared the rows)
-    if (warp < kConvWarp && (warp & 4u) == 0u) {
-        rs.max[warp >> 3][(warp & 3u) * 32u + lane] = row_m;
-        rs.sum[warp >> 3][(warp & 3u) * 32u + lane] = row_l;
-    }
-    // Rows rank, rank + C, ... of the cluster's states, four at a time per warp:
-    // lane = (row, CTA) for the maxima and sums, then 4 dimensions. A state that
-    // saw no position counts nothing.
-    static_assert(kMaxSplit == 8, "eight lanes per row");
-    cluster_sync();
-    for (uint32_t k0 = 4u * warp; rank + C * k0 < rows; k0 += 4u * (kPromptThreads / 32u)) {
-        // two CTAs' outputs are on their way meanwhile
-        float4 y[2][4];
-        auto load = [&](float4(&to)[4], uint32_t c) {
-#pragma unroll
-            for (uint32_t v = 0; v < 4; ++v) {
-                const uint32_t r = min(rank + C * (k0 + v), rows - 1u), row = r & (kTileRows - 1u);
-                to[v] = ld_cluster4(reinterpret_cast<const float4 *>(qs + (r / kTileRows) * kQTile) + row * 32u + (lane ^ (row & 31u)), c);
-            }
-        };
-        auto add = [&](float4(&x)[4], const float4(&from)[4], float f, uint32_t c) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const float fc = __shfl_sync(0xffffffffu, f, 8 * v + (int)c);
-                x[v].x = fmaf(fc, from[v].x, x[v].x);
-                x[v].y = fmaf(fc, from[v].y, x[v].y);
-                x[v].z = fmaf(fc, from[v].z, x[v].z);
-                x[v].w = fmaf(fc, from[v].w, x[v].w);
-            }
-        };
-        load(y[0], 0u);
-        load(y[1], 1u);
-        const uint32_t u = lane >> 3, cta = lane & 7u, i = rank + C * (k0 + u);
-        const bool there = cta < C && i < rows;
-        const float mc = there ? ld_cluster1(&rs.max[i / kTileRows][i & (kTileRows - 1u)], cta) : -INFINITY;
-        const float lc = there ? ld_cluster1(&rs.sum[i / kTileRows][i & (kTileRows - 1u)], cta) : 0.f;
-        const bool bad = there && __float_as_uint(ld_cluster1(&b.status, cta)) != kStatusOk;
-        float M = mc;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float f = mc == -INFINITY && lc == 0.f ? 0.f : ex2(mc - M);
-        float L = f * lc;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        const bool any_bad = __any_sync(0xffffffffu, bad);
-        float4 x[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) x[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t c = 0; c < C; c += 2u) {
-            add(x, y[0], f, c);
-            if (c + 2u < C) load(y[0], c + 2u);
-            if (c + 1u < C) add(x, y[1], f, c + 1u);
-            if (c + 3u < C) load(y[1], c + 3u);
-        }
-#pragma unroll
-        for (uint32_t v = 0; v < 4; ++v) {
-            const uint32_t r = rank + C * (k0 + v);
-            const float sum = __shfl_sync(0xffffffffu, L, 8 * v);
-            if (r >= rows) continue;
-            const uint2 at = tr.at(r);
-            const float inv = any_bad || p0 + at.x >= a.c.max_context ? __int_as_float(0x7fffffff) : (1.0f / kOutUnit) / sum;
-            reinterpret_cast<float4 *>(a.out + ((size_t)s * a.r.tokens + at.x) * a.ldo + (size_t)(h * a.group + at.y) * kDim)[lane] =
-                make_float4(x[v].x * inv, x[v].y * inv, x[v].z * inv, x[v].w * inv);
-        }
-    }
-    cluster_sync();   // no CTA leaves while the cluster may read its states
+    leave();
+    if (C > 1u) merge();
 }
 
 }  // namespace
@@ -874,10 +831,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 // units; what does goes by the time: a tile of keys takes 4400 cycles with one
 // tile of rows and 6300 with two, what is before and after 14500 and 18000, a
 // merge of two tiles 10000 (of one, nothing that shows). Measured on 333 tokens
-// over 5001 positions (44 units of two tiles: 160 / 89 / 67 us as 1 / 2 / 3
-// CTAs), 64 units of one tile as 2 CTAs each (2000 and 16000 positions: 28 and
-// 161 us) and 512 tokens (112 units of one tile 17.3 us, 56 of two 23.6 us, as 2
-// CTAs each 20.5 us).
+// over 5001 positions (44 units of two tiles: 150 / 87 / 68 us as 1 / 2 / 3
+// CTAs), 64 units of one tile as 2 CTAs each (2000 and 16000 positions: 32 and
+// 193 us) and 512 tokens (112 units of one tile 19.4 us, 56 of two 26.9 us, as 2
+// CTAs each 23.2 us). The positions are those that the cache has room for, not
+// those of the call, which only the device knows.
 PromptCut prompt_cut(const AttnArgs &a, int sms)
 {
     const uint32_t rows = a.r.tokens * a.group, keys = (a.c.max_context + kTileKeys - 1) / kTileKeys;
@@ -900,12 +858,13 @@ PromptCut prompt_cut(const AttnArgs &a, int sms)
 // Attention of many query rows; see AttnArgs
 cudaError_t launch_prompt(AttnArgs a, const PromptCut &cut, int dev, int sms, cudaStream_t stream)
 {
-    cudaError_t e = allow<prompt_kernel>(dev, (int)kPromptSmem);
-    if (e != cudaSuccess) return e;
     const uint32_t rows = a.r.tokens * a.group, C = cut.split;
-    a.cta_tiles = cut.tiles;
-    a.tiles = (rows + a.cta_tiles * kTileRows - 1) / (a.cta_tiles * kTileRows);
-    return launch(prompt_kernel, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), kPromptThreads, kPromptSmem, C, a, sms, stream);
+    a.tiles = (rows + cut.tiles * kTileRows - 1) / (cut.tiles * kTileRows);
+    const dim3 grid(C * a.tiles, a.c.kv_heads, a.c.nseq);
+    cudaError_t e = cut.tiles == 1 ? allow<prompt_kernel<true>>(dev, (int)kPromptSmem) : allow<prompt_kernel<false>>(dev, (int)kPromptSmem);
+    if (e != cudaSuccess) return e;
+    return cut.tiles == 1 ? launch(prompt_kernel<true>, grid, kPromptThreads, kPromptSmem, C, a, sms, stream)
+                          : launch(prompt_kernel<false>, grid, kPromptThreads, kPromptSmem, C, a, sms, stream);
 }
 
 }  // namespace k8
