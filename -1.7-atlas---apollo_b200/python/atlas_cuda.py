@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_DIR, "libatlas_cuda.so")
@@ -407,6 +408,11 @@ def gemm(type_id: int, d_w, rows: int, cols: int, d_x, tokens: int, d_y, stream:
                                 ctypes.c_void_p(stream)), "atlas_cuda_gemm")
 
 
+def _kind(t) -> str:
+    """The name of a tensor's element type."""
+    return str(t.dtype).rpartition(".")[2]
+
+
 class Kv8Cache:
     """An 8-bit KV cache of one layer in caller-owned device buffers (AtlasKv8, include/atlas_cuda.h).
 
@@ -416,9 +422,9 @@ class Kv8Cache:
 
     def __init__(self, k, v, k_scale, v_scale, k_sum=None, *, nseq: int, kv_heads: int, max_context: int, block: int):
         blocks = -(-max_context // block) if block > 0 else 0
-        for t, n, size in ((k, max_context * 128, 1), (v, max_context * 128, 1), (k_scale, blocks, 4),
-                           (v_scale, blocks, 4), (k_sum, blocks * 128, 2)):
-            if hasattr(t, "is_contiguous") and (not t.is_contiguous() or t.element_size() != size
+        for t, n, kind in ((k, max_context * 128, "int8"), (v, max_context * 128, "int8"), (k_scale, blocks, "float32"),
+                           (v_scale, blocks, "float32"), (k_sum, blocks * 128, "int16")):
+            if hasattr(t, "is_contiguous") and (not t.is_contiguous() or _kind(t) != kind
                                                 or t.numel() != nseq * kv_heads * n):
                 raise ValueError("Kv8Cache: a buffer of another size or type, or one that is not dense")
         self.buffers = (k, v, k_scale, v_scale, k_sum)
@@ -426,15 +432,64 @@ class Kv8Cache:
         self.desc = Kv8Desc(*(None if t is None else t.data_ptr() for t in self.buffers), nseq, kv_heads, max_context,
                             block)
         self._ref = ctypes.byref(self.desc)
+        # the types that the calls look for first, where the buffers are torch's
+        self._f32 = getattr(k_scale, "dtype", None)
+        self._i32 = sys.modules["torch"].int32 if "torch" in sys.modules else None
 
 
 def _addr(t):
     return None if t is None else t.data_ptr()
 
 
+def _kv8_ints(who: str, name: str, t, n: int) -> None:
+    """Refuses a tensor that does not begin with n dense 32-bit integers."""
+    if t is not None and hasattr(t, "dtype") and (
+            _kind(t) not in ("int32", "uint32") or t.numel() < n or not t.is_contiguous()):
+        raise AtlasError(-1, f"{who}: {name} must be {n} dense 32-bit integers")
+
+
+def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: int) -> None:
+    """Refuses a tensor that is not token rows [nseq, tokens, heads, 128], ld floats from token to token (0: dense). One that
+    is not 4-dimensional must be dense, and long enough."""
+    if not tokens or not hasattr(t, "dtype"):
+        return
+    step = ld or heads * 128
+    if t.dim() == 4:
+        shape, stride = t.shape, t.stride()
+        ok = (shape[0] >= nseq and shape[1] >= tokens and shape[2] >= heads and shape[3] == 128 and stride[3] == 1
+              and (heads == 1 or stride[2] == 128) and (tokens == 1 or stride[1] == step)
+              and (nseq == 1 or stride[0] == tokens * step))
+    else:
+        ok = t.is_contiguous() and t.numel() >= (nseq * tokens - 1) * step + heads * 128
+    if not ok or _kind(t) != "float32":
+        raise AtlasError(-1, f"{who}: {name} must be float32 rows of {nseq} sequences x {tokens} tokens x {heads} heads x 128, "
+                             f"{step} floats from token to token")
+
+
+def _kv8_check(who: str, cache: Kv8Cache, tokens: int, heads: int, pos0, n_tok, names, a, lda: int, b, ldb: int) -> None:
+    """Refuses tensors of another type, layout or size. a, b: rows of `heads` each. Dense ones of just the size, as most
+    calls have, pass at once."""
+    n = cache.nseq
+    size, f32, i32 = n * tokens * heads * 512, cache._f32, cache._i32
+    try:
+        if (a.dtype is f32 and b.dtype is f32 and pos0.dtype is i32 and a.nbytes == size and b.nbytes == size
+                and pos0.nbytes == 4 * n and a.is_contiguous() and b.is_contiguous() and pos0.is_contiguous()
+                and (n_tok is None or n_tok.dtype is i32 and n_tok.nbytes == 4 * n and n_tok.is_contiguous())
+                and not lda and not ldb):
+            return
+    except AttributeError:   # not a tensor, but an object with an address: what can be seen of it is checked
+        pass
+    _kv8_rows(who, names[0], a, n, tokens, heads, lda)
+    _kv8_rows(who, names[1], b, n, tokens, heads, ldb)
+    _kv8_ints(who, "pos0", pos0, n)
+    _kv8_ints(who, "n_tok", n_tok, n)
+
+
 def kv8_append(cache: Kv8Cache, tokens: int, pos0, k, v, n_tok=None, ld: int = 0, stream: int = 0) -> None:
     """Stores up to `tokens` new rows k, v [nseq, tokens, kv_heads, 128] of each sequence s at positions pos0[s], ...
-    (pos0, n_tok: 32-bit device integers; n_tok None: all of them). atlas_cuda_kv8_append."""
+    (pos0, n_tok: 32-bit device integers; n_tok None: all of them). atlas_cuda_kv8_append. Here and below, `stream` is a
+    cudaStream_t (0: the legacy default stream), and tensors of another type, layout or size are refused."""
+    _kv8_check("kv8_append", cache, tokens, cache.kv_heads, pos0, n_tok, ("k", "v"), k, ld, v, ld)
     check(lib().atlas_cuda_kv8_append(cache._ref, tokens, pos0.data_ptr(), _addr(n_tok), k.data_ptr(), v.data_ptr(), ld,
                                       stream), "kv8_append")
 
@@ -442,6 +497,7 @@ def kv8_append(cache: Kv8Cache, tokens: int, pos0, k, v, n_tok=None, ld: int = 0
 def kv8_read(cache: Kv8Cache, tokens: int, pos0, k, v, n_tok=None, ld: int = 0, stream: int = 0) -> None:
     """The rows at positions pos0[s], ... as the values that they stand for, into k, v [nseq, tokens, kv_heads, 128].
     atlas_cuda_kv8_read."""
+    _kv8_check("kv8_read", cache, tokens, cache.kv_heads, pos0, n_tok, ("k", "v"), k, ld, v, ld)
     check(lib().atlas_cuda_kv8_read(cache._ref, tokens, pos0.data_ptr(), _addr(n_tok), k.data_ptr(), v.data_ptr(), ld,
                                     stream), "kv8_read")
 
@@ -449,6 +505,7 @@ def kv8_read(cache: Kv8Cache, tokens: int, pos0, k, v, n_tok=None, ld: int = 0, 
 def kv8_attn(cache: Kv8Cache, q_heads: int, tokens: int, pos0, q, out, n_tok=None, ldq: int = 0, ldo: int = 0,
              stream: int = 0) -> None:
     """Causal attention of q [nseq, tokens, q_heads, 128] over the cache into out. atlas_cuda_kv8_attn."""
+    _kv8_check("kv8_attn", cache, tokens, q_heads, pos0, n_tok, ("q", "out"), q, ldq, out, ldo)
     check(lib().atlas_cuda_kv8_attn(cache._ref, q_heads, tokens, pos0.data_ptr(), _addr(n_tok), q.data_ptr(), ldq,
                                     out.data_ptr(), ldo, stream), "kv8_attn")
 
@@ -457,6 +514,8 @@ def kv8_attn_sparse(cache: Kv8Cache, q_heads: int, tokens: int, n_sel: int, pos0
                     ldo: int = 0, stream: int = 0) -> None:
     """Attention over the n_sel blocks that each token and KV head selects; sel [nseq, tokens, kv_heads, n_sel] (int32)
     receives them. atlas_cuda_kv8_attn_sparse."""
+    _kv8_check("kv8_attn_sparse", cache, tokens, q_heads, pos0, n_tok, ("q", "out"), q, ldq, out, ldo)
+    _kv8_ints("kv8_attn_sparse", "sel", sel, cache.nseq * tokens * cache.kv_heads * n_sel)
     check(lib().atlas_cuda_kv8_attn_sparse(cache._ref, q_heads, tokens, n_sel, pos0.data_ptr(), _addr(n_tok),
                                            q.data_ptr(), ldq, out.data_ptr(), ldo, sel.data_ptr(), stream),
           "kv8_attn_sparse")
