@@ -1373,13 +1373,20 @@ int done(const char *who, cudaError_t e)
     return api_fail(ATLAS_ECUDA, "%s: %s", who, cudaGetErrorString(e));
 }
 
+// CTAs that share a unit's positions; the kernel is allowed its shared memory before
+template <int NT, uint32_t W>
+uint32_t attn_cluster(const FewArgs &a, int dev)
+{
+    const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
+    return cluster_of<attn_kernel<NT, W>>(dev, W * 32, sizeof(Smem<NT, W>), units, a.c.max_context);
+}
+
 template <int NT, uint32_t W>
 cudaError_t launch_attn(const FewArgs &a, int dev, int sms, cudaStream_t stream)
 {
     cudaError_t e = allow<attn_kernel<NT, W>>(dev, (int)kMaxSmem);
     if (e != cudaSuccess) return e;
-    const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
-    const uint32_t C = cluster_of<attn_kernel<NT, W>>(dev, W * 32, sizeof(Smem<NT, W>), units, a.c.max_context);
+    const uint32_t C = attn_cluster<NT, W>(a, dev);
     return launch(attn_kernel<NT, W>, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), W * 32, sizeof(Smem<NT, W>), C, a, sms, stream);
 }
 
@@ -1394,7 +1401,7 @@ uint64_t few_cycles(const FewArgs &a, int dev)
     constexpr auto kernel = attn_kernel<2, 8>;
     if (allow<kernel>(dev, (int)kMaxSmem) != cudaSuccess) return 0;   // the launch will say so
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * a.tiles;
-    const uint32_t C = cluster_of<kernel>(dev, 256, sizeof(Smem<2, 8>), units, a.c.max_context);
+    const uint32_t C = attn_cluster<2, 8>(a, dev);
     const uint64_t at_once = std::max(clusters_at_once<kernel>(dev, C, 256, sizeof(Smem<2, 8>)), 1u);
     return (units + at_once - 1) / at_once * ((a.c.max_context + C - 1) / C) * 37 / 2 + 9000;
 }
@@ -1490,6 +1497,47 @@ int attn_args(const char *who, const AtlasKv8 *cache, uint32_t q_heads, uint32_t
 
 }  // namespace
 
+namespace {
+
+// The form of a call: `one` (up to eight rows per KV head), else prompt or not; fills a.tiles for the few-rows forms
+struct AttnForm {
+    bool one, prompt;
+    PromptCut cut;
+};
+
+AttnForm attn_form(FewArgs &a, int dev, int sms)
+{
+    const uint32_t rows = a.r.tokens * a.group;
+    AttnForm f{rows <= 8, false, {}};
+    a.tiles = f.one ? 1 : (rows + 15) / 16;
+    if (!f.one) {
+        f.cut = prompt_cut(a, sms);
+        f.prompt = f.cut.cycles < few_cycles(a, dev);
+    }
+    return f;
+}
+
+}  // namespace
+
+extern "C" int atlas_cuda_kv8_attn_form(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, uint32_t *rows, uint32_t *ctas)
+{
+    const char *who = "kv8_attn_form";
+    FewArgs a{};
+    int dev, sms;
+    if (!cache || !rows || !ctas) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
+    // rows and positions are not looked at: any memory that passes as theirs
+    const int rc = attn_args(who, cache, q_heads, tokens, reinterpret_cast<const uint32_t *>(cache->k_scale), nullptr,
+                             static_cast<const float *>(cache->k), 0, static_cast<float *>(cache->v), 0, a, dev, sms);
+    if (rc != ATLAS_OK) return rc;
+    if (!tokens) return api_fail(ATLAS_EINVAL, "%s: no tokens", who);
+    const AttnForm f = attn_form(a, dev, sms);
+    const cudaError_t e = allow<attn_kernel<1, 16>>(dev, (int)kMaxSmem);
+    if (e != cudaSuccess) return done(who, e);
+    *rows = f.one ? 8 : f.prompt ? 128 * f.cut.tiles : 16;
+    *ctas = f.one ? attn_cluster<1, 16>(a, dev) : f.prompt ? f.cut.split : attn_cluster<2, 8>(a, dev);
+    return ATLAS_OK;
+}
+
 extern "C" int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
                                    const uint32_t *d_ntok, const float *d_q, uint64_t ldq, float *d_out, uint64_t ldo,
                                    void *stream)
@@ -1499,15 +1547,10 @@ extern "C" int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint
     int dev, sms;
     int rc = attn_args(who, cache, q_heads, tokens, d_pos0, d_ntok, d_q, ldq, d_out, ldo, a, dev, sms);
     if (rc != ATLAS_OK || !tokens) return rc;
-    const uint32_t rows = tokens * a.group;
-    const bool one = rows <= 8;
-    a.tiles = one ? 1 : (rows + 15) / 16;
-    if (!one) {
-        const PromptCut cut = prompt_cut(a, sms);
-        if (cut.cycles < few_cycles(a, dev)) return done(who, launch_prompt(a, cut, dev, sms, (cudaStream_t)stream));
-    }
+    const AttnForm f = attn_form(a, dev, sms);
+    if (f.prompt) return done(who, launch_prompt(a, f.cut, dev, sms, (cudaStream_t)stream));
     if ((rc = map_codes(who, a)) != ATLAS_OK) return rc;
-    return done(who, one ? launch_attn<1, 16>(a, dev, sms, (cudaStream_t)stream)
+    return done(who, f.one ? launch_attn<1, 16>(a, dev, sms, (cudaStream_t)stream)
                          : launch_attn<2, 8>(a, dev, sms, (cudaStream_t)stream));
 }
 

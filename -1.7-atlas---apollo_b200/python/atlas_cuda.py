@@ -31,6 +31,7 @@ EXPORTS = [
     "atlas_cuda_device_ms", "atlas_cuda_trace_graph", "atlas_cuda_gemv_noalloc", "atlas_cuda_tp_slice", "atlas_cuda_tp_handle",
     "atlas_cuda_tp_connect", "atlas_cuda_prefill_seq", "atlas_cuda_generate_batch", "atlas_cuda_decode_batch",
     "atlas_cuda_kv8_append", "atlas_cuda_kv8_read", "atlas_cuda_kv8_attn", "atlas_cuda_kv8_attn_sparse",
+    "atlas_cuda_kv8_attn_form",
     "brain_gpu_init", "brain_gpu_matvec_batch", "brain_gpu_matvec", "brain_gpu_shutdown",
     "atlas_rt_open", "atlas_rt_close", "atlas_rt_error", "atlas_rt_shape", "atlas_rt_data_base",
     "atlas_rt_find_tensor", "atlas_rt_file_bytes", "atlas_rt_device", "atlas_rt_forward_token",
@@ -154,6 +155,7 @@ def lib() -> ctypes.CDLL:
         L.atlas_cuda_kv8_append.argtypes = [P, U32, P, P, P, P, U64, P]
         L.atlas_cuda_kv8_read.argtypes = [P, U32, P, P, P, P, U64, P]
         L.atlas_cuda_kv8_attn.argtypes = [P, U32, U32, P, P, P, U64, P, U64, P]
+        L.atlas_cuda_kv8_attn_form.argtypes = [P, U32, U32, P, P]
         L.atlas_cuda_kv8_attn_sparse.argtypes = [P, U32, U32, U32, P, P, P, U64, P, U64, P, P]
         L.atlas_synth_write_gguf.argtypes = [P, ctypes.c_char_p]
         L.atlas_synth_q4k_blocks.argtypes = [U64, U64, P, U64]
@@ -508,6 +510,15 @@ def kv8_attn(cache: Kv8Cache, q_heads: int, tokens: int, pos0, q, out, n_tok=Non
     _kv8_check("kv8_attn", cache, tokens, q_heads, pos0, n_tok, ("q", "out"), q, ldq, out, ldo)
     check(lib().atlas_cuda_kv8_attn(cache._ref, q_heads, tokens, pos0.data_ptr(), _addr(n_tok), q.data_ptr(), ldq,
                                     out.data_ptr(), ldo, stream), "kv8_attn")
+
+
+def kv8_attn_form(cache: Kv8Cache, q_heads: int, tokens: int) -> tuple:
+    """(rows of a KV head that a CTA takes, CTAs that share their positions) of such a kv8_attn on the current device.
+    atlas_cuda_kv8_attn_form."""
+    rows, ctas = ctypes.c_uint32(), ctypes.c_uint32()
+    check(lib().atlas_cuda_kv8_attn_form(cache._ref, q_heads, tokens, ctypes.byref(rows), ctypes.byref(ctas)),
+          "kv8_attn_form")
+    return rows.value, ctas.value
 
 
 def kv8_attn_sparse(cache: Kv8Cache, q_heads: int, tokens: int, n_sel: int, pos0, q, out, sel, n_tok=None, ldq: int = 0,

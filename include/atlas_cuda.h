@@ -295,7 +295,15 @@ int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens
                         const uint32_t *d_ntok, const float *d_q, uint64_t ldq, float *d_out, uint64_t ldo,
                         void *stream);
 
-/* The same over n_sel (1 .. 4096) blocks per token and KV head: the block of
+/* How a call of these sizes would be run on the current device, for who
+   measures or tests it: the query rows of a KV head that a CTA takes at most
+   (rows: 8 or 16, the forms for few rows; 128 or 256, those for prompts), and
+   how many CTAs share their positions. It goes by the positions that the cache
+   has room for (max_context), not by those of a call. */
+int atlas_cuda_kv8_attn_form(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, uint32_t *rows,
+                             uint32_t *ctas);
+
+/* Attention over n_sel (1 .. 4096) blocks per token and KV head: the block of
    the token's own position, and the n_sel - 1 blocks before it with the highest
    scores (all of them where there are no more). Score of a block: (c . k_sum) *
    k_scale, where c = rint(127 qbar / max|qbar|) and qbar is the sum of the
