@@ -576,8 +576,8 @@ __device__ __forceinline__ void attend(const FewArgs &a, Smem<NT, W> &sm, const 
         float unit = sv * (kOutUnit / kWeightUnit);
         const bool steep = far >> (i & 31u) & 1u;
         if (__any_sync(0xffffffffu, raise) || steep) {
-            const float poison = sv != sv ? sv : 0.f;   // a NaN scale, into the rows that see the chunk
-            if (sv != sv) unit = 0.f;
+            const float poison = sv - sv;   // NaN for a scale that is NaN or infinite: into the rows that see the chunk
+            if (poison != 0.f) unit = 0.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float f[2] = {1.0f, 1.0f};
@@ -1527,7 +1527,7 @@ extern "C" int atlas_cuda_kv8_attn_form(const AtlasKv8 *cache, uint32_t q_heads,
     if (!cache || !rows || !ctas) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
     // rows and positions are not looked at: any memory that passes as theirs
     const int rc = attn_args(who, cache, q_heads, tokens, reinterpret_cast<const uint32_t *>(cache->k_scale), nullptr,
-                             static_cast<const float *>(cache->k), 0, static_cast<float *>(cache->v), 0, a, dev, sms);
+                             static_cast<const float *>(cache->k), 0, static_cast<float *>(cache->k) + 4, 0, a, dev, sms);
     if (rc != ATLAS_OK) return rc;
     if (!tokens) return api_fail(ATLAS_EINVAL, "%s: no tokens", who);
     const AttnForm f = attn_form(a, dev, sms);

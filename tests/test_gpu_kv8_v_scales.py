@@ -139,3 +139,31 @@ def test_zero_blocks_with_weight(torch_cuda, shape, zero):
              "every second": lambda b, n: b % 2 == 0}[zero]
     args = cache_and_queries(shape, 16, grown, -3.0, -np.inf)
     check(torch_cuda, *args)
+
+
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s != "single token"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_blocks_that_only_later_tokens_see_may_be_anything(torch_cuda, shape, bad, which):
+    """A scale of NaN or infinity shows in the rows that see its block, and leaves the others as they were."""
+    torch = torch_cuda
+    ref, q, pos, q_heads, n_sel = cache_and_queries(shape, 16, lambda b, n: b >= 0, 0.0, 0)
+    nseq, heads = ref.shape[:2]
+    tokens = q.shape[1]
+    blk = (pos + tokens - 1) // 16
+    out = []
+    for scale in (ref.vs[0, 0, blk], bad):
+        (ref.ks if which == "k" else ref.vs)[:, :, blk] = scale
+        dev = DevCache(torch, ref)
+        out.append(torch.zeros(nseq, tokens, q_heads, DIM, device="cuda"))
+        at = _i32(torch, [pos] * nseq)
+        if n_sel:
+            sel = torch.zeros(nseq, tokens, heads, n_sel, dtype=torch.int32, device="cuda")
+            atlas_cuda.kv8_attn_sparse(dev.c, q_heads, tokens, n_sel, at, _f32(torch, q), out[-1], sel)
+        else:
+            atlas_cuda.kv8_attn(dev.c, q_heads, tokens, at, _f32(torch, q), out[-1])
+    was, now = (x.cpu().numpy() for x in out)
+    sees = pos + np.arange(tokens) >= 16 * blk
+    if which == "v" or np.isnan(bad):   # an infinite K scale may make every score of the block -inf: no weight
+        assert not np.isfinite(now[:, sees]).all(-1).any()
+    np.testing.assert_array_equal(now[:, ~sees], was[:, ~sees])

@@ -1,5 +1,7 @@
 """CPU: the Python calls of the 8-bit KV cache refuse tensors of another type, layout or size before the library sees their
 addresses. (Tensors that pass get the library's own answer: no device, or memory of another one.)"""
+import ctypes
+
 import pytest
 
 import atlas_cuda
@@ -116,3 +118,15 @@ def test_cache_types():
                 (k, k, sc, sc, sums.view(torch.float16)), (k, k, sc, sc, sums.view(torch.bfloat16))):
         with pytest.raises(ValueError):
             atlas_cuda.Kv8Cache(*bad, **ok)
+
+
+def test_form_needs_a_cache_and_a_device(lib):
+    rows, ctas = ctypes.c_uint32(7), ctypes.c_uint32(7)
+    args = ctypes.byref(rows), ctypes.byref(ctas)
+    assert lib.atlas_cuda_kv8_attn_form(None, 4, 1, *args) == EINVAL
+    assert lib.atlas_cuda_kv8_attn_form(_cache()._ref, 4, 1, None, args[1]) == EINVAL
+    if not torch.cuda.is_available():
+        with pytest.raises(atlas_cuda.AtlasError) as e:
+            atlas_cuda.kv8_attn_form(_cache(), 4, 1)
+        assert e.value.code == -2
+    assert rows.value == ctas.value == 7
