@@ -1390,12 +1390,13 @@ cudaError_t launch_attn(const FewArgs &a, int dev, int sms, cudaStream_t stream)
     return launch(attn_kernel<NT, W>, dim3(C * a.tiles, a.c.kv_heads, a.c.nseq), W * 32, sizeof(Smem<NT, W>), C, a, sms, stream);
 }
 
-// The longest CTA's time in cycles for more than eight rows, to be compared with
-// the prompt form's: 18.5 per position of a tile of 16 rows (8 warps), 9000
-// before and after. Rows: this form, the prompt form, in us: one sequence of 28
-// heads on 4, 500 positions, 112: 7.2, 19; 8000, 42 and 112: 14.7, 27 and 25.7,
-// 28; 40 heads on 8, 30000, 20 and 65: 54, 83 and 160, 83; 8 sequences of them,
-// 2000, 20 and 35: 25, 28 and 50, 28; 16000: 165, 161 and 328, 161.
+// The longest CTA's time in cycles (1.8 per ns) for more than eight rows, to be
+// compared with the prompt form's: 18.5 per position of a tile of 16 rows (8
+// warps), 9000 before and after. Rows: this form, the prompt form, in us: one
+// sequence of 28 heads on 4, 500 positions, 112: 6.7, 15.3; 8000, 42 and 112:
+// 15.4, 28 and 27, 30; 40 heads on 8, 30000, 20 and 65: 57, 81 and 107, 82; 8
+// sequences of them, 2000, 20 and 35: 26, 32 and 51, 32; 16000: 166, 197 and 325,
+// 197.
 uint64_t few_cycles(const FewArgs &a, int dev)
 {
     constexpr auto kernel = attn_kernel<2, 8>;

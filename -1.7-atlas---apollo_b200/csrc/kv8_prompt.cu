@@ -825,17 +825,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 
 }  // namespace
 
-// How a call is cut up, and an estimate of its longest CTA's time in cycles.
-// Two tiles per CTA, or one; and up to 8 CTAs per unit, two tiles of keys each
-// at least. What does not fit the device at once takes two tiles and whole
-// units; what does goes by the time: a tile of keys takes 4400 cycles with one
-// tile of rows and 6300 with two, what is before and after 14500 and 18000, a
-// merge of two tiles 10000 (of one, nothing that shows). Measured on 333 tokens
-// over 5001 positions (44 units of two tiles: 150 / 87 / 68 us as 1 / 2 / 3
-// CTAs), 64 units of one tile as 2 CTAs each (2000 and 16000 positions: 32 and
-// 193 us) and 512 tokens (112 units of one tile 19.4 us, 56 of two 26.9 us, as 2
-// CTAs each 23.2 us). The positions are those that the cache has room for, not
-// those of the call, which only the device knows.
+// How a call is cut up, and an estimate of its longest CTA's time in cycles
+// (1.8 per ns, as few_cycles'). Two tiles per CTA, or one; and up to 8 CTAs per
+// unit, two tiles of keys each at least. What does not fit the device at once
+// takes two tiles and whole units; what does goes by the time: a tile of keys
+// takes 5400 cycles with one tile of rows and 6900 with two, what is before and
+// after 14500 and 18000, a merge of two tiles 10000 (of one, nothing that shows).
+// Measured, us, tiles of rows x CTAs per unit: 333 tokens over 5001 positions of
+// 16 heads on 2, one 132, two x 1 / 2 / 3 151 / 99 / 69; 512 tokens of 28 on 4,
+// one 20.0, two 27.4 and 23.8; 256 over 2048, one x 1 / 2 43.8 / 35.0, two x 2 /
+// 3 / 4 43.8 / 37.2 / 33.4; 8 sequences of 40 on 8, 35 rows over 2000 and 16000
+// positions, one x 2 32.7 and 196, two x 2 37.6 and 215. The positions are those
+// that the cache has room for, not those of the call, which only the device knows:
+// 512 tokens with room for 32768 take two x 2, 23.3 us.
 PromptCut prompt_cut(const AttnArgs &a, int sms)
 {
     const uint32_t rows = a.r.tokens * a.group, keys = (a.c.max_context + kTileKeys - 1) / kTileKeys;
@@ -844,13 +846,13 @@ PromptCut prompt_cut(const AttnArgs &a, int sms)
     for (uint32_t t = 1; t <= 2; ++t) {
         const uint64_t units = (rows + t * kTileRows - 1) / (t * kTileRows) * heads;
         for (uint32_t c = 1; c <= kMaxSplit && units * c <= (uint64_t)sms && (c == 1 || 2 * c <= keys); ++c) {
-            const uint64_t cycles = (uint64_t)(t == 1 ? 4400 : 6300) * ((keys + c - 1) / c) + (t == 1 ? 14500 : c == 1 ? 18000 : 28000);
+            const uint64_t cycles = (uint64_t)(t == 1 ? 5400 : 6900) * ((keys + c - 1) / c) + (t == 1 ? 14500 : c == 1 ? 18000 : 28000);
             if (cycles < best.cycles) best = PromptCut{t, c, cycles};
         }
     }
     if (best.cycles == ~0ull) {
         const uint64_t units = (rows + 2u * kTileRows - 1) / (2u * kTileRows) * heads;
-        best.cycles = (units + (uint64_t)sms - 1) / (uint64_t)sms * (6300ull * keys + 18000ull);
+        best.cycles = (units + (uint64_t)sms - 1) / (uint64_t)sms * (6900ull * keys + 18000ull);
     }
     return best;
 }

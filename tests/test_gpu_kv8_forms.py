@@ -109,3 +109,26 @@ def test_refusals(torch_cuda):
         with pytest.raises(atlas_cuda.AtlasError) as e:
             atlas_cuda.kv8_attn_form(c, q_heads, tokens)
         assert e.value.code == -1
+
+
+# The sizes at which both forms were measured: whichever took less time, in us (few rows, prompt)
+MEASURED = [
+    ((1, 28, 4, 16, 500), 6.7, 15.3), ((1, 28, 4, 6, 8000), 15.4, 28.0), ((1, 28, 4, 16, 8000), 27.1, 29.9),
+    ((1, 40, 8, 4, 30000), 57.1, 81.4), ((1, 40, 8, 13, 30000), 107.4, 82.3), ((8, 40, 8, 4, 2000), 26.1, 32.1),
+    ((8, 40, 8, 7, 2000), 50.7, 32.2), ((8, 40, 8, 4, 16000), 166.1, 196.8), ((8, 40, 8, 7, 16000), 324.6, 196.9),
+]
+
+
+def form_of(torch, nseq, q_heads, heads, tokens, ctx, block=64):
+    """Only the sizes count: buffers of the right size without contents."""
+    n = -(-ctx // block)
+    k = torch.empty(nseq, heads, ctx, DIM, dtype=torch.int8, device="cuda")
+    sc = torch.empty(nseq, heads, n, device="cuda")
+    c = atlas_cuda.Kv8Cache(k, torch.empty_like(k), sc, torch.empty_like(sc), nseq=nseq, kv_heads=heads, max_context=ctx,
+                            block=block)
+    return atlas_cuda.kv8_attn_form(c, q_heads, tokens)
+
+
+@pytest.mark.parametrize("sizes,few,prompt", MEASURED)
+def test_the_faster_form_is_taken(torch_cuda, sizes, few, prompt):
+    assert (form_of(torch_cuda, *sizes)[0] <= 16) == (few < prompt)
