@@ -23,7 +23,7 @@ int api_device(int device, int *sms);
 namespace k8 {
 
 // kv8_prompt.cu
-PromptCut prompt_cut(const AttnArgs &a, int sms);
+PromptCut prompt_cut(const AttnArgs &a, int dev, int sms);
 cudaError_t launch_prompt(AttnArgs a, const PromptCut &cut, int dev, int sms, cudaStream_t stream);
 
 namespace {
@@ -248,7 +248,6 @@ constexpr uint32_t kStages = 3;
 constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;   // block selection
 constexpr uint32_t kSlot = 8 * 32 * 16;                     // bytes of a chunk: 16 rows of K and V
 
-constexpr uint32_t kMaxCluster = 16;
 // The states that a CTA receives at most, C ceil(8 NT / C) over the sizes of a cluster: 16, or 30 at C = 15
 constexpr uint32_t received(int NT) { return NT == 1 ? 16u : 30u; }
 constexpr uint32_t kRecStride = kDim + 4;                   // output, maximum, sum
@@ -1234,31 +1233,6 @@ __global__ void __launch_bounds__(32 * kChosenWarps, (NT == 1 ? 16 : 8) / kChose
 
 // ------------------------------------------------------------- host side ----
 
-// How many clusters of `c` CTAs of a kernel are on the device at once; asked once per device and size.
-template <auto KERNEL>
-uint32_t clusters_at_once(int dev, uint32_t c, uint32_t threads, size_t smem)
-{
-    static std::atomic<uint32_t> known[64][kMaxCluster + 1];   // + 1; 0: not asked yet
-    uint32_t n = known[dev][c].load(std::memory_order_relaxed);
-    if (!n) {
-        cudaLaunchConfig_t cfg{};
-        cudaLaunchAttribute at;
-        at.id = cudaLaunchAttributeClusterDimension;
-        at.val.clusterDim.x = c;
-        at.val.clusterDim.y = at.val.clusterDim.z = 1;
-        cfg.gridDim = dim3(c);
-        cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.attrs = &at;
-        cfg.numAttrs = 1;
-        int most = 0;
-        if (cudaOccupancyMaxActiveClusters(&most, KERNEL, &cfg) != cudaSuccess) cudaGetLastError();
-        n = (uint32_t)std::max(most, 0) + 1;
-        known[dev][c].store(n, std::memory_order_relaxed);
-    }
-    return n - 1;
-}
-
 // CTAs per unit of work: the largest cluster of which all units are on the
 // device at once (a second wave costs more than the smaller share saves: 8
 // units of 8447 positions take 16.2 us as clusters of 16, of which 7 fit, and
@@ -1512,7 +1486,7 @@ AttnForm attn_form(FewArgs &a, int dev, int sms)
     AttnForm f{rows <= 8, false, {}};
     a.tiles = f.one ? 1 : (rows + 15) / 16;
     if (!f.one) {
-        f.cut = prompt_cut(a, sms);
+        f.cut = prompt_cut(a, dev, sms);
         f.prompt = f.cut.cycles < few_cycles(a, dev);
     }
     return f;

@@ -147,6 +147,32 @@ cudaError_t allow(int dev, int bytes)
 }
 
 constexpr size_t kMaxSmem = 232448;   // shared memory a CTA may have
+constexpr uint32_t kMaxCluster = 16;
+
+// How many clusters of `c` CTAs of a kernel are on the device at once; asked once per device and size.
+template <auto KERNEL>
+uint32_t clusters_at_once(int dev, uint32_t c, uint32_t threads, size_t smem)
+{
+    static std::atomic<uint32_t> known[64][kMaxCluster + 1];   // + 1; 0: not asked yet
+    uint32_t n = known[dev][c].load(std::memory_order_relaxed);
+    if (!n) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = c;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.gridDim = dim3(c);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        int most = 0;
+        if (cudaOccupancyMaxActiveClusters(&most, KERNEL, &cfg) != cudaSuccess) cudaGetLastError();
+        n = (uint32_t)std::max(most, 0) + 1;
+        known[dev][c].store(n, std::memory_order_relaxed);
+    }
+    return n - 1;
+}
 
 }  // namespace
 }  // namespace k8

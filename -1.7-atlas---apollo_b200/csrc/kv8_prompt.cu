@@ -834,18 +834,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 // Measured, us, tiles of rows x CTAs per unit: 333 tokens over 5001 positions of
 // 16 heads on 2, one 132, two x 1 / 2 / 3 151 / 99 / 69; 512 tokens of 28 on 4,
 // one 20.0, two 27.4 and 23.8; 256 over 2048, one x 1 / 2 43.8 / 35.0, two x 2 /
-// 3 / 4 43.8 / 37.2 / 33.4; 8 sequences of 40 on 8, 35 rows over 2000 and 16000
+// 3 / 4 / 5 43.8 / 37.2 / 33.4 / 53.9 (28 clusters of 5 do not fit at once); 8 sequences of 40 on 8, 35 rows over 2000 and 16000
 // positions, one x 2 32.7 and 196, two x 2 37.6 and 215. The positions are those
 // that the cache has room for, not those of the call, which only the device knows:
 // 512 tokens with room for 32768 take two x 2, 23.3 us.
-PromptCut prompt_cut(const AttnArgs &a, int sms)
+PromptCut prompt_cut(const AttnArgs &a, int dev, int sms)
 {
+    auto at_once = [&](uint32_t t, uint32_t c) -> uint32_t {   // units of c CTAs; clusters do not fill all SMs
+        if (c == 1) return (uint32_t)sms;
+        const cudaError_t e = t == 1 ? allow<prompt_kernel<true>>(dev, (int)kPromptSmem) : allow<prompt_kernel<false>>(dev, (int)kPromptSmem);
+        if (e != cudaSuccess) return 0u;   // the launch will say so
+        return t == 1 ? clusters_at_once<prompt_kernel<true>>(dev, c, kPromptThreads, kPromptSmem)
+                      : clusters_at_once<prompt_kernel<false>>(dev, c, kPromptThreads, kPromptSmem);
+    };
     const uint32_t rows = a.r.tokens * a.group, keys = (a.c.max_context + kTileKeys - 1) / kTileKeys;
     const uint64_t heads = (uint64_t)a.c.kv_heads * a.c.nseq;
     PromptCut best{2u, 1u, ~0ull};
     for (uint32_t t = 1; t <= 2; ++t) {
         const uint64_t units = (rows + t * kTileRows - 1) / (t * kTileRows) * heads;
         for (uint32_t c = 1; c <= kMaxSplit && units * c <= (uint64_t)sms && (c == 1 || 2 * c <= keys); ++c) {
+            if (units > at_once(t, c)) continue;   // a second wave costs more than the split saves
             const uint64_t cycles = (uint64_t)(t == 1 ? 5400 : 6900) * ((keys + c - 1) / c) + (t == 1 ? 14500 : c == 1 ? 18000 : 28000);
             if (cycles < best.cycles) best = PromptCut{t, c, cycles};
         }
