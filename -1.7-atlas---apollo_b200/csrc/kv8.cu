@@ -1398,7 +1398,7 @@ cudaError_t launch_sparse(const FewArgs &a, int dev, int sms, cudaStream_t strea
     }
     if ((e = allow<sparse_kernel<NT>>(dev, (int)kMaxSmem)) != cudaSuccess) return e;
     const size_t smem = sizeof(Smem<NT, kWarps>) + (size_t)a.n_sel * 4u;
-    const uint32_t C = cluster_of<sparse_kernel<NT>>(dev, kThreads, sizeof(Smem<NT, kWarps>), units,
+    const uint32_t C = cluster_of<sparse_kernel<NT>>(dev, kThreads, smem, units,
                                                      std::max<uint64_t>((uint64_t)a.n_sel << a.c.block_log2, a.c.max_context / 8));
     return launch(sparse_kernel<NT>, dim3(C * a.r.tokens * a.tiles, a.c.kv_heads, a.c.nseq), kThreads,
                   smem, C, a, sms, stream);

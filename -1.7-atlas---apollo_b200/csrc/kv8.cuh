@@ -149,12 +149,14 @@ cudaError_t allow(int dev, int bytes)
 constexpr size_t kMaxSmem = 232448;   // shared memory a CTA may have
 constexpr uint32_t kMaxCluster = 16;
 
-// How many clusters of `c` CTAs of a kernel are on the device at once; asked once per device and size.
+// How many clusters of `c` CTAs of a kernel are on the device at once; asked once per device and size, for shared memory
+// that leaves an SM room for two CTAs (228 KB, of which each takes 1 KB more) and that does not.
 template <auto KERNEL>
 uint32_t clusters_at_once(int dev, uint32_t c, uint32_t threads, size_t smem)
 {
-    static std::atomic<uint32_t> known[64][kMaxCluster + 1];   // + 1; 0: not asked yet
-    uint32_t n = known[dev][c].load(std::memory_order_relaxed);
+    static std::atomic<uint32_t> known[2][64][kMaxCluster + 1];   // + 1; 0: not asked yet
+    std::atomic<uint32_t> &entry = known[smem > 113 * 1024][dev][c];
+    uint32_t n = entry.load(std::memory_order_relaxed);
     if (!n) {
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute at;
@@ -169,7 +171,7 @@ uint32_t clusters_at_once(int dev, uint32_t c, uint32_t threads, size_t smem)
         int most = 0;
         if (cudaOccupancyMaxActiveClusters(&most, KERNEL, &cfg) != cudaSuccess) cudaGetLastError();
         n = (uint32_t)std::max(most, 0) + 1;
-        known[dev][c].store(n, std::memory_order_relaxed);
+        entry.store(n, std::memory_order_relaxed);
     }
     return n - 1;
 }

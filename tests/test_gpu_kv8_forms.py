@@ -151,3 +151,11 @@ def test_no_second_wave_of_clusters(torch_cuda, sizes, took):
     """The cut is one of those measured, and not a fifth slower than the best."""
     cut = form_of(torch_cuda, *sizes)
     assert took[cut] <= 1.2 * min(took.values())
+
+
+@pytest.mark.parametrize("n_sel", [768, 769, 1000])
+def test_many_chosen_blocks(torch_cuda, n_sel):
+    """More blocks than a list beside which two CTAs fit an SM holds: clusters of another size."""
+    rng = np.random.default_rng(n_sel)
+    ref = filled(rng, 2, 2, 17100, 16, [17001, 9000])
+    check_attn(torch_cuda, rng, ref, 10, 1, [17000, 8999], n_sel=n_sel)
