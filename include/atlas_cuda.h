@@ -260,7 +260,11 @@ int atlas_cuda_gemm(uint32_t type, const void *d_weights, uint64_t rows, uint64_
    were, so 0 leaves a sequence out. Token rows are [seq][tokens][heads][128]
    floats, `ld` floats from token to token (0: dense; a multiple of 4; the
    sequence stride is tokens * ld), 16-byte aligned. A position at or past
-   max_context is not stored, and reads and attends as NaN. */
+   max_context is not stored, and reads and attends as NaN.
+
+   Scales are not negative. Every wait in a kernel is bounded; one that runs out
+   (which only a fault of the device could bring about) leaves NaN in the rows
+   concerned, after the call has returned ATLAS_OK: nothing else reports it. */
 typedef struct {
     void *k, *v;                /* int8 [nseq][kv_heads][max_context][128], 16-byte aligned */
     float *k_scale, *v_scale;   /* [nseq][kv_heads][n_blocks], n_blocks = ceil(max_context / block) */
@@ -289,8 +293,12 @@ int atlas_cuda_kv8_read(const AtlasKv8 *cache, uint32_t tokens, const uint32_t *
 /* Causal grouped-query attention: the query rows of position p attend to the
    cached positions 0 .. p (the rows of p itself must have been stored), scores
    q.k / sqrt(128), softmax in fp32, fp32-level accuracy for the values that
-   the codes stand for. q_heads is a multiple of kv_heads; q and out must not
-   overlap. */
+   the codes stand for: errors are about those of a plain fp32 computation,
+   relative to what each position contributes to the row, so that blocks
+   without weight and positions that the row does not see have no part in them,
+   whatever their scales. (V scales below 2^-100 lose bits.) Which kernels run,
+   and so the last bits of a row, depends on the call's sizes. q_heads is a
+   multiple of kv_heads; q and out must not overlap. */
 int atlas_cuda_kv8_attn(const AtlasKv8 *cache, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
                         const uint32_t *d_ntok, const float *d_q, uint64_t ldq, float *d_out, uint64_t ldo,
                         void *stream);
