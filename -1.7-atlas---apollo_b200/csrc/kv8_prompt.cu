@@ -56,6 +56,7 @@
 // for two products.
 // Every wait is bounded; after a timeout the CTA's rows are NaN.
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include "../../include/atlas_cuda.h"
@@ -823,6 +824,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     if (C > 1u) merge();
 }
 
+// Lets the kernel take its shared memory; refuses a build of it whose launch has fewer registers than the warpgroups then
+// ask for, as that would wait for good.
+template <auto KERNEL>
+cudaError_t prepare(int dev)
+{
+    static std::atomic<int> registers{0};
+    int n = registers.load(std::memory_order_relaxed);
+    if (!n) {
+        cudaFuncAttributes at{};
+        const cudaError_t e = cudaFuncGetAttributes(&at, KERNEL);
+        if (e != cudaSuccess) return e;
+        registers.store(n = at.numRegs, std::memory_order_relaxed);
+    }
+    if ((uint32_t)n * 4u < 2u * kSoftmaxRegs + kConvertRegs + kMmaRegs) return cudaErrorLaunchOutOfResources;
+    return allow<KERNEL>(dev, (int)kPromptSmem);
+}
+
 }  // namespace
 
 // How a call is cut up, and an estimate of its longest CTA's time in cycles
@@ -842,7 +860,7 @@ PromptCut prompt_cut(const AttnArgs &a, int dev, int sms)
 {
     auto at_once = [&](uint32_t t, uint32_t c) -> uint32_t {   // units of c CTAs; clusters do not fill all SMs
         if (c == 1) return (uint32_t)sms;
-        const cudaError_t e = t == 1 ? allow<prompt_kernel<true>>(dev, (int)kPromptSmem) : allow<prompt_kernel<false>>(dev, (int)kPromptSmem);
+        const cudaError_t e = t == 1 ? prepare<prompt_kernel<true>>(dev) : prepare<prompt_kernel<false>>(dev);
         if (e != cudaSuccess) return 0u;   // the launch will say so
         return t == 1 ? clusters_at_once<prompt_kernel<true>>(dev, c, kPromptThreads, kPromptSmem)
                       : clusters_at_once<prompt_kernel<false>>(dev, c, kPromptThreads, kPromptSmem);
@@ -871,7 +889,7 @@ cudaError_t launch_prompt(AttnArgs a, const PromptCut &cut, int dev, int sms, cu
     const uint32_t rows = a.r.tokens * a.group, C = cut.split;
     a.tiles = (rows + cut.tiles * kTileRows - 1) / (cut.tiles * kTileRows);
     const dim3 grid(C * a.tiles, a.c.kv_heads, a.c.nseq);
-    cudaError_t e = cut.tiles == 1 ? allow<prompt_kernel<true>>(dev, (int)kPromptSmem) : allow<prompt_kernel<false>>(dev, (int)kPromptSmem);
+    const cudaError_t e = cut.tiles == 1 ? prepare<prompt_kernel<true>>(dev) : prepare<prompt_kernel<false>>(dev);
     if (e != cudaSuccess) return e;
     return cut.tiles == 1 ? launch(prompt_kernel<true>, grid, kPromptThreads, kPromptSmem, C, a, sms, stream)
                           : launch(prompt_kernel<false>, grid, kPromptThreads, kPromptSmem, C, a, sms, stream);
