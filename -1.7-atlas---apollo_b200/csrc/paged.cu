@@ -1,0 +1,697 @@
+// Paged KV cache (sm_100a): storing rows, and the calls that change which
+// sequence has which pages. The attention is in paged_attn.cu.
+//
+// The reference keeps one region of its whole context per process
+// (src/brain_runtime.c:2019-2020). Here sequences of different lengths share a
+// pool of pages, and one page may be part of several of them.
+#include <algorithm>
+#include <atomic>
+#include <cuda.h>
+#include "../../include/atlas_cuda.h"
+#include "paged.cuh"
+
+namespace atlas {
+
+int api_fail(int code, const char *fmt, ...);
+int api_device(int device, int *sms);
+
+namespace paged {
+
+using k8::launch;
+using k8::wait_predecessor;
+
+// paged_attn.cu
+cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtensorMap &vmap, bool bf, int nt, int dev, int sms,
+                       cudaStream_t stream);
+
+namespace {
+
+// --------------------------------------------------------------- append ----
+//
+// Rows of 256 bytes from [seq][token][kv_head] to their places: sixteen threads
+// a row, one thread for 16 bytes of K and of V. Nothing is computed; bound by
+// HBM for prompts (1024 bytes per token and KV head), by the launch for single
+// tokens.
+
+struct AppendArgs {
+    Cache c;
+    Rows r;
+    const uint16_t *k, *v;    // [seq][tokens][kv_heads][128], ld elements between tokens
+    uint64_t ld;
+    uint32_t layer, early;
+};
+
+constexpr uint32_t kAppendThreads = 256, kAppendRows = 4;   // rows (token, head) of a sequence that 16 threads take
+
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a)
+{
+    const uint32_t s = blockIdx.y, part = threadIdx.x & 15u;
+    wait_predecessor(a.early);
+    const uint64_t p0 = __ldcg(a.r.pos0 + s);
+    const uint64_t rows = (uint64_t)row_count(a.r, s) * a.c.kv_heads;
+    const uint64_t row0 = (uint64_t)blockIdx.x * (kAppendThreads / 16u * kAppendRows) + (threadIdx.x >> 4);
+    uint4 k[kAppendRows], v[kAppendRows];
+    uint64_t to[kAppendRows];
+#pragma unroll
+    for (uint32_t i = 0; i < kAppendRows; ++i) {
+        const uint64_t row = row0 + i * (kAppendThreads / 16u);
+        to[i] = ~0ull;
+        if (row >= rows) continue;
+        const uint32_t t = (uint32_t)(row / a.c.kv_heads), h = (uint32_t)(row - (uint64_t)t * a.c.kv_heads);
+        const uint64_t p = p0 + t;
+        if (p >= a.c.limit) continue;
+        const uint32_t e = (uint32_t)__ldcg(a.c.table + (size_t)s * a.c.max_pages + (p >> a.c.page_log2));
+        // a page that other sequences have too is not written to
+        if (e >= a.c.pages || __ldcg(a.c.refs + e) > 1) continue;
+        const size_t from = ((size_t)s * a.r.tokens + t) * a.ld + (size_t)h * kDim;
+        k[i] = __ldcs(reinterpret_cast<const uint4 *>(a.k + from) + part);
+        v[i] = __ldcs(reinterpret_cast<const uint4 *>(a.v + from) + part);
+        to[i] = (((((uint64_t)a.layer * a.c.pages + e) * a.c.kv_heads + h) << a.c.page_log2) + (p & ((1u << a.c.page_log2) - 1u))) * 16u + part;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kAppendRows; ++i)
+        if (to[i] != ~0ull) {
+            reinterpret_cast<uint4 *>(a.c.k)[to[i]] = k[i];
+            reinterpret_cast<uint4 *>(a.c.v)[to[i]] = v[i];
+        }
+}
+
+// ----------------------------------------------------------------- fork ----
+//
+// New entry (s, j) is the old entry (parent[s], j): column j of the table needs
+// nothing but itself, so a CTA reads its columns whole before it writes them,
+// and one launch suffices. The counts change by atomic additions of integers:
+// their order does not show.
+
+struct ForkArgs {
+    Cache c;
+    const int32_t *parent;
+    const uint32_t *length, *first;
+    uint32_t early;
+};
+
+constexpr uint32_t kForkColumns = 8, kForkThreads = 256;
+
+__global__ void __launch_bounds__(kForkThreads) fork_kernel(const __grid_constant__ ForkArgs a)
+{
+    extern __shared__ uint32_t was[];   // [nseq][kForkColumns]
+    wait_predecessor(a.early);
+    const uint32_t j = blockIdx.x * kForkColumns + threadIdx.x % kForkColumns, s0 = threadIdx.x / kForkColumns;
+    const bool there = j < a.c.max_pages;
+    for (uint32_t s = s0; s < a.c.nseq; s += kForkThreads / kForkColumns)
+        was[s * kForkColumns + threadIdx.x % kForkColumns] = there ? (uint32_t)__ldcg(a.c.table + (size_t)s * a.c.max_pages + j) : ~0u;
+    __syncthreads();
+    if (!there) return;
+    for (uint32_t s = s0; s < a.c.nseq; s += kForkThreads / kForkColumns) {
+        const uint32_t parent = (uint32_t)__ldcg(a.parent + s), old = was[s * kForkColumns + threadIdx.x % kForkColumns];
+        const uint64_t begin = (uint64_t)j << a.c.page_log2, end = begin + (1u << a.c.page_log2);
+        uint32_t now = ~0u;
+        if (parent < a.c.nseq && begin < __ldcg(a.length + s) && (!a.first || end > __ldcg(a.first + s)))
+            now = was[parent * kForkColumns + threadIdx.x % kForkColumns];
+        if (now >= a.c.pages) now = ~0u;
+        if (now == old) continue;
+        a.c.table[(size_t)s * a.c.max_pages + j] = (int32_t)now;
+        if (old < a.c.pages) atomicSub(a.c.refs + old, 1);
+        if (now < a.c.pages) atomicAdd(a.c.refs + now, 1);
+    }
+}
+
+// ---------------------------------------------- which pages: one CTA plans ----
+
+constexpr uint32_t kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
+
+struct PlanArgs {
+    Cache c;
+    Rows r;
+    uint32_t *out;                        // pages lacking (reserve), pages in use (compact)
+    uint32_t early;
+};
+
+__device__ __forceinline__ WorkHead *head_of(const Cache &c) { return reinterpret_cast<WorkHead *>(c.work); }
+__device__ __forceinline__ uint32_t *array_of(const Cache &c, WorkArray i)
+{
+    return c.work + sizeof(WorkHead) / 4u + (size_t)i * c.pages;
+}
+
+struct Scan {
+    uint32_t warp[2][kPlanWarps];
+};
+
+// The sum of x over the threads before this one; `all`: over all threads. `turn` alternates between two calls.
+__device__ __forceinline__ uint32_t scan_all(Scan &sm, uint32_t turn, uint32_t x, uint32_t &all)
+{
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    uint32_t inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= (uint32_t)o) inc += up;
+    }
+    if (lane == 31u) sm.warp[turn][warp] = inc;
+    __syncthreads();
+    uint32_t w = sm.warp[turn][lane];     // 32 warps
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= (uint32_t)o) w += up;
+    }
+    all = __shfl_sync(0xffffffffu, w, 31);
+    const uint32_t before = __shfl_sync(0xffffffffu, w, warp ? (int)warp - 1 : 0);
+    return inc - x + (warp ? before : 0u);
+}
+
+constexpr uint32_t kPlanPages = 16;       // pages that a thread looks at at a time
+
+// Bit i: page p0 + i is in use (i < kPlanPages); pages behind the last one are neither. 16-byte loads where `wide`.
+__device__ __forceinline__ uint32_t used_mask(const Cache &c, uint32_t p0, uint32_t &exist)
+{
+    uint32_t m = 0u;
+    exist = p0 >= c.pages ? 0u : c.pages - p0 >= kPlanPages ? (1u << kPlanPages) - 1u : (1u << (c.pages - p0)) - 1u;
+#pragma unroll
+    for (uint32_t i = 0; i < kPlanPages; i += 4u) {
+        if (p0 + i + 4u <= c.pages) {
+            const int4 x = __ldcg(reinterpret_cast<const int4 *>(c.refs + p0 + i));
+            m |= ((x.x > 0 ? 1u : 0u) | (x.y > 0 ? 2u : 0u) | (x.z > 0 ? 4u : 0u) | (x.w > 0 ? 8u : 0u)) << i;
+        } else {
+            for (uint32_t k = i; k < i + 4u; ++k)
+                if (p0 + k < c.pages && __ldcg(c.refs + p0 + k) > 0) m |= 1u << k;
+        }
+    }
+    return m;
+}
+
+// The first `want` free pages, ascending, into `list`; how many there are (up to want). All threads.
+__device__ __forceinline__ uint32_t find_free(const Cache &c, Scan &sm, uint32_t want, uint32_t *list)
+{
+    uint32_t found = 0u;
+    for (uint32_t b = 0, turn = 0; b < c.pages && found < want; b += kPlanThreads * kPlanPages, turn ^= 1u) {
+        const uint32_t p0 = b + threadIdx.x * kPlanPages;
+        uint32_t exist, all;
+        uint32_t m = used_mask(c, p0, exist);
+        m = exist & ~m;
+        uint32_t at = found + scan_all(sm, turn, __popc(m), all);
+        for (; m && at < want; m &= m - 1u) list[at++] = p0 + (uint32_t)__ffs((int)m) - 1u;
+        found += all;
+    }
+    __syncthreads();                      // the list is there, and `sm` free again
+    return min(found, want);
+}
+
+// The entries that a call's tokens are written to, in order: sequence by sequence, position by position
+struct Entries {
+    uint32_t before[kMaxSeqs + 1];        // entries of the sequences before
+    uint32_t j0[kMaxSeqs];                // the first entry's column
+};
+
+__device__ __forceinline__ void list_entries(const PlanArgs &a, Scan &sm, Entries &en)
+{
+    uint32_t done = 0u;
+    for (uint32_t b = 0, turn = 0; b < a.c.nseq; b += kPlanThreads, turn ^= 1u) {
+        const uint32_t s = b + threadIdx.x;
+        uint32_t n = 0u, all;
+        if (s < a.c.nseq) {
+            const uint32_t m = row_count(a.r, s);
+            const uint64_t p0 = __ldcg(a.r.pos0 + s), p1 = min(p0 + m, (uint64_t)a.c.limit);
+            const uint32_t j0 = (uint32_t)(p0 >> a.c.page_log2);
+            if (p0 < p1) n = (uint32_t)((p1 - 1u) >> a.c.page_log2) - j0 + 1u;
+            en.j0[s] = j0;
+        }
+        const uint32_t at = done + scan_all(sm, turn, n, all);
+        if (s < a.c.nseq) en.before[s] = at;
+        done += all;
+    }
+    if (threadIdx.x == 0) en.before[a.c.nseq] = done;
+    __syncthreads();
+}
+
+// The sequence that entry `e` is of
+__device__ __forceinline__ uint32_t sequence_of(const Entries &en, uint32_t nseq, uint32_t e)
+{
+    uint32_t lo = 0u, hi = nseq;          // before[lo] <= e < before[hi]
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (en.before[mid] <= e) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Who gets which page. An entry of the call needs a new page if it has none, or
+// one that is named elsewhere too; but of a page that only entries of this call
+// name, the last one keeps it. (One entry after the other: whoever finds its
+// page named by others leaves it, until one is left.) New pages are the lowest
+// free ones, in the entries' order; all or nothing. One CTA: the orders are
+// those of scans over entries and pages. Bound by latency: about six dependent
+// reads of L2 and three to ten scans of a few hundred cycles.
+__global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const __grid_constant__ PlanArgs a)
+{
+    __shared__ Scan sm;
+    __shared__ uint32_t copies;
+    extern __shared__ uint8_t entries_smem[];
+    Entries &en = *reinterpret_cast<Entries *>(entries_smem);
+    if (threadIdx.x == 0) copies = 0u;
+    wait_predecessor(a.early);
+    list_entries(a, sm, en);
+    const uint32_t total = en.before[a.c.nseq];
+    uint32_t *const writers = array_of(a.c, kWriters), *const last = array_of(a.c, kLastWriter);
+    // page and place of entry e
+    auto entry = [&](uint32_t e, uint32_t &s, size_t &at) {
+        s = sequence_of(en, a.c.nseq, e);
+        at = (size_t)s * a.c.max_pages + en.j0[s] + (e - en.before[s]);
+        return (uint32_t)__ldcg(a.c.table + at);
+    };
+    // how many entries of the call name each page that has several names, and which of them is last
+    bool shares = false;
+    uint32_t s;
+    size_t at;
+    for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) {
+        const uint32_t p = entry(e, s, at);
+        if (p < a.c.pages && __ldcg(a.c.refs + p) > 1) {
+            writers[p] = 0u;
+            last[p] = 0u;
+            shares = true;
+        }
+    }
+    if (__syncthreads_or(shares)) {
+        for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) {
+            const uint32_t p = entry(e, s, at);
+            if (p < a.c.pages && __ldcg(a.c.refs + p) > 1) {
+                atomicAdd(writers + p, 1u);
+                atomicMax(last + p, e);
+            }
+        }
+        __syncthreads();
+    }
+    // 0: keeps its page; 1: needs one; 2: and leaves its page as the last of the call that names it
+    auto needs = [&](uint32_t e, uint32_t p) -> uint32_t {
+        if (p >= a.c.pages) return 1u;
+        const uint32_t names = (uint32_t)max(__ldcg(a.c.refs + p), 0);
+        if (names <= 1u) return 0u;
+        if (__ldcg(last + p) != e) return 1u;
+        return __ldcg(writers + p) >= names ? 0u : 2u;
+    };
+    uint32_t mine = 0u, need;
+    for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) mine += needs(e, entry(e, s, at)) != 0u;
+    scan_all(sm, 0u, mine, need);
+    __syncthreads();
+    uint32_t *const fresh = array_of(a.c, kFresh);
+    const uint32_t found = need ? find_free(a.c, sm, need, fresh) : 0u;
+    if (threadIdx.x == 0) *a.out = need - found;
+    uint32_t *const from = array_of(a.c, kCopyFrom), *const to_page = array_of(a.c, kCopyTo), *const rows = array_of(a.c, kCopyRows);
+    if (found == need) {
+        uint32_t given = 0u;
+        for (uint32_t b = 0, turn = 0; b < total; b += kPlanThreads, turn ^= 1u) {
+            const uint32_t e = b + threadIdx.x;
+            uint32_t p = 0u, want = 0u, all, names = 0u, written = 0u;
+            if (e < total) {
+                p = entry(e, s, at);
+                want = needs(e, p);
+                if (p < a.c.pages && (names = (uint32_t)max(__ldcg(a.c.refs + p), 0)) > 1u) written = __ldcg(writers + p);
+            }
+            const uint32_t rank = given + scan_all(sm, turn, want != 0u, all);
+            given += all;
+            // the entry that is the page's last writer comes last: nobody after it looks at the page's count
+            if (e < total && names > 1u && __ldcg(last + p) == e) a.c.refs[p] = (int32_t)(written >= names ? 1u : names - written);
+            if (want) {
+                const uint32_t to = __ldcg(fresh + rank);
+                a.c.table[at] = (int32_t)to;
+                a.c.refs[to] = 1;
+                const uint32_t r = e == en.before[s] ? __ldcg(a.r.pos0 + s) & ((1u << a.c.page_log2) - 1u) : 0u;
+                if (p < a.c.pages && r) {
+                    const uint32_t i = atomicAdd(&copies, 1u);
+                    from[i] = p;
+                    to_page[i] = to;
+                    rows[i] = r;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        head_of(a.c)->copies = copies;
+        head_of(a.c)->from = ~0u;
+    }
+}
+
+// U pages are in use. The i-th used page from number U on goes to the i-th free
+// one below U, so that the first U are the used ones, and as few move as can be.
+// One CTA, two passes over the counts.
+__global__ void __launch_bounds__(kPlanThreads) compact_kernel(const __grid_constant__ PlanArgs a)
+{
+    __shared__ Scan sm;
+    wait_predecessor(a.early);
+    uint32_t mine = 0u, used, exist;
+    for (uint32_t p0 = threadIdx.x * kPlanPages; p0 < a.c.pages; p0 += kPlanThreads * kPlanPages) mine += __popc(used_mask(a.c, p0, exist));
+    scan_all(sm, 0u, mine, used);
+    uint32_t *const from = array_of(a.c, kCopyFrom), *const to = array_of(a.c, kCopyTo), *const rows = array_of(a.c, kCopyRows);
+    uint32_t *const moved = array_of(a.c, (WorkArray)kMovedTo);
+    uint32_t holes = 0u, high = 0u;
+    for (uint32_t b = 0, turn = 1; b < a.c.pages; b += kPlanThreads * kPlanPages, turn ^= 1u) {
+        const uint32_t p0 = b + threadIdx.x * kPlanPages, m = used_mask(a.c, p0, exist);
+        const uint32_t low = used <= p0 ? 0u : used - p0 >= kPlanPages ? (1u << kPlanPages) - 1u : (1u << (used - p0)) - 1u;
+        uint32_t free = exist & ~m & low, over = m & ~low, all;
+        // both counts in one scan: at most 2^14 each
+        const uint32_t before = scan_all(sm, turn, __popc(free) | (uint32_t)__popc(over) << 16, all);
+        for (uint32_t i = holes + (before & 0xffffu); free; free &= free - 1u) to[i++] = p0 + (uint32_t)__ffs((int)free) - 1u;
+        for (uint32_t i = high + (before >> 16); over; over &= over - 1u) from[i++] = p0 + (uint32_t)__ffs((int)over) - 1u;
+        holes += all & 0xffffu;
+        high += all >> 16;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < high; i += kPlanThreads) {
+        const uint32_t p = from[i], q = to[i];
+        a.c.refs[q] = a.c.refs[p];
+        a.c.refs[p] = 0;
+        moved[p] = q;
+        rows[i] = 1u << a.c.page_log2;
+    }
+    if (threadIdx.x == 0) {
+        head_of(a.c)->copies = high;
+        head_of(a.c)->from = used;
+        *a.out = used;
+    }
+}
+
+// Carries out a plan: the first rows of pages, in every layer, K and V, to other
+// pages, and the table's new numbers. No target is a source. A CTA takes 16 rows
+// of a KV head at a time (4 KB, one 16-byte access a thread), four such pieces on
+// their way at once. Bound by HBM.
+struct MoveArgs {
+    Cache c;
+    uint32_t early;
+};
+
+constexpr uint32_t kMoveThreads = 256, kMoveAtOnce = 4;
+
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveArgs a)
+{
+    wait_predecessor(a.early);
+    const uint32_t copies = __ldcg(&head_of(a.c)->copies), moved_from = __ldcg(&head_of(a.c)->from);
+    const uint32_t *from = array_of(a.c, kCopyFrom), *to = array_of(a.c, kCopyTo), *rows = array_of(a.c, kCopyRows);
+    const uint32_t subs_log2 = a.c.page_log2 - 4u;
+    const uint32_t pieces = copies * a.c.layers * 2u * a.c.kv_heads << subs_log2;
+    for (uint32_t b = blockIdx.x; b < pieces; b += gridDim.x * kMoveAtOnce) {
+        uint4 x[kMoveAtOnce];
+        uint4 *dst[kMoveAtOnce];
+#pragma unroll
+        for (uint32_t u = 0; u < kMoveAtOnce; ++u) {
+            const uint32_t piece = b + u * gridDim.x;
+            dst[u] = nullptr;
+            if (piece >= pieces) continue;
+            const uint32_t row = ((piece & ((1u << subs_log2) - 1u)) << 4) + (threadIdx.x >> 4);
+            uint32_t at = piece >> subs_log2;
+            const uint32_t h = at % a.c.kv_heads;
+            at /= a.c.kv_heads;
+            uint4 *pool = reinterpret_cast<uint4 *>(at & 1u ? a.c.v : a.c.k);
+            at >>= 1;
+            const uint32_t layer = at % a.c.layers, i = at / a.c.layers;
+            if (row >= __ldcg(rows + i)) continue;
+            auto place = [&](uint32_t page) {
+                return pool + ((((((uint64_t)layer * a.c.pages + page) * a.c.kv_heads + h) << a.c.page_log2) + row) * 16u + (threadIdx.x & 15u));
+            };
+            x[u] = __ldcs(place(__ldcg(from + i)));
+            dst[u] = place(__ldcg(to + i));
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kMoveAtOnce; ++u)
+            if (dst[u]) __stcs(dst[u], x[u]);
+    }
+    if (moved_from == ~0u) return;
+    const uint32_t *moved = array_of(a.c, (WorkArray)kMovedTo);
+    const size_t entries = (size_t)a.c.nseq * a.c.max_pages;
+    for (size_t i = (size_t)blockIdx.x * kMoveThreads + threadIdx.x; i < entries; i += (size_t)gridDim.x * kMoveThreads) {
+        const uint32_t p = (uint32_t)__ldcg(a.c.table + i);
+        if (p >= moved_from && p < a.c.pages) a.c.table[i] = (int32_t)__ldcg(moved + p);
+    }
+}
+
+// ------------------------------------------------------------- host side ----
+
+bool on_device(const void *p, int dev)
+{
+    cudaPointerAttributes at{};
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev);
+}
+
+bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+constexpr uint32_t kMaxRecordRows = 256;
+
+size_t parts_offset(uint32_t pages)
+{
+    return (sizeof(WorkHead) + (size_t)kWorkArrays * pages * 4u + 255u) & ~(size_t)255u;
+}
+
+size_t work_bytes(uint32_t pages) { return parts_offset(pages) + kPartsBytes + 2u * kMaxCtas * (size_t)record_floats(kMaxRecordRows) * 4u; }
+
+int check_shape(const char *who, const AtlasPaged *c)
+{
+    if (c->type != ATLAS_PAGED_FP16 && c->type != ATLAS_PAGED_BF16)
+        return api_fail(ATLAS_EINVAL, "%s: type %u is neither ATLAS_PAGED_FP16 nor ATLAS_PAGED_BF16", who, c->type);
+    if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
+        return api_fail(ATLAS_EINVAL, "%s: pages of 16, 32, 64 or 128 positions, not %u", who, c->page);
+    if (!c->layers || !c->pages || !c->kv_heads || c->kv_heads > 16384u || c->pages > 0x0fffffffu ||
+        (uint64_t)c->pages * c->kv_heads * c->page > 0x7fffffffull / c->layers)
+        return api_fail(ATLAS_EINVAL, "%s: bad pool (%u layers, %u pages of %u positions, %u KV heads): at most 2^31 - 1 rows", who,
+                        c->layers, c->pages, c->page, c->kv_heads);
+    if (!c->nseq || c->nseq > kMaxSeqs || !c->max_pages || (uint64_t)c->max_pages * c->page > 0x7fffff00ull ||
+        (uint64_t)c->nseq * c->max_pages > 0x7fffffffull)
+        return api_fail(ATLAS_EINVAL, "%s: bad table (%u sequences of %u pages)", who, c->nseq, c->max_pages);
+    return ATLAS_OK;
+}
+
+// The checks that all calls share; fills the kernels' view of the cache.
+int open_cache(const char *who, const AtlasPaged *c, Cache &out, int &dev, int &sms)
+{
+    if (!c || !c->k || !c->v || !c->table || !c->refs || !c->work) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
+    const int rc = check_shape(who, c);
+    if (rc != ATLAS_OK) return rc;
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->refs, 16) || !aligned(c->table, 4) || !aligned(c->work, 256))
+        return api_fail(ATLAS_EINVAL, "%s: the pool and refs must be 16-byte aligned, the table 4-byte, the workspace 256-byte", who);
+    if (c->work_bytes < work_bytes(c->pages))
+        return api_fail(ATLAS_EINVAL, "%s: a workspace of %llu bytes, not %llu", who, (unsigned long long)work_bytes(c->pages),
+                        (unsigned long long)c->work_bytes);
+    dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || api_device(dev, &sms) != ATLAS_OK)
+        return api_fail(ATLAS_ENODEV, "%s: no sm_100 device", who);
+    const void *need[] = {c->k, c->v, c->table, c->refs, c->work};
+    for (const void *p : need)
+        if (!on_device(p, dev)) return api_fail(ATLAS_EINVAL, "%s: the cache must be memory of the current device", who);
+    out.k = static_cast<uint16_t *>(c->k);
+    out.v = static_cast<uint16_t *>(c->v);
+    out.table = c->table;
+    out.refs = c->refs;
+    out.work = static_cast<uint32_t *>(c->work);
+    out.layers = c->layers;
+    out.pages = c->pages;
+    out.kv_heads = c->kv_heads;
+    out.page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+    out.nseq = c->nseq;
+    out.max_pages = c->max_pages;
+    out.limit = c->max_pages << out.page_log2;
+    return ATLAS_OK;
+}
+
+// Device integers of a call; null where `optional`
+int check_ints(const char *who, const char *name, const void *p, int dev, bool optional = false)
+{
+    if (!p && optional) return ATLAS_OK;
+    if (!p) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
+    if (!aligned(p, 4) || !on_device(p, dev))
+        return api_fail(ATLAS_EINVAL, "%s: %s must be 4-byte aligned memory of the current device", who, name);
+    return ATLAS_OK;
+}
+
+int check_tokens(const char *who, uint32_t tokens, const uint32_t *pos0, const uint32_t *n_tok, Rows &rows, int dev)
+{
+    if (tokens > 0x00ffffffu) return api_fail(ATLAS_EINVAL, "%s: at most 2^24 - 1 tokens, not %u", who, tokens);
+    int rc = check_ints(who, "pos0", pos0, dev);
+    if (rc == ATLAS_OK) rc = check_ints(who, "n_tok", n_tok, dev, true);
+    rows = Rows{pos0, n_tok, tokens};
+    return rc;
+}
+
+// Token rows of `heads` x 128 values, ld values apart (0: dense).
+int check_rows(const char *who, const void *p, uint32_t heads, uint64_t &ld, int dev)
+{
+    if (!p) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
+    if (!ld) ld = (uint64_t)heads * kDim;
+    if (ld < (uint64_t)heads * kDim || ld % 8 || ld > 0xffffffffull)
+        return api_fail(ATLAS_EINVAL, "%s: token rows %llu values apart: at least heads x 128, a multiple of 8", who, (unsigned long long)ld);
+    if (!aligned(p, 16)) return api_fail(ATLAS_EINVAL, "%s: token rows must be 16-byte aligned", who);
+    if (!on_device(p, dev)) return api_fail(ATLAS_EINVAL, "%s: token rows must be memory of the current device", who);
+    return ATLAS_OK;
+}
+
+using Encode = decltype(&cuTensorMapEncodeTiled);
+
+int find_encode(const char *who, Encode &encode)
+{
+    static std::atomic<Encode> known{nullptr};
+    encode = known.load(std::memory_order_acquire);
+    if (!encode) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess || !p) {
+            cudaGetLastError();
+            return api_fail(ATLAS_ECUDA, "%s: the driver has no cuTensorMapEncodeTiled", who);
+        }
+        encode = reinterpret_cast<Encode>(p);
+        known.store(encode, std::memory_order_release);
+    }
+    return ATLAS_OK;
+}
+
+// A pool as [2 halves of 64 dimensions][rows][64], for copies of `box` rows of both halves
+int map_pool(const char *who, Encode encode, const Cache &c, bool bf, void *pool, uint32_t box, uint32_t halves, CUtensorMap &map)
+{
+    const cuuint64_t rows = ((cuuint64_t)c.layers * c.pages * c.kv_heads) << c.page_log2;
+    const cuuint64_t dims[3] = {kDim / 2, rows, 2}, strides[2] = {kRowBytes, kRowBytes / 2};
+    const cuuint32_t boxes[3] = {kDim / 2, box, halves}, steps[3] = {1, 1, 1};
+    if (encode(&map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, pool, dims, strides, boxes, steps,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return api_fail(ATLAS_ECUDA, "%s: the pool cannot be described to the copy engine", who);
+    return ATLAS_OK;
+}
+
+int done(const char *who, cudaError_t e)
+{
+    if (e == cudaSuccess) return ATLAS_OK;
+    cudaGetLastError();
+    return api_fail(ATLAS_ECUDA, "%s: %s", who, cudaGetErrorString(e));
+}
+
+// Carries out the plan of the launch before, which copies at most `copies` pages
+cudaError_t launch_move(const Cache &c, uint64_t copies, uint64_t entries, int sms, cudaStream_t stream)
+{
+    MoveArgs a{};
+    a.c = c;
+    const uint64_t pieces = copies * c.layers * 2 * c.kv_heads << (c.page_log2 - 4u);
+    const uint64_t ctas = std::max((pieces + kMoveAtOnce - 1) / kMoveAtOnce, (entries + kMoveThreads - 1) / kMoveThreads);
+    return launch(move_kernel, dim3((uint32_t)std::min<uint64_t>(ctas, (uint64_t)sms * 8)), kMoveThreads, 0, 1, a, sms, stream);
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace atlas
+
+using namespace atlas;
+using namespace atlas::paged;
+
+extern "C" int atlas_cuda_paged_work(const AtlasPaged *cache, uint64_t *bytes)
+{
+    const char *who = "paged_work";
+    if (!cache || !bytes) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
+    const int rc = check_shape(who, cache);
+    if (rc == ATLAS_OK) *bytes = work_bytes(cache->pages);
+    return rc;
+}
+
+extern "C" int atlas_cuda_paged_append(const AtlasPaged *cache, uint32_t layer, uint32_t tokens, const uint32_t *d_pos0,
+                                       const uint32_t *d_ntok, const void *d_k, const void *d_v, uint64_t ld, void *stream)
+{
+    const char *who = "paged_append";
+    AppendArgs a{};
+    int dev, sms, rc = open_cache(who, cache, a.c, dev, sms);
+    if (rc == ATLAS_OK) rc = check_tokens(who, tokens, d_pos0, d_ntok, a.r, dev);
+    if (rc == ATLAS_OK && layer >= cache->layers) rc = api_fail(ATLAS_EINVAL, "%s: layer %u of %u", who, layer, cache->layers);
+    if (rc != ATLAS_OK || !tokens) return rc;   // no rows need no memory
+    if ((rc = check_rows(who, d_k, cache->kv_heads, ld, dev)) != ATLAS_OK) return rc;
+    if ((rc = check_rows(who, d_v, cache->kv_heads, ld, dev)) != ATLAS_OK) return rc;
+    a.k = static_cast<const uint16_t *>(d_k);
+    a.v = static_cast<const uint16_t *>(d_v);
+    a.ld = ld;
+    a.layer = layer;
+    constexpr uint64_t per = kAppendThreads / 16u * kAppendRows;
+    const uint64_t ctas = ((uint64_t)tokens * cache->kv_heads + per - 1) / per;
+    if (ctas > 0x7fffffffull) return api_fail(ATLAS_EINVAL, "%s: too many rows", who);
+    return done(who, launch(append_kernel, dim3((uint32_t)ctas, cache->nseq), kAppendThreads, 0, 1, a, sms, (cudaStream_t)stream));
+}
+
+extern "C" int atlas_cuda_paged_fork(const AtlasPaged *cache, const int32_t *d_parent, const uint32_t *d_length, const uint32_t *d_first,
+                                     void *stream)
+{
+    const char *who = "paged_fork";
+    ForkArgs a{};
+    int dev, sms, rc = open_cache(who, cache, a.c, dev, sms);
+    if (rc == ATLAS_OK) rc = check_ints(who, "parent", d_parent, dev);
+    if (rc == ATLAS_OK) rc = check_ints(who, "length", d_length, dev);
+    if (rc == ATLAS_OK) rc = check_ints(who, "first", d_first, dev, true);
+    if (rc != ATLAS_OK) return rc;
+    a.parent = d_parent;
+    a.length = d_length;
+    a.first = d_first;
+    const cudaError_t e = k8::allow<fork_kernel>(dev, (int)(kMaxSeqs * kForkColumns * 4u));
+    if (e != cudaSuccess) return done(who, e);
+    return done(who, launch(fork_kernel, dim3((cache->max_pages + kForkColumns - 1) / kForkColumns), kForkThreads,
+                            (size_t)cache->nseq * kForkColumns * 4u, 1, a, sms, (cudaStream_t)stream));
+}
+
+extern "C" int atlas_cuda_paged_reserve(const AtlasPaged *cache, uint32_t tokens, const uint32_t *d_pos0, const uint32_t *d_ntok,
+                                        uint32_t *d_short, void *stream)
+{
+    const char *who = "paged_reserve";
+    PlanArgs a{};
+    int dev, sms, rc = open_cache(who, cache, a.c, dev, sms);
+    if (rc == ATLAS_OK) rc = check_tokens(who, tokens, d_pos0, d_ntok, a.r, dev);
+    if (rc == ATLAS_OK) rc = check_ints(who, "short", d_short, dev);
+    if (rc != ATLAS_OK) return rc;
+    a.out = d_short;
+    const cudaError_t e = launch(reserve_kernel, dim3(1), kPlanThreads, sizeof(Entries), 1, a, sms, (cudaStream_t)stream);
+    if (e != cudaSuccess) return done(who, e);
+    // a sequence's first page at most is copied
+    return done(who, launch_move(a.c, std::min(cache->nseq, cache->pages), 0, sms, (cudaStream_t)stream));
+}
+
+extern "C" int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_used, void *stream)
+{
+    const char *who = "paged_compact";
+    PlanArgs a{};
+    int dev, sms, rc = open_cache(who, cache, a.c, dev, sms);
+    if (rc == ATLAS_OK) rc = check_ints(who, "used", d_used, dev);
+    if (rc != ATLAS_OK) return rc;
+    a.out = d_used;
+    const cudaError_t e = launch(compact_kernel, dim3(1), kPlanThreads, 0, 1, a, sms, (cudaStream_t)stream);
+    if (e != cudaSuccess) return done(who, e);
+    return done(who, launch_move(a.c, cache->pages / 2u, (uint64_t)cache->nseq * cache->max_pages, sms, (cudaStream_t)stream));
+}
+
+extern "C" int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
+                                     const uint32_t *d_ntok, const void *d_q, uint64_t ldq, void *d_out, uint64_t ldo, void *stream)
+{
+    const char *who = "paged_attn";
+    AttnArgs a{};
+    // a row of `out` may be written before another CTA has read its neighbours in `q`
+    if (d_q && d_q == d_out && tokens) return api_fail(ATLAS_EINVAL, "%s: out must not be q", who);
+    int dev, sms, rc = open_cache(who, cache, a.c, dev, sms);
+    if (rc == ATLAS_OK) rc = check_tokens(who, tokens, d_pos0, d_ntok, a.r, dev);
+    if (rc != ATLAS_OK) return rc;
+    if (!q_heads || q_heads % cache->kv_heads || q_heads > 32768u || (uint64_t)q_heads * tokens > 0x3fffffffull)
+        return api_fail(ATLAS_EINVAL, "%s: %u query heads over %u KV heads, %u tokens", who, q_heads, cache->kv_heads, tokens);
+    if (layer >= cache->layers) return api_fail(ATLAS_EINVAL, "%s: layer %u of %u", who, layer, cache->layers);
+    if (!tokens) return ATLAS_OK;               // no rows need no memory
+    if ((rc = check_rows(who, d_q, q_heads, ldq, dev)) != ATLAS_OK) return rc;
+    if ((rc = check_rows(who, d_out, q_heads, ldo, dev)) != ATLAS_OK) return rc;
+    a.q = static_cast<const uint16_t *>(d_q);
+    a.out = static_cast<uint16_t *>(d_out);
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.q_heads = q_heads;
+    a.group = q_heads / cache->kv_heads;
+    a.layer = layer;
+    a.parts = reinterpret_cast<float *>(static_cast<char *>(cache->work) + parts_offset(cache->pages));
+    const bool bf = cache->type == ATLAS_PAGED_BF16;
+    const uint32_t rows = tokens * a.group;
+    Encode encode;
+    if ((rc = find_encode(who, encode)) != ATLAS_OK) return rc;
+    CUtensorMap kmap, vmap;
+    if ((rc = map_pool(who, encode, a.c, bf, cache->k, 16, 2, kmap)) != ATLAS_OK) return rc;
+    if ((rc = map_pool(who, encode, a.c, bf, cache->v, 16, 2, vmap)) != ATLAS_OK) return rc;
+    return done(who, launch_few(a, kmap, vmap, bf, rows <= 8 ? 1 : rows <= 16 ? 2 : 4, dev, sms, (cudaStream_t)stream));
+}

@@ -1,0 +1,290 @@
+// What the attention kernels over pages share: how a call's work is dealt out
+// over the CTAs, the partial sums' places, 16-bit types.
+//
+// A unit is a tile of a sequence's query rows and a KV head; its work is the
+// tiles of keys (of KEYS positions) that its last row sees. All units' tiles of
+// keys, in the order sequence, head, rows, make one line, of which each CTA
+// takes an equal piece: whole units inside it are finished by the CTA; of those
+// that its ends cut, it leaves partial sums (Part), which part_merge_kernel
+// joins. So every SM has the same to read and compute whatever the lengths,
+// which only the device knows, and the pieces do not depend on timing.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include "kv8.cuh"
+#include "paged.h"
+
+namespace atlas {
+namespace paged {
+
+// Of each CTA: two records of partial sums, that of the unit that its piece
+// begins in, and that of the one it ends in. A record: [rows][128] sums, then
+// [rows] (maximum, sum of weights), for `rows` = the form's rows per unit.
+// In front of all, a Part per CTA.
+struct Part {
+    uint32_t first;       // the record that the unit begins in; ~0: no unit that others began ends in this CTA's piece
+    uint32_t count;       // records of the unit: `first`, then 2 x its CTA's following numbers
+    uint32_t s, h, row0, rows;
+    uint32_t pad[2];
+};
+
+constexpr size_t kPartsBytes = kMaxCtas * sizeof(Part);
+constexpr uint32_t record_floats(uint32_t rows) { return rows * (kDim + 2u); }
+
+namespace {
+
+using k8::ex2;
+using k8::TileRows;
+
+// Two floats as a pair of 16-bit values, `lo` in the lower half
+template <bool BF>
+__device__ __forceinline__ uint32_t pack(float lo, float hi)
+{
+    uint32_t d;
+    if (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+// One 16-bit value as a float
+template <bool BF>
+__device__ __forceinline__ float unpack1(uint32_t x)
+{
+    return BF ? __uint_as_float(x << 16) : __half2float(__ushort_as_half((unsigned short)x));
+}
+
+// Bits of the halves of x that are infinite or NaN: 0xffff each
+template <bool BF>
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x)
+{
+    constexpr uint32_t e = BF ? 0x7f80u : 0x7c00u;
+    return ((x & e) == e ? 0xffffu : 0u) | ((x >> 16 & e) == e ? 0xffff0000u : 0u);
+}
+
+// A sequence as its units see it: tiles of keys [k0, ..), k0 behind the pages that are gone at its start
+struct Seq {
+    uint64_t p0;
+    uint32_t rows, k0;
+};
+
+// The sequence's first tile of keys that has a page, or behind: its leading entries that name none are passed over, 128 at
+// a time. The whole warp.
+__device__ __forceinline__ uint32_t first_page(const Cache &c, uint32_t s, uint32_t pages)
+{
+    const int32_t *row = c.table + (size_t)s * c.max_pages;
+    const uint32_t lane = threadIdx.x & 31u;
+    if (!pages || (uint32_t)__ldcg(row) < c.pages) return 0u;
+    for (uint32_t b = 0; b < pages; b += 128u) {
+        uint32_t x[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) x[i] = b + 32u * i + lane < pages ? (uint32_t)__ldcg(row + b + 32u * i + lane) : ~0u;
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t have = __ballot_sync(0xffffffffu, x[i] < c.pages);
+            if (have) return b + 32u * i + (uint32_t)__ffs((int)have) - 1u;
+        }
+    }
+    return pages;
+}
+
+// How a call's rows are cut into tiles: `tile` rows each, those of whole tokens where `tokens` is not 0
+template <uint32_t KEYS>
+struct Cut {
+    const AttnArgs &a;
+    uint32_t tile;        // query rows of a unit
+
+    // the tiles of keys that rows before `row1` see, from the front
+    __device__ __forceinline__ uint32_t keys(const Seq &q, uint32_t row1) const
+    {
+        const uint64_t last = min(q.p0 + (row1 - 1u) / a.group + 1u, (uint64_t)a.c.limit);
+        return (uint32_t)((last + KEYS - 1u) / KEYS);
+    }
+    __device__ __forceinline__ uint32_t units(const Seq &q) const { return (q.rows + tile - 1u) / tile; }
+    // work of a unit: at least one tile of keys, so that its rows are written
+    __device__ __forceinline__ uint32_t cost(const Seq &q, uint32_t i) const
+    {
+        const uint32_t k = keys(q, min((i + 1u) * tile, q.rows));
+        return k > q.k0 ? k - q.k0 : 1u;
+    }
+    // the whole warp
+    __device__ __forceinline__ Seq open(uint32_t s) const
+    {
+        Seq q;
+        q.p0 = __ldcg(a.r.pos0 + s);
+        q.rows = row_count(a.r, s) * a.group;
+        q.k0 = 0u;
+        if (q.rows) {
+            const uint32_t seen = (uint32_t)min(q.p0 + (q.rows - 1u) / a.group + 1u, (uint64_t)a.c.limit);
+            q.k0 = (uint32_t)(((uint64_t)first_page(a.c, s, (seen + (1u << a.c.page_log2) - 1u) >> a.c.page_log2) << a.c.page_log2) / KEYS);
+        }
+        return q;
+    }
+};
+
+// The piece of a CTA: it begins in unit (s, h, i), `skip` tiles of keys behind the unit's first one, and has `left` of them
+struct Piece {
+    uint64_t begin, each; // in the line of all; a CTA's share
+    uint32_t s, h, i, skip;
+    uint64_t left;
+};
+
+struct PieceSmem {
+    uint64_t before[kMaxSeqs + 1];        // the line's length before each sequence
+};
+
+// This CTA's piece. All WARPS warps; `sm` may be used for something else after the next barrier. `least`: tiles of keys
+// that a CTA takes at least.
+template <uint32_t KEYS, uint32_t WARPS>
+__device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, uint32_t least)
+{
+    const AttnArgs &a = cut.a;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = a.c.nseq;
+    for (uint32_t s = warp; s < n; s += WARPS) {
+        const Seq q = cut.open(s);
+        uint64_t sum = 0u;
+        const uint32_t units = q.rows ? cut.units(q) : 0u;
+        for (uint32_t i = lane; i < units; i += 32u) sum += cut.cost(q, i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0u) sm.before[s + 1u] = sum * a.c.kv_heads;
+    }
+    if (threadIdx.x == 0u) sm.before[0] = 0u;
+    __syncthreads();
+    if (warp == 0u) {
+        uint64_t done = 0u;
+        for (uint32_t b = 1u; b <= n; b += 32u) {
+            uint64_t x = b + lane <= n ? sm.before[b + lane] : 0u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t up = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= (uint32_t)o) x += up;
+            }
+            if (b + lane <= n) sm.before[b + lane] = done + x;
+            done += __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
+    __syncthreads();
+    Piece p;
+    const uint64_t total = sm.before[n];
+    p.each = max((total + gridDim.x - 1u) / gridDim.x, (uint64_t)least);
+    p.begin = p.each * blockIdx.x;
+    p.left = p.begin < total ? min(p.each, total - p.begin) : 0u;
+    p.s = p.h = p.i = p.skip = 0u;
+    if (!p.left) return p;
+    uint32_t lo = 0u, hi = n;             // before[lo] <= begin < before[hi]
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (sm.before[mid] <= p.begin) lo = mid;
+        else hi = mid;
+    }
+    p.s = lo;
+    const Seq q = cut.open(lo);
+    const uint64_t of_head = (sm.before[lo + 1u] - sm.before[lo]) / a.c.kv_heads, in = p.begin - sm.before[lo];
+    p.h = (uint32_t)(in / of_head);
+    uint64_t rest = in - of_head * p.h;
+    const uint32_t units = cut.units(q);
+    for (uint32_t b = 0;; b += 32u) {     // the unit that holds place `rest`
+        const uint32_t mine = b + lane < units ? cut.cost(q, b + lane) : 0u;
+        uint64_t x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t up = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= (uint32_t)o) x += up;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, x > rest);
+        if (past || b + 32u >= units) {
+            const uint32_t at = past ? (uint32_t)__ffs((int)past) - 1u : 31u;
+            p.i = min(b + at, units - 1u);
+            p.skip = (uint32_t)(rest - __shfl_sync(0xffffffffu, x - mine, (int)at));
+            return p;
+        }
+        rest -= __shfl_sync(0xffffffffu, x, 31);
+    }
+}
+
+// Walks over the units of a piece. The whole warp.
+template <uint32_t KEYS>
+struct Walk {
+    const Cut<KEYS> &cut;
+    Piece p;
+    Seq q;
+    uint32_t k_begin, k_end;              // this piece's tiles of keys of the current unit
+    bool head, tail;                      // the unit's first tile is in the piece, and its last
+    bool first;                           // it is the piece's first unit
+
+    __device__ __forceinline__ Walk(const Cut<KEYS> &cut_, const Piece &p_) : cut(cut_), p(p_), first(true)
+    {
+        if (p.left) {
+            q = cut.open(p.s);
+            set();
+        }
+    }
+    __device__ __forceinline__ bool more() const { return p.left != 0u; }
+    __device__ __forceinline__ uint32_t row0() const { return p.i * cut.tile; }
+    __device__ __forceinline__ uint32_t rows() const { return min(q.rows - row0(), cut.tile); }
+    __device__ __forceinline__ void set()
+    {
+        const uint32_t all = cut.cost(q, p.i);
+        head = p.skip == 0u;
+        k_begin = q.k0 + p.skip;
+        const uint32_t n = (uint32_t)min((uint64_t)(all - p.skip), p.left);
+        k_end = k_begin + n;
+        tail = p.skip + n == all;
+    }
+    __device__ __forceinline__ void next()
+    {
+        p.left -= k_end - k_begin;
+        p.skip = 0u;
+        first = false;
+        if (!p.left) return;
+        if (++p.i >= cut.units(q)) {
+            p.i = 0u;
+            if (++p.h >= cut.a.c.kv_heads) {
+                p.h = 0u;
+                do q = cut.open(++p.s);
+                while (!q.rows);          // there is more, so a sequence with rows comes
+            }
+        }
+        set();
+    }
+    // where this piece's part of a cut unit goes
+    __device__ __forceinline__ uint32_t record() const { return 2u * blockIdx.x + (first ? 0u : 1u); }
+    // what the merge has to know: of the piece's first unit, if others began it and it ends here
+    __device__ __forceinline__ Part part() const
+    {
+        Part r{};
+        r.first = ~0u;
+        if (p.left && !head && tail) {
+            const uint64_t unit = p.begin - p.skip;
+            const uint32_t c = (uint32_t)(unit / p.each);
+            r.first = 2u * c + (unit == p.each * c ? 0u : 1u);
+            r.count = blockIdx.x - c + 1u;
+            r.s = p.s;
+            r.h = p.h;
+            r.row0 = row0();
+            r.rows = rows();
+        }
+        return r;
+    }
+};
+
+__device__ __forceinline__ float *record_of(const AttnArgs &a, uint32_t i, uint32_t rows)
+{
+    return a.parts + kPartsBytes / 4u + (size_t)i * record_floats(rows);
+}
+
+// Four dimensions of an output row
+template <bool BF>
+__device__ __forceinline__ void store4(const AttnArgs &a, uint32_t s, uint32_t h, uint2 at, uint32_t d4, float4 x)
+{
+    reinterpret_cast<uint2 *>(a.out + ((size_t)s * a.r.tokens + at.x) * a.ldo + (size_t)(h * a.group + at.y) * kDim)[d4] =
+        make_uint2(pack<BF>(x.x, x.y), pack<BF>(x.z, x.w));
+}
+
+}  // namespace
+
+// paged_attn.cu: joins the partial sums of units of `rows` rows
+cudaError_t launch_merge(const AttnArgs &a, bool bf, uint32_t rows, uint32_t ctas, int sms, cudaStream_t stream);
+
+}  // namespace paged
+}  // namespace atlas

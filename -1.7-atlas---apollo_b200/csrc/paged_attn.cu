@@ -1,0 +1,495 @@
+// Attention over a paged KV cache for few query rows per KV head (sm_100a), and
+// the kernel that joins partial sums. The form for many rows is in
+// paged_prompt.cu. (gqa_single_token in the reference, src/brain_runtime.c:1407-1528,
+// over one region of fp32 rows.)
+//
+// A unit is 8 NT query rows (token, head of the group; token-major) of a KV
+// head. A CTA takes a piece of the line of all units' keys (paged.cuh), 16
+// positions at a time dealt out over its eight warps, each with a softmax state
+// of its own (running maximum, sum, output), joined in shared memory at a unit's
+// end. 16 positions lie in one page: two TMA copies (16 rows of K, 16 of V,
+// swizzled) bring them into a ring of the warp's own, and positions without a
+// page are passed over.
+//
+//   S^T = K Q^T     m16n8k16 (rows are positions, columns query rows)
+//   O^T += V^T P^T  m16n8k16 (rows are dimensions); P in two 16-bit terms
+//                   hi + lo, so that it costs the output nothing; the MMAs truncate
+//                   their sums, so each 16 positions' is added to the output in fp32
+//
+// The maximum is lazy: a row's is raised only when a score passes it by 2^6, so
+// 16 positions need no reduction over lanes.
+// Bound by HBM for long caches, by latency for short ones.
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include "../../include/atlas_cuda.h"
+#include "paged.cuh"
+
+namespace atlas {
+namespace paged {
+
+using k8::kScoreScale;
+using k8::pair;
+using k8::unpair;
+using k8::add2;
+using k8::mul2;
+using k8::wait_predecessor;
+
+namespace {
+
+constexpr uint32_t kChunk = 16, kWarps = 8, kThreads = kWarps * 32, kStages = 3;
+constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
+constexpr uint32_t kRecStride = kDim + 4;
+constexpr float kLazy = 6.0f;
+// Weights are 2^(score - maximum + kUnit). binary16: their largest, 2^15, keeps the low term's bits; bfloat16 has fp32's
+// range, and small weights leave the sums of large values room
+template <bool BF>
+constexpr float kUnit = BF ? -24.0f : 9.0f;
+
+struct FewArgs : AttnArgs {
+    CUtensorMap kmap, vmap;      // [2][rows of the pool][64] each
+};
+
+template <int NT>
+struct alignas(1024) Smem {
+    union {
+        uint8_t ring[kWarps][kStages][kSlot];
+        float wrec[kWarps][8 * NT][kRecStride];    // the warps' outputs, once the ring is done with
+        PieceSmem piece;
+    } u;
+    uint64_t full[kWarps][kStages];
+    uint32_t err;
+    float2 wml[kWarps][8 * NT];
+};
+
+template <bool BF>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ void load_matrices(uint32_t (&d)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void load_matrices_t(uint32_t (&d)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// 16 rows of the pool from row `row` on, as two halves of 64 dimensions, each [16][128 bytes], 16-byte chunk c of row r
+// at chunk c ^ (r % 8)
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, uint32_t row, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"((int)row), "r"(0), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// What this thread did to the ring's place comes before the copies that follow
+__device__ __forceinline__ void fence_ring() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+constexpr uint32_t kNone = ~0u;
+
+template <bool BF, int NT>
+__global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant__ FewArgs a)
+{
+    constexpr uint32_t R = 8 * NT;
+    extern __shared__ __align__(1024) uint8_t few_smem[];
+    Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(few_smem);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    if (lane == 0u) {
+        for (uint32_t i = 0; i < kStages; ++i) mbar_init(&sm.full[warp][i], 1u);
+        fence_mbar_init();
+    }
+    if (threadIdx.x == 0u) {
+        sm.err = kStatusOk;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a.kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a.vmap) : "memory");
+    }
+    __syncthreads();
+    wait_predecessor(a.early);
+    const Cut<kChunk> cut{a, R};
+    const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, kWarps);
+    Walk<kChunk> w(cut, piece);
+    if (threadIdx.x == 0u) reinterpret_cast<Part *>(a.parts)[blockIdx.x] = w.part();
+    if (!w.more()) return;
+    fence_ring();
+    __syncthreads();                      // the ring's place is free
+    const uint32_t ring = smem_addr(sm.u.ring[warp][0]);
+    uint64_t *const full = sm.full[warp];
+    const float inv_group = 1.000001f / (float)a.group;
+    uint32_t slot = 0u, phase = 0u, slot_in = 0u;
+    bool ok = true;
+
+    for (; w.more(); w.next()) {
+        const uint32_t rows = w.rows(), row0 = w.row0(), s = w.p.s, h = w.p.h;
+        TileRows tr{row0 / a.group, 0u, a.group, inv_group};
+        tr.rem = row0 - tr.tok * a.group;
+        const uint64_t p0 = w.q.p0;
+        const uint32_t seen = cut.keys(w.q, row0 + rows);          // chunks that some row sees
+        const uint32_t k_end = min(w.k_end, seen), first = w.k_begin + warp;
+        const int32_t *const entries = a.c.table + (size_t)s * a.c.max_pages;
+        const uint32_t page_chunks = a.c.page_log2 - 4u;           // log2 of chunks per page
+        // the entries of this warp's chunks first + 8 (base + lane), and the next 32
+        auto entry_of = [&](uint32_t base) {
+            const uint32_t c = first + kWarps * (base + lane);
+            return c < k_end ? (uint32_t)__ldcg(entries + (c >> page_chunks)) : ~0u;
+        };
+        uint32_t base = 0u, ent = entry_of(0u), ent_next = entry_of(32u), have = __ballot_sync(0xffffffffu, ent < a.c.pages);
+        // the next chunk of this warp's that has a page; its copies are issued into the next slot
+        auto issue = [&]() -> uint32_t {
+            while (!have) {
+                base += 32u;
+                if (first + kWarps * base >= k_end) return kNone;
+                ent = ent_next;
+                ent_next = entry_of(base + 32u);
+                have = __ballot_sync(0xffffffffu, ent < a.c.pages);
+            }
+            const uint32_t b = (uint32_t)__ffs((int)have) - 1u;
+            have &= have - 1u;
+            const uint32_t e = __shfl_sync(0xffffffffu, ent, (int)b), c = first + kWarps * (base + b);
+            if (lane == 0u) {
+                const uint32_t row = (((a.layer * a.c.pages + e) * a.c.kv_heads + h) << a.c.page_log2) + ((c & ((1u << page_chunks) - 1u)) << 4);
+                const uint32_t dst = ring + slot_in * kSlot;
+                mbar_arrive_expect_tx(full + slot_in, kSlot);
+                load_rows(dst, &a.kmap, row, full + slot_in);
+                load_rows(dst + kSlot / 2u, &a.vmap, row, full + slot_in);
+            }
+            if (++slot_in == kStages) slot_in = 0u;
+            return c;
+        };
+        uint32_t chunk[kStages];          // on their way; kNone: nothing more
+#pragma unroll
+        for (uint32_t i = 0; i < kStages - 1u; ++i) chunk[i] = issue();
+        chunk[kStages - 1u] = kNone;
+
+        // B operands: column g, dimensions 16 st + 2 t, + 1, + 8, + 9
+        uint32_t qf[NT][8][2];
+        uint32_t last[NT][2];             // the last position that columns 2 t and 2 t + 1 see
+        const uint32_t open = (uint32_t)min(p0 + tr.tok, (uint64_t)0x7fffffffu);   // every row sees the positions up to it
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t i = 8u * (uint32_t)nt + g;
+            const uint2 at = tr.at(min(i, rows - 1u));
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(a.q + ((size_t)s * a.r.tokens + at.x) * a.ldq + (size_t)(h * a.group + at.y) * kDim);
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                qf[nt][st][0] = __ldcg(src + 8 * st + t);
+                qf[nt][st][1] = __ldcg(src + 8 * st + 4 + t);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t r = 8u * (uint32_t)nt + 2u * t + (uint32_t)e;
+                last[nt][e] = r < rows ? (uint32_t)min(p0 + tr.at(r).x, (uint64_t)0x7fffffffu) : open;
+            }
+        }
+
+        uint64_t o[NT][8][2];             // dimensions 16 j + g and 16 j + g + 8: columns 2 t and 2 t + 1
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = 0ull;
+        }
+        const uint32_t koff = (lane & 15u) * 128u, kx = (lane >> 4) ^ (lane & 7u);
+        const uint32_t vkey = (lane & 7u) + 8u * (lane >> 4), voff = 2u * kHalfChunk + vkey * 128u, vx = ((lane >> 3) & 1u) ^ (lane & 7u);
+        while (ok && chunk[0] != kNone) {
+            __syncwarp();                 // every lane is done with the slot that the last chunk left
+            const uint32_t key = chunk[0] * kChunk;
+#pragma unroll
+            for (uint32_t i = 0; i + 1u < kStages; ++i) chunk[i] = chunk[i + 1u];
+            chunk[kStages - 2u] = issue();
+            ok = __all_sync(0xffffffffu, mbar_wait(full + slot, phase, &sm.err));
+            if (!ok) break;
+            const uint32_t in = ring + slot * kSlot;
+            if (++slot == kStages) slot = 0u, phase ^= 1u;
+            float y[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = 0.f;
+#pragma unroll
+            for (uint32_t st = 0; st < 8u; ++st) {
+                uint32_t ka[4];
+                load_matrices(ka, in + (st >> 2) * kHalfChunk + koff + ((kx ^ (2u * (st & 3u))) << 4));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma<BF>(y[nt], ka, qf[nt][st][0], qf[nt][st][1]);
+            }
+            // scores: positions key + g (elements 0, 1) and key + g + 8 (2, 3), columns 2 t and 2 t + 1
+            const bool masked = key + kChunk - 1u > open;   // some row does not see all of the chunk
+            const uint32_t pa = key + g, pb = key + g + 8u;
+            bool raise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    y[nt][e] *= kScoreScale;
+                    if (masked && (e < 2 ? pa : pb) > last[nt][e & 1]) y[nt][e] = -INFINITY;
+                    raise |= y[nt][e] > m[nt][e & 1] + kLazy;
+                }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float f[2] = {1.0f, 1.0f};
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(y[nt][e], y[nt][2 + e]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        if (x > m[nt][e] + kLazy) {
+                            f[e] = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - x);
+                            m[nt][e] = x;
+                            l[nt][e] *= f[e];
+                        }
+                    }
+                    const uint64_t f2 = pair(f[0], f[1]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        o[nt][j][0] = mul2(o[nt][j][0], f2);
+                        o[nt][j][1] = mul2(o[nt][j][1], f2);
+                    }
+                }
+            }
+            uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float z[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // a row that has seen no position yet has no maximum: its weights are 0 (NaN scores stay)
+                    z[e] = y[nt][e] == -INFINITY ? 0.f : ex2(y[nt][e] - m[nt][e & 1] + kUnit<BF>);
+                    l[nt][e & 1] += z[e];
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t hi = pack<BF>(z[2 * half], z[2 * half + 1]);
+                    bh[nt][half] = transpose8(hi);
+                    bl[nt][half] = transpose8(pack<BF>(z[2 * half] - unpack1<BF>(hi & 0xffffu), z[2 * half + 1] - unpack1<BF>(hi >> 16)));
+                }
+            }
+            uint32_t bad = 0u;            // a value that is not finite where some row does not see it
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t va[4];           // dimensions 16 j + g (0, 2) and + 8 (1, 3); positions 2 t, 2 t + 1 (0, 1) and + 8 (2, 3)
+                load_matrices_t(va, in + (uint32_t)(j >> 2) * kHalfChunk + voff + ((vx ^ (2u * (uint32_t)(j & 3))) << 4));
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t p = key + 2u * t + (i < 2 ? 0u : 8u);
+                        uint32_t n = nonfinite2<BF>(va[i]);
+                        n &= (p > open ? 0xffffu : 0u) | (p + 1u > open ? 0xffff0000u : 0u);
+                        va[i] &= ~n;
+                        bad |= n;
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float x[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma<BF>(x, va, bl[nt][0], bl[nt][1]);
+                    mma<BF>(x, va, bh[nt][0], bh[nt][1]);
+                    o[nt][j][0] = add2(o[nt][j][0], pair(x[0], x[1]));
+                    o[nt][j][1] = add2(o[nt][j][1], pair(x[2], x[3]));
+                }
+            }
+            if (masked && __any_sync(0xffffffffu, bad != 0u)) {   // into the rows that do see them
+                for (uint32_t k = 0; k < kChunk; ++k) {
+                    if (key + k <= open) continue;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf) {
+                            const uint32_t c = (2u * (uint32_t)(j & 3) + (uint32_t)hf) ^ (k & 7u);
+                            uint16_t b;
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(in + 2u * kHalfChunk + (uint32_t)(j >> 2) * kHalfChunk + k * 128u + c * 16u + 2u * g) : "memory");
+                            const float v = unpack1<BF>(b);
+                            if (v - v == 0.f) continue;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                o[nt][j][hf] = add2(o[nt][j][hf], pair(key + k <= last[nt][0] ? v : 0.f, key + k <= last[nt][1] ? v : 0.f));
+                        }
+                }
+            }
+        }
+        if (!ok) {                        // nothing of this warp is left in flight; the rest of its rows become NaN
+#pragma unroll
+            for (uint32_t i = 0; i < kStages; ++i) {
+                const uint64_t t0 = global_ns();
+                while (slot != slot_in && !mbar_try_wait(full + slot, phase) && global_ns() - t0 < kWaitLimitNs) {
+                }
+                if (slot != slot_in && ++slot == kStages) slot = 0u, phase ^= 1u;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __int_as_float(0x7fffffff);
+        }
+        __syncthreads();                  // every warp is done with the ring: it takes the warps' outputs
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = l[nt][e];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const uint32_t i = 8u * (uint32_t)nt + 2u * t + (uint32_t)e;
+                if (g == 0u) sm.wml[warp][i] = make_float2(m[nt][e], x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        float v[2];
+                        unpair(o[nt][j][hf], v[0], v[1]);
+                        sm.u.wrec[warp][i][16 * j + 8 * hf + (int)g] = v[e];
+                    }
+            }
+        __syncthreads();
+        const bool whole = w.head && w.tail;
+        float *const rec = record_of(a, w.record(), R);
+        for (uint32_t x = threadIdx.x; x < rows * (kDim / 4u); x += kThreads) {
+            const uint32_t i = x / (kDim / 4u), d = x % (kDim / 4u);
+            float M = -INFINITY, L = 0.f, f[kWarps];
+#pragma unroll
+            for (uint32_t v = 0; v < kWarps; ++v) M = fmaxf(M, sm.wml[v][i].x);
+#pragma unroll
+            for (uint32_t v = 0; v < kWarps; ++v) {
+                const float2 ml = sm.wml[v][i];
+                f[v] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - M);   // a state of NaNs stays one
+                L = fmaf(f[v], ml.y, L);
+            }
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (uint32_t v = 0; v < kWarps; ++v) {
+                const float4 z = *reinterpret_cast<const float4 *>(&sm.u.wrec[v][i][4u * d]);
+                y.x = fmaf(f[v], z.x, y.x);
+                y.y = fmaf(f[v], z.y, y.y);
+                y.z = fmaf(f[v], z.z, y.z);
+                y.w = fmaf(f[v], z.w, y.w);
+            }
+            if (whole) {
+                const float inv = L == 0.f ? 0.f : 1.0f / L;
+                store4<BF>(a, s, h, tr.at(i), d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+            } else {
+                __stcg(reinterpret_cast<float4 *>(rec) + i * (kDim / 4u) + d, y);
+                if (d == 0u) __stcg(reinterpret_cast<float2 *>(rec + R * kDim) + i, make_float2(M, L));
+            }
+        }
+        fence_ring();
+        __syncthreads();                  // the ring may fill again
+    }
+}
+
+// --------------------------------------------------------- partial sums ----
+//
+// The units that pieces cut: the CTA whose number is that of the piece that a
+// unit ends in joins its records, a warp per row (lane: a record's maximum and
+// sum, then 4 dimensions). Bound by latency: a call whose pieces are whole units
+// leaves nothing to join.
+struct MergeArgs : AttnArgs {
+    uint32_t tile, per;                   // rows of a record; of rows that a CTA takes
+};
+
+constexpr uint32_t kMergeWarps = 8;
+
+template <bool BF>
+__global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __grid_constant__ MergeArgs a)
+{
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    wait_predecessor(a.early);
+    const uint4 lo = __ldcg(reinterpret_cast<const uint4 *>(a.parts) + 2u * blockIdx.x), hi = __ldcg(reinterpret_cast<const uint4 *>(a.parts) + 2u * blockIdx.x + 1u);
+    const uint32_t first = lo.x, count = lo.y, s = lo.z, h = lo.w, row0 = hi.x, rows = hi.y;
+    if (first == ~0u) return;
+    // record i of the unit
+    auto record = [&](uint32_t i) { return record_of(a, i ? 2u * (first / 2u + i) : first, a.tile); };
+    for (uint32_t r = blockIdx.y * a.per + warp; r < min(rows, (blockIdx.y + 1u) * a.per); r += kMergeWarps) {
+        float M = -INFINITY, L = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t b = 0; b < count; b += 32u) {
+            const float2 ml = b + lane < count ? __ldcg(reinterpret_cast<const float2 *>(record(b + lane) + a.tile * kDim) + r) : make_float2(-INFINITY, 0.f);
+            float most = ml.x;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            most = fmaxf(most, M);
+            const float before = M == -INFINITY ? (L == 0.f ? 0.f : 1.f) : ex2(M - most);
+            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - most);
+            float sum = f * ml.y;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            M = most;
+            L = fmaf(before, L, sum);
+            x = make_float4(x.x * before, x.y * before, x.z * before, x.w * before);
+            const uint32_t n = min(count - b, 32u);
+#pragma unroll 4
+            for (uint32_t i = 0; i < n; ++i) {
+                const float4 y = __ldcg(reinterpret_cast<const float4 *>(record(b + i)) + r * (kDim / 4u) + lane);
+                const float fi = __shfl_sync(0xffffffffu, f, (int)i);
+                x.x = fmaf(fi, y.x, x.x);
+                x.y = fmaf(fi, y.y, x.y);
+                x.z = fmaf(fi, y.z, x.z);
+                x.w = fmaf(fi, y.w, x.w);
+            }
+        }
+        const float inv = L == 0.f ? 0.f : 1.0f / L;
+        const uint32_t row = row0 + r, tok = row / a.group;
+        store4<BF>(a, s, h, make_uint2(tok, row - tok * a.group), lane, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    }
+}
+
+template <bool BF, int NT>
+cudaError_t launch_few_of(const FewArgs &a, int dev, int sms, cudaStream_t stream)
+{
+    const cudaError_t e = k8::allow<few_kernel<BF, NT>>(dev, (int)sizeof(Smem<NT>));
+    if (e != cudaSuccess) return e;
+    return k8::launch(few_kernel<BF, NT>, dim3(std::min((uint32_t)sms, kMaxCtas)), kThreads, sizeof(Smem<NT>), 1, a, sms, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_merge(const AttnArgs &a, bool bf, uint32_t rows, uint32_t ctas, int sms, cudaStream_t stream)
+{
+    MergeArgs m{};
+    static_cast<AttnArgs &>(m) = a;
+    m.tile = rows;
+    m.per = std::min(rows, 32u);
+    const dim3 grid(ctas, (rows + m.per - 1) / m.per);
+    return bf ? k8::launch(part_merge_kernel<true>, grid, kMergeWarps * 32, 0, 1, m, sms, stream)
+              : k8::launch(part_merge_kernel<false>, grid, kMergeWarps * 32, 0, 1, m, sms, stream);
+}
+
+// The few-rows form, for units of 8 nt rows; maps: see FewArgs
+cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtensorMap &vmap, bool bf, int nt, int dev, int sms,
+                       cudaStream_t stream)
+{
+    FewArgs f{};
+    static_cast<AttnArgs &>(f) = a;
+    f.kmap = kmap;
+    f.vmap = vmap;
+    cudaError_t e = nt == 1   ? (bf ? launch_few_of<true, 1>(f, dev, sms, stream) : launch_few_of<false, 1>(f, dev, sms, stream))
+                    : nt == 2 ? (bf ? launch_few_of<true, 2>(f, dev, sms, stream) : launch_few_of<false, 2>(f, dev, sms, stream))
+                              : (bf ? launch_few_of<true, 4>(f, dev, sms, stream) : launch_few_of<false, 4>(f, dev, sms, stream));
+    if (e != cudaSuccess) return e;
+    return launch_merge(a, bf, 8u * (uint32_t)nt, std::min((uint32_t)sms, kMaxCtas), sms, stream);
+}
+
+}  // namespace paged
+}  // namespace atlas

@@ -32,6 +32,8 @@ EXPORTS = [
     "atlas_cuda_tp_connect", "atlas_cuda_prefill_seq", "atlas_cuda_generate_batch", "atlas_cuda_decode_batch",
     "atlas_cuda_kv8_append", "atlas_cuda_kv8_read", "atlas_cuda_kv8_attn", "atlas_cuda_kv8_attn_sparse",
     "atlas_cuda_kv8_attn_form",
+    "atlas_cuda_paged_work", "atlas_cuda_paged_fork", "atlas_cuda_paged_reserve", "atlas_cuda_paged_compact",
+    "atlas_cuda_paged_append", "atlas_cuda_paged_attn",
     "brain_gpu_init", "brain_gpu_matvec_batch", "brain_gpu_matvec", "brain_gpu_shutdown",
     "atlas_rt_open", "atlas_rt_close", "atlas_rt_error", "atlas_rt_shape", "atlas_rt_data_base",
     "atlas_rt_find_tensor", "atlas_rt_file_bytes", "atlas_rt_device", "atlas_rt_forward_token",
@@ -98,6 +100,12 @@ class Kv8Desc(ctypes.Structure):
         (n, ctypes.c_uint32) for n in ("nseq", "kv_heads", "max_context", "block")]
 
 
+class PagedDesc(ctypes.Structure):
+    """AtlasPaged (include/atlas_cuda.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "table", "refs", "work")] + [("work_bytes", ctypes.c_uint64)] + [
+        (n, ctypes.c_uint32) for n in ("type", "layers", "pages", "kv_heads", "page", "nseq", "max_pages")]
+
+
 TP_HANDLE_BYTES = 64
 
 
@@ -157,6 +165,12 @@ def lib() -> ctypes.CDLL:
         L.atlas_cuda_kv8_attn.argtypes = [P, U32, U32, P, P, P, U64, P, U64, P]
         L.atlas_cuda_kv8_attn_form.argtypes = [P, U32, U32, P, P]
         L.atlas_cuda_kv8_attn_sparse.argtypes = [P, U32, U32, U32, P, P, P, U64, P, U64, P, P]
+        L.atlas_cuda_paged_work.argtypes = [P, P]
+        L.atlas_cuda_paged_fork.argtypes = [P, P, P, P, P]
+        L.atlas_cuda_paged_reserve.argtypes = [P, U32, P, P, P, P]
+        L.atlas_cuda_paged_compact.argtypes = [P, P, P]
+        L.atlas_cuda_paged_append.argtypes = [P, U32, U32, P, P, P, P, U64, P]
+        L.atlas_cuda_paged_attn.argtypes = [P, U32, U32, U32, P, P, P, U64, P, U64, P]
         L.atlas_synth_write_gguf.argtypes = [P, ctypes.c_char_p]
         L.atlas_synth_q4k_blocks.argtypes = [U64, U64, P, U64]
         L.atlas_synth_q6k_blocks.argtypes = [U64, U64, P, U64]
@@ -450,9 +464,9 @@ def _kv8_ints(who: str, name: str, t, n: int) -> None:
         raise AtlasError(-1, f"{who}: {name} must be {n} dense 32-bit integers")
 
 
-def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: int) -> None:
-    """Refuses a tensor that is not token rows [nseq, tokens, heads, 128], ld floats from token to token (0: dense). One that
-    is not 4-dimensional must be dense, and long enough."""
+def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: int, kind: str = "float32") -> None:
+    """Refuses a tensor that is not token rows [nseq, tokens, heads, 128] of type `kind`, ld values from token to token (0:
+    dense). One that is not 4-dimensional must be dense, and long enough."""
     if not tokens or not hasattr(t, "dtype"):
         return
     step = ld or heads * 128
@@ -463,9 +477,9 @@ def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: in
               and (nseq == 1 or stride[0] == tokens * step))
     else:
         ok = t.is_contiguous() and t.numel() >= (nseq * tokens - 1) * step + heads * 128
-    if not ok or _kind(t) != "float32":
-        raise AtlasError(-1, f"{who}: {name} must be float32 rows of {nseq} sequences x {tokens} tokens x {heads} heads x 128, "
-                             f"{step} floats from token to token")
+    if not ok or _kind(t) != kind:
+        raise AtlasError(-1, f"{who}: {name} must be {kind} rows of {nseq} sequences x {tokens} tokens x {heads} heads x 128, "
+                             f"{step} values from token to token")
 
 
 def _kv8_check(who: str, cache: Kv8Cache, tokens: int, heads: int, pos0, n_tok, names, a, lda: int, b, ldb: int) -> None:
@@ -530,3 +544,97 @@ def kv8_attn_sparse(cache: Kv8Cache, q_heads: int, tokens: int, n_sel: int, pos0
     check(lib().atlas_cuda_kv8_attn_sparse(cache._ref, q_heads, tokens, n_sel, pos0.data_ptr(), _addr(n_tok),
                                            q.data_ptr(), ldq, out.data_ptr(), ldo, sel.data_ptr(), stream),
           "kv8_attn_sparse")
+
+
+_PAGED_TYPES = {"float16": 0, "bfloat16": 1}
+
+
+class PagedCache:
+    """A paged KV cache of all layers in caller-owned device buffers (AtlasPaged, include/atlas_cuda.h).
+
+    k, v: float16 or bfloat16 [layers, pages, kv_heads, page, 128]; table: int32 [nseq, max_pages], -1 where there is no page;
+    refs: int32 [pages], how many entries name each page. An empty cache has a table of -1 and refs of 0. `work`: the calls'
+    workspace, at least paged_work_bytes(pages) bytes of the same device (None: one is made). The object keeps references to
+    the tensors. Calls on one cache are ordered by their streams; caches that share a workspace count as one."""
+
+    def __init__(self, k, v, table, refs, work=None):
+        if (k.dim() != 5 or k.shape[4] != 128 or tuple(v.shape) != tuple(k.shape) or _kind(k) not in _PAGED_TYPES
+                or _kind(v) != _kind(k) or not k.is_contiguous() or not v.is_contiguous()):
+            raise ValueError("PagedCache: k and v must be dense float16 or bfloat16 [layers, pages, kv_heads, page, 128]")
+        self.layers, self.pages, self.kv_heads, self.page = (int(x) for x in k.shape[:4])
+        if table.dim() != 2 or _kind(table) != "int32" or not table.is_contiguous():
+            raise ValueError("PagedCache: the table must be dense int32 [nseq, max_pages]")
+        if refs.dim() != 1 or refs.numel() != self.pages or _kind(refs) != "int32" or not refs.is_contiguous():
+            raise ValueError("PagedCache: refs must be dense int32 [pages]")
+        self.nseq, self.max_pages = (int(x) for x in table.shape)
+        self.kind, self.dtype, self._i32 = _kind(k), k.dtype, table.dtype
+        self.desc = PagedDesc(k.data_ptr(), v.data_ptr(), table.data_ptr(), refs.data_ptr(), None, 0, _PAGED_TYPES[self.kind],
+                              self.layers, self.pages, self.kv_heads, self.page, self.nseq, self.max_pages)
+        self._ref = ctypes.byref(self.desc)
+        need = ctypes.c_uint64()
+        check(lib().atlas_cuda_paged_work(self._ref, ctypes.byref(need)), "paged_work")
+        if work is None:
+            work = k.new_empty((need.value + 1) // 2)   # of 2-byte values
+        if not work.is_contiguous() or work.nbytes < need.value:
+            raise ValueError(f"PagedCache: the workspace must be {need.value} dense bytes")
+        self.buffers = (k, v, table, refs, work)
+        if len({t.device for t in self.buffers}) != 1:
+            raise ValueError("PagedCache: the buffers must be of one device")
+        self.desc.work, self.desc.work_bytes = work.data_ptr(), work.nbytes
+
+
+def _paged_check(who: str, cache: PagedCache, tokens: int, heads: int, pos0, n_tok, names=(), a=None, lda: int = 0, b=None,
+                 ldb: int = 0) -> None:
+    """Refuses tensors of another type, layout or size. a, b: rows of `heads` each, or None. Dense ones of just the size, as
+    most calls have, pass at once."""
+    n, size, kind, i32 = cache.nseq, cache.nseq * tokens * heads * 256, cache.dtype, cache._i32
+    if ((a is None or a.dtype is kind and b.dtype is kind and a.nbytes == size and b.nbytes == size and not lda and not ldb
+         and a.is_contiguous() and b.is_contiguous())
+            and pos0.dtype is i32 and pos0.nbytes == 4 * n and pos0.is_contiguous()
+            and (n_tok is None or n_tok.dtype is i32 and n_tok.nbytes == 4 * n and n_tok.is_contiguous())):
+        return
+    if a is not None:
+        _kv8_rows(who, names[0], a, n, tokens, heads, lda, cache.kind)
+        _kv8_rows(who, names[1], b, n, tokens, heads, ldb, cache.kind)
+    _kv8_ints(who, "pos0", pos0, n)
+    _kv8_ints(who, "n_tok", n_tok, n)
+
+
+def paged_fork(cache: PagedCache, parent, length, first=None, stream: int = 0) -> None:
+    """Sequence s becomes what sequence parent[s] was up to position length[s] (and from first[s] on): int32 [nseq] each.
+    atlas_cuda_paged_fork. Here and below, `stream` is a cudaStream_t (0: the legacy default stream), and tensors of another
+    type, layout or size are refused."""
+    for name, t in (("parent", parent), ("length", length), ("first", first)):
+        _kv8_ints("paged_fork", name, t, cache.nseq)
+    check(lib().atlas_cuda_paged_fork(cache._ref, parent.data_ptr(), length.data_ptr(), _addr(first), stream), "paged_fork")
+
+
+def paged_reserve(cache: PagedCache, tokens: int, pos0, short, n_tok=None, stream: int = 0) -> None:
+    """Gives each sequence s pages of its own for positions pos0[s], ... of its next n_tok[s] tokens (None: `tokens`); short
+    (int32 [1]) receives how many pages are lacking, and then nothing has changed. atlas_cuda_paged_reserve."""
+    _paged_check("paged_reserve", cache, tokens, 0, pos0, n_tok)
+    _kv8_ints("paged_reserve", "short", short, 1)
+    check(lib().atlas_cuda_paged_reserve(cache._ref, tokens, pos0.data_ptr(), _addr(n_tok), short.data_ptr(), stream),
+          "paged_reserve")
+
+
+def paged_compact(cache: PagedCache, used, stream: int = 0) -> None:
+    """Moves the pages in use to the pool's start; used (int32 [1]) receives how many there are. atlas_cuda_paged_compact."""
+    _kv8_ints("paged_compact", "used", used, 1)
+    check(lib().atlas_cuda_paged_compact(cache._ref, used.data_ptr(), stream), "paged_compact")
+
+
+def paged_append(cache: PagedCache, layer: int, tokens: int, pos0, k, v, n_tok=None, ld: int = 0, stream: int = 0) -> None:
+    """Stores up to `tokens` new rows k, v [nseq, tokens, kv_heads, 128] of a layer at positions pos0[s], ... (pos0, n_tok:
+    int32 [nseq]; n_tok None: all of them). atlas_cuda_paged_append."""
+    _paged_check("paged_append", cache, tokens, cache.kv_heads, pos0, n_tok, ("k", "v"), k, ld, v, ld)
+    check(lib().atlas_cuda_paged_append(cache._ref, layer, tokens, pos0.data_ptr(), _addr(n_tok), k.data_ptr(), v.data_ptr(),
+                                        ld, stream), "paged_append")
+
+
+def paged_attn(cache: PagedCache, layer: int, q_heads: int, tokens: int, pos0, q, out, n_tok=None, ldq: int = 0, ldo: int = 0,
+               stream: int = 0) -> None:
+    """Causal attention of q [nseq, tokens, q_heads, 128] over a layer's pages into out. atlas_cuda_paged_attn."""
+    _paged_check("paged_attn", cache, tokens, q_heads, pos0, n_tok, ("q", "out"), q, ldq, out, ldo)
+    check(lib().atlas_cuda_paged_attn(cache._ref, layer, q_heads, tokens, pos0.data_ptr(), _addr(n_tok), q.data_ptr(), ldq,
+                                      out.data_ptr(), ldo, stream), "paged_attn")

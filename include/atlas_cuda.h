@@ -322,6 +322,96 @@ int atlas_cuda_kv8_attn_sparse(const AtlasKv8 *cache, uint32_t q_heads, uint32_t
                                const uint32_t *d_pos0, const uint32_t *d_ntok, const float *d_q, uint64_t ldq,
                                float *d_out, uint64_t ldo, int32_t *d_sel, void *stream);
 
+/* ---- paged 16-bit KV cache over caller-owned DEVICE memory ----
+
+   K and V of all layers and of sequences of different lengths in one pool of
+   pages, binary16 or bfloat16: k, v [layers][pages][kv_heads][page][128]. (The
+   reference has one region of its whole context per process,
+   src/brain_runtime.c:2019-2020, and attends per token, :1407-1528.) Entry j of
+   a sequence's row of `table` is the page that holds its positions j * page ..
+   j * page + page - 1; a number that is no page's (-1) means none. refs[p] is
+   how many entries name page p, 0: it is free. A page may be part of several
+   sequences. An empty cache has a table of -1 and refs of 0. Whoever writes
+   table or refs by other means than the calls below keeps refs the count of the
+   table's entries; entries that name no page are never followed.
+
+   All calls are asynchronous on `stream` (a cudaStream_t or NULL), allocate
+   nothing and may be captured into a graph: positions, table and counts are read
+   and changed on the device. They run on the current device; every pointer must
+   be memory of that device, or the call returns ATLAS_EINVAL. Calls on the same
+   cache must be ordered by their streams, replays of captured ones too, and each
+   cache needs a workspace of its own; calls on different caches may overlap. The
+   workspace's contents mean nothing between calls.
+
+   A call handles all `nseq` sequences: sequence s has n_tok[s] token rows
+   (d_ntok NULL: all `tokens`; a larger n_tok[s] counts as `tokens`) at positions
+   pos0[s], pos0[s] + 1, ... Rows from n_tok[s] on are left as they were, so 0
+   leaves a sequence out. Token rows are [seq][tokens][heads][128] values of the
+   cache's type, `ld` values from token to token (0: dense; a multiple of 8; the
+   sequence stride is tokens * ld), 16-byte aligned. */
+#define ATLAS_PAGED_FP16 0u
+#define ATLAS_PAGED_BF16 1u
+
+typedef struct AtlasPaged {
+    void *k, *v;                /* 16-byte aligned */
+    int32_t *table;             /* [nseq][max_pages] */
+    int32_t *refs;              /* [pages], 16-byte aligned */
+    void *work;                 /* atlas_cuda_paged_work bytes, 256-byte aligned */
+    uint64_t work_bytes;
+    uint32_t type;              /* ATLAS_PAGED_FP16 or ATLAS_PAGED_BF16 */
+    uint32_t layers, pages, kv_heads;   /* layers * pages * kv_heads * page < 2^31 */
+    uint32_t page;              /* positions per page: 16, 32, 64 or 128 */
+    uint32_t nseq, max_pages;   /* up to 4096 sequences */
+} AtlasPaged;
+
+/* The workspace that a cache of this shape (type to max_pages) needs. */
+int atlas_cuda_paged_work(const AtlasPaged *cache, uint64_t *bytes);
+
+/* Sequence s becomes what sequence parent[s] was up to position length[s]: its
+   entries are the parent's, of the pages that begin before length[s] and, where
+   d_first is not NULL, end behind position first[s]; the others become -1. All
+   sequences are read before any is written, so parents may be forked, replaced
+   and exchanged in one call. parent[s] = s with a smaller length frees a
+   sequence's end, with `first` its beginning; a parent that is no sequence (-1)
+   frees all of it. No row moves: forked sequences have pages in common until
+   paged_reserve parts them. */
+int atlas_cuda_paged_fork(const AtlasPaged *cache, const int32_t *d_parent, const uint32_t *d_length, const uint32_t *d_first,
+                          void *stream);
+
+/* Before new rows are stored: gives every sequence pages of its own for its
+   positions pos0[s] .. pos0[s] + n_tok[s] - 1 (positions behind the table's end
+   are left out). Entries without a page, or whose page is named by other entries
+   too, get the lowest free pages, in the order of sequences and positions; of a
+   page that only entries of this call name, the last one keeps it. Where the
+   first of a sequence's pages is replaced, the rows before pos0[s] in it are
+   copied, in all layers; other rows of a new page are left as they were. All or
+   nothing: *d_short receives how many pages are lacking; if it is not 0,
+   nothing has changed. */
+int atlas_cuda_paged_reserve(const AtlasPaged *cache, uint32_t tokens, const uint32_t *d_pos0, const uint32_t *d_ntok,
+                             uint32_t *d_short, void *stream);
+
+/* Moves the pages in use together: of U pages in use (*d_used receives U), the
+   i-th one numbered U or more goes to the i-th free one below U, in all layers,
+   and table and refs follow. */
+int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_used, void *stream);
+
+/* Stores new rows of a layer (K after RoPE) at their positions. A row whose
+   position has no page, or one that more than one entry names, is dropped. */
+int atlas_cuda_paged_append(const AtlasPaged *cache, uint32_t layer, uint32_t tokens, const uint32_t *d_pos0, const uint32_t *d_ntok,
+                            const void *d_k, const void *d_v, uint64_t ld, void *stream);
+
+/* Causal grouped-query attention of a chunk of new tokens: the query rows of
+   position p see the positions 0 .. p that have a page, scores q.k / sqrt(128),
+   softmax and sums in fp32, rounded once at the end. Rows that see nothing are
+   zeros. What lies at positions that a row does not see has no part in it,
+   infinities and NaN among it; a value that is not finite at a position that it
+   does see makes what it enters infinite or NaN. q_heads is a multiple of
+   kv_heads; q and out must not overlap. Which kernels run, and so the last bits
+   of a row, depends on the call's sizes and positions; the same call gives the
+   same bits. */
+int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
+                          const uint32_t *d_ntok, const void *d_q, uint64_t ldq, void *d_out, uint64_t ldo, void *stream);
+
 /* Number of SMs / compute capability of `device`, or a negative code. */
 int atlas_cuda_device_info(int device, int *sm_count, int *cc_major, int *cc_minor);
 
