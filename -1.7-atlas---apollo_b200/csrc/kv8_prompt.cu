@@ -61,6 +61,7 @@
 #include <cmath>
 #include "../../include/atlas_cuda.h"
 #include "kv8.cuh"
+#include "tcgen05.cuh"
 
 namespace atlas {
 namespace k8 {
@@ -94,91 +95,8 @@ constexpr size_t kRawTile = 128 * 128;             // bytes of 128 rows of codes
 constexpr size_t kPromptSmem = 2 * kQTile + 4 * kHalf + 2 * kRawTile + sizeof(PromptBars);
 static_assert(kPromptSmem <= kMaxSmem, "the tiles exceed a CTA's shared memory");
 
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile uint32_t *err)
-{
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
-}
-
-// Shared-memory operand: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart
-__device__ __forceinline__ uint64_t operand(uint32_t saddr)
-{
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) |
-           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
-}
-
 // fp32 accumulator, binary16 operands, K-major, M = 128, N = 128
 constexpr uint32_t kInstr = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate)
-{
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(kInstr), "r"(accumulate)
-                 : "memory");
-}
-
-// A from tensor memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate)
-{
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 ::"r"(d), "r"(a), "l"(b), "r"(kInstr), "r"(accumulate)
-                 : "memory");
-}
-
-// Arrives on `bar` once every MMA that this lane issued is done
-__device__ __forceinline__ void commit(uint64_t *bar)
-{
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-// One lane of the (converged) warp
-__device__ __forceinline__ bool elected()
-{
-    uint32_t e;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
-    return e != 0u;
-}
-
-// 16 columns of this warp's lanes; the values are there after tmem_wait_ld
-__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&r)[16])
-{
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-        : "r"(addr)
-        : "memory");
-}
-
-// Names the registers, so that no use of them moves before the wait
-__device__ __forceinline__ void tmem_wait_ld(float (&r)[16])
-{
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
-                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
-                 :
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[16])
-{
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// Byte offset of 16-byte chunk `chunk` of a row of a swizzled tile of 128-byte rows
-__device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk)
-{
-    return row * 128u + ((chunk ^ (row & 7u)) << 4);
-}
 
 __device__ __forceinline__ float4 ld_cluster4(const void *p, uint32_t cta)
 {
@@ -195,13 +113,6 @@ __device__ __forceinline__ float ld_cluster1(const void *p, uint32_t cta)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(cta));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r));
     return v;
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c)
-{
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
 }
 
 // What a warp knows of a tile's 16-key groups: lane i has the scale of the K codes (i < 8) or V codes (8 <= i < 16) of
@@ -310,9 +221,6 @@ __device__ __forceinline__ float tile_weights(uint32_t at, const Scales &sc, flo
 // The integer below x; 0 for none
 __device__ __forceinline__ int below(float x) { return x == x ? (int)fminf(fmaxf(floorf(x), -250.0f), 250.0f) : 0; }
 
-// Barrier `id` of `threads` threads (whole warps)
-__device__ __forceinline__ void meet(uint32_t id, uint32_t threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there)   // zeros where !there
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
@@ -320,12 +228,6 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copy_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 __device__ __forceinline__ void copy_wait0() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
-
-// Registers of the calling warpgroup's threads: taken once others have left them
-template <uint32_t N>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <uint32_t N>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <bool ONE>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_constant__ AttnArgs a)
@@ -496,8 +398,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 #pragma unroll
                     for (uint32_t st = 0; st < 4u; ++st) {
                         const uint32_t off = hf * (kHalf >> 4) + st * 2u;
-                        mma_ss(tmem + 128u * t, q + off, k + off, hf != 0u || st != 0u);
-                        mma_ss(tmem + 128u * t, q + (2u * kHalf >> 4) + off, k + off, 1u);
+                        mma_ss(tmem + 128u * t, q + off, k + off, kInstr, hf != 0u || st != 0u);
+                        mma_ss(tmem + 128u * t, q + (2u * kHalf >> 4) + off, k + off, kInstr, 1u);
                     }
                     if (last_use) commit(&b.k_empty[buffer(j)][hf]);
                 }
@@ -513,8 +415,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                     for (uint32_t st = 0; st < 4u; ++st) {
                         const uint64_t v = (buffer(j) ? vd[1] : vd[0]) + hf * (kHalf >> 4) + st * 2u;
                         const uint32_t p = tmem + 128u * t + 64u * hf + 16u * st;
-                        mma_ts(tmem + 256u + 128u * t, p, v, hf != 0u || st != 0u);
-                        mma_ts(tmem + 256u + 128u * t, p + 8u, v, 1u);
+                        mma_ts(tmem + 256u + 128u * t, p, v, kInstr, hf != 0u || st != 0u);
+                        mma_ts(tmem + 256u + 128u * t, p + 8u, v, kInstr, 1u);
                     }
                     if (last_use) commit(&b.v_empty[buffer(j)][hf]);
                 }

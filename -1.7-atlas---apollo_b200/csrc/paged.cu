@@ -23,6 +23,9 @@ using k8::wait_predecessor;
 // paged_attn.cu
 cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtensorMap &vmap, bool bf, int nt, int dev, int sms,
                        cudaStream_t stream);
+// paged_prompt.cu
+cudaError_t launch_prompt(const AttnArgs &a, const CUtensorMap &kmap, const CUtensorMap &vmap, const CUtensorMap &qmap, bool bf, uint32_t tiles, int dev,
+                          int sms, cudaStream_t stream);
 
 namespace {
 
@@ -662,6 +665,51 @@ extern "C" int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_use
     return done(who, launch_move(a.c, cache->pages / 2u, (uint64_t)cache->nseq * cache->max_pages, sms, (cudaStream_t)stream));
 }
 
+namespace {
+
+// The query rows of a KV head that a CTA takes at a time: 8, 16 or 32 (the form for few rows), 128 or 256
+uint32_t attn_rows(const Cache &c, uint32_t group, uint32_t tokens, int sms)
+{
+    const uint64_t rows = (uint64_t)tokens * group;
+    if (rows <= 32 || group > 128) return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    const uint32_t per = 128 / group;
+    return (uint64_t)c.nseq * c.kv_heads * ((tokens + per - 1) / per) <= (uint64_t)sms ? 128 : 256;
+}
+
+// The token rows of q as [2 halves of 64 dimensions][token][head][64], for copies of a KV head's group of heads of `tokens` tokens
+int map_queries(const char *who, Encode encode, const AttnArgs &a, bool bf, uint32_t tokens, CUtensorMap &map)
+{
+    const cuuint64_t dims[4] = {kDim / 2, a.q_heads, (cuuint64_t)a.c.nseq * a.r.tokens, 2}, strides[3] = {kRowBytes, a.ldq * 2, kRowBytes / 2};
+    const cuuint32_t boxes[4] = {kDim / 2, a.group, tokens, 1}, steps[4] = {1, 1, 1, 1};
+    if (encode(&map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t *>(a.q), dims, strides, boxes,
+               steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return api_fail(ATLAS_ECUDA, "%s: the token rows cannot be described to the copy engine", who);
+    return ATLAS_OK;
+}
+
+int check_heads(const char *who, const AtlasPaged *cache, uint32_t q_heads, uint32_t tokens)
+{
+    if (!q_heads || q_heads % cache->kv_heads || q_heads > 32768u || (uint64_t)q_heads * tokens > 0x3fffffffull ||
+        (uint64_t)tokens * cache->nseq > 0x7fffffffull)
+        return api_fail(ATLAS_EINVAL, "%s: %u query heads over %u KV heads, %u tokens", who, q_heads, cache->kv_heads, tokens);
+    return ATLAS_OK;
+}
+
+}  // namespace
+
+extern "C" int atlas_cuda_paged_attn_form(const AtlasPaged *cache, uint32_t q_heads, uint32_t tokens, uint32_t *rows)
+{
+    const char *who = "paged_attn_form";
+    if (!cache || !rows) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
+    Cache c;
+    int dev, sms, rc = open_cache(who, cache, c, dev, sms);
+    if (rc == ATLAS_OK) rc = check_heads(who, cache, q_heads, tokens);
+    if (rc == ATLAS_OK && !tokens) rc = api_fail(ATLAS_EINVAL, "%s: no tokens", who);
+    if (rc == ATLAS_OK) *rows = attn_rows(c, q_heads / cache->kv_heads, tokens, sms);
+    return rc;
+}
+
 extern "C" int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
                                      const uint32_t *d_ntok, const void *d_q, uint64_t ldq, void *d_out, uint64_t ldo, void *stream)
 {
@@ -672,8 +720,7 @@ extern "C" int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, ui
     int dev, sms, rc = open_cache(who, cache, a.c, dev, sms);
     if (rc == ATLAS_OK) rc = check_tokens(who, tokens, d_pos0, d_ntok, a.r, dev);
     if (rc != ATLAS_OK) return rc;
-    if (!q_heads || q_heads % cache->kv_heads || q_heads > 32768u || (uint64_t)q_heads * tokens > 0x3fffffffull)
-        return api_fail(ATLAS_EINVAL, "%s: %u query heads over %u KV heads, %u tokens", who, q_heads, cache->kv_heads, tokens);
+    if ((rc = check_heads(who, cache, q_heads, tokens)) != ATLAS_OK) return rc;
     if (layer >= cache->layers) return api_fail(ATLAS_EINVAL, "%s: layer %u of %u", who, layer, cache->layers);
     if (!tokens) return ATLAS_OK;               // no rows need no memory
     if ((rc = check_rows(who, d_q, q_heads, ldq, dev)) != ATLAS_OK) return rc;
@@ -687,11 +734,16 @@ extern "C" int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, ui
     a.layer = layer;
     a.parts = reinterpret_cast<float *>(static_cast<char *>(cache->work) + parts_offset(cache->pages));
     const bool bf = cache->type == ATLAS_PAGED_BF16;
-    const uint32_t rows = tokens * a.group;
+    const uint32_t rows = attn_rows(a.c, a.group, tokens, sms);
+    const bool prompt = rows >= 128;
     Encode encode;
     if ((rc = find_encode(who, encode)) != ATLAS_OK) return rc;
-    CUtensorMap kmap, vmap;
-    if ((rc = map_pool(who, encode, a.c, bf, cache->k, 16, 2, kmap)) != ATLAS_OK) return rc;
-    if ((rc = map_pool(who, encode, a.c, bf, cache->v, 16, 2, vmap)) != ATLAS_OK) return rc;
-    return done(who, launch_few(a, kmap, vmap, bf, rows <= 8 ? 1 : rows <= 16 ? 2 : 4, dev, sms, (cudaStream_t)stream));
+    CUtensorMap kmap, vmap, qmap;
+    // 16 rows of all dimensions at a time, or a page's of half of them
+    const uint32_t box = prompt ? cache->page : 16, halves = prompt ? 1 : 2;
+    if ((rc = map_pool(who, encode, a.c, bf, cache->k, box, halves, kmap)) != ATLAS_OK) return rc;
+    if ((rc = map_pool(who, encode, a.c, bf, cache->v, box, halves, vmap)) != ATLAS_OK) return rc;
+    if (!prompt) return done(who, launch_few(a, kmap, vmap, bf, (int)rows / 8, dev, sms, (cudaStream_t)stream));
+    if ((rc = map_queries(who, encode, a, bf, 128 / a.group, qmap)) != ATLAS_OK) return rc;
+    return done(who, launch_prompt(a, kmap, vmap, qmap, bf, rows / 128, dev, sms, (cudaStream_t)stream));
 }

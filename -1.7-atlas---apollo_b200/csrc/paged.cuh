@@ -202,17 +202,18 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
     }
 }
 
-// Walks over the units of a piece. The whole warp.
-template <uint32_t KEYS>
+// Walks over the units of a piece, MOST tiles of keys at a time. The whole warp.
+template <uint32_t KEYS, uint32_t MOST = 0x7fffffffu>
 struct Walk {
     const Cut<KEYS> &cut;
     Piece p;
     Seq q;
-    uint32_t k_begin, k_end;              // this piece's tiles of keys of the current unit
-    bool head, tail;                      // the unit's first tile is in the piece, and its last
+    uint32_t k_begin, k_end;              // the step's tiles of keys of the current unit
+    bool head, tail;                      // the unit's first tile is in the piece, and its last in the step
     bool first;                           // it is the piece's first unit
+    bool again;                           // there were steps of the unit before in this piece
 
-    __device__ __forceinline__ Walk(const Cut<KEYS> &cut_, const Piece &p_) : cut(cut_), p(p_), first(true)
+    __device__ __forceinline__ Walk(const Cut<KEYS> &cut_, const Piece &p_) : cut(cut_), p(p_), first(true), again(false)
     {
         if (p.left) {
             q = cut.open(p.s);
@@ -225,17 +226,23 @@ struct Walk {
     __device__ __forceinline__ void set()
     {
         const uint32_t all = cut.cost(q, p.i);
-        head = p.skip == 0u;
+        if (!again) head = p.skip == 0u;
         k_begin = q.k0 + p.skip;
-        const uint32_t n = (uint32_t)min((uint64_t)(all - p.skip), p.left);
+        const uint32_t n = (uint32_t)min((uint64_t)min(all - p.skip, MOST), p.left);
         k_end = k_begin + n;
         tail = p.skip + n == all;
     }
     __device__ __forceinline__ void next()
     {
         p.left -= k_end - k_begin;
+        if (!tail && p.left) {
+            p.skip += k_end - k_begin;
+            again = true;
+            set();
+            return;
+        }
         p.skip = 0u;
-        first = false;
+        first = again = false;
         if (!p.left) return;
         if (++p.i >= cut.units(q)) {
             p.i = 0u;
@@ -249,12 +256,14 @@ struct Walk {
     }
     // where this piece's part of a cut unit goes
     __device__ __forceinline__ uint32_t record() const { return 2u * blockIdx.x + (first ? 0u : 1u); }
-    // what the merge has to know: of the piece's first unit, if others began it and it ends here
+    // nothing of the unit follows in this piece
+    __device__ __forceinline__ bool leaves() const { return tail || p.left == k_end - k_begin; }
+    // what the merge has to know: of the piece's first unit, if others began it and it ends here. Before the first next().
     __device__ __forceinline__ Part part() const
     {
         Part r{};
         r.first = ~0u;
-        if (p.left && !head && tail) {
+        if (p.left && !head && cut.cost(q, p.i) - p.skip <= p.left) {
             const uint64_t unit = p.begin - p.skip;
             const uint32_t c = (uint32_t)(unit / p.each);
             r.first = 2u * c + (unit == p.each * c ? 0u : 1u);

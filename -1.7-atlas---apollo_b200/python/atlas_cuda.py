@@ -33,7 +33,7 @@ EXPORTS = [
     "atlas_cuda_kv8_append", "atlas_cuda_kv8_read", "atlas_cuda_kv8_attn", "atlas_cuda_kv8_attn_sparse",
     "atlas_cuda_kv8_attn_form",
     "atlas_cuda_paged_work", "atlas_cuda_paged_fork", "atlas_cuda_paged_reserve", "atlas_cuda_paged_compact",
-    "atlas_cuda_paged_append", "atlas_cuda_paged_attn",
+    "atlas_cuda_paged_append", "atlas_cuda_paged_attn", "atlas_cuda_paged_attn_form",
     "brain_gpu_init", "brain_gpu_matvec_batch", "brain_gpu_matvec", "brain_gpu_shutdown",
     "atlas_rt_open", "atlas_rt_close", "atlas_rt_error", "atlas_rt_shape", "atlas_rt_data_base",
     "atlas_rt_find_tensor", "atlas_rt_file_bytes", "atlas_rt_device", "atlas_rt_forward_token",
@@ -170,6 +170,7 @@ def lib() -> ctypes.CDLL:
         L.atlas_cuda_paged_reserve.argtypes = [P, U32, P, P, P, P]
         L.atlas_cuda_paged_compact.argtypes = [P, P, P]
         L.atlas_cuda_paged_append.argtypes = [P, U32, U32, P, P, P, P, U64, P]
+        L.atlas_cuda_paged_attn_form.argtypes = [P, U32, U32, P]
         L.atlas_cuda_paged_attn.argtypes = [P, U32, U32, U32, P, P, P, U64, P, U64, P]
         L.atlas_synth_write_gguf.argtypes = [P, ctypes.c_char_p]
         L.atlas_synth_q4k_blocks.argtypes = [U64, U64, P, U64]
@@ -638,3 +639,10 @@ def paged_attn(cache: PagedCache, layer: int, q_heads: int, tokens: int, pos0, q
     _paged_check("paged_attn", cache, tokens, q_heads, pos0, n_tok, ("q", "out"), q, ldq, out, ldo)
     check(lib().atlas_cuda_paged_attn(cache._ref, layer, q_heads, tokens, pos0.data_ptr(), _addr(n_tok), q.data_ptr(), ldq,
                                       out.data_ptr(), ldo, stream), "paged_attn")
+
+
+def paged_attn_form(cache: PagedCache, q_heads: int, tokens: int) -> int:
+    """The rows of a KV head that a CTA takes at a time in such a paged_attn on the current device. atlas_cuda_paged_attn_form."""
+    rows = ctypes.c_uint32()
+    check(lib().atlas_cuda_paged_attn_form(cache._ref, q_heads, tokens, ctypes.byref(rows)), "paged_attn_form")
+    return rows.value

@@ -62,8 +62,7 @@ class Setup:
         n, tokens, heads, _ = q.shape
         kvh = self.k.shape[2]
         grp = heads // kvh
-        # rows that enter MMAs by their 16-bit weights are those of the form for many rows
-        one_term = True
+        one_term = atlas_cuda.paged_attn_form(self.c, heads, tokens) >= 128
         for s in range(n):
             m = tokens if ntok is None else min(int(ntok[s]), tokens)
             assert torch.equal(out[s, m:], torch.full_like(out[s, m:], 7.0))
