@@ -376,48 +376,106 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(const __grid_cons
 }
 
 // Carries out a plan: the first rows of pages, in every layer, K and V, to other
-// pages, and the table's new numbers. No target is a source. A CTA takes 16 rows
-// of a KV head at a time (4 KB, one 16-byte access a thread), four such pieces on
-// their way at once. Bound by HBM.
+// pages, and the table's new numbers. No target is a source. Rows that follow one
+// another in both pages go 64 at a time (16 KB): pieces of whole pages, whose KV
+// heads follow one another too, or of a head's first rows. Each of a CTA's warps
+// has one lane bring pieces into shared memory and out again by bulk copies, four
+// buffers a warp, so that 192 KB an SM are on their way without a register.
+// Bound by HBM.
 struct MoveArgs {
     Cache c;
     uint32_t early;
 };
 
-constexpr uint32_t kMoveThreads = 256, kMoveAtOnce = 4;
+constexpr uint32_t kMoveWarps = 3, kMoveThreads = kMoveWarps * 32, kMoveStages = 4, kMoveRows = 64;
+
+struct alignas(128) MoveSmem {
+    uint8_t buffer[kMoveWarps][kMoveStages][kMoveRows * kRowBytes];
+    uint64_t full[kMoveWarps][kMoveStages];
+    uint32_t err;
+};
 
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveArgs a)
 {
+    extern __shared__ __align__(128) uint8_t move_smem[];
+    MoveSmem &sm = *reinterpret_cast<MoveSmem *>(move_smem);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    if (lane == 0u) {
+        for (uint32_t i = 0; i < kMoveStages; ++i) mbar_init(&sm.full[warp][i], 1u);
+        fence_mbar_init();
+    }
+    if (threadIdx.x == 0u) sm.err = kStatusOk;
+    __syncthreads();
     wait_predecessor(a.early);
     const uint32_t copies = __ldcg(&head_of(a.c)->copies), moved_from = __ldcg(&head_of(a.c)->from);
-    const uint32_t *from = array_of(a.c, kCopyFrom), *to = array_of(a.c, kCopyTo), *rows = array_of(a.c, kCopyRows);
-    const uint32_t subs_log2 = a.c.page_log2 - 4u;
-    const uint32_t pieces = copies * a.c.layers * 2u * a.c.kv_heads << subs_log2;
-    for (uint32_t b = blockIdx.x; b < pieces; b += gridDim.x * kMoveAtOnce) {
-        uint4 x[kMoveAtOnce];
-        uint4 *dst[kMoveAtOnce];
-#pragma unroll
-        for (uint32_t u = 0; u < kMoveAtOnce; ++u) {
-            const uint32_t piece = b + u * gridDim.x;
-            dst[u] = nullptr;
-            if (piece >= pieces) continue;
-            const uint32_t row = ((piece & ((1u << subs_log2) - 1u)) << 4) + (threadIdx.x >> 4);
-            uint32_t at = piece >> subs_log2;
-            const uint32_t h = at % a.c.kv_heads;
-            at /= a.c.kv_heads;
-            uint4 *pool = reinterpret_cast<uint4 *>(at & 1u ? a.c.v : a.c.k);
-            at >>= 1;
-            const uint32_t layer = at % a.c.layers, i = at / a.c.layers;
-            if (row >= __ldcg(rows + i)) continue;
-            auto place = [&](uint32_t page) {
-                return pool + ((((((uint64_t)layer * a.c.pages + page) * a.c.kv_heads + h) << a.c.page_log2) + row) * 16u + (threadIdx.x & 15u));
+    if (lane == 0u && copies) {
+        const uint32_t *from = array_of(a.c, kCopyFrom), *to = array_of(a.c, kCopyTo), *rows = array_of(a.c, kCopyRows);
+        const bool whole = moved_from != ~0u;
+        const uint32_t page = 1u << a.c.page_log2;
+        // runs of a page that lie together, and pieces of a run
+        const uint32_t runs = whole ? 1u : a.c.kv_heads, run_rows = whole ? a.c.kv_heads << a.c.page_log2 : page;
+        const uint32_t subs = (run_rows + kMoveRows - 1u) / kMoveRows, per_page = runs * subs;
+        const uint32_t pieces = copies * a.c.layers * 2u * per_page, step = gridDim.x * kMoveWarps;
+        struct Copy {
+            const uint8_t *src;
+            uint8_t *dst;
+            uint32_t bytes;
+        };
+        auto piece_of = [&](uint32_t x) {
+            Copy c;
+            const uint32_t at = x / per_page, in = x - at * per_page, run = in / subs, row = (in - run * subs) * kMoveRows;
+            const uint32_t layer2 = at % (2u * a.c.layers), i = at / (2u * a.c.layers);
+            uint8_t *pool = reinterpret_cast<uint8_t *>(layer2 & 1u ? a.c.v : a.c.k);
+            const uint32_t have = whole ? run_rows : __ldcg(rows + i);
+            auto place = [&](uint32_t p) {
+                return pool + (((((uint64_t)(layer2 >> 1) * a.c.pages + p) * a.c.kv_heads + run) << a.c.page_log2) + row) * kRowBytes;
             };
-            x[u] = __ldcs(place(__ldcg(from + i)));
-            dst[u] = place(__ldcg(to + i));
-        }
+            c.src = place(__ldcg(from + i));
+            c.dst = place(__ldcg(to + i));
+            c.bytes = row < have ? min(have - row, kMoveRows) * kRowBytes : 0u;
+            return c;
+        };
+        // the pieces x, x + step, ...: load number n into buffer n % kMoveStages, kMoveStages - 1 ahead of the stores
+        uint32_t x = blockIdx.x * kMoveWarps + warp, loaded = 0u, stored = 0u;
+        Copy c[kMoveStages];
+        bool ok = true;
+        auto load = [&](uint32_t slot) {
+            Copy &d = c[slot];
+            d.bytes = 0u;
+            while (x < pieces && !d.bytes) {
+                d = piece_of(x);
+                x += step;
+            }
+            if (!d.bytes) return false;
+            mbar_arrive_expect_tx(&sm.full[warp][slot], d.bytes);
+            bulk_g2s(sm.buffer[warp][slot], d.src, d.bytes, &sm.full[warp][slot]);
+            ++loaded;
+            return true;
+        };
+        bool more = true;
 #pragma unroll
-        for (uint32_t u = 0; u < kMoveAtOnce; ++u)
-            if (dst[u]) __stcs(dst[u], x[u]);
+        for (uint32_t i = 0; i + 1u < kMoveStages; ++i) more = more && load(i);
+        while (stored < loaded) {
+#pragma unroll
+            for (uint32_t slot = 0; slot < kMoveStages; ++slot) {
+                if (stored >= loaded) break;
+                ok = ok && mbar_wait(&sm.full[warp][slot], stored / kMoveStages & 1u, &sm.err);
+                if (ok) {
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(c[slot].dst), "r"(smem_addr(sm.buffer[warp][slot])),
+                                 "r"(c[slot].bytes)
+                                 : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                } else {   // a wait that ran out: by hand
+                    for (uint32_t b = 0; b < c[slot].bytes; b += 16u)
+                        *reinterpret_cast<uint4 *>(c[slot].dst + b) = __ldcg(reinterpret_cast<const uint4 *>(c[slot].src + b));
+                }
+                ++stored;
+                // the buffer before this one is free once its store has read it
+                asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                if (more) more = load((slot + kMoveStages - 1u) % kMoveStages);
+            }
+        }
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     if (moved_from == ~0u) return;
     const uint32_t *moved = array_of(a.c, (WorkArray)kMovedTo);
@@ -571,13 +629,16 @@ int done(const char *who, cudaError_t e)
 }
 
 // Carries out the plan of the launch before, which copies at most `copies` pages
-cudaError_t launch_move(const Cache &c, uint64_t copies, uint64_t entries, int sms, cudaStream_t stream)
+cudaError_t launch_move(const Cache &c, uint64_t copies, uint64_t entries, int dev, int sms, cudaStream_t stream)
 {
     MoveArgs a{};
     a.c = c;
-    const uint64_t pieces = copies * c.layers * 2 * c.kv_heads << (c.page_log2 - 4u);
-    const uint64_t ctas = std::max((pieces + kMoveAtOnce - 1) / kMoveAtOnce, (entries + kMoveThreads - 1) / kMoveThreads);
-    return launch(move_kernel, dim3((uint32_t)std::min<uint64_t>(ctas, (uint64_t)sms * 8)), kMoveThreads, 0, 1, a, sms, stream);
+    const cudaError_t e = k8::allow<move_kernel>(dev, (int)sizeof(MoveSmem));
+    if (e != cudaSuccess) return e;
+    const uint64_t pieces = copies * c.layers * 2 * (((uint64_t)c.kv_heads << c.page_log2) + kMoveRows - 1) / kMoveRows;
+    const uint64_t ctas = std::max((pieces + kMoveWarps - 1) / kMoveWarps, (entries + kMoveThreads - 1) / kMoveThreads);
+    return launch(move_kernel, dim3((uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(ctas, (uint64_t)sms))), kMoveThreads, sizeof(MoveSmem), 1, a, sms,
+                  stream);
 }
 
 }  // namespace
@@ -649,7 +710,7 @@ extern "C" int atlas_cuda_paged_reserve(const AtlasPaged *cache, uint32_t tokens
     const cudaError_t e = launch(reserve_kernel, dim3(1), kPlanThreads, sizeof(Entries), 1, a, sms, (cudaStream_t)stream);
     if (e != cudaSuccess) return done(who, e);
     // a sequence's first page at most is copied
-    return done(who, launch_move(a.c, std::min(cache->nseq, cache->pages), 0, sms, (cudaStream_t)stream));
+    return done(who, launch_move(a.c, std::min(cache->nseq, cache->pages), 0, dev, sms, (cudaStream_t)stream));
 }
 
 extern "C" int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_used, void *stream)
@@ -662,7 +723,7 @@ extern "C" int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_use
     a.out = d_used;
     const cudaError_t e = launch(compact_kernel, dim3(1), kPlanThreads, 0, 1, a, sms, (cudaStream_t)stream);
     if (e != cudaSuccess) return done(who, e);
-    return done(who, launch_move(a.c, cache->pages / 2u, (uint64_t)cache->nseq * cache->max_pages, sms, (cudaStream_t)stream));
+    return done(who, launch_move(a.c, cache->pages / 2u, (uint64_t)cache->nseq * cache->max_pages, dev, sms, (cudaStream_t)stream));
 }
 
 namespace {

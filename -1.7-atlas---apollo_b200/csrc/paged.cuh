@@ -61,33 +61,24 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t x)
     return ((x & e) == e ? 0xffffu : 0u) | ((x >> 16 & e) == e ? 0xffff0000u : 0u);
 }
 
-// A sequence as its units see it: tiles of keys [k0, ..), k0 behind the pages that are gone at its start
-struct Seq {
-    uint64_t p0;
-    uint32_t rows, k0;
-};
-
-// The sequence's first tile of keys that has a page, or behind: its leading entries that name none are passed over, 128 at
-// a time. The whole warp.
-__device__ __forceinline__ uint32_t first_page(const Cache &c, uint32_t s, uint32_t pages)
+// Dividing 64-bit numbers that mostly have 32 bits
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
 {
-    const int32_t *row = c.table + (size_t)s * c.max_pages;
-    const uint32_t lane = threadIdx.x & 31u;
-    if (!pages || (uint32_t)__ldcg(row) < c.pages) return 0u;
-    for (uint32_t b = 0; b < pages; b += 128u) {
-        uint32_t x[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) x[i] = b + 32u * i + lane < pages ? (uint32_t)__ldcg(row + b + 32u * i + lane) : ~0u;
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            const uint32_t have = __ballot_sync(0xffffffffu, x[i] < c.pages);
-            if (have) return b + 32u * i + (uint32_t)__ffs((int)have) - 1u;
-        }
-    }
-    return pages;
+    return ((a | b) >> 32) == 0u ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-// How a call's rows are cut into tiles: `tile` rows each, those of whole tokens where `tokens` is not 0
+// A sequence as its units see it: tiles of keys [k0, ..), k0 behind the pages that are gone at its start
+struct Seq {
+    uint32_t p0, rows, k0;
+};
+
+// What a CTA keeps of its call's sequences, where they are few: a lane each
+constexpr uint32_t kKeptSeqs = 32;
+struct Kept {
+    Seq seq[kKeptSeqs];
+};
+
+// How a call's rows are cut into tiles of `tile` rows
 template <uint32_t KEYS>
 struct Cut {
     const AttnArgs &a;
@@ -96,7 +87,7 @@ struct Cut {
     // the tiles of keys that rows before `row1` see, from the front
     __device__ __forceinline__ uint32_t keys(const Seq &q, uint32_t row1) const
     {
-        const uint64_t last = min(q.p0 + (row1 - 1u) / a.group + 1u, (uint64_t)a.c.limit);
+        const uint64_t last = min((uint64_t)q.p0 + (row1 - 1u) / a.group + 1u, (uint64_t)a.c.limit);
         return (uint32_t)((last + KEYS - 1u) / KEYS);
     }
     __device__ __forceinline__ uint32_t units(const Seq &q) const { return (q.rows + tile - 1u) / tile; }
@@ -109,16 +100,31 @@ struct Cut {
     // the whole warp
     __device__ __forceinline__ Seq open(uint32_t s) const
     {
+        const int32_t *entries = a.c.table + (size_t)s * a.c.max_pages;
+        const uint32_t lane = threadIdx.x & 31u, e0 = (uint32_t)__ldcg(entries);
         Seq q;
         q.p0 = __ldcg(a.r.pos0 + s);
         q.rows = row_count(a.r, s) * a.group;
         q.k0 = 0u;
-        if (q.rows) {
-            const uint32_t seen = (uint32_t)min(q.p0 + (q.rows - 1u) / a.group + 1u, (uint64_t)a.c.limit);
-            q.k0 = (uint32_t)(((uint64_t)first_page(a.c, s, (seen + (1u << a.c.page_log2) - 1u) >> a.c.page_log2) << a.c.page_log2) / KEYS);
+        if (!q.rows || e0 < a.c.pages) return q;
+        // its leading entries that name no page are passed over, 128 at a time
+        const uint32_t seen = (uint32_t)min((uint64_t)q.p0 + (q.rows - 1u) / a.group + 1u, (uint64_t)a.c.limit);
+        const uint32_t pages = (seen + (1u << a.c.page_log2) - 1u) >> a.c.page_log2;
+        uint32_t page = pages;
+        for (uint32_t b = 0; b < pages && page == pages; b += 128u) {
+            uint32_t x[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) x[i] = b + 32u * i + lane < pages ? (uint32_t)__ldcg(entries + b + 32u * i + lane) : ~0u;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) {
+                const uint32_t have = __ballot_sync(0xffffffffu, x[i] < a.c.pages);
+                if (have && page == pages) page = b + 32u * i + (uint32_t)__ffs((int)have) - 1u;
+            }
         }
+        q.k0 = (uint32_t)(((uint64_t)page << a.c.page_log2) / KEYS);
         return q;
     }
+    __device__ __forceinline__ Seq open(uint32_t s, const Kept &kept) const { return a.c.nseq <= kKeptSeqs ? kept.seq[s] : open(s); }
 };
 
 // The piece of a CTA: it begins in unit (s, h, i), `skip` tiles of keys behind the unit's first one, and has `left` of them
@@ -129,73 +135,145 @@ struct Piece {
 };
 
 struct PieceSmem {
-    uint64_t before[kMaxSeqs + 1];        // the line's length before each sequence
+    uint64_t work[kMaxSeqs + 1];          // a sequence's tiles of keys; then those of the sequences up to it
+    uint32_t units[kMaxSeqs + 1];         // its units, likewise
+    uint32_t most[32];                    // the largest unit that a warp has seen
+    uint32_t all_units;
 };
 
-// This CTA's piece. All WARPS warps; `sm` may be used for something else after the next barrier. `least`: tiles of keys
-// that a CTA takes at least.
+__device__ __forceinline__ uint64_t up_to(uint64_t x)   // the sum of the lanes' x up to this one
+{
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if ((threadIdx.x & 31u) >= (uint32_t)o) x += y;
+    }
+    return x;
+}
+__device__ __forceinline__ uint32_t up_to(uint32_t x)
+{
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if ((threadIdx.x & 31u) >= (uint32_t)o) x += y;
+    }
+    return x;
+}
+
+// This CTA's piece. All WARPS warps; `sm` may be used for something else after the next barrier. Where there are no more units
+// than CTAs, and the largest is at most `worth` longer than an equal share, each unit is a piece (joining partial sums
+// takes as long as `worth` tiles of keys); else a CTA takes `least` tiles of keys at least.
 template <uint32_t KEYS, uint32_t WARPS>
-__device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, uint32_t least)
+__device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, Kept &kept, uint32_t least, uint32_t worth)
 {
     const AttnArgs &a = cut.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = a.c.nseq;
+    uint32_t most = 0u;
     for (uint32_t s = warp; s < n; s += WARPS) {
         const Seq q = cut.open(s);
         uint64_t sum = 0u;
         const uint32_t units = q.rows ? cut.units(q) : 0u;
-        for (uint32_t i = lane; i < units; i += 32u) sum += cut.cost(q, i);
+        for (uint32_t i = lane; i < units; i += 32u) {
+            const uint32_t c = cut.cost(q, i);
+            sum += c;
+            most = max(most, c);
+        }
+        if (units == 1u) sum = __shfl_sync(0xffffffffu, (uint32_t)sum, 0);
+        else
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0u) sm.before[s + 1u] = sum * a.c.kv_heads;
-    }
-    if (threadIdx.x == 0u) sm.before[0] = 0u;
-    __syncthreads();
-    if (warp == 0u) {
-        uint64_t done = 0u;
-        for (uint32_t b = 1u; b <= n; b += 32u) {
-            uint64_t x = b + lane <= n ? sm.before[b + lane] : 0u;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t up = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= (uint32_t)o) x += up;
-            }
-            if (b + lane <= n) sm.before[b + lane] = done + x;
-            done += __shfl_sync(0xffffffffu, x, 31);
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0u) {
+            sm.work[s] = sum;
+            sm.units[s] = units;
+            if (s < kKeptSeqs) kept.seq[s] = q;
         }
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0u) sm.most[warp] = most;
     __syncthreads();
-    Piece p;
-    const uint64_t total = sm.before[n];
-    p.each = max((total + gridDim.x - 1u) / gridDim.x, (uint64_t)least);
-    p.begin = p.each * blockIdx.x;
-    p.left = p.begin < total ? min(p.each, total - p.begin) : 0u;
-    p.s = p.h = p.i = p.skip = 0u;
-    if (!p.left) return p;
-    uint32_t lo = 0u, hi = n;             // before[lo] <= begin < before[hi]
-    while (hi - lo > 1u) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (sm.before[mid] <= p.begin) lo = mid;
-        else hi = mid;
+    most = __reduce_max_sync(0xffffffffu, lane < WARPS ? sm.most[lane] : 0u);
+    // the line's length before each sequence: by every warp for itself, or by the first one for all
+    uint64_t total = 0u;
+    uint32_t all_units = 0u;
+    uint64_t mine = 0u;                   // few sequences: lane s has those up to s
+    uint32_t mine_units = 0u;
+    if (n <= kKeptSeqs) {
+        mine = up_to(lane < n ? sm.work[lane] * a.c.kv_heads : 0u);
+        mine_units = up_to(lane < n ? sm.units[lane] * a.c.kv_heads : 0u);
+        total = __shfl_sync(0xffffffffu, mine, 31);
+        all_units = __shfl_sync(0xffffffffu, mine_units, 31);
+    } else {
+        if (warp == 0u) {
+            uint64_t work = 0u, units = 0u;
+            for (uint32_t b = 0u; b < n; b += 32u) {
+                const uint64_t w = up_to(b + lane < n ? sm.work[b + lane] * a.c.kv_heads : 0u), u = up_to((uint64_t)(b + lane < n ? sm.units[b + lane] : 0u) * a.c.kv_heads);
+                if (b + lane < n) {
+                    sm.work[b + lane] = work + w;
+                    sm.units[b + lane] = (uint32_t)(units + u);
+                }
+                work += __shfl_sync(0xffffffffu, w, 31);
+                units += __shfl_sync(0xffffffffu, u, 31);
+            }
+            if (lane == 0u) sm.all_units = units >> 32 ? ~0u : (uint32_t)units;
+        }
+        __syncthreads();
+        total = sm.work[n - 1u];
+        all_units = sm.all_units;
     }
-    p.s = lo;
-    const Seq q = cut.open(lo);
-    const uint64_t of_head = (sm.before[lo + 1u] - sm.before[lo]) / a.c.kv_heads, in = p.begin - sm.before[lo];
-    p.h = (uint32_t)(in / of_head);
-    uint64_t rest = in - of_head * p.h;
+    Piece p;
+    p.s = p.h = p.i = p.skip = 0u;
+    p.begin = 0u;
+    p.left = 0u;
+    p.each = quotient(total + gridDim.x - 1u, gridDim.x);
+    // the sequence that place `at` is in, by the sums up to each one, and the sum before it
+    auto find = [&](auto at, auto up, const auto *sums, auto &before) {
+        uint32_t s;
+        if (n <= kKeptSeqs) {
+            s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, up > at)) - 1u;
+            before = __shfl_sync(0xffffffffu, up, s ? (int)s - 1 : 0);
+        } else {
+            uint32_t lo = 0u, hi = n - 1u;   // sums[hi] > at
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (sums[mid] > at) hi = mid;
+                else lo = mid + 1u;
+            }
+            s = lo;
+            before = s ? sums[s - 1u] : 0u;
+        }
+        if (s == 0u) before = 0u;
+        return s;
+    };
+    if (all_units <= gridDim.x && most <= p.each + worth) {
+        if (blockIdx.x >= all_units) return p;
+        uint32_t before;
+        p.s = find(blockIdx.x, mine_units, sm.units, before);
+        const Seq q = cut.open(p.s, kept);
+        const uint32_t units = cut.units(q);
+        p.h = (blockIdx.x - before) / units;
+        p.i = blockIdx.x - before - p.h * units;
+        p.left = cut.cost(q, p.i);
+        return p;
+    }
+    p.each = max(p.each, (uint64_t)least);
+    p.begin = p.each * blockIdx.x;
+    if (p.begin >= total) return p;
+    p.left = min(p.each, total - p.begin);
+    uint64_t before;
+    p.s = find(p.begin, mine, sm.work, before);
+    const Seq q = cut.open(p.s, kept);
+    const uint64_t of_head = n <= kKeptSeqs ? sm.work[p.s] : quotient(sm.work[p.s] - before, a.c.kv_heads);
+    p.h = (uint32_t)quotient(p.begin - before, of_head);
+    uint64_t rest = p.begin - before - of_head * p.h;
     const uint32_t units = cut.units(q);
     for (uint32_t b = 0;; b += 32u) {     // the unit that holds place `rest`
-        const uint32_t mine = b + lane < units ? cut.cost(q, b + lane) : 0u;
-        uint64_t x = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t up = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= (uint32_t)o) x += up;
-        }
+        const uint32_t c = b + lane < units ? cut.cost(q, b + lane) : 0u;
+        const uint64_t x = up_to((uint64_t)c);
         const uint32_t past = __ballot_sync(0xffffffffu, x > rest);
         if (past || b + 32u >= units) {
             const uint32_t at = past ? (uint32_t)__ffs((int)past) - 1u : 31u;
             p.i = min(b + at, units - 1u);
-            p.skip = (uint32_t)(rest - __shfl_sync(0xffffffffu, x - mine, (int)at));
+            p.skip = (uint32_t)(rest - __shfl_sync(0xffffffffu, x - c, (int)at));
             return p;
         }
         rest -= __shfl_sync(0xffffffffu, x, 31);
@@ -206,6 +284,7 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
 template <uint32_t KEYS, uint32_t MOST = 0x7fffffffu>
 struct Walk {
     const Cut<KEYS> &cut;
+    const Kept &kept;
     Piece p;
     Seq q;
     uint32_t k_begin, k_end;              // the step's tiles of keys of the current unit
@@ -213,10 +292,10 @@ struct Walk {
     bool first;                           // it is the piece's first unit
     bool again;                           // there were steps of the unit before in this piece
 
-    __device__ __forceinline__ Walk(const Cut<KEYS> &cut_, const Piece &p_) : cut(cut_), p(p_), first(true), again(false)
+    __device__ __forceinline__ Walk(const Cut<KEYS> &cut_, const Piece &p_, const Kept &kept_) : cut(cut_), kept(kept_), p(p_), first(true), again(false)
     {
         if (p.left) {
-            q = cut.open(p.s);
+            q = cut.open(p.s, kept);
             set();
         }
     }
@@ -248,7 +327,7 @@ struct Walk {
             p.i = 0u;
             if (++p.h >= cut.a.c.kv_heads) {
                 p.h = 0u;
-                do q = cut.open(++p.s);
+                do q = cut.open(++p.s, kept);
                 while (!q.rows);          // there is more, so a sequence with rows comes
             }
         }
@@ -265,7 +344,7 @@ struct Walk {
         r.first = ~0u;
         if (p.left && !head && cut.cost(q, p.i) - p.skip <= p.left) {
             const uint64_t unit = p.begin - p.skip;
-            const uint32_t c = (uint32_t)(unit / p.each);
+            const uint32_t c = (uint32_t)quotient(unit, p.each);
             r.first = 2u * c + (unit == p.each * c ? 0u : 1u);
             r.count = blockIdx.x - c + 1u;
             r.s = p.s;
@@ -288,6 +367,12 @@ __device__ __forceinline__ void store4(const AttnArgs &a, uint32_t s, uint32_t h
 {
     reinterpret_cast<uint2 *>(a.out + ((size_t)s * a.r.tokens + at.x) * a.ldo + (size_t)(h * a.group + at.y) * kDim)[d4] =
         make_uint2(pack<BF>(x.x, x.y), pack<BF>(x.z, x.w));
+}
+
+// Whatever the positions, each unit will be a piece of its own (find_piece): a sequence has room for no more
+inline bool always_whole(const AttnArgs &a, uint64_t units, uint32_t ctas, uint32_t keys, uint32_t worth)
+{
+    return units <= ctas && (a.c.limit + keys - 1u) / keys <= worth;
 }
 
 }  // namespace

@@ -40,6 +40,7 @@ namespace {
 constexpr uint32_t kChunk = 16, kWarps = 8, kThreads = kWarps * 32, kStages = 3;
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
+constexpr uint32_t kWorth = 64;               // chunks: what joining partial sums takes
 constexpr float kLazy = 6.0f;
 // Weights are 2^(score - maximum + kUnit). binary16: their largest, 2^15, keeps the low term's bits; bfloat16 has fp32's
 // range, and small weights leave the sums of large values room
@@ -59,6 +60,7 @@ struct alignas(1024) Smem {
     } u;
     uint64_t full[kWarps][kStages];
     uint32_t err;
+    Kept kept;
     float2 wml[kWarps][8 * NT];
 };
 
@@ -130,8 +132,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     __syncthreads();
     wait_predecessor(a.early);
     const Cut<kChunk> cut{a, R};
-    const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, kWarps);
-    Walk<kChunk> w(cut, piece);
+    const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, sm.kept, kWarps, kWorth);
+    Walk<kChunk> w(cut, piece, sm.kept);
     if (threadIdx.x == 0u) reinterpret_cast<Part *>(a.parts)[blockIdx.x] = w.part();
     if (!w.more()) return;
     fence_ring();
@@ -401,15 +403,16 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 
 // --------------------------------------------------------- partial sums ----
 //
-// The units that pieces cut: the CTA whose number is that of the piece that a
-// unit ends in joins its records, a warp per row (lane: a record's maximum and
-// sum, then 4 dimensions). Bound by latency: a call whose pieces are whole units
+// The units that pieces cut: the CTAs whose number is that of the piece that a
+// unit ends in join its records, two rows a warp (lane: a record's maximum and
+// sum, then 4 dimensions), with the first records' loads on their way before
+// their weights are known. Bound by latency; a call whose pieces are whole units
 // leaves nothing to join.
 struct MergeArgs : AttnArgs {
-    uint32_t tile, per;                   // rows of a record; of rows that a CTA takes
+    uint32_t tile;                        // rows of a record
 };
 
-constexpr uint32_t kMergeWarps = 8;
+constexpr uint32_t kMergeWarps = 8, kMergeRows = 2, kAhead = 4;
 
 template <bool BF>
 __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __grid_constant__ MergeArgs a)
@@ -418,40 +421,68 @@ __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __gr
     wait_predecessor(a.early);
     const uint4 lo = __ldcg(reinterpret_cast<const uint4 *>(a.parts) + 2u * blockIdx.x), hi = __ldcg(reinterpret_cast<const uint4 *>(a.parts) + 2u * blockIdx.x + 1u);
     const uint32_t first = lo.x, count = lo.y, s = lo.z, h = lo.w, row0 = hi.x, rows = hi.y;
-    if (first == ~0u) return;
+    const uint32_t r0 = (blockIdx.y * kMergeWarps + warp) * kMergeRows;
+    if (first == ~0u || r0 >= rows) return;
     // record i of the unit
     auto record = [&](uint32_t i) { return record_of(a, i ? 2u * (first / 2u + i) : first, a.tile); };
-    for (uint32_t r = blockIdx.y * a.per + warp; r < min(rows, (blockIdx.y + 1u) * a.per); r += kMergeWarps) {
-        float M = -INFINITY, L = 0.f;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t b = 0; b < count; b += 32u) {
-            const float2 ml = b + lane < count ? __ldcg(reinterpret_cast<const float2 *>(record(b + lane) + a.tile * kDim) + r) : make_float2(-INFINITY, 0.f);
-            float most = ml.x;
+    float M[kMergeRows], L[kMergeRows], f[kMergeRows];   // f: record b + lane's factor
+    float4 x[kMergeRows], y[kMergeRows][kAhead];
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t u = 0; u < kMergeRows; ++u)
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i)
+                if (i0 + i < count) y[u][i] = __ldcg(reinterpret_cast<const float4 *>(record(i0 + i)) + min(r0 + u, rows - 1u) * (kDim / 4u) + lane);
+    };
+    load(0u);
+#pragma unroll
+    for (uint32_t u = 0; u < kMergeRows; ++u) {
+        M[u] = -INFINITY;
+        L[u] = 0.f;
+        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (uint32_t b = 0; b < count; b += 32u) {
+        float2 ml[kMergeRows];
+#pragma unroll
+        for (uint32_t u = 0; u < kMergeRows; ++u)
+            ml[u] = b + lane < count ? __ldcg(reinterpret_cast<const float2 *>(record(b + lane) + a.tile * kDim) + min(r0 + u, rows - 1u)) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (uint32_t u = 0; u < kMergeRows; ++u) {
+            float most = ml[u].x;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            most = fmaxf(most, M);
-            const float before = M == -INFINITY ? (L == 0.f ? 0.f : 1.f) : ex2(M - most);
-            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - most);
-            float sum = f * ml.y;
+            most = fmaxf(most, M[u]);
+            const float before = M[u] == -INFINITY ? (L[u] == 0.f ? 0.f : 1.f) : ex2(M[u] - most);
+            f[u] = ml[u].x == -INFINITY ? (ml[u].y == 0.f ? 0.f : 1.f) : ex2(ml[u].x - most);
+            float sum = f[u] * ml[u].y;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            M = most;
-            L = fmaf(before, L, sum);
-            x = make_float4(x.x * before, x.y * before, x.z * before, x.w * before);
-            const uint32_t n = min(count - b, 32u);
-#pragma unroll 4
-            for (uint32_t i = 0; i < n; ++i) {
-                const float4 y = __ldcg(reinterpret_cast<const float4 *>(record(b + i)) + r * (kDim / 4u) + lane);
-                const float fi = __shfl_sync(0xffffffffu, f, (int)i);
-                x.x = fmaf(fi, y.x, x.x);
-                x.y = fmaf(fi, y.y, x.y);
-                x.z = fmaf(fi, y.z, x.z);
-                x.w = fmaf(fi, y.w, x.w);
-            }
+            M[u] = most;
+            L[u] = fmaf(before, L[u], sum);
+            x[u] = make_float4(x[u].x * before, x[u].y * before, x[u].z * before, x[u].w * before);
         }
-        const float inv = L == 0.f ? 0.f : 1.0f / L;
-        const uint32_t row = row0 + r, tok = row / a.group;
-        store4<BF>(a, s, h, make_uint2(tok, row - tok * a.group), lane, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        const uint32_t n = min(count - b, 32u);
+        for (uint32_t i0 = 0; i0 < n; i0 += kAhead) {
+#pragma unroll
+            for (uint32_t u = 0; u < kMergeRows; ++u)
+#pragma unroll
+                for (uint32_t i = 0; i < kAhead; ++i) {
+                    const float fi = __shfl_sync(0xffffffffu, f[u], (int)(i0 + i));
+                    if (i0 + i >= n) continue;
+                    x[u].x = fmaf(fi, y[u][i].x, x[u].x);
+                    x[u].y = fmaf(fi, y[u][i].y, x[u].y);
+                    x[u].z = fmaf(fi, y[u][i].z, x[u].z);
+                    x[u].w = fmaf(fi, y[u][i].w, x[u].w);
+                }
+            load(b + i0 + kAhead);
+        }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kMergeRows; ++u) {
+        if (r0 + u >= rows) break;
+        const float inv = L[u] == 0.f ? 0.f : 1.0f / L[u];
+        const uint32_t row = row0 + r0 + u, tok = row / a.group;
+        store4<BF>(a, s, h, make_uint2(tok, row - tok * a.group), lane, make_float4(x[u].x * inv, x[u].y * inv, x[u].z * inv, x[u].w * inv));
     }
 }
 
@@ -470,8 +501,7 @@ cudaError_t launch_merge(const AttnArgs &a, bool bf, uint32_t rows, uint32_t cta
     MergeArgs m{};
     static_cast<AttnArgs &>(m) = a;
     m.tile = rows;
-    m.per = std::min(rows, 32u);
-    const dim3 grid(ctas, (rows + m.per - 1) / m.per);
+    const dim3 grid(ctas, (rows + kMergeWarps * kMergeRows - 1) / (kMergeWarps * kMergeRows));
     return bf ? k8::launch(part_merge_kernel<true>, grid, kMergeWarps * 32, 0, 1, m, sms, stream)
               : k8::launch(part_merge_kernel<false>, grid, kMergeWarps * 32, 0, 1, m, sms, stream);
 }
@@ -488,7 +518,10 @@ cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtenso
                     : nt == 2 ? (bf ? launch_few_of<true, 2>(f, dev, sms, stream) : launch_few_of<false, 2>(f, dev, sms, stream))
                               : (bf ? launch_few_of<true, 4>(f, dev, sms, stream) : launch_few_of<false, 4>(f, dev, sms, stream));
     if (e != cudaSuccess) return e;
-    return launch_merge(a, bf, 8u * (uint32_t)nt, std::min((uint32_t)sms, kMaxCtas), sms, stream);
+    const uint32_t rows = 8u * (uint32_t)nt, ctas = std::min((uint32_t)sms, kMaxCtas);
+    const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * (((uint64_t)a.r.tokens * a.group + rows - 1) / rows);
+    if (always_whole(a, units, ctas, kChunk, kWorth)) return cudaSuccess;
+    return launch_merge(a, bf, rows, ctas, sms, stream);
 }
 
 }  // namespace paged

@@ -60,6 +60,7 @@ static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "what the softma
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 values, swizzled
 constexpr uint32_t kTile = 2 * kHalf;
 constexpr uint32_t kMaxStages = 6;
+constexpr uint32_t kWorth = 4;                     // tiles of keys: what joining partial sums takes
 constexpr float kLazy = 8.0f;
 // Weights are 2^(score - maximum + kUnit): binary16 keeps 24 bits below the largest; bfloat16 has fp32's range, and small
 // weights leave the sums of large values room
@@ -76,6 +77,7 @@ struct PromptArgs : AttnArgs {
 struct Bars {
     uint64_t s_full[2], p_full[2][2], o_full[2], o_free[2], full[kMaxStages], free[kMaxStages], checked[kMaxStages], q_full, q_free, fin;
     uint32_t tmem, status;
+    Kept kept;
     uint32_t bad[4];                               // the step in which a value was taken out, at its number % 4
     float2 state[2][kTileRows];                    // one tile of rows: the groups' maxima and sums
 };
@@ -166,13 +168,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     wait_predecessor(a.early);
     const uint32_t tile_rows = a.tokens_per_tile * a.group;      // of 128 in tensor memory
     const Cut<kTileKeys> cut{a, (ONE ? 1u : 2u) * tile_rows};
-    const Piece piece = find_piece<kTileKeys, kThreads / 32u>(cut, *reinterpret_cast<PieceSmem *>(kv), 2u);
+    const Piece piece = find_piece<kTileKeys, kThreads / 32u>(cut, *reinterpret_cast<PieceSmem *>(kv), b.kept, 2u, kWorth);
     fence_before();
     fence_async();
     __syncthreads();
     fence_after();
     const uint32_t tmem = b.tmem;   // scores / weights of group t: column 128 t; output: 256 + 128 t
-    Walk<kTileKeys, kMostTiles> w(cut, piece);
+    Walk<kTileKeys, kMostTiles> w(cut, piece, b.kept);
 
     // The end of a CTA, for every warp in the branch of its registers
     auto leave = [&]() {
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const uint32_t nowhere = (a.c.layers * a.c.pages * a.c.kv_heads) << page_log2;   // behind the pool's end: zeros
         for (; ok && w.more(); w.next(), ++steps) {
             const uint32_t s = w.p.s, h = w.p.h, row0 = w.row0(), rows = w.rows(), tiles = tiles_of(rows);
-            const uint32_t seen = (uint32_t)min(w.q.p0 + (row0 + rows - 1u) / a.group + 1u, (uint64_t)a.c.limit);
+            const uint32_t seen = (uint32_t)min((uint64_t)w.q.p0 + (row0 + rows - 1u) / a.group + 1u, (uint64_t)a.c.limit);
             const int32_t *const entries = a.c.table + (size_t)s * a.c.max_pages;
             // where this lane's page of tile j begins
             auto page_row = [&](uint32_t j) {
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const uint64_t qd = operand(smem_addr(qs)), kd = operand(smem_addr(kv)), vd = operand_across(smem_addr(kv), kHalf);
         for (; ok && w.more(); w.next(), ++steps) {
             const uint32_t tiles = tiles_of(w.rows()), n = w.k_end - w.k_begin;
-            const uint64_t open = w.q.p0 + w.row0() / a.group;   // every row sees the positions up to it
+            const uint64_t open = (uint64_t)w.q.p0 + w.row0() / a.group;   // every row sees the positions up to it
             if (leader) {
                 ok = mbar_wait(&b.q_full, steps & 1u, err);
                 // scores of the keys in ring slot `slot` by tile of rows qt, into group t's columns
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         bool ok = true;
         for (; ok && w.more(); w.next(), ++steps) {
             const uint32_t n = w.k_end - w.k_begin;
-            const uint64_t open = w.q.p0 + w.row0() / a.group;
+            const uint64_t open = (uint64_t)w.q.p0 + w.row0() / a.group;
             auto pass = [&]() {
                 ok = ok && wait_warp(&b.full[ring.slot], ring.phase, err);
                 ring.next();
@@ -697,7 +699,10 @@ cudaError_t launch_prompt(const AttnArgs &a, const CUtensorMap &kmap, const CUte
     const cudaError_t e = tiles == 1 ? (bf ? launch_prompt_of<true, true>(p, dev, sms, stream) : launch_prompt_of<false, true>(p, dev, sms, stream))
                                      : (bf ? launch_prompt_of<true, false>(p, dev, sms, stream) : launch_prompt_of<false, false>(p, dev, sms, stream));
     if (e != cudaSuccess) return e;
-    return launch_merge(a, bf, tiles * kTileRows, std::min((uint32_t)sms, kMaxCtas), sms, stream);
+    const uint32_t ctas = std::min((uint32_t)sms, kMaxCtas), per = tiles * p.tokens_per_tile;
+    const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * ((a.r.tokens + per - 1) / per);
+    if (always_whole(a, units, ctas, kTileKeys, kWorth)) return cudaSuccess;
+    return launch_merge(a, bf, tiles * kTileRows, ctas, sms, stream);
 }
 
 }  // namespace paged
