@@ -792,6 +792,7 @@ extern "C" int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, ui
     a.ldo = ldo;
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
+    a.by_group = divisor(a.group);
     a.layer = layer;
     a.parts = reinterpret_cast<float *>(static_cast<char *>(cache->work) + parts_offset(cache->pages));
     const bool bf = cache->type == ATLAS_PAGED_BF16;

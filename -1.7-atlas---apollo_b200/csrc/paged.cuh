@@ -72,11 +72,8 @@ struct Seq {
     uint32_t p0, rows, k0;
 };
 
-// What a CTA keeps of its call's sequences, where they are few: a lane each
+// Up to this many sequences, each lane of a warp keeps one's Seq
 constexpr uint32_t kKeptSeqs = 32;
-struct Kept {
-    Seq seq[kKeptSeqs];
-};
 
 // How a call's rows are cut into tiles of `tile` rows
 template <uint32_t KEYS>
@@ -87,7 +84,7 @@ struct Cut {
     // the tiles of keys that rows before `row1` see, from the front
     __device__ __forceinline__ uint32_t keys(const Seq &q, uint32_t row1) const
     {
-        const uint64_t last = min((uint64_t)q.p0 + (row1 - 1u) / a.group + 1u, (uint64_t)a.c.limit);
+        const uint64_t last = min((uint64_t)q.p0 + divide(row1 - 1u, a.by_group) + 1u, (uint64_t)a.c.limit);
         return (uint32_t)((last + KEYS - 1u) / KEYS);
     }
     __device__ __forceinline__ uint32_t units(const Seq &q) const { return (q.rows + tile - 1u) / tile; }
@@ -97,18 +94,13 @@ struct Cut {
         const uint32_t k = keys(q, min((i + 1u) * tile, q.rows));
         return k > q.k0 ? k - q.k0 : 1u;
     }
-    // the whole warp
-    __device__ __forceinline__ Seq open(uint32_t s) const
+    // The first tile of keys behind the pages that are gone at a sequence's start: its leading entries that name none are
+    // passed over, 128 at a time. The whole warp.
+    __device__ __forceinline__ uint32_t begin(uint32_t s, uint32_t p0, uint32_t rows) const
     {
         const int32_t *entries = a.c.table + (size_t)s * a.c.max_pages;
-        const uint32_t lane = threadIdx.x & 31u, e0 = (uint32_t)__ldcg(entries);
-        Seq q;
-        q.p0 = __ldcg(a.r.pos0 + s);
-        q.rows = row_count(a.r, s) * a.group;
-        q.k0 = 0u;
-        if (!q.rows || e0 < a.c.pages) return q;
-        // its leading entries that name no page are passed over, 128 at a time
-        const uint32_t seen = (uint32_t)min((uint64_t)q.p0 + (q.rows - 1u) / a.group + 1u, (uint64_t)a.c.limit);
+        const uint32_t lane = threadIdx.x & 31u;
+        const uint32_t seen = (uint32_t)min((uint64_t)p0 + divide(rows - 1u, a.by_group) + 1u, (uint64_t)a.c.limit);
         const uint32_t pages = (seen + (1u << a.c.page_log2) - 1u) >> a.c.page_log2;
         uint32_t page = pages;
         for (uint32_t b = 0; b < pages && page == pages; b += 128u) {
@@ -121,10 +113,44 @@ struct Cut {
                 if (have && page == pages) page = b + 32u * i + (uint32_t)__ffs((int)have) - 1u;
             }
         }
-        q.k0 = (uint32_t)(((uint64_t)page << a.c.page_log2) / KEYS);
+        return (uint32_t)(((uint64_t)page << a.c.page_log2) / KEYS);
+    }
+    // the whole warp
+    __device__ __forceinline__ Seq open(uint32_t s) const
+    {
+        const uint32_t e0 = (uint32_t)__ldcg(a.c.table + (size_t)s * a.c.max_pages);
+        Seq q;
+        q.p0 = __ldcg(a.r.pos0 + s);
+        q.rows = row_count(a.r, s) * a.group;
+        q.k0 = q.rows && e0 >= a.c.pages ? begin(s, q.p0, q.rows) : 0u;
         return q;
     }
-    __device__ __forceinline__ Seq open(uint32_t s, const Kept &kept) const { return a.c.nseq <= kKeptSeqs ? kept.seq[s] : open(s); }
+    // `kept`: this lane's, where there are no more than kKeptSeqs
+    __device__ __forceinline__ Seq open(uint32_t s, const Seq &kept) const
+    {
+        if (a.c.nseq > kKeptSeqs) return open(s);
+        Seq q;
+        q.p0 = __shfl_sync(0xffffffffu, kept.p0, (int)s);
+        q.rows = __shfl_sync(0xffffffffu, kept.rows, (int)s);
+        q.k0 = __shfl_sync(0xffffffffu, kept.k0, (int)s);
+        return q;
+    }
+    // a sequence's work, and its largest unit's; the whole warp
+    __device__ __forceinline__ uint64_t all(const Seq &q, uint32_t &most) const
+    {
+        const uint32_t lane = threadIdx.x & 31u, n = q.rows ? units(q) : 0u;
+        uint64_t sum = 0u;
+        uint32_t m = 0u;
+        for (uint32_t i = lane; i < n; i += 32u) {
+            const uint32_t c = cost(q, i);
+            sum += c;
+            m = max(m, c);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        most = max(most, __reduce_max_sync(0xffffffffu, m));
+        return sum;
+    }
 };
 
 // The piece of a CTA: it begins in unit (s, h, i), `skip` tiles of keys behind the unit's first one, and has `left` of them
@@ -132,6 +158,7 @@ struct Piece {
     uint64_t begin, each; // in the line of all; a CTA's share
     uint32_t s, h, i, skip;
     uint64_t left;
+    Seq kept;             // lane s has sequence s, where there are no more than kKeptSeqs
 };
 
 struct PieceSmem {
@@ -160,49 +187,64 @@ __device__ __forceinline__ uint32_t up_to(uint32_t x)
     return x;
 }
 
-// This CTA's piece. All WARPS warps; `sm` may be used for something else after the next barrier. Where there are no more units
-// than CTAs, and the largest is at most `worth` longer than an equal share, each unit is a piece (joining partial sums
-// takes as long as `worth` tiles of keys); else a CTA takes `least` tiles of keys at least.
+// This CTA's piece. All WARPS warps, each for itself where each lane can keep a sequence, else together through `sm`, which is
+// free again behind the call. Where there are no more units than CTAs, and the largest is at most `worth` longer than an
+// equal share, each unit is a piece (joining partial sums takes as long as `worth` tiles of keys); else a CTA takes
+// `least` tiles of keys at least.
 template <uint32_t KEYS, uint32_t WARPS>
-__device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, Kept &kept, uint32_t least, uint32_t worth)
+__device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, uint32_t least, uint32_t worth)
 {
     const AttnArgs &a = cut.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = a.c.nseq;
-    uint32_t most = 0u;
-    for (uint32_t s = warp; s < n; s += WARPS) {
-        const Seq q = cut.open(s);
-        uint64_t sum = 0u;
-        const uint32_t units = q.rows ? cut.units(q) : 0u;
-        for (uint32_t i = lane; i < units; i += 32u) {
-            const uint32_t c = cut.cost(q, i);
-            sum += c;
-            most = max(most, c);
+    const bool keep = n <= kKeptSeqs;
+    Piece p;
+    uint32_t most = 0u, all_units;
+    uint64_t total;
+    uint64_t of_seq = 0u, mine = 0u;      // keep: lane s has its sequence's work per KV head, the line up to its end,
+    uint32_t mine_units = 0u;             // and the units
+    if (keep) {
+        const bool there = lane < n;
+        const uint32_t e0 = there ? (uint32_t)__ldcg(a.c.table + (size_t)lane * a.c.max_pages) : 0u;
+        p.kept.p0 = there ? __ldcg(a.r.pos0 + lane) : 0u;
+        p.kept.rows = there ? row_count(a.r, lane) * a.group : 0u;
+        p.kept.k0 = 0u;
+        for (uint32_t gone = __ballot_sync(0xffffffffu, p.kept.rows && e0 >= a.c.pages); gone; gone &= gone - 1u) {
+            const uint32_t s = (uint32_t)__ffs((int)gone) - 1u;
+            const uint32_t k0 = cut.begin(s, __shfl_sync(0xffffffffu, p.kept.p0, (int)s), __shfl_sync(0xffffffffu, p.kept.rows, (int)s));
+            if (lane == s) p.kept.k0 = k0;
         }
-        if (units == 1u) sum = __shfl_sync(0xffffffffu, (uint32_t)sum, 0);
-        else
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0u) {
-            sm.work[s] = sum;
-            sm.units[s] = units;
-            if (s < kKeptSeqs) kept.seq[s] = q;
+        const uint32_t units = p.kept.rows ? cut.units(p.kept) : 0u;
+        if (__all_sync(0xffffffffu, units <= 4u)) {   // a lane does its own
+            uint32_t sum = 0u;            // at most 2^29
+            for (uint32_t i = 0; i < units; ++i) {
+                const uint32_t c = cut.cost(p.kept, i);
+                sum += c;
+                most = max(most, c);
+            }
+            of_seq = sum;
+            most = __reduce_max_sync(0xffffffffu, most);
+        } else {
+            for (uint32_t s = 0; s < n; ++s) {
+                const uint64_t sum = cut.all(cut.open(s, p.kept), most);
+                if (lane == s) of_seq = sum;
+            }
         }
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0u) sm.most[warp] = most;
-    __syncthreads();
-    most = __reduce_max_sync(0xffffffffu, lane < WARPS ? sm.most[lane] : 0u);
-    // the line's length before each sequence: by every warp for itself, or by the first one for all
-    uint64_t total = 0u;
-    uint32_t all_units = 0u;
-    uint64_t mine = 0u;                   // few sequences: lane s has those up to s
-    uint32_t mine_units = 0u;
-    if (n <= kKeptSeqs) {
-        mine = up_to(lane < n ? sm.work[lane] * a.c.kv_heads : 0u);
-        mine_units = up_to(lane < n ? sm.units[lane] * a.c.kv_heads : 0u);
+        mine = up_to(of_seq * a.c.kv_heads);
+        mine_units = up_to(units * a.c.kv_heads);     // units < 2^30 / 8 over 32 sequences: checked below
         total = __shfl_sync(0xffffffffu, mine, 31);
-        all_units = __shfl_sync(0xffffffffu, mine_units, 31);
+        all_units = __any_sync(0xffffffffu, units > gridDim.x) ? ~0u : __shfl_sync(0xffffffffu, mine_units, 31);
     } else {
+        for (uint32_t s = warp; s < n; s += WARPS) {
+            const Seq q = cut.open(s);
+            const uint64_t sum = cut.all(q, most);
+            if (lane == 0u) {
+                sm.work[s] = sum;
+                sm.units[s] = q.rows ? cut.units(q) : 0u;
+            }
+        }
+        if (lane == 0u) sm.most[warp] = most;
+        __syncthreads();
+        most = __reduce_max_sync(0xffffffffu, lane < WARPS ? sm.most[lane] : 0u);
         if (warp == 0u) {
             uint64_t work = 0u, units = 0u;
             for (uint32_t b = 0u; b < n; b += 32u) {
@@ -220,15 +262,15 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
         total = sm.work[n - 1u];
         all_units = sm.all_units;
     }
-    Piece p;
     p.s = p.h = p.i = p.skip = 0u;
     p.begin = 0u;
     p.left = 0u;
     p.each = quotient(total + gridDim.x - 1u, gridDim.x);
+    const bool whole = all_units <= gridDim.x && most <= p.each + worth;
     // the sequence that place `at` is in, by the sums up to each one, and the sum before it
     auto find = [&](auto at, auto up, const auto *sums, auto &before) {
         uint32_t s;
-        if (n <= kKeptSeqs) {
+        if (keep) {
             s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, up > at)) - 1u;
             before = __shfl_sync(0xffffffffu, up, s ? (int)s - 1 : 0);
         } else {
@@ -244,28 +286,31 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
         if (s == 0u) before = 0u;
         return s;
     };
-    if (all_units <= gridDim.x && most <= p.each + worth) {
-        if (blockIdx.x >= all_units) return p;
-        uint32_t before;
-        p.s = find(blockIdx.x, mine_units, sm.units, before);
-        const Seq q = cut.open(p.s, kept);
-        const uint32_t units = cut.units(q);
-        p.h = (blockIdx.x - before) / units;
-        p.i = blockIdx.x - before - p.h * units;
+    uint64_t before = 0u, of_head = 1u;
+    uint32_t before_units = 0u;
+    if (whole) {
+        if (blockIdx.x < all_units) p.s = find(blockIdx.x, mine_units, sm.units, before_units);
+    } else {
+        p.each = max(p.each, (uint64_t)least);
+        p.begin = p.each * blockIdx.x;
+        if (p.begin < total) {
+            p.left = min(p.each, total - p.begin);
+            p.s = find(p.begin, mine, sm.work, before);
+            of_head = keep ? __shfl_sync(0xffffffffu, of_seq, (int)p.s) : quotient(sm.work[p.s] - before, a.c.kv_heads);
+        }
+    }
+    if (!keep) __syncthreads();           // `sm` is free
+    if (whole ? blockIdx.x >= all_units : !p.left) return p;
+    const Seq q = cut.open(p.s, p.kept);
+    const uint32_t units = cut.units(q);
+    if (whole) {
+        p.h = (blockIdx.x - before_units) / units;
+        p.i = blockIdx.x - before_units - p.h * units;
         p.left = cut.cost(q, p.i);
         return p;
     }
-    p.each = max(p.each, (uint64_t)least);
-    p.begin = p.each * blockIdx.x;
-    if (p.begin >= total) return p;
-    p.left = min(p.each, total - p.begin);
-    uint64_t before;
-    p.s = find(p.begin, mine, sm.work, before);
-    const Seq q = cut.open(p.s, kept);
-    const uint64_t of_head = n <= kKeptSeqs ? sm.work[p.s] : quotient(sm.work[p.s] - before, a.c.kv_heads);
     p.h = (uint32_t)quotient(p.begin - before, of_head);
     uint64_t rest = p.begin - before - of_head * p.h;
-    const uint32_t units = cut.units(q);
     for (uint32_t b = 0;; b += 32u) {     // the unit that holds place `rest`
         const uint32_t c = b + lane < units ? cut.cost(q, b + lane) : 0u;
         const uint64_t x = up_to((uint64_t)c);
@@ -284,7 +329,6 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
 template <uint32_t KEYS, uint32_t MOST = 0x7fffffffu>
 struct Walk {
     const Cut<KEYS> &cut;
-    const Kept &kept;
     Piece p;
     Seq q;
     uint32_t k_begin, k_end;              // the step's tiles of keys of the current unit
@@ -292,10 +336,10 @@ struct Walk {
     bool first;                           // it is the piece's first unit
     bool again;                           // there were steps of the unit before in this piece
 
-    __device__ __forceinline__ Walk(const Cut<KEYS> &cut_, const Piece &p_, const Kept &kept_) : cut(cut_), kept(kept_), p(p_), first(true), again(false)
+    __device__ __forceinline__ Walk(const Cut<KEYS> &cut_, const Piece &p_) : cut(cut_), p(p_), first(true), again(false)
     {
         if (p.left) {
-            q = cut.open(p.s, kept);
+            q = cut.open(p.s, p.kept);
             set();
         }
     }
@@ -327,7 +371,7 @@ struct Walk {
             p.i = 0u;
             if (++p.h >= cut.a.c.kv_heads) {
                 p.h = 0u;
-                do q = cut.open(++p.s, kept);
+                do q = cut.open(++p.s, p.kept);
                 while (!q.rows);          // there is more, so a sequence with rows comes
             }
         }

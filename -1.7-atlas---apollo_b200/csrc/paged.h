@@ -46,6 +46,22 @@ struct WorkHead {
 enum WorkArray : uint32_t { kCopyFrom, kCopyTo, kCopyRows, kWriters, kLastWriter, kFresh, kWorkArrays };
 constexpr uint32_t kMovedTo = kWriters;  // compact: the new number of a page that has moved
 
+// Division by a number known at the launch: for x < 2^31, x * m >> (31 + L) is x / d, where 2^L >= d and m = ceil(2^(31 + L) / d)
+// < 2^32 (m d exceeds 2^(31 + L) by less than d, so x m / 2^(31 + L) exceeds x / d by less than 2^-L <= 1 / d)
+struct Divisor {
+    uint32_t m, shift;                    // shift: L
+};
+inline Divisor divisor(uint32_t d)
+{
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return Divisor{(uint32_t)(((1ull << (31u + l)) + d - 1u) / d), l};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t x, const Divisor &d)
+{
+    return (uint32_t)((uint64_t)x * d.m >> 31) >> d.shift;
+}
+
 struct AttnArgs {
     Cache c;
     Rows r;
@@ -53,6 +69,7 @@ struct AttnArgs {
     uint16_t *out;
     uint64_t ldq, ldo;
     uint32_t q_heads, group, layer;
+    Divisor by_group;
     float *parts;                         // partial sums: see Part
     uint32_t early;                       // the successor may start at once
 };

@@ -60,7 +60,6 @@ struct alignas(1024) Smem {
     } u;
     uint64_t full[kWarps][kStages];
     uint32_t err;
-    Kept kept;
     float2 wml[kWarps][8 * NT];
 };
 
@@ -132,12 +131,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     __syncthreads();
     wait_predecessor(a.early);
     const Cut<kChunk> cut{a, R};
-    const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, sm.kept, kWarps, kWorth);
-    Walk<kChunk> w(cut, piece, sm.kept);
-    if (threadIdx.x == 0u) reinterpret_cast<Part *>(a.parts)[blockIdx.x] = w.part();
-    if (!w.more()) return;
-    fence_ring();
-    __syncthreads();                      // the ring's place is free
+    const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, kWarps, kWorth);
+    Walk<kChunk> w(cut, piece);
+    if (a.c.nseq > kKeptSeqs) {           // the ring's place is free
+        fence_ring();
+        __syncthreads();
+    }
     const uint32_t ring = smem_addr(sm.u.ring[warp][0]);
     uint64_t *const full = sm.full[warp];
     const float inv_group = 1.000001f / (float)a.group;
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 
     for (; w.more(); w.next()) {
         const uint32_t rows = w.rows(), row0 = w.row0(), s = w.p.s, h = w.p.h;
-        TileRows tr{row0 / a.group, 0u, a.group, inv_group};
+        TileRows tr{divide(row0, a.by_group), 0u, a.group, inv_group};
         tr.rem = row0 - tr.tok * a.group;
         const uint64_t p0 = w.q.p0;
         const uint32_t seen = cut.keys(w.q, row0 + rows);          // chunks that some row sees
@@ -219,25 +218,30 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         const uint32_t koff = (lane & 15u) * 128u, kx = (lane >> 4) ^ (lane & 7u);
         const uint32_t vkey = (lane & 7u) + 8u * (lane >> 4), voff = 2u * kHalfChunk + vkey * 128u, vx = ((lane >> 3) & 1u) ^ (lane & 7u);
         while (ok && chunk[0] != kNone) {
-            __syncwarp();                 // every lane is done with the slot that the last chunk left
             const uint32_t key = chunk[0] * kChunk;
-#pragma unroll
-            for (uint32_t i = 0; i + 1u < kStages; ++i) chunk[i] = chunk[i + 1u];
-            chunk[kStages - 2u] = issue();
             ok = __all_sync(0xffffffffu, mbar_wait(full + slot, phase, &sm.err));
             if (!ok) break;
             const uint32_t in = ring + slot * kSlot;
             if (++slot == kStages) slot = 0u, phase ^= 1u;
-            float y[NT][4];
+            // two sums, so that the products wait for one another half as long
+            float y[NT][4], y2[NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = 0.f;
+            for (int nt = 0; nt < NT; ++nt) y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = y2[nt][0] = y2[nt][1] = y2[nt][2] = y2[nt][3] = 0.f;
 #pragma unroll
-            for (uint32_t st = 0; st < 8u; ++st) {
-                uint32_t ka[4];
-                load_matrices(ka, in + (st >> 2) * kHalfChunk + koff + ((kx ^ (2u * (st & 3u))) << 4));
+            for (uint32_t st = 0; st < 4u; ++st) {
+                uint32_t ka[4], kb[4];
+                load_matrices(ka, in + koff + ((kx ^ (2u * st)) << 4));
+                load_matrices(kb, in + kHalfChunk + koff + ((kx ^ (2u * st)) << 4));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma<BF>(y[nt], ka, qf[nt][st][0], qf[nt][st][1]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma<BF>(y[nt], ka, qf[nt][st][0], qf[nt][st][1]);
+                    mma<BF>(y2[nt], kb, qf[nt][4 + st][0], qf[nt][4 + st][1]);
+                }
             }
+            // the slot that the last chunk left, which every lane is done with, takes the next copies meanwhile
+#pragma unroll
+            for (uint32_t i = 0; i + 1u < kStages; ++i) chunk[i] = chunk[i + 1u];
+            chunk[kStages - 2u] = issue();
             // scores: positions key + g (elements 0, 1) and key + g + 8 (2, 3), columns 2 t and 2 t + 1
             const bool masked = key + kChunk - 1u > open;   // some row does not see all of the chunk
             const uint32_t pa = key + g, pb = key + g + 8u;
@@ -246,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    y[nt][e] *= kScoreScale;
+                    y[nt][e] = (y[nt][e] + y2[nt][e]) * kScoreScale;
                     if (masked && (e < 2 ? pa : pb) > last[nt][e & 1]) y[nt][e] = -INFINITY;
                     raise |= y[nt][e] > m[nt][e & 1] + kLazy;
                 }
@@ -398,6 +402,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         }
         fence_ring();
         __syncthreads();                  // the ring may fill again
+    }
+    if (warp == 0u) {
+        const Part part = Walk<kChunk>(cut, piece).part();
+        if (lane == 0u) reinterpret_cast<Part *>(a.parts)[blockIdx.x] = part;
     }
 }
 

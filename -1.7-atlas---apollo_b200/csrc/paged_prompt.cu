@@ -77,7 +77,6 @@ struct PromptArgs : AttnArgs {
 struct Bars {
     uint64_t s_full[2], p_full[2][2], o_full[2], o_free[2], full[kMaxStages], free[kMaxStages], checked[kMaxStages], q_full, q_free, fin;
     uint32_t tmem, status;
-    Kept kept;
     uint32_t bad[4];                               // the step in which a value was taken out, at its number % 4
     float2 state[2][kTileRows];                    // one tile of rows: the groups' maxima and sums
 };
@@ -168,13 +167,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     wait_predecessor(a.early);
     const uint32_t tile_rows = a.tokens_per_tile * a.group;      // of 128 in tensor memory
     const Cut<kTileKeys> cut{a, (ONE ? 1u : 2u) * tile_rows};
-    const Piece piece = find_piece<kTileKeys, kThreads / 32u>(cut, *reinterpret_cast<PieceSmem *>(kv), b.kept, 2u, kWorth);
+    const Piece piece = find_piece<kTileKeys, kThreads / 32u>(cut, *reinterpret_cast<PieceSmem *>(kv), 2u, kWorth);
     fence_before();
     fence_async();
     __syncthreads();
     fence_after();
     const uint32_t tmem = b.tmem;   // scores / weights of group t: column 128 t; output: 256 + 128 t
-    Walk<kTileKeys, kMostTiles> w(cut, piece, b.kept);
+    Walk<kTileKeys, kMostTiles> w(cut, piece);
 
     // The end of a CTA, for every warp in the branch of its registers
     auto leave = [&]() {
@@ -200,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const uint32_t nowhere = (a.c.layers * a.c.pages * a.c.kv_heads) << page_log2;   // behind the pool's end: zeros
         for (; ok && w.more(); w.next(), ++steps) {
             const uint32_t s = w.p.s, h = w.p.h, row0 = w.row0(), rows = w.rows(), tiles = tiles_of(rows);
-            const uint32_t seen = (uint32_t)min((uint64_t)w.q.p0 + (row0 + rows - 1u) / a.group + 1u, (uint64_t)a.c.limit);
+            const uint32_t seen = (uint32_t)min((uint64_t)w.q.p0 + divide(row0 + rows - 1u, a.by_group) + 1u, (uint64_t)a.c.limit);
             const int32_t *const entries = a.c.table + (size_t)s * a.c.max_pages;
             // where this lane's page of tile j begins
             auto page_row = [&](uint32_t j) {
@@ -212,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             if (!ok) break;
             if (lane == 0u) {
                 mbar_arrive_expect_tx(&b.q_full, tiles * tile_rows * 256u);
-                const uint32_t token = s * a.r.tokens + row0 / a.group;
+                const uint32_t token = s * a.r.tokens + divide(row0, a.by_group);
                 for (uint32_t t = 0; t < tiles; ++t)
                     for (uint32_t hf = 0; hf < 2u; ++hf)
                         load_queries(smem_addr(qs + t * kTile + hf * kHalf), &a.qmap, h * a.group, token + t * a.tokens_per_tile, hf, &b.q_full);
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const uint64_t qd = operand(smem_addr(qs)), kd = operand(smem_addr(kv)), vd = operand_across(smem_addr(kv), kHalf);
         for (; ok && w.more(); w.next(), ++steps) {
             const uint32_t tiles = tiles_of(w.rows()), n = w.k_end - w.k_begin;
-            const uint64_t open = (uint64_t)w.q.p0 + w.row0() / a.group;   // every row sees the positions up to it
+            const uint64_t open = (uint64_t)w.q.p0 + divide(w.row0(), a.by_group);   // every row sees the positions up to it
             if (leader) {
                 ok = mbar_wait(&b.q_full, steps & 1u, err);
                 // scores of the keys in ring slot `slot` by tile of rows qt, into group t's columns
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         bool ok = true;
         for (; ok && w.more(); w.next(), ++steps) {
             const uint32_t n = w.k_end - w.k_begin;
-            const uint64_t open = (uint64_t)w.q.p0 + w.row0() / a.group;
+            const uint64_t open = (uint64_t)w.q.p0 + divide(w.row0(), a.by_group);
             auto pass = [&]() {
                 ok = ok && wait_warp(&b.full[ring.slot], ring.phase, err);
                 ring.next();
@@ -462,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         for (; w.more(); w.next(), ++steps) {
             const uint32_t s = w.p.s, h = w.p.h, row0 = w.row0(), rows = w.rows(), tiles = tiles_of(rows), n = w.k_end - w.k_begin;
             if (!ONE && t >= tiles) continue;
-            const uint32_t base = ONE ? 0u : t * tile_rows, tok0 = row0 / a.group + (ONE ? 0u : t * a.tokens_per_tile);
+            const uint32_t base = ONE ? 0u : t * tile_rows, tok0 = divide(row0, a.by_group) + (ONE ? 0u : t * a.tokens_per_tile);
             const uint2 mine = TileRows{tok0, 0u, a.group, group_inv}.at(row);
             const bool there = row < tile_rows && base + row < rows;
             const uint64_t p0 = w.q.p0;
@@ -613,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 if (!there) continue;
                 if (bad == steps) {   // what was taken out of V, to the rows that see it
                     const uint64_t k1 = min((uint64_t)last + 1u, (uint64_t)w.k_end * kTileKeys);
-                    for (uint64_t p = max((uint64_t)w.k_begin * kTileKeys, (uint64_t)p0 + row0 / a.group + 1u); p < min(k1, (uint64_t)a.c.limit); ++p) {
+                    for (uint64_t p = max((uint64_t)w.k_begin * kTileKeys, (uint64_t)p0 + divide(row0, a.by_group) + 1u); p < min(k1, (uint64_t)a.c.limit); ++p) {
                         const uint32_t e = (uint32_t)__ldcg(entries + (p >> page_log2));
                         if (e >= a.c.pages) continue;
                         const uint16_t *v = a.c.v + (((((size_t)a.layer * a.c.pages + e) * a.c.kv_heads + h) << page_log2) + (p & ((1u << page_log2) - 1u))) * kDim + c;

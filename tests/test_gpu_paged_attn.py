@@ -87,7 +87,8 @@ SHAPES = [
     (2, 4, [100], 2, None), (1, 3, [0], 5, None), (2, 8, [1000, 30], 4, [4, 3]), (8, 5, [801] * 4, 7, None), (2, 1, [50], 16, None),
     (1, 1, [0], 17, None), (1, 1, [0], 130, None), (4, 7, [0], 40, None), (2, 8, [0, 513], 33, [33, 20]), (1, 5, [63], 100, None),
     (4, 7, [0], 300, None), (2, 8, [700, 0, 40], 260, [260, 1, 255]), (1, 12, [129], 129, None), (1, 40, [10], 70, None), (1, 64, [3], 9, None),
-    (1, 100, [9], 30, None), (1, 130, [9], 5, None),
+    (1, 100, [9], 30, None), (1, 130, [9], 5, None), (1, 7, [13 * i for i in range(40)], 1, None), (2, 2, [300 - 5 * i for i in range(37)], 5, [i % 7 for i in range(37)]),
+    (1, 4, [11 * i for i in range(45)], 50, [(7 * i) % 60 for i in range(45)]), (1, 8, [0] * 33, 70, None),
 ]
 
 
@@ -96,10 +97,10 @@ SHAPES = [
 @pytest.mark.parametrize("page", [16, 32, 64, 128])
 def test_against_the_definition(torch_cuda, kind, shape, page):
     kvh, grp, pos, tokens, ntok = shape
-    lens = [p + (tokens if ntok is None else ntok[s]) for s, p in enumerate(pos)]
+    lens = [p + (tokens if ntok is None else min(ntok[s], tokens)) for s, p in enumerate(pos)]
     x = Setup(torch_cuda, kind, page, kvh, lens, -(-max(lens) // page) + 2, seed=page + tokens)
     q = x.rand(len(pos), tokens, kvh * grp, DIM)
-    x.check(x.attn(q, pos, ntok), q, pos, ntok, sample=12)
+    x.check(x.attn(q, pos, ntok), q, pos, ntok, sample=12 if len(pos) < 10 else 2)
 
 
 @pytest.mark.parametrize("kind,page,kvh,grp,pos,tokens", [
