@@ -728,11 +728,13 @@ extern "C" int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_use
 
 namespace {
 
-// The query rows of a KV head that a CTA takes at a time: 8, 16 or 32 (the form for few rows), 128 or 256
+constexpr uint32_t kFewRows = 16;
+
+// The query rows of a KV head that a CTA takes at a time: 8 or 16 (the form for few rows), 128 or 256
 uint32_t attn_rows(const Cache &c, uint32_t group, uint32_t tokens, int sms)
 {
     const uint64_t rows = (uint64_t)tokens * group;
-    if (rows <= 32 || group > 128) return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    if (rows <= kFewRows || group > 128) return rows <= 8 ? 8 : 16;
     const uint32_t per = 128 / group;
     return (uint64_t)c.nseq * c.kv_heads * ((tokens + per - 1) / per) <= (uint64_t)sms ? 128 : 256;
 }

@@ -72,14 +72,15 @@ struct Seq {
     uint32_t p0, rows, k0;
 };
 
-// Up to this many sequences, each lane of a warp keeps one's Seq
+// Up to this many sequences, each lane of a warp keeps one's Seq (where the line has less than 2^31 tiles of keys)
 constexpr uint32_t kKeptSeqs = 32;
 
 // How a call's rows are cut into tiles of `tile` rows
 template <uint32_t KEYS>
 struct Cut {
     const AttnArgs &a;
-    uint32_t tile;        // query rows of a unit
+    const uint32_t tile;  // query rows of a unit
+    const Divisor by_tile;
 
     // the tiles of keys that rows before `row1` see, from the front
     __device__ __forceinline__ uint32_t keys(const Seq &q, uint32_t row1) const
@@ -87,7 +88,7 @@ struct Cut {
         const uint64_t last = min((uint64_t)q.p0 + divide(row1 - 1u, a.by_group) + 1u, (uint64_t)a.c.limit);
         return (uint32_t)((last + KEYS - 1u) / KEYS);
     }
-    __device__ __forceinline__ uint32_t units(const Seq &q) const { return (q.rows + tile - 1u) / tile; }
+    __device__ __forceinline__ uint32_t units(const Seq &q) const { return divide(q.rows + tile - 1u, by_tile); }
     // work of a unit: at least one tile of keys, so that its rows are written
     __device__ __forceinline__ uint32_t cost(const Seq &q, uint32_t i) const
     {
@@ -125,10 +126,10 @@ struct Cut {
         q.k0 = q.rows && e0 >= a.c.pages ? begin(s, q.p0, q.rows) : 0u;
         return q;
     }
-    // `kept`: this lane's, where there are no more than kKeptSeqs
+    // `kept`: this lane's, where lanes keep them
     __device__ __forceinline__ Seq open(uint32_t s, const Seq &kept) const
     {
-        if (a.c.nseq > kKeptSeqs) return open(s);
+        if (!a.keep) return open(s);
         Seq q;
         q.p0 = __shfl_sync(0xffffffffu, kept.p0, (int)s);
         q.rows = __shfl_sync(0xffffffffu, kept.rows, (int)s);
@@ -158,7 +159,7 @@ struct Piece {
     uint64_t begin, each; // in the line of all; a CTA's share
     uint32_t s, h, i, skip;
     uint64_t left;
-    Seq kept;             // lane s has sequence s, where there are no more than kKeptSeqs
+    Seq kept;             // lane s has sequence s, where lanes keep them
 };
 
 struct PieceSmem {
@@ -196,13 +197,34 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
 {
     const AttnArgs &a = cut.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = a.c.nseq;
-    const bool keep = n <= kKeptSeqs;
     Piece p;
-    uint32_t most = 0u, all_units;
-    uint64_t total;
-    uint64_t of_seq = 0u, mine = 0u;      // keep: lane s has its sequence's work per KV head, the line up to its end,
-    uint32_t mine_units = 0u;             // and the units
-    if (keep) {
+    p.s = p.h = p.i = p.skip = 0u;
+    p.begin = 0u;
+    p.left = 0u;
+    uint32_t most = 0u;
+    // the unit of sequence p.s that place `rest` of a KV head's units is in
+    auto unit_at = [&](auto rest) {
+        using T = decltype(rest);
+        const Seq q = cut.open(p.s, p.kept);
+        const uint32_t units = cut.units(q);
+        if (units == 1u) {
+            p.skip = (uint32_t)rest;
+            return;
+        }
+        for (uint32_t b = 0;; b += 32u) {
+            const uint32_t c = b + lane < units ? cut.cost(q, b + lane) : 0u;
+            const T x = up_to((T)c);
+            const uint32_t past = __ballot_sync(0xffffffffu, x > rest);
+            if (past || b + 32u >= units) {
+                const uint32_t at = past ? (uint32_t)__ffs((int)past) - 1u : 31u;
+                p.i = min(b + at, units - 1u);
+                p.skip = (uint32_t)(rest - __shfl_sync(0xffffffffu, x - c, (int)at));
+                return;
+            }
+            rest -= __shfl_sync(0xffffffffu, x, 31);
+        }
+    };
+    if (a.keep) {
         const bool there = lane < n;
         const uint32_t e0 = there ? (uint32_t)__ldcg(a.c.table + (size_t)lane * a.c.max_pages) : 0u;
         p.kept.p0 = there ? __ldcg(a.r.pos0 + lane) : 0u;
@@ -213,116 +235,121 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
             const uint32_t k0 = cut.begin(s, __shfl_sync(0xffffffffu, p.kept.p0, (int)s), __shfl_sync(0xffffffffu, p.kept.rows, (int)s));
             if (lane == s) p.kept.k0 = k0;
         }
+        // lane s: its sequence's units and work per KV head
         const uint32_t units = p.kept.rows ? cut.units(p.kept) : 0u;
-        if (__all_sync(0xffffffffu, units <= 4u)) {   // a lane does its own
-            uint32_t sum = 0u;            // at most 2^29
+        uint32_t work = 0u;
+        if (__all_sync(0xffffffffu, units <= 4u)) {
             for (uint32_t i = 0; i < units; ++i) {
                 const uint32_t c = cut.cost(p.kept, i);
-                sum += c;
+                work += c;
                 most = max(most, c);
             }
-            of_seq = sum;
             most = __reduce_max_sync(0xffffffffu, most);
         } else {
             for (uint32_t s = 0; s < n; ++s) {
-                const uint64_t sum = cut.all(cut.open(s, p.kept), most);
-                if (lane == s) of_seq = sum;
+                const uint32_t sum = (uint32_t)cut.all(cut.open(s, p.kept), most);
+                if (lane == s) work = sum;
             }
         }
-        mine = up_to(of_seq * a.c.kv_heads);
-        mine_units = up_to(units * a.c.kv_heads);     // units < 2^30 / 8 over 32 sequences: checked below
-        total = __shfl_sync(0xffffffffu, mine, 31);
-        all_units = __any_sync(0xffffffffu, units > gridDim.x) ? ~0u : __shfl_sync(0xffffffffu, mine_units, 31);
-    } else {
-        for (uint32_t s = warp; s < n; s += WARPS) {
-            const Seq q = cut.open(s);
-            const uint64_t sum = cut.all(q, most);
-            if (lane == 0u) {
-                sm.work[s] = sum;
-                sm.units[s] = q.rows ? cut.units(q) : 0u;
-            }
+        // the line up to the end of each sequence
+        const uint32_t all_units = __reduce_add_sync(0xffffffffu, units) * a.c.kv_heads;
+        const uint32_t line = n == 1u ? work * a.c.kv_heads : up_to(work * a.c.kv_heads);
+        const uint32_t total = __shfl_sync(0xffffffffu, line, (int)n - 1);
+        uint32_t each = (total + gridDim.x - 1u) / gridDim.x;
+        const bool whole = all_units <= gridDim.x && most <= each + worth;
+        const uint32_t ends = whole ? (n == 1u ? all_units : up_to(units * a.c.kv_heads)) : line;
+        each = whole ? 1u : max(each, least);
+        p.each = each;
+        const uint32_t at = each * blockIdx.x, end = whole ? all_units : total;
+        if (at >= end) return p;
+        uint32_t before = 0u;
+        if (n > 1u) {
+            p.s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, lane < n && ends > at)) - 1u;
+            before = __shfl_sync(0xffffffffu, ends, p.s ? (int)p.s - 1 : 0);
+            if (p.s == 0u) before = 0u;
         }
-        if (lane == 0u) sm.most[warp] = most;
-        __syncthreads();
-        most = __reduce_max_sync(0xffffffffu, lane < WARPS ? sm.most[lane] : 0u);
-        if (warp == 0u) {
-            uint64_t work = 0u, units = 0u;
-            for (uint32_t b = 0u; b < n; b += 32u) {
-                const uint64_t w = up_to(b + lane < n ? sm.work[b + lane] * a.c.kv_heads : 0u), u = up_to((uint64_t)(b + lane < n ? sm.units[b + lane] : 0u) * a.c.kv_heads);
-                if (b + lane < n) {
-                    sm.work[b + lane] = work + w;
-                    sm.units[b + lane] = (uint32_t)(units + u);
-                }
-                work += __shfl_sync(0xffffffffu, w, 31);
-                units += __shfl_sync(0xffffffffu, u, 31);
-            }
-            if (lane == 0u) sm.all_units = units >> 32 ? ~0u : (uint32_t)units;
+        const uint32_t of_head = __shfl_sync(0xffffffffu, whole ? units : work, (int)p.s);
+        p.h = (at - before) / of_head;
+        const uint32_t rest = at - before - of_head * p.h;
+        if (whole) {
+            p.i = rest;
+            p.left = cut.cost(cut.open(p.s, p.kept), p.i);
+        } else {
+            p.begin = at;
+            p.left = min(each, end - at);
+            unit_at(rest);
         }
-        __syncthreads();
-        total = sm.work[n - 1u];
-        all_units = sm.all_units;
+        return p;
     }
-    p.s = p.h = p.i = p.skip = 0u;
-    p.begin = 0u;
-    p.left = 0u;
+    for (uint32_t s = warp; s < n; s += WARPS) {
+        const Seq q = cut.open(s);
+        const uint64_t sum = cut.all(q, most);
+        if (lane == 0u) {
+            sm.work[s] = sum;
+            sm.units[s] = q.rows ? cut.units(q) : 0u;
+        }
+    }
+    if (lane == 0u) sm.most[warp] = most;
+    __syncthreads();
+    most = __reduce_max_sync(0xffffffffu, lane < WARPS ? sm.most[lane] : 0u);
+    if (warp == 0u) {
+        uint64_t work = 0u, units = 0u;
+        for (uint32_t b = 0u; b < n; b += 32u) {
+            const uint64_t w = up_to(b + lane < n ? sm.work[b + lane] * a.c.kv_heads : 0u), u = up_to((uint64_t)(b + lane < n ? sm.units[b + lane] : 0u) * a.c.kv_heads);
+            if (b + lane < n) {
+                sm.work[b + lane] = work + w;
+                sm.units[b + lane] = (uint32_t)(units + u);
+            }
+            work += __shfl_sync(0xffffffffu, w, 31);
+            units += __shfl_sync(0xffffffffu, u, 31);
+        }
+        if (lane == 0u) sm.all_units = units >> 32 ? ~0u : (uint32_t)units;
+    }
+    __syncthreads();
+    const uint64_t total = sm.work[n - 1u];
+    const uint32_t all_units = sm.all_units;
     p.each = quotient(total + gridDim.x - 1u, gridDim.x);
     const bool whole = all_units <= gridDim.x && most <= p.each + worth;
-    // the sequence that place `at` is in, by the sums up to each one, and the sum before it
-    auto find = [&](auto at, auto up, const auto *sums, auto &before) {
-        uint32_t s;
-        if (keep) {
-            s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, up > at)) - 1u;
-            before = __shfl_sync(0xffffffffu, up, s ? (int)s - 1 : 0);
-        } else {
-            uint32_t lo = 0u, hi = n - 1u;   // sums[hi] > at
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (sums[mid] > at) hi = mid;
-                else lo = mid + 1u;
-            }
-            s = lo;
-            before = s ? sums[s - 1u] : 0u;
+    // the sequence that place `at` is in, by the sums up to each one
+    auto find = [&](auto at, const auto *sums) {
+        uint32_t lo = 0u, hi = n - 1u;   // sums[hi] > at
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (sums[mid] > at) hi = mid;
+            else lo = mid + 1u;
         }
-        if (s == 0u) before = 0u;
-        return s;
+        return lo;
     };
     uint64_t before = 0u, of_head = 1u;
     uint32_t before_units = 0u;
     if (whole) {
-        if (blockIdx.x < all_units) p.s = find(blockIdx.x, mine_units, sm.units, before_units);
+        if (blockIdx.x < all_units) {
+            p.s = find(blockIdx.x, sm.units);
+            before_units = p.s ? sm.units[p.s - 1u] : 0u;
+        }
     } else {
         p.each = max(p.each, (uint64_t)least);
         p.begin = p.each * blockIdx.x;
         if (p.begin < total) {
             p.left = min(p.each, total - p.begin);
-            p.s = find(p.begin, mine, sm.work, before);
-            of_head = keep ? __shfl_sync(0xffffffffu, of_seq, (int)p.s) : quotient(sm.work[p.s] - before, a.c.kv_heads);
+            p.s = find(p.begin, sm.work);
+            before = p.s ? sm.work[p.s - 1u] : 0u;
+            of_head = quotient(sm.work[p.s] - before, a.c.kv_heads);
         }
     }
-    if (!keep) __syncthreads();           // `sm` is free
+    __syncthreads();                      // `sm` is free
     if (whole ? blockIdx.x >= all_units : !p.left) return p;
-    const Seq q = cut.open(p.s, p.kept);
-    const uint32_t units = cut.units(q);
     if (whole) {
+        const Seq q = cut.open(p.s);
+        const uint32_t units = cut.units(q);
         p.h = (blockIdx.x - before_units) / units;
         p.i = blockIdx.x - before_units - p.h * units;
         p.left = cut.cost(q, p.i);
-        return p;
+    } else {
+        p.h = (uint32_t)quotient(p.begin - before, of_head);
+        unit_at(p.begin - before - of_head * p.h);
     }
-    p.h = (uint32_t)quotient(p.begin - before, of_head);
-    uint64_t rest = p.begin - before - of_head * p.h;
-    for (uint32_t b = 0;; b += 32u) {     // the unit that holds place `rest`
-        const uint32_t c = b + lane < units ? cut.cost(q, b + lane) : 0u;
-        const uint64_t x = up_to((uint64_t)c);
-        const uint32_t past = __ballot_sync(0xffffffffu, x > rest);
-        if (past || b + 32u >= units) {
-            const uint32_t at = past ? (uint32_t)__ffs((int)past) - 1u : 31u;
-            p.i = min(b + at, units - 1u);
-            p.skip = (uint32_t)(rest - __shfl_sync(0xffffffffu, x - c, (int)at));
-            return p;
-        }
-        rest -= __shfl_sync(0xffffffffu, x, 31);
-    }
+    return p;
 }
 
 // Walks over the units of a piece, MOST tiles of keys at a time. The whole warp.
@@ -411,6 +438,13 @@ __device__ __forceinline__ void store4(const AttnArgs &a, uint32_t s, uint32_t h
 {
     reinterpret_cast<uint2 *>(a.out + ((size_t)s * a.r.tokens + at.x) * a.ldo + (size_t)(h * a.group + at.y) * kDim)[d4] =
         make_uint2(pack<BF>(x.x, x.y), pack<BF>(x.z, x.w));
+}
+
+// Whether a warp's lanes can keep the call's sequences: see kKeptSeqs. Units of `tile` rows, each at least KEYS positions long.
+inline bool lanes_keep(const AttnArgs &a, uint32_t tile, uint32_t keys)
+{
+    const uint64_t units = ((uint64_t)a.r.tokens * a.group + tile - 1u) / tile, line = units * a.c.nseq * a.c.kv_heads;
+    return a.c.nseq <= kKeptSeqs && line < (1ull << 31) && line * ((a.c.limit + keys - 1u) / keys) < (1ull << 31);
 }
 
 // Whatever the positions, each unit will be a piece of its own (find_piece): a sequence has room for no more

@@ -71,6 +71,7 @@ struct AttnArgs {
     uint32_t q_heads, group, layer;
     Divisor by_group;
     float *parts;                         // partial sums: see Part
+    uint32_t keep;                        // a warp's lanes keep the sequences' state
     uint32_t early;                       // the successor may start at once
 };
 

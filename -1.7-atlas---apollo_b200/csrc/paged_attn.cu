@@ -5,7 +5,7 @@
 //
 // A unit is 8 NT query rows (token, head of the group; token-major) of a KV
 // head. A CTA takes a piece of the line of all units' keys (paged.cuh), 16
-// positions at a time dealt out over its eight warps, each with a softmax state
+// positions at a time dealt out over its warps, each with a softmax state
 // of its own (running maximum, sum, output), joined in shared memory at a unit's
 // end. 16 positions lie in one page: two TMA copies (16 rows of K, 16 of V,
 // swizzled) bring them into a ring of the warp's own, and positions without a
@@ -37,7 +37,7 @@ using k8::wait_predecessor;
 
 namespace {
 
-constexpr uint32_t kChunk = 16, kWarps = 8, kThreads = kWarps * 32, kStages = 3;
+constexpr uint32_t kChunk = 16, kWarps = 12, kThreads = kWarps * 32, kStages = 2;
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
 constexpr uint32_t kWorth = 64;               // chunks: what joining partial sums takes
@@ -74,6 +74,20 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same onto zeros
+template <bool BF>
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x)
@@ -130,15 +144,22 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     }
     __syncthreads();
     wait_predecessor(a.early);
-    const Cut<kChunk> cut{a, R};
+    const Cut<kChunk> cut{a, R, Divisor{1u << 31, NT == 1 ? 3u : 4u}};
     const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, kWarps, kWorth);
     Walk<kChunk> w(cut, piece);
-    if (a.c.nseq > kKeptSeqs) {           // the ring's place is free
+    if (!a.keep) {                        // the ring's place is free
         fence_ring();
         __syncthreads();
     }
     const uint32_t ring = smem_addr(sm.u.ring[warp][0]);
     uint64_t *const full = sm.full[warp];
+    // where ldmatrix reads: K of 16 dimensions (16 positions x 2 chunks), V of 16 dimensions (the same, to be transposed)
+    uint32_t koff[4], voff[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+        koff[i] = (lane & 15u) * 128u + (((2u * i + (lane >> 4)) ^ (lane & 7u)) << 4);
+        voff[i] = 2u * kHalfChunk + ((lane & 7u) + 8u * (lane >> 4)) * 128u + (((2u * i + ((lane >> 3) & 1u)) ^ (lane & 7u)) << 4);
+    }
     const float inv_group = 1.000001f / (float)a.group;
     uint32_t slot = 0u, phase = 0u, slot_in = 0u;
     bool ok = true;
@@ -152,39 +173,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         const uint32_t k_end = min(w.k_end, seen), first = w.k_begin + warp;
         const int32_t *const entries = a.c.table + (size_t)s * a.c.max_pages;
         const uint32_t page_chunks = a.c.page_log2 - 4u;           // log2 of chunks per page
-        // the entries of this warp's chunks first + 8 (base + lane), and the next 32
-        auto entry_of = [&](uint32_t base) {
-            const uint32_t c = first + kWarps * (base + lane);
-            return c < k_end ? (uint32_t)__ldcg(entries + (c >> page_chunks)) : ~0u;
-        };
-        uint32_t base = 0u, ent = entry_of(0u), ent_next = entry_of(32u), have = __ballot_sync(0xffffffffu, ent < a.c.pages);
-        // the next chunk of this warp's that has a page; its copies are issued into the next slot
-        auto issue = [&]() -> uint32_t {
-            while (!have) {
-                base += 32u;
-                if (first + kWarps * base >= k_end) return kNone;
-                ent = ent_next;
-                ent_next = entry_of(base + 32u);
-                have = __ballot_sync(0xffffffffu, ent < a.c.pages);
-            }
-            const uint32_t b = (uint32_t)__ffs((int)have) - 1u;
-            have &= have - 1u;
-            const uint32_t e = __shfl_sync(0xffffffffu, ent, (int)b), c = first + kWarps * (base + b);
-            if (lane == 0u) {
-                const uint32_t row = (((a.layer * a.c.pages + e) * a.c.kv_heads + h) << a.c.page_log2) + ((c & ((1u << page_chunks) - 1u)) << 4);
-                const uint32_t dst = ring + slot_in * kSlot;
-                mbar_arrive_expect_tx(full + slot_in, kSlot);
-                load_rows(dst, &a.kmap, row, full + slot_in);
-                load_rows(dst + kSlot / 2u, &a.vmap, row, full + slot_in);
-            }
-            if (++slot_in == kStages) slot_in = 0u;
-            return c;
-        };
-        uint32_t chunk[kStages];          // on their way; kNone: nothing more
-#pragma unroll
-        for (uint32_t i = 0; i < kStages - 1u; ++i) chunk[i] = issue();
-        chunk[kStages - 1u] = kNone;
-
         // B operands: column g, dimensions 16 st + 2 t, + 1, + 8, + 9
         uint32_t qf[NT][8][2];
         uint32_t last[NT][2];             // the last position that columns 2 t and 2 t + 1 see
@@ -206,6 +194,39 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
             }
         }
 
+        const uint32_t head0 = a.layer * a.c.pages * a.c.kv_heads + h;
+        // the entries of this warp's chunks first + kWarps (base + lane), and the next 32
+        auto entry_of = [&](uint32_t base) {
+            const uint32_t c = first + kWarps * (base + lane);
+            return c < k_end ? (uint32_t)__ldcg(entries + (c >> page_chunks)) : ~0u;
+        };
+        uint32_t base = 0u, ent = entry_of(0u), ent_next = entry_of(32u), have = __ballot_sync(0xffffffffu, ent < a.c.pages);
+        // the next chunk of this warp's that has a page; its copies are issued into the next slot
+        auto issue = [&]() -> uint32_t {
+            while (!have) {
+                base += 32u;
+                if (first + kWarps * base >= k_end) return kNone;
+                ent = ent_next;
+                ent_next = entry_of(base + 32u);
+                have = __ballot_sync(0xffffffffu, ent < a.c.pages);
+            }
+            const uint32_t b = (uint32_t)__ffs((int)have) - 1u;
+            have &= have - 1u;
+            const uint32_t e = __shfl_sync(0xffffffffu, ent, (int)b), c = first + kWarps * (base + b);
+            if (lane == 0u) {
+                const uint32_t row = ((head0 + e * a.c.kv_heads) << a.c.page_log2) + ((c & ((1u << page_chunks) - 1u)) << 4);
+                const uint32_t dst = ring + slot_in * kSlot;
+                mbar_arrive_expect_tx(full + slot_in, kSlot);
+                load_rows(dst, &a.kmap, row, full + slot_in);
+                load_rows(dst + kSlot / 2u, &a.vmap, row, full + slot_in);
+            }
+            if (++slot_in == kStages) slot_in = 0u;
+            return c;
+        };
+        uint32_t chunk[kStages];          // on their way; kNone: nothing more
+#pragma unroll
+        for (uint32_t i = 0; i < kStages; ++i) chunk[i] = issue();
+
         uint64_t o[NT][8][2];             // dimensions 16 j + g and 16 j + g + 8: columns 2 t and 2 t + 1
         float m[NT][2], l[NT][2];
 #pragma unroll
@@ -215,8 +236,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = 0ull;
         }
-        const uint32_t koff = (lane & 15u) * 128u, kx = (lane >> 4) ^ (lane & 7u);
-        const uint32_t vkey = (lane & 7u) + 8u * (lane >> 4), voff = 2u * kHalfChunk + vkey * 128u, vx = ((lane >> 3) & 1u) ^ (lane & 7u);
         while (ok && chunk[0] != kNone) {
             const uint32_t key = chunk[0] * kChunk;
             ok = __all_sync(0xffffffffu, mbar_wait(full + slot, phase, &sm.err));
@@ -226,22 +245,21 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
             // two sums, so that the products wait for one another half as long
             float y[NT][4], y2[NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = y2[nt][0] = y2[nt][1] = y2[nt][2] = y2[nt][3] = 0.f;
-#pragma unroll
             for (uint32_t st = 0; st < 4u; ++st) {
                 uint32_t ka[4], kb[4];
-                load_matrices(ka, in + koff + ((kx ^ (2u * st)) << 4));
-                load_matrices(kb, in + kHalfChunk + koff + ((kx ^ (2u * st)) << 4));
+                load_matrices(ka, in + koff[st]);
+                load_matrices(kb, in + kHalfChunk + koff[st]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    mma<BF>(y[nt], ka, qf[nt][st][0], qf[nt][st][1]);
-                    mma<BF>(y2[nt], kb, qf[nt][4 + st][0], qf[nt][4 + st][1]);
+                    if (st == 0u) {
+                        mma_first<BF>(y[nt], ka, qf[nt][0][0], qf[nt][0][1]);
+                        mma_first<BF>(y2[nt], kb, qf[nt][4][0], qf[nt][4][1]);
+                    } else {
+                        mma<BF>(y[nt], ka, qf[nt][st][0], qf[nt][st][1]);
+                        mma<BF>(y2[nt], kb, qf[nt][4 + st][0], qf[nt][4 + st][1]);
+                    }
                 }
             }
-            // the slot that the last chunk left, which every lane is done with, takes the next copies meanwhile
-#pragma unroll
-            for (uint32_t i = 0; i + 1u < kStages; ++i) chunk[i] = chunk[i + 1u];
-            chunk[kStages - 2u] = issue();
             // scores: positions key + g (elements 0, 1) and key + g + 8 (2, 3), columns 2 t and 2 t + 1
             const bool masked = key + kChunk - 1u > open;   // some row does not see all of the chunk
             const uint32_t pa = key + g, pb = key + g + 8u;
@@ -249,11 +267,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    y[nt][e] = (y[nt][e] + y2[nt][e]) * kScoreScale;
-                    if (masked && (e < 2 ? pa : pb) > last[nt][e & 1]) y[nt][e] = -INFINITY;
-                    raise |= y[nt][e] > m[nt][e & 1] + kLazy;
-                }
+                for (int e = 0; e < 4; ++e) y[nt][e] = (y[nt][e] + y2[nt][e]) * kScoreScale;
+            if (masked)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if ((e < 2 ? pa : pb) > last[nt][e & 1]) y[nt][e] = -INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) raise |= y[nt][e] > m[nt][e & 1] + kLazy;
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -299,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 uint32_t va[4];           // dimensions 16 j + g (0, 2) and + 8 (1, 3); positions 2 t, 2 t + 1 (0, 1) and + 8 (2, 3)
-                load_matrices_t(va, in + (uint32_t)(j >> 2) * kHalfChunk + voff + ((vx ^ (2u * (uint32_t)(j & 3))) << 4));
+                load_matrices_t(va, in + (uint32_t)(j >> 2) * kHalfChunk + voff[j & 3]);
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -312,8 +336,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float x[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma<BF>(x, va, bl[nt][0], bl[nt][1]);
+                    float x[4];
+                    mma_first<BF>(x, va, bl[nt][0], bl[nt][1]);
                     mma<BF>(x, va, bh[nt][0], bh[nt][1]);
                     o[nt][j][0] = add2(o[nt][j][0], pair(x[0], x[1]));
                     o[nt][j][1] = add2(o[nt][j][1], pair(x[2], x[3]));
@@ -337,14 +361,19 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
                         }
                 }
             }
+            __syncwarp();                 // every lane is done with the slot
+#pragma unroll
+            for (uint32_t i = 0; i + 1u < kStages; ++i) chunk[i] = chunk[i + 1u];
+            chunk[kStages - 1u] = issue();
         }
         if (!ok) {                        // nothing of this warp is left in flight; the rest of its rows become NaN
 #pragma unroll
             for (uint32_t i = 0; i < kStages; ++i) {
+                if (chunk[i] == kNone) break;
                 const uint64_t t0 = global_ns();
-                while (slot != slot_in && !mbar_try_wait(full + slot, phase) && global_ns() - t0 < kWaitLimitNs) {
+                while (!mbar_try_wait(full + slot, phase) && global_ns() - t0 < kWaitLimitNs) {
                 }
-                if (slot != slot_in && ++slot == kStages) slot = 0u, phase ^= 1u;
+                if (++slot == kStages) slot = 0u, phase ^= 1u;
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __int_as_float(0x7fffffff);
@@ -522,9 +551,9 @@ cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtenso
     static_cast<AttnArgs &>(f) = a;
     f.kmap = kmap;
     f.vmap = vmap;
-    cudaError_t e = nt == 1   ? (bf ? launch_few_of<true, 1>(f, dev, sms, stream) : launch_few_of<false, 1>(f, dev, sms, stream))
-                    : nt == 2 ? (bf ? launch_few_of<true, 2>(f, dev, sms, stream) : launch_few_of<false, 2>(f, dev, sms, stream))
-                              : (bf ? launch_few_of<true, 4>(f, dev, sms, stream) : launch_few_of<false, 4>(f, dev, sms, stream));
+    f.keep = lanes_keep(a, 8u * (uint32_t)nt, kChunk);
+    const cudaError_t e = nt == 1 ? (bf ? launch_few_of<true, 1>(f, dev, sms, stream) : launch_few_of<false, 1>(f, dev, sms, stream))
+                                  : (bf ? launch_few_of<true, 2>(f, dev, sms, stream) : launch_few_of<false, 2>(f, dev, sms, stream));
     if (e != cudaSuccess) return e;
     const uint32_t rows = 8u * (uint32_t)nt, ctas = std::min((uint32_t)sms, kMaxCtas);
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * (((uint64_t)a.r.tokens * a.group + rows - 1) / rows);

@@ -71,6 +71,7 @@ struct PromptArgs : AttnArgs {
     CUtensorMap kmap, vmap;      // [2][rows of the pool][64] each
     CUtensorMap qmap;            // [2][token][head][64]
     uint32_t tokens_per_tile;
+    Divisor by_tile;             // by a unit's rows
     uint32_t wide;               // output rows lie on 32-byte boundaries
 };
 
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0u ? &a.qmap : lane == 1u ? &a.kmap : &a.vmap) : "memory");
     wait_predecessor(a.early);
     const uint32_t tile_rows = a.tokens_per_tile * a.group;      // of 128 in tensor memory
-    const Cut<kTileKeys> cut{a, (ONE ? 1u : 2u) * tile_rows};
+    const Cut<kTileKeys> cut{a, (ONE ? 1u : 2u) * tile_rows, a.by_tile};
     const Piece piece = find_piece<kTileKeys, kThreads / 32u>(cut, *reinterpret_cast<PieceSmem *>(kv), 2u, kWorth);
     fence_before();
     fence_async();
@@ -694,6 +695,8 @@ cudaError_t launch_prompt(const AttnArgs &a, const CUtensorMap &kmap, const CUte
     p.vmap = vmap;
     p.qmap = qmap;
     p.tokens_per_tile = kTileRows / a.group;
+    p.by_tile = divisor(tiles * p.tokens_per_tile * a.group);
+    p.keep = lanes_keep(a, tiles * p.tokens_per_tile * a.group, kTileKeys);
     p.wide = ((reinterpret_cast<uintptr_t>(a.out) | a.ldo * 2) & 31u) == 0;
     const cudaError_t e = tiles == 1 ? (bf ? launch_prompt_of<true, true>(p, dev, sms, stream) : launch_prompt_of<false, true>(p, dev, sms, stream))
                                      : (bf ? launch_prompt_of<true, false>(p, dev, sms, stream) : launch_prompt_of<false, false>(p, dev, sms, stream));

@@ -413,9 +413,9 @@ int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, uint32_t q_he
                           const uint32_t *d_ntok, const void *d_q, uint64_t ldq, void *d_out, uint64_t ldo, void *stream);
 
 /* How a call of these sizes would be run on the current device, for who measures
-   or tests it: the query rows of a KV head that a CTA takes at a time at most (8,
-   16 or 32: the form for few rows; 128 or 256: tensor-memory tiles of whole
-   tokens' rows, whose weights are rounded to 16 bits before they meet V). */
+   or tests it: the query rows of a KV head that a CTA takes at a time at most (8 or
+   16: the form for few rows; 128 or 256: tensor-memory tiles of whole tokens'
+   rows, whose weights are rounded to 16 bits before they meet V). */
 int atlas_cuda_paged_attn_form(const AtlasPaged *cache, uint32_t q_heads, uint32_t tokens, uint32_t *rows);
 
 /* Number of SMs / compute capability of `device`, or a negative code. */
