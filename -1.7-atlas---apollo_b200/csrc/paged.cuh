@@ -127,9 +127,10 @@ struct Cut {
         return q;
     }
     // `kept`: this lane's, where lanes keep them
-    __device__ __forceinline__ Seq open(uint32_t s, const Seq &kept) const
+    __device__ __forceinline__ Seq open(uint32_t s, const Seq &kept) const { return a.keep ? open_each(s, kept) : open(s); }
+    // the same for a sequence of each lane's own, where lanes keep them
+    __device__ __forceinline__ Seq open_each(uint32_t s, const Seq &kept) const
     {
-        if (!a.keep) return open(s);
         Seq q;
         q.p0 = __shfl_sync(0xffffffffu, kept.p0, (int)s);
         q.rows = __shfl_sync(0xffffffffu, kept.rows, (int)s);
@@ -156,7 +157,8 @@ struct Cut {
 
 // The piece of a CTA: it begins in unit (s, h, i), `skip` tiles of keys behind the unit's first one, and has `left` of them
 struct Piece {
-    uint64_t begin, each; // in the line of all; a CTA's share
+    uint64_t begin, each; // in the line of all; a CTA's share, or 0: pieces are of one unit, and
+    uint32_t behind;      // so many pieces of it come before this one
     uint32_t s, h, i, skip;
     uint64_t left;
     Seq kept;             // lane s has sequence s, where lanes keep them
@@ -188,18 +190,22 @@ __device__ __forceinline__ uint32_t up_to(uint32_t x)
     return x;
 }
 
-// This CTA's piece. All WARPS warps, each for itself where each lane can keep a sequence, else together through `sm`, which is
-// free again behind the call. Where there are no more units than CTAs, and the largest is at most `worth` longer than an
-// equal share, each unit is a piece (joining partial sums takes as long as `worth` tiles of keys); else a CTA takes
-// `least` tiles of keys at least.
+// Where units are no more than CTAs, and so many (of a KV head), they may be cut one by one
+constexpr uint32_t kPairSlots = 4, kMostPairs = 32 * kPairSlots;
+
+// This CTA's piece. All WARPS warps, each for itself where lanes keep the sequences, else together through `sm`, which is
+// free again behind the call. The line is cut into equal pieces of `least` tiles of keys at least; but units that are no
+// more than CTAs are cut one by one, if that makes the largest piece at most `cross` tiles longer (what passing from
+// unit to unit inside a piece costs), and left whole if that makes it at most `worth` longer (what joining partial sums costs).
 template <uint32_t KEYS, uint32_t WARPS>
-__device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, uint32_t least, uint32_t worth)
+__device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, uint32_t least, uint32_t worth, uint32_t cross)
 {
     const AttnArgs &a = cut.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = a.c.nseq;
     Piece p;
     p.s = p.h = p.i = p.skip = 0u;
-    p.begin = 0u;
+    p.begin = p.each = 0u;
+    p.behind = 0u;
     p.left = 0u;
     uint32_t most = 0u;
     // the unit of sequence p.s that place `rest` of a KV head's units is in
@@ -255,30 +261,87 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
         const uint32_t all_units = __reduce_add_sync(0xffffffffu, units) * a.c.kv_heads;
         const uint32_t line = n == 1u ? work * a.c.kv_heads : up_to(work * a.c.kv_heads);
         const uint32_t total = __shfl_sync(0xffffffffu, line, (int)n - 1);
-        uint32_t each = (total + gridDim.x - 1u) / gridDim.x;
-        const bool whole = all_units <= gridDim.x && most <= each + worth;
-        const uint32_t ends = whole ? (n == 1u ? all_units : up_to(units * a.c.kv_heads)) : line;
-        each = whole ? 1u : max(each, least);
+        const uint32_t each = max((total + gridDim.x - 1u) / gridDim.x, least);
+        if (all_units <= gridDim.x && all_units <= kMostPairs * a.c.kv_heads) {
+            // Units cut into pieces of their own, the shortest that are no more than CTAs. Lane l has the tiles of sequence and
+            // rows number l, l + 32, ..: (sequence, tile) and its work.
+            const uint32_t pairs_to = n == 1u ? units : up_to(units), pairs = __shfl_sync(0xffffffffu, pairs_to, (int)n - 1);
+            uint32_t seq[kPairSlots], tile[kPairSlots], cost[kPairSlots];
+#pragma unroll
+            for (uint32_t k = 0; k < kPairSlots; ++k) {
+                const uint32_t x = 32u * k + lane;
+                seq[k] = tile[k] = cost[k] = 0u;
+                if (32u * k >= pairs) break;
+                if (n > 1u)
+#pragma unroll
+                    for (uint32_t step = 16u; step; step >>= 1)
+                        if (__shfl_sync(0xffffffffu, pairs_to, (int)(seq[k] + step - 1u)) <= x) seq[k] += step;
+                seq[k] = min(seq[k], n - 1u);
+                const uint32_t upto = __shfl_sync(0xffffffffu, pairs_to, (int)seq[k]), own = __shfl_sync(0xffffffffu, units, (int)seq[k]);
+                const Seq q = cut.open_each(seq[k], p.kept);
+                tile[k] = x - (upto - own);
+                if (x < pairs) cost[k] = cut.cost(q, tile[k]);
+            }
+            auto count = [&](uint32_t size) {     // CTAs for pieces of that size
+                uint32_t c = 0u;
+#pragma unroll
+                for (uint32_t k = 0; k < kPairSlots; ++k)
+                    if (32u * k < pairs) c += (cost[k] + size - 1u) / size;
+                return __reduce_add_sync(0xffffffffu, c) * a.c.kv_heads;
+            };
+            // between an equal share and the largest unit; one less than a piece per unit is lost to rounding up
+            uint32_t size = most;
+            if (most > each + worth) {
+                uint32_t low = each;
+                size = min(most, max(each, all_units < gridDim.x ? total / (gridDim.x - all_units) + 1u : most));
+                for (uint32_t i = 0; i < 5u && low < size; ++i) {
+                    const uint32_t mid = (low + size) >> 1;
+                    if (count(mid) <= gridDim.x) size = mid;
+                    else low = mid + 1u;
+                }
+                if (size + worth >= most) size = most;
+            }
+            // as long as the line's pieces take, with what joining costs either
+            if (size == most ? most <= each + cross + worth : size <= each + cross) {
+                uint32_t at = blockIdx.x;
+#pragma unroll
+                for (uint32_t k = 0; k < kPairSlots; ++k) {
+                    if (32u * k >= pairs) break;
+                    const uint32_t cuts = (cost[k] + size - 1u) / size, ends = up_to(cuts * a.c.kv_heads), all = __shfl_sync(0xffffffffu, ends, 31);
+                    if (at >= all) {
+                        at -= all;
+                        continue;
+                    }
+                    const int l = __ffs((int)__ballot_sync(0xffffffffu, ends > at)) - 1;
+                    const uint32_t own_cuts = __shfl_sync(0xffffffffu, cuts, l), c = __shfl_sync(0xffffffffu, cost[k], l);
+                    at -= __shfl_sync(0xffffffffu, ends, l) - own_cuts * a.c.kv_heads;
+                    p.s = __shfl_sync(0xffffffffu, seq[k], l);
+                    p.i = __shfl_sync(0xffffffffu, tile[k], l);
+                    p.h = at / own_cuts;
+                    p.behind = at - p.h * own_cuts;
+                    // as even as can be
+                    const uint32_t even = c / own_cuts, more = c - even * own_cuts;
+                    p.skip = p.behind * even + min(p.behind, more);
+                    p.left = even + (p.behind < more ? 1u : 0u);
+                    break;
+                }
+                return p;
+            }
+        }
         p.each = each;
-        const uint32_t at = each * blockIdx.x, end = whole ? all_units : total;
-        if (at >= end) return p;
+        const uint32_t at = each * blockIdx.x;
+        if (at >= total) return p;
         uint32_t before = 0u;
         if (n > 1u) {
-            p.s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, lane < n && ends > at)) - 1u;
-            before = __shfl_sync(0xffffffffu, ends, p.s ? (int)p.s - 1 : 0);
+            p.s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, lane < n && line > at)) - 1u;
+            before = __shfl_sync(0xffffffffu, line, p.s ? (int)p.s - 1 : 0);
             if (p.s == 0u) before = 0u;
         }
-        const uint32_t of_head = __shfl_sync(0xffffffffu, whole ? units : work, (int)p.s);
+        const uint32_t of_head = __shfl_sync(0xffffffffu, work, (int)p.s);
         p.h = (at - before) / of_head;
-        const uint32_t rest = at - before - of_head * p.h;
-        if (whole) {
-            p.i = rest;
-            p.left = cut.cost(cut.open(p.s, p.kept), p.i);
-        } else {
-            p.begin = at;
-            p.left = min(each, end - at);
-            unit_at(rest);
-        }
+        p.begin = at;
+        p.left = min(each, total - at);
+        unit_at(at - before - of_head * p.h);
         return p;
     }
     for (uint32_t s = warp; s < n; s += WARPS) {
@@ -414,9 +477,13 @@ struct Walk {
         Part r{};
         r.first = ~0u;
         if (p.left && !head && cut.cost(q, p.i) - p.skip <= p.left) {
-            const uint64_t unit = p.begin - p.skip;
-            const uint32_t c = (uint32_t)quotient(unit, p.each);
-            r.first = 2u * c + (unit == p.each * c ? 0u : 1u);
+            uint32_t c = blockIdx.x - p.behind;
+            r.first = 2u * c;
+            if (p.each) {
+                const uint64_t unit = p.begin - p.skip;
+                c = (uint32_t)quotient(unit, p.each);
+                r.first = 2u * c + (unit == p.each * c ? 0u : 1u);
+            }
             r.count = blockIdx.x - c + 1u;
             r.s = p.s;
             r.h = p.h;
@@ -450,7 +517,7 @@ inline bool lanes_keep(const AttnArgs &a, uint32_t tile, uint32_t keys)
 // Whatever the positions, each unit will be a piece of its own (find_piece): a sequence has room for no more
 inline bool always_whole(const AttnArgs &a, uint64_t units, uint32_t ctas, uint32_t keys, uint32_t worth)
 {
-    return units <= ctas && (a.c.limit + keys - 1u) / keys <= worth;
+    return units <= ctas && (!a.keep || units <= (uint64_t)kMostPairs * a.c.kv_heads) && (a.c.limit + keys - 1u) / keys <= worth;
 }
 
 }  // namespace

@@ -40,7 +40,7 @@ namespace {
 constexpr uint32_t kChunk = 16, kWarps = 12, kThreads = kWarps * 32, kStages = 2;
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
-constexpr uint32_t kWorth = 64;               // chunks: what joining partial sums takes
+constexpr uint32_t kWorth = 64, kCross = 40;      // chunks: what joining partial sums takes, and passing to another unit
 constexpr float kLazy = 6.0f;
 // Weights are 2^(score - maximum + kUnit). binary16: their largest, 2^15, keeps the low term's bits; bfloat16 has fp32's
 // range, and small weights leave the sums of large values room
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     __syncthreads();
     wait_predecessor(a.early);
     const Cut<kChunk> cut{a, R, Divisor{1u << 31, NT == 1 ? 3u : 4u}};
-    const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, kWarps, kWorth);
+    const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, kWarps, kWorth, kCross);
     Walk<kChunk> w(cut, piece);
     if (!a.keep) {                        // the ring's place is free
         fence_ring();
@@ -441,50 +441,51 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 // --------------------------------------------------------- partial sums ----
 //
 // The units that pieces cut: the CTAs whose number is that of the piece that a
-// unit ends in join its records, two rows a warp (lane: a record's maximum and
-// sum, then 4 dimensions), with the first records' loads on their way before
+// unit ends in join its records, a warp one or two rows (lane: a record's maximum
+// and sum, then 4 dimensions), with the first records' loads on their way before
 // their weights are known. Bound by latency; a call whose pieces are whole units
 // leaves nothing to join.
 struct MergeArgs : AttnArgs {
     uint32_t tile;                        // rows of a record
 };
 
-constexpr uint32_t kMergeWarps = 8, kMergeRows = 2, kAhead = 4;
+constexpr uint32_t kMergeWarps = 8;
 
-template <bool BF>
+// ROWS a warp, AHEAD records on their way: few rows have many records, many rows few
+template <bool BF, uint32_t ROWS, uint32_t AHEAD>   // AHEAD divides 32
 __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __grid_constant__ MergeArgs a)
 {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     wait_predecessor(a.early);
     const uint4 lo = __ldcg(reinterpret_cast<const uint4 *>(a.parts) + 2u * blockIdx.x), hi = __ldcg(reinterpret_cast<const uint4 *>(a.parts) + 2u * blockIdx.x + 1u);
     const uint32_t first = lo.x, count = lo.y, s = lo.z, h = lo.w, row0 = hi.x, rows = hi.y;
-    const uint32_t r0 = (blockIdx.y * kMergeWarps + warp) * kMergeRows;
+    const uint32_t r0 = (blockIdx.y * kMergeWarps + warp) * ROWS;
     if (first == ~0u || r0 >= rows) return;
     // record i of the unit
     auto record = [&](uint32_t i) { return record_of(a, i ? 2u * (first / 2u + i) : first, a.tile); };
-    float M[kMergeRows], L[kMergeRows], f[kMergeRows];   // f: record b + lane's factor
-    float4 x[kMergeRows], y[kMergeRows][kAhead];
+    float M[ROWS], L[ROWS], f[ROWS];   // f: record b + lane's factor
+    float4 x[ROWS], y[ROWS][AHEAD];
     auto load = [&](uint32_t i0) {
 #pragma unroll
-        for (uint32_t u = 0; u < kMergeRows; ++u)
+        for (uint32_t u = 0; u < ROWS; ++u)
 #pragma unroll
-            for (uint32_t i = 0; i < kAhead; ++i)
+            for (uint32_t i = 0; i < AHEAD; ++i)
                 if (i0 + i < count) y[u][i] = __ldcg(reinterpret_cast<const float4 *>(record(i0 + i)) + min(r0 + u, rows - 1u) * (kDim / 4u) + lane);
     };
     load(0u);
 #pragma unroll
-    for (uint32_t u = 0; u < kMergeRows; ++u) {
+    for (uint32_t u = 0; u < ROWS; ++u) {
         M[u] = -INFINITY;
         L[u] = 0.f;
         x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     for (uint32_t b = 0; b < count; b += 32u) {
-        float2 ml[kMergeRows];
+        float2 ml[ROWS];
 #pragma unroll
-        for (uint32_t u = 0; u < kMergeRows; ++u)
+        for (uint32_t u = 0; u < ROWS; ++u)
             ml[u] = b + lane < count ? __ldcg(reinterpret_cast<const float2 *>(record(b + lane) + a.tile * kDim) + min(r0 + u, rows - 1u)) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (uint32_t u = 0; u < kMergeRows; ++u) {
+        for (uint32_t u = 0; u < ROWS; ++u) {
             float most = ml[u].x;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -499,11 +500,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __gr
             x[u] = make_float4(x[u].x * before, x[u].y * before, x[u].z * before, x[u].w * before);
         }
         const uint32_t n = min(count - b, 32u);
-        for (uint32_t i0 = 0; i0 < n; i0 += kAhead) {
+        for (uint32_t i0 = 0; i0 < n; i0 += AHEAD) {
 #pragma unroll
-            for (uint32_t u = 0; u < kMergeRows; ++u)
+            for (uint32_t u = 0; u < ROWS; ++u)
 #pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i) {
+                for (uint32_t i = 0; i < AHEAD; ++i) {
                     const float fi = __shfl_sync(0xffffffffu, f[u], (int)(i0 + i));
                     if (i0 + i >= n) continue;
                     x[u].x = fmaf(fi, y[u][i].x, x[u].x);
@@ -511,11 +512,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __gr
                     x[u].z = fmaf(fi, y[u][i].z, x[u].z);
                     x[u].w = fmaf(fi, y[u][i].w, x[u].w);
                 }
-            load(b + i0 + kAhead);
+            load(b + i0 + AHEAD);
         }
     }
 #pragma unroll
-    for (uint32_t u = 0; u < kMergeRows; ++u) {
+    for (uint32_t u = 0; u < ROWS; ++u) {
         if (r0 + u >= rows) break;
         const float inv = L[u] == 0.f ? 0.f : 1.0f / L[u];
         const uint32_t row = row0 + r0 + u, tok = row / a.group;
@@ -538,9 +539,15 @@ cudaError_t launch_merge(const AttnArgs &a, bool bf, uint32_t rows, uint32_t cta
     MergeArgs m{};
     static_cast<AttnArgs &>(m) = a;
     m.tile = rows;
-    const dim3 grid(ctas, (rows + kMergeWarps * kMergeRows - 1) / (kMergeWarps * kMergeRows));
-    return bf ? k8::launch(part_merge_kernel<true>, grid, kMergeWarps * 32, 0, 1, m, sms, stream)
-              : k8::launch(part_merge_kernel<false>, grid, kMergeWarps * 32, 0, 1, m, sms, stream);
+    const uint32_t threads = kMergeWarps * 32;
+    if (rows <= 16) {
+        const dim3 grid(ctas, (rows + kMergeWarps - 1) / kMergeWarps);
+        return bf ? k8::launch(part_merge_kernel<true, 1, 8>, grid, threads, 0, 1, m, sms, stream)
+                  : k8::launch(part_merge_kernel<false, 1, 8>, grid, threads, 0, 1, m, sms, stream);
+    }
+    const dim3 grid(ctas, (rows + 2 * kMergeWarps - 1) / (2 * kMergeWarps));
+    return bf ? k8::launch(part_merge_kernel<true, 2, 4>, grid, threads, 0, 1, m, sms, stream)
+              : k8::launch(part_merge_kernel<false, 2, 4>, grid, threads, 0, 1, m, sms, stream);
 }
 
 // The few-rows form, for units of 8 nt rows; maps: see FewArgs
@@ -557,7 +564,7 @@ cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtenso
     if (e != cudaSuccess) return e;
     const uint32_t rows = 8u * (uint32_t)nt, ctas = std::min((uint32_t)sms, kMaxCtas);
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * (((uint64_t)a.r.tokens * a.group + rows - 1) / rows);
-    if (always_whole(a, units, ctas, kChunk, kWorth)) return cudaSuccess;
+    if (always_whole(f, units, ctas, kChunk, kWorth)) return cudaSuccess;
     return launch_merge(a, bf, rows, ctas, sms, stream);
 }
 
