@@ -190,14 +190,12 @@ __device__ __forceinline__ uint32_t up_to(uint32_t x)
     return x;
 }
 
-// Where units are no more than CTAs, and so many (of a KV head), they may be cut one by one
-constexpr uint32_t kPairSlots = 4, kMostPairs = 32 * kPairSlots;
-
 // This CTA's piece. All WARPS warps, each for itself where lanes keep the sequences, else together through `sm`, which is
 // free again behind the call. The line is cut into equal pieces of `least` tiles of keys at least; but units that are no
 // more than CTAs are cut one by one, if that makes the largest piece at most `cross` tiles longer (what passing from
 // unit to unit inside a piece costs), and left whole if that makes it at most `worth` longer (what joining partial sums costs).
-template <uint32_t KEYS, uint32_t WARPS>
+// Of a KV head, at most 32 SLOTS units can be cut one by one.
+template <uint32_t KEYS, uint32_t WARPS, uint32_t SLOTS>
 __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, uint32_t least, uint32_t worth, uint32_t cross)
 {
     const AttnArgs &a = cut.a;
@@ -262,50 +260,48 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
         const uint32_t line = n == 1u ? work * a.c.kv_heads : up_to(work * a.c.kv_heads);
         const uint32_t total = __shfl_sync(0xffffffffu, line, (int)n - 1);
         const uint32_t each = max((total + gridDim.x - 1u) / gridDim.x, least);
-        if (all_units <= gridDim.x && all_units <= kMostPairs * a.c.kv_heads) {
-            // Units cut into pieces of their own, the shortest that are no more than CTAs. Lane l has the tiles of sequence and
-            // rows number l, l + 32, ..: (sequence, tile) and its work.
-            const uint32_t pairs_to = n == 1u ? units : up_to(units), pairs = __shfl_sync(0xffffffffu, pairs_to, (int)n - 1);
-            uint32_t seq[kPairSlots], tile[kPairSlots], cost[kPairSlots];
+        if (all_units <= gridDim.x && all_units <= 32u * SLOTS * a.c.kv_heads) {
+            // Units cut into pieces of their own. Lane l has the tiles of sequence and rows number l, l + 32, ..: (sequence,
+            // tile) and its work.
+            uint32_t seq[SLOTS], tile[SLOTS], cost[SLOTS], pairs = n;
+            const bool single = __all_sync(0xffffffffu, units <= 1u);
 #pragma unroll
-            for (uint32_t k = 0; k < kPairSlots; ++k) {
-                const uint32_t x = 32u * k + lane;
-                seq[k] = tile[k] = cost[k] = 0u;
-                if (32u * k >= pairs) break;
-                if (n > 1u)
+            for (uint32_t k = 0; k < SLOTS; ++k) seq[k] = tile[k] = cost[k] = 0u;
+            if (single) {
+                seq[0] = lane;
+                cost[0] = work;
+            } else {
+                const uint32_t pairs_to = n == 1u ? units : up_to(units);
+                pairs = __shfl_sync(0xffffffffu, pairs_to, (int)n - 1);
 #pragma unroll
-                    for (uint32_t step = 16u; step; step >>= 1)
-                        if (__shfl_sync(0xffffffffu, pairs_to, (int)(seq[k] + step - 1u)) <= x) seq[k] += step;
-                seq[k] = min(seq[k], n - 1u);
-                const uint32_t upto = __shfl_sync(0xffffffffu, pairs_to, (int)seq[k]), own = __shfl_sync(0xffffffffu, units, (int)seq[k]);
-                const Seq q = cut.open_each(seq[k], p.kept);
-                tile[k] = x - (upto - own);
-                if (x < pairs) cost[k] = cut.cost(q, tile[k]);
+                for (uint32_t k = 0; k < SLOTS; ++k) {
+                    const uint32_t x = 32u * k + lane;
+                    if (32u * k >= pairs) break;
+                    if (n > 1u)
+#pragma unroll
+                        for (uint32_t step = 16u; step; step >>= 1)
+                            if (__shfl_sync(0xffffffffu, pairs_to, (int)(seq[k] + step - 1u)) <= x) seq[k] += step;
+                    seq[k] = min(seq[k], n - 1u);
+                    const uint32_t upto = __shfl_sync(0xffffffffu, pairs_to, (int)seq[k]), own = __shfl_sync(0xffffffffu, units, (int)seq[k]);
+                    const Seq q = cut.open_each(seq[k], p.kept);
+                    tile[k] = x - (upto - own);
+                    if (x < pairs) cost[k] = cut.cost(q, tile[k]);
+                }
             }
-            auto count = [&](uint32_t size) {     // CTAs for pieces of that size
-                uint32_t c = 0u;
-#pragma unroll
-                for (uint32_t k = 0; k < kPairSlots; ++k)
-                    if (32u * k < pairs) c += (cost[k] + size - 1u) / size;
-                return __reduce_add_sync(0xffffffffu, c) * a.c.kv_heads;
-            };
-            // between an equal share and the largest unit; one less than a piece per unit is lost to rounding up
+            // The pieces' size: sum ceil(work / size) <= CTAs holds where size >= total / (CTAs - units), as rounding up adds
+            // less than one a unit, and where every unit gets as many pieces as the largest one
             uint32_t size = most;
             if (most > each + worth) {
-                uint32_t low = each;
-                size = min(most, max(each, all_units < gridDim.x ? total / (gridDim.x - all_units) + 1u : most));
-                for (uint32_t i = 0; i < 5u && low < size; ++i) {
-                    const uint32_t mid = (low + size) >> 1;
-                    if (count(mid) <= gridDim.x) size = mid;
-                    else low = mid + 1u;
-                }
+                size = (most + gridDim.x / all_units - 1u) / (gridDim.x / all_units);
+                if (all_units < gridDim.x) size = min(size, total / (gridDim.x - all_units) + 1u);
+                size = max(size, least);
                 if (size + worth >= most) size = most;
             }
             // as long as the line's pieces take, with what joining costs either
             if (size == most ? most <= each + cross + worth : size <= each + cross) {
                 uint32_t at = blockIdx.x;
 #pragma unroll
-                for (uint32_t k = 0; k < kPairSlots; ++k) {
+                for (uint32_t k = 0; k < SLOTS; ++k) {
                     if (32u * k >= pairs) break;
                     const uint32_t cuts = (cost[k] + size - 1u) / size, ends = up_to(cuts * a.c.kv_heads), all = __shfl_sync(0xffffffffu, ends, 31);
                     if (at >= all) {
@@ -515,9 +511,9 @@ inline bool lanes_keep(const AttnArgs &a, uint32_t tile, uint32_t keys)
 }
 
 // Whatever the positions, each unit will be a piece of its own (find_piece): a sequence has room for no more
-inline bool always_whole(const AttnArgs &a, uint64_t units, uint32_t ctas, uint32_t keys, uint32_t worth)
+inline bool always_whole(const AttnArgs &a, uint64_t units, uint32_t ctas, uint32_t keys, uint32_t worth, uint32_t slots)
 {
-    return units <= ctas && (!a.keep || units <= (uint64_t)kMostPairs * a.c.kv_heads) && (a.c.limit + keys - 1u) / keys <= worth;
+    return units <= ctas && (!a.keep || units <= 32ull * slots * a.c.kv_heads) && (a.c.limit + keys - 1u) / keys <= worth;
 }
 
 }  // namespace

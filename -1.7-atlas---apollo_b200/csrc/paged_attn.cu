@@ -40,7 +40,7 @@ namespace {
 constexpr uint32_t kChunk = 16, kWarps = 12, kThreads = kWarps * 32, kStages = 2;
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
-constexpr uint32_t kWorth = 64, kCross = 40;      // chunks: what joining partial sums takes, and passing to another unit
+constexpr uint32_t kSlots = 1, kWorth = 64, kCross = 40;      // chunks: what joining partial sums takes, and passing to another unit
 constexpr float kLazy = 6.0f;
 // Weights are 2^(score - maximum + kUnit). binary16: their largest, 2^15, keeps the low term's bits; bfloat16 has fp32's
 // range, and small weights leave the sums of large values room
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     __syncthreads();
     wait_predecessor(a.early);
     const Cut<kChunk> cut{a, R, Divisor{1u << 31, NT == 1 ? 3u : 4u}};
-    const Piece piece = find_piece<kChunk, kWarps>(cut, sm.u.piece, kWarps, kWorth, kCross);
+    const Piece piece = find_piece<kChunk, kWarps, kSlots>(cut, sm.u.piece, kWarps, kWorth, kCross);
     Walk<kChunk> w(cut, piece);
     if (!a.keep) {                        // the ring's place is free
         fence_ring();
@@ -173,10 +173,15 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         const uint32_t k_end = min(w.k_end, seen), first = w.k_begin + warp;
         const int32_t *const entries = a.c.table + (size_t)s * a.c.max_pages;
         const uint32_t page_chunks = a.c.page_log2 - 4u;           // log2 of chunks per page
+        const uint32_t head0 = a.layer * a.c.pages * a.c.kv_heads + h;
+        // the pages of this warp's chunks first + kWarps (base + lane), and of the next 32; their loads are on their way first
+        auto entry_of = [&](uint32_t base) {
+            const uint32_t c = first + kWarps * (base + lane);
+            return c < k_end ? (uint32_t)__ldcg(entries + (c >> page_chunks)) : ~0u;
+        };
+        uint32_t base = 0u, ent = entry_of(0u), ent_next = entry_of(32u);
         // B operands: column g, dimensions 16 st + 2 t, + 1, + 8, + 9
         uint32_t qf[NT][8][2];
-        uint32_t last[NT][2];             // the last position that columns 2 t and 2 t + 1 see
-        const uint32_t open = (uint32_t)min(p0 + tr.tok, (uint64_t)0x7fffffffu);   // every row sees the positions up to it
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const uint32_t i = 8u * (uint32_t)nt + g;
@@ -187,20 +192,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
                 qf[nt][st][0] = __ldcg(src + 8 * st + t);
                 qf[nt][st][1] = __ldcg(src + 8 * st + 4 + t);
             }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint32_t r = 8u * (uint32_t)nt + 2u * t + (uint32_t)e;
-                last[nt][e] = r < rows ? (uint32_t)min(p0 + tr.at(r).x, (uint64_t)0x7fffffffu) : open;
-            }
         }
-
-        const uint32_t head0 = a.layer * a.c.pages * a.c.kv_heads + h;
-        // the entries of this warp's chunks first + kWarps (base + lane), and the next 32
-        auto entry_of = [&](uint32_t base) {
-            const uint32_t c = first + kWarps * (base + lane);
-            return c < k_end ? (uint32_t)__ldcg(entries + (c >> page_chunks)) : ~0u;
-        };
-        uint32_t base = 0u, ent = entry_of(0u), ent_next = entry_of(32u), have = __ballot_sync(0xffffffffu, ent < a.c.pages);
+        uint32_t have = __ballot_sync(0xffffffffu, ent < a.c.pages);
         // the next chunk of this warp's that has a page; its copies are issued into the next slot
         auto issue = [&]() -> uint32_t {
             while (!have) {
@@ -226,6 +219,16 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         uint32_t chunk[kStages];          // on their way; kNone: nothing more
 #pragma unroll
         for (uint32_t i = 0; i < kStages; ++i) chunk[i] = issue();
+
+        uint32_t last[NT][2];             // the last position that columns 2 t and 2 t + 1 see
+        const uint32_t open = (uint32_t)min(p0 + tr.tok, (uint64_t)0x7fffffffu);   // every row sees the positions up to it
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t r = 8u * (uint32_t)nt + 2u * t + (uint32_t)e;
+                last[nt][e] = r < rows ? (uint32_t)min(p0 + tr.at(r).x, (uint64_t)0x7fffffffu) : open;
+            }
 
         uint64_t o[NT][8][2];             // dimensions 16 j + g and 16 j + g + 8: columns 2 t and 2 t + 1
         float m[NT][2], l[NT][2];
@@ -452,9 +455,10 @@ struct MergeArgs : AttnArgs {
 constexpr uint32_t kMergeWarps = 8;
 
 // ROWS a warp, AHEAD records on their way: few rows have many records, many rows few
-template <bool BF, uint32_t ROWS, uint32_t AHEAD>   // AHEAD divides 32
+template <bool BF, uint32_t ROWS, uint32_t AHEAD>
 __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __grid_constant__ MergeArgs a)
 {
+    static_assert(32u % AHEAD == 0u, "the records of a round are loaded whole");
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     wait_predecessor(a.early);
     const uint4 lo = __ldcg(reinterpret_cast<const uint4 *>(a.parts) + 2u * blockIdx.x), hi = __ldcg(reinterpret_cast<const uint4 *>(a.parts) + 2u * blockIdx.x + 1u);
@@ -564,7 +568,7 @@ cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtenso
     if (e != cudaSuccess) return e;
     const uint32_t rows = 8u * (uint32_t)nt, ctas = std::min((uint32_t)sms, kMaxCtas);
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * (((uint64_t)a.r.tokens * a.group + rows - 1) / rows);
-    if (always_whole(f, units, ctas, kChunk, kWorth)) return cudaSuccess;
+    if (always_whole(f, units, ctas, kChunk, kWorth, kSlots)) return cudaSuccess;
     return launch_merge(a, bf, rows, ctas, sms, stream);
 }
 

@@ -60,7 +60,7 @@ static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "what the softma
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 values, swizzled
 constexpr uint32_t kTile = 2 * kHalf;
 constexpr uint32_t kMaxStages = 6;
-constexpr uint32_t kWorth = 4, kCross = 2;         // tiles of keys: what joining partial sums takes, and passing to another unit
+constexpr uint32_t kSlots = 4, kWorth = 4, kCross = 2;        // tiles of keys: what joining partial sums takes, and passing to another unit
 constexpr float kLazy = 8.0f;
 // Weights are 2^(score - maximum + kUnit): binary16 keeps 24 bits below the largest; bfloat16 has fp32's range, and small
 // weights leave the sums of large values room
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     wait_predecessor(a.early);
     const uint32_t tile_rows = a.tokens_per_tile * a.group;      // of 128 in tensor memory
     const Cut<kTileKeys> cut{a, (ONE ? 1u : 2u) * tile_rows, a.by_tile};
-    const Piece piece = find_piece<kTileKeys, kThreads / 32u>(cut, *reinterpret_cast<PieceSmem *>(kv), 2u, kWorth, kCross);
+    const Piece piece = find_piece<kTileKeys, kThreads / 32u, kSlots>(cut, *reinterpret_cast<PieceSmem *>(kv), 2u, kWorth, kCross);
     fence_before();
     fence_async();
     __syncthreads();
@@ -703,7 +703,7 @@ cudaError_t launch_prompt(const AttnArgs &a, const CUtensorMap &kmap, const CUte
     if (e != cudaSuccess) return e;
     const uint32_t ctas = std::min((uint32_t)sms, kMaxCtas), per = tiles * p.tokens_per_tile;
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * ((a.r.tokens + per - 1) / per);
-    if (always_whole(p, units, ctas, kTileKeys, kWorth)) return cudaSuccess;
+    if (always_whole(p, units, ctas, kTileKeys, kWorth, kSlots)) return cudaSuccess;
     return launch_merge(a, bf, tiles * kTileRows, ctas, sms, stream);
 }
 
