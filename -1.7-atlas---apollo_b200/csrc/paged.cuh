@@ -75,8 +75,9 @@ struct Seq {
 // Up to this many sequences, each lane of a warp keeps one's Seq (where the line has less than 2^31 tiles of keys)
 constexpr uint32_t kKeptSeqs = 32;
 
-// How a call's rows are cut into tiles of `tile` rows
-template <uint32_t KEYS>
+// How a call's rows are cut into tiles of `tile` rows. Beginning and ending a unit takes as long as EXTRA tiles of keys: in the
+// line, each unit has that many places before its tiles of keys.
+template <uint32_t KEYS, uint32_t EXTRA>
 struct Cut {
     const AttnArgs &a;
     const uint32_t tile;  // query rows of a unit
@@ -145,7 +146,7 @@ struct Cut {
         uint32_t m = 0u;
         for (uint32_t i = lane; i < n; i += 32u) {
             const uint32_t c = cost(q, i);
-            sum += c;
+            sum += c + EXTRA;
             m = max(m, c);
         }
 #pragma unroll
@@ -192,11 +193,11 @@ __device__ __forceinline__ uint32_t up_to(uint32_t x)
 
 // This CTA's piece. All WARPS warps, each for itself where lanes keep the sequences, else together through `sm`, which is
 // free again behind the call. The line is cut into equal pieces of `least` tiles of keys at least; but units that are no
-// more than CTAs are cut one by one, if that makes the largest piece at most `cross` tiles longer (what passing from
-// unit to unit inside a piece costs), and left whole if that makes it at most `worth` longer (what joining partial sums costs).
+// more than CTAs are cut one by one if no piece gets longer than that, and left whole if none gets more than `worth`
+// tiles longer (what joining partial sums costs).
 // Of a KV head, at most 32 SLOTS units can be cut one by one.
-template <uint32_t KEYS, uint32_t WARPS, uint32_t SLOTS>
-__device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm, uint32_t least, uint32_t worth, uint32_t cross)
+template <uint32_t WARPS, uint32_t SLOTS, uint32_t KEYS, uint32_t EXTRA>
+__device__ __forceinline__ Piece find_piece(const Cut<KEYS, EXTRA> &cut, PieceSmem &sm, uint32_t least, uint32_t worth)
 {
     const AttnArgs &a = cut.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = a.c.nseq;
@@ -211,18 +212,23 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
         using T = decltype(rest);
         const Seq q = cut.open(p.s, p.kept);
         const uint32_t units = cut.units(q);
+        // a place in the unit -> tiles of keys before it; what lies before the first one is not work
+        auto enter = [&](uint32_t place) {
+            p.skip = place > EXTRA ? place - EXTRA : 0u;
+            if (place < EXTRA) p.left -= min(p.left, (uint64_t)(EXTRA - place));
+        };
         if (units == 1u) {
-            p.skip = (uint32_t)rest;
+            enter((uint32_t)rest);
             return;
         }
         for (uint32_t b = 0;; b += 32u) {
-            const uint32_t c = b + lane < units ? cut.cost(q, b + lane) : 0u;
+            const uint32_t c = b + lane < units ? cut.cost(q, b + lane) + EXTRA : 0u;
             const T x = up_to((T)c);
             const uint32_t past = __ballot_sync(0xffffffffu, x > rest);
             if (past || b + 32u >= units) {
                 const uint32_t at = past ? (uint32_t)__ffs((int)past) - 1u : 31u;
                 p.i = min(b + at, units - 1u);
-                p.skip = (uint32_t)(rest - __shfl_sync(0xffffffffu, x - c, (int)at));
+                enter((uint32_t)(rest - __shfl_sync(0xffffffffu, x - c, (int)at)));
                 return;
             }
             rest -= __shfl_sync(0xffffffffu, x, 31);
@@ -245,7 +251,7 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
         if (__all_sync(0xffffffffu, units <= 4u)) {
             for (uint32_t i = 0; i < units; ++i) {
                 const uint32_t c = cut.cost(p.kept, i);
-                work += c;
+                work += c + EXTRA;
                 most = max(most, c);
             }
             most = __reduce_max_sync(0xffffffffu, most);
@@ -269,7 +275,7 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
             for (uint32_t k = 0; k < SLOTS; ++k) seq[k] = tile[k] = cost[k] = 0u;
             if (single) {
                 seq[0] = lane;
-                cost[0] = work;
+                cost[0] = units ? work - EXTRA : 0u;
             } else {
                 const uint32_t pairs_to = n == 1u ? units : up_to(units);
                 pairs = __shfl_sync(0xffffffffu, pairs_to, (int)n - 1);
@@ -293,12 +299,11 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
             uint32_t size = most;
             if (most > each + worth) {
                 size = (most + gridDim.x / all_units - 1u) / (gridDim.x / all_units);
-                if (all_units < gridDim.x) size = min(size, total / (gridDim.x - all_units) + 1u);
+                if (all_units < gridDim.x) size = min(size, (total - all_units * EXTRA) / (gridDim.x - all_units) + 1u);
                 size = max(size, least);
                 if (size + worth >= most) size = most;
             }
-            // as long as the line's pieces take, with what joining costs either
-            if (size == most ? most <= each + cross + worth : size <= each + cross) {
+            if (size == most ? most <= each + worth : size <= each) {
                 uint32_t at = blockIdx.x;
 #pragma unroll
                 for (uint32_t k = 0; k < SLOTS; ++k) {
@@ -412,9 +417,9 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS> &cut, PieceSmem &sm,
 }
 
 // Walks over the units of a piece, MOST tiles of keys at a time. The whole warp.
-template <uint32_t KEYS, uint32_t MOST = 0x7fffffffu>
+template <uint32_t KEYS, uint32_t EXTRA, uint32_t MOST = 0x7fffffffu>
 struct Walk {
-    const Cut<KEYS> &cut;
+    const Cut<KEYS, EXTRA> &cut;
     Piece p;
     Seq q;
     uint32_t k_begin, k_end;              // the step's tiles of keys of the current unit
@@ -422,7 +427,7 @@ struct Walk {
     bool first;                           // it is the piece's first unit
     bool again;                           // there were steps of the unit before in this piece
 
-    __device__ __forceinline__ Walk(const Cut<KEYS> &cut_, const Piece &p_) : cut(cut_), p(p_), first(true), again(false)
+    __device__ __forceinline__ Walk(const Cut<KEYS, EXTRA> &cut_, const Piece &p_) : cut(cut_), p(p_), first(true), again(false)
     {
         if (p.left) {
             q = cut.open(p.s, p.kept);
@@ -452,6 +457,7 @@ struct Walk {
         }
         p.skip = 0u;
         first = again = false;
+        p.left -= min(p.left, (uint64_t)EXTRA);
         if (!p.left) return;
         if (++p.i >= cut.units(q)) {
             p.i = 0u;
@@ -476,9 +482,9 @@ struct Walk {
             uint32_t c = blockIdx.x - p.behind;
             r.first = 2u * c;
             if (p.each) {
-                const uint64_t unit = p.begin - p.skip;
+                const uint64_t unit = p.begin - p.skip;   // the place of its first tile of keys
                 c = (uint32_t)quotient(unit, p.each);
-                r.first = 2u * c + (unit == p.each * c ? 0u : 1u);
+                r.first = 2u * c + (unit - p.each * c <= EXTRA ? 0u : 1u);
             }
             r.count = blockIdx.x - c + 1u;
             r.s = p.s;
@@ -503,11 +509,11 @@ __device__ __forceinline__ void store4(const AttnArgs &a, uint32_t s, uint32_t h
         make_uint2(pack<BF>(x.x, x.y), pack<BF>(x.z, x.w));
 }
 
-// Whether a warp's lanes can keep the call's sequences: see kKeptSeqs. Units of `tile` rows, each at least KEYS positions long.
-inline bool lanes_keep(const AttnArgs &a, uint32_t tile, uint32_t keys)
+// Whether a warp's lanes can keep the call's sequences: see kKeptSeqs. Units of `tile` rows, and tiles of `keys` positions.
+inline bool lanes_keep(const AttnArgs &a, uint32_t tile, uint32_t keys, uint32_t extra)
 {
     const uint64_t units = ((uint64_t)a.r.tokens * a.group + tile - 1u) / tile, line = units * a.c.nseq * a.c.kv_heads;
-    return a.c.nseq <= kKeptSeqs && line < (1ull << 31) && line * ((a.c.limit + keys - 1u) / keys) < (1ull << 31);
+    return a.c.nseq <= kKeptSeqs && line < (1ull << 31) && line * ((a.c.limit + keys - 1u) / keys + extra) < (1ull << 31);
 }
 
 // Whatever the positions, each unit will be a piece of its own (find_piece): a sequence has room for no more

@@ -40,7 +40,7 @@ namespace {
 constexpr uint32_t kChunk = 16, kWarps = 12, kThreads = kWarps * 32, kStages = 2;
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
-constexpr uint32_t kSlots = 1, kWorth = 64, kCross = 40;      // chunks: what joining partial sums takes, and passing to another unit
+constexpr uint32_t kSlots = 1, kWorth = 64, kExtra = 32;      // chunks: what joining partial sums takes, and beginning and ending a unit
 constexpr float kLazy = 6.0f;
 // Weights are 2^(score - maximum + kUnit). binary16: their largest, 2^15, keeps the low term's bits; bfloat16 has fp32's
 // range, and small weights leave the sums of large values room
@@ -144,9 +144,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     }
     __syncthreads();
     wait_predecessor(a.early);
-    const Cut<kChunk> cut{a, R, Divisor{1u << 31, NT == 1 ? 3u : 4u}};
-    const Piece piece = find_piece<kChunk, kWarps, kSlots>(cut, sm.u.piece, kWarps, kWorth, kCross);
-    Walk<kChunk> w(cut, piece);
+    const Cut<kChunk, kExtra> cut{a, R, Divisor{1u << 31, NT == 1 ? 3u : 4u}};
+    const Piece piece = find_piece<kWarps, kSlots>(cut, sm.u.piece, kWarps, kWorth);
+    Walk<kChunk, kExtra> w(cut, piece);
     if (!a.keep) {                        // the ring's place is free
         fence_ring();
         __syncthreads();
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         __syncthreads();                  // the ring may fill again
     }
     if (warp == 0u) {
-        const Part part = Walk<kChunk>(cut, piece).part();
+        const Part part = Walk<kChunk, kExtra>(cut, piece).part();
         if (lane == 0u) reinterpret_cast<Part *>(a.parts)[blockIdx.x] = part;
     }
 }
@@ -562,7 +562,7 @@ cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtenso
     static_cast<AttnArgs &>(f) = a;
     f.kmap = kmap;
     f.vmap = vmap;
-    f.keep = lanes_keep(a, 8u * (uint32_t)nt, kChunk);
+    f.keep = lanes_keep(a, 8u * (uint32_t)nt, kChunk, kExtra);
     const cudaError_t e = nt == 1 ? (bf ? launch_few_of<true, 1>(f, dev, sms, stream) : launch_few_of<false, 1>(f, dev, sms, stream))
                                   : (bf ? launch_few_of<true, 2>(f, dev, sms, stream) : launch_few_of<false, 2>(f, dev, sms, stream));
     if (e != cudaSuccess) return e;
