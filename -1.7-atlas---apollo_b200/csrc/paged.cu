@@ -141,7 +141,7 @@ struct Scan {
 };
 
 // The sum of x over the threads before this one; `all`: over all threads. `turn` alternates between two calls.
-__device__ __forceinline__ uint32_t scan_all(Scan &sm, uint32_t turn, uint32_t x, uint32_t &all)
+__device__ __forceinline__ uint32_t scan_all(Scan &sm, uint32_t &turn, uint32_t x, uint32_t &all)
 {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     uint32_t inc = x;
@@ -150,22 +150,18 @@ __device__ __forceinline__ uint32_t scan_all(Scan &sm, uint32_t turn, uint32_t x
         const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= (uint32_t)o) inc += up;
     }
+    turn ^= 1u;
     if (lane == 31u) sm.warp[turn][warp] = inc;
     __syncthreads();
     uint32_t w = sm.warp[turn][lane];     // 32 warps
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= (uint32_t)o) w += up;
-    }
-    all = __shfl_sync(0xffffffffu, w, 31);
-    const uint32_t before = __shfl_sync(0xffffffffu, w, warp ? (int)warp - 1 : 0);
-    return inc - x + (warp ? before : 0u);
+    all = __reduce_add_sync(0xffffffffu, w);
+    w = lane < warp ? w : 0u;
+    return inc - x + __reduce_add_sync(0xffffffffu, w);
 }
 
 constexpr uint32_t kPlanPages = 16;       // pages that a thread looks at at a time
 
-// Bit i: page p0 + i is in use (i < kPlanPages); pages behind the last one are neither. 16-byte loads where `wide`.
+// Bit i: page p0 + i is in use (i < kPlanPages); pages behind the last one are neither
 __device__ __forceinline__ uint32_t used_mask(const Cache &c, uint32_t p0, uint32_t &exist)
 {
     uint32_t m = 0u;
@@ -183,57 +179,44 @@ __device__ __forceinline__ uint32_t used_mask(const Cache &c, uint32_t p0, uint3
     return m;
 }
 
-// The first `want` free pages, ascending, into `list`; how many there are (up to want). All threads.
-__device__ __forceinline__ uint32_t find_free(const Cache &c, Scan &sm, uint32_t want, uint32_t *list)
+// The first `want` free pages, ascending, into `list`; how many there are (up to want). All threads. `free0`: this thread's
+// of the first kPlanThreads * kPlanPages pages.
+__device__ __forceinline__ uint32_t find_free(const Cache &c, Scan &sm, uint32_t &turn, uint32_t free0, uint32_t want, uint32_t *list)
 {
     uint32_t found = 0u;
-    for (uint32_t b = 0, turn = 0; b < c.pages && found < want; b += kPlanThreads * kPlanPages, turn ^= 1u) {
+    for (uint32_t b = 0; b < c.pages && found < want; b += kPlanThreads * kPlanPages) {
         const uint32_t p0 = b + threadIdx.x * kPlanPages;
-        uint32_t exist, all;
-        uint32_t m = used_mask(c, p0, exist);
-        m = exist & ~m;
+        uint32_t exist, all, m = free0;
+        if (b) {
+            m = used_mask(c, p0, exist);
+            m = exist & ~m;
+        }
         uint32_t at = found + scan_all(sm, turn, __popc(m), all);
         for (; m && at < want; m &= m - 1u) list[at++] = p0 + (uint32_t)__ffs((int)m) - 1u;
         found += all;
     }
-    __syncthreads();                      // the list is there, and `sm` free again
+    __syncthreads();                      // the list is there
     return min(found, want);
 }
 
-// The entries that a call's tokens are written to, in order: sequence by sequence, position by position
-struct Entries {
+struct ReserveSmem {
+    Scan scan;
+    uint32_t copies;
+    // The entries that the call's tokens are written to, in order: sequence by sequence, position by position
     uint32_t before[kMaxSeqs + 1];        // entries of the sequences before
     uint32_t j0[kMaxSeqs];                // the first entry's column
+    uint8_t r0[kMaxSeqs];                 // the rows before the first position in its page
+    alignas(16) uint32_t page[kPlanThreads];
+    uint32_t fresh[kPlanThreads];   // few entries: the shared pages; the new ones
 };
 
-__device__ __forceinline__ void list_entries(const PlanArgs &a, Scan &sm, Entries &en)
-{
-    uint32_t done = 0u;
-    for (uint32_t b = 0, turn = 0; b < a.c.nseq; b += kPlanThreads, turn ^= 1u) {
-        const uint32_t s = b + threadIdx.x;
-        uint32_t n = 0u, all;
-        if (s < a.c.nseq) {
-            const uint32_t m = row_count(a.r, s);
-            const uint64_t p0 = __ldcg(a.r.pos0 + s), p1 = min(p0 + m, (uint64_t)a.c.limit);
-            const uint32_t j0 = (uint32_t)(p0 >> a.c.page_log2);
-            if (p0 < p1) n = (uint32_t)((p1 - 1u) >> a.c.page_log2) - j0 + 1u;
-            en.j0[s] = j0;
-        }
-        const uint32_t at = done + scan_all(sm, turn, n, all);
-        if (s < a.c.nseq) en.before[s] = at;
-        done += all;
-    }
-    if (threadIdx.x == 0) en.before[a.c.nseq] = done;
-    __syncthreads();
-}
-
 // The sequence that entry `e` is of
-__device__ __forceinline__ uint32_t sequence_of(const Entries &en, uint32_t nseq, uint32_t e)
+__device__ __forceinline__ uint32_t sequence_of(const ReserveSmem &sm, uint32_t nseq, uint32_t e)
 {
     uint32_t lo = 0u, hi = nseq;          // before[lo] <= e < before[hi]
     while (hi - lo > 1u) {
         const uint32_t mid = (lo + hi) >> 1;
-        if (en.before[mid] <= e) lo = mid;
+        if (sm.before[mid] <= e) lo = mid;
         else hi = mid;
     }
     return lo;
@@ -244,94 +227,140 @@ __device__ __forceinline__ uint32_t sequence_of(const Entries &en, uint32_t nseq
 // name, the last one keeps it. (One entry after the other: whoever finds its
 // page named by others leaves it, until one is left.) New pages are the lowest
 // free ones, in the entries' order; all or nothing. One CTA: the orders are
-// those of scans over entries and pages. Bound by latency: about six dependent
-// reads of L2 and three to ten scans of a few hundred cycles.
-__global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const __grid_constant__ PlanArgs a)
+// those of scans over entries and pages. Up to a thread's entry each, the entries
+// are looked at once, and those of one page find each other in shared memory;
+// more go through arrays in the workspace, in several passes.
+// Bound by latency: three dependent reads of L2 and three scans of some hundred
+// cycles for few entries.
+__device__ __forceinline__ void plan_reserve(const PlanArgs &a, ReserveSmem &sm)
 {
-    __shared__ Scan sm;
-    __shared__ uint32_t copies;
-    extern __shared__ uint8_t entries_smem[];
-    Entries &en = *reinterpret_cast<Entries *>(entries_smem);
-    if (threadIdx.x == 0) copies = 0u;
-    wait_predecessor(a.early);
-    list_entries(a, sm, en);
-    const uint32_t total = en.before[a.c.nseq];
+    uint32_t turn = 0u, exist;
+    if (threadIdx.x == 0) sm.copies = 0u;
+    // on its way with the positions: what will be free
+    const uint32_t used0 = used_mask(a.c, threadIdx.x * kPlanPages, exist), free0 = exist & ~used0;
+    uint32_t total = 0u;
+    for (uint32_t b = 0; b < a.c.nseq; b += kPlanThreads) {
+        const uint32_t s = b + threadIdx.x;
+        uint32_t n = 0u, all;
+        if (s < a.c.nseq) {
+            const uint32_t m = row_count(a.r, s);
+            const uint64_t p0 = __ldcg(a.r.pos0 + s), p1 = min(p0 + m, (uint64_t)a.c.limit);
+            const uint32_t j0 = (uint32_t)(p0 >> a.c.page_log2);
+            if (p0 < p1) n = (uint32_t)((p1 - 1u) >> a.c.page_log2) - j0 + 1u;
+            sm.j0[s] = j0;
+            sm.r0[s] = (uint8_t)(p0 & ((1u << a.c.page_log2) - 1u));
+        }
+        const uint32_t at = total + scan_all(sm.scan, turn, n, all);
+        if (s < a.c.nseq) sm.before[s] = at;
+        total += all;
+    }
+    if (threadIdx.x == 0) sm.before[a.c.nseq] = total;
+    __syncthreads();
     uint32_t *const writers = array_of(a.c, kWriters), *const last = array_of(a.c, kLastWriter);
+    uint32_t *const from = array_of(a.c, kCopyFrom), *const to_page = array_of(a.c, kCopyTo), *const rows = array_of(a.c, kCopyRows);
     // page and place of entry e
-    auto entry = [&](uint32_t e, uint32_t &s, size_t &at) {
-        s = sequence_of(en, a.c.nseq, e);
-        at = (size_t)s * a.c.max_pages + en.j0[s] + (e - en.before[s]);
-        return (uint32_t)__ldcg(a.c.table + at);
-    };
-    // how many entries of the call name each page that has several names, and which of them is last
-    bool shares = false;
     uint32_t s;
     size_t at;
-    for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) {
-        const uint32_t p = entry(e, s, at);
-        if (p < a.c.pages && __ldcg(a.c.refs + p) > 1) {
-            writers[p] = 0u;
-            last[p] = 0u;
-            shares = true;
-        }
-    }
-    if (__syncthreads_or(shares)) {
-        for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) {
-            const uint32_t p = entry(e, s, at);
-            if (p < a.c.pages && __ldcg(a.c.refs + p) > 1) {
-                atomicAdd(writers + p, 1u);
-                atomicMax(last + p, e);
-            }
-        }
-        __syncthreads();
-    }
-    // 0: keeps its page; 1: needs one; 2: and leaves its page as the last of the call that names it
-    auto needs = [&](uint32_t e, uint32_t p) -> uint32_t {
-        if (p >= a.c.pages) return 1u;
-        const uint32_t names = (uint32_t)max(__ldcg(a.c.refs + p), 0);
-        if (names <= 1u) return 0u;
-        if (__ldcg(last + p) != e) return 1u;
-        return __ldcg(writers + p) >= names ? 0u : 2u;
+    auto entry = [&](uint32_t e) {
+        s = sequence_of(sm, a.c.nseq, e);
+        at = (size_t)s * a.c.max_pages + sm.j0[s] + (e - sm.before[s]);
+        return (uint32_t)__ldcg(a.c.table + at);
     };
-    uint32_t mine = 0u, need;
-    for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) mine += needs(e, entry(e, s, at)) != 0u;
-    scan_all(sm, 0u, mine, need);
-    __syncthreads();
-    uint32_t *const fresh = array_of(a.c, kFresh);
-    const uint32_t found = need ? find_free(a.c, sm, need, fresh) : 0u;
-    if (threadIdx.x == 0) *a.out = need - found;
-    uint32_t *const from = array_of(a.c, kCopyFrom), *const to_page = array_of(a.c, kCopyTo), *const rows = array_of(a.c, kCopyRows);
-    if (found == need) {
-        uint32_t given = 0u;
-        for (uint32_t b = 0, turn = 0; b < total; b += kPlanThreads, turn ^= 1u) {
-            const uint32_t e = b + threadIdx.x;
-            uint32_t p = 0u, want = 0u, all, names = 0u, written = 0u;
-            if (e < total) {
-                p = entry(e, s, at);
-                want = needs(e, p);
-                if (p < a.c.pages && (names = (uint32_t)max(__ldcg(a.c.refs + p), 0)) > 1u) written = __ldcg(writers + p);
+    auto names_of = [&](uint32_t p) { return p < a.c.pages ? (uint32_t)max(__ldcg(a.c.refs + p), 0) : 0u; };
+    // entry e of sequence s, at `at`, leaves page p for page `to`
+    auto give = [&](uint32_t e, uint32_t p, uint32_t to) {
+        a.c.table[at] = (int32_t)to;
+        a.c.refs[to] = 1;
+        const uint32_t r = e == sm.before[s] ? sm.r0[s] : 0u;
+        if (p < a.c.pages && r) {
+            const uint32_t i = atomicAdd(&sm.copies, 1u);
+            from[i] = p;
+            to_page[i] = to;
+            rows[i] = r;
+        }
+    };
+    uint32_t need;
+    if (total <= kPlanThreads) {
+        const uint32_t e = threadIdx.x;
+        const bool mine = e < total;
+        uint32_t p = ~0u, names = 0u;
+        if (mine) {
+            p = entry(e);
+            names = names_of(p);
+        }
+        const bool shared = names > 1u;
+        sm.page[e] = shared ? p : ~0u;
+        uint32_t written = 0u, behind = 0u;       // entries of the call that name the page, and such ones behind this one
+        if (__syncthreads_or(shared) && shared)
+            for (uint32_t k = 0; k < total; k += 4u) {   // those behind the last one name none
+                const uint4 x = *reinterpret_cast<const uint4 *>(sm.page + k);
+                const uint32_t same = (x.x == p ? 1u : 0u) | (x.y == p ? 2u : 0u) | (x.z == p ? 4u : 0u) | (x.w == p ? 8u : 0u);
+                written += __popc(same);
+                behind += k + 4u <= e ? 0u : k > e ? __popc(same) : __popc(same >> (e - k) >> 1);
             }
-            const uint32_t rank = given + scan_all(sm, turn, want != 0u, all);
-            given += all;
-            // the entry that is the page's last writer comes last: nobody after it looks at the page's count
-            if (e < total && names > 1u && __ldcg(last + p) == e) a.c.refs[p] = (int32_t)(written >= names ? 1u : names - written);
-            if (want) {
-                const uint32_t to = __ldcg(fresh + rank);
-                a.c.table[at] = (int32_t)to;
-                a.c.refs[to] = 1;
-                const uint32_t r = e == en.before[s] ? __ldcg(a.r.pos0 + s) & ((1u << a.c.page_log2) - 1u) : 0u;
-                if (p < a.c.pages && r) {
-                    const uint32_t i = atomicAdd(&copies, 1u);
-                    from[i] = p;
-                    to_page[i] = to;
-                    rows[i] = r;
+        const bool is_last = shared && behind == 0u, keeps = mine && (names == 1u || (p < a.c.pages && names == 0u) || (is_last && written >= names));
+        const bool want = mine && !keeps;
+        const uint32_t rank = scan_all(sm.scan, turn, want ? 1u : 0u, need);
+        const uint32_t found = need ? find_free(a.c, sm.scan, turn, free0, need, sm.fresh) : 0u;
+        if (threadIdx.x == 0) *a.out = need - found;
+        if (found == need) {
+            if (is_last) a.c.refs[p] = (int32_t)(written >= names ? 1u : names - written);
+            if (want) give(e, p, sm.fresh[rank]);
+        }
+    } else {
+        // how many entries of the call name each page that has several names, and which of them is last
+        bool shares = false;
+        for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) {
+            const uint32_t p = entry(e);
+            if (names_of(p) > 1u) {
+                writers[p] = 0u;
+                last[p] = 0u;
+                shares = true;
+            }
+        }
+        if (__syncthreads_or(shares)) {
+            for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) {
+                const uint32_t p = entry(e);
+                if (names_of(p) > 1u) {
+                    atomicAdd(writers + p, 1u);
+                    atomicMax(last + p, e);
                 }
+            }
+            __syncthreads();
+        }
+        auto needs = [&](uint32_t e, uint32_t p) {
+            if (p >= a.c.pages) return true;
+            const uint32_t names = names_of(p);
+            return names > 1u && (__ldcg(last + p) != e || __ldcg(writers + p) < names);
+        };
+        uint32_t mine = 0u;
+        for (uint32_t e = threadIdx.x; e < total; e += kPlanThreads) mine += needs(e, entry(e)) ? 1u : 0u;
+        scan_all(sm.scan, turn, mine, need);
+        uint32_t *const fresh = array_of(a.c, kFresh);
+        const uint32_t found = need ? find_free(a.c, sm.scan, turn, free0, need, fresh) : 0u;
+        if (threadIdx.x == 0) *a.out = need - found;
+        if (found == need) {
+            uint32_t given = 0u;
+            for (uint32_t b = 0; b < total; b += kPlanThreads) {
+                const uint32_t e = b + threadIdx.x;
+                uint32_t p = ~0u, all, names = 0u, written = 0u;
+                bool want = false;
+                if (e < total) {
+                    p = entry(e);
+                    want = needs(e, p);
+                    if ((names = names_of(p)) > 1u) written = __ldcg(writers + p);
+                }
+                const uint32_t rank = given + scan_all(sm.scan, turn, want ? 1u : 0u, all);
+                given += all;
+                // the entry that is the page's last writer comes last: nobody after it looks at the page's count
+                if (names > 1u && __ldcg(last + p) == e) a.c.refs[p] = (int32_t)(written >= names ? 1u : names - written);
+                if (want) give(e, p, __ldcg(fresh + rank));
             }
         }
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        head_of(a.c)->copies = copies;
+        head_of(a.c)->copies = sm.copies;
         head_of(a.c)->from = ~0u;
     }
 }
@@ -339,18 +368,21 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const __grid_cons
 // U pages are in use. The i-th used page from number U on goes to the i-th free
 // one below U, so that the first U are the used ones, and as few move as can be.
 // One CTA, two passes over the counts.
-__global__ void __launch_bounds__(kPlanThreads) compact_kernel(const __grid_constant__ PlanArgs a)
+__device__ __forceinline__ void plan_compact(const PlanArgs &a, Scan &sm)
 {
-    __shared__ Scan sm;
-    wait_predecessor(a.early);
-    uint32_t mine = 0u, used, exist;
-    for (uint32_t p0 = threadIdx.x * kPlanPages; p0 < a.c.pages; p0 += kPlanThreads * kPlanPages) mine += __popc(used_mask(a.c, p0, exist));
-    scan_all(sm, 0u, mine, used);
+    uint32_t turn = 0u, exist0, exist, used;
+    const uint32_t mask0 = used_mask(a.c, threadIdx.x * kPlanPages, exist0);   // the first pages' are kept for the second pass
+    uint32_t mine = __popc(mask0);
+    for (uint32_t b = kPlanThreads * kPlanPages; b < a.c.pages; b += kPlanThreads * kPlanPages) mine += __popc(used_mask(a.c, b + threadIdx.x * kPlanPages, exist));
+    scan_all(sm, turn, mine, used);
     uint32_t *const from = array_of(a.c, kCopyFrom), *const to = array_of(a.c, kCopyTo), *const rows = array_of(a.c, kCopyRows);
     uint32_t *const moved = array_of(a.c, (WorkArray)kMovedTo);
     uint32_t holes = 0u, high = 0u;
-    for (uint32_t b = 0, turn = 1; b < a.c.pages; b += kPlanThreads * kPlanPages, turn ^= 1u) {
-        const uint32_t p0 = b + threadIdx.x * kPlanPages, m = used_mask(a.c, p0, exist);
+    for (uint32_t b = 0; b < a.c.pages; b += kPlanThreads * kPlanPages) {
+        const uint32_t p0 = b + threadIdx.x * kPlanPages;
+        uint32_t m = mask0;
+        exist = exist0;
+        if (b) m = used_mask(a.c, p0, exist);
         const uint32_t low = used <= p0 ? 0u : used - p0 >= kPlanPages ? (1u << kPlanPages) - 1u : (1u << (used - p0)) - 1u;
         uint32_t free = exist & ~m & low, over = m & ~low, all;
         // both counts in one scan: at most 2^14 each
@@ -378,10 +410,11 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(const __grid_cons
 // Carries out a plan: the first rows of pages, in every layer, K and V, to other
 // pages, and the table's new numbers. No target is a source. Rows that follow one
 // another in both pages go 64 at a time (16 KB): pieces of whole pages, whose KV
-// heads follow one another too, or of a head's first rows. Each of a CTA's warps
-// has one lane bring pieces into shared memory and out again by bulk copies, four
-// buffers a warp, so that 192 KB an SM are on their way without a register.
-// Bound by HBM.
+// heads follow one another too, or of a head's first rows. One lane of each of a
+// CTA's moving warps brings pieces into shared memory and out again by bulk copies,
+// four buffers a warp, so that 192 KB an SM are on their way without a register.
+// Bound by HBM (268 MB to another place 82.7 us, 6.5 TB/s, 99 % of the copy rate;
+// 16-byte loads and stores by all threads, four on their way each: 154 us).
 struct MoveArgs {
     Cache c;
     uint32_t early;
@@ -389,101 +422,132 @@ struct MoveArgs {
 
 constexpr uint32_t kMoveWarps = 3, kMoveThreads = kMoveWarps * 32, kMoveStages = 4, kMoveRows = 64;
 
+struct MovePiece {
+    uint8_t *src, *dst;
+    uint32_t bytes;
+};
+
 struct alignas(128) MoveSmem {
     uint8_t buffer[kMoveWarps][kMoveStages][kMoveRows * kRowBytes];
     uint64_t full[kMoveWarps][kMoveStages];
+    MovePiece piece[kMoveWarps][kMoveStages];
     uint32_t err;
 };
+
+// The barriers; before a barrier of the CTA
+__device__ __forceinline__ void init_move(MoveSmem &sm)
+{
+    const uint32_t warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31u) == 0u && warp < kMoveWarps) {
+        for (uint32_t i = 0; i < kMoveStages; ++i) mbar_init(&sm.full[warp][i], 1u);
+        fence_mbar_init();
+    }
+    if (threadIdx.x == 0u) sm.err = kStatusOk;
+}
+
+// By CTA `cta` of `ctas`
+__device__ __forceinline__ void move_pages(const Cache &ca, MoveSmem &sm, uint32_t cta, uint32_t ctas)
+{
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t copies = __ldcg(&head_of(ca)->copies), moved_from = __ldcg(&head_of(ca)->from);
+    if (warp < kMoveWarps && copies) {
+        const uint32_t *from = array_of(ca, kCopyFrom), *to = array_of(ca, kCopyTo), *rows = array_of(ca, kCopyRows);
+        const bool whole = moved_from != ~0u;
+        const uint32_t page = 1u << ca.page_log2;
+        // runs of a page that lie together, and pieces of a run
+        const uint32_t runs = whole ? 1u : ca.kv_heads, run_rows = whole ? ca.kv_heads << ca.page_log2 : page;
+        const uint32_t subs = (run_rows + kMoveRows - 1u) / kMoveRows, per_page = runs * subs;
+        const uint32_t pieces = copies * ca.layers * 2u * per_page, step = ctas * kMoveWarps;
+        MovePiece *const slot = sm.piece[warp];
+        uint64_t *const full = sm.full[warp];
+        uint32_t loaded = 0u;
+        bool ok = true;
+        // lane 0: piece n, which was loaded, goes out
+        auto store = [&](uint32_t n) {
+            const MovePiece p = slot[n % kMoveStages];
+            uint8_t *const buffer = sm.buffer[warp][n % kMoveStages];
+            ok = ok && mbar_wait(full + n % kMoveStages, n / kMoveStages & 1u, &sm.err);
+            if (ok) {
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.dst), "r"(smem_addr(buffer)), "r"(p.bytes) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            } else {   // a wait that ran out: by hand
+                for (uint32_t b = 0; b < p.bytes; b += 16u) *reinterpret_cast<uint4 *>(p.dst + b) = __ldcg(reinterpret_cast<const uint4 *>(p.src + b));
+            }
+        };
+        // every lane looks a piece up, 32 at a time; lane 0 then copies them
+        for (uint32_t x0 = cta * kMoveWarps + warp; x0 < pieces; x0 += 32u * step) {
+            const uint32_t x = x0 + lane * step;
+            MovePiece mine{nullptr, nullptr, 0u};
+            if (x < pieces) {
+                const uint32_t at = x / per_page, in = x - at * per_page, run = in / subs, row = (in - run * subs) * kMoveRows;
+                const uint32_t i = at / (2u * ca.layers), layer2 = at - i * 2u * ca.layers;
+                uint8_t *pool = reinterpret_cast<uint8_t *>(layer2 & 1u ? ca.v : ca.k);
+                const uint32_t have = whole ? run_rows : __ldcg(rows + i), p = __ldcg(from + i), q = __ldcg(to + i);
+                auto place = [&](uint32_t number) {
+                    return pool + (((((uint64_t)(layer2 >> 1) * ca.pages + number) * ca.kv_heads + run) << ca.page_log2) + row) * kRowBytes;
+                };
+                if (row < have) mine = MovePiece{place(p), place(q), min(have - row, kMoveRows) * kRowBytes};
+            }
+            for (uint32_t there = __ballot_sync(0xffffffffu, mine.bytes != 0u); there; there &= there - 1u) {
+                const int l = __ffs((int)there) - 1;
+                MovePiece p;
+                p.src = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine.src), l));
+                p.dst = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine.dst), l));
+                p.bytes = __shfl_sync(0xffffffffu, mine.bytes, l);
+                if (lane == 0u) {
+                    // loads are kMoveStages - 1 ahead of the stores; a buffer is free once its last store has read it
+                    if (loaded >= kMoveStages - 1u) store(loaded - (kMoveStages - 1u));
+                    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    slot[loaded % kMoveStages] = p;
+                    mbar_arrive_expect_tx(full + loaded % kMoveStages, p.bytes);
+                    bulk_g2s(sm.buffer[warp][loaded % kMoveStages], p.src, p.bytes, full + loaded % kMoveStages);
+                }
+                ++loaded;
+            }
+        }
+        if (lane == 0u) {
+            for (uint32_t n = loaded - min(loaded, kMoveStages - 1u); n < loaded; ++n) store(n);
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
+    }
+    if (moved_from == ~0u) return;
+    const uint32_t *moved = array_of(ca, (WorkArray)kMovedTo);
+    const size_t entries = (size_t)ca.nseq * ca.max_pages;
+    for (size_t i = (size_t)cta * blockDim.x + threadIdx.x; i < entries; i += (size_t)ctas * blockDim.x) {
+        const uint32_t p = (uint32_t)__ldcg(ca.table + i);
+        if (p >= moved_from && p < ca.pages) ca.table[i] = (int32_t)__ldcg(moved + p);
+    }
+}
 
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveArgs a)
 {
     extern __shared__ __align__(128) uint8_t move_smem[];
     MoveSmem &sm = *reinterpret_cast<MoveSmem *>(move_smem);
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    if (lane == 0u) {
-        for (uint32_t i = 0; i < kMoveStages; ++i) mbar_init(&sm.full[warp][i], 1u);
-        fence_mbar_init();
-    }
-    if (threadIdx.x == 0u) sm.err = kStatusOk;
+    init_move(sm);
     __syncthreads();
     wait_predecessor(a.early);
-    const uint32_t copies = __ldcg(&head_of(a.c)->copies), moved_from = __ldcg(&head_of(a.c)->from);
-    if (lane == 0u && copies) {
-        const uint32_t *from = array_of(a.c, kCopyFrom), *to = array_of(a.c, kCopyTo), *rows = array_of(a.c, kCopyRows);
-        const bool whole = moved_from != ~0u;
-        const uint32_t page = 1u << a.c.page_log2;
-        // runs of a page that lie together, and pieces of a run
-        const uint32_t runs = whole ? 1u : a.c.kv_heads, run_rows = whole ? a.c.kv_heads << a.c.page_log2 : page;
-        const uint32_t subs = (run_rows + kMoveRows - 1u) / kMoveRows, per_page = runs * subs;
-        const uint32_t pieces = copies * a.c.layers * 2u * per_page, step = gridDim.x * kMoveWarps;
-        struct Copy {
-            const uint8_t *src;
-            uint8_t *dst;
-            uint32_t bytes;
-        };
-        auto piece_of = [&](uint32_t x) {
-            Copy c;
-            const uint32_t at = x / per_page, in = x - at * per_page, run = in / subs, row = (in - run * subs) * kMoveRows;
-            const uint32_t layer2 = at % (2u * a.c.layers), i = at / (2u * a.c.layers);
-            uint8_t *pool = reinterpret_cast<uint8_t *>(layer2 & 1u ? a.c.v : a.c.k);
-            const uint32_t have = whole ? run_rows : __ldcg(rows + i);
-            auto place = [&](uint32_t p) {
-                return pool + (((((uint64_t)(layer2 >> 1) * a.c.pages + p) * a.c.kv_heads + run) << a.c.page_log2) + row) * kRowBytes;
-            };
-            c.src = place(__ldcg(from + i));
-            c.dst = place(__ldcg(to + i));
-            c.bytes = row < have ? min(have - row, kMoveRows) * kRowBytes : 0u;
-            return c;
-        };
-        // the pieces x, x + step, ...: load number n into buffer n % kMoveStages, kMoveStages - 1 ahead of the stores
-        uint32_t x = blockIdx.x * kMoveWarps + warp, loaded = 0u, stored = 0u;
-        Copy c[kMoveStages];
-        bool ok = true;
-        auto load = [&](uint32_t slot) {
-            Copy &d = c[slot];
-            d.bytes = 0u;
-            while (x < pieces && !d.bytes) {
-                d = piece_of(x);
-                x += step;
-            }
-            if (!d.bytes) return false;
-            mbar_arrive_expect_tx(&sm.full[warp][slot], d.bytes);
-            bulk_g2s(sm.buffer[warp][slot], d.src, d.bytes, &sm.full[warp][slot]);
-            ++loaded;
-            return true;
-        };
-        bool more = true;
-#pragma unroll
-        for (uint32_t i = 0; i + 1u < kMoveStages; ++i) more = more && load(i);
-        while (stored < loaded) {
-#pragma unroll
-            for (uint32_t slot = 0; slot < kMoveStages; ++slot) {
-                if (stored >= loaded) break;
-                ok = ok && mbar_wait(&sm.full[warp][slot], stored / kMoveStages & 1u, &sm.err);
-                if (ok) {
-                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(c[slot].dst), "r"(smem_addr(sm.buffer[warp][slot])),
-                                 "r"(c[slot].bytes)
-                                 : "memory");
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                } else {   // a wait that ran out: by hand
-                    for (uint32_t b = 0; b < c[slot].bytes; b += 16u)
-                        *reinterpret_cast<uint4 *>(c[slot].dst + b) = __ldcg(reinterpret_cast<const uint4 *>(c[slot].src + b));
-                }
-                ++stored;
-                // the buffer before this one is free once its store has read it
-                asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                if (more) more = load((slot + kMoveStages - 1u) % kMoveStages);
-            }
-        }
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    move_pages(a.c, sm, blockIdx.x, gridDim.x);
+}
+
+// The plan, by one CTA; in a cluster, all its CTAs then carry it out.
+template <bool COMPACT>
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanArgs a)
+{
+    extern __shared__ __align__(128) uint8_t plan_smem[];
+    const uint32_t ctas = k8::cluster_size();
+    MoveSmem &move = *reinterpret_cast<MoveSmem *>(plan_smem);
+    if (ctas > 1u) init_move(move);
+    // the plan's own memory lies in the buffers
+    static_assert(sizeof(ReserveSmem) <= sizeof(move.buffer), "the plan exceeds the buffers' memory");
+    wait_predecessor(a.early);
+    if (k8::cluster_rank() == 0u) {
+        if (COMPACT) plan_compact(a, reinterpret_cast<ReserveSmem *>(plan_smem)->scan);
+        else plan_reserve(a, *reinterpret_cast<ReserveSmem *>(plan_smem));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (moved_from == ~0u) return;
-    const uint32_t *moved = array_of(a.c, (WorkArray)kMovedTo);
-    const size_t entries = (size_t)a.c.nseq * a.c.max_pages;
-    for (size_t i = (size_t)blockIdx.x * kMoveThreads + threadIdx.x; i < entries; i += (size_t)gridDim.x * kMoveThreads) {
-        const uint32_t p = (uint32_t)__ldcg(a.c.table + i);
-        if (p >= moved_from && p < a.c.pages) a.c.table[i] = (int32_t)__ldcg(moved + p);
-    }
+    if (ctas == 1u) return;
+    k8::cluster_sync();
+    move_pages(a.c, move, k8::cluster_rank(), ctas);
 }
 
 // ------------------------------------------------------------- host side ----
@@ -628,17 +692,27 @@ int done(const char *who, cudaError_t e)
     return api_fail(ATLAS_ECUDA, "%s: %s", who, cudaGetErrorString(e));
 }
 
-// Carries out the plan of the launch before, which copies at most `copies` pages
-cudaError_t launch_move(const Cache &c, uint64_t copies, uint64_t entries, int dev, int sms, cudaStream_t stream)
+// Plans, and copies at most `copies` pages: in one launch of a cluster where that is little (16 SMs copy 1.5 TB/s or so; a second
+// launch costs 2.4 us on the host and 2 on the device), in two where it may be much
+constexpr uint64_t kLittle = 8u << 20;
+constexpr uint32_t kPlanCluster = 16;
+
+template <bool COMPACT>
+cudaError_t launch_plan(const PlanArgs &p, uint64_t copies, int dev, int sms, cudaStream_t stream)
 {
+    const Cache &c = p.c;
+    cudaError_t e = k8::allow<plan_kernel<COMPACT>>(dev, (int)sizeof(MoveSmem));
+    if (e != cudaSuccess) return e;
+    const uint64_t bytes = copies * c.layers * 2 * ((uint64_t)c.kv_heads << c.page_log2) * kRowBytes;
+    if (bytes <= kLittle && k8::clusters_at_once<plan_kernel<COMPACT>>(dev, kPlanCluster, kPlanThreads, sizeof(MoveSmem)))
+        return launch(plan_kernel<COMPACT>, dim3(kPlanCluster), kPlanThreads, sizeof(MoveSmem), kPlanCluster, p, sms, stream);
+    if ((e = launch(plan_kernel<COMPACT>, dim3(1), kPlanThreads, sizeof(ReserveSmem), 1, p, sms, stream)) != cudaSuccess) return e;
+    if ((e = k8::allow<move_kernel>(dev, (int)sizeof(MoveSmem))) != cudaSuccess) return e;
     MoveArgs a{};
     a.c = c;
-    const cudaError_t e = k8::allow<move_kernel>(dev, (int)sizeof(MoveSmem));
-    if (e != cudaSuccess) return e;
-    const uint64_t pieces = copies * c.layers * 2 * (((uint64_t)c.kv_heads << c.page_log2) + kMoveRows - 1) / kMoveRows;
-    const uint64_t ctas = std::max((pieces + kMoveWarps - 1) / kMoveWarps, (entries + kMoveThreads - 1) / kMoveThreads);
-    return launch(move_kernel, dim3((uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(ctas, (uint64_t)sms))), kMoveThreads, sizeof(MoveSmem), 1, a, sms,
-                  stream);
+    const uint64_t entries = COMPACT ? (uint64_t)c.nseq * c.max_pages : 0;
+    const uint64_t ctas = std::max(bytes / (kMoveWarps * kMoveRows * kRowBytes), entries / kMoveThreads) + 1;
+    return launch(move_kernel, dim3((uint32_t)std::min<uint64_t>(ctas, (uint64_t)sms)), kMoveThreads, sizeof(MoveSmem), 1, a, sms, stream);
 }
 
 }  // namespace
@@ -707,10 +781,8 @@ extern "C" int atlas_cuda_paged_reserve(const AtlasPaged *cache, uint32_t tokens
     if (rc == ATLAS_OK) rc = check_ints(who, "short", d_short, dev);
     if (rc != ATLAS_OK) return rc;
     a.out = d_short;
-    const cudaError_t e = launch(reserve_kernel, dim3(1), kPlanThreads, sizeof(Entries), 1, a, sms, (cudaStream_t)stream);
-    if (e != cudaSuccess) return done(who, e);
     // a sequence's first page at most is copied
-    return done(who, launch_move(a.c, std::min(cache->nseq, cache->pages), 0, dev, sms, (cudaStream_t)stream));
+    return done(who, launch_plan<false>(a, std::min(cache->nseq, cache->pages), dev, sms, (cudaStream_t)stream));
 }
 
 extern "C" int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_used, void *stream)
@@ -721,9 +793,7 @@ extern "C" int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_use
     if (rc == ATLAS_OK) rc = check_ints(who, "used", d_used, dev);
     if (rc != ATLAS_OK) return rc;
     a.out = d_used;
-    const cudaError_t e = launch(compact_kernel, dim3(1), kPlanThreads, 0, 1, a, sms, (cudaStream_t)stream);
-    if (e != cudaSuccess) return done(who, e);
-    return done(who, launch_move(a.c, cache->pages / 2u, (uint64_t)cache->nseq * cache->max_pages, dev, sms, (cudaStream_t)stream));
+    return done(who, launch_plan<true>(a, cache->pages / 2u, dev, sms, (cudaStream_t)stream));
 }
 
 namespace {

@@ -584,6 +584,12 @@ class PagedCache:
         self.desc.work, self.desc.work_bytes = work.data_ptr(), work.nbytes
 
 
+def _paged_ints(who: str, cache: PagedCache, name: str, t, n: int) -> None:
+    """_kv8_ints; a tensor of just the size and type, as most calls have, passes at once."""
+    if t is not None and not (t.dtype is cache._i32 and t.nbytes == 4 * n and t.is_contiguous()):
+        _kv8_ints(who, name, t, n)
+
+
 def _paged_check(who: str, cache: PagedCache, tokens: int, heads: int, pos0, n_tok, names=(), a=None, lda: int = 0, b=None,
                  ldb: int = 0) -> None:
     """Refuses tensors of another type, layout or size. a, b: rows of `heads` each, or None. Dense ones of just the size, as
@@ -605,24 +611,25 @@ def paged_fork(cache: PagedCache, parent, length, first=None, stream: int = 0) -
     """Sequence s becomes what sequence parent[s] was up to position length[s] (and from first[s] on): int32 [nseq] each.
     atlas_cuda_paged_fork. Here and below, `stream` is a cudaStream_t (0: the legacy default stream), and tensors of another
     type, layout or size are refused."""
-    for name, t in (("parent", parent), ("length", length), ("first", first)):
-        _kv8_ints("paged_fork", name, t, cache.nseq)
-    check(lib().atlas_cuda_paged_fork(cache._ref, parent.data_ptr(), length.data_ptr(), _addr(first), stream), "paged_fork")
+    _paged_ints("paged_fork", cache, "parent", parent, cache.nseq)
+    _paged_ints("paged_fork", cache, "length", length, cache.nseq)
+    _paged_ints("paged_fork", cache, "first", first, cache.nseq)
+    check(lib().atlas_cuda_paged_fork(cache._ref, _addr(parent), _addr(length), _addr(first), stream), "paged_fork")
 
 
 def paged_reserve(cache: PagedCache, tokens: int, pos0, short, n_tok=None, stream: int = 0) -> None:
     """Gives each sequence s pages of its own for positions pos0[s], ... of its next n_tok[s] tokens (None: `tokens`); short
     (int32 [1]) receives how many pages are lacking, and then nothing has changed. atlas_cuda_paged_reserve."""
     _paged_check("paged_reserve", cache, tokens, 0, pos0, n_tok)
-    _kv8_ints("paged_reserve", "short", short, 1)
-    check(lib().atlas_cuda_paged_reserve(cache._ref, tokens, pos0.data_ptr(), _addr(n_tok), short.data_ptr(), stream),
+    _paged_ints("paged_reserve", cache, "short", short, 1)
+    check(lib().atlas_cuda_paged_reserve(cache._ref, tokens, pos0.data_ptr(), _addr(n_tok), _addr(short), stream),
           "paged_reserve")
 
 
 def paged_compact(cache: PagedCache, used, stream: int = 0) -> None:
     """Moves the pages in use to the pool's start; used (int32 [1]) receives how many there are. atlas_cuda_paged_compact."""
-    _kv8_ints("paged_compact", "used", used, 1)
-    check(lib().atlas_cuda_paged_compact(cache._ref, used.data_ptr(), stream), "paged_compact")
+    _paged_ints("paged_compact", cache, "used", used, 1)
+    check(lib().atlas_cuda_paged_compact(cache._ref, _addr(used), stream), "paged_compact")
 
 
 def paged_append(cache: PagedCache, layer: int, tokens: int, pos0, k, v, n_tok=None, ld: int = 0, stream: int = 0) -> None:
