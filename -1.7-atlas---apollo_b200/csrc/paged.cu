@@ -44,7 +44,7 @@ struct AppendArgs {
     uint32_t layer, early;
 };
 
-constexpr uint32_t kAppendThreads = 256, kAppendRows = 4;   // rows (token, head) of a sequence that 16 threads take
+constexpr uint32_t kAppendThreads = 256, kAppendRows = 2;   // rows (token, head) of a sequence that 16 threads take
 
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a)
 {
@@ -55,21 +55,28 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     const uint64_t row0 = (uint64_t)blockIdx.x * (kAppendThreads / 16u * kAppendRows) + (threadIdx.x >> 4);
     uint4 k[kAppendRows], v[kAppendRows];
     uint64_t to[kAppendRows];
+    uint32_t e[kAppendRows];
+    // the rows are on their way while their pages are looked up
 #pragma unroll
     for (uint32_t i = 0; i < kAppendRows; ++i) {
         const uint64_t row = row0 + i * (kAppendThreads / 16u);
-        to[i] = ~0ull;
+        e[i] = ~0u;
+        to[i] = 0u;
         if (row >= rows) continue;
         const uint32_t t = (uint32_t)(row / a.c.kv_heads), h = (uint32_t)(row - (uint64_t)t * a.c.kv_heads);
-        const uint64_t p = p0 + t;
-        if (p >= a.c.limit) continue;
-        const uint32_t e = (uint32_t)__ldcg(a.c.table + (size_t)s * a.c.max_pages + (p >> a.c.page_log2));
-        // a page that other sequences have too is not written to
-        if (e >= a.c.pages || __ldcg(a.c.refs + e) > 1) continue;
         const size_t from = ((size_t)s * a.r.tokens + t) * a.ld + (size_t)h * kDim;
         k[i] = __ldcs(reinterpret_cast<const uint4 *>(a.k + from) + part);
         v[i] = __ldcs(reinterpret_cast<const uint4 *>(a.v + from) + part);
-        to[i] = (((((uint64_t)a.layer * a.c.pages + e) * a.c.kv_heads + h) << a.c.page_log2) + (p & ((1u << a.c.page_log2) - 1u))) * 16u + part;
+        const uint64_t p = p0 + t;
+        if (p >= a.c.limit) continue;
+        e[i] = (uint32_t)__ldcg(a.c.table + (size_t)s * a.c.max_pages + (p >> a.c.page_log2));
+        to[i] = ((((uint64_t)a.layer * a.c.pages * a.c.kv_heads + h) << a.c.page_log2) + (p & ((1u << a.c.page_log2) - 1u))) * 16u + part;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kAppendRows; ++i) {
+        // a page that other sequences have too is not written to
+        if (e[i] < a.c.pages && __ldcg(a.c.refs + e[i]) <= 1) to[i] += ((uint64_t)e[i] * a.c.kv_heads << a.c.page_log2) * 16u;
+        else to[i] = ~0ull;
     }
 #pragma unroll
     for (uint32_t i = 0; i < kAppendRows; ++i)
