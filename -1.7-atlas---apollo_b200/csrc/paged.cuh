@@ -160,6 +160,7 @@ struct Cut {
 struct Piece {
     uint64_t begin, each; // in the line of all; a CTA's share, or 0: pieces are of one unit, and
     uint32_t behind;      // so many pieces of it come before this one
+    uint32_t shared;      // CTAs of a cluster that have the piece together: one unit, whole
     uint32_t s, h, i, skip;
     uint64_t left;
     Seq kept;             // lane s has sequence s, where lanes keep them
@@ -194,10 +195,10 @@ __device__ __forceinline__ uint32_t up_to(uint32_t x)
 // This CTA's piece. All WARPS warps, each for itself where lanes keep the sequences, else together through `sm`, which is
 // free again behind the call. The line is cut into equal pieces of `least` tiles of keys at least; but units that are no
 // more than CTAs are cut one by one if no piece gets longer than that, and left whole if none gets more than `worth`
-// tiles longer (what joining partial sums costs).
+// tiles longer (what joining partial sums costs). In clusters, if there are enough of them, each has a unit together.
 // Of a KV head, at most 32 SLOTS units can be cut one by one.
 template <uint32_t WARPS, uint32_t SLOTS, uint32_t KEYS, uint32_t EXTRA>
-__device__ __forceinline__ Piece find_piece(const Cut<KEYS, EXTRA> &cut, PieceSmem &sm, uint32_t least, uint32_t worth)
+__device__ __forceinline__ Piece find_piece(const Cut<KEYS, EXTRA> &cut, PieceSmem &sm, uint32_t least, uint32_t worth, uint32_t cluster = 1u)
 {
     const AttnArgs &a = cut.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = a.c.nseq;
@@ -205,6 +206,7 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS, EXTRA> &cut, PieceSm
     p.s = p.h = p.i = p.skip = 0u;
     p.begin = p.each = 0u;
     p.behind = 0u;
+    p.shared = 1u;
     p.left = 0u;
     uint32_t most = 0u;
     // the unit of sequence p.s that place `rest` of a KV head's units is in
@@ -266,6 +268,23 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS, EXTRA> &cut, PieceSm
         const uint32_t line = n == 1u ? work * a.c.kv_heads : up_to(work * a.c.kv_heads);
         const uint32_t total = __shfl_sync(0xffffffffu, line, (int)n - 1);
         const uint32_t each = max((total + gridDim.x - 1u) / gridDim.x, least);
+        if (cluster > 1u && all_units * cluster <= gridDim.x && (most + cluster - 1u) / cluster <= each + worth) {
+            const uint32_t u = blockIdx.x / cluster;
+            if (u >= all_units) return p;
+            const uint32_t ends = n == 1u ? all_units : up_to(units * a.c.kv_heads);
+            uint32_t before = 0u;
+            if (n > 1u) {
+                p.s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, lane < n && ends > u)) - 1u;
+                before = __shfl_sync(0xffffffffu, ends, p.s ? (int)p.s - 1 : 0);
+                if (p.s == 0u) before = 0u;
+            }
+            const uint32_t own = __shfl_sync(0xffffffffu, units, (int)p.s);
+            p.h = (u - before) / own;
+            p.i = u - before - p.h * own;
+            p.left = cut.cost(cut.open(p.s, p.kept), p.i);
+            p.shared = cluster;
+            return p;
+        }
         if (all_units <= gridDim.x && all_units <= 32u * SLOTS * a.c.kv_heads) {
             // Units cut into pieces of their own. Lane l has the tiles of sequence and rows number l, l + 32, ..: (sequence,
             // tile) and its work.
@@ -501,6 +520,9 @@ __device__ __forceinline__ float *record_of(const AttnArgs &a, uint32_t i, uint3
     return a.parts + kPartsBytes / 4u + (size_t)i * record_floats(rows);
 }
 
+// What a state (maximum, sum) counts against the maximum M; one that saw no position counts nothing, one of NaN stays
+__device__ __forceinline__ float factor(float2 s, float M) { return s.x == -INFINITY ? (s.y == 0.f ? 0.f : 1.f) : ex2(s.x - M); }
+
 // Four dimensions of an output row
 template <bool BF>
 __device__ __forceinline__ void store4(const AttnArgs &a, uint32_t s, uint32_t h, uint2 at, uint32_t d4, float4 x)
@@ -516,9 +538,11 @@ inline bool lanes_keep(const AttnArgs &a, uint32_t tile, uint32_t keys, uint32_t
     return a.c.nseq <= kKeptSeqs && line < (1ull << 31) && line * ((a.c.limit + keys - 1u) / keys + extra) < (1ull << 31);
 }
 
-// Whatever the positions, each unit will be a piece of its own (find_piece): a sequence has room for no more
-inline bool always_whole(const AttnArgs &a, uint64_t units, uint32_t ctas, uint32_t keys, uint32_t worth, uint32_t slots)
+// Whatever the positions, each unit will be a piece of its own (find_piece), of a CTA or a cluster: a sequence has room for no
+// more
+inline bool always_whole(const AttnArgs &a, uint64_t units, uint32_t ctas, uint32_t keys, uint32_t worth, uint32_t slots, uint32_t cluster = 1)
 {
+    if (cluster > 1 && units * cluster <= ctas && ((a.c.limit + keys - 1u) / keys + cluster - 1u) / cluster <= worth) return true;
     return units <= ctas && (!a.keep || units <= 32ull * slots * a.c.kv_heads) && (a.c.limit + keys - 1u) / keys <= worth;
 }
 

@@ -40,7 +40,7 @@ namespace {
 constexpr uint32_t kChunk = 16, kWarps = 12, kThreads = kWarps * 32, kStages = 2;
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
-constexpr uint32_t kSlots = 1, kWorth = 64, kExtra = 32;      // chunks: what joining partial sums takes, and beginning and ending a unit
+constexpr uint32_t kSlots = 1, kWorth = 96, kExtra = 32;      // chunks: what joining partial sums takes, and beginning and ending a unit
 constexpr float kLazy = 6.0f;
 // Weights are 2^(score - maximum + kUnit). binary16: their largest, 2^15, keeps the low term's bits; bfloat16 has fp32's
 // range, and small weights leave the sums of large values room
@@ -61,6 +61,9 @@ struct alignas(1024) Smem {
     uint64_t full[kWarps][kStages];
     uint32_t err;
     float2 wml[kWarps][8 * NT];
+    // what the cluster's CTAs send: of each, this CTA's share of the rows' dimensions, and all rows' maxima and sums
+    float4 sent[8 * NT * (kDim / 4) + k8::kMaxCluster];
+    float2 sent_ml[k8::kMaxCluster][8 * NT];
 };
 
 template <bool BF>
@@ -121,6 +124,23 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, 
                  : "memory");
 }
 
+// To another CTA of the cluster
+__device__ __forceinline__ void send(const float4 *p, uint32_t cta, float4 v)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(cta));
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(r), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void send(const float2 *p, uint32_t cta, float2 v)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(cta));
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(r), "f"(v.x), "f"(v.y) : "memory");
+}
+// Split: arrive once the CTA runs, wait before the first access to another CTA's shared memory
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // What this thread did to the ring's place comes before the copies that follow
 __device__ __forceinline__ void fence_ring() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -132,7 +152,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     constexpr uint32_t R = 8 * NT;
     extern __shared__ __align__(1024) uint8_t few_smem[];
     Smem<NT> &sm = *reinterpret_cast<Smem<NT> *>(few_smem);
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, cluster = k8::cluster_size();
+    if (cluster > 1u) cluster_arrive();
     if (lane == 0u) {
         for (uint32_t i = 0; i < kStages; ++i) mbar_init(&sm.full[warp][i], 1u);
         fence_mbar_init();
@@ -145,7 +166,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     __syncthreads();
     wait_predecessor(a.early);
     const Cut<kChunk, kExtra> cut{a, R, Divisor{1u << 31, NT == 1 ? 3u : 4u}};
-    const Piece piece = find_piece<kWarps, kSlots>(cut, sm.u.piece, kWarps, kWorth);
+    const Piece piece = find_piece<kWarps, kSlots>(cut, sm.u.piece, kWarps, kWorth, cluster);
+    if (cluster > 1u && (piece.shared == 1u || !piece.left)) cluster_wait();
+    const uint32_t deal = kWarps * piece.shared;   // warps that share a unit's chunks
     Walk<kChunk, kExtra> w(cut, piece);
     if (!a.keep) {                        // the ring's place is free
         fence_ring();
@@ -170,13 +193,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         tr.rem = row0 - tr.tok * a.group;
         const uint64_t p0 = w.q.p0;
         const uint32_t seen = cut.keys(w.q, row0 + rows);          // chunks that some row sees
-        const uint32_t k_end = min(w.k_end, seen), first = w.k_begin + warp;
+        const uint32_t k_end = min(w.k_end, seen), first = w.k_begin + (piece.shared > 1u ? k8::cluster_rank() * kWarps : 0u) + warp;
         const int32_t *const entries = a.c.table + (size_t)s * a.c.max_pages;
         const uint32_t page_chunks = a.c.page_log2 - 4u;           // log2 of chunks per page
         const uint32_t head0 = a.layer * a.c.pages * a.c.kv_heads + h;
-        // the pages of this warp's chunks first + kWarps (base + lane), and of the next 32; their loads are on their way first
+        // the pages of this warp's chunks first + deal (base + lane), and of the next 32; their loads are on their way first
         auto entry_of = [&](uint32_t base) {
-            const uint32_t c = first + kWarps * (base + lane);
+            const uint32_t c = first + deal * (base + lane);
             return c < k_end ? (uint32_t)__ldcg(entries + (c >> page_chunks)) : ~0u;
         };
         uint32_t base = 0u, ent = entry_of(0u), ent_next = entry_of(32u);
@@ -198,14 +221,14 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         auto issue = [&]() -> uint32_t {
             while (!have) {
                 base += 32u;
-                if (first + kWarps * base >= k_end) return kNone;
+                if (first + deal * base >= k_end) return kNone;
                 ent = ent_next;
                 ent_next = entry_of(base + 32u);
                 have = __ballot_sync(0xffffffffu, ent < a.c.pages);
             }
             const uint32_t b = (uint32_t)__ffs((int)have) - 1u;
             have &= have - 1u;
-            const uint32_t e = __shfl_sync(0xffffffffu, ent, (int)b), c = first + kWarps * (base + b);
+            const uint32_t e = __shfl_sync(0xffffffffu, ent, (int)b), c = first + deal * (base + b);
             if (lane == 0u) {
                 const uint32_t row = ((head0 + e * a.c.kv_heads) << a.c.page_log2) + ((c & ((1u << page_chunks) - 1u)) << 4);
                 const uint32_t dst = ring + slot_in * kSlot;
@@ -403,6 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
             }
         __syncthreads();
         const bool whole = w.head && w.tail;
+        const uint32_t share = (R * (kDim / 4u) + piece.shared - 1u) / piece.shared;   // of a unit's sums, for each CTA that has it
+        if (piece.shared > 1u) cluster_wait();
         float *const rec = record_of(a, w.record(), R);
         for (uint32_t x = threadIdx.x; x < rows * (kDim / 4u); x += kThreads) {
             const uint32_t i = x / (kDim / 4u), d = x % (kDim / 4u);
@@ -412,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 #pragma unroll
             for (uint32_t v = 0; v < kWarps; ++v) {
                 const float2 ml = sm.wml[v][i];
-                f[v] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - M);   // a state of NaNs stays one
+                f[v] = factor(ml, M);
                 L = fmaf(f[v], ml.y, L);
             }
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -424,12 +449,39 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
                 y.z = fmaf(f[v], z.z, y.z);
                 y.w = fmaf(f[v], z.w, y.w);
             }
-            if (whole) {
+            if (piece.shared > 1u) {
+                const uint32_t to = x / share, rank = k8::cluster_rank();
+                send(&sm.sent[rank * share + (x - to * share)], to, y);
+                if (d < cluster) send(&sm.sent_ml[rank][i], d, make_float2(M, L));
+            } else if (whole) {
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
                 store4<BF>(a, s, h, tr.at(i), d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
                 __stcg(reinterpret_cast<float4 *>(rec) + i * (kDim / 4u) + d, y);
                 if (d == 0u) __stcg(reinterpret_cast<float2 *>(rec + R * kDim) + i, make_float2(M, L));
+            }
+        }
+        if (piece.shared > 1u) {          // each CTA of the cluster joins its share
+            k8::cluster_sync();           // nothing remote is touched from here on
+            const uint32_t x = k8::cluster_rank() * share + threadIdx.x, i = x / (kDim / 4u), d = x % (kDim / 4u);
+            static_assert(R * (kDim / 4u) <= 2u * kThreads, "a thread has one of the share's");
+            if (threadIdx.x < share && i < rows) {
+                float M = -INFINITY, L = 0.f;
+                for (uint32_t c = 0; c < cluster; ++c) M = fmaxf(M, sm.sent_ml[c][i].x);
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                for (uint32_t c = 0; c < cluster; ++c) {
+                    const float2 ml = sm.sent_ml[c][i];
+                    const float4 z = sm.sent[c * share + threadIdx.x];
+                    const float f = factor(ml, M);
+                    L = fmaf(f, ml.y, L);
+                    y.x = fmaf(f, z.x, y.x);
+                    y.y = fmaf(f, z.y, y.y);
+                    y.z = fmaf(f, z.z, y.z);
+                    y.w = fmaf(f, z.w, y.w);
+                }
+                const float inv = L == 0.f ? 0.f : 1.0f / L;
+                store4<BF>(a, s, h, tr.at(i), d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             }
         }
         fence_ring();
@@ -494,8 +546,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __gr
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             most = fmaxf(most, M[u]);
-            const float before = M[u] == -INFINITY ? (L[u] == 0.f ? 0.f : 1.f) : ex2(M[u] - most);
-            f[u] = ml[u].x == -INFINITY ? (ml[u].y == 0.f ? 0.f : 1.f) : ex2(ml[u].x - most);
+            const float before = factor(make_float2(M[u], L[u]), most);
+            f[u] = factor(ml[u], most);
             float sum = f[u] * ml[u].y;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -528,12 +580,24 @@ __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __gr
     }
 }
 
+// CTAs that share a unit, and CTAs in all: the largest clusters that give each unit one, all on the device at once, with a
+// round of chunks for each CTA; else none, and all SMs
 template <bool BF, int NT>
-cudaError_t launch_few_of(const FewArgs &a, int dev, int sms, cudaStream_t stream)
+cudaError_t launch_few_of(const FewArgs &a, uint64_t units, int dev, int sms, uint32_t &cluster, uint32_t &ctas, cudaStream_t stream)
 {
     const cudaError_t e = k8::allow<few_kernel<BF, NT>>(dev, (int)sizeof(Smem<NT>));
     if (e != cudaSuccess) return e;
-    return k8::launch(few_kernel<BF, NT>, dim3(std::min((uint32_t)sms, kMaxCtas)), kThreads, sizeof(Smem<NT>), 1, a, sms, stream);
+    cluster = 1;
+    ctas = std::min((uint32_t)sms, kMaxCtas);
+    const uint32_t rounds = (a.c.limit + kChunk * kWarps - 1) / (kChunk * kWarps);
+    for (uint32_t c = std::min({k8::kMaxCluster, rounds, (uint32_t)(units <= (uint64_t)sms ? sms / units : 0)}); a.keep && c > 1; --c) {
+        const uint32_t n = std::min(k8::clusters_at_once<few_kernel<BF, NT>>(dev, c, kThreads, sizeof(Smem<NT>)), kMaxCtas / c);
+        if (n < units) continue;
+        cluster = c;
+        ctas = n * c;
+        break;
+    }
+    return k8::launch(few_kernel<BF, NT>, dim3(ctas), kThreads, sizeof(Smem<NT>), cluster, a, sms, stream);
 }
 
 }  // namespace
@@ -563,12 +627,12 @@ cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtenso
     f.kmap = kmap;
     f.vmap = vmap;
     f.keep = lanes_keep(a, 8u * (uint32_t)nt, kChunk, kExtra);
-    const cudaError_t e = nt == 1 ? (bf ? launch_few_of<true, 1>(f, dev, sms, stream) : launch_few_of<false, 1>(f, dev, sms, stream))
-                                  : (bf ? launch_few_of<true, 2>(f, dev, sms, stream) : launch_few_of<false, 2>(f, dev, sms, stream));
-    if (e != cudaSuccess) return e;
-    const uint32_t rows = 8u * (uint32_t)nt, ctas = std::min((uint32_t)sms, kMaxCtas);
+    const uint32_t rows = 8u * (uint32_t)nt;
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * (((uint64_t)a.r.tokens * a.group + rows - 1) / rows);
-    if (always_whole(f, units, ctas, kChunk, kWorth, kSlots)) return cudaSuccess;
+    uint32_t cluster, ctas;
+    const cudaError_t e = nt == 1 ? (bf ? launch_few_of<true, 1>(f, units, dev, sms, cluster, ctas, stream) : launch_few_of<false, 1>(f, units, dev, sms, cluster, ctas, stream))
+                                  : (bf ? launch_few_of<true, 2>(f, units, dev, sms, cluster, ctas, stream) : launch_few_of<false, 2>(f, units, dev, sms, cluster, ctas, stream));
+    if (e != cudaSuccess || always_whole(f, units, ctas, kChunk, kWorth, kSlots, cluster)) return e;
     return launch_merge(a, bf, rows, ctas, sms, stream);
 }
 

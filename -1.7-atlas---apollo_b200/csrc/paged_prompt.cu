@@ -153,9 +153,6 @@ struct Ring {
     }
 };
 
-// What a state (maximum, sum) counts against the maximum M; one that saw no position counts nothing, one of NaN stays
-__device__ __forceinline__ float factor(float2 s, float M) { return s.x == -INFINITY ? (s.y == 0.f ? 0.f : 1.f) : ex2(s.x - M); }
-
 template <bool BF, bool ONE>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs a)
 {
