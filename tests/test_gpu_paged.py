@@ -242,3 +242,68 @@ def test_captured_step_replays(torch_cuda):
         ref.append(0, p, [3] * nseq, k.cpu(), k.cpu())
         assert ref.compact() == int(dev.out)
         dev.equals(torch, ref)
+
+
+def test_many_copies(torch_cuda):
+    """More to copy than one cluster is given: forks of one sequence that each go on inside its last page, in several layers."""
+    torch = torch_cuda
+    nseq, layers, heads, page = 60, 4, 3, 64
+    ref, dev = _both(torch, "fp16", layers, 200, heads, page, nseq, 4, seed=3)
+    assert _reserve(torch, ref, dev, [0] * nseq, [150] + [0] * (nseq - 1)) == 0
+    _fork(torch, ref, dev, [0] * nseq, [150 - s for s in range(nseq)])
+    assert _reserve(torch, ref, dev, [150 - s for s in range(nseq)], [1 + s % 3 for s in range(nseq)]) == 0
+    dev.equals(torch, ref)
+    _compact(torch, ref, dev)
+    dev.equals(torch, ref)
+
+
+@pytest.mark.parametrize("nseq,tokens,pages", [(3, 400, 90), (1024, 16, 1100), (40, 700, 2000)])
+def test_more_entries_than_threads_or_as_many(torch_cuda, nseq, tokens, pages):
+    """Reservations of about a thousand entries and more, of pages that sequences share."""
+    torch = torch_cuda
+    width = -(-tokens // 16) + 2
+    ref, dev = _both(torch, "bf16", 1, pages, 1, 16, nseq, width, seed=nseq)
+    _reserve(torch, ref, dev, [0] * nseq, [min(tokens, 16 * (pages // (2 * nseq)) + 5)] * nseq)
+    dev.equals(torch, ref)
+    _fork(torch, ref, dev, [s // 3 for s in range(nseq)], [tokens] * nseq)
+    dev.equals(torch, ref)
+    _reserve(torch, ref, dev, [7 * (s % 2) for s in range(nseq)], [tokens if s % 4 else 0 for s in range(nseq)])
+    dev.equals(torch, ref)
+
+
+def test_first_calls_inside_a_capture(torch_cuda):
+    """A program whose first calls of all are captured: nothing they set up at first use spoils the capture. In a process of its
+    own, with both forms of attention."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path[:0] = %r
+import atlas_cuda
+pool = lambda: torch.zeros(2, 40, 2, 32, 128, dtype=torch.bfloat16, device="cuda")
+table = torch.full((2, 16), -1, dtype=torch.int32, device="cuda")
+c = atlas_cuda.PagedCache(pool(), pool(), table, torch.zeros(40, dtype=torch.int32, device="cuda"))
+i = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+pos, zero, parent, length, short = i(0, 0), i(0, 0), i(0, 1), i(0, 0), i(5)
+q = torch.ones(2, 300, 4, 128, dtype=torch.bfloat16, device="cuda")
+out, one = torch.zeros_like(q), torch.zeros(2, 1, 4, 128, dtype=torch.bfloat16, device="cuda")
+k = torch.ones(2, 300, 2, 128, dtype=torch.bfloat16, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    atlas_cuda.paged_fork(c, parent, length, stream=s)
+    atlas_cuda.paged_reserve(c, 300, pos, short, stream=s)
+    atlas_cuda.paged_compact(c, short, stream=s)
+    atlas_cuda.paged_reserve(c, 300, pos, short, stream=s)
+    atlas_cuda.paged_append(c, 1, 300, pos, k, k, stream=s)
+    atlas_cuda.paged_attn(c, 1, 4, 300, pos, q, out, stream=s)
+    atlas_cuda.paged_attn(c, 1, 4, 1, pos, q[:, :1].contiguous(), one, stream=s)
+for _ in range(2):
+    g.replay()
+torch.cuda.synchronize()
+assert int(short) == 0 and bool((out == 1).all()) and bool((one == 1).all())
+""" % ([os.path.dirname(atlas_cuda.__file__)],)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

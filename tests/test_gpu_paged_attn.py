@@ -302,3 +302,54 @@ def test_refusals_on_the_device(torch_cuda):
             f()
     torch.cuda.synchronize()
     assert torch.equal(out, before)
+
+
+def test_two_graphs_of_one_cache(torch_cuda):
+    """A prompt's graph and a decode step's, captured over one cache and its workspace, replayed in turn on one stream."""
+    torch = torch_cuda
+    x = Setup(torch, "bf16", 32, 2, [1500, 1300], 60, seed=31)
+    long_q, step_q = x.rand(2, 200, 10, DIM), x.rand(2, 1, 10, DIM)
+    long_out, step_out = torch.zeros_like(long_q), torch.zeros_like(step_q)
+    long_pos, step_pos = _i32(torch, [1300, 1100]), _i32(torch, [1499, 1299])
+    want = x.attn(long_q, [1300, 1100]), x.attn(step_q, [1499, 1299])
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for g, args in zip(graphs, ((200, long_pos, long_q, long_out), (1, step_pos, step_q, step_out))):
+        with torch.cuda.graph(g):
+            atlas_cuda.paged_attn(x.c, 0, 10, *args, stream=torch.cuda.current_stream().cuda_stream)
+    for _ in range(10):
+        for g in graphs + graphs[::-1]:
+            g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(long_out, want[0]) and torch.equal(step_out, want[1])
+
+
+@pytest.mark.parametrize("kvh,grp,lens,tokens", [(1, 7, [5000], 1), (2, 8, [9000], 1), (8, 5, [8447], 1), (4, 7, [640] * 5, 1), (4, 7, [3000, 10, 700], 1), (8, 5, [2000] * 9, 1),
+                                                 (1, 5, [20, 9000, 300, 40], 2), (6, 5, [4000, 3900, 3800], 3), (16, 1, [1000] * 9, 1), (3, 4, [100, 20000], 4)])
+def test_units_shared_by_clusters_and_not(torch_cuda, kvh, grp, lens, tokens):
+    """Few sequences (a cluster has a unit), many or uneven ones (a line of all), with room for much more than they have."""
+    torch = torch_cuda
+    x = Setup(torch, "fp16", 64, kvh, lens, 600, seed=sum(lens))
+    pos = [n - tokens for n in lens]
+    q = x.rand(len(lens), tokens, kvh * grp, DIM)
+    out = x.attn(q, pos)
+    x.check(out, q, pos)
+    assert torch.equal(out, x.attn(q, pos))
+
+
+def test_a_row_goes_by_what_it_sees(torch_cuda):
+    """Other rows' queries, and keys and values behind it, change no bit of a row."""
+    torch = torch_cuda
+    for tokens in (3, 60, 500):
+        x = Setup(torch, "bf16", 16, 2, [300 + tokens], 60, seed=8)
+        q = x.rand(1, tokens, 10, DIM)
+        out = x.attn(q, [300])
+        t = tokens // 2
+        other = q.clone()
+        other[:, :t] = x.rand(1, t, 10, DIM, size=5.0)
+        other[:, t + 1:] = x.rand(1, tokens - t - 1, 10, DIM, size=5.0)
+        e = x.table[0].long()[torch.arange(300 + t + 1, 300 + tokens, device="cuda") // 16]
+        at = torch.arange(300 + t + 1, 300 + tokens, device="cuda") % 16
+        x.k[0, e, :, at] = x.rand(tokens - t - 1, 2, DIM, size=5.0)
+        x.v[0, e, :, at] = x.rand(tokens - t - 1, 2, DIM, size=5.0)
+        assert torch.equal(x.attn(other, [300])[0, t], out[0, t])
