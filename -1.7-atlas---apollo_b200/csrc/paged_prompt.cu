@@ -61,7 +61,7 @@ static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "what the softma
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 values, swizzled
 constexpr uint32_t kTile = 2 * kHalf;
 constexpr uint32_t kMaxStages = 6;
-constexpr uint32_t kSlots = 4, kWorth = 4, kExtra = 3;   // tiles of keys: what joining partial sums takes, and beginning and ending a unit
+constexpr uint32_t kSlots = 4, kWorth = 6, kExtra = 3;   // tiles of keys: what joining partial sums takes, and beginning and ending a unit
 constexpr float kLazy = 8.0f;
 // Weights are 2^(score - maximum + kUnit): binary16 keeps 24 bits below the largest; bfloat16 has fp32's range, and small
 // weights leave the sums of large values room
