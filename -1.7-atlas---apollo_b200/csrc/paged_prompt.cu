@@ -240,7 +240,29 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 const bool more = w.more();
                 if (i >= kSteps) ok = wait_warp(&b.step_free[i % kSteps], (i / kSteps - 1u) & 1u, err);
                 if (!ok) break;
-                const uint32_t n = more ? w.k_end - w.k_begin : 0u;
+                const uint32_t n = more ? w.k_end - w.k_begin : 0u, k_begin = w.k_begin;
+                // this lane's page of the step's tile j, and where it begins; the first ones' loads are on their way first of all
+                const uint32_t seen = more ? (uint32_t)min((uint64_t)w.q.p0 + divide(w.row0() + w.rows() - 1u, a.by_group) + 1u, (uint64_t)a.c.limit) : 0u;
+                const int32_t *const entries = a.c.table + (size_t)w.p.s * a.c.max_pages;
+                const uint32_t head0 = a.layer * a.c.pages * a.c.kv_heads + w.p.h;
+                auto page_of = [&](uint32_t j) {
+                    const uint32_t e = ((k_begin + j) << per) + of;
+                    return mine && j < n && (uint64_t)e << page_log2 < seen ? (uint32_t)__ldcg(entries + e) : ~0u;
+                };
+                auto row_of = [&](uint32_t e) { return e < a.c.pages ? (head0 + e * a.c.kv_heads) << page_log2 : nowhere; };
+                uint32_t page = page_of(0u), page_next = page_of(1u);
+                const uint32_t tiles = more ? tiles_of(w.rows()) : 0u, tok0 = more ? divide(w.row0(), a.by_group) : 0u;
+                if (more) {
+                    if (i) ok = wait_warp(&b.q_free, (i - 1u) & 1u, err);
+                    if (!ok) break;
+                    if (lane == 0u) {
+                        mbar_arrive_expect_tx(&b.q_full, tiles * tile_rows * 256u);
+                        for (uint32_t t = 0; t < tiles; ++t)
+                            for (uint32_t hf = 0; hf < 2u; ++hf)
+                                load_queries(smem_addr(qs + t * kTile + hf * kHalf), &a.qmap, w.p.h * a.group, w.p.s * a.r.tokens + tok0 + t * a.tokens_per_tile, hf,
+                                             &b.q_full);
+                    }
+                }
                 if (lane == 0u) {
                     Step &st = b.step[i % kSteps];
                     st.n = n;
@@ -249,9 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         st.s = w.p.s;
                         st.h = w.p.h;
                         st.rows = w.rows();
-                        st.tok0 = divide(w.row0(), a.by_group);
+                        st.tok0 = tok0;
                         st.p0 = w.q.p0;
-                        st.k_begin = w.k_begin;
+                        st.k_begin = k_begin;
                         st.record = w.record();
                         st.again = w.again ? 1u : 0u;
                         st.whole = w.leaves() && w.head && w.tail ? 1u : 0u;
@@ -260,26 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 __syncwarp();
                 if (!more) break;
-                const uint32_t tiles = tiles_of(w.rows()), k_begin = w.k_begin;
-                const uint32_t seen = (uint32_t)min((uint64_t)w.q.p0 + divide(w.row0() + w.rows() - 1u, a.by_group) + 1u, (uint64_t)a.c.limit);
-                const int32_t *const entries = a.c.table + (size_t)w.p.s * a.c.max_pages;
-                const uint32_t head0 = a.layer * a.c.pages * a.c.kv_heads + w.p.h;
-                // where this lane's page of the step's tile j begins
-                auto page_row = [&](uint32_t j) {
-                    const uint32_t e0 = ((k_begin + j) << per) + of;
-                    const uint32_t e = mine && j < n && (uint64_t)e0 << page_log2 < seen ? (uint32_t)__ldcg(entries + e0) : ~0u;
-                    return e < a.c.pages ? (head0 + e * a.c.kv_heads) << page_log2 : nowhere;
-                };
-                uint32_t at = page_row(0u), next = page_row(1u);
-                if (i) ok = wait_warp(&b.q_free, (i - 1u) & 1u, err);
-                if (!ok) break;
-                if (lane == 0u) {
-                    mbar_arrive_expect_tx(&b.q_full, tiles * tile_rows * 256u);
-                    const uint32_t token = w.p.s * a.r.tokens + divide(w.row0(), a.by_group);
-                    for (uint32_t t = 0; t < tiles; ++t)
-                        for (uint32_t hf = 0; hf < 2u; ++hf)
-                            load_queries(smem_addr(qs + t * kTile + hf * kHalf), &a.qmap, w.p.h * a.group, token + t * a.tokens_per_tile, hf, &b.q_full);
-                }
+                uint32_t at = row_of(page), next = row_of(page_next);
                 // which of a tile's 16 positions have a page, for the softmax warps; before K's copies, whose end they wait for
                 auto tell = [&](uint32_t row) {
                     const uint32_t have = __ballot_sync(0xffffffffu, mine && row != nowhere);   // lane 2 i: page i
@@ -305,14 +308,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     copy(&a.kmap, at);
                 }
                 for (uint32_t j = 0; ok && j < n; ++j) {
-                    const uint32_t after = page_row(j + 2u);
+                    page = page_of(j + 2u);
                     if (!ONE || j + 1u < n) {
                         tell(ONE ? next : at);
                         copy(&a.kmap, ONE ? next : at);
                     }
                     copy(&a.vmap, at);
                     at = next;
-                    next = after;
+                    next = row_of(page);
                 }
                 if (!ok) break;
                 w.next();

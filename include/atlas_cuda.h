@@ -348,7 +348,11 @@ int atlas_cuda_kv8_attn_sparse(const AtlasKv8 *cache, uint32_t q_heads, uint32_t
    pos0[s], pos0[s] + 1, ... Rows from n_tok[s] on are left as they were, so 0
    leaves a sequence out. Token rows are [seq][tokens][heads][128] values of the
    cache's type, `ld` values from token to token (0: dense; a multiple of 8; the
-   sequence stride is tokens * ld), 16-byte aligned. */
+   sequence stride is tokens * ld), 16-byte aligned.
+
+   Every wait in a kernel is bounded; one that runs out (which only a fault of the
+   device could bring about) leaves NaN in the rows concerned of an attention,
+   after the call has returned ATLAS_OK: nothing else reports it. */
 #define ATLAS_PAGED_FP16 0u
 #define ATLAS_PAGED_BF16 1u
 
