@@ -248,15 +248,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
             if (x < R * 16u) *reinterpret_cast<uint4 *>(&sm.q[x / 16u][8u * (x % 16u)]) = qv[k];
         }
         __syncthreads();
-        // B operands: column g, dimensions 16 st + 2 t, + 1, + 8, + 9
-        uint32_t qf[NT][8][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        // B operands: column g, dimensions 16 st + 2 t, + 1, + 8, + 9. Those of two tiles of rows stay in shared memory: with them
+        // in registers, too, the loop spills
+        auto operand = [&](int nt, int st, int half) { return *reinterpret_cast<const uint32_t *>(&sm.q[8u * (uint32_t)nt + g][16 * st + 8 * half + 2u * t]); };
+        uint32_t qf[NT == 1 ? 8 : 1][2];
+        if (NT == 1)
 #pragma unroll
             for (int st = 0; st < 8; ++st) {
-                qf[nt][st][0] = *reinterpret_cast<const uint32_t *>(&sm.q[8u * (uint32_t)nt + g][16 * st + 2u * t]);
-                qf[nt][st][1] = *reinterpret_cast<const uint32_t *>(&sm.q[8u * (uint32_t)nt + g][16 * st + 8 + 2u * t]);
+                qf[NT == 1 ? st : 0][0] = operand(0, st, 0);
+                qf[NT == 1 ? st : 0][1] = operand(0, st, 1);
             }
+        auto query = [&](int nt, int st, int half) { return NT == 1 ? qf[NT == 1 ? st : 0][half] : operand(nt, st, half); };
         uint32_t last[NT][2];             // the last position that columns 2 t and 2 t + 1 see
         const uint32_t open = (uint32_t)min(p0 + tr.tok, (uint64_t)0x7fffffffu);   // every row sees the positions up to it
 #pragma unroll
@@ -292,11 +294,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     if (st == 0u) {
-                        mma_first<BF>(y[nt], ka, qf[nt][0][0], qf[nt][0][1]);
-                        mma_first<BF>(y2[nt], kb, qf[nt][4][0], qf[nt][4][1]);
+                        mma_first<BF>(y[nt], ka, query(nt, 0, 0), query(nt, 0, 1));
+                        mma_first<BF>(y2[nt], kb, query(nt, 4, 0), query(nt, 4, 1));
                     } else {
-                        mma<BF>(y[nt], ka, qf[nt][st][0], qf[nt][st][1]);
-                        mma<BF>(y2[nt], kb, qf[nt][4 + st][0], qf[nt][4 + st][1]);
+                        mma<BF>(y[nt], ka, query(nt, (int)st, 0), query(nt, (int)st, 1));
+                        mma<BF>(y2[nt], kb, query(nt, (int)st + 4, 0), query(nt, (int)st + 4, 1));
                     }
                 }
             }
