@@ -192,13 +192,160 @@ __device__ __forceinline__ uint32_t up_to(uint32_t x)
     return x;
 }
 
-// This CTA's piece. All WARPS warps, each for itself where lanes keep the sequences, else together through `sm`, which is
-// free again behind the call. The line is cut into equal pieces of `least` tiles of keys at least; but units that are no
-// more than CTAs are cut one by one if no piece gets longer than that, and left whole if none gets more than `worth`
-// tiles longer (what joining partial sums costs). In clusters, if there are enough of them, each has a unit together.
-// Of a KV head, at most 32 SLOTS units can be cut one by one.
-template <uint32_t WARPS, uint32_t SLOTS, uint32_t KEYS, uint32_t EXTRA>
-__device__ __forceinline__ Piece find_piece(const Cut<KEYS, EXTRA> &cut, PieceSmem &sm, uint32_t least, uint32_t worth, uint32_t cluster = 1u)
+// The unit of sequence p.s that place `rest` of a KV head's units is in, from its place in the line
+template <class T, uint32_t KEYS, uint32_t EXTRA>
+__device__ __forceinline__ void enter_unit(const Cut<KEYS, EXTRA> &cut, Piece &p, T rest)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    const Seq q = cut.open(p.s, p.kept);
+    const uint32_t units = cut.units(q);
+    for (uint32_t b = 0; units > 1u; b += 32u) {
+        const uint32_t c = b + lane < units ? cut.cost(q, b + lane) + EXTRA : 0u;
+        const T x = up_to((T)c);
+        const uint32_t past = __ballot_sync(0xffffffffu, x > rest);
+        if (past || b + 32u >= units) {
+            const uint32_t at = past ? (uint32_t)__ffs((int)past) - 1u : 31u;
+            p.i = min(b + at, units - 1u);
+            rest -= __shfl_sync(0xffffffffu, x - c, (int)at);
+            break;
+        }
+        rest -= __shfl_sync(0xffffffffu, x, 31);
+    }
+    // what lies before the first tile of keys is not work
+    const uint32_t place = (uint32_t)rest;
+    p.skip = place > EXTRA ? place - EXTRA : 0u;
+    if (place < EXTRA) p.left -= min(p.left, (uint64_t)(EXTRA - place));
+}
+
+// This CTA's piece where a warp's lanes keep the sequences; by each warp that wants it, for itself. The line is cut into equal
+// pieces of `least` tiles of keys at least; but units that are no more than CTAs (and 32 of a KV head) are cut one by one
+// if no piece gets longer than that, and left whole if none gets more than `worth` tiles longer (what joining partial
+// sums costs). In clusters, if there are enough of them, each has a unit together. (Short code on purpose: its first run after
+// a launch waits for its instructions; with up to 128 units of a KV head in four registers a lane, a prompt's calls
+// took 2 to 4 us longer.)
+template <uint32_t KEYS, uint32_t EXTRA>
+__device__ __forceinline__ Piece find_kept(const Cut<KEYS, EXTRA> &cut, uint32_t least, uint32_t worth, uint32_t cluster = 1u)
+{
+    const AttnArgs &a = cut.a;
+    const uint32_t lane = threadIdx.x & 31u, n = a.c.nseq;
+    Piece p;
+    p.s = p.h = p.i = p.skip = 0u;
+    p.begin = p.each = 0u;
+    p.behind = 0u;
+    p.shared = 1u;
+    p.left = 0u;
+    uint32_t most = 0u;
+    const bool there = lane < n;
+    const uint32_t e0 = there ? (uint32_t)__ldcg(a.c.table + (size_t)lane * a.c.max_pages) : 0u;
+    p.kept.p0 = there ? __ldcg(a.r.pos0 + lane) : 0u;
+    p.kept.rows = there ? row_count(a.r, lane) * a.group : 0u;
+    p.kept.k0 = 0u;
+    for (uint32_t gone = __ballot_sync(0xffffffffu, p.kept.rows && e0 >= a.c.pages); gone; gone &= gone - 1u) {
+        const uint32_t s = (uint32_t)__ffs((int)gone) - 1u;
+        const uint32_t k0 = cut.begin(s, __shfl_sync(0xffffffffu, p.kept.p0, (int)s), __shfl_sync(0xffffffffu, p.kept.rows, (int)s));
+        if (lane == s) p.kept.k0 = k0;
+    }
+    // lane s: its sequence's units and work per KV head
+    const uint32_t units = p.kept.rows ? cut.units(p.kept) : 0u;
+    uint32_t work = 0u;
+    if (__all_sync(0xffffffffu, units <= 4u)) {
+        for (uint32_t i = 0; i < units; ++i) {
+            const uint32_t c = cut.cost(p.kept, i);
+            work += c + EXTRA;
+            most = max(most, c);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+    } else {
+        for (uint32_t s = 0; s < n; ++s) {
+            const uint32_t sum = (uint32_t)cut.all(cut.open(s, p.kept), most);
+            if (lane == s) work = sum;
+        }
+    }
+    // the line up to the end of each sequence
+    const uint32_t all_units = __reduce_add_sync(0xffffffffu, units) * a.c.kv_heads;
+    const uint32_t line = n == 1u ? work * a.c.kv_heads : up_to(work * a.c.kv_heads);
+    const uint32_t total = __shfl_sync(0xffffffffu, line, (int)n - 1);
+    if (!total) return p;
+    const uint32_t each = max((total + gridDim.x - 1u) / gridDim.x, least);
+    if (cluster > 1u && all_units * cluster <= gridDim.x && (most + cluster - 1u) / cluster <= each + worth) {
+        const uint32_t u = blockIdx.x / cluster;
+        if (u >= all_units) return p;
+        const uint32_t ends = n == 1u ? all_units : up_to(units * a.c.kv_heads);
+        uint32_t before = 0u;
+        if (n > 1u) {
+            p.s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, lane < n && ends > u)) - 1u;
+            before = __shfl_sync(0xffffffffu, ends, p.s ? (int)p.s - 1 : 0);
+            if (p.s == 0u) before = 0u;
+        }
+        const uint32_t own = __shfl_sync(0xffffffffu, units, (int)p.s);
+        p.h = (u - before) / own;
+        p.i = u - before - p.h * own;
+        p.left = cut.cost(cut.open(p.s, p.kept), p.i);
+        p.shared = cluster;
+        return p;
+    }
+    if (all_units <= gridDim.x && all_units <= 32u * a.c.kv_heads) {
+        // Units cut into pieces of their own. Lane l has tile number l of all sequences' tiles of rows: its sequence, its number
+        // there and its work.
+        uint32_t seq = lane, tile = 0u, cost = units ? work - EXTRA : 0u;
+        if (!__all_sync(0xffffffffu, units <= 1u)) {
+            const uint32_t tiles_to = up_to(units), all_tiles = __shfl_sync(0xffffffffu, tiles_to, 31);
+            seq = 0u;
+#pragma unroll
+            for (uint32_t step = 16u; step; step >>= 1)
+                if (__shfl_sync(0xffffffffu, tiles_to, (int)(seq + step - 1u)) <= lane) seq += step;
+            tile = lane - (__shfl_sync(0xffffffffu, tiles_to, (int)seq) - __shfl_sync(0xffffffffu, units, (int)seq));
+            const Seq q = cut.open_each(seq, p.kept);
+            cost = lane < all_tiles ? cut.cost(q, tile) : 0u;
+        }
+        // The pieces' size: sum ceil(work / size) <= CTAs holds where size >= total / (CTAs - units), as rounding up adds
+        // less than one a unit, and where every unit gets as many pieces as the largest one
+        uint32_t size = most;
+        if (most > each + worth) {
+            size = (most + gridDim.x / all_units - 1u) / (gridDim.x / all_units);
+            if (all_units < gridDim.x) size = min(size, (total - all_units * EXTRA) / (gridDim.x - all_units) + 1u);
+            size = max(size, least);
+            if (size + worth >= most) size = most;
+        }
+        if (size == most ? most <= each + worth : size <= each) {
+            const uint32_t cuts = (cost + size - 1u) / size, ends = up_to(cuts * a.c.kv_heads);
+            const uint32_t mine = __ballot_sync(0xffffffffu, ends > blockIdx.x);
+            if (!mine) return p;
+            const int l = __ffs((int)mine) - 1;
+            const uint32_t own_cuts = __shfl_sync(0xffffffffu, cuts, l), c = __shfl_sync(0xffffffffu, cost, l);
+            const uint32_t at = blockIdx.x - (__shfl_sync(0xffffffffu, ends, l) - own_cuts * a.c.kv_heads);
+            p.s = __shfl_sync(0xffffffffu, seq, l);
+            p.i = __shfl_sync(0xffffffffu, tile, l);
+            p.h = at / own_cuts;
+            p.behind = at - p.h * own_cuts;
+            // as even as can be
+            const uint32_t even = c / own_cuts, more = c - even * own_cuts;
+            p.skip = p.behind * even + min(p.behind, more);
+            p.left = even + (p.behind < more ? 1u : 0u);
+            return p;
+        }
+    }
+    p.each = each;
+    const uint32_t at = each * blockIdx.x;
+    if (at >= total) return p;
+    uint32_t before = 0u;
+    if (n > 1u) {
+        p.s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, lane < n && line > at)) - 1u;
+        before = __shfl_sync(0xffffffffu, line, p.s ? (int)p.s - 1 : 0);
+        if (p.s == 0u) before = 0u;
+    }
+    const uint32_t of_head = __shfl_sync(0xffffffffu, work, (int)p.s);
+    p.h = (at - before) / of_head;
+    p.begin = at;
+    p.left = min(each, total - at);
+    enter_unit(cut, p, at - before - of_head * p.h);
+    return p;
+}
+
+// The same for any number of sequences; by all WARPS warps together through `sm`, which is free again behind the call. Units are
+// pieces of their own, or the line is cut.
+template <uint32_t WARPS, uint32_t KEYS, uint32_t EXTRA>
+__device__ __forceinline__ Piece find_together(const Cut<KEYS, EXTRA> &cut, PieceSmem &sm, uint32_t least, uint32_t worth)
 {
     const AttnArgs &a = cut.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, n = a.c.nseq;
@@ -209,161 +356,6 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS, EXTRA> &cut, PieceSm
     p.shared = 1u;
     p.left = 0u;
     uint32_t most = 0u;
-    // the unit of sequence p.s that place `rest` of a KV head's units is in
-    auto unit_at = [&](auto rest) {
-        using T = decltype(rest);
-        const Seq q = cut.open(p.s, p.kept);
-        const uint32_t units = cut.units(q);
-        // a place in the unit -> tiles of keys before it; what lies before the first one is not work
-        auto enter = [&](uint32_t place) {
-            p.skip = place > EXTRA ? place - EXTRA : 0u;
-            if (place < EXTRA) p.left -= min(p.left, (uint64_t)(EXTRA - place));
-        };
-        if (units == 1u) {
-            enter((uint32_t)rest);
-            return;
-        }
-        for (uint32_t b = 0;; b += 32u) {
-            const uint32_t c = b + lane < units ? cut.cost(q, b + lane) + EXTRA : 0u;
-            const T x = up_to((T)c);
-            const uint32_t past = __ballot_sync(0xffffffffu, x > rest);
-            if (past || b + 32u >= units) {
-                const uint32_t at = past ? (uint32_t)__ffs((int)past) - 1u : 31u;
-                p.i = min(b + at, units - 1u);
-                enter((uint32_t)(rest - __shfl_sync(0xffffffffu, x - c, (int)at)));
-                return;
-            }
-            rest -= __shfl_sync(0xffffffffu, x, 31);
-        }
-    };
-    if (a.keep) {
-        const bool there = lane < n;
-        const uint32_t e0 = there ? (uint32_t)__ldcg(a.c.table + (size_t)lane * a.c.max_pages) : 0u;
-        p.kept.p0 = there ? __ldcg(a.r.pos0 + lane) : 0u;
-        p.kept.rows = there ? row_count(a.r, lane) * a.group : 0u;
-        p.kept.k0 = 0u;
-        for (uint32_t gone = __ballot_sync(0xffffffffu, p.kept.rows && e0 >= a.c.pages); gone; gone &= gone - 1u) {
-            const uint32_t s = (uint32_t)__ffs((int)gone) - 1u;
-            const uint32_t k0 = cut.begin(s, __shfl_sync(0xffffffffu, p.kept.p0, (int)s), __shfl_sync(0xffffffffu, p.kept.rows, (int)s));
-            if (lane == s) p.kept.k0 = k0;
-        }
-        // lane s: its sequence's units and work per KV head
-        const uint32_t units = p.kept.rows ? cut.units(p.kept) : 0u;
-        uint32_t work = 0u;
-        if (__all_sync(0xffffffffu, units <= 4u)) {
-            for (uint32_t i = 0; i < units; ++i) {
-                const uint32_t c = cut.cost(p.kept, i);
-                work += c + EXTRA;
-                most = max(most, c);
-            }
-            most = __reduce_max_sync(0xffffffffu, most);
-        } else {
-            for (uint32_t s = 0; s < n; ++s) {
-                const uint32_t sum = (uint32_t)cut.all(cut.open(s, p.kept), most);
-                if (lane == s) work = sum;
-            }
-        }
-        // the line up to the end of each sequence
-        const uint32_t all_units = __reduce_add_sync(0xffffffffu, units) * a.c.kv_heads;
-        const uint32_t line = n == 1u ? work * a.c.kv_heads : up_to(work * a.c.kv_heads);
-        const uint32_t total = __shfl_sync(0xffffffffu, line, (int)n - 1);
-        const uint32_t each = max((total + gridDim.x - 1u) / gridDim.x, least);
-        if (cluster > 1u && all_units * cluster <= gridDim.x && (most + cluster - 1u) / cluster <= each + worth) {
-            const uint32_t u = blockIdx.x / cluster;
-            if (u >= all_units) return p;
-            const uint32_t ends = n == 1u ? all_units : up_to(units * a.c.kv_heads);
-            uint32_t before = 0u;
-            if (n > 1u) {
-                p.s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, lane < n && ends > u)) - 1u;
-                before = __shfl_sync(0xffffffffu, ends, p.s ? (int)p.s - 1 : 0);
-                if (p.s == 0u) before = 0u;
-            }
-            const uint32_t own = __shfl_sync(0xffffffffu, units, (int)p.s);
-            p.h = (u - before) / own;
-            p.i = u - before - p.h * own;
-            p.left = cut.cost(cut.open(p.s, p.kept), p.i);
-            p.shared = cluster;
-            return p;
-        }
-        if (all_units <= gridDim.x && all_units <= 32u * SLOTS * a.c.kv_heads) {
-            // Units cut into pieces of their own. Lane l has the tiles of sequence and rows number l, l + 32, ..: (sequence,
-            // tile) and its work.
-            uint32_t seq[SLOTS], tile[SLOTS], cost[SLOTS], pairs = n;
-            const bool single = __all_sync(0xffffffffu, units <= 1u);
-#pragma unroll
-            for (uint32_t k = 0; k < SLOTS; ++k) seq[k] = tile[k] = cost[k] = 0u;
-            if (single) {
-                seq[0] = lane;
-                cost[0] = units ? work - EXTRA : 0u;
-            } else {
-                const uint32_t pairs_to = n == 1u ? units : up_to(units);
-                pairs = __shfl_sync(0xffffffffu, pairs_to, (int)n - 1);
-#pragma unroll
-                for (uint32_t k = 0; k < SLOTS; ++k) {
-                    const uint32_t x = 32u * k + lane;
-                    if (32u * k >= pairs) break;
-                    if (n > 1u)
-#pragma unroll
-                        for (uint32_t step = 16u; step; step >>= 1)
-                            if (__shfl_sync(0xffffffffu, pairs_to, (int)(seq[k] + step - 1u)) <= x) seq[k] += step;
-                    seq[k] = min(seq[k], n - 1u);
-                    const uint32_t upto = __shfl_sync(0xffffffffu, pairs_to, (int)seq[k]), own = __shfl_sync(0xffffffffu, units, (int)seq[k]);
-                    const Seq q = cut.open_each(seq[k], p.kept);
-                    tile[k] = x - (upto - own);
-                    if (x < pairs) cost[k] = cut.cost(q, tile[k]);
-                }
-            }
-            // The pieces' size: sum ceil(work / size) <= CTAs holds where size >= total / (CTAs - units), as rounding up adds
-            // less than one a unit, and where every unit gets as many pieces as the largest one
-            uint32_t size = most;
-            if (most > each + worth) {
-                size = (most + gridDim.x / all_units - 1u) / (gridDim.x / all_units);
-                if (all_units < gridDim.x) size = min(size, (total - all_units * EXTRA) / (gridDim.x - all_units) + 1u);
-                size = max(size, least);
-                if (size + worth >= most) size = most;
-            }
-            if (size == most ? most <= each + worth : size <= each) {
-                uint32_t at = blockIdx.x;
-#pragma unroll
-                for (uint32_t k = 0; k < SLOTS; ++k) {
-                    if (32u * k >= pairs) break;
-                    const uint32_t cuts = (cost[k] + size - 1u) / size, ends = up_to(cuts * a.c.kv_heads), all = __shfl_sync(0xffffffffu, ends, 31);
-                    if (at >= all) {
-                        at -= all;
-                        continue;
-                    }
-                    const int l = __ffs((int)__ballot_sync(0xffffffffu, ends > at)) - 1;
-                    const uint32_t own_cuts = __shfl_sync(0xffffffffu, cuts, l), c = __shfl_sync(0xffffffffu, cost[k], l);
-                    at -= __shfl_sync(0xffffffffu, ends, l) - own_cuts * a.c.kv_heads;
-                    p.s = __shfl_sync(0xffffffffu, seq[k], l);
-                    p.i = __shfl_sync(0xffffffffu, tile[k], l);
-                    p.h = at / own_cuts;
-                    p.behind = at - p.h * own_cuts;
-                    // as even as can be
-                    const uint32_t even = c / own_cuts, more = c - even * own_cuts;
-                    p.skip = p.behind * even + min(p.behind, more);
-                    p.left = even + (p.behind < more ? 1u : 0u);
-                    break;
-                }
-                return p;
-            }
-        }
-        p.each = each;
-        const uint32_t at = each * blockIdx.x;
-        if (at >= total) return p;
-        uint32_t before = 0u;
-        if (n > 1u) {
-            p.s = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, lane < n && line > at)) - 1u;
-            before = __shfl_sync(0xffffffffu, line, p.s ? (int)p.s - 1 : 0);
-            if (p.s == 0u) before = 0u;
-        }
-        const uint32_t of_head = __shfl_sync(0xffffffffu, work, (int)p.s);
-        p.h = (at - before) / of_head;
-        p.begin = at;
-        p.left = min(each, total - at);
-        unit_at(at - before - of_head * p.h);
-        return p;
-    }
     for (uint32_t s = warp; s < n; s += WARPS) {
         const Seq q = cut.open(s);
         const uint64_t sum = cut.all(q, most);
@@ -430,7 +422,7 @@ __device__ __forceinline__ Piece find_piece(const Cut<KEYS, EXTRA> &cut, PieceSm
         p.left = cut.cost(q, p.i);
     } else {
         p.h = (uint32_t)quotient(p.begin - before, of_head);
-        unit_at(p.begin - before - of_head * p.h);
+        enter_unit(cut, p, p.begin - before - of_head * p.h);
     }
     return p;
 }
@@ -538,12 +530,12 @@ inline bool lanes_keep(const AttnArgs &a, uint32_t tile, uint32_t keys, uint32_t
     return a.c.nseq <= kKeptSeqs && line < (1ull << 31) && line * ((a.c.limit + keys - 1u) / keys + extra) < (1ull << 31);
 }
 
-// Whatever the positions, each unit will be a piece of its own (find_piece), of a CTA or a cluster: a sequence has room for no
+// Whatever the positions, each unit will be a piece of its own (find_kept, find_together), of a CTA or a cluster: a sequence has room for no
 // more
-inline bool always_whole(const AttnArgs &a, uint64_t units, uint32_t ctas, uint32_t keys, uint32_t worth, uint32_t slots, uint32_t cluster = 1)
+inline bool always_whole(const AttnArgs &a, uint64_t units, uint32_t ctas, uint32_t keys, uint32_t worth, uint32_t cluster = 1)
 {
     if (cluster > 1 && units * cluster <= ctas && ((a.c.limit + keys - 1u) / keys + cluster - 1u) / cluster <= worth) return true;
-    return units <= ctas && (!a.keep || units <= 32ull * slots * a.c.kv_heads) && (a.c.limit + keys - 1u) / keys <= worth;
+    return units <= ctas && (!a.keep || units <= 32ull * a.c.kv_heads) && (a.c.limit + keys - 1u) / keys <= worth;
 }
 
 }  // namespace

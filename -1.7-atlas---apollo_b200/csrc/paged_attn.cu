@@ -40,7 +40,7 @@ namespace {
 constexpr uint32_t kChunk = 16, kWarps = 12, kThreads = kWarps * 32, kStages = 2;
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
-constexpr uint32_t kSlots = 1, kWorth = 96, kExtra = 32;      // chunks: what joining partial sums takes, and beginning and ending a unit
+constexpr uint32_t kWorth = 96, kExtra = 32;      // chunks: what joining partial sums takes, and beginning and ending a unit
 constexpr float kLazy = 6.0f;
 // Weights are 2^(score - maximum + kUnit). binary16: their largest, 2^15, keeps the low term's bits; bfloat16 has fp32's
 // range, and small weights leave the sums of large values room
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     __syncthreads();
     wait_predecessor(a.early);
     const Cut<kChunk, kExtra> cut{a, R, Divisor{1u << 31, NT == 1 ? 3u : 4u}};
-    const Piece piece = find_piece<kWarps, kSlots>(cut, sm.u.piece, kWarps, kWorth, cluster);
+    const Piece piece = a.keep ? find_kept(cut, kWarps, kWorth, cluster) : find_together<kWarps>(cut, sm.u.piece, kWarps, kWorth);
     if (cluster > 1u && (piece.shared == 1u || !piece.left)) cluster_wait();
     const uint32_t deal = kWarps * piece.shared;   // warps that share a unit's chunks
     Walk<kChunk, kExtra> w(cut, piece);
@@ -175,6 +175,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         fence_ring();
         __syncthreads();
     }
+    auto tell_part = [&]() {
+        const Part part = w.part();
+        if (lane == 0u) reinterpret_cast<Part *>(a.parts)[blockIdx.x] = part;
+    };
+    if (!w.more() && warp == kWarps - 1u) tell_part();
     const uint32_t ring = smem_addr(sm.u.ring[warp][0]);
     uint64_t *const full = sm.full[warp];
     // where ldmatrix reads: K of 16 dimensions (16 positions x 2 chunks), V of 16 dimensions (the same, to be transposed)
@@ -241,6 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         uint32_t chunk[kStages];          // on their way; kNone: nothing more
 #pragma unroll
         for (uint32_t i = 0; i < kStages; ++i) chunk[i] = issue();
+        if (w.first && warp == kWarps - 1u) tell_part();
 
 #pragma unroll
         for (uint32_t k = 0; k < sizeof(qv) / 16u; ++k) {
@@ -503,10 +509,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
         fence_ring();
         __syncthreads();                  // the ring may fill again
     }
-    if (warp == 0u) {
-        const Part part = Walk<kChunk, kExtra>(cut, piece).part();
-        if (lane == 0u) reinterpret_cast<Part *>(a.parts)[blockIdx.x] = part;
-    }
 }
 
 // --------------------------------------------------------- partial sums ----
@@ -648,7 +650,7 @@ cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtenso
     uint32_t cluster, ctas;
     const cudaError_t e = nt == 1 ? (bf ? launch_few_of<true, 1>(f, units, dev, sms, cluster, ctas, stream) : launch_few_of<false, 1>(f, units, dev, sms, cluster, ctas, stream))
                                   : (bf ? launch_few_of<true, 2>(f, units, dev, sms, cluster, ctas, stream) : launch_few_of<false, 2>(f, units, dev, sms, cluster, ctas, stream));
-    if (e != cudaSuccess || always_whole(f, units, ctas, kChunk, kWorth, kSlots, cluster)) return e;
+    if (e != cudaSuccess || always_whole(f, units, ctas, kChunk, kWorth, cluster)) return e;
     return launch_merge(a, bf, rows, ctas, sms, stream);
 }
 

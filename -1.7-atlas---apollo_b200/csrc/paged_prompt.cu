@@ -61,7 +61,7 @@ static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "what the softma
 constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 values, swizzled
 constexpr uint32_t kTile = 2 * kHalf;
 constexpr uint32_t kMaxStages = 6;
-constexpr uint32_t kSlots = 4, kWorth = 6, kExtra = 3;   // tiles of keys: what joining partial sums takes, and beginning and ending a unit
+constexpr uint32_t kWorth = 6, kExtra = 3;   // tiles of keys: what joining partial sums takes, and beginning and ending a unit
 constexpr float kLazy = 8.0f;
 // Weights are 2^(score - maximum + kUnit): binary16 keeps 24 bits below the largest; bfloat16 has fp32's range, and small
 // weights leave the sums of large values room
@@ -111,7 +111,7 @@ constexpr size_t kSmem = (ONE ? 1 : 2) * kTile + kStages<ONE> * kTile + sizeof(B
 template <bool ONE>
 constexpr uint32_t kRecordRows = ONE ? kTileRows : 2 * kTileRows;
 static_assert(kSmem<true> <= k8::kMaxSmem && kSmem<false> <= k8::kMaxSmem, "the tiles exceed a CTA's shared memory");
-static_assert(sizeof(PieceSmem) <= 2 * kTile, "find_piece works in the stages' place");
+static_assert(sizeof(PieceSmem) <= 2 * kTile, "find_together works in the stages' place");
 
 // fp32 accumulator, M = 128, N = 128; A and B of one 16-bit type; B as rows along N where ACROSS
 template <bool BF, bool ACROSS>
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const Cut<kTileKeys, kExtra> cut{a, (ONE ? 1u : 2u) * tile_rows, a.by_tile};
     Piece piece;
     piece.left = 0u;
-    if (!a.keep) piece = find_piece<kThreads / 32u, kSlots>(cut, *reinterpret_cast<PieceSmem *>(kv), 2u, kWorth);
+    if (!a.keep) piece = find_together<kThreads / 32u>(cut, *reinterpret_cast<PieceSmem *>(kv), 2u, kWorth);
     fence_before();
     fence_async();
     __syncthreads();
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         if (warp == kLoadWarp) {
             // ------------------------------------------- plan and copies --
             // The only warp that follows the piece through its units; the others get steps. It is ahead of them all.
-            if (a.keep) piece = find_piece<kThreads / 32u, kSlots>(cut, *reinterpret_cast<PieceSmem *>(kv), 2u, kWorth);
+            if (a.keep) piece = find_kept(cut, 2u, kWorth);
             Walk<kTileKeys, kExtra, kMostTiles> w(cut, piece);
             Ring<STAGES> ring;
             uint32_t used = 0u, i = 0u, number = 0u;   // copies so far; steps; tiles of keys
@@ -832,7 +832,7 @@ cudaError_t launch_prompt(const AttnArgs &a, const CUtensorMap &kmap, const CUte
     if (e != cudaSuccess) return e;
     const uint32_t ctas = std::min((uint32_t)sms, kMaxCtas), per = tiles * p.tokens_per_tile;
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * ((a.r.tokens + per - 1) / per);
-    if (always_whole(p, units, ctas, kTileKeys, kWorth, kSlots)) return cudaSuccess;
+    if (always_whole(p, units, ctas, kTileKeys, kWorth)) return cudaSuccess;
     return launch_merge(a, bf, tiles * kTileRows, ctas, sms, stream);
 }
 
