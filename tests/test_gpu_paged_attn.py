@@ -353,3 +353,19 @@ def test_a_row_goes_by_what_it_sees(torch_cuda):
         x.k[0, e, :, at] = x.rand(tokens - t - 1, 2, DIM, size=5.0)
         x.v[0, e, :, at] = x.rand(tokens - t - 1, 2, DIM, size=5.0)
         assert torch.equal(x.attn(other, [300])[0, t], out[0, t])
+
+
+@pytest.mark.parametrize("kvh,grp,pos,tokens,ntok", [
+    (1, 1, [5 * i for i in range(32)], 200, [37 * i % 201 for i in range(32)]), (1, 1, [0], 4300, None), (1, 1, [0], 4096, None), (2, 1, [0] * 31 + [900], 40, None),
+    (1, 4, list(range(33)), 100, [0] * 32 + [100]), (1, 4, list(range(32)), 100, [0] * 31 + [100]), (3, 2, [100] * 16, 140, [0] * 7 + [140] + [0] * 8),
+    (1, 2, [300] * 32, 8, [8, 0] * 16), (1, 2, [300] * 33, 8, [0, 0, 8] * 11), (2, 8, [50] * 32, 6, [0] * 32), (2, 8, [50] * 33, 6, [0] * 33), (1, 1, [0], 18000, None)])
+def test_sequences_and_units_at_the_edges(torch_cuda, kvh, grp, pos, tokens, ntok):
+    """As many sequences and tiles of rows as a warp has lanes, one more, and sequences without rows around those that have some."""
+    torch = torch_cuda
+    lens = [p + (tokens if ntok is None else ntok[s]) for s, p in enumerate(pos)]
+    for width in (-(-max(lens) // 32), 700):   # with room for what they have, and for much more
+        x = Setup(torch, "fp16", 32, kvh, lens, width, seed=len(pos) + tokens)
+        q = x.rand(len(pos), tokens, kvh * grp, DIM)
+        out = x.attn(q, pos, ntok)
+        x.check(out, q, pos, ntok, sample=2)
+        assert torch.equal(out, x.attn(q, pos, ntok))
