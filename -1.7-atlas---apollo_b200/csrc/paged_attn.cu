@@ -45,10 +45,13 @@ namespace {
 constexpr uint32_t kChunk = 16, kWarps = 12, kThreads = kWarps * 32, kStages = 2;
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
-// chunks: what joining partial sums takes, and beginning and ending a unit. With 48 instead of 96: 8447 positions 12.7 us
-// instead of 11.5, 8 sequences over 2303 14.2 instead of 13.3, but 16 heads on 2 over 32767 16.0 instead of 18.7; with 8
-// instead of 32 nothing changes by 1 %
-constexpr uint32_t kWorth = 96, kExtra = 32;
+// Chunks: what joining partial sums takes, where a sequence has no room for more than leaves none, so that the launch
+// that joins them is left out (640 positions 6.8 us instead of 8.2; 8447 11.5 instead of 12.7), and where it follows in any case;
+// and what beginning and ending a unit takes. With 95, 48 or 32 instead of 64: 16 heads on 2 over 32767 18.8, 15.2 or 15.2 us
+// instead of 15.1; 28 on 4 over 20000 16.2, 16.2 or 14.2 instead of 16.2; 40 on 8 over 30000 27.5, 28.6 or 28.6 instead of 27.5. With
+// 8 instead of 32 for a unit's ends nothing changes by 1 %.
+constexpr uint32_t kWorth = 96, kWorthMore = 64, kExtra = 32;
+static_assert(kWorthMore < kWorth, "it tells a call that may leave partial sums");
 constexpr float kLazy = 6.0f;
 // Weights are 2^(score - maximum + kUnit). binary16: their largest, 2^15, keeps the low term's bits; bfloat16 has fp32's
 // range, and small weights leave the sums of large values room
@@ -57,6 +60,7 @@ constexpr float kUnit = BF ? -24.0f : 9.0f;
 
 struct FewArgs : AttnArgs {
     CUtensorMap kmap, vmap;      // [2][rows of the pool][64] each
+    uint32_t worth;              // so many chunks longer may a CTA's work get before units are cut
 };
 
 template <int NT>
@@ -175,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     __syncthreads();
     wait_predecessor(a.early);
     const Cut<kChunk, kExtra> cut{a, R, Divisor{1u << 31, NT == 1 ? 3u : 4u}};
-    const Piece piece = a.keep ? find_kept(cut, kWarps, kWorth, cluster) : find_together<kWarps>(cut, sm.u.piece, kWarps, kWorth);
+    const Piece piece = a.keep ? find_kept(cut, kWarps, a.worth, cluster) : find_together<kWarps>(cut, sm.u.piece, kWarps, a.worth);
     if (cluster > 1u && (piece.shared == 1u || !piece.left)) cluster_wait();
     const uint32_t deal = kWarps * piece.shared;   // warps that share a unit's chunks
     Walk<kChunk, kExtra> w(cut, piece);
@@ -524,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 // The units that pieces cut: the CTAs whose number is that of the piece that a
 // unit ends in join its records, a warp one or two rows (lane: a record's maximum
 // and sum, then 4 dimensions), with the first records' loads on their way before
-// their weights are known. Bound by latency (7.0 us behind a chunk's call, cold and
+// their weights are known. Bound by latency (6.6 us behind a chunk's call, cold and
 // alone); a call whose pieces are whole units leaves nothing to join, and one that
 // cannot leave anything does not launch this.
 struct MergeArgs : AttnArgs {
@@ -610,11 +614,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) part_merge_kernel(const __gr
 // CTAs that share a unit, and CTAs in all: the largest clusters that give each unit one, all on the device at once, with a
 // round of chunks for each CTA; else none, and all SMs
 template <bool BF, int NT>
-cudaError_t launch_few_of(const FewArgs &a, uint64_t units, int dev, int sms, uint32_t &cluster, uint32_t &ctas, cudaStream_t stream)
+cudaError_t launch_few_of(FewArgs &a, uint64_t units, int dev, int sms, uint32_t &ctas, cudaStream_t stream)
 {
     const cudaError_t e = k8::allow<few_kernel<BF, NT>>(dev, (int)sizeof(Smem<NT>));
     if (e != cudaSuccess) return e;
-    cluster = 1;
+    uint32_t cluster = 1;
     ctas = std::min((uint32_t)sms, kMaxCtas);
     const uint32_t rounds = (a.c.limit + kChunk * kWarps - 1) / (kChunk * kWarps);
     for (uint32_t c = std::min({k8::kMaxCluster, rounds, (uint32_t)(units <= (uint64_t)sms ? sms / units : 0)}); a.keep && c > 1; --c) {
@@ -624,6 +628,7 @@ cudaError_t launch_few_of(const FewArgs &a, uint64_t units, int dev, int sms, ui
         ctas = n * c;
         break;
     }
+    a.worth = always_whole(a, units, ctas, kChunk, kWorth, cluster) ? kWorth : kWorthMore;
     return k8::launch(few_kernel<BF, NT>, dim3(ctas), kThreads, sizeof(Smem<NT>), cluster, a, sms, stream);
 }
 
@@ -656,10 +661,10 @@ cudaError_t launch_few(const AttnArgs &a, const CUtensorMap &kmap, const CUtenso
     f.keep = lanes_keep(a, 8u * (uint32_t)nt, kChunk, kExtra);
     const uint32_t rows = 8u * (uint32_t)nt;
     const uint64_t units = (uint64_t)a.c.nseq * a.c.kv_heads * (((uint64_t)a.r.tokens * a.group + rows - 1) / rows);
-    uint32_t cluster, ctas;
-    const cudaError_t e = nt == 1 ? (bf ? launch_few_of<true, 1>(f, units, dev, sms, cluster, ctas, stream) : launch_few_of<false, 1>(f, units, dev, sms, cluster, ctas, stream))
-                                  : (bf ? launch_few_of<true, 2>(f, units, dev, sms, cluster, ctas, stream) : launch_few_of<false, 2>(f, units, dev, sms, cluster, ctas, stream));
-    if (e != cudaSuccess || always_whole(f, units, ctas, kChunk, kWorth, cluster)) return e;
+    uint32_t ctas;
+    const cudaError_t e = nt == 1 ? (bf ? launch_few_of<true, 1>(f, units, dev, sms, ctas, stream) : launch_few_of<false, 1>(f, units, dev, sms, ctas, stream))
+                                  : (bf ? launch_few_of<true, 2>(f, units, dev, sms, ctas, stream) : launch_few_of<false, 2>(f, units, dev, sms, ctas, stream));
+    if (e != cudaSuccess || f.worth == kWorth) return e;
     return launch_merge(a, bf, rows, ctas, sms, stream);
 }
 
