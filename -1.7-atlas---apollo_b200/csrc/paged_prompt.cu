@@ -35,9 +35,9 @@
 //
 // Bound by the chain of a row tile's scores, softmax and second product, about 3200
 // cycles per 128 keys, of which two run: the tensor pipe and the exponentials are both
-// busy 57 % of the time. 8192 tokens of 40 heads on 8: 627 us with the partial sums, 1.10
-// PFLOP/s, 66 % of the measured bfloat16 rate; 690 when repeated under the power cap. A
-// quarter of the exponentials on the FMA units instead: 633 where this took 623. Short
+// busy 57 % of the time. 8192 tokens of 40 heads on 8: 671 us with the partial sums, 1.02
+// PFLOP/s, 61 % of the measured bfloat16 rate; 757 when repeated under the power cap. A
+// quarter of the exponentials on the FMA units instead: 633 where a build took 623. Short
 // calls are bound by what comes before the first scores and behind the last: 512 tokens
 // of 28 heads on 4 15.0 us, 7 tokens of 4 sequences over 8001 28.3.
 #include <algorithm>
