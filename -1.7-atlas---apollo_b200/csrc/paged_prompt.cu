@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         }
         for (uint32_t i = 0; i < STAGES; ++i) {
             mbar_init(&b.full[i], 1u);
-            mbar_init(&b.free[i], 1u);
+            mbar_init(&b.free[i], 1u + kCheckers);     // the MMAs and the warps that look through V
             mbar_init(&b.checked[i], kCheckers);
         }
         for (uint32_t i = 0; i < kSteps; ++i) {
@@ -500,13 +500,18 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             leave();
         } else {
             // ------------------------------------------------------ checks --
-            // Every copy is waited for, in order: a barrier tells a phase only from the one before.
+            // Every copy is waited for, in order: a barrier tells a phase only from the one before. So that the next copy into a slot
+            // is not done before a warp has seen this one, each arrives on the slot's `free`, too.
             Ring<STAGES> ring;
             uint32_t i = 0u;
             bool ok = true;
+            auto leave_slot = [&]() {
+                if (lane == 0u) mbar_arrive(&b.free[ring.slot]);
+                ring.next();
+            };
             auto pass = [&]() {
                 ok = ok && wait_warp(&b.full[ring.slot], ring.phase, err);
-                ring.next();
+                if (ok) leave_slot();
             };
             for (; ok && there_is(i); ++i) {
                 Step &st = b.step[i % kSteps];
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         __syncwarp();
                         if (lane == 0u) mbar_arrive(&b.checked[ring.slot]);
                     }
-                    ring.next();
+                    leave_slot();
                 }
                 done_with(i);
             }
