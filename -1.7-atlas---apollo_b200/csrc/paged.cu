@@ -6,6 +6,7 @@
 // pool of pages, and one page may be part of several of them.
 #include <algorithm>
 #include <atomic>
+#include <utility>
 #include <cuda.h>
 #include "../../include/atlas_cuda.h"
 #include "paged.cuh"
@@ -576,6 +577,10 @@ bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0;
 
 constexpr uint32_t kMaxRecordRows = 256;
 
+// What a call may have: query heads, values from token to token, tokens of all sequences
+constexpr uint32_t kMaxHeads = 32768u;
+constexpr uint64_t kMaxStep = 0xffffffffull, kMaxRows = 0x7fffffffull;
+
 size_t parts_offset(uint32_t pages)
 {
     return (sizeof(WorkHead) + (size_t)kWorkArrays * pages * 4u + 255u) & ~(size_t)255u;
@@ -655,11 +660,27 @@ int check_rows(const char *who, const void *p, uint32_t heads, uint64_t &ld, int
 {
     if (!p) return api_fail(ATLAS_EINVAL, "%s: null argument", who);
     if (!ld) ld = (uint64_t)heads * kDim;
-    if (ld < (uint64_t)heads * kDim || ld % 8 || ld > 0xffffffffull)
+    if (ld < (uint64_t)heads * kDim || ld % 8 || ld > kMaxStep)
         return api_fail(ATLAS_EINVAL, "%s: token rows %llu values apart: at least heads x 128, a multiple of 8", who, (unsigned long long)ld);
     if (!aligned(p, 16)) return api_fail(ATLAS_EINVAL, "%s: token rows must be 16-byte aligned", who);
     if (!on_device(p, dev)) return api_fail(ATLAS_EINVAL, "%s: token rows must be memory of the current device", who);
     return ATLAS_OK;
+}
+
+// Whether `n` rows of `width` values from a on, lda values apart, share memory with rows of b, ldb apart (at least `width` each).
+// Rows the same distance apart may lie beside one another, as in a buffer of both; others share it where their ranges do.
+bool rows_overlap(const void *a, uint64_t lda, const void *b, uint64_t ldb, uint64_t width, uint64_t n)
+{
+    if ((uintptr_t)a > (uintptr_t)b) {
+        std::swap(a, b);
+        std::swap(lda, ldb);
+    }
+    const uint64_t ahead = (uintptr_t)b - (uintptr_t)a, bytes = 2 * width, step = 2 * lda;   // b's first row lies `ahead` behind a's
+    if (ahead >= (n - 1) * step + bytes) return false;
+    if (lda != ldb || n == 1) return true;
+    // b's first row begins in the step of a's row `ahead` / `step`; the next of a's, if there is one, may reach into its end
+    const uint64_t row = ahead / step, in = ahead - row * step;
+    return in < bytes || (row + 1 < n && step - in < bytes);
 }
 
 using Encode = decltype(&cuTensorMapEncodeTiled);
@@ -837,8 +858,8 @@ int map_queries(const char *who, Encode encode, const AttnArgs &a, bool bf, uint
 
 int check_heads(const char *who, const AtlasPaged *cache, uint32_t q_heads, uint32_t tokens)
 {
-    if (!q_heads || q_heads % cache->kv_heads || q_heads > 32768u || (uint64_t)q_heads * tokens > 0x3fffffffull ||
-        (uint64_t)tokens * cache->nseq > 0x7fffffffull)
+    if (!q_heads || q_heads % cache->kv_heads || q_heads > kMaxHeads || (uint64_t)q_heads * tokens > 0x3fffffffull ||
+        (uint64_t)tokens * cache->nseq > kMaxRows)
         return api_fail(ATLAS_EINVAL, "%s: %u query heads over %u KV heads, %u tokens", who, q_heads, cache->kv_heads, tokens);
     return ATLAS_OK;
 }
@@ -862,9 +883,15 @@ extern "C" int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, ui
 {
     const char *who = "paged_attn";
     AttnArgs a{};
+    int dev, sms, rc = cache ? check_shape(who, cache) : ATLAS_OK;
+    if (rc != ATLAS_OK) return rc;
     // a row of `out` may be written before another CTA has read its neighbours in `q`
-    if (d_q && d_q == d_out && tokens) return api_fail(ATLAS_EINVAL, "%s: out must not be q", who);
-    int dev, sms, rc = open_cache(who, cache, a.c, dev, sms);
+    if (cache && d_q && d_out && tokens && q_heads && q_heads <= kMaxHeads) {   // sizes past the limits are refused below
+        const uint64_t width = (uint64_t)q_heads * kDim, lq = ldq ? ldq : width, lo = ldo ? ldo : width, n = (uint64_t)cache->nseq * tokens;
+        if (lq >= width && lo >= width && lq <= kMaxStep && lo <= kMaxStep && n <= kMaxRows && rows_overlap(d_q, lq, d_out, lo, width, n))
+            return api_fail(ATLAS_EINVAL, "%s: q and out must not overlap", who);
+    }
+    rc = open_cache(who, cache, a.c, dev, sms);
     if (rc == ATLAS_OK) rc = check_tokens(who, tokens, d_pos0, d_ntok, a.r, dev);
     if (rc != ATLAS_OK) return rc;
     if ((rc = check_heads(who, cache, q_heads, tokens)) != ATLAS_OK) return rc;

@@ -410,7 +410,8 @@ int atlas_cuda_paged_append(const AtlasPaged *cache, uint32_t layer, uint32_t to
    zeros. What lies at positions that a row does not see has no part in it,
    infinities and NaN among it; a value that is not finite at a position that it
    does see makes what it enters infinite or NaN. q_heads is a multiple of
-   kv_heads; q and out must not overlap. Which kernels run, and so the last bits
+   kv_heads; q and out that overlap are refused (their rows may lie beside one
+   another in one buffer, with ldq = ldo). Which kernels run, and so the last bits
    of a row, depends on the call's sizes and positions; the same call gives the
    same bits. */
 int atlas_cuda_paged_attn(const AtlasPaged *cache, uint32_t layer, uint32_t q_heads, uint32_t tokens, const uint32_t *d_pos0,
