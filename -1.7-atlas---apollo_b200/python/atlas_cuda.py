@@ -467,7 +467,8 @@ def _kv8_ints(who: str, name: str, t, n: int) -> None:
 
 def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: int, kind: str = "float32") -> None:
     """Refuses a tensor that is not token rows [nseq, tokens, heads, 128] of type `kind`, ld values from token to token (0:
-    dense). One that is not 4-dimensional must be dense, and long enough."""
+    dense). One that is not 4-dimensional must be dense, and long enough; so may one of just the size be whose dimensions put
+    the same rows in the same places ([nseq, heads, 1, 128] of one token)."""
     if not tokens or not hasattr(t, "dtype"):
         return
     step = ld or heads * 128
@@ -475,7 +476,9 @@ def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: in
         shape, stride = t.shape, t.stride()
         ok = (shape[0] >= nseq and shape[1] >= tokens and shape[2] >= heads and shape[3] == 128 and stride[3] == 1
               and (heads == 1 or stride[2] == 128) and (tokens == 1 or stride[1] == step)
-              and (nseq == 1 or stride[0] == tokens * step))
+              and (nseq == 1 or stride[0] == tokens * step)
+              or t.is_contiguous() and t.numel() == nseq * tokens * step and step == heads * 128 and shape[3] % 128 == 0
+              and (tokens == 1 or heads == 1 or shape[2] * shape[3] == step))
     else:
         ok = t.is_contiguous() and t.numel() >= (nseq * tokens - 1) * step + heads * 128
     if not ok or _kind(t) != kind:
@@ -484,12 +487,12 @@ def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: in
 
 
 def _kv8_check(who: str, cache: Kv8Cache, tokens: int, heads: int, pos0, n_tok, names, a, lda: int, b, ldb: int) -> None:
-    """Refuses tensors of another type, layout or size. a, b: rows of `heads` each. Dense ones of just the size, as most
+    """Refuses tensors of another type, layout or size. a, b: rows of `heads` each. Dense ones of just the shape, as most
     calls have, pass at once."""
     n = cache.nseq
-    size, f32, i32 = n * tokens * heads * 512, cache._f32, cache._i32
+    shape, f32, i32 = (n, tokens, heads, 128), cache._f32, cache._i32
     try:
-        if (a.dtype is f32 and b.dtype is f32 and pos0.dtype is i32 and a.nbytes == size and b.nbytes == size
+        if (a.dtype is f32 and b.dtype is f32 and pos0.dtype is i32 and a.shape == shape and b.shape == shape
                 and pos0.nbytes == 4 * n and a.is_contiguous() and b.is_contiguous() and pos0.is_contiguous()
                 and (n_tok is None or n_tok.dtype is i32 and n_tok.nbytes == 4 * n and n_tok.is_contiguous())
                 and not lda and not ldb):
@@ -592,10 +595,10 @@ def _paged_ints(who: str, cache: PagedCache, name: str, t, n: int) -> None:
 
 def _paged_check(who: str, cache: PagedCache, tokens: int, heads: int, pos0, n_tok, names=(), a=None, lda: int = 0, b=None,
                  ldb: int = 0) -> None:
-    """Refuses tensors of another type, layout or size. a, b: rows of `heads` each, or None. Dense ones of just the size, as
+    """Refuses tensors of another type, layout or size. a, b: rows of `heads` each, or None. Dense ones of just the shape, as
     most calls have, pass at once."""
-    n, size, kind, i32 = cache.nseq, cache.nseq * tokens * heads * 256, cache.dtype, cache._i32
-    if ((a is None or a.dtype is kind and b.dtype is kind and a.nbytes == size and b.nbytes == size and not lda and not ldb
+    n, shape, kind, i32 = cache.nseq, (cache.nseq, tokens, heads, 128), cache.dtype, cache._i32
+    if ((a is None or a.dtype is kind and b.dtype is kind and a.shape == shape and b.shape == shape and not lda and not ldb
          and a.is_contiguous() and b.is_contiguous())
             and pos0.dtype is i32 and pos0.nbytes == 4 * n and pos0.is_contiguous()
             and (n_tok is None or n_tok.dtype is i32 and n_tok.nbytes == 4 * n and n_tok.is_contiguous())):
