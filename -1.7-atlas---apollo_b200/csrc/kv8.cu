@@ -1336,9 +1336,11 @@ int map_codes(const char *who, FewArgs &a)
     const cuuint64_t dims[2] = {kDim, rows}, strides[1] = {kDim};
     const cuuint32_t box[2] = {kDim, kChunk}, steps[2] = {1, 1};
     for (int i = 0; i < 2; ++i)
-        if (encode(i ? &a.vmap : &a.kmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i ? a.c.v : a.c.k, dims, strides, box, steps,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        if (!in_context([&] {
+                return encode(i ? &a.vmap : &a.kmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i ? a.c.v : a.c.k, dims, strides, box, steps,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            }))
             return api_fail(ATLAS_ECUDA, "%s: the codes cannot be described to the copy engine", who);
     return ATLAS_OK;
 }

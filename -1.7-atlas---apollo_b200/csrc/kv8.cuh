@@ -146,6 +146,16 @@ cudaError_t allow(int dev, int bytes)
     return e;
 }
 
+// f(), which describes memory to the copy engine. That goes by the thread's current context, which none of the calls before it
+// set: where it fails, the first such call of a host thread may have come too early, so once more with the device's context.
+template <class F>
+bool in_context(F f)
+{
+    if (f()) return true;
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && f();
+}
+
 constexpr size_t kMaxSmem = 232448;   // shared memory a CTA may have
 constexpr uint32_t kMaxCluster = 16;
 

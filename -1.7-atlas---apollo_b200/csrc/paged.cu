@@ -721,9 +721,11 @@ int map_pool(const char *who, Encode encode, const Cache &c, bool bf, void *pool
     const cuuint64_t rows = ((cuuint64_t)c.layers * c.pages * c.kv_heads) << c.page_log2;
     const cuuint64_t dims[3] = {kDim / 2, rows, 2}, strides[2] = {kRowBytes, kRowBytes / 2};
     const cuuint32_t boxes[3] = {kDim / 2, box, halves}, steps[3] = {1, 1, 1};
-    if (encode(&map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, pool, dims, strides, boxes, steps,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    if (!k8::in_context([&] {
+            return encode(&map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, pool, dims, strides, boxes, steps,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        }))
         return api_fail(ATLAS_ECUDA, "%s: the pool cannot be described to the copy engine", who);
     return ATLAS_OK;
 }
@@ -861,9 +863,11 @@ int map_queries(const char *who, Encode encode, const AttnArgs &a, bool bf, uint
 {
     const cuuint64_t dims[4] = {kDim / 2, a.q_heads, (cuuint64_t)a.c.nseq * a.r.tokens, 2}, strides[3] = {kRowBytes, a.ldq * 2, kRowBytes / 2};
     const cuuint32_t boxes[4] = {kDim / 2, a.group, tokens, 1}, steps[4] = {1, 1, 1, 1};
-    if (encode(&map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t *>(a.q), dims, strides, boxes,
-               steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    if (!k8::in_context([&] {
+            return encode(&map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t *>(a.q), dims, strides,
+                          boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        }))
         return api_fail(ATLAS_ECUDA, "%s: the token rows cannot be described to the copy engine", who);
     return ATLAS_OK;
 }
