@@ -712,7 +712,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             uint16_t *const out = a.out + ((size_t)st.s * a.r.tokens + mine.x) * a.ldo + (size_t)(st.h * a.group + mine.y) * kDim;
             constexpr uint32_t kColumns = ONE ? kDim / 2u : kDim;
             const uint32_t c0 = ONE ? t * kColumns : 0u;
-            // some columns' outputs, times their factors, into o; RARE: with what was taken out of V, and the steps before
+            // some columns' outputs, times their factors, into o; RARE: with what was taken out of V, and the steps before. A factor of 0
+            // is multiplied by, too: infinities that the row sees stay to be seen.
             auto outputs = [&](auto &o, uint32_t c, auto rare) {
                 constexpr bool RARE = decltype(rare)::value;
                 constexpr int N = sizeof(o) / sizeof(o[0]);
@@ -720,13 +721,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 tmem_wait_ld(o);
                 if (ONE || RARE)
 #pragma unroll
-                    for (int k = 0; k < N; ++k) o[k] = f[ONE ? 0 : t] == 0.f ? 0.f : o[k] * f[ONE ? 0 : t];
+                    for (int k = 0; k < N; ++k) o[k] *= f[ONE ? 0 : t];
                 if (ONE && have[1]) {
                     float y[N];
                     tmem_ld(out_at + 128u + c, y);
                     tmem_wait_ld(y);
 #pragma unroll
-                    for (int k = 0; k < N; ++k) o[k] = f[1] == 0.f ? o[k] : fmaf(f[1], y[k], o[k]);
+                    for (int k = 0; k < N; ++k) o[k] = fmaf(f[1], y[k], o[k]);
                 }
                 if (!RARE || !there) return;
                 if (bad) {   // what was taken out of V, to the rows that see it
