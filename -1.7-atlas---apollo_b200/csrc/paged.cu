@@ -46,7 +46,7 @@ struct AppendArgs {
     uint32_t layer, early;
 };
 
-// Rows (token, head) of a sequence that 16 threads take: 8192 tokens of 8 heads take 13.8 us; with 1, 4 or 8 rows 16.2, 16.5, 23.4
+// Rows (token, head) of a sequence that 16 threads take: 8192 tokens of 8 heads take 13.8 us; with 1 or 4 rows 16.4 or 16.2
 constexpr uint32_t kAppendThreads = 256, kAppendRows = 2;
 
 // Through L2, whose lines of it go first: a row is read once, and the pages should stay (without that 14.7 us instead of 13.8)
@@ -844,10 +844,11 @@ extern "C" int atlas_cuda_paged_compact(const AtlasPaged *cache, uint32_t *d_use
 namespace {
 
 // The query rows of a KV head that a CTA takes at a time: 8 or 16 (the form for few rows), 128 or 256. Measured, us in a row
-// of calls. Up to 16 rows in the form for few, or units of 128: 2 and 3 tokens of 8 sequences over 2303, 40 heads on 8,
-// 21.8 and 27.2, 22.1 and 27.6; 3 over 8447 15.8 and 18.0; 2 of 4 sequences over 640, 28 on 4, 9.3 and 13.4. 128 or 256,
-// where 128 leave no CTA a second unit: 7 tokens of 4 sequences over 8001 28.3 and 32.1, 333 of 16 on 2 over 5001 42.5 and
-// 45.3, 512 of 28 on 4 15.0 and 18.1; where they do: 1000 of 40 on 8 45.0 and 41.6, 8 x 2048 645 and 506, 8192 734 and 695.
+// of calls, all with the build as it is, in turn. Up to 16 rows in the form for few, or units of 128: 2 and 3 tokens of 8
+// sequences over 2303, 40 heads on 8, 22.0 and 26.7, 22.2 and 27.4; 3 over 8447 15.8 and 18.0; 2 of 4 sequences over 640, 28
+// on 4, 9.3 and 13.4. 128 or 256, where 128 leave no CTA a second unit: 7 tokens of 4 sequences over 8001 27.8 and 31.5, 333
+// of 16 on 2 over 5001 42 to 44 and 46, 512 of 28 on 4 16 and 19; where they do: 1000 of 40 on 8 44 and 41, 8 x 2048 652 and
+// 509, 8192 704 to 712 and 669 to 697.
 constexpr uint32_t kFewRows = 16;
 
 uint32_t attn_rows(const Cache &c, uint32_t group, uint32_t tokens, int sms)

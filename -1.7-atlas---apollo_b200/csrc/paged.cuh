@@ -221,8 +221,8 @@ __device__ __forceinline__ void enter_unit(const Cut<KEYS, EXTRA> &cut, Piece &p
 // pieces of `least` tiles of keys at least; but units that are no more than CTAs (and 32 of a KV head) are cut one by one
 // if no piece gets longer than that, and left whole if none gets more than `worth` tiles longer (what joining partial
 // sums costs). In clusters, if there are enough of them, each has a unit together. (Short code on purpose: its first run after
-// a launch waits for its instructions; with up to 128 units of a KV head in four registers a lane, a prompt's calls
-// took 2 to 4 us longer.)
+// a launch waits for its instructions; in an earlier build, with up to 128 units of a KV head in four registers a lane, a
+// prompt's calls took 2 to 4 us longer.)
 template <uint32_t KEYS, uint32_t EXTRA>
 __device__ __forceinline__ Piece find_kept(const Cut<KEYS, EXTRA> &cut, uint32_t least, uint32_t worth, uint32_t cluster = 1u)
 {

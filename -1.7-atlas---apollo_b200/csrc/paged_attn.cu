@@ -21,9 +21,13 @@
 // Where there are enough clusters to give each unit one, its CTAs have the unit
 // together, and join their states through distributed shared memory.
 // Bound by HBM for long caches (8 sequences of 32768 positions, 40 heads on 8, 1.07
-// GB: 165 to 167 us, 98 % of the copy rate), by latency for short ones: launch, piece,
-// pages' numbers, first copies, a round of chunks a microsecond, sums (640 positions
-// 6.8 us, 8447 11.5, 8 sequences around 2303 13.3).
+// GB: 165 to 167 us in a row of calls, 98 % of the copy rate; 171 to 173 for calls one by
+// one; 256 sequences of 100 to 8000 positions, 28 heads on 4, 362 us, 96 %; 64 of them
+// 94, 85 %), by latency for short ones: launch, piece, pages' numbers, first copies, a
+// round of chunks a microsecond, sums (640 positions 6.9 us, 8447 11.5, 8 sequences
+// around 2303 13.7 in tables that have no room for more; where there is room for 32768,
+// 8.3, 12.6 and 14.2: the launch that joins partial sums follows), and by the search for a
+// CTA's piece for very many sequences (4096 of 100 to 300 positions 725 us, 37 %).
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -46,10 +50,10 @@ constexpr uint32_t kChunk = 16, kWarps = 12, kThreads = kWarps * 32, kStages = 2
 constexpr uint32_t kHalfChunk = kChunk * 128, kSlot = 4 * kHalfChunk;   // 16 rows x 64 dimensions; K and V of 16 positions
 constexpr uint32_t kRecStride = kDim + 4;
 // Chunks: what joining partial sums takes, where a sequence has no room for more than leaves none, so that the launch
-// that joins them is left out (640 positions 6.8 us instead of 8.2; 8447 11.5 instead of 12.7), and where it follows in any case;
-// and what beginning and ending a unit takes. With 95, 48 or 32 instead of 64: 16 heads on 2 over 32767 18.8, 15.2 or 15.2 us
-// instead of 15.1; 28 on 4 over 20000 16.2, 16.2 or 14.2 instead of 16.2; 40 on 8 over 30000 27.5, 28.6 or 28.6 instead of 27.5. With
-// 8 instead of 32 for a unit's ends nothing changes by 1 %.
+// that joins them is left out (640 positions 6.9 us instead of 8.3; 8447 11.5 instead of 12.6), and where it follows in any case;
+// and what beginning and ending a unit takes. In tables with room for 32768 positions, with 95, 48 or 32 instead of 64: 16 heads
+// on 2 over 32767 18.8, 15.4 or 15.4 us instead of 15.4; 28 on 4 over 20000 15.1, 15.1 or 14.1 instead of 15.1; 40 on 8 over 30000
+// 27.5, 28.3 or 28.3 instead of 27.6. With 8 instead of 32 for a unit's ends nothing changes by 1 %.
 constexpr uint32_t kWorth = 96, kWorthMore = 64, kExtra = 32;
 static_assert(kWorthMore < kWorth, "it tells a call that may leave partial sums");
 constexpr float kLazy = 6.0f;

@@ -23,9 +23,17 @@
 //         MMAs;
 //   10-11 of a tile of keys that not all rows see, take values out of V that are
 //         not finite: a weight of 0 would not hide them. The softmax threads
-//         add them to the rows that do see them.
+//         add them to the rows that do see them. A slot of the ring waits for them as
+//         for the MMAs.
 // With one tile of rows, both softmax groups have it and take turns at the keys,
 // each with an output and a state of its own, joined at the end.
+//
+// P is rounded to the cache's type, as the product's operand, while its sum is not: a
+// choice. Its rest as a second term would make three products of two, on the pipe that
+// bounds long prompts. Each weight is off by half a step at most and independently of the
+// others: against 64 bits, outputs are off by 2.8e-4 (binary16) and 2.0e-3 (bfloat16),
+// relative 2-norm, where a plain form in fp32, rounded once at the end, is off by 2.1e-4
+// and 1.6e-3. (paged_attn.cu, where the products cost nothing, takes both terms.)
 //
 // Tensor cores truncate their sums: 2^-24 of the output per MMA of 16 keys at
 // most, so 256 tiles of keys (2048 MMAs, 2^-13) are summed in tensor memory, and
@@ -35,11 +43,13 @@
 //
 // Bound by the chain of a row tile's scores, softmax and second product, about 3200
 // cycles per 128 keys, of which two run: the tensor pipe and the exponentials are both
-// busy 57 % of the time. 8192 tokens of 40 heads on 8: 671 us with the partial sums, 1.02
-// PFLOP/s, 61 % of the measured bfloat16 rate; 757 when repeated under the power cap. A
-// quarter of the exponentials on the FMA units instead: 633 where a build took 623. Short
-// calls are bound by what comes before the first scores and behind the last: 512 tokens
-// of 28 heads on 4 15.0 us, 7 tokens of 4 sequences over 8001 28.3.
+// busy 56 % of the time. 8192 tokens of 40 heads on 8: 661 to 686 us with the partial sums
+// in short rows of calls, 1.0 to 1.04 PFLOP/s, 60 to 62 % of the measured bfloat16 rate;
+// 757, 0.91 PFLOP/s and 54 %, when repeated under the power cap. (An earlier build with a
+// quarter of the exponentials on the FMA units: 633 instead of 623.) Short calls are bound
+// by what comes before the first scores and behind the last: 512 tokens of 28 heads on 4
+// 16 us, 7 tokens of 4 sequences over 8001 27.8; in tables with room for 32768 positions 19
+// and 28, as the launch that joins follows.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -70,7 +80,7 @@ constexpr uint32_t kHalf = 128 * 128;              // bytes of 128 rows x 64 val
 constexpr uint32_t kTile = 2 * kHalf;
 constexpr uint32_t kMaxStages = 6;
 // tiles of keys: what joining partial sums takes, and beginning and ending a unit. With 1 or 5 instead of 3: 7 tokens of 4
-// sequences over 8001 30.8 or 28.4 us instead of 28.3, 8192 tokens 730 or 686 instead of 695, 8 x 2048 514 or 524 instead of 506
+// sequences over 8001 30.3 or 28.8 us instead of 27.8, 8192 tokens 743 or 684 instead of 677, 8 x 2048 517 or 526 instead of 517
 constexpr uint32_t kWorth = 6, kExtra = 3;
 constexpr float kLazy = 8.0f;
 // Weights are 2^(score - maximum + kUnit): binary16 keeps 24 bits below the largest; bfloat16 has fp32's range, and small
@@ -78,8 +88,9 @@ constexpr float kLazy = 8.0f;
 template <bool BF>
 constexpr float kUnit = BF ? -24.0f : 6.0f;
 
-// Weights go to the second product in so many parts: with four, the softmax warps' extra waits cost more (679 us for 8192
-// tokens of 40 heads on 8) than the product's earlier start gains (623)
+// Weights go to the second product in so many parts: with four, the softmax warps' extra waits cost more than the product's
+// earlier start gains but in the longest calls (7 tokens of 4 sequences over 8001 29.7 us instead of 27.8, 333 over 5001 48
+// instead of 42, 8 x 2048 531 instead of 517, 8192 635 to 667 instead of 669 to 686)
 constexpr uint32_t kParts = 2;
 
 struct PromptArgs : AttnArgs {

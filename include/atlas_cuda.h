@@ -406,10 +406,14 @@ int atlas_cuda_paged_append(const AtlasPaged *cache, uint32_t layer, uint32_t to
 
 /* Causal grouped-query attention of a chunk of new tokens: the query rows of
    position p see the positions 0 .. p that have a page, scores q.k / sqrt(128),
-   softmax and sums in fp32, rounded once at the end. Rows that see nothing are
-   zeros. What lies at positions that a row does not see has no part in it,
-   infinities and NaN among it; a value that is not finite at a position that it
-   does see makes what it enters infinite or NaN. q_heads is a multiple of
+   softmax and sums in fp32, rounded at the end; with more than 16 query rows per
+   KV head, of groups of up to 128 heads, weights are rounded once more, to the
+   cache's type (see paged_attn_form). Rows that see nothing are zeros. What lies at positions that a
+   row does not see has no part in it, infinities and NaN among it; a value that is
+   not finite at a position that it does see makes what it enters infinite or NaN,
+   however small its weight. A score of -infinity (of infinite keys, or beyond
+   fp32's range) has no weight, and a row that has no other is zeros. bfloat16
+   values below 2^-112 in size lose bits. q_heads is a multiple of
    kv_heads; q and out that overlap are refused (their rows may lie beside one
    another in one buffer, with ldq = ldo). Which kernels run, and so the last bits
    of a row, depends on the call's sizes and positions; the same call gives the
