@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes
 import os
 import sys
+from itertools import accumulate
+from operator import mul
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_DIR, "libatlas_cuda.so")
@@ -467,8 +469,8 @@ def _kv8_ints(who: str, name: str, t, n: int) -> None:
 
 def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: int, kind: str = "float32") -> None:
     """Refuses a tensor that is not token rows [nseq, tokens, heads, 128] of type `kind`, ld values from token to token (0:
-    dense). One that is not 4-dimensional must be dense, and long enough; so may one of just the size be whose dimensions put
-    the same rows in the same places ([nseq, heads, 1, 128] of one token)."""
+    dense). One that is not 4-dimensional must be dense, and long enough. A dense one of just the size passes if its dimensions
+    begin and end where those do, so that the same values are in the same places ([nseq, heads, 1, 128] of one token)."""
     if not tokens or not hasattr(t, "dtype"):
         return
     step = ld or heads * 128
@@ -477,8 +479,8 @@ def _kv8_rows(who: str, name: str, t, nseq: int, tokens: int, heads: int, ld: in
         ok = (shape[0] >= nseq and shape[1] >= tokens and shape[2] >= heads and shape[3] == 128 and stride[3] == 1
               and (heads == 1 or stride[2] == 128) and (tokens == 1 or stride[1] == step)
               and (nseq == 1 or stride[0] == tokens * step)
-              or t.is_contiguous() and t.numel() == nseq * tokens * step and step == heads * 128 and shape[3] % 128 == 0
-              and (tokens == 1 or heads == 1 or shape[2] * shape[3] == step))
+              or t.is_contiguous() and t.numel() == nseq * tokens * step and step == heads * 128
+              and {1, 128, step, tokens * step, nseq * tokens * step}.issuperset(accumulate(reversed(shape), mul)))
     else:
         ok = t.is_contiguous() and t.numel() >= (nseq * tokens - 1) * step + heads * 128
     if not ok or _kind(t) != kind:

@@ -49,8 +49,9 @@ def _calls(which, tokens):
 def test_the_order_of_dimensions(seen, which, tokens):
     for call, heads, kind in _calls(which, tokens):
         right = torch.zeros(N, tokens, heads, 128, dtype=kind)
-        takes = [(N, tokens, heads, 128), (1, N * tokens, heads, 128), (N * tokens, heads, 128), (N, tokens, 1, heads * 128), (N * tokens * heads * 128,)]
-        refuses = [(N, tokens, 128, heads), (128, N, tokens, heads)]
+        takes = [(N, tokens, heads, 128), (1, N * tokens, heads, 128), (N * tokens, heads, 128), (N, tokens, 1, heads * 128), (N * tokens * heads * 128,),
+                 (N, tokens * heads, 1, 128), (N, tokens, heads * 128, 1)]
+        refuses = [(N, tokens, 128, heads), (128, N, tokens, heads)] + [(3, N, heads, 128)] * (tokens == 3) + [(heads, N, 1, 128)] * (tokens == 1 and heads != N)
         (takes if tokens == 1 else refuses).append((N, heads, tokens, 128))
         for shape in takes:
             for pair in ((torch.zeros(shape, dtype=kind), right), (right, torch.zeros(shape, dtype=kind))):
